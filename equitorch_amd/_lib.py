@@ -144,6 +144,31 @@ class UvgArgs(C.Structure):
                 ("c", C.c_int32), ("cy", C.c_int32)]
 
 
+class GffArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("w_down", C.c_void_p),
+                ("gate", C.c_void_p), ("up", C.c_void_p), ("mid", C.c_void_p), ("out", C.c_void_p),
+                ("grad_out", C.c_void_p), ("grad_gate", C.c_void_p), ("grad_up", C.c_void_p), ("grad_x", C.c_void_p),
+                ("grad_w_gate", C.c_void_p), ("grad_w_up", C.c_void_p), ("grad_w_down", C.c_void_p),
+                ("workspace", C.c_void_p), ("n_rows", C.c_int64),
+                ("c_in", C.c_int32), ("hidden", C.c_int32), ("c_out", C.c_int32), ("activation", C.c_int32),
+                ("dtype", C.c_int32), ("reserved_", C.c_int32)]
+
+
+class AttnArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("q_node", C.c_int64), ("q_head", C.c_int64), ("k_node", C.c_int64), ("k_head", C.c_int64),
+                ("v_node", C.c_int64), ("v_head", C.c_int64),
+                ("pos_q", C.c_void_p), ("pos_k", C.c_void_p), ("slope", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+                ("q_items", C.c_void_p), ("q_joins", C.c_void_p), ("k_items", C.c_void_p), ("k_joins", C.c_void_p),
+                ("n_q_items", C.c_int32), ("n_q_joins", C.c_int32), ("n_q_slots", C.c_int32),
+                ("n_k_items", C.c_int32), ("n_k_joins", C.c_int32), ("n_k_slots", C.c_int32),
+                ("grad_out", C.c_void_p), ("grad_q", C.c_void_p), ("grad_k", C.c_void_p), ("grad_v", C.c_void_p),
+                ("grad_pos_q", C.c_void_p), ("grad_pos_k", C.c_void_p), ("grad_slope", C.c_void_p), ("workspace", C.c_void_p),
+                ("n_q", C.c_int64), ("n_k", C.c_int64), ("h_q", C.c_int32), ("h_kv", C.c_int32), ("dim", C.c_int32),
+                ("dtype", C.c_int32), ("wide_q", C.c_int32), ("wide_k", C.c_int32), ("same_pos", C.c_int32),
+                ("reserved_", C.c_int32), ("scale", C.c_float), ("cap", C.c_float)]
+
+
 def _load():
     if not os.path.exists(_LIB_PATH):
         raise ImportError(
@@ -265,6 +290,16 @@ def _load():
                                        _seg, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]
     lib.cgtp_wigner_rotate_backward.argtypes = [C.c_void_p] * 6 + [_seg, _seg, C.c_int, C.c_int64, C.c_int, C.c_int] + \
         [C.c_void_p] * 4 + [C.c_int, C.c_void_p]
+    lib.cgtp_embed_workspace_bytes.restype = C.c_int64
+    lib.cgtp_embed_workspace_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int, C.c_int]
+    lib.cgtp_embed_forward.argtypes = [C.c_void_p] * 3 + [C.c_int64, C.c_int64, C.c_int, C.c_double, C.c_int, C.c_void_p]
+    lib.cgtp_embed_backward.argtypes = [C.c_void_p] * 4 + [C.c_int64, C.c_int64, C.c_int, C.c_double, C.c_int, C.c_void_p]
+    for name in ("cgtp_gff", "cgtp_attn"):
+        args = C.POINTER(GffArgs if name == "cgtp_gff" else AttnArgs)
+        ws = getattr(lib, name + "_workspace_bytes")
+        ws.restype, ws.argtypes = C.c_int64, [args] if name == "cgtp_gff" else [args, C.c_int]
+        getattr(lib, name + "_forward").argtypes = [args, C.c_void_p]
+        getattr(lib, name + "_backward").argtypes = [args, C.c_void_p]
     lib.cgtp_abi_layout.argtypes = [C.c_int, C.POINTER(C.c_int64), C.c_int]
     return lib
 

@@ -1,0 +1,595 @@
+// Kernels of the attention among the nodes of a structure for one element type (attn_f32.hip, attn_bf16.hip, attn_f16.hip).
+//
+//   t_ij = log2(e) s_ij,  s_ij = cap tanh(scale q_i.k_j / cap) - slope_h |r_i - r_j|
+//   out_i = sum_j 2^(t_ij - lse_i) v_j,  lse_i = log2 sum_j 2^t_ij
+//   p_ij = 2^(t_ij - lse_i),  dp_ij = dout_i.v_j,  delta_i = dout_i.out_i,  ds_ij = p_ij (dp_ij - delta_i)
+//   dv_j = sum_i p_ij dout_i,   du_ij = ds_ij (1 - tanh^2),   dq_i = scale sum_j du_ij k_j,  dk_j = scale sum_i du_ij q_i
+//   dslope_h = -sum ds_ij |r_i - r_j|,   dr_i = -slope sum_j ds_ij (r_i - r_j) / |r_i - r_j|,  dr_j the opposite
+//
+// One pass over the keys with the running maximum and sum of each row (forward); the backward forms the scores again, once
+// with the rows fixed (dq, dr_i, dslope) and once with the keys fixed (dk, dv, dr_j), so that every sum is held by one
+// workgroup and no result depends on timing.
+//
+// A row is a (query, query head) pair of one head of keys: heads that share keys and values share the tiles in LDS, and a
+// single query of a structure brings all its heads to one tile.  A wavefront owns 32 rows (or 32 keys) and forms the scores with
+// the other operand's rows down the registers, so that a row's statistics take one exchange between the halves of the
+// wavefront and the probabilities are the next product's operand as they lie.  Tiles never cross structures: what another
+// structure holds, infinities and NaN included, is never read.  A key or row of a tile beyond its range is a zero in LDS and
+// its score -inf.
+#pragma once
+
+#include "attn_tiles.h"
+#include "attn_host.h"
+
+namespace cgtp {
+namespace {
+
+constexpr float kLog2E = 1.4426950408889634f;
+
+template <int NW> constexpr int kRowsOf = 32 * NW;
+
+// What scores are made of, in units of log2(e).
+struct ScoreScale {
+  float linear;        // cap <= 0: t = linear * q.k
+  float inner, outer;  // else t = outer - 2 outer / (2^(inner q.k) + 1)
+  bool capped, biased;
+};
+__device__ __forceinline__ ScoreScale score_scale(const cgtp_attn_args& a) {
+  ScoreScale s;
+  s.capped = a.cap > 0.f;
+  s.biased = a.slope != nullptr;
+  s.linear = a.scale * kLog2E;
+  s.inner = s.capped ? 2.f * kLog2E * a.scale / a.cap : 0.f;
+  s.outer = a.cap * kLog2E;
+  return s;
+}
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// tanh of half of what `inner` makes of q.k.
+__device__ __forceinline__ float capped_tanh(float inner_qk) {
+  return 1.f - 2.f * __builtin_amdgcn_rcpf(exp2_fast(inner_qk) + 1.f);
+}
+__device__ __forceinline__ float half_swap(float x) { return __shfl_xor(x, 32, kWave); }
+
+struct Row {
+  int query, head;     // of the tensors
+  bool ok;
+};
+__device__ __forceinline__ Row row_of(const cgtp_attn_item& it, int r, int kv_head, int group) {
+  Row o;
+  o.ok = r < it.row_end;
+  const int rr = o.ok ? r : it.row_begin;
+  o.query = it.node + rr / group;
+  o.head = kv_head * group + rr % group;
+  return o;
+}
+
+// ---- forward ----------------------------------------------------------------------------------------------------
+template <typename T, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW) attn_fwd_kernel(cgtp_attn_args a, float* __restrict__ parts) {
+  using S = AttnShape<T, DP>;
+  __shared__ alignas(16) char k_rows[S::kRowsBytes];
+  __shared__ alignas(16) char v_tile[S::kTransposed ? S::kColsBytes : S::kRowsBytes];
+  __shared__ alignas(16) float pos[3][kBlock];
+  const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
+  const cgtp_attn_item it = a.q_items[blockIdx.x / a.h_kv];
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+  const int r = it.row_begin + wave * 32 + (lane & 31);
+  const Row row = row_of(it, r, hk, group);
+  const ScoreScale sc = score_scale(a);
+  RowFrag<T, DP> q;
+  q.load(row.ok ? (const T*)a.q + row.query * a.q_node + row.head * a.q_head : nullptr, a.dim);
+  float x = 0.f, y = 0.f, z = 0.f, slope = 0.f;
+  if (sc.biased && row.ok) {
+    x = a.pos_q[(int64_t)row.query * 3];
+    y = a.pos_q[(int64_t)row.query * 3 + 1];
+    z = a.pos_q[(int64_t)row.query * 3 + 2];
+    slope = a.slope[row.head] * kLog2E;
+  }
+  AttnAcc<T, DP> acc;
+#pragma unroll
+  for (int o = 0; o < S::kOut; ++o)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[o][e] = 0.f;
+  float top = -INFINITY, sum = 0.f;           // of this lane's keys (sum), of the row's (top)
+  const T* kp = (const T*)a.k + hk * a.k_head;
+  const T* vp = (const T*)a.v + hk * a.v_head;
+  for (int k0 = it.k_begin; k0 < it.k_end; k0 += kBlock) {
+    const int n = it.k_end - k0;
+    __syncthreads();
+    stage_rows<T, DP, 64 * NW>(k_rows, a.dim, [&](int i) { return i < n ? kp + (int64_t)(k0 + i) * a.k_node : nullptr; });
+    if constexpr (S::kTransposed)
+      stage_cols<T, DP, 64 * NW>(v_tile, a.dim, [&](int i) { return i < n ? vp + (int64_t)(k0 + i) * a.v_node : nullptr; });
+    else
+      stage_rows<T, DP, 64 * NW>(v_tile, a.dim, [&](int i) { return i < n ? vp + (int64_t)(k0 + i) * a.v_node : nullptr; });
+    if (sc.biased)
+      for (int i = threadIdx.x; i < kBlock; i += 64 * NW)
+#pragma unroll
+        for (int d = 0; d < 3; ++d) pos[d][i] = i < n ? a.pos_k[(int64_t)(k0 + i) * 3 + d] : 0.f;
+    __syncthreads();
+    f32x16_t t[2];
+    float most = top;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if (b * 32 >= n) continue;
+      t[b] = rows_times<T, DP>(k_rows, 32 * b, q);
+      if (sc.capped) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[b][e] = sc.outer * capped_tanh(sc.inner * t[b][e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[b][e] *= sc.linear;
+      }
+      if (sc.biased) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int at = 32 * b + 8 * g + 4 * half;
+          const f32x4 px = *reinterpret_cast<const f32x4*>(&pos[0][at]), py = *reinterpret_cast<const f32x4*>(&pos[1][at]),
+                      pz = *reinterpret_cast<const f32x4*>(&pos[2][at]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float dx = x - px[e], dy = y - py[e], dz = z - pz[e];
+            t[b][4 * g + e] -= slope * __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz);
+          }
+        }
+      }
+      if (n < 32 * b + 32)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (32 * b + 8 * (e >> 2) + 4 * half + (e & 3) >= n) t[b][e] = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) most = fmaxf(most, t[b][e]);
+    }
+    most = fmaxf(most, half_swap(most));
+    if (__any(most > top)) {
+      const float by = top == most ? 1.f : exp2_fast(top - most);      // equal: also both -inf
+      sum *= by;
+#pragma unroll
+      for (int o = 0; o < S::kOut; ++o)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[o][e] *= by;
+      top = most;
+    }
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if (b * 32 >= n) continue;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        t[b][e] = exp2_fast(t[b][e] - base);
+        sum += t[b][e];
+      }
+      cols_times<T, DP>(acc, v_tile, v_tile, 32 * b, t[b]);
+    }
+  }
+  sum += half_swap(sum);
+  if (!row.ok) return;
+  if (it.slot < 0) {
+    const bool some = sum > 0.f || sum != sum;
+    const int64_t at = (int64_t)row.query * a.h_q + row.head;
+    const float by = some ? 1.f / sum : 0.f;
+    store_cols<T, DP>((T*)a.out + at * a.dim, acc, by, a.dim);
+    if (a.lse && half == 0) ((float*)a.lse)[at] = some ? top + __log2f(sum) : INFINITY;
+  } else {
+    float* p = parts + (((int64_t)it.slot * a.h_kv + hk) * kRowsOf<NW> + (r - it.row_begin)) * (a.dim + 2);
+    store_cols<float, (DP < 32 ? 32 : DP)>(p, acc, 1.f, a.dim);
+    if (half == 0) {
+      p[a.dim] = top;
+      p[a.dim + 1] = sum;
+    }
+  }
+}
+
+// Adds the parts of a row: a workgroup for each (tile, head of keys, row), its slots shared out over slices of threads.
+constexpr int kJoinThreads = 1024;
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) attn_fwd_join_kernel(cgtp_attn_args a, const float* __restrict__ parts, int rows) {
+  __shared__ float acc[kJoinThreads], red[kJoinThreads / kWave];
+  const int group = a.h_q / a.h_kv, rr = blockIdx.x % rows, hk = blockIdx.x / rows % a.h_kv;
+  const cgtp_attn_item it = a.q_joins[blockIdx.x / rows / a.h_kv];
+  const Row row = row_of(it, it.row_begin + rr, hk, group);
+  if (!row.ok) return;
+  const int tid = threadIdx.x, width = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128, slices = kJoinThreads / width;
+  const int64_t step = (int64_t)a.h_kv * rows * (a.dim + 2);
+  const float* p = parts + (((int64_t)it.first * a.h_kv + hk) * rows + rr) * (a.dim + 2);
+  float top = -INFINITY;
+  for (int s = tid; s < it.count; s += kJoinThreads) top = fmaxf(top, p[s * step + a.dim]);
+  for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+  if ((tid & 63) == 0) red[tid >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / kWave; ++w) top = fmaxf(top, red[w]);
+  const float base = top == -INFINITY ? 0.f : top;
+  const int d = tid % width;
+  float o = 0.f, sum = 0.f;
+#pragma unroll 4
+  for (int s = tid / width; s < it.count; s += slices) {
+    const float* ps = p + s * step;
+    const float by = exp2_fast(ps[a.dim] - base);
+    sum += by * ps[a.dim + 1];
+    o += by * (d < a.dim ? ps[d] : 0.f);
+  }
+  acc[tid] = o;
+  __syncthreads();
+  float total = 0.f;
+  if (tid < width)
+    for (int s = 0; s < slices; ++s) total += acc[s * width + tid];
+  __syncthreads();
+  acc[tid] = sum;
+  __syncthreads();
+  if (tid >= width) return;
+  sum = 0.f;
+  for (int s = 0; s < slices; ++s) sum += acc[s * width];
+  const bool some = sum > 0.f || sum != sum;
+  const int64_t at = (int64_t)row.query * a.h_q + row.head;
+  if (d < a.dim) ((T*)a.out)[at * a.dim + d] = (T)(some ? total / sum : 0.f);
+  if (a.lse && tid == 0) ((float*)a.lse)[at] = some ? top + __log2f(sum) : INFINITY;
+}
+
+// A row's sums over its keys besides its gradient, and its delta.
+struct QSums {
+  float v[kQSums];
+  __device__ __forceinline__ void finish(const AttnScratch& w, int64_t at, float slope, bool biased) const {
+    const float off = v[8];
+    w.delta[at] = v[9] + off;
+    if (!biased) return;
+    w.row_part[at] = f32x4{-slope * (v[0] - off * v[4]), -slope * (v[1] - off * v[5]), -slope * (v[2] - off * v[6]),
+                           off * v[7] - v[3]};
+  }
+};
+
+// ---- gradient with the rows fixed ---------------------------------------------------------------------------------
+template <typename T, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW) attn_bwd_q_kernel(cgtp_attn_args a, AttnScratch w) {
+  using S = AttnShape<T, DP>;
+  __shared__ alignas(16) char k_rows[S::kRowsBytes], v_rows[S::kRowsBytes];
+  __shared__ alignas(16) char k_cols[S::kTransposed ? S::kColsBytes : 16];
+  __shared__ alignas(16) float pos[3][kBlock];
+  const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
+  const cgtp_attn_item it = a.q_items[blockIdx.x / a.h_kv];
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+  const int r = it.row_begin + wave * 32 + (lane & 31);
+  const Row row = row_of(it, r, hk, group);
+  const int64_t at = (int64_t)row.query * a.h_q + row.head;
+  const ScoreScale sc = score_scale(a);
+  RowFrag<T, DP> q, g;
+  q.load(row.ok ? (const T*)a.q + row.query * a.q_node + row.head * a.q_head : nullptr, a.dim);
+  g.load(row.ok ? (const T*)a.grad_out + at * a.dim : nullptr, a.dim);
+  float delta = 0.f;
+  {
+    RowFrag<T, DP> o;
+    o.load(row.ok ? (const T*)a.out + at * a.dim : nullptr, a.dim);
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s) {
+      typedef T vec __attribute__((ext_vector_type(S::kChunk)));
+      const vec go = __builtin_bit_cast(vec, g.f[s]), oo = __builtin_bit_cast(vec, o.f[s]);
+#pragma unroll
+      for (int j = 0; j < S::kChunk; ++j) delta = fmaf((float)go[j], (float)oo[j], delta);
+    }
+    delta += half_swap(delta);
+  }
+  const float lse = row.ok ? ((const float*)a.lse)[at] : INFINITY;
+  float x = 0.f, y = 0.f, z = 0.f, slope = 0.f;
+  if (sc.biased && row.ok) {
+    x = a.pos_q[(int64_t)row.query * 3];
+    y = a.pos_q[(int64_t)row.query * 3 + 1];
+    z = a.pos_q[(int64_t)row.query * 3 + 2];
+    slope = a.slope[row.head];
+  }
+  AttnAcc<T, DP> acc;
+#pragma unroll
+  for (int o = 0; o < S::kOut; ++o)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[o][e] = 0.f;
+  // Sums over the keys of ds (r_i - r_j) / |r_i - r_j| and of ds |r_i - r_j|; in 16-bit types also of ds, and of the others with
+  // p for ds (kFix).  delta is against an output that was summed from rounded probabilities and rounded itself: the
+  // exact one is delta + sum ds, and with it the gradients of positions and slopes, which are fp32, err as in fp32.
+  constexpr bool kFix = sizeof(T) == 2;
+  QSums m = {};
+  const T* kp = (const T*)a.k + hk * a.k_head;
+  const T* vp = (const T*)a.v + hk * a.v_head;
+  for (int k0 = it.k_begin; k0 < it.k_end; k0 += kBlock) {
+    const int n = it.k_end - k0;
+    auto k_row = [&](int i) { return i < n ? kp + (int64_t)(k0 + i) * a.k_node : nullptr; };
+    __syncthreads();
+    stage_rows<T, DP, 64 * NW>(k_rows, a.dim, k_row);
+    if constexpr (S::kTransposed) stage_cols<T, DP, 64 * NW>(k_cols, a.dim, k_row);
+    stage_rows<T, DP, 64 * NW>(v_rows, a.dim, [&](int i) { return i < n ? vp + (int64_t)(k0 + i) * a.v_node : nullptr; });
+    if (sc.biased)
+      for (int i = threadIdx.x; i < kBlock; i += 64 * NW)
+#pragma unroll
+        for (int d = 0; d < 3; ++d) pos[d][i] = i < n ? a.pos_k[(int64_t)(k0 + i) * 3 + d] : 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if (b * 32 >= n) continue;
+      f32x16_t t = rows_times<T, DP>(k_rows, 32 * b, q);
+      f32x16_t ds = rows_times<T, DP>(v_rows, 32 * b, g);
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        const int first = 32 * b + 8 * gq + 4 * half;
+        f32x4 px = {}, py = {}, pz = {};
+        if (sc.biased) {
+          px = *reinterpret_cast<const f32x4*>(&pos[0][first]);
+          py = *reinterpret_cast<const f32x4*>(&pos[1][first]);
+          pz = *reinterpret_cast<const f32x4*>(&pos[2][first]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * gq + e;
+          float th = 0.f, s;
+          if (sc.capped) {
+            th = capped_tanh(sc.inner * t[i]);
+            s = sc.outer * th;
+          } else {
+            s = sc.linear * t[i];
+          }
+          float dx = 0.f, dy = 0.f, dz = 0.f, d2 = 0.f, inv = 0.f;
+          if (sc.biased) {
+            dx = x - px[e];
+            dy = y - py[e];
+            dz = z - pz[e];
+            d2 = dx * dx + dy * dy + dz * dz;
+            inv = __builtin_amdgcn_rsqf(fmaxf(d2, 1e-37f));
+            s -= slope * kLog2E * (d2 * inv);
+          }
+          float p = exp2_fast(s - lse);
+          if (first + e >= n) p = 0.f;
+          float d = p * (ds[i] - delta);
+          if (sc.biased) {
+            const float u = d * inv;
+            m.v[0] = fmaf(u, dx, m.v[0]);
+            m.v[1] = fmaf(u, dy, m.v[1]);
+            m.v[2] = fmaf(u, dz, m.v[2]);
+            m.v[3] = fmaf(u, d2, m.v[3]);
+            if constexpr (kFix) {
+              const float c = p * inv;
+              m.v[4] = fmaf(c, dx, m.v[4]);
+              m.v[5] = fmaf(c, dy, m.v[5]);
+              m.v[6] = fmaf(c, dz, m.v[6]);
+              m.v[7] = fmaf(c, d2, m.v[7]);
+              m.v[8] += d;
+            }
+          }
+          if (sc.capped) d *= 1.f - th * th;
+          ds[i] = d;
+        }
+      }
+      cols_times<T, DP>(acc, k_rows, k_cols, 32 * b, ds);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < (kFix ? 9 : 4); ++i) m.v[i] += half_swap(m.v[i]);
+  m.v[9] = delta;
+  if (!row.ok) return;
+  if (it.slot < 0) {
+    if (a.grad_q) store_cols<T, DP>((T*)a.grad_q + at * a.dim, acc, a.scale, a.dim);
+    if (half == 0) m.finish(w, at, slope, sc.biased);
+  } else {
+    float* p = w.parts + (((int64_t)it.slot * a.h_kv + hk) * kRowsOf<NW> + (r - it.row_begin)) * (a.dim + kQSums);
+    store_cols<float, (DP < 32 ? 32 : DP)>(p, acc, a.scale, a.dim);
+    if (half == 0)
+#pragma unroll
+      for (int i = 0; i < kQSums; ++i) p[a.dim + i] = m.v[i];
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(192) attn_bwd_q_join_kernel(cgtp_attn_args a, AttnScratch w, int rows) {
+  __shared__ float sums[kQSums];
+  const int group = a.h_q / a.h_kv, rr = blockIdx.x % rows, hk = blockIdx.x / rows % a.h_kv;
+  const cgtp_attn_item it = a.q_joins[blockIdx.x / rows / a.h_kv];
+  const Row row = row_of(it, it.row_begin + rr, hk, group);
+  if (!row.ok) return;
+  const int d = threadIdx.x, width = a.dim + kQSums;
+  const int64_t step = (int64_t)a.h_kv * rows * width, at = (int64_t)row.query * a.h_q + row.head;
+  const float* p = w.parts + (((int64_t)it.first * a.h_kv + hk) * rows + rr) * width + d;
+  float s = 0.f;
+  const int count = d == width - 1 ? 1 : d < width ? it.count : 0;       // delta: the same in every piece
+#pragma unroll 8
+  for (int k = 0; k < count; ++k) s += p[k * step];
+  if (d < a.dim) {
+    if (a.grad_q) ((T*)a.grad_q)[at * a.dim + d] = (T)s;
+  } else if (d < width) {
+    sums[d - a.dim] = s;
+  }
+  __syncthreads();
+  if (d != 0) return;
+  QSums m;
+#pragma unroll
+  for (int i = 0; i < kQSums; ++i) m.v[i] = sums[i];
+  m.finish(w, at, a.slope ? a.slope[row.head] : 0.f, a.slope != nullptr);
+}
+
+// ---- gradient with the keys fixed ---------------------------------------------------------------------------------
+template <typename T, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW) attn_bwd_k_kernel(cgtp_attn_args a, AttnScratch w) {
+  using S = AttnShape<T, DP>;
+  __shared__ alignas(16) char q_rows[S::kRowsBytes], g_rows[S::kRowsBytes];
+  __shared__ alignas(16) char q_cols[S::kTransposed ? S::kColsBytes : 16], g_cols[S::kTransposed ? S::kColsBytes : 16];
+  __shared__ alignas(16) float stat[6][kBlock];       // lse, delta, slope, position
+  const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
+  const cgtp_attn_item it = a.k_items[blockIdx.x / a.h_kv];
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+  const int key = it.k_begin + wave * 32 + (lane & 31);
+  const bool ok = key < it.k_end;
+  const ScoreScale sc = score_scale(a);
+  RowFrag<T, DP> k, v;
+  k.load(ok ? (const T*)a.k + key * a.k_node + hk * a.k_head : nullptr, a.dim);
+  v.load(ok ? (const T*)a.v + key * a.v_node + hk * a.v_head : nullptr, a.dim);
+  float x = 0.f, y = 0.f, z = 0.f;
+  if (sc.biased && ok) {
+    x = a.pos_k[(int64_t)key * 3];
+    y = a.pos_k[(int64_t)key * 3 + 1];
+    z = a.pos_k[(int64_t)key * 3 + 2];
+  }
+  AttnAcc<T, DP> gk, gv;
+#pragma unroll
+  for (int o = 0; o < S::kOut; ++o)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) gk[o][e] = gv[o][e] = 0.f;
+  float gx = 0.f, gy = 0.f, gz = 0.f;
+  for (int r0 = it.row_begin; r0 < it.row_end; r0 += kBlock) {
+    const int n = it.row_end - r0;
+    auto q_row = [&](int i) {
+      const Row o = row_of(it, r0 + i, hk, group);
+      return o.ok ? (const T*)a.q + o.query * a.q_node + o.head * a.q_head : nullptr;
+    };
+    auto g_row = [&](int i) {
+      const Row o = row_of(it, r0 + i, hk, group);
+      return o.ok ? (const T*)a.grad_out + ((int64_t)o.query * a.h_q + o.head) * a.dim : nullptr;
+    };
+    __syncthreads();
+    stage_rows<T, DP, 64 * NW>(q_rows, a.dim, q_row);
+    stage_rows<T, DP, 64 * NW>(g_rows, a.dim, g_row);
+    if constexpr (S::kTransposed) {
+      stage_cols<T, DP, 64 * NW>(q_cols, a.dim, q_row);
+      stage_cols<T, DP, 64 * NW>(g_cols, a.dim, g_row);
+    }
+    for (int i = threadIdx.x; i < kBlock; i += 64 * NW) {
+      const Row o = row_of(it, r0 + i, hk, group);
+      const int64_t at = (int64_t)o.query * a.h_q + o.head;
+      stat[0][i] = o.ok ? ((const float*)a.lse)[at] : INFINITY;        // +inf: probability zero
+      stat[1][i] = o.ok ? w.delta[at] : 0.f;
+      if (sc.biased) {
+        stat[2][i] = o.ok ? a.slope[o.head] : 0.f;
+#pragma unroll
+        for (int d = 0; d < 3; ++d) stat[3 + d][i] = o.ok ? a.pos_q[(int64_t)o.query * 3 + d] : 0.f;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if (b * 32 >= n) continue;
+      f32x16_t t = rows_times<T, DP>(q_rows, 32 * b, k);
+      f32x16_t ds = rows_times<T, DP>(g_rows, 32 * b, v);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int first = 32 * b + 8 * g + 4 * half;
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[0][first]);
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[1][first]);
+        f32x4 slope = {}, px = {}, py = {}, pz = {};
+        if (sc.biased) {
+          slope = *reinterpret_cast<const f32x4*>(&stat[2][first]);
+          px = *reinterpret_cast<const f32x4*>(&stat[3][first]);
+          py = *reinterpret_cast<const f32x4*>(&stat[4][first]);
+          pz = *reinterpret_cast<const f32x4*>(&stat[5][first]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * g + e;
+          float th = 0.f, s;
+          if (sc.capped) {
+            th = capped_tanh(sc.inner * t[i]);
+            s = sc.outer * th;
+          } else {
+            s = sc.linear * t[i];
+          }
+          float dx = 0.f, dy = 0.f, dz = 0.f, inv = 0.f;
+          if (sc.biased) {
+            dx = px[e] - x;
+            dy = py[e] - y;
+            dz = pz[e] - z;
+            const float d2 = dx * dx + dy * dy + dz * dz;
+            inv = __builtin_amdgcn_rsqf(fmaxf(d2, 1e-37f));
+            s -= slope[e] * kLog2E * (d2 * inv);
+          }
+          const float p = exp2_fast(s - lse[e]);
+          float d = p * (ds[i] - delta[e]);
+          if (sc.biased) {
+            const float u = d * inv * slope[e];
+            gx = fmaf(u, dx, gx);
+            gy = fmaf(u, dy, gy);
+            gz = fmaf(u, dz, gz);
+          }
+          if (sc.capped) d *= 1.f - th * th;
+          t[i] = p;
+          ds[i] = d;
+        }
+      }
+      cols_times<T, DP>(gv, g_rows, g_cols, 32 * b, t);
+      cols_times<T, DP>(gk, q_rows, q_cols, 32 * b, ds);
+    }
+  }
+  gx += half_swap(gx);
+  gy += half_swap(gy);
+  gz += half_swap(gz);
+  if (!ok) return;
+  const int64_t at = (int64_t)key * a.h_kv + hk;
+  if (it.slot < 0) {
+    if (a.grad_k) store_cols<T, DP>((T*)a.grad_k + at * a.dim, gk, a.scale, a.dim);
+    if (a.grad_v) store_cols<T, DP>((T*)a.grad_v + at * a.dim, gv, 1.f, a.dim);
+    if (sc.biased && half == 0) w.key_part[at] = f32x4{gx, gy, gz, 0.f};
+  } else {
+    float* p = w.parts + (((int64_t)it.slot * a.h_kv + hk) * kRowsOf<NW> + (key - it.k_begin)) * (2 * a.dim + 4);
+    store_cols<float, (DP < 32 ? 32 : DP)>(p, gk, a.scale, a.dim);
+    store_cols<float, (DP < 32 ? 32 : DP)>(p + a.dim, gv, 1.f, a.dim);
+    if (half == 0) {
+      p[2 * a.dim] = gx;
+      p[2 * a.dim + 1] = gy;
+      p[2 * a.dim + 2] = gz;
+      p[2 * a.dim + 3] = 0.f;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512) attn_bwd_k_join_kernel(cgtp_attn_args a, AttnScratch w, int rows) {
+  const int kk = blockIdx.x % rows, hk = blockIdx.x / rows % a.h_kv;
+  const cgtp_attn_item it = a.k_joins[blockIdx.x / rows / a.h_kv];
+  const int key = it.k_begin + kk, d = threadIdx.x, width = 2 * a.dim + 4;
+  if (key >= it.k_end || d >= width) return;
+  const int64_t step = (int64_t)a.h_kv * rows * width, at = (int64_t)key * a.h_kv + hk;
+  const float* p = w.parts + (((int64_t)it.first * a.h_kv + hk) * rows + kk) * width + d;
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < it.count; ++k) s += p[k * step];
+  if (d < a.dim) {
+    if (a.grad_k) ((T*)a.grad_k)[at * a.dim + d] = (T)s;
+  } else if (d < 2 * a.dim) {
+    if (a.grad_v) ((T*)a.grad_v)[at * a.dim + d - a.dim] = (T)s;
+  } else if (a.slope) {
+    ((float*)&w.key_part[at])[d - 2 * a.dim] = s;
+  }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------
+template <typename T, int DP, int NW>
+void q_launch(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) {
+  const dim3 grid((unsigned)a.n_q_items * a.h_kv), joins((unsigned)a.n_q_joins * a.h_kv * kRowsOf<NW>);
+  float* parts = (float*)a.workspace;
+  if (a.n_q_items) {
+    if (w) hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NW>), grid, dim3(64 * NW), 0, s, a, *w);
+    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW>), grid, dim3(64 * NW), 0, s, a, parts);
+  }
+  if (a.n_q_joins) {
+    if (w) hipLaunchKernelGGL((attn_bwd_q_join_kernel<T>), joins, dim3(192), 0, s, a, *w, kRowsOf<NW>);
+    else hipLaunchKernelGGL((attn_fwd_join_kernel<T>), joins, dim3(kJoinThreads), 0, s, a, (const float*)parts, kRowsOf<NW>);
+  }
+}
+template <typename T, int DP, int NW>
+void k_launch(const cgtp_attn_args& a, const AttnScratch& w, hipStream_t s) {
+  if (a.n_k_items)
+    hipLaunchKernelGGL((attn_bwd_k_kernel<T, DP, NW>), dim3((unsigned)a.n_k_items * a.h_kv), dim3(64 * NW), 0, s, a, w);
+  if (a.n_k_joins)
+    hipLaunchKernelGGL((attn_bwd_k_join_kernel<T>), dim3((unsigned)a.n_k_joins * a.h_kv * kRowsOf<NW>), dim3(512), 0, s, a, w,
+                       kRowsOf<NW>);
+}
+template <typename T, int DP>
+void launch_dim(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) {
+  if (a.wide_q) q_launch<T, DP, 4>(a, w, s);
+  else q_launch<T, DP, 1>(a, w, s);
+  if (!w) return;
+  if (a.wide_k) k_launch<T, DP, 4>(a, *w, s);
+  else k_launch<T, DP, 1>(a, *w, s);
+}
+template <typename T>
+void launch_type(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) {
+  if (a.dim <= 16) launch_dim<T, 16>(a, w, s);
+  else if (a.dim <= 32) launch_dim<T, 32>(a, w, s);
+  else if (a.dim <= 64) launch_dim<T, 64>(a, w, s);
+  else if (a.dim <= 96) launch_dim<T, 96>(a, w, s);
+  else launch_dim<T, 128>(a, w, s);
+}
+
+}  // namespace
+}  // namespace cgtp

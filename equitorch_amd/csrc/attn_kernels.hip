@@ -1,0 +1,133 @@
+// Attention among the nodes of a structure: entry points, and the kernels that add the heads' parts of the gradients of
+// positions and slopes (attn_impl.h has the rest).
+#include "attn_host.h"
+
+#include <algorithm>
+
+namespace cgtp {
+namespace {
+
+// Gradient of the positions of 64 nodes: the parts of their rows (as queries) and of their head of keys (as keys, where the
+// positions are one tensor), heads in order; and the 64 queries' part of the gradient of every slope.
+constexpr int kPosNodes = 64;
+__global__ void __launch_bounds__(256) attn_pos_kernel(cgtp_attn_args a, AttnScratch w) {
+  const int64_t i0 = (int64_t)blockIdx.x * kPosNodes;
+  const int n = (int)(a.n_q - i0 < kPosNodes ? a.n_q - i0 : kPosNodes);
+  if (a.grad_pos_q && threadIdx.x < 192) {
+    const int i = threadIdx.x / 3, d = threadIdx.x % 3;
+    if (i < n) {
+      float s = 0.f;
+      for (int h = 0; h < a.h_q; ++h) s += ((const float*)&w.row_part[(i0 + i) * a.h_q + h])[d];
+      if (a.same_pos)
+        for (int h = 0; h < a.h_kv; ++h) s += ((const float*)&w.key_part[(i0 + i) * a.h_kv + h])[d];
+      a.grad_pos_q[(i0 + i) * 3 + d] = s;
+    }
+  }
+  if (a.grad_slope)
+    for (int h = threadIdx.x; h < a.h_q; h += 256) {
+      float s = 0.f;
+      for (int i = 0; i < n; ++i) s += w.row_part[(i0 + i) * a.h_q + h][3];
+      w.slope_part[(int64_t)blockIdx.x * a.h_q + h] = s;
+    }
+}
+__global__ void __launch_bounds__(192) attn_pos_k_kernel(cgtp_attn_args a, AttnScratch w) {
+  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x / 3;
+  const int d = threadIdx.x % 3;
+  if (i >= a.n_k) return;
+  float s = 0.f;
+  for (int h = 0; h < a.h_kv; ++h) s += ((const float*)&w.key_part[i * a.h_kv + h])[d];
+  a.grad_pos_k[i * 3 + d] = s;
+}
+
+int64_t blocks_of(int64_t n) { return (n + kPosNodes - 1) / kPosNodes; }
+
+// Workspace of the backward; every buffer starts at a multiple of 256 bytes.  The pieces' results of the two passes share a place.
+struct AttnLayout { int64_t row_part, key_part, slope_part, parts, bytes; };
+AttnLayout attn_layout(const cgtp_attn_args& a) {
+  AttnLayout l;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) { const int64_t was = at; at += (bytes + 255) / 256 * 256; return was; };
+  take(a.n_q * a.h_q * 4);
+  l.row_part = take(a.slope ? a.n_q * a.h_q * 16 : 0);
+  l.key_part = take(a.slope ? a.n_k * a.h_kv * 16 : 0);
+  l.slope_part = take(a.slope ? blocks_of(a.n_q) * a.h_q * 4 : 0);
+  const int64_t heads = a.h_kv * 4;
+  l.parts = take(std::max(a.n_q_slots * heads * cgtp_attn_rows(a.wide_q) * (a.dim + kQSums),
+                          a.n_k_slots * heads * cgtp_attn_rows(a.wide_k) * (2 * a.dim + 4)));
+  l.bytes = at;
+  return l;
+}
+
+int attn_check(const cgtp_attn_args* a) {
+  if (!a) return CGTP_ERR_NULL;
+  if (a->dtype != CGTP_F32 && a->dtype != CGTP_BF16 && a->dtype != CGTP_F16) return CGTP_ERR_DTYPE;
+  if (a->n_q < 0 || a->n_k < 0 || a->n_q > 0x7fffffff || a->n_k > 0x7fffffff) return CGTP_ERR_SHAPE;
+  if (a->dim <= 0 || a->dim > 128 || a->h_kv <= 0 || a->h_q <= 0 || a->h_q % a->h_kv || a->h_q > 0x3fff) return CGTP_ERR_SHAPE;
+  // rows are counted in 32 bits, and a grid has fewer than 2^32 threads
+  if (a->n_q * (a->h_q / a->h_kv) > 0x7fffffff) return CGTP_ERR_SHAPE;
+  if (a->n_q_items < 0 || a->n_q_joins < 0 || a->n_q_slots < 0 || a->n_k_items < 0 || a->n_k_joins < 0 || a->n_k_slots < 0)
+    return CGTP_ERR_SHAPE;
+  if ((int64_t)std::max(a->n_q_items, a->n_k_items) * a->h_kv >= (1 << 24)) return CGTP_ERR_SHAPE;
+  if ((int64_t)a->n_q_joins * a->h_kv * cgtp_attn_rows(a->wide_q) >= (1 << 22) ||
+      (int64_t)a->n_k_joins * a->h_kv * cgtp_attn_rows(a->wide_k) >= (1 << 22))
+    return CGTP_ERR_SHAPE;
+  if ((a->n_q_items && !a->q_items) || (a->n_q_joins && !a->q_joins)) return CGTP_ERR_NULL;
+  if (a->n_q > 0 && (!a->q || !a->out)) return CGTP_ERR_NULL;
+  if (a->n_k > 0 && (!a->k || !a->v)) return CGTP_ERR_NULL;
+  if (a->slope && ((a->n_q > 0 && !a->pos_q) || (a->n_k > 0 && !a->pos_k))) return CGTP_ERR_NULL;
+  return CGTP_OK;
+}
+
+void launch(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) {
+  if (a.dtype == CGTP_F32) attn_launch_f32(a, w, s);
+  else if (a.dtype == CGTP_BF16) attn_launch_bf16(a, w, s);
+  else attn_launch_f16(a, w, s);
+}
+
+}  // namespace
+}  // namespace cgtp
+
+extern "C" {
+
+int cgtp_attn_rows(int wide) { return wide ? 128 : 32; }
+
+int64_t cgtp_attn_workspace_bytes(const cgtp_attn_args* a, int backward) {
+  using namespace cgtp;
+  if (attn_check(a) != CGTP_OK) return 0;
+  if (backward) return attn_layout(*a).bytes;
+  return (int64_t)a->n_q_slots * a->h_kv * cgtp_attn_rows(a->wide_q) * (a->dim + 2) * 4;
+}
+
+int cgtp_attn_forward(const cgtp_attn_args* a, void* stream) {
+  using namespace cgtp;
+  if (int rc = attn_check(a)) return rc;
+  if (a->n_q == 0) return CGTP_OK;
+  if (a->n_q_slots > 0 && !a->workspace) return CGTP_ERR_WORKSPACE;
+  launch(*a, nullptr, (hipStream_t)stream);
+  return hipGetLastError() == hipSuccess ? CGTP_OK : CGTP_ERR_LAUNCH;
+}
+
+int cgtp_attn_backward(const cgtp_attn_args* a, void* stream) {
+  using namespace cgtp;
+  if (int rc = attn_check(a)) return rc;
+  if ((a->n_k_items && !a->k_items) || (a->n_k_joins && !a->k_joins)) return CGTP_ERR_NULL;
+  if (a->n_q > 0 && (!a->lse || !a->grad_out)) return CGTP_ERR_NULL;
+  const AttnLayout l = attn_layout(*a);
+  if (l.bytes > 0 && !a->workspace) return CGTP_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  char* ws = (char*)a->workspace;
+  const AttnScratch w = {(float*)ws, (f32x4*)(ws + l.row_part), (f32x4*)(ws + l.key_part), (float*)(ws + l.slope_part),
+                         (float*)(ws + l.parts)};
+  launch(*a, &w, s);
+  if (a->slope) {
+    const unsigned blocks = (unsigned)blocks_of(a->n_q);
+    if (blocks && (a->grad_pos_q || a->grad_slope))
+      hipLaunchKernelGGL(attn_pos_kernel, dim3(blocks), dim3(256), 0, s, *a, w);
+    if (a->grad_slope) launch_partial_sum<float>(w.slope_part, a->grad_slope, blocks, a->h_q, s);
+    if (!a->same_pos && a->grad_pos_k && a->n_k > 0)
+      hipLaunchKernelGGL(attn_pos_k_kernel, dim3((unsigned)blocks_of(a->n_k)), dim3(192), 0, s, *a, w);
+  }
+  return hipGetLastError() == hipSuccess ? CGTP_OK : CGTP_ERR_LAUNCH;
+}
+
+}  // extern "C"

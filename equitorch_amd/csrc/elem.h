@@ -1,0 +1,80 @@
+// Element types of the operators on invariant features (embedding, attention, gated feed-forward): storage types, the
+// type sums are held in, and loads and stores of V consecutive elements as one transaction.
+#pragma once
+
+#include "cgtp_device.h"
+#include "cgtp_host.h"
+
+namespace cgtp {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+template <typename T> struct AccOf { using type = float; };
+template <> struct AccOf<double> { using type = double; };
+
+template <typename T, int V> struct ElemVec { typedef T type __attribute__((ext_vector_type(V))); };
+template <typename T> struct ElemVec<T, 1> { typedef T type; };
+
+// V consecutive elements, widened to the accumulation type.
+template <typename T, int V, typename A>
+__device__ __forceinline__ void load_elems(A (&dst)[V], const T* p) {
+  if constexpr (V == 1) {
+    dst[0] = (A)p[0];
+  } else {
+    const typename ElemVec<T, V>::type v = *reinterpret_cast<const typename ElemVec<T, V>::type*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) dst[i] = (A)v[i];
+  }
+}
+template <typename T, int V, typename A>
+__device__ __forceinline__ void store_elems(T* p, const A (&src)[V]) {
+  if constexpr (V == 1) {
+    p[0] = (T)src[0];
+  } else {
+    typename ElemVec<T, V>::type v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (T)src[i];
+    *reinterpret_cast<typename ElemVec<T, V>::type*>(p) = v;
+  }
+}
+
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+// N elements of T from an address aligned to an element only, the ones from `valid` on as zeros.  Vector loads from
+// such addresses are what the hardware does by itself; only a vector that crosses the end is taken apart.
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose { T v[N]; };
+
+template <typename R, typename T>
+__device__ __forceinline__ R load_part(const T* p, int64_t valid) {
+  constexpr int N = sizeof(R) / sizeof(T);
+  if (valid >= N) return __builtin_bit_cast(R, *reinterpret_cast<const Loose<T, N>*>(p));
+  T e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = i < valid ? p[i] : T(0);
+  R r;
+  __builtin_memcpy(&r, e, sizeof(R));
+  return r;
+}
+// The first `valid` of N elements to an address aligned to an element only.
+template <typename T, int N>
+__device__ __forceinline__ void store_part(T* p, const T (&e)[N], int64_t valid) {
+  if (valid >= N) {
+    Loose<T, N> v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v.v[i] = e[i];
+    *reinterpret_cast<Loose<T, N>*>(p) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < valid) p[i] = e[i];
+  }
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline int launch_status() { return hipGetLastError() == hipSuccess ? CGTP_OK : CGTP_ERR_LAUNCH; }
+
+}  // namespace cgtp

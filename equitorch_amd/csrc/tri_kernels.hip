@@ -667,16 +667,56 @@ int cgtp_abi_layout(int which, int64_t* out, int capacity) {
                                         CGTP_OFF(cgtp_uvl_gw_args, n_paths), CGTP_OFF(cgtp_uvl_gw_args, max_pairs),
                                         CGTP_OFF(cgtp_uvl_gw_args, dx), CGTP_OFF(cgtp_uvl_gw_args, dg),
                                         CGTP_OFF(cgtp_uvl_gw_args, cx), CGTP_OFF(cgtp_uvl_gw_args, cout)};
+  static const int64_t gff_args[] = {sizeof(cgtp_gff_args), CGTP_OFF(cgtp_gff_args, x), CGTP_OFF(cgtp_gff_args, w_gate),
+                                     CGTP_OFF(cgtp_gff_args, w_up), CGTP_OFF(cgtp_gff_args, w_down),
+                                     CGTP_OFF(cgtp_gff_args, gate), CGTP_OFF(cgtp_gff_args, up),
+                                     CGTP_OFF(cgtp_gff_args, mid), CGTP_OFF(cgtp_gff_args, out),
+                                     CGTP_OFF(cgtp_gff_args, grad_out), CGTP_OFF(cgtp_gff_args, grad_gate),
+                                     CGTP_OFF(cgtp_gff_args, grad_up), CGTP_OFF(cgtp_gff_args, grad_x),
+                                     CGTP_OFF(cgtp_gff_args, grad_w_gate), CGTP_OFF(cgtp_gff_args, grad_w_up),
+                                     CGTP_OFF(cgtp_gff_args, grad_w_down), CGTP_OFF(cgtp_gff_args, workspace),
+                                     CGTP_OFF(cgtp_gff_args, n_rows), CGTP_OFF(cgtp_gff_args, c_in),
+                                     CGTP_OFF(cgtp_gff_args, hidden), CGTP_OFF(cgtp_gff_args, c_out),
+                                     CGTP_OFF(cgtp_gff_args, activation), CGTP_OFF(cgtp_gff_args, dtype),
+                                     CGTP_OFF(cgtp_gff_args, reserved_)};
+  static const int64_t attn_args[] = {sizeof(cgtp_attn_args), CGTP_OFF(cgtp_attn_args, q), CGTP_OFF(cgtp_attn_args, k),
+                                      CGTP_OFF(cgtp_attn_args, v), CGTP_OFF(cgtp_attn_args, q_node),
+                                      CGTP_OFF(cgtp_attn_args, q_head), CGTP_OFF(cgtp_attn_args, k_node),
+                                      CGTP_OFF(cgtp_attn_args, k_head), CGTP_OFF(cgtp_attn_args, v_node),
+                                      CGTP_OFF(cgtp_attn_args, v_head), CGTP_OFF(cgtp_attn_args, pos_q),
+                                      CGTP_OFF(cgtp_attn_args, pos_k), CGTP_OFF(cgtp_attn_args, slope),
+                                      CGTP_OFF(cgtp_attn_args, out), CGTP_OFF(cgtp_attn_args, lse),
+                                      CGTP_OFF(cgtp_attn_args, q_items), CGTP_OFF(cgtp_attn_args, q_joins),
+                                      CGTP_OFF(cgtp_attn_args, k_items), CGTP_OFF(cgtp_attn_args, k_joins),
+                                      CGTP_OFF(cgtp_attn_args, n_q_items), CGTP_OFF(cgtp_attn_args, n_q_joins),
+                                      CGTP_OFF(cgtp_attn_args, n_q_slots), CGTP_OFF(cgtp_attn_args, n_k_items),
+                                      CGTP_OFF(cgtp_attn_args, n_k_joins), CGTP_OFF(cgtp_attn_args, n_k_slots),
+                                      CGTP_OFF(cgtp_attn_args, grad_out), CGTP_OFF(cgtp_attn_args, grad_q),
+                                      CGTP_OFF(cgtp_attn_args, grad_k), CGTP_OFF(cgtp_attn_args, grad_v),
+                                      CGTP_OFF(cgtp_attn_args, grad_pos_q), CGTP_OFF(cgtp_attn_args, grad_pos_k),
+                                      CGTP_OFF(cgtp_attn_args, grad_slope), CGTP_OFF(cgtp_attn_args, workspace),
+                                      CGTP_OFF(cgtp_attn_args, n_q), CGTP_OFF(cgtp_attn_args, n_k),
+                                      CGTP_OFF(cgtp_attn_args, h_q), CGTP_OFF(cgtp_attn_args, h_kv),
+                                      CGTP_OFF(cgtp_attn_args, dim), CGTP_OFF(cgtp_attn_args, dtype),
+                                      CGTP_OFF(cgtp_attn_args, wide_q), CGTP_OFF(cgtp_attn_args, wide_k),
+                                      CGTP_OFF(cgtp_attn_args, same_pos), CGTP_OFF(cgtp_attn_args, reserved_),
+                                      CGTP_OFF(cgtp_attn_args, scale), CGTP_OFF(cgtp_attn_args, cap)};
+  static const int64_t attn_item[] = {sizeof(cgtp_attn_item), CGTP_OFF(cgtp_attn_item, node),
+                                      CGTP_OFF(cgtp_attn_item, row_begin), CGTP_OFF(cgtp_attn_item, row_end),
+                                      CGTP_OFF(cgtp_attn_item, k_begin), CGTP_OFF(cgtp_attn_item, k_end),
+                                      CGTP_OFF(cgtp_attn_item, slot), CGTP_OFF(cgtp_attn_item, first),
+                                      CGTP_OFF(cgtp_attn_item, count)};
 #undef CGTP_OFF
   const int64_t* tabs[] = {operand, tri, gen_operand, gen, uvu, uvt_item, uvt, uvt_gw, uvt_gy, uvu_tab, psw_table,
-                           psw_args, uvu_mx, uvl_args, uvg_args, uvl_gw_args};
+                           psw_args, uvu_mx, uvl_args, uvg_args, uvl_gw_args, nullptr, gff_args, attn_args, attn_item};
   const int counts[] = {(int)(sizeof(operand) / 8), (int)(sizeof(tri) / 8), (int)(sizeof(gen_operand) / 8),
                         (int)(sizeof(gen) / 8), (int)(sizeof(uvu) / 8), (int)(sizeof(uvt_item) / 8),
                         (int)(sizeof(uvt) / 8), (int)(sizeof(uvt_gw) / 8), (int)(sizeof(uvt_gy) / 8),
                         (int)(sizeof(uvu_tab) / 8), (int)(sizeof(psw_table) / 8), (int)(sizeof(psw_args) / 8), (int)(sizeof(uvu_mx) / 8),
                         (int)(sizeof(uvl_args) / 8), (int)(sizeof(uvg_args) / 8),
-                        (int)(sizeof(uvl_gw_args) / 8)};
-  if (which < 0 || which >= 16) return -1;
+                        (int)(sizeof(uvl_gw_args) / 8), 0, (int)(sizeof(gff_args) / 8),
+                        (int)(sizeof(attn_args) / 8), (int)(sizeof(attn_item) / 8)};
+  if (which < 0 || which > CGTP_LAYOUT_ATTN_ITEM || !tabs[which]) return -1;
   for (int i = 0; out && i < counts[which] && i < capacity; ++i) out[i] = tabs[which][i];
   return counts[which];
 }

@@ -42,7 +42,8 @@ int cgtp_version(void);
  * in declaration order to out[0 .. capacity) and returns how many numbers the full description has (-1: bad id). */
 enum { CGTP_LAYOUT_OPERAND = 0, CGTP_LAYOUT_TRI_ARGS = 1, CGTP_LAYOUT_GEN_OPERAND = 2, CGTP_LAYOUT_GEN_ARGS = 3,
        CGTP_LAYOUT_UVU_ARGS = 4, CGTP_LAYOUT_UVT_ITEM = 5, CGTP_LAYOUT_UVT_ARGS = 6, CGTP_LAYOUT_UVT_GW_ARGS = 7,
-       CGTP_LAYOUT_UVT_GY_ARGS = 8, CGTP_LAYOUT_UVU_TABLE = 9, CGTP_LAYOUT_PSW_TABLE = 10, CGTP_LAYOUT_PSW_ARGS = 11 };
+       CGTP_LAYOUT_UVT_GY_ARGS = 8, CGTP_LAYOUT_UVU_TABLE = 9, CGTP_LAYOUT_PSW_TABLE = 10, CGTP_LAYOUT_PSW_ARGS = 11,
+       CGTP_LAYOUT_GFF_ARGS = 17, CGTP_LAYOUT_ATTN_ARGS = 18, CGTP_LAYOUT_ATTN_ITEM = 19 };   /* 16: none */
 int cgtp_abi_layout(int which, int64_t* out, int capacity);
 
 /* ---- generic sparse trilinear contraction -------------------------------------------------------------
@@ -757,6 +758,88 @@ int cgtp_wigner_rotate_backward(const void* x, const void* grad_out, const void*
                                 const int32_t* irrep_degree, int n_irreps, int64_t n_rows, int C, int cs_dim,
                                 void* grad_x, void* grad_alpha, void* grad_beta, void* grad_gamma, int dtype,
                                 void* stream);
+
+/* ---- embedding of node kinds ---------------------------------------------------------------------------------
+ *   out[i, c] = scale * table[kind[i], c]
+ * cgtp_embed_backward: grad_table[t, c] = scale * sum over the rows i of kind t of grad_out[i, c], every row of
+ * grad_table written; summed in fp32 (fp64 for CGTP_F64) in an order that the kinds alone determine (no atomics).
+ * A kind outside 0 .. n_kinds - 1 gives zeros and no gradient.  kind: (n_rows) int64, table / grad_table: (n_kinds, C),
+ * out / grad_out: (n_rows, C), all contiguous; n_rows < 2^31, C < 2^15.  The backward's workspace:
+ * cgtp_embed_workspace_bytes, 16-byte aligned.  dtype: any.
+ */
+int64_t cgtp_embed_workspace_bytes(int64_t n_rows, int64_t n_kinds, int C, int dtype);
+int cgtp_embed_forward(const int64_t* kind, const void* table, void* out, int64_t n_rows, int64_t n_kinds, int C,
+                       double scale, int dtype, void* stream);
+int cgtp_embed_backward(const int64_t* kind, const void* grad_out, void* grad_table, void* workspace, int64_t n_rows,
+                        int64_t n_kinds, int C, double scale, int dtype, void* stream);
+
+/* ---- gated feed-forward block on invariant channels -------------------------------------------------------------
+ *   g = x Wg,  u = x Wu,  m = act(g) * u,  out = m Wd
+ * x: (n_rows, c_in); w_gate, w_up: (c_in, hidden); w_down: (hidden, c_out); out: (n_rows, c_out), all contiguous, aligned to
+ * an element.  Products and the activation in fp32; mid (and gate, up), which the forward leaves for the next product
+ * and for the backward, are (n_rows, hidden) in the operands' type.  gate and up NULL: not wanted (inference).
+ * cgtp_gff_backward reads gate, up and mid, writes grad_gate and grad_up (buffers of the caller, (n_rows, hidden)) and those
+ * of grad_x, grad_w_gate, grad_w_up, grad_w_down that are not NULL; the weight gradients are summed over rows in a
+ * fixed order.  workspace: cgtp_gff_workspace_bytes (0: may be NULL), 16-byte aligned.
+ * n_rows < 2^31, c_in and c_out < 2^15, hidden < 2^17.  dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16.
+ */
+enum { CGTP_ACT_SILU = 0, CGTP_ACT_GELU = 1 /* with the error function */, CGTP_ACT_SIGMOID = 2 };
+typedef struct {
+  const void *x, *w_gate, *w_up, *w_down;
+  void *gate, *up, *mid, *out;
+  const void* grad_out;
+  void *grad_gate, *grad_up, *grad_x, *grad_w_gate, *grad_w_up, *grad_w_down, *workspace;
+  int64_t n_rows;
+  int32_t c_in, hidden, c_out, activation, dtype, reserved_;
+} cgtp_gff_args;
+int64_t cgtp_gff_workspace_bytes(const cgtp_gff_args* args);
+int cgtp_gff_forward(const cgtp_gff_args* args, void* stream);
+int cgtp_gff_backward(const cgtp_gff_args* args, void* stream);
+
+/* ---- attention among the nodes of a structure ---------------------------------------------------------------------
+ * Nodes of many structures lie one after the other; every query of a structure sees all keys of the same structure:
+ *   s_ij = cap tanh(scale q_i.k_j / cap) - slope_h |r_i - r_j|     (cap <= 0: scale q_i.k_j;  slope NULL: no distance)
+ *   out_i = sum_j softmax_j(s_ij) v_j,  lse_i = log2 of the sum of 2^(s log2 e);  no key, or every score -inf: out_i = 0 and
+ *   lse_i = +inf.
+ * q: (n_q, h_q, dim), k and v: (n_k, h_kv, dim), h_q a multiple of h_kv (query head h reads head h / (h_q / h_kv)), with
+ * element strides *_node and *_head and contiguous along dim; out, grad_out and the gradients contiguous; lse (n_q, h_q)
+ * fp32; pos_q (n_q, 3), pos_k (n_k, 3), slope (h_q) fp32.  lse NULL: not wanted.  Elements may lie anywhere an element may.  dim <= 128.
+ *
+ * The caller cuts the work into items.  The rows of a structure and a head of keys are its (query, query head) pairs, row =
+ * query * (h_q / h_kv) + head.  q_items: tiles of at most cgtp_attn_rows(wide_q) rows against a range of keys, which the
+ * forward and the gradient of q walk; k_items: at most cgtp_attn_rows(wide_k) keys against a range of rows.  An item that
+ * covers all keys (rows) of its structure writes its result and has slot -1 and first 0; one that covers a part has a
+ * slot of its own, where it leaves partial results, and first = its place among the pieces of its tile; one entry of q_joins /
+ * k_joins adds the slots first .. first + count - 1 of a tile, in that order.  A structure without keys has items with an
+ * empty range.  Every query and every key belongs to exactly one tile.
+ * workspace: cgtp_attn_workspace_bytes(args, backward), 16-byte aligned (0: may be NULL).
+ * cgtp_attn_backward writes grad_q, grad_k, grad_v and, with slope, grad_slope (h_q) and grad_pos_q (n_q, 3) where they are
+ * not NULL; same_pos != 0: the queries' and the keys' positions are one tensor, and grad_pos_q is the whole gradient, else
+ * grad_pos_k (n_k, 3) is that of pos_k.  All sums have an order that the arguments alone determine.
+ * dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16.
+ */
+typedef struct { int32_t node, row_begin, row_end, k_begin, k_end, slot, first, count; } cgtp_attn_item;
+/* q_items / q_joins: node = first query of the structure, rows row_begin .. row_end - 1 of it, keys k_begin .. k_end - 1.
+ * k_items / k_joins: keys k_begin .. k_end - 1 (a tile), the structure's first query and rows.  count: joins only. */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_node, q_head, k_node, k_head, v_node, v_head;
+  const float *pos_q, *pos_k, *slope;
+  void *out, *lse;
+  const cgtp_attn_item *q_items, *q_joins, *k_items, *k_joins;
+  int32_t n_q_items, n_q_joins, n_q_slots, n_k_items, n_k_joins, n_k_slots;
+  const void* grad_out;
+  void *grad_q, *grad_k, *grad_v;
+  float *grad_pos_q, *grad_pos_k, *grad_slope;
+  void* workspace;
+  int64_t n_q, n_k;
+  int32_t h_q, h_kv, dim, dtype, wide_q, wide_k, same_pos, reserved_;
+  float scale, cap;
+} cgtp_attn_args;
+int cgtp_attn_rows(int wide);
+int64_t cgtp_attn_workspace_bytes(const cgtp_attn_args* args, int backward);
+int cgtp_attn_forward(const cgtp_attn_args* args, void* stream);
+int cgtp_attn_backward(const cgtp_attn_args* args, void* stream);
 
 #ifdef __cplusplus
 }

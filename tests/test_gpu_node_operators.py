@@ -1,0 +1,439 @@
+"""Embedding of node kinds, attention among the nodes of a structure and the gated feed-forward block against plain
+implementations in 64 bits on the CPU.
+
+Tolerances are bounds on rounding, element by element: the result's own rounding, plus a number of roundings of what the
+kernels hold in fewer bits times the sum of the magnitudes that enter the element (the same formula with absolute values)."""
+import pytest
+import torch
+
+from equitorch_amd._lib import CgtpError
+from helpers import stable_seed
+
+pytestmark = pytest.mark.gpu
+
+F32, F64, BF16, F16 = torch.float32, torch.float64, torch.bfloat16, torch.float16
+EPS = {F64: 2.0 ** -53, F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}      # half a unit in the last place
+TINY = {F64: 0.0, F32: 1e-37, BF16: 1e-37, F16: 2.0 ** -24}                      # below: subnormal
+
+
+def _rand(gen, *shape, dtype=F32, std=1.0):
+    return (torch.randn(*shape, generator=gen, dtype=F64) * std).to(dtype)
+
+
+def _within(got, want, bound, what):
+    got, want = got.detach().cpu().double(), want.double()
+    assert got.shape == want.shape, f"{what}: {tuple(got.shape)} vs {tuple(want.shape)}"
+    excess = ((got - want).abs() - bound).max() if want.numel() else torch.tensor(-1.0)
+    assert float(excess) <= 0 and torch.isfinite(got).all(), f"{what}: {float(excess):.3e} over the bound"
+
+
+# ---- embedding ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, F64, BF16, F16])
+@pytest.mark.parametrize("rows,kinds,channels", [(1, 1, 1), (30, 100, 64), (257, 3, 7), (5000, 255, 33), (4099, 256, 128),
+                                                 (20011, 1000, 24), (9000, 70001, 16), (130001, 5, 8), (700, 90, 1200)])
+def test_embedding(device, dtype, rows, kinds, channels):
+    from equitorch_amd.nn.functional import embedding
+    gen = torch.Generator().manual_seed(stable_seed(rows, kinds, channels))
+    # a few kinds hold most rows; a kind below zero and one beyond the table give zeros
+    kind = (torch.rand(rows, generator=gen, dtype=F64) ** 3 * kinds).long()
+    if rows > 20:
+        kind[3], kind[rows // 2] = -1, kinds
+    table, ct = _rand(gen, kinds, channels, dtype=dtype), _rand(gen, rows, channels, dtype=dtype)
+    scale = channels ** 0.5
+    t = table.to(device).requires_grad_(True)
+    out = embedding(kind.to(device), t, scale)
+    (grad,) = torch.autograd.grad(out, t, ct.to(device))
+    ok = ((kind >= 0) & (kind < kinds)).double()[:, None]
+    at = kind.clamp(0, kinds - 1)
+    want = table.double()[at] * scale * ok
+    unit = EPS[F64] if dtype == F64 else EPS[F32]
+    _within(out, want, (EPS[dtype] + 2 * unit) * want.abs() + TINY[dtype], "out")
+    sums, size = torch.zeros(kinds, channels, dtype=F64), torch.zeros(kinds, channels, dtype=F64)
+    sums.index_add_(0, at, ct.double() * scale * ok)
+    size.index_add_(0, at, (ct.double() * scale * ok).abs())
+    # the chunks' sums and their sum: no element is added in a chain longer than its kind's rows
+    count = torch.bincount(at, minlength=kinds).double()[:, None]
+    _within(grad, sums, EPS[dtype] * sums.abs() + (count + 4) * unit * size + TINY[dtype], "grad")
+    (again,) = torch.autograd.grad(embedding(kind.to(device), t, scale), t, ct.to(device))
+    assert torch.equal(again, grad)
+
+
+def test_embedding_shapes_and_second_order(device):
+    from equitorch_amd.nn.functional import embedding
+    gen = torch.Generator().manual_seed(5)
+    kind = torch.randint(0, 9, (4, 5), generator=gen)
+    table = _rand(gen, 9, 6).to(device).requires_grad_(True)
+    assert embedding(kind.to(device), table).shape == (4, 5, 6)
+    assert embedding(torch.zeros(0, dtype=torch.int64, device=device), table).shape == (0, 6)
+    (empty,) = torch.autograd.grad(embedding(torch.zeros(0, dtype=torch.int64, device=device), table).sum(), table)
+    assert torch.equal(empty, torch.zeros_like(empty))
+    # an unaligned table: rows from an offset that is no multiple of 16 bytes
+    loose = torch.empty(9 * 6 + 1, device=device)[1:].view(9, 6).copy_(table.detach()).requires_grad_(True)
+    assert torch.equal(embedding(kind.to(device), loose), embedding(kind.to(device), table))
+    ct = _rand(gen, 4, 5, 6).to(device).requires_grad_(True)
+    (g,) = torch.autograd.grad(embedding(kind.to(device), table, 2.0), table, ct, create_graph=True)
+    v = _rand(gen, 9, 6).to(device)
+    (gg,) = torch.autograd.grad((g * v).sum(), ct)
+    assert torch.equal(gg, 2.0 * v[kind.to(device)])
+
+
+def test_embedding_refuses(device):
+    from equitorch_amd.nn.functional import embedding
+    kind, table = torch.zeros(3, dtype=torch.int64, device=device), torch.zeros(4, 5, device=device)
+    for bad in ((kind.int(), table), (kind, table[0]), (kind, table.long()), (kind, table[:0]), (kind.cpu(), table),
+                (kind, table.cpu())):
+        with pytest.raises(CgtpError):
+            embedding(*bad)
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------
+def _reference(q, k, v, len_q, len_k, pos, pos_k, slope, scale, cap, ct):
+    """``{name: (value, bound on rounding in units)}``: the magnitudes are sums of absolute values, once for what is rounded
+    to the operands' type and once for what errs in fp32 (the scores)."""
+    q, k, v, ct = (t.double() for t in (q, k, v, ct))
+    group = q.shape[1] // k.shape[1]
+    z = torch.zeros_like
+    names = ("out", "q", "k", "v")
+    val = {"out": z(q), "q": z(q), "k": z(k), "v": z(v)}
+    mag = {n: z(t) for n, t in val.items()}
+    if slope is not None:
+        pos, pos_k, slope = pos.double(), pos_k.double(), slope.double()
+        for n, t in (("pos", pos), ("pos_k", pos_k), ("slope", slope)):
+            val[n], mag[n] = z(t), z(t)
+    top = 0.0
+    a = b = 0
+    for lq, lk in zip(len_q, len_k):
+        rq, rk = slice(a, a + lq), slice(b, b + lk)
+        a, b = a + lq, b + lk
+        if not lq or not lk:
+            continue
+        for h in range(q.shape[1]):
+            hk = h // group
+            x = q[rq, h] @ k[rk, hk].T * scale
+            th = torch.tanh(x / cap) if cap else z(x)
+            s = cap * th if cap else x
+            if slope is not None:
+                delta = pos[rq, None] - pos_k[None, rk]
+                dist = delta.norm(dim=-1)
+                unit = torch.where(dist[..., None] > 0, delta / dist[..., None].clamp(min=1e-300), z(delta))
+                s = s - slope[h] * dist
+            top = max(top, float(s.abs().max()), float((q[rq, h].abs() @ k[rk, hk].abs().T * scale).max()))
+            p = torch.softmax(s, 1)
+            o = p @ v[rk, hk]
+            val["out"][rq, h], mag["out"][rq, h] = o, p @ v[rk, hk].abs()
+            g = ct[rq, h]
+            dp = g @ v[rk, hk].T
+            ds = p * (dp - (p * dp).sum(1, keepdim=True))
+            size = p * (g.abs() @ v[rk, hk].abs().T + (g.abs() * mag["out"][rq, h]).sum(1, keepdim=True))
+            val["v"][rk, hk] += p.T @ g
+            mag["v"][rk, hk] += p.T @ g.abs()
+            if slope is not None:
+                val["slope"][h] -= (ds * dist).sum()
+                mag["slope"][h] += (size * dist).sum()
+                pull, most = -slope[h] * ds[..., None] * unit, slope[h].abs() * size[..., None] * unit.abs()
+                val["pos"][rq] += pull.sum(1)
+                mag["pos"][rq] += most.sum(1)
+                val["pos_k"][rk] -= pull.sum(0)
+                mag["pos_k"][rk] += most.sum(0)
+            ds = ds * (1 - th * th)
+            val["q"][rq, h], mag["q"][rq, h] = scale * ds @ k[rk, hk], scale * size @ k[rk, hk].abs()
+            val["k"][rk, hk] += scale * ds.T @ q[rq, h]
+            mag["k"][rk, hk] += scale * size.T @ q[rq, h].abs()
+    return val, mag, top
+
+
+LENGTHS = {
+    "one": ([1], [1]),
+    "short": ([3, 0, 1, 17, 31, 32, 33, 2], None),
+    "odd": ([65, 130, 7, 64, 1], None),
+    "long": ([700], None),
+    "readout": ([1, 1, 1, 1, 0], [5, 0, 63, 300, 4]),
+    "one_long": ([1], [5003]),
+    "few_keys": ([1500, 2], [3, 1]),
+    "mixed": ([129, 0, 40], [0, 9, 260]),
+}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,biased,cap", [
+    ("one", 1, 1, 1, True, 0.0), ("short", 8, 8, 16, True, 0.0), ("short", 6, 2, 13, True, 5.0), ("odd", 4, 4, 32, True, 4.0),
+    ("odd", 4, 1, 64, False, 0.0), ("long", 2, 1, 72, True, 3.0), ("long", 2, 2, 128, False, 0.0), ("readout", 8, 8, 32, True, 0.0),
+    ("readout", 8, 2, 64, False, 2.0), ("one_long", 8, 2, 64, True, 30.0), ("one_long", 2, 2, 100, False, 0.0),
+    ("few_keys", 4, 2, 24, True, 0.0), ("mixed", 3, 3, 96, True, 6.0), ("mixed", 4, 4, 8, False, 0.0)])
+def test_attention(device, dtype, lengths, heads, kv_heads, dim, biased, cap):
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    len_q, len_k = LENGTHS[lengths]
+    own = len_k is None
+    len_k = len_q if own else len_k
+    nq, nk = sum(len_q), sum(len_k)
+    gen = torch.Generator().manual_seed(stable_seed(lengths, heads, kv_heads, dim))
+    # slices of wider tensors: rows, heads and the start of a row lie anywhere
+    q = _rand(gen, nq, heads + 1, dim + 3, dtype=dtype)
+    kv = _rand(gen, nk, 2 * kv_heads, dim + 1, dtype=dtype)
+    ct = _rand(gen, nq, heads, dim, dtype=dtype)
+    pos = _rand(gen, nq, 3, std=2.0) if biased else None
+    pos_k = (pos if own else _rand(gen, nk, 3, std=2.0)) if biased else None
+    slope = torch.rand(heads, generator=gen) if biased else None
+    cut = lambda q, kv: (q[:, 1:, 2:dim + 2], kv[:, :kv_heads, 1:], kv[:, kv_heads:, 1:])
+    scale = dim ** -0.5
+    val, mag, top = _reference(*cut(q, kv), len_q, len_k, pos, pos_k, slope, scale, cap, ct)
+
+    ptr = lambda n: torch.tensor([0] + n, device=device).cumsum(0)
+    plan = AttentionPlan(ptr(len_q)) if own else AttentionPlan(ptr(len_q), ptr(len_k))
+    leaves = [t.detach().requires_grad_(True) for t in cut(q.to(device), kv.to(device))]
+    more = [None if t is None else t.to(device).requires_grad_(True) for t in (pos, None if own else pos_k, slope)]
+    run = lambda: segment_attention(*leaves, plan, pos=more[0], pos_k=more[1], slope=more[2], cap=cap or None)
+    out = run()
+    wrt = leaves + [t for t in more if t is not None]
+    grads = torch.autograd.grad(out, wrt, ct.to(device))
+    names = ["q", "k", "v"] + [n for n, t in zip(("pos", "pos_k", "slope"), more) if t is not None]
+    if biased and own:
+        val["pos"], mag["pos"] = val["pos"] + val["pos_k"], mag["pos"] + mag["pos_k"]
+    # 16-bit: the probability, the score's gradient, the output inside delta and one more rounding of each term; fp32: the sums
+    # over dim and the keys, and the score's error, which moves every probability
+    unit = 4 * EPS[dtype] + EPS[F32] * (32 + dim + 16 * top) if dtype != F32 else EPS[F32] * (32 + dim + 16 * top)
+    for name, got in zip(["out"] + names, [out, *grads]):
+        own_type = EPS[F32] if name in ("pos", "pos_k", "slope") else EPS[dtype]
+        _within(got, val[name], own_type * val[name].abs() + unit * mag[name] + 64 * TINY[dtype], name)
+    again = torch.autograd.grad(run(), wrt, ct.to(device))
+    assert all(torch.equal(a, b) for a, b in zip(again, grads))
+    with torch.no_grad():
+        assert torch.equal(run(), out)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attention_structures_do_not_touch(device, dtype, bad):
+    """What one structure holds does not reach another, whatever it is."""
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    gen = torch.Generator().manual_seed(3)
+    lengths = [9, 20, 70, 5]
+    n = sum(lengths)
+    plan = AttentionPlan(torch.tensor([0] + lengths, device=device).cumsum(0))
+    data = [_rand(gen, n, 2, 32, dtype=dtype).to(device) for _ in range(4)]
+    pos, slope = _rand(gen, n, 3).to(device), torch.rand(2, generator=gen).to(device)
+
+    def run(tensors, pos):
+        q, k, v = (t.clone().requires_grad_(True) for t in tensors[:3])
+        p = pos.clone().requires_grad_(True)
+        out = segment_attention(q, k, v, plan, pos=p, slope=slope)
+        return (out, *torch.autograd.grad(out, (q, k, v, p), tensors[3]))
+    clean = run(data, pos)
+    rows = slice(9, 29)                                    # the second structure
+    spoiled = [t.clone() for t in data]
+    for t in spoiled:
+        t[rows] = bad
+    p = pos.clone()
+    p[rows] = bad
+    keep = torch.ones(n, dtype=torch.bool, device=device)
+    keep[rows] = False
+    for a, b in zip(clean, run(spoiled, p)):
+        assert torch.equal(a[keep], b[keep])
+
+
+def test_attention_scores_out_of_range(device):
+    """Scores of -inf mask a key; a row of nothing else is zeros, and so are its gradients."""
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    q = torch.ones(4, 1, 8, device=device).requires_grad_(True)
+    k = torch.ones(4, 1, 8, device=device)
+    k[2:] = -torch.inf
+    v = torch.arange(32.0, device=device).view(4, 1, 8)
+    plan = AttentionPlan(torch.tensor([0, 3, 4], device=device))
+    out = segment_attention(q, k, v, plan)
+    assert torch.equal(out[:3, 0], v[:2, 0].mean(0).expand(3, 8)) and torch.equal(out[3], torch.zeros_like(out[3]))
+    finite = torch.full((4, 1, 8), -3.0e38, device=device)
+    far = segment_attention(q.detach() * 1e3, finite, v, plan)      # every score the lowest of the type, or -inf
+    assert torch.isfinite(far).all()
+
+
+def test_attention_differences(device):
+    """Gradients of a scalar against differences of the forward itself, and second order against differences of the first."""
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    gen = torch.Generator().manual_seed(11)
+    lengths = [5, 0, 12]
+    n = sum(lengths)
+    plan = AttentionPlan.from_batch(torch.repeat_interleave(torch.arange(3), torch.tensor(lengths)).to(device), 3)
+    data = [_rand(gen, n, 4, 16), _rand(gen, n, 2, 16), _rand(gen, n, 2, 16), _rand(gen, n, 3), torch.rand(4, generator=gen)]
+    step = [_rand(gen, *t.shape) for t in data]
+    ct = _rand(gen, n, 4, 16).to(device)
+
+    def value(eps, create_graph=False):
+        x = [(t + eps * d).to(device).requires_grad_(True) for t, d in zip(data, step)]
+        out = segment_attention(*x[:3], plan, pos=x[3], slope=x[4], cap=4.0)
+        return x, (out * ct).sum().double() if not create_graph else (out * ct).sum()
+
+    x, y = value(0.0, True)
+    grads = torch.autograd.grad(y, x, create_graph=True)
+    along = sum((g.double() * d.to(device).double()).sum() for g, d in zip(grads, step))
+    eps = 2.0 ** -7          # error eps^2 of the difference and 2^-24 * sqrt(sum) / eps of the values
+    diff = (value(eps)[1] - value(-eps)[1]) / (2 * eps)
+    assert abs(float(diff - along)) <= 5e-3 * (1 + abs(float(along)))
+    # second order: the gradient's change along the step
+    second = torch.autograd.grad(along, x)
+
+    def gradient(eps):
+        x, y = value(eps, True)
+        return torch.autograd.grad(y, x)
+    up, down = gradient(eps), gradient(-eps)
+    for s, a, b in zip(second, up, down):
+        want = (a.double() - b.double()) / (2 * eps)
+        assert float((s.double() - want).abs().max()) <= 2e-2 * (1 + float(want.abs().max()))
+
+
+def test_attention_refuses(device):
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    ptr = torch.tensor([0, 2, 6], device=device)
+    plan = AttentionPlan(ptr)
+    q, k, v = (torch.zeros(6, 2, 8, device=device) for _ in range(3))
+    pos, slope = torch.zeros(6, 3, device=device), torch.zeros(2, device=device)
+    segment_attention(q, k, v, plan, pos=pos, slope=slope, cap=1.0)
+    wrong = torch.zeros(6, 3, 8, device=device)
+    wide = torch.zeros(6, 2, 130, device=device)
+    for args, kw in (((q[:5], k, v, plan), {}), ((q, k[:5], v[:5], plan), {}), ((q, wrong, wrong, plan), {}), ((q, k, v[:, :1], plan), {}),
+                     ((wide, wide, wide, plan), {}), ((q.double(), k.double(), v.double(), plan), {}), ((q, k.bfloat16(), v, plan), {}),
+                     ((q.cpu(), k, v, plan), {}), ((q, k, v, plan), {"pos": pos}), ((q, k, v, plan), {"slope": slope}),
+                     ((q, k, v, plan), {"slope": slope[:1], "pos": pos}), ((q, k, v, plan), {"slope": slope, "pos": pos[:, :2]}),
+                     ((q, k, v, plan), {"slope": slope.double(), "pos": pos}), ((q, k, v, plan), {"cap": -1.0}),
+                     ((q, k, v, plan), {"cap": float("inf")}), ((q, k, v, plan), {"cap": float("nan")}),
+                     ((q, k, v, AttentionPlan(ptr, ptr)), {"slope": slope, "pos": pos})):
+        with pytest.raises(CgtpError):
+            segment_attention(*args, **kw)
+
+
+def test_attention_under_a_stream_and_a_graph(device):
+    from equitorch_amd.nn.functional import AttentionPlan, embedding, gated_feed_forward, segment_attention
+    gen = torch.Generator().manual_seed(7)
+    n = 90
+    kind, table = torch.randint(0, 9, (n,), generator=gen).to(device), _rand(gen, 9, 64).to(device)
+    plan = AttentionPlan(torch.tensor([0, 50, n], device=device))
+    pos, slope = _rand(gen, n, 3).to(device), torch.rand(2, generator=gen).to(device)
+    w = [_rand(gen, *s, std=0.1).to(device) for s in ((64, 96), (64, 96), (96, 64))]
+
+    def step(pos):
+        t = [x.detach().requires_grad_(True) for x in (table, pos, *w)]
+        x = embedding(kind, t[0]).view(n, 2, 32)
+        y = gated_feed_forward(segment_attention(x, x, x, plan, pos=t[1], slope=slope).reshape(n, 64), *t[2:])
+        return (y, *torch.autograd.grad((y * y).sum(), t))
+    want = [step(pos), step(2 * pos)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(pos)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    graph, given = torch.cuda.CUDAGraph(), pos.clone()
+    with torch.cuda.graph(graph):
+        kept = step(given)
+    for i in (0, 1, 0):
+        given.copy_((1 + i) * pos)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(kept, want[i]))
+        step(pos)                              # eager work between the replays
+
+
+# ---- gated feed-forward --------------------------------------------------------------------------------------------
+def _act64(name, u):
+    if name == "gelu":
+        cdf = 0.5 * (1 + torch.erf(u / 2 ** 0.5))
+        return u * cdf, cdf + u * torch.exp(-u * u / 2) / (2 * torch.pi) ** 0.5
+    s = torch.sigmoid(u)
+    return (u * s, s + u * s * (1 - s)) if name == "silu" else (s, s * (1 - s))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,c,h,co,activation", [(1, 256, 1024, 256, "silu"), (1, 1, 1, 1, "silu"), (7, 16, 33, 5, "gelu"),
+                                                    (16, 128, 512, 128, "silu"), (33, 70, 129, 65, "sigmoid"),
+                                                    (129, 129, 64, 130, "silu"), (1000, 64, 256, 64, "gelu"),
+                                                    (5003, 40, 72, 24, "silu"), (640, 256, 130, 256, "silu")])
+def test_gated_feed_forward(device, dtype, rows, c, h, co, activation):
+    from equitorch_amd.nn.functional import gated_feed_forward
+    gen = torch.Generator().manual_seed(stable_seed(rows, c, h, co))
+    x, ct = _rand(gen, rows, c, dtype=dtype), _rand(gen, rows, co, dtype=dtype)
+    ws = [_rand(gen, c, h, dtype=dtype, std=c ** -0.5), _rand(gen, c, h, dtype=dtype, std=c ** -0.5),
+          _rand(gen, h, co, dtype=dtype, std=h ** -0.5)]
+    leaves = [t.to(device).requires_grad_(True) for t in (x, *ws)]
+    out = gated_feed_forward(*leaves, activation)
+    grads = torch.autograd.grad(out, leaves, ct.to(device))
+    xd, gd, (wg, wu, wd) = x.double(), ct.double(), (t.double() for t in ws)
+    u, r = xd @ wg, xd @ wu
+    act, slope = _act64(activation, u)
+    mid = act * r
+    dm = gd @ wd.T
+    dg, du = dm * r * slope, dm * act
+    want = (mid @ wd, dg @ wg.T + du @ wu.T, xd.T @ dg, xd.T @ du, mid.T @ gd)
+    # magnitudes of what each factor errs by in units: the projections over their sums' sizes, the rest over its own
+    su, sr = xd.abs() @ wg.abs(), xd.abs() @ wu.abs()
+    sm = act.abs() * sr + 1.2 * su * r.abs()
+    sd = gd.abs() @ wd.abs().T
+    sg, sdu = sd * (r.abs() + sr) * 1.2 + dm.abs() * r.abs() * su, sd * act.abs() + dm.abs() * 1.2 * su
+    size = (sm @ wd.abs(), sg @ wg.abs().T + sdu @ wu.abs().T, xd.abs().T @ sg, xd.abs().T @ sdu, sm.T @ gd.abs())
+    # 16-bit: the projections, the product and its gradients are rounded once each; fp32: sums over the longest axis
+    unit = 4 * EPS[dtype] if dtype != F32 else EPS[F32] * (16 + max(c, h, co, rows) ** 0.5)
+    for name, got, w, s in zip(("out", "x", "w_gate", "w_up", "w_down"), (out, *grads), want, size):
+        _within(got, w, EPS[dtype] * w.abs() + unit * s + 64 * TINY[dtype], name)
+    with torch.no_grad():
+        assert torch.equal(gated_feed_forward(*leaves, activation), out)
+    again = torch.autograd.grad(gated_feed_forward(*leaves, activation), leaves, ct.to(device))
+    assert all(torch.equal(a, b) for a, b in zip(again, grads))
+
+
+def test_gated_feed_forward_layouts_and_higher_order(device):
+    from equitorch_amd.nn.functional import gated_feed_forward
+    gen = torch.Generator().manual_seed(9)
+    x, ws = _rand(gen, 3, 4, 10).to(device), [_rand(gen, *s, std=0.3).to(device) for s in ((10, 12), (10, 12), (12, 6))]
+    out = gated_feed_forward(x, *ws)
+    assert out.shape == (3, 4, 6)
+    # transposed weights and a strided x give the same
+    same = gated_feed_forward(x.transpose(0, 1).contiguous().transpose(0, 1), *[w.T.contiguous().T for w in ws])
+    assert torch.equal(out, same)
+    assert gated_feed_forward(x[:0], *ws).shape == (0, 4, 6)
+    leaves = [t.detach().requires_grad_(True) for t in (x[:0], *ws)]
+    for g in torch.autograd.grad(gated_feed_forward(*leaves).sum(), leaves):
+        assert torch.equal(g, torch.zeros_like(g))
+    # only some gradients wanted
+    w_only = [x, ws[0].detach().requires_grad_(True), ws[1], ws[2].detach().requires_grad_(True)]
+    part = torch.autograd.grad(gated_feed_forward(*w_only).sum(), [w_only[1], w_only[3]])
+    every = [t.detach().requires_grad_(True) for t in (x, *ws)]
+    full = torch.autograd.grad(gated_feed_forward(*every).sum(), every)
+    assert torch.equal(part[0], full[1]) and torch.equal(part[1], full[3])
+    # against differences, first and second order
+    step = [_rand(gen, *t.shape).to(device) for t in every]
+    ct = _rand(gen, 3, 4, 6).to(device)
+
+    def gradient(eps, create_graph=False):
+        t = [(a + eps * d).detach().requires_grad_(True) for a, d in zip((x, *ws), step)]
+        y = (gated_feed_forward(*t) * ct).sum()
+        return t, y, torch.autograd.grad(y, t, create_graph=create_graph)
+    eps = 2.0 ** -7
+    t, _, grads = gradient(0.0, True)
+    along = sum((g * d).sum() for g, d in zip(grads, step))
+    up, down = gradient(eps), gradient(-eps)
+    diff = (float(up[1]) - float(down[1])) / (2 * eps)
+    assert abs(diff - float(along)) <= 5e-3 * (1 + abs(diff))
+    for s, a, b in zip(torch.autograd.grad(along, t), up[2], down[2]):
+        want = (a - b) / (2 * eps)
+        assert float((s - want).abs().max()) <= 2e-2 * (1 + float(want.abs().max()))
+
+
+def test_gated_feed_forward_passes_on_what_is_not_finite(device):
+    """A row with a NaN spoils its own results and the weights' gradients, no other row's."""
+    from equitorch_amd.nn.functional import gated_feed_forward
+    gen = torch.Generator().manual_seed(2)
+    x = _rand(gen, 200, 48).to(device)
+    ws = [_rand(gen, *s, std=0.2).to(device) for s in ((48, 80), (48, 80), (80, 40))]
+    clean = gated_feed_forward(x, *ws)
+    x[77, 5] = float("nan")
+    out = gated_feed_forward(x, *ws)
+    keep = torch.arange(200, device=device) != 77
+    assert torch.equal(out[keep], clean[keep]) and torch.isnan(out[77]).all()
+
+
+def test_gated_feed_forward_refuses(device):
+    from equitorch_amd.nn.functional import gated_feed_forward
+    x, wg, wu, wd = (torch.zeros(*s, device=device) for s in ((3, 8), (8, 6), (8, 6), (6, 4)))
+    for bad in ((x, wg, wu[:, :5], wd), (x[:, :7], wg, wu, wd), (x, wg, wu, wd[:5]), (x.double(), wg.double(), wu.double(), wd.double()),
+                (x.bfloat16(), wg, wu, wd), (x.cpu(), wg, wu, wd), (x, wg[0], wu[0], wd), (x, wg[:, :0], wu[:, :0], wd[:0]),
+                (x, wg, wu, wd, "relu")):
+        with pytest.raises(CgtpError):
+            gated_feed_forward(*bad)
