@@ -1,5 +1,5 @@
 #include "attn_impl.h"
 
 namespace cgtp {
-void attn_launch_bf16(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) { launch_type<bf16_t>(a, w, s); }
+template void attn_launch<bf16_t, false, false>(const AttnLaunch&, const AttnScratch*, hipStream_t);
 }  // namespace cgtp

@@ -1,5 +1,5 @@
 #include "attn_impl.h"
 
 namespace cgtp {
-void attn_launch_f16(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) { launch_type<f16_t>(a, w, s); }
+template void attn_launch<f16_t, false, false>(const AttnLaunch&, const AttnScratch*, hipStream_t);
 }  // namespace cgtp

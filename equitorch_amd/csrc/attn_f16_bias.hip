@@ -1,0 +1,5 @@
+#include "attn_impl.h"
+
+namespace cgtp {
+template void attn_launch<f16_t, true, false>(const AttnLaunch&, const AttnScratch*, hipStream_t);
+}  // namespace cgtp

@@ -1,5 +1,5 @@
 #include "attn_impl.h"
 
 namespace cgtp {
-void attn_launch_f32(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) { launch_type<float>(a, w, s); }
+template void attn_launch<float, false, false>(const AttnLaunch&, const AttnScratch*, hipStream_t);
 }  // namespace cgtp

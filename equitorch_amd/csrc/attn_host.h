@@ -1,10 +1,14 @@
 // Host-side declarations shared by the translation units of the attention among the nodes of a structure.
 #pragma once
 
-#include "cgtp_device.h"
-#include "cgtp_host.h"
+#include "elem.h"
 
 namespace cgtp {
+
+// A call's arguments and what follows from them.
+struct AttnLaunch : cgtp_attn_args {
+  int fast;            // rows are whole 16-byte chunks, aligned, and a tile's offsets fit 31 bits
+};
 
 constexpr int kQSums = 10;     // what a piece leaves for each row besides the gradient of q (attn_impl.h, QSums)
 
@@ -17,9 +21,8 @@ struct AttnScratch {
   float* parts;        // partial results of pieces
 };
 
-// w null: forward.
-void attn_launch_f32(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s);
-void attn_launch_bf16(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s);
-void attn_launch_f16(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s);
+// w null: forward.  Defined in attn_impl.h, instantiated once for each type and kind of score.
+template <typename T, bool BIASED, bool CAPPED>
+void attn_launch(const AttnLaunch& a, const AttnScratch* w, hipStream_t s);
 
 }  // namespace cgtp

@@ -1,4 +1,5 @@
-// Kernels of the attention among the nodes of a structure for one element type (attn_f32.hip, attn_bf16.hip, attn_f16.hip).
+// Kernels of the attention among the nodes of a structure for one element type, with or without distances and cap (the
+// attn_<type>_*.hip: both are known when a kernel is compiled, a branch on them costs more than what it leaves out).
 //
 //   t_ij = log2(e) s_ij,  s_ij = cap tanh(scale q_i.k_j / cap) - slope_h |r_i - r_j|
 //   out_i = sum_j 2^(t_ij - lse_i) v_j,  lse_i = log2 sum_j 2^t_ij
@@ -27,22 +28,22 @@ namespace {
 constexpr float kLog2E = 1.4426950408889634f;
 
 template <int NW> constexpr int kRowsOf = 32 * NW;
+template <int NW> constexpr int kBlockOf = NW == 1 ? 32 : 64;      // rows of a tile in LDS
 
-// What scores are made of, in units of log2(e).
+// What scores are made of.  A score in units of 1 / unit binary orders: t = q.k where that is all (linear > 0, which then is
+// the unit), else in binary orders: t = linear q.k or outer tanh, less slope |r_i - r_j|.
+template <bool BIASED, bool CAPPED>
 struct ScoreScale {
-  float linear;        // cap <= 0: t = linear * q.k
-  float inner, outer;  // else t = outer - 2 outer / (2^(inner q.k) + 1)
-  bool capped, biased;
+  static constexpr bool biased = BIASED, capped = CAPPED;
+  float linear, inner, outer, unit;
+  __device__ __forceinline__ explicit ScoreScale(const AttnLaunch& a) {
+    linear = a.scale * kLog2E;
+    inner = capped ? 2.f * kLog2E * a.scale / a.cap : 0.f;
+    outer = a.cap * kLog2E;
+    unit = plain() ? linear : 1.f;
+  }
+  __device__ __forceinline__ bool plain() const { return !capped && !biased && linear > 0.f; }
 };
-__device__ __forceinline__ ScoreScale score_scale(const cgtp_attn_args& a) {
-  ScoreScale s;
-  s.capped = a.cap > 0.f;
-  s.biased = a.slope != nullptr;
-  s.linear = a.scale * kLog2E;
-  s.inner = s.capped ? 2.f * kLog2E * a.scale / a.cap : 0.f;
-  s.outer = a.cap * kLog2E;
-  return s;
-}
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // tanh of half of what `inner` makes of q.k.
 __device__ __forceinline__ float capped_tanh(float inner_qk) {
@@ -63,23 +64,61 @@ __device__ __forceinline__ Row row_of(const cgtp_attn_item& it, int r, int kv_he
   return o;
 }
 
+// The keys of a tile, from k0 on, n of them.
+template <typename T>
+struct KeyRows {
+  const T* base;
+  int64_t node;
+  int n;
+  __device__ __forceinline__ KeyRows(const T* p, int64_t node, int64_t head, int hk, int k0, int n)
+      : base(p + (int64_t)k0 * node + hk * head), node(node), n(n) {}
+  __device__ __forceinline__ unsigned offset(int i) const { return i < n ? (unsigned)i * (unsigned)(node * sizeof(T)) : kNoRow; }
+  __device__ __forceinline__ const T* pointer(int i) const { return i < n ? base + i * node : nullptr; }
+};
+// The rows of a tile, from r0 on, n of them: query0 + (at + i) / group, head (at + i) % group of the kv head's.
+template <typename T>
+struct QueryRows {
+  const T* base;       // first query's first head
+  int64_t node, head;
+  int n, at, group;
+  float inv;
+  __device__ __forceinline__ QueryRows(const T* p, int64_t node, int64_t head, int first_query, int hk, int group, int r0, int n)
+      : node(node), head(head), n(n), at(r0 % group), group(group), inv(1.f / (float)group) {
+    base = p + (int64_t)(first_query + r0 / group) * node + (int64_t)hk * group * head;
+  }
+  // Quotients of small numbers: (x + 1 / 2) / group is at least 1 / (2 group) away from an integer.
+  __device__ __forceinline__ int query(int i) const { return (int)(((float)(at + i) + 0.5f) * inv); }
+  __device__ __forceinline__ unsigned offset(int i) const {
+    const int q = query(i), h = at + i - q * group;
+    return i < n ? (unsigned)q * (unsigned)(node * sizeof(T)) + (unsigned)h * (unsigned)(head * sizeof(T)) : kNoRow;
+  }
+  __device__ __forceinline__ const T* pointer(int i) const {
+    const int q = query(i), h = at + i - q * group;
+    return i < n ? base + q * node + h * head : nullptr;
+  }
+};
+
+// One tile buffer of LDS where two would not leave room for two workgroups.
+template <int BYTES> constexpr int kBuffers = 2 * BYTES <= 64 * 1024 ? 2 : 1;
+
 // ---- forward ----------------------------------------------------------------------------------------------------
-template <typename T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW) attn_fwd_kernel(cgtp_attn_args a, float* __restrict__ parts) {
+template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
+__global__ void __launch_bounds__(64 * NW, (sizeof(T) == 2 && NW == 4) || DP <= 64 ? 2 : 1)
+attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
   using S = AttnShape<T, DP>;
-  __shared__ alignas(16) char k_rows[S::kRowsBytes];
-  __shared__ alignas(16) char v_tile[S::kTransposed ? S::kColsBytes : S::kRowsBytes];
-  __shared__ alignas(16) float pos[3][kBlock];
+  constexpr int kBlock = kBlockOf<NW>, kTile = kBlock * S::kRow, kBuf = kBuffers<2 * kTile>;
+  __shared__ alignas(16) char tiles[kBuf][2][kTile];
+  __shared__ alignas(16) float pos[2][3][kBlock];
   const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
   const cgtp_attn_item it = a.q_items[blockIdx.x / a.h_kv];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
   const int r = it.row_begin + wave * 32 + (lane & 31);
   const Row row = row_of(it, r, hk, group);
-  const ScoreScale sc = score_scale(a);
+  const ScoreScale<BIASED, CAPPED> sc(a);
   RowFrag<T, DP> q;
   q.load(row.ok ? (const T*)a.q + row.query * a.q_node + row.head * a.q_head : nullptr, a.dim);
   float x = 0.f, y = 0.f, z = 0.f, slope = 0.f;
-  if (sc.biased && row.ok) {
+  if (BIASED && row.ok) {
     x = a.pos_q[(int64_t)row.query * 3];
     y = a.pos_q[(int64_t)row.query * 3 + 1];
     z = a.pos_q[(int64_t)row.query * 3 + 2];
@@ -90,41 +129,52 @@ __global__ void __launch_bounds__(64 * NW) attn_fwd_kernel(cgtp_attn_args a, flo
   for (int o = 0; o < S::kOut; ++o)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[o][e] = 0.f;
-  float top = -INFINITY, sum = 0.f;           // of this lane's keys (sum), of the row's (top)
-  const T* kp = (const T*)a.k + hk * a.k_head;
-  const T* vp = (const T*)a.v + hk * a.v_head;
-  for (int k0 = it.k_begin; k0 < it.k_end; k0 += kBlock) {
+  float top = -INFINITY, sum = 0.f;           // of the row's keys (top), of this lane's (sum)
+  TileStage<T, DP, 64 * NW, kBlock> ks, vs;
+  float ps[3] = {};
+  auto fetch = [&](int k0) {
     const int n = it.k_end - k0;
-    __syncthreads();
-    stage_rows<T, DP, 64 * NW>(k_rows, a.dim, [&](int i) { return i < n ? kp + (int64_t)(k0 + i) * a.k_node : nullptr; });
-    if constexpr (S::kTransposed)
-      stage_cols<T, DP, 64 * NW>(v_tile, a.dim, [&](int i) { return i < n ? vp + (int64_t)(k0 + i) * a.v_node : nullptr; });
-    else
-      stage_rows<T, DP, 64 * NW>(v_tile, a.dim, [&](int i) { return i < n ? vp + (int64_t)(k0 + i) * a.v_node : nullptr; });
-    if (sc.biased)
-      for (int i = threadIdx.x; i < kBlock; i += 64 * NW)
+    const KeyRows<T> kr((const T*)a.k, a.k_node, a.k_head, hk, k0, n), vr((const T*)a.v, a.v_node, a.v_head, hk, k0, n);
+    ks.load(a.fast, kr.base, a.dim, [&](int i) { return kr.offset(i); }, [&](int i) { return kr.pointer(i); });
+    vs.load(a.fast, vr.base, a.dim, [&](int i) { return vr.offset(i); }, [&](int i) { return vr.pointer(i); });
+    if (BIASED && threadIdx.x < kBlock)
 #pragma unroll
-        for (int d = 0; d < 3; ++d) pos[d][i] = i < n ? a.pos_k[(int64_t)(k0 + i) * 3 + d] : 0.f;
+      for (int d = 0; d < 3; ++d) ps[d] = (int)threadIdx.x < n ? a.pos_k[(int64_t)(k0 + threadIdx.x) * 3 + d] : 0.f;
+  };
+  if (it.k_begin < it.k_end) fetch(it.k_begin);
+  int buf = 0;
+  for (int k0 = it.k_begin; k0 < it.k_end; k0 += kBlock, buf ^= 1) {
+    const int n = it.k_end - k0;
+    char* const k_tile = tiles[kBuf == 2 ? buf : 0][0];
+    char* const v_tile = tiles[kBuf == 2 ? buf : 0][1];
+    if (kBuf == 1) __syncthreads();
+    ks.store(k_tile);
+    vs.store(v_tile);
+    if (BIASED && threadIdx.x < kBlock)
+#pragma unroll
+      for (int d = 0; d < 3; ++d) pos[buf][d][threadIdx.x] = ps[d];
     __syncthreads();
-    f32x16_t t[2];
+    if (k0 + kBlock < it.k_end) fetch(k0 + kBlock);
+    f32x16_t t[kBlock / 32];
     float most = top;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBlock / 32; ++b) {
       if (b * 32 >= n) continue;
-      t[b] = rows_times<T, DP>(k_rows, 32 * b, q);
-      if (sc.capped) {
+      t[b] = rows_times<T, DP>(k_tile, 32 * b, q);
+      if constexpr (CAPPED) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) t[b][e] = sc.outer * capped_tanh(sc.inner * t[b][e]);
-      } else {
+      } else if (BIASED || !sc.plain()) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) t[b][e] *= sc.linear;
       }
-      if (sc.biased) {
+      if constexpr (BIASED) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int at = 32 * b + 8 * g + 4 * half;
-          const f32x4 px = *reinterpret_cast<const f32x4*>(&pos[0][at]), py = *reinterpret_cast<const f32x4*>(&pos[1][at]),
-                      pz = *reinterpret_cast<const f32x4*>(&pos[2][at]);
+          const f32x4 px = *reinterpret_cast<const f32x4*>(&pos[buf][0][at]),
+                      py = *reinterpret_cast<const f32x4*>(&pos[buf][1][at]),
+                      pz = *reinterpret_cast<const f32x4*>(&pos[buf][2][at]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float dx = x - px[e], dy = y - py[e], dz = z - pz[e];
@@ -141,7 +191,7 @@ __global__ void __launch_bounds__(64 * NW) attn_fwd_kernel(cgtp_attn_args a, flo
     }
     most = fmaxf(most, half_swap(most));
     if (__any(most > top)) {
-      const float by = top == most ? 1.f : exp2_fast(top - most);      // equal: also both -inf
+      const float by = top == most ? 1.f : exp2_fast((top - most) * sc.unit);      // equal: also both -inf
       sum *= by;
 #pragma unroll
       for (int o = 0; o < S::kOut; ++o)
@@ -149,18 +199,19 @@ __global__ void __launch_bounds__(64 * NW) attn_fwd_kernel(cgtp_attn_args a, flo
         for (int e = 0; e < 16; ++e) acc[o][e] *= by;
       top = most;
     }
-    const float base = top == -INFINITY ? 0.f : top;
+    const float base = top == -INFINITY ? 0.f : -top * sc.unit;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBlock / 32; ++b) {
       if (b * 32 >= n) continue;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        t[b][e] = exp2_fast(t[b][e] - base);
+        t[b][e] = exp2_fast(fmaf(t[b][e], sc.unit, base));
         sum += t[b][e];
       }
-      cols_times<T, DP>(acc, v_tile, v_tile, 32 * b, t[b]);
+      cols_times<T, DP>(acc, v_tile, 32 * b, t[b]);
     }
   }
+  top *= sc.unit;
   sum += half_swap(sum);
   if (!row.ok) return;
   if (it.slot < 0) {
@@ -182,7 +233,7 @@ __global__ void __launch_bounds__(64 * NW) attn_fwd_kernel(cgtp_attn_args a, flo
 // Adds the parts of a row: a workgroup for each (tile, head of keys, row), its slots shared out over slices of threads.
 constexpr int kJoinThreads = 1024;
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) attn_fwd_join_kernel(cgtp_attn_args a, const float* __restrict__ parts, int rows) {
+__global__ void __launch_bounds__(kJoinThreads) attn_fwd_join_kernel(AttnLaunch a, const float* __restrict__ parts, int rows) {
   __shared__ float acc[kJoinThreads], red[kJoinThreads / kWave];
   const int group = a.h_q / a.h_kv, rr = blockIdx.x % rows, hk = blockIdx.x / rows % a.h_kv;
   const cgtp_attn_item it = a.q_joins[blockIdx.x / rows / a.h_kv];
@@ -238,19 +289,20 @@ struct QSums {
 };
 
 // ---- gradient with the rows fixed ---------------------------------------------------------------------------------
-template <typename T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW) attn_bwd_q_kernel(cgtp_attn_args a, AttnScratch w) {
+template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
+__global__ void __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || DP <= 32 ? 2 : 1)
+attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
   using S = AttnShape<T, DP>;
-  __shared__ alignas(16) char k_rows[S::kRowsBytes], v_rows[S::kRowsBytes];
-  __shared__ alignas(16) char k_cols[S::kTransposed ? S::kColsBytes : 16];
-  __shared__ alignas(16) float pos[3][kBlock];
+  constexpr int kBlock = kBlockOf<NW>, kTile = kBlock * S::kRow, kBuf = kBuffers<2 * kTile>;
+  __shared__ alignas(16) char tiles[kBuf][2][kTile];
+  __shared__ alignas(16) float pos[2][3][kBlock];
   const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
   const cgtp_attn_item it = a.q_items[blockIdx.x / a.h_kv];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
   const int r = it.row_begin + wave * 32 + (lane & 31);
   const Row row = row_of(it, r, hk, group);
   const int64_t at = (int64_t)row.query * a.h_q + row.head;
-  const ScoreScale sc = score_scale(a);
+  const ScoreScale<BIASED, CAPPED> sc(a);
   RowFrag<T, DP> q, g;
   q.load(row.ok ? (const T*)a.q + row.query * a.q_node + row.head * a.q_head : nullptr, a.dim);
   g.load(row.ok ? (const T*)a.grad_out + at * a.dim : nullptr, a.dim);
@@ -269,7 +321,7 @@ __global__ void __launch_bounds__(64 * NW) attn_bwd_q_kernel(cgtp_attn_args a, A
   }
   const float lse = row.ok ? ((const float*)a.lse)[at] : INFINITY;
   float x = 0.f, y = 0.f, z = 0.f, slope = 0.f;
-  if (sc.biased && row.ok) {
+  if (BIASED && row.ok) {
     x = a.pos_q[(int64_t)row.query * 3];
     y = a.pos_q[(int64_t)row.query * 3 + 1];
     z = a.pos_q[(int64_t)row.query * 3 + 2];
@@ -285,46 +337,57 @@ __global__ void __launch_bounds__(64 * NW) attn_bwd_q_kernel(cgtp_attn_args a, A
   // exact one is delta + sum ds, and with it the gradients of positions and slopes, which are fp32, err as in fp32.
   constexpr bool kFix = sizeof(T) == 2;
   QSums m = {};
-  const T* kp = (const T*)a.k + hk * a.k_head;
-  const T* vp = (const T*)a.v + hk * a.v_head;
-  for (int k0 = it.k_begin; k0 < it.k_end; k0 += kBlock) {
+  TileStage<T, DP, 64 * NW, kBlock> ks, vs;
+  float ps[3] = {};
+  auto fetch = [&](int k0) {
     const int n = it.k_end - k0;
-    auto k_row = [&](int i) { return i < n ? kp + (int64_t)(k0 + i) * a.k_node : nullptr; };
-    __syncthreads();
-    stage_rows<T, DP, 64 * NW>(k_rows, a.dim, k_row);
-    if constexpr (S::kTransposed) stage_cols<T, DP, 64 * NW>(k_cols, a.dim, k_row);
-    stage_rows<T, DP, 64 * NW>(v_rows, a.dim, [&](int i) { return i < n ? vp + (int64_t)(k0 + i) * a.v_node : nullptr; });
-    if (sc.biased)
-      for (int i = threadIdx.x; i < kBlock; i += 64 * NW)
+    const KeyRows<T> kr((const T*)a.k, a.k_node, a.k_head, hk, k0, n), vr((const T*)a.v, a.v_node, a.v_head, hk, k0, n);
+    ks.load(a.fast, kr.base, a.dim, [&](int i) { return kr.offset(i); }, [&](int i) { return kr.pointer(i); });
+    vs.load(a.fast, vr.base, a.dim, [&](int i) { return vr.offset(i); }, [&](int i) { return vr.pointer(i); });
+    if (BIASED && threadIdx.x < kBlock)
 #pragma unroll
-        for (int d = 0; d < 3; ++d) pos[d][i] = i < n ? a.pos_k[(int64_t)(k0 + i) * 3 + d] : 0.f;
-    __syncthreads();
+      for (int d = 0; d < 3; ++d) ps[d] = (int)threadIdx.x < n ? a.pos_k[(int64_t)(k0 + threadIdx.x) * 3 + d] : 0.f;
+  };
+  if (it.k_begin < it.k_end) fetch(it.k_begin);
+  int buf = 0;
+  for (int k0 = it.k_begin; k0 < it.k_end; k0 += kBlock, buf ^= 1) {
+    const int n = it.k_end - k0;
+    char* const k_tile = tiles[kBuf == 2 ? buf : 0][0];
+    char* const v_tile = tiles[kBuf == 2 ? buf : 0][1];
+    if (kBuf == 1) __syncthreads();
+    ks.store(k_tile);
+    vs.store(v_tile);
+    if (BIASED && threadIdx.x < kBlock)
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+      for (int d = 0; d < 3; ++d) pos[buf][d][threadIdx.x] = ps[d];
+    __syncthreads();
+    if (k0 + kBlock < it.k_end) fetch(k0 + kBlock);
+#pragma unroll 1
+    for (int b = 0; b < kBlock / 32; ++b) {
       if (b * 32 >= n) continue;
-      f32x16_t t = rows_times<T, DP>(k_rows, 32 * b, q);
-      f32x16_t ds = rows_times<T, DP>(v_rows, 32 * b, g);
+      f32x16_t t = rows_times<T, DP>(k_tile, 32 * b, q);
+      f32x16_t ds = rows_times<T, DP>(v_tile, 32 * b, g);
 #pragma unroll
       for (int gq = 0; gq < 4; ++gq) {
         const int first = 32 * b + 8 * gq + 4 * half;
         f32x4 px = {}, py = {}, pz = {};
-        if (sc.biased) {
-          px = *reinterpret_cast<const f32x4*>(&pos[0][first]);
-          py = *reinterpret_cast<const f32x4*>(&pos[1][first]);
-          pz = *reinterpret_cast<const f32x4*>(&pos[2][first]);
+        if constexpr (BIASED) {
+          px = *reinterpret_cast<const f32x4*>(&pos[buf][0][first]);
+          py = *reinterpret_cast<const f32x4*>(&pos[buf][1][first]);
+          pz = *reinterpret_cast<const f32x4*>(&pos[buf][2][first]);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * gq + e;
           float th = 0.f, s;
-          if (sc.capped) {
+          if constexpr (CAPPED) {
             th = capped_tanh(sc.inner * t[i]);
             s = sc.outer * th;
           } else {
             s = sc.linear * t[i];
           }
           float dx = 0.f, dy = 0.f, dz = 0.f, d2 = 0.f, inv = 0.f;
-          if (sc.biased) {
+          if constexpr (BIASED) {
             dx = x - px[e];
             dy = y - py[e];
             dz = z - pz[e];
@@ -335,7 +398,7 @@ __global__ void __launch_bounds__(64 * NW) attn_bwd_q_kernel(cgtp_attn_args a, A
           float p = exp2_fast(s - lse);
           if (first + e >= n) p = 0.f;
           float d = p * (ds[i] - delta);
-          if (sc.biased) {
+          if constexpr (BIASED) {
             const float u = d * inv;
             m.v[0] = fmaf(u, dx, m.v[0]);
             m.v[1] = fmaf(u, dy, m.v[1]);
@@ -350,11 +413,12 @@ __global__ void __launch_bounds__(64 * NW) attn_bwd_q_kernel(cgtp_attn_args a, A
               m.v[8] += d;
             }
           }
-          if (sc.capped) d *= 1.f - th * th;
+          if constexpr (CAPPED) d *= 1.f - th * th;
           ds[i] = d;
         }
+        __builtin_amdgcn_sched_barrier(0);      // keeps the next group's reads from LDS out of the registers
       }
-      cols_times<T, DP>(acc, k_rows, k_cols, 32 * b, ds);
+      cols_times<T, DP>(acc, k_tile, 32 * b, ds);
     }
   }
 #pragma unroll
@@ -363,7 +427,7 @@ __global__ void __launch_bounds__(64 * NW) attn_bwd_q_kernel(cgtp_attn_args a, A
   if (!row.ok) return;
   if (it.slot < 0) {
     if (a.grad_q) store_cols<T, DP>((T*)a.grad_q + at * a.dim, acc, a.scale, a.dim);
-    if (half == 0) m.finish(w, at, slope, sc.biased);
+    if (half == 0) m.finish(w, at, slope, BIASED);
   } else {
     float* p = w.parts + (((int64_t)it.slot * a.h_kv + hk) * kRowsOf<NW> + (r - it.row_begin)) * (a.dim + kQSums);
     store_cols<float, (DP < 32 ? 32 : DP)>(p, acc, a.scale, a.dim);
@@ -374,7 +438,7 @@ __global__ void __launch_bounds__(64 * NW) attn_bwd_q_kernel(cgtp_attn_args a, A
 }
 
 template <typename T>
-__global__ void __launch_bounds__(192) attn_bwd_q_join_kernel(cgtp_attn_args a, AttnScratch w, int rows) {
+__global__ void __launch_bounds__(192) attn_bwd_q_join_kernel(AttnLaunch a, AttnScratch w, int rows) {
   __shared__ float sums[kQSums];
   const int group = a.h_q / a.h_kv, rr = blockIdx.x % rows, hk = blockIdx.x / rows % a.h_kv;
   const cgtp_attn_item it = a.q_joins[blockIdx.x / rows / a.h_kv];
@@ -401,23 +465,24 @@ __global__ void __launch_bounds__(192) attn_bwd_q_join_kernel(cgtp_attn_args a, 
 }
 
 // ---- gradient with the keys fixed ---------------------------------------------------------------------------------
-template <typename T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW) attn_bwd_k_kernel(cgtp_attn_args a, AttnScratch w) {
+template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
+__global__ void __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || DP <= 32 ? 2 : 1)
+attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
   using S = AttnShape<T, DP>;
-  __shared__ alignas(16) char q_rows[S::kRowsBytes], g_rows[S::kRowsBytes];
-  __shared__ alignas(16) char q_cols[S::kTransposed ? S::kColsBytes : 16], g_cols[S::kTransposed ? S::kColsBytes : 16];
-  __shared__ alignas(16) float stat[6][kBlock];       // lse, delta, slope, position
+  constexpr int kBlock = kBlockOf<NW>, kTile = kBlock * S::kRow, kBuf = kBuffers<2 * kTile>;
+  __shared__ alignas(16) char tiles[kBuf][2][kTile];
+  __shared__ alignas(16) float stat[2][6][kBlock];       // lse, delta, slope, position
   const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
   const cgtp_attn_item it = a.k_items[blockIdx.x / a.h_kv];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
   const int key = it.k_begin + wave * 32 + (lane & 31);
   const bool ok = key < it.k_end;
-  const ScoreScale sc = score_scale(a);
+  const ScoreScale<BIASED, CAPPED> sc(a);
   RowFrag<T, DP> k, v;
   k.load(ok ? (const T*)a.k + key * a.k_node + hk * a.k_head : nullptr, a.dim);
   v.load(ok ? (const T*)a.v + key * a.v_node + hk * a.v_head : nullptr, a.dim);
   float x = 0.f, y = 0.f, z = 0.f;
-  if (sc.biased && ok) {
+  if (BIASED && ok) {
     x = a.pos_k[(int64_t)key * 3];
     y = a.pos_k[(int64_t)key * 3 + 1];
     z = a.pos_k[(int64_t)key * 3 + 2];
@@ -428,64 +493,69 @@ __global__ void __launch_bounds__(64 * NW) attn_bwd_k_kernel(cgtp_attn_args a, A
 #pragma unroll
     for (int e = 0; e < 16; ++e) gk[o][e] = gv[o][e] = 0.f;
   float gx = 0.f, gy = 0.f, gz = 0.f;
-  for (int r0 = it.row_begin; r0 < it.row_end; r0 += kBlock) {
+  TileStage<T, DP, 64 * NW, kBlock> qs, gs;
+  float st[6] = {};
+  auto fetch = [&](int r0) {
     const int n = it.row_end - r0;
-    auto q_row = [&](int i) {
-      const Row o = row_of(it, r0 + i, hk, group);
-      return o.ok ? (const T*)a.q + o.query * a.q_node + o.head * a.q_head : nullptr;
-    };
-    auto g_row = [&](int i) {
-      const Row o = row_of(it, r0 + i, hk, group);
-      return o.ok ? (const T*)a.grad_out + ((int64_t)o.query * a.h_q + o.head) * a.dim : nullptr;
-    };
-    __syncthreads();
-    stage_rows<T, DP, 64 * NW>(q_rows, a.dim, q_row);
-    stage_rows<T, DP, 64 * NW>(g_rows, a.dim, g_row);
-    if constexpr (S::kTransposed) {
-      stage_cols<T, DP, 64 * NW>(q_cols, a.dim, q_row);
-      stage_cols<T, DP, 64 * NW>(g_cols, a.dim, g_row);
-    }
-    for (int i = threadIdx.x; i < kBlock; i += 64 * NW) {
-      const Row o = row_of(it, r0 + i, hk, group);
+    const QueryRows<T> qr((const T*)a.q, a.q_node, a.q_head, it.node, hk, group, r0, n),
+        gr((const T*)a.grad_out, (int64_t)a.h_q * a.dim, a.dim, it.node, hk, group, r0, n);
+    qs.load(a.fast, qr.base, a.dim, [&](int i) { return qr.offset(i); }, [&](int i) { return qr.pointer(i); });
+    gs.load(a.fast, gr.base, a.dim, [&](int i) { return gr.offset(i); }, [&](int i) { return gr.pointer(i); });
+    if (threadIdx.x < kBlock) {
+      const Row o = row_of(it, r0 + threadIdx.x, hk, group);
       const int64_t at = (int64_t)o.query * a.h_q + o.head;
-      stat[0][i] = o.ok ? ((const float*)a.lse)[at] : INFINITY;        // +inf: probability zero
-      stat[1][i] = o.ok ? w.delta[at] : 0.f;
-      if (sc.biased) {
-        stat[2][i] = o.ok ? a.slope[o.head] : 0.f;
+      st[0] = o.ok ? ((const float*)a.lse)[at] : INFINITY;        // +inf: probability zero
+      st[1] = o.ok ? w.delta[at] : 0.f;
+      if constexpr (BIASED) {
+        st[2] = o.ok ? a.slope[o.head] : 0.f;
 #pragma unroll
-        for (int d = 0; d < 3; ++d) stat[3 + d][i] = o.ok ? a.pos_q[(int64_t)o.query * 3 + d] : 0.f;
+        for (int d = 0; d < 3; ++d) st[3 + d] = o.ok ? a.pos_q[(int64_t)o.query * 3 + d] : 0.f;
       }
     }
-    __syncthreads();
+  };
+  if (it.row_begin < it.row_end) fetch(it.row_begin);
+  int buf = 0;
+  for (int r0 = it.row_begin; r0 < it.row_end; r0 += kBlock, buf ^= 1) {
+    const int n = it.row_end - r0;
+    char* const q_tile = tiles[kBuf == 2 ? buf : 0][0];
+    char* const g_tile = tiles[kBuf == 2 ? buf : 0][1];
+    if (kBuf == 1) __syncthreads();
+    qs.store(q_tile);
+    gs.store(g_tile);
+    if (threadIdx.x < kBlock)
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+      for (int d = 0; d < 6; ++d) stat[buf][d][threadIdx.x] = st[d];
+    __syncthreads();
+    if (r0 + kBlock < it.row_end) fetch(r0 + kBlock);
+#pragma unroll 1
+    for (int b = 0; b < kBlock / 32; ++b) {
       if (b * 32 >= n) continue;
-      f32x16_t t = rows_times<T, DP>(q_rows, 32 * b, k);
-      f32x16_t ds = rows_times<T, DP>(g_rows, 32 * b, v);
+      f32x16_t t = rows_times<T, DP>(q_tile, 32 * b, k);
+      f32x16_t ds = rows_times<T, DP>(g_tile, 32 * b, v);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int first = 32 * b + 8 * g + 4 * half;
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[0][first]);
-        const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[1][first]);
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[buf][0][first]);
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[buf][1][first]);
         f32x4 slope = {}, px = {}, py = {}, pz = {};
-        if (sc.biased) {
-          slope = *reinterpret_cast<const f32x4*>(&stat[2][first]);
-          px = *reinterpret_cast<const f32x4*>(&stat[3][first]);
-          py = *reinterpret_cast<const f32x4*>(&stat[4][first]);
-          pz = *reinterpret_cast<const f32x4*>(&stat[5][first]);
+        if constexpr (BIASED) {
+          slope = *reinterpret_cast<const f32x4*>(&stat[buf][2][first]);
+          px = *reinterpret_cast<const f32x4*>(&stat[buf][3][first]);
+          py = *reinterpret_cast<const f32x4*>(&stat[buf][4][first]);
+          pz = *reinterpret_cast<const f32x4*>(&stat[buf][5][first]);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * g + e;
           float th = 0.f, s;
-          if (sc.capped) {
+          if constexpr (CAPPED) {
             th = capped_tanh(sc.inner * t[i]);
             s = sc.outer * th;
           } else {
             s = sc.linear * t[i];
           }
           float dx = 0.f, dy = 0.f, dz = 0.f, inv = 0.f;
-          if (sc.biased) {
+          if constexpr (BIASED) {
             dx = px[e] - x;
             dy = py[e] - y;
             dz = pz[e] - z;
@@ -495,19 +565,20 @@ __global__ void __launch_bounds__(64 * NW) attn_bwd_k_kernel(cgtp_attn_args a, A
           }
           const float p = exp2_fast(s - lse[e]);
           float d = p * (ds[i] - delta[e]);
-          if (sc.biased) {
+          if constexpr (BIASED) {
             const float u = d * inv * slope[e];
             gx = fmaf(u, dx, gx);
             gy = fmaf(u, dy, gy);
             gz = fmaf(u, dz, gz);
           }
-          if (sc.capped) d *= 1.f - th * th;
+          if constexpr (CAPPED) d *= 1.f - th * th;
           t[i] = p;
           ds[i] = d;
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      cols_times<T, DP>(gv, g_rows, g_cols, 32 * b, t);
-      cols_times<T, DP>(gk, q_rows, q_cols, 32 * b, ds);
+      cols_times<T, DP>(gv, g_tile, 32 * b, t);
+      cols_times<T, DP>(gk, q_tile, 32 * b, ds);
     }
   }
   gx += half_swap(gx);
@@ -518,7 +589,7 @@ __global__ void __launch_bounds__(64 * NW) attn_bwd_k_kernel(cgtp_attn_args a, A
   if (it.slot < 0) {
     if (a.grad_k) store_cols<T, DP>((T*)a.grad_k + at * a.dim, gk, a.scale, a.dim);
     if (a.grad_v) store_cols<T, DP>((T*)a.grad_v + at * a.dim, gv, 1.f, a.dim);
-    if (sc.biased && half == 0) w.key_part[at] = f32x4{gx, gy, gz, 0.f};
+    if (BIASED && half == 0) w.key_part[at] = f32x4{gx, gy, gz, 0.f};
   } else {
     float* p = w.parts + (((int64_t)it.slot * a.h_kv + hk) * kRowsOf<NW> + (key - it.k_begin)) * (2 * a.dim + 4);
     store_cols<float, (DP < 32 ? 32 : DP)>(p, gk, a.scale, a.dim);
@@ -533,7 +604,7 @@ __global__ void __launch_bounds__(64 * NW) attn_bwd_k_kernel(cgtp_attn_args a, A
 }
 
 template <typename T>
-__global__ void __launch_bounds__(512) attn_bwd_k_join_kernel(cgtp_attn_args a, AttnScratch w, int rows) {
+__global__ void __launch_bounds__(512) attn_bwd_k_join_kernel(AttnLaunch a, AttnScratch w, int rows) {
   const int kk = blockIdx.x % rows, hk = blockIdx.x / rows % a.h_kv;
   const cgtp_attn_item it = a.k_joins[blockIdx.x / rows / a.h_kv];
   const int key = it.k_begin + kk, d = threadIdx.x, width = 2 * a.dim + 4;
@@ -553,43 +624,46 @@ __global__ void __launch_bounds__(512) attn_bwd_k_join_kernel(cgtp_attn_args a, 
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
-template <typename T, int DP, int NW>
-void q_launch(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) {
+template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
+void q_launch(const AttnLaunch& a, const AttnScratch* w, hipStream_t s) {
   const dim3 grid((unsigned)a.n_q_items * a.h_kv), joins((unsigned)a.n_q_joins * a.h_kv * kRowsOf<NW>);
   float* parts = (float*)a.workspace;
   if (a.n_q_items) {
-    if (w) hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NW>), grid, dim3(64 * NW), 0, s, a, *w);
-    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW>), grid, dim3(64 * NW), 0, s, a, parts);
+    if (w) hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NW, BIASED, CAPPED>), grid, dim3(64 * NW), 0, s, a, *w);
+    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, BIASED, CAPPED>), grid, dim3(64 * NW), 0, s, a, parts);
   }
   if (a.n_q_joins) {
     if (w) hipLaunchKernelGGL((attn_bwd_q_join_kernel<T>), joins, dim3(192), 0, s, a, *w, kRowsOf<NW>);
     else hipLaunchKernelGGL((attn_fwd_join_kernel<T>), joins, dim3(kJoinThreads), 0, s, a, (const float*)parts, kRowsOf<NW>);
   }
 }
-template <typename T, int DP, int NW>
-void k_launch(const cgtp_attn_args& a, const AttnScratch& w, hipStream_t s) {
+template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
+void k_launch(const AttnLaunch& a, const AttnScratch& w, hipStream_t s) {
   if (a.n_k_items)
-    hipLaunchKernelGGL((attn_bwd_k_kernel<T, DP, NW>), dim3((unsigned)a.n_k_items * a.h_kv), dim3(64 * NW), 0, s, a, w);
+    hipLaunchKernelGGL((attn_bwd_k_kernel<T, DP, NW, BIASED, CAPPED>), dim3((unsigned)a.n_k_items * a.h_kv), dim3(64 * NW), 0, s,
+                       a, w);
   if (a.n_k_joins)
     hipLaunchKernelGGL((attn_bwd_k_join_kernel<T>), dim3((unsigned)a.n_k_joins * a.h_kv * kRowsOf<NW>), dim3(512), 0, s, a, w,
                        kRowsOf<NW>);
 }
-template <typename T, int DP>
-void launch_dim(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) {
-  if (a.wide_q) q_launch<T, DP, 4>(a, w, s);
-  else q_launch<T, DP, 1>(a, w, s);
+template <typename T, int DP, bool BIASED, bool CAPPED>
+void launch_dim(const AttnLaunch& a, const AttnScratch* w, hipStream_t s) {
+  if (a.wide_q) q_launch<T, DP, 4, BIASED, CAPPED>(a, w, s);
+  else q_launch<T, DP, 1, BIASED, CAPPED>(a, w, s);
   if (!w) return;
-  if (a.wide_k) k_launch<T, DP, 4>(a, *w, s);
-  else k_launch<T, DP, 1>(a, *w, s);
-}
-template <typename T>
-void launch_type(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) {
-  if (a.dim <= 16) launch_dim<T, 16>(a, w, s);
-  else if (a.dim <= 32) launch_dim<T, 32>(a, w, s);
-  else if (a.dim <= 64) launch_dim<T, 64>(a, w, s);
-  else if (a.dim <= 96) launch_dim<T, 96>(a, w, s);
-  else launch_dim<T, 128>(a, w, s);
+  if (a.wide_k) k_launch<T, DP, 4, BIASED, CAPPED>(a, *w, s);
+  else k_launch<T, DP, 1, BIASED, CAPPED>(a, *w, s);
 }
 
 }  // namespace
+
+template <typename T, bool BIASED, bool CAPPED>
+void attn_launch(const AttnLaunch& a, const AttnScratch* w, hipStream_t s) {
+  if (a.dim <= 16) launch_dim<T, 16, BIASED, CAPPED>(a, w, s);
+  else if (a.dim <= 32) launch_dim<T, 32, BIASED, CAPPED>(a, w, s);
+  else if (a.dim <= 64) launch_dim<T, 64, BIASED, CAPPED>(a, w, s);
+  else if (a.dim <= 96) launch_dim<T, 96, BIASED, CAPPED>(a, w, s);
+  else launch_dim<T, 128, BIASED, CAPPED>(a, w, s);
+}
+
 }  // namespace cgtp

@@ -3,6 +3,7 @@
 #include "attn_host.h"
 
 #include <algorithm>
+#include <cstdlib>
 
 namespace cgtp {
 namespace {
@@ -78,10 +79,32 @@ int attn_check(const cgtp_attn_args* a) {
   return CGTP_OK;
 }
 
-void launch(const cgtp_attn_args& a, const AttnScratch* w, hipStream_t s) {
-  if (a.dtype == CGTP_F32) attn_launch_f32(a, w, s);
-  else if (a.dtype == CGTP_BF16) attn_launch_bf16(a, w, s);
-  else attn_launch_f16(a, w, s);
+bool is_fast(const cgtp_attn_args& a, bool backward) {
+  const int64_t size = elem_size(a.dtype), chunk = 16 / size, group = a.h_q / a.h_kv;
+  const int64_t strides[] = {a.q_node, a.q_head, a.k_node, a.k_head, a.v_node, a.v_head};
+  for (int64_t s : strides)
+    if (s % chunk) return false;
+  const void* ptrs[] = {a.q, a.k, a.v, backward ? a.grad_out : nullptr};
+  for (const void* p : ptrs)
+    if ((uintptr_t)p & 15) return false;
+  // 64 rows of a tile are at most 65 queries' heads
+  auto small = [&](int64_t node, int64_t head) { return 65 * std::abs(node * size) + group * std::abs(head * size) < (1ll << 31) - 512; };
+  return a.dim % chunk == 0 && small(a.k_node, 0) && small(a.v_node, 0) && small(a.q_node, a.q_head) &&
+         small((int64_t)a.h_q * a.dim, a.dim) && a.q_node >= 0 && a.q_head >= 0 && a.k_node >= 0 && a.v_node >= 0;
+}
+
+template <typename T>
+void launch_type(const AttnLaunch& a, const AttnScratch* w, hipStream_t s) {
+  if (a.slope) a.cap > 0.f ? attn_launch<T, true, true>(a, w, s) : attn_launch<T, true, false>(a, w, s);
+  else a.cap > 0.f ? attn_launch<T, false, true>(a, w, s) : attn_launch<T, false, false>(a, w, s);
+}
+void launch(const cgtp_attn_args& args, const AttnScratch* w, hipStream_t s) {
+  AttnLaunch a;
+  static_cast<cgtp_attn_args&>(a) = args;
+  a.fast = is_fast(args, w != nullptr);
+  if (a.dtype == CGTP_F32) launch_type<float>(a, w, s);
+  else if (a.dtype == CGTP_BF16) launch_type<bf16_t>(a, w, s);
+  else launch_type<f16_t>(a, w, s);
 }
 
 }  // namespace

@@ -4,19 +4,21 @@
 // 8 g + 4 (lane / 32) + e.  A result can be the B operand of the next product as it lies in the registers: its rows become k,
 // eight (16-bit) or one (fp32) of a lane's rows for each instruction, and A's k are taken in the same order.
 //
-// A tile of kBlock rows (nodes) is kept row by row, chunks of 16 bytes, chunk c of row r at a place that puts the eight rows a
-// quarter wavefront reads into different groups of banks; for 16-bit types also column by column (RowsT), where the
-// rows become k: a chunk there holds the eight rows of one lane and instruction.  fp32 needs no such copy: an
-// instruction takes one row for each half of the wavefront, 32 neighbouring columns of it.
+// A tile of 64 rows (nodes), 32 where one wavefront works alone, lies in LDS row by row in chunks of 16 bytes, chunk c of row r at a place that puts the eight
+// rows a quarter wavefront reads into different groups of banks.  Where the rows become k, 16-bit types read it through
+// the LDS's transposing loads (four rows of 16 columns for each 16 lanes) and fp32 as it is, one row for each half of the
+// wavefront: no second, transposed copy.
+//
+// A tile goes from memory through registers to LDS: loaded while the tile before it is worked on, stored after.  Where rows
+// are whole aligned chunks (`fast`) the loads are buffer loads with 32-bit offsets, whose range check turns what is
+// beyond the structure into zeros; other layouts take element-aligned loads with the last chunk of a row cut.
 #pragma once
 
 #include "elem.h"
 
 namespace cgtp {
 
-
-
-constexpr int kBlock = 64;                      // rows of a tile in LDS
+constexpr unsigned kNoRow = 0x80000000u;        // an offset beyond every buffer
 
 template <typename T, int DP>
 struct AttnShape {
@@ -24,14 +26,11 @@ struct AttnShape {
   static constexpr int kChunks = DP / kChunk;                 // chunks of a row
   static constexpr int kSteps = kChunks / 2;                  // pairs of chunks: one per half wavefront
   static constexpr int kOut = (DP + 31) / 32;                 // 32-wide blocks of dim in a result
-  static constexpr bool kTransposed = sizeof(T) == 2;
-  static constexpr int kRowsBytes = kBlock * DP * (int)sizeof(T);
-  static constexpr int kColsBytes = kTransposed ? kOut * 32 * kBlock * 2 : 0;
-  __device__ static __forceinline__ int slot(int row, int c) {
-    constexpr int kMix = kChunks % 8 == 0 ? 8 : kChunks % 4 == 0 ? 4 : 2;      // chunks that change places
-    constexpr int kPer = kMix == 8 ? 1 : kMix == 4 ? 2 : 4;                    // rows before the pattern moves on
-    return (row * kChunks + (c ^ ((row / kPer) & (kMix - 1)))) << 4;
-  }
+  static constexpr int kRow = DP * (int)sizeof(T);            // bytes
+  static constexpr int kMix = kChunks % 8 == 0 ? 8 : kChunks % 4 == 0 ? 4 : 2;      // chunks that change places
+  static constexpr int kPer = kMix == 8 ? 1 : kMix == 4 ? 2 : 4;                    // rows before the pattern moves on
+  __device__ static __forceinline__ int mixed(int row, int c) { return c ^ ((row / kPer) & (kMix - 1)); }
+  __device__ static __forceinline__ int slot(int row, int c) { return (row * kChunks + mixed(row, c)) << 4; }
 };
 
 template <typename T>
@@ -68,48 +67,45 @@ struct RowFrag {
   }
 };
 
-// Rows row(0) .. row(kBlock - 1) (null: zeros) to LDS, row by row.
-template <typename T, int DP, int THREADS, typename Row>
-__device__ __forceinline__ void stage_rows(char* lds, int dim, Row&& row) {
+// A tile between memory and LDS.  Offset(i): bytes from `base` of row i, kNoRow for none; Pointer(i): the row, null for none.
+template <typename T, int DP, int THREADS, int BLOCK>
+struct TileStage {
   using S = AttnShape<T, DP>;
+  static constexpr int kAll = BLOCK * S::kChunks, kEach = (kAll + THREADS - 1) / THREADS;
+  u32x4_t reg[kEach];
+
+  template <typename Offset, typename Pointer>
+  __device__ __forceinline__ void load(bool fast, const T* base, int dim, Offset&& offset, Pointer&& pointer) {
+    if (fast) {
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kNoRow, 0x00027000);
 #pragma unroll
-  for (int i = 0; i < (kBlock * S::kChunks + THREADS - 1) / THREADS; ++i) {
-    const int id = i * THREADS + threadIdx.x, r = id / S::kChunks, c = id % S::kChunks;
-    if (kBlock * S::kChunks % THREADS != 0 && id >= kBlock * S::kChunks) break;
-    const T* p = row(r);
-    u32x4_t v = {0, 0, 0, 0};
-    if (p && c * S::kChunk < dim) v = load_part<u32x4_t, T>(p + c * S::kChunk, dim - c * S::kChunk);
-    *reinterpret_cast<u32x4_t*>(lds + S::slot(r, c)) = v;
-  }
-}
-// The same column by column (16-bit types): chunk c of column d holds rows 16 (c / 2) + 4 (c % 2) + {0 .. 3, 8 .. 11}.
-template <typename T, int DP, int THREADS, typename Row>
-__device__ __forceinline__ void stage_cols(char* lds, int dim, Row&& row) {
-  using S = AttnShape<T, DP>;
-  constexpr int kQuads = S::kOut * 8;           // groups of four columns
-  constexpr int kTasks = kQuads * 8;
+      for (int i = 0; i < kEach; ++i) {
+        const int id = i * THREADS + (int)threadIdx.x, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
+        if (kAll % THREADS != 0 && id >= kAll) break;
+        const unsigned o = offset(r);
+        reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+            rsrc, o == kNoRow || c * S::kChunk >= dim ? kNoRow : o + c * 16, 0, 0));
+      }
+    } else {
 #pragma unroll
-  for (int i = 0; i < (kTasks + THREADS - 1) / THREADS; ++i) {
-    const int id = i * THREADS + threadIdx.x;
-    if (kTasks % THREADS != 0 && id >= kTasks) break;
-    const int c = id & 7, d = (id >> 3) * 4;
-    u32x2_t t[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const T* p = row(16 * (c >> 1) + 4 * (c & 1) + (j & 3) + 8 * (j >> 2));
-      t[j] = u32x2_t{0, 0};
-      if (p && d < dim) t[j] = load_part<u32x2_t, T>(p + d, dim - d);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      u32x4_t v;
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        v[w] = __builtin_amdgcn_perm(t[2 * w + 1][j >> 1], t[2 * w][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
-      *reinterpret_cast<u32x4_t*>(lds + (d + j) * 128 + ((c ^ ((d + j) & 7)) << 4)) = v;
+      for (int i = 0; i < kEach; ++i) {
+        const int id = i * THREADS + (int)threadIdx.x, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
+        if (kAll % THREADS != 0 && id >= kAll) break;
+        const T* p = pointer(r);
+        reg[i] = u32x4_t{0, 0, 0, 0};
+        if (p && c * S::kChunk < dim) reg[i] = load_part<u32x4_t, T>(p + c * S::kChunk, dim - c * S::kChunk);
+      }
     }
   }
-}
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int id = i * THREADS + (int)threadIdx.x;
+      if (kAll % THREADS != 0 && id >= kAll) break;
+      *reinterpret_cast<u32x4_t*>(lds + id * 16) = reg[i];
+    }
+  }
+};
 
 // D = rows of the tile (32 from `first` on) times the lanes' rows: 32 x 32 products over dim.
 template <typename T, int DP>
@@ -125,26 +121,33 @@ __device__ __forceinline__ f32x16_t rows_times(const char* lds, int first, const
   return acc;
 }
 
-// acc[o] += columns 32 o .. of the 32 rows from `first` on, transposed, times p (rows by lanes' columns).  `rows` and `cols`
-// are the two copies of the tile; only the one the type needs is read.
+// Four rows of 16 columns, transposed: lane i of 16 reads four columns from 4 (i % 4) on of row i / 4, and gets column i.
+__device__ __forceinline__ u32x2_t lds_transposed(const char* p) {
+  typedef short v4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4 lds_v4;
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)p));
+}
+
+// acc[o] += columns 32 o .. of the tile's 32 rows from `first` on, transposed, times p (rows by lanes' columns).
 template <typename T, int DP>
-__device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* rows, const char* cols, int first,
-                                           const f32x16_t& p) {
+__device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* lds, int first, const f32x16_t& p) {
   using S = AttnShape<T, DP>;
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  if constexpr (S::kTransposed) {
+  if constexpr (sizeof(T) == 2) {
+    const int r = first + 4 * half + ((lane & 15) >> 2), d = (lane & 16) + 4 * (lane & 3);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       typedef T v8 __attribute__((ext_vector_type(8)));
       v8 b;
 #pragma unroll
       for (int j = 0; j < 8; ++j) b[j] = (T)p[8 * t + j];
-      const int c = (first >> 3) + 2 * t + half;
 #pragma unroll
       for (int o = 0; o < S::kOut; ++o) {
-        const int d = 32 * o + (lane & 31);
-        acc[o] = mma_pair<T>(*reinterpret_cast<const u32x4_t*>(cols + d * 128 + ((c ^ (d & 7)) << 4)),
-                             __builtin_bit_cast(u32x4_t, b), acc[o]);
+        // DP = 16: the columns 16 .. 31 of the result do not exist; its lanes read the others again
+        const int col = DP < 32 ? d & 15 : 32 * o + d;
+        const u32x2_t lo = lds_transposed(lds + S::slot(r + 16 * t, col >> 3) + (col & 7) * 2);
+        const u32x2_t hi = lds_transposed(lds + S::slot(r + 16 * t + 8, col >> 3) + (col & 7) * 2);
+        acc[o] = mma_pair<T>(u32x4_t{lo[0], lo[1], hi[0], hi[1]}, __builtin_bit_cast(u32x4_t, b), acc[o]);
       }
     }
   } else {
@@ -153,10 +156,9 @@ __device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* rows
       const int r = first + 8 * (e >> 2) + 4 * half + (e & 3);
 #pragma unroll
       for (int o = 0; o < S::kOut; ++o) {
-        const int d = 32 * o + (lane & 31);
-        const bool in = DP % 32 == 0 || d < DP;
-        const float v = *reinterpret_cast<const float*>(rows + S::slot(r, (in ? d : 0) >> 2) + ((d & 3) << 2));
-        acc[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? v : 0.f, p[e], acc[o], 0, 0, 0);
+        const int d = DP < 32 ? lane & 15 : 32 * o + (lane & 31);
+        const float v = *reinterpret_cast<const float*>(lds + S::slot(r, d >> 2) + ((d & 3) << 2));
+        acc[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[e], acc[o], 0, 0, 0);
       }
     }
   }

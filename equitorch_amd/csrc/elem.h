@@ -43,8 +43,8 @@ typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
-// N elements of T from an address aligned to an element only, the ones from `valid` on as zeros.  Vector loads from
-// such addresses are what the hardware does by itself; only a vector that crosses the end is taken apart.
+// N elements of T from an address aligned to an element only, the ones from `valid` (at least 1) on as zeros.  Vector loads
+// from such addresses are what the hardware does by itself; only a vector that crosses the end is taken apart.
 template <typename T, int N>
 struct __attribute__((packed, aligned(sizeof(T)))) Loose { T v[N]; };
 
@@ -54,7 +54,10 @@ __device__ __forceinline__ R load_part(const T* p, int64_t valid) {
   if (valid >= N) return __builtin_bit_cast(R, *reinterpret_cast<const Loose<T, N>*>(p));
   T e[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) e[i] = i < valid ? p[i] : T(0);
+  for (int i = 0; i < N; ++i) {
+    const T v = p[i < valid ? i : 0];
+    e[i] = i < valid ? v : T(0);
+  }
   R r;
   __builtin_memcpy(&r, e, sizeof(R));
   return r;
