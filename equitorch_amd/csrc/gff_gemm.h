@@ -1,25 +1,29 @@
 // Matrix products of the gated feed-forward block on the matrix cores: tiles of 128 x 128, four wavefronts of 64 x 64 each,
-// operands staged through registers into two LDS buffers.
+// operands brought through registers into two LDS buffers, the next tile loaded while one is worked on.
 //
-// An operand is a matrix whose rows or whose columns are contiguous.  In LDS both look alike: per row of the tile eight chunks of
-// 16 bytes along k, chunk c of row r at place c ^ (r & 7), so that the eight rows a quarter wavefront reads lie in eight
-// different groups of banks.  An operand contiguous along its rows is transposed on the way in registers: a thread takes
-// a chunk's worth of k for four neighbouring rows.
+// An operand is a matrix whose k or whose rows are contiguous.  In LDS a tile is 1024 chunks of 16 bytes either way:
+//   k contiguous    128 rows of eight chunks along k, chunk c of row r at place c ^ (r & 7);
+//   rows contiguous two halves of 64 rows, in each the rows of one k after the other, chunks exchanged by
+//                   (k & 3) | (k >> 1 & 4), which the transposing loads of 16-bit types (four k of 16 rows for each 16
+//                   lanes, k and k + 8 in one instruction) find in different groups of banks.
+// 16-bit types use 32 x 32 x 16 instructions, fp32 32 x 32 x 2 ones, four for a pair of chunks, whose k are taken in the order
+// that lets a lane read its four in one access.
 //
-// 16-bit operands use 32 x 32 x 16 instructions; fp32 operands 32 x 32 x 2 ones, four per pair of chunks, whose k
-// are taken in the order that lets a lane read its four in one access.
+// Aligned operands (16 bytes, rows of whole chunks) are read by buffer loads with 32-bit offsets, where an offset beyond the
+// buffer gives zeros; others by element-aligned loads with the last chunk of a row cut.
 #pragma once
 
 #include "elem.h"
 
 namespace cgtp {
 
+constexpr int kGemmTile = 128, kGemmThreads = 256;
+constexpr int kGemmTileBytes = 16 * 1024;
+constexpr unsigned kOutside = 0x80000000u;
 
-
-constexpr int kGemmTile = 128, kGemmThreads = 256, kGemmChunks = 8;
-constexpr int kGemmTileBytes = kGemmTile * kGemmChunks * 16;
-
-template <typename T> struct GemmType { static constexpr int kChunk = 16 / (int)sizeof(T), kDepth = kGemmChunks * kChunk; };
+template <typename T> struct GemmType {
+  static constexpr int kChunk = 16 / (int)sizeof(T), kDepth = 8 * kChunk;     // elements of a chunk; k of a tile
+};
 
 template <typename T>
 __device__ __forceinline__ void mma_chunk(f32x16_t& acc, const u32x4_t& a, const u32x4_t& b) {
@@ -36,73 +40,102 @@ __device__ __forceinline__ void mma_chunk(f32x16_t& acc, const u32x4_t& a, const
   }
 }
 
-// One operand's tile in registers between memory and LDS.
+// An operand's tile.  k contiguous: `base` at the tile's first row, `ld` elements between rows, `rows` of them left.  Rows
+// contiguous: base[i] at the first row of half i at k = 0, ld between k, rows[i] left.  The second half of a k-contiguous
+// operand is not used.
+template <typename T>
+struct GemmOperand {
+  const T* base[2];
+  int64_t ld;
+  int rows[2];
+};
+
 template <typename T, bool K_CONTIGUOUS>
 struct GemmStage {
   static constexpr int CH = GemmType<T>::kChunk;
   u32x4_t reg[4];
 
-  // Where row r of the tile is: row(r) gives its pointer at k = 0 (K_CONTIGUOUS) or at (0, r), or null outside the matrix.
-  // k0: first k of the tile; depth: end of k; ld: elements between rows of memory; end: number of columns of memory from
-  // the pointer's own on that belong to this operand (row-contiguous only).
-  template <typename Row>
-  __device__ __forceinline__ void load(Row&& row, int64_t k0, int64_t depth, int64_t ld) {
-    const int tid = threadIdx.x;
+  // k0: first k of the tile, depth: end of k.
+  __device__ __forceinline__ void load(bool fast, const GemmOperand<T>& p, int64_t k0, int64_t depth) {
+    const int tid = threadIdx.x, left = (int)(depth - k0 < GemmType<T>::kDepth ? depth - k0 : GemmType<T>::kDepth);
     if constexpr (K_CONTIGUOUS) {
+      const T* base = p.base[0] + k0;
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kOutside, 0x00027000);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int id = i * kGemmThreads + tid, r = id >> 3, c = id & 7;
-        int64_t end;
-        const T* p = row(r, end);
-        const int64_t k = k0 + c * CH;
-        reg[i] = u32x4_t{0, 0, 0, 0};
-        if (p && k < depth) reg[i] = load_part<u32x4_t, T>(p + k, depth - k);
+        const int id = i * kGemmThreads + tid, r = id >> 3, c = (id & 7) ^ (r & 7);
+        const bool in = r < p.rows[0] && c * CH < left;
+        if (fast) {
+          const unsigned at = (unsigned)r * (unsigned)(p.ld * sizeof(T)) + c * 16;
+          reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, in ? at : kOutside, 0, 0));
+        } else {
+          reg[i] = u32x4_t{0, 0, 0, 0};
+          if (in) reg[i] = load_part<u32x4_t, T>(base + r * p.ld + c * CH, left - c * CH);
+        }
       }
     } else {
-      const int c = tid & 7, r = (tid >> 3) * 4;
-      int64_t end;
-      const T* p = row(r, end);
-      const int64_t k = k0 + c * CH;
-      if constexpr (sizeof(T) == 4) {
-        u32x4_t t[4];
+      constexpr int kRow = 64 / CH;             // chunks of one k in a half
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          t[i] = u32x4_t{0, 0, 0, 0};
-          if (p && k + i < depth) t[i] = load_part<u32x4_t, T>(p + (k + i) * ld, end);
+      for (int i = 0; i < 4; ++i) {
+        const int id = (i & 1) * kGemmThreads + tid, k = id / kRow, c = (id % kRow) ^ ((k & 3) | ((k >> 1) & 4));
+        const T* base = p.base[i >> 1] + k0 * p.ld;
+        const bool in = k < left && c * CH < p.rows[i >> 1];
+        if (fast) {
+          const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kOutside, 0x00027000);
+          const unsigned at = (unsigned)k * (unsigned)(p.ld * sizeof(T)) + c * 16;
+          reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, in ? at : kOutside, 0, 0));
+        } else {
+          reg[i] = u32x4_t{0, 0, 0, 0};
+          if (in) reg[i] = load_part<u32x4_t, T>(base + k * p.ld + c * CH, p.rows[i >> 1] - c * CH);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) reg[i] = u32x4_t{t[0][i], t[1][i], t[2][i], t[3][i]};
-      } else {
-        u32x2_t t[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          t[i] = u32x2_t{0, 0};
-          if (p && k + i < depth) t[i] = load_part<u32x2_t, T>(p + (k + i) * ld, end);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-            reg[i][d] = __builtin_amdgcn_perm(t[2 * d + 1][i >> 1], t[2 * d][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
       }
     }
   }
   __device__ __forceinline__ void store(char* lds) const {
-    const int tid = threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = K_CONTIGUOUS ? (i * kGemmThreads + tid) >> 3 : (tid >> 3) * 4 + i, c = tid & 7;
-      *reinterpret_cast<u32x4_t*>(lds + r * 128 + ((c ^ (r & 7)) << 4)) = reg[i];
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4_t*>(lds + (i * kGemmThreads + (int)threadIdx.x) * 16) = reg[i];
+  }
+  // Rows 32 `block` .. + 31 of the tile (rows contiguous: 32 (block % 2) .. of half block / 2) at the s-th pair of chunks of k.
+  __device__ static __forceinline__ u32x4_t frag(const char* lds, int block, int s) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    if constexpr (K_CONTIGUOUS) {
+      const int r = block * 32 + (lane & 31);
+      return *reinterpret_cast<const u32x4_t*>(lds + r * 128 + (((2 * s + half) ^ (r & 7)) << 4));
+    } else if constexpr (sizeof(T) == 2) {
+      const char* h = lds + (block >> 1) * (kGemmTileBytes / 2);
+      const int k = 16 * s + 8 * half + ((lane & 15) >> 2), m = (block & 1) * 32 + (lane & 16) + 4 * (lane & 3);
+      u32x4_t f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int kk = k + 4 * i;
+        typedef short v4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) v4 lds_v4;
+        const char* at = h + kk * 128 + (((m >> 3) ^ ((kk & 3) | ((kk >> 1) & 4))) << 4) + (m & 7) * 2;
+        const u32x2_t v = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)at));
+        f[2 * i] = v[0];
+        f[2 * i + 1] = v[1];
+      }
+      return f;
+    } else {
+      const char* h = lds + (block >> 1) * (kGemmTileBytes / 2);
+      const int k = 8 * s + 4 * half, m = (block & 1) * 32 + (lane & 31);
+      u32x4_t f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int kk = k + j;
+        f[j] = *reinterpret_cast<const unsigned*>(h + kk * 256 + (((m >> 2) ^ ((kk & 3) | ((kk >> 1) & 4))) << 4) + (m & 3) * 4);
+      }
+      return f;
     }
   }
 };
 
-// acc[i][j] of wavefront (wm, wn): rows 64 wm + 32 i of the first operand, 64 wn + 32 j of the second.  A lane holds row lane % 32
-// of the first and, at index 4 g + e, row 8 g + 4 (lane / 32) + e of the second: four neighbours for one store.
-// first / second(k tile) load the next tile into their stage; tiles: number of k tiles, the same for all threads.
-template <typename T, bool KA, bool KB, typename LoadA, typename LoadB>
-__device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[2][2], char* lds, int64_t tiles, LoadA&& load_a, LoadB&& load_b) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
+// acc[i][j] of wavefront (wm, wn): rows 64 wm + 32 i of the first operand; of the second 64 wn + 32 j, or with SPLIT row 32 wn of
+// half j.  A lane holds row lane % 32 of the first and, at index 4 g + e, row 8 g + 4 (lane / 32) + e of the second.
+// a(t, k0, depth) / b(...): the operands of tile t, and where its k begin and end; tiles: the same for all threads.
+template <typename T, bool KA, bool KB, bool SPLIT, typename A, typename B>
+__device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[2][2], char* lds, bool fast, int64_t tiles, A&& a, B&& b) {
+  const int wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -110,34 +143,77 @@ __device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[2][2], char* lds, int6
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   if (tiles <= 0) return;
-  GemmStage<T, KA> a;
-  GemmStage<T, KB> b;
-  load_a(a, (int64_t)0);
-  load_b(b, (int64_t)0);
-  const int ra = wm * 64 + (lane & 31), rb = wn * 64 + (lane & 31), half = lane >> 5, sw = lane & 7;
+  GemmStage<T, KA> sa;
+  GemmStage<T, KB> sb;
+  auto fetch = [&](int64_t t) {
+    int64_t k0, depth;
+    const GemmOperand<T> pa = a(t, k0, depth), pb = b(t);
+    sa.load(fast, pa, k0, depth);
+    sb.load(fast, pb, k0, depth);
+  };
+  fetch(0);
   for (int64_t t = 0; t < tiles; ++t) {
     char* la = lds + (t & 1) * 2 * kGemmTileBytes;
     char* lb = la + kGemmTileBytes;
-    a.store(la);
-    b.store(lb);
+    sa.store(la);
+    sb.store(lb);
     __syncthreads();
-    if (t + 1 < tiles) {
-      load_a(a, t + 1);
-      load_b(b, t + 1);
-    }
+    if (t + 1 < tiles) fetch(t + 1);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const int at = ((2 * s + half) ^ sw) << 4;
       u32x4_t fa[2], fb[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fa[i] = *reinterpret_cast<const u32x4_t*>(la + (ra + 32 * i) * 128 + at);
-        fb[i] = *reinterpret_cast<const u32x4_t*>(lb + (rb + 32 * i) * 128 + at);
-      }
+      for (int i = 0; i < 2; ++i) fa[i] = sa.frag(la, 2 * wm + i, s);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) fb[j] = sb.frag(lb, SPLIT ? 2 * j + wn : 2 * wn + j, s);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) mma_chunk<T>(acc[i][j], fb[j], fa[i]);
+    }
+  }
+}
+
+// The results through LDS in fp32, so that a row leaves in whole lines: each thread is handed, for kGemmTile * 128 / 8 / 256 = 8
+// places, eight neighbouring columns of a row: use(row, column, values).  SPLIT: column 32 wn + .. of half j is column
+// 64 j + 32 wn + .., and use gets the same eight columns of both halves: use(row, column, first half, second half), for
+// four places.
+template <bool SPLIT, typename Use>
+__device__ __forceinline__ void gemm_results(const f32x16_t (&acc)[2][2], char* lds, Use&& use) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
+  float* tile = reinterpret_cast<float*>(lds);           // 128 rows of 32 chunks, chunk c of row r at c ^ (r & 31)
+  auto chunk = [&](int r, int c) { return reinterpret_cast<f32x4*>(tile + r * 128 + ((c ^ (r & 31)) << 2)); };
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int r = 64 * wm + 32 * i + (lane & 31), n = (SPLIT ? 64 * j + 32 * wn : 64 * wn + 32 * j) + 8 * g + 4 * (lane >> 5);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
+        *chunk(r, n >> 2) = v;
+      }
+  __syncthreads();
+  constexpr int kRow = SPLIT ? 8 : 16;
+#pragma unroll
+  for (int i = 0; i < (SPLIT ? 4 : 8); ++i) {
+    const int id = i * kGemmThreads + (int)threadIdx.x, r = id / kRow, c = id % kRow;
+    float v[8];
+    auto take = [&](int first, float (&to)[8]) {
+      const f32x4 x = *chunk(r, first), y = *chunk(r, first + 1);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { to[e] = x[e]; to[4 + e] = y[e]; }
+    };
+    take(2 * c, v);
+    if constexpr (SPLIT) {
+      float u[8];
+      take(16 + 2 * c, u);
+      use(r, c * 8, v, u);
+    } else {
+      use(r, c * 8, v);
     }
   }
 }

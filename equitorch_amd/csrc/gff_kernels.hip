@@ -9,6 +9,7 @@
 #include "gff_gemm.h"
 
 #include <algorithm>
+#include <initializer_list>
 
 namespace cgtp {
 namespace {
@@ -52,69 +53,46 @@ __device__ __forceinline__ TilePlace tile_place(int inner_tiles) {
 }
 unsigned tile_grid(int64_t outer, int64_t inner) { return (unsigned)((outer + 7) / 8 * 8 * inner); }
 
-// Where a lane's results are within its wavefront's part.
-struct LanePlace { int m, n; };       // of acc[i][j]: row 32 i + m, columns 32 j + n + 8 g + e
-__device__ __forceinline__ LanePlace lane_place() {
-  const int lane = threadIdx.x & 63;
-  return {lane & 31, (lane >> 5) * 4};
-}
-
 template <typename T>
 struct UpArgs {
   const T *x, *wg, *wu;
   T *gate, *up, *mid;            // gate and up may be null (inference)
   int64_t n_rows;
-  int C, H, act;
+  int C, H, act, fast;
 };
 
-// g, u and m.  A tile is 128 rows x 64 hidden channels, the columns of a wavefront 32 of Wg and the same 32 of Wu.
+__device__ __forceinline__ int rows_left(int64_t n, int64_t from) { return (int)(n - from < kGemmTile ? n - from : kGemmTile); }
+
+// g, u and m.  A tile is 128 rows x 64 hidden channels, of Wg and of Wu.
 template <typename T>
-__global__ void __launch_bounds__(kGemmThreads) gff_up_kernel(UpArgs<T> a) {
+__global__ void __launch_bounds__(kGemmThreads, 2) gff_up_kernel(UpArgs<T> a) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
   const TilePlace at = tile_place((a.H + 63) / 64);
   const int64_t m0 = at.outer * kGemmTile;
   if (m0 >= a.n_rows) return;
   const int h0 = at.inner * 64;
+  const GemmOperand<T> x = {{a.x + m0 * a.C, nullptr}, a.C, {rows_left(a.n_rows, m0), 0}};
+  const GemmOperand<T> w = {{a.wg + h0, a.wu + h0}, a.H, {a.H - h0, a.H - h0}};
   f32x16_t acc[2][2];
-  gemm_loop<T, true, false>(
-      acc, lds, (a.C + D - 1) / D,
-      [&](auto& st, int64_t t) {
-        st.load([&](int r, int64_t&) { return m0 + r < a.n_rows ? a.x + (m0 + r) * a.C : nullptr; }, t * D, a.C, 0);
-      },
-      [&](auto& st, int64_t t) {
-        st.load([&](int r, int64_t& end) {
-          const int h = h0 + (r >> 6) * 32 + (r & 31);
-          end = a.H - h;
-          return end > 0 ? ((r & 32) ? a.wu : a.wg) + h : nullptr;
-        }, t * D, a.C, a.H);
-      });
-  const LanePlace lp = lane_place();
-  const int wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
+  gemm_loop<T, true, false, true>(acc, lds, a.fast, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+    k0 = t * D;
+    depth = a.C;
+    return x;
+  }, [&](int64_t) { return w; });
+  gemm_results<true>(acc, lds, [&](int r, int c, const float (&g)[8], const float (&u)[8]) {
+    const int left = a.H - h0 - c;
+    if (r >= x.rows[0] || left <= 0) return;
+    const int64_t to = (m0 + r) * a.H + h0 + c;
+    float m[8];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t m = m0 + wm * 64 + 32 * i + lp.m;
-    if (m >= a.n_rows) continue;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int h = h0 + wn * 32 + 8 * g + lp.n;
-      if (h >= a.H) continue;
-      T vg[4], vu[4], vm[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float fg = acc[i][0][4 * g + e], fu = acc[i][1][4 * g + e];
-        vg[e] = (T)fg;
-        vu[e] = (T)fu;
-        vm[e] = (T)(gff_act<T>(a.act, fg) * fu);
-      }
-      const int64_t to = m * a.H + h;
-      store_part<T, 4>(a.mid + to, vm, a.H - h);
-      if (a.gate) {
-        store_part<T, 4>(a.gate + to, vg, a.H - h);
-        store_part<T, 4>(a.up + to, vu, a.H - h);
-      }
+    for (int e = 0; e < 8; ++e) m[e] = gff_act<T>(a.act, g[e]) * u[e];
+    store_eight(a.mid + to, m, left);
+    if (a.gate) {
+      store_eight(a.gate + to, g, left);
+      store_eight(a.up + to, u, left);
     }
-  }
+  });
 }
 
 template <typename T>
@@ -122,57 +100,43 @@ struct MidGradArgs {
   const T *gy, *wd, *gate, *up;
   T *g_gate, *g_up;
   int64_t n_rows;
-  int H, C, act;
+  int H, C, act, fast;
 };
 
 // dg and du from dm = dy Wd^T.
 template <typename T>
-__global__ void __launch_bounds__(kGemmThreads) gff_mid_grad_kernel(MidGradArgs<T> a) {
+__global__ void __launch_bounds__(kGemmThreads, 2) gff_mid_grad_kernel(MidGradArgs<T> a) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
   const TilePlace at = tile_place((a.H + kGemmTile - 1) / kGemmTile);
   const int64_t m0 = at.outer * kGemmTile;
   if (m0 >= a.n_rows) return;
   const int h0 = at.inner * kGemmTile;
+  const GemmOperand<T> gy = {{a.gy + m0 * a.C, nullptr}, a.C, {rows_left(a.n_rows, m0), 0}};
+  const GemmOperand<T> wd = {{a.wd + (int64_t)h0 * a.C, nullptr}, a.C, {rows_left(a.H, h0), 0}};
   f32x16_t acc[2][2];
-  gemm_loop<T, true, true>(
-      acc, lds, (a.C + D - 1) / D,
-      [&](auto& st, int64_t t) {
-        st.load([&](int r, int64_t&) { return m0 + r < a.n_rows ? a.gy + (m0 + r) * a.C : nullptr; }, t * D, a.C, 0);
-      },
-      [&](auto& st, int64_t t) {
-        st.load([&](int r, int64_t&) { return h0 + r < a.H ? a.wd + (int64_t)(h0 + r) * a.C : nullptr; }, t * D, a.C, 0);
-      });
-  const LanePlace lp = lane_place();
-  const int wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
+  gemm_loop<T, true, true, false>(acc, lds, a.fast, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+    k0 = t * D;
+    depth = a.C;
+    return gy;
+  }, [&](int64_t) { return wd; });
+  gemm_results<false>(acc, lds, [&](int r, int c, const float (&dm)[8]) {
+    const int left = a.H - h0 - c;
+    if (r >= gy.rows[0] || left <= 0) return;
+    const int64_t to = (m0 + r) * a.H + h0 + c;
+    float g[8], u[8];
+    load_eight(g, a.gate + to, left);
+    load_eight(u, a.up + to, left);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t m = m0 + wm * 64 + 32 * i + lp.m;
-    if (m >= a.n_rows) continue;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int h = h0 + wn * 64 + 32 * j + 8 * g + lp.n;
-        if (h >= a.H) continue;
-        const int64_t to = m * a.H + h;
-        typedef Loose<T, 4> V4;
-        typedef unsigned raw_t __attribute__((ext_vector_type(sizeof(T))));
-        const V4 vg = __builtin_bit_cast(V4, load_part<raw_t, T>(a.gate + to, a.H - h));
-        const V4 vu = __builtin_bit_cast(V4, load_part<raw_t, T>(a.up + to, a.H - h));
-        T dg[4], du[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float dm = acc[i][j][4 * g + e];
-          float value;
-          const float slope = gff_act_grad<T>(a.act, (float)vg.v[e], value);
-          dg[e] = (T)(dm * (float)vu.v[e] * slope);
-          du[e] = (T)(dm * value);
-        }
-        store_part<T, 4>(a.g_gate + to, dg, a.H - h);
-        store_part<T, 4>(a.g_up + to, du, a.H - h);
-      }
-  }
+    for (int e = 0; e < 8; ++e) {
+      float value;
+      const float slope = gff_act_grad<T>(a.act, g[e], value);
+      g[e] = dm[e] * u[e] * slope;
+      u[e] = dm[e] * value;
+    }
+    store_eight(a.g_gate + to, g, left);
+    store_eight(a.g_up + to, u, left);
+  });
 }
 
 // out = sum over segments of A_s B_s: y = m Wd (one segment), dx = dg Wg^T + du Wu^T (two).  A is contiguous along k.
@@ -181,50 +145,30 @@ struct RowsArgs {
   const T *a[2], *b[2];
   T* out;
   int64_t n_rows, ldb;
-  int segments, K, N;            // per segment
+  int segments, K, N, fast;      // K: per segment
 };
 template <typename T, bool KB>
-__global__ void __launch_bounds__(kGemmThreads) gff_rows_kernel(RowsArgs<T> a) {
+__global__ void __launch_bounds__(kGemmThreads, 2) gff_rows_kernel(RowsArgs<T> a) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
   const TilePlace at = tile_place((a.N + kGemmTile - 1) / kGemmTile);
   const int64_t m0 = at.outer * kGemmTile;
   if (m0 >= a.n_rows) return;
-  const int n0 = at.inner * kGemmTile, tiles = (a.K + D - 1) / D;
+  const int n0 = at.inner * kGemmTile, tiles = (a.K + D - 1) / D, rows = rows_left(a.n_rows, m0), cols = rows_left(a.N, n0);
   f32x16_t acc[2][2];
-  gemm_loop<T, true, KB>(
-      acc, lds, (int64_t)tiles * a.segments,
-      [&](auto& st, int64_t t) {
-        const T* p = t < tiles ? a.a[0] : a.a[1];
-        if (t >= tiles) t -= tiles;
-        st.load([&](int r, int64_t&) { return m0 + r < a.n_rows ? p + (m0 + r) * a.K : nullptr; }, t * D, a.K, 0);
-      },
-      [&](auto& st, int64_t t) {
-        const T* p = t < tiles ? a.b[0] : a.b[1];
-        if (t >= tiles) t -= tiles;
-        st.load([&](int r, int64_t& end) {
-          end = a.N - n0 - r;
-          return end > 0 ? p + (KB ? (int64_t)(n0 + r) * a.ldb : n0 + r) : nullptr;
-        }, t * D, a.K, a.ldb);
-      });
-  const LanePlace lp = lane_place();
-  const int wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t m = m0 + wm * 64 + 32 * i + lp.m;
-    if (m >= a.n_rows) continue;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int n = n0 + wn * 64 + 32 * j + 8 * g + lp.n;
-        if (n >= a.N) continue;
-        T v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)acc[i][j][4 * g + e];
-        store_part<T, 4>(a.out + m * a.N + n, v, a.N - n);
-      }
-  }
+  gemm_loop<T, true, KB, false>(acc, lds, a.fast, (int64_t)tiles * a.segments, [&](int64_t t, int64_t& k0, int64_t& depth) {
+    k0 = (t < tiles ? t : t - tiles) * D;
+    depth = a.K;
+    return GemmOperand<T>{{(t < tiles ? a.a[0] : a.a[1]) + m0 * a.K, nullptr}, a.K, {rows, 0}};
+  }, [&](int64_t t) {
+    const T* b = t < tiles ? a.b[0] : a.b[1];
+    if (KB) return GemmOperand<T>{{b + n0 * a.ldb, nullptr}, a.ldb, {cols, 0}};
+    return GemmOperand<T>{{b + n0, b + n0 + 64}, a.ldb, {cols, cols - 64}};
+  });
+  gemm_results<false>(acc, lds, [&](int r, int c, const float (&v)[8]) {
+    const int left = a.N - n0 - c;
+    if (r < rows && left > 0) store_eight(a.out + (m0 + r) * a.N + n0 + c, v, left);
+  });
 }
 
 // Weight gradients out_j = A_j^T B_j over all rows: both operands contiguous along the tile's rows.  The rows are cut
@@ -241,10 +185,10 @@ struct WeightArgs {
   WeightJob<T> job[3];
   float* parts;
   int64_t n_rows, rows_per_split, part_elems;
-  int jobs, tiles, splits;
+  int jobs, tiles, splits, fast;
 };
 template <typename T>
-__global__ void __launch_bounds__(kGemmThreads) gff_weight_kernel(WeightArgs<T> w) {
+__global__ void __launch_bounds__(kGemmThreads, 2) gff_weight_kernel(WeightArgs<T> w) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
   const TilePlace at = tile_place(w.tiles);
@@ -254,48 +198,23 @@ __global__ void __launch_bounds__(kGemmThreads) gff_weight_kernel(WeightArgs<T> 
   const int tile = at.inner - job.first_tile;
   const int m0 = tile / job.tiles_n * kGemmTile, n0 = tile % job.tiles_n * kGemmTile;
   const int64_t r0 = at.outer * w.rows_per_split;
-  const int64_t depth = std::min(w.rows_per_split, w.n_rows - r0);
+  const int64_t end = std::min(w.rows_per_split, w.n_rows - r0);
+  const int rows = rows_left(job.M, m0), cols = rows_left(job.N, n0);
+  const T *ja = job.a + r0 * job.M + m0, *jb = job.b + r0 * job.N + n0;
+  const GemmOperand<T> pa = {{ja, ja + 64}, job.M, {rows, rows - 64}}, pb = {{jb, jb + 64}, job.N, {cols, cols - 64}};
   f32x16_t acc[2][2];
-  gemm_loop<T, false, false>(
-      acc, lds, (depth + D - 1) / D,
-      [&](auto& st, int64_t t) {
-        st.load([&](int r, int64_t& end) {
-          end = job.M - m0 - r;
-          return end > 0 ? job.a + r0 * job.M + m0 + r : nullptr;
-        }, t * D, depth, job.M);
-      },
-      [&](auto& st, int64_t t) {
-        st.load([&](int r, int64_t& end) {
-          end = job.N - n0 - r;
-          return end > 0 ? job.b + r0 * job.N + n0 + r : nullptr;
-        }, t * D, depth, job.N);
-      });
-  const LanePlace lp = lane_place();
-  const int wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int m = m0 + wm * 64 + 32 * i + lp.m;
-    if (m >= job.M) continue;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int n = n0 + wn * 64 + 32 * j + 8 * g + lp.n;
-        if (n >= job.N) continue;
-        const int64_t to = (int64_t)m * job.N + n;
-        if (w.splits > 1) {
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
-          store_part<float, 4>(w.parts + at.outer * w.part_elems + job.first_part + to, v, job.N - n);
-        } else {
-          T v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (T)acc[i][j][4 * g + e];
-          store_part<T, 4>(job.out + to, v, job.N - n);
-        }
-      }
-  }
+  gemm_loop<T, false, false, false>(acc, lds, w.fast, (end + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+    k0 = t * D;
+    depth = end;
+    return pa;
+  }, [&](int64_t) { return pb; });
+  gemm_results<false>(acc, lds, [&](int r, int c, const float (&v)[8]) {
+    const int left = job.N - n0 - c;
+    if (r >= rows || left <= 0) return;
+    const int64_t to = (int64_t)(m0 + r) * job.N + n0 + c;
+    if (w.splits > 1) store_eight(w.parts + at.outer * w.part_elems + job.first_part + to, v, left);
+    else store_eight(job.out + to, v, left);
+  });
 }
 template <typename T>
 __global__ void __launch_bounds__(256) gff_add_kernel(WeightArgs<T> w) {
@@ -323,6 +242,16 @@ int gff_check(const cgtp_gff_args* a) {
   return CGTP_OK;
 }
 
+// Whether rows of `ld` elements are whole aligned chunks, and a tile's offsets fit 31 bits.
+template <typename T>
+bool whole_chunks(std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> lds) {
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return false;
+  for (int64_t ld : lds)
+    if (ld % (16 / (int)sizeof(T)) || ld * (int64_t)sizeof(T) * kGemmTile > 0x7fffffff) return false;
+  return true;
+}
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Ranges the rows are cut into for the weight gradients: two workgroups for each compute unit, at least eight k tiles each.
@@ -344,10 +273,10 @@ template <typename T>
 int gff_forward(const cgtp_gff_args* a, hipStream_t s) {
   const int64_t mt = ceil_div(a->n_rows, kGemmTile);
   UpArgs<T> u = {(const T*)a->x, (const T*)a->w_gate, (const T*)a->w_up, (T*)a->gate, (T*)a->up, (T*)a->mid, a->n_rows,
-                 a->c_in, a->hidden, a->activation};
+                 a->c_in, a->hidden, a->activation, whole_chunks<T>({a->x, a->w_gate, a->w_up}, {a->c_in, a->hidden})};
   hipLaunchKernelGGL(gff_up_kernel<T>, dim3(tile_grid(mt, ceil_div(a->hidden, 64))), dim3(kGemmThreads), 0, s, u);
   RowsArgs<T> d = {{(const T*)a->mid, nullptr}, {(const T*)a->w_down, nullptr}, (T*)a->out, a->n_rows, a->c_out, 1, a->hidden,
-                   a->c_out};
+                   a->c_out, whole_chunks<T>({a->mid, a->w_down}, {a->hidden, a->c_out})};
   hipLaunchKernelGGL((gff_rows_kernel<T, false>), dim3(tile_grid(mt, ceil_div(a->c_out, kGemmTile))), dim3(kGemmThreads), 0,
                      s, d);
   return launch_status();
@@ -358,12 +287,14 @@ int gff_backward(const cgtp_gff_args* a, hipStream_t s) {
   const int64_t mt = ceil_div(a->n_rows, kGemmTile);
   if (a->n_rows > 0 && (a->grad_x || a->grad_w_gate || a->grad_w_up)) {
     MidGradArgs<T> m = {(const T*)a->grad_out, (const T*)a->w_down, (const T*)a->gate, (const T*)a->up, (T*)a->grad_gate,
-                        (T*)a->grad_up, a->n_rows, a->hidden, a->c_out, a->activation};
+                        (T*)a->grad_up, a->n_rows, a->hidden, a->c_out, a->activation,
+                        whole_chunks<T>({a->grad_out, a->w_down}, {a->c_out})};
     hipLaunchKernelGGL(gff_mid_grad_kernel<T>, dim3(tile_grid(mt, ceil_div(a->hidden, kGemmTile))), dim3(kGemmThreads), 0, s, m);
   }
   if (a->n_rows > 0 && a->grad_x) {
     RowsArgs<T> d = {{(const T*)a->grad_gate, (const T*)a->grad_up}, {(const T*)a->w_gate, (const T*)a->w_up}, (T*)a->grad_x,
-                     a->n_rows, a->hidden, 2, a->hidden, a->c_in};
+                     a->n_rows, a->hidden, 2, a->hidden, a->c_in,
+                     whole_chunks<T>({a->grad_gate, a->grad_up, a->w_gate, a->w_up}, {a->hidden})};
     hipLaunchKernelGGL((gff_rows_kernel<T, true>), dim3(tile_grid(mt, ceil_div(a->c_in, kGemmTile))), dim3(kGemmThreads), 0, s, d);
   }
   const WeightShape shape = weight_shape(a);
@@ -381,6 +312,7 @@ int gff_backward(const cgtp_gff_args* a, hipStream_t s) {
   job(a->x, a->grad_gate, a->grad_w_gate, a->c_in, a->hidden);
   job(a->x, a->grad_up, a->grad_w_up, a->c_in, a->hidden);
   job(a->mid, a->grad_out, a->grad_w_down, a->hidden, a->c_out);
+  w.fast = whole_chunks<T>({a->x, a->grad_gate, a->grad_up, a->mid, a->grad_out}, {a->c_in, a->hidden, a->c_out});
   if (w.jobs) {
     hipLaunchKernelGGL(gff_weight_kernel<T>, dim3(tile_grid(w.splits, w.tiles)), dim3(kGemmThreads), 0, s, w);
     if (w.splits > 1)
