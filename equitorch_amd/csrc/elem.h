@@ -77,22 +77,7 @@ __device__ __forceinline__ void store_part(T* p, const T (&e)[N], int64_t valid)
   }
 }
 
-// Eight elements in at most two 16-byte vectors: as float from an element-aligned address, and rounded to one.
-template <typename T>
-__device__ __forceinline__ void load_eight(float (&dst)[8], const T* p, int64_t valid) {
-  constexpr int N = 16 / sizeof(T);
-#pragma unroll
-  for (int i = 0; i < 8; i += N) {
-    if (valid <= i) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) dst[i + j] = 0.f;
-      continue;
-    }
-    const Loose<T, N> v = __builtin_bit_cast(Loose<T, N>, load_part<u32x4_t, T>(p + i, valid - i));
-#pragma unroll
-    for (int j = 0; j < N; ++j) dst[i + j] = (float)v.v[j];
-  }
-}
+// Eight values rounded to an element-aligned address, the first `valid` of them.
 template <typename T>
 __device__ __forceinline__ void store_eight(T* p, const float (&src)[8], int64_t valid) {
   constexpr int N = 16 / sizeof(T);

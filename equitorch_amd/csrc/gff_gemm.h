@@ -1,5 +1,5 @@
 // Matrix products of the gated feed-forward block on the matrix cores: tiles of 128 x 128, four wavefronts of 64 x 64 each,
-// operands brought through registers into two LDS buffers, the next tile loaded while one is worked on.
+// operands brought through registers into two LDS buffers, the next two tiles being loaded while one is worked on.
 //
 // An operand is a matrix whose k or whose rows are contiguous.  In LDS a tile is 1024 chunks of 16 bytes either way:
 //   k contiguous    128 rows of eight chunks along k, chunk c of row r at place c ^ (r & 7);
@@ -56,7 +56,8 @@ struct GemmStage {
   u32x4_t reg[4];
 
   // k0: first k of the tile, depth: end of k.
-  __device__ __forceinline__ void load(bool fast, const GemmOperand<T>& p, int64_t k0, int64_t depth) {
+  template <bool FAST>
+  __device__ __forceinline__ void load(const GemmOperand<T>& p, int64_t k0, int64_t depth) {
     const int tid = threadIdx.x, left = (int)(depth - k0 < GemmType<T>::kDepth ? depth - k0 : GemmType<T>::kDepth);
     if constexpr (K_CONTIGUOUS) {
       const T* base = p.base[0] + k0;
@@ -65,7 +66,7 @@ struct GemmStage {
       for (int i = 0; i < 4; ++i) {
         const int id = i * kGemmThreads + tid, r = id >> 3, c = (id & 7) ^ (r & 7);
         const bool in = r < p.rows[0] && c * CH < left;
-        if (fast) {
+        if constexpr (FAST) {
           const unsigned at = (unsigned)r * (unsigned)(p.ld * sizeof(T)) + c * 16;
           reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, in ? at : kOutside, 0, 0));
         } else {
@@ -80,7 +81,7 @@ struct GemmStage {
         const int id = (i & 1) * kGemmThreads + tid, k = id / kRow, c = (id % kRow) ^ ((k & 3) | ((k >> 1) & 4));
         const T* base = p.base[i >> 1] + k0 * p.ld;
         const bool in = k < left && c * CH < p.rows[i >> 1];
-        if (fast) {
+        if constexpr (FAST) {
           const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kOutside, 0x00027000);
           const unsigned at = (unsigned)k * (unsigned)(p.ld * sizeof(T)) + c * 16;
           reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, in ? at : kOutside, 0, 0));
@@ -133,8 +134,8 @@ struct GemmStage {
 // acc[i][j] of wavefront (wm, wn): rows 64 wm + 32 i of the first operand; of the second 64 wn + 32 j, or with SPLIT row 32 wn of
 // half j.  A lane holds row lane % 32 of the first and, at index 4 g + e, row 8 g + 4 (lane / 32) + e of the second.
 // a(t, k0, depth) / b(...): the operands of tile t, and where its k begin and end; tiles: the same for all threads.
-template <typename T, bool KA, bool KB, bool SPLIT, typename A, typename B>
-__device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[2][2], char* lds, bool fast, int64_t tiles, A&& a, B&& b) {
+template <typename T, bool FAST, bool KA, bool KB, bool SPLIT, typename A, typename B>
+__device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[2][2], char* lds, int64_t tiles, A&& a, B&& b) {
   const int wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -143,43 +144,84 @@ __device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[2][2], char* lds, bool
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   if (tiles <= 0) return;
-  GemmStage<T, KA> sa;
-  GemmStage<T, KB> sb;
-  auto fetch = [&](int64_t t) {
+  GemmStage<T, KA> sa[2];
+  GemmStage<T, KB> sb[2];
+  auto fetch = [&](int which, int64_t t) {
     int64_t k0, depth;
     const GemmOperand<T> pa = a(t, k0, depth), pb = b(t);
-    sa.load(fast, pa, k0, depth);
-    sb.load(fast, pb, k0, depth);
+    sa[which].template load<FAST>(pa, k0, depth);
+    sb[which].template load<FAST>(pb, k0, depth);
   };
-  fetch(0);
-  for (int64_t t = 0; t < tiles; ++t) {
-    char* la = lds + (t & 1) * 2 * kGemmTileBytes;
+  auto step = [&](int which, int64_t t) {
+    char* la = lds + which * 2 * kGemmTileBytes;
     char* lb = la + kGemmTileBytes;
-    sa.store(la);
-    sb.store(lb);
+    sa[which].store(la);
+    sb[which].store(lb);
     __syncthreads();
-    if (t + 1 < tiles) fetch(t + 1);
+    if (t + 2 < tiles) fetch(which, t + 2);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       u32x4_t fa[2], fb[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) fa[i] = sa.frag(la, 2 * wm + i, s);
+      for (int i = 0; i < 2; ++i) fa[i] = GemmStage<T, KA>::frag(la, 2 * wm + i, s);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) fb[j] = sb.frag(lb, SPLIT ? 2 * j + wn : 2 * wn + j, s);
+      for (int j = 0; j < 2; ++j) fb[j] = GemmStage<T, KB>::frag(lb, SPLIT ? 2 * j + wn : 2 * wn + j, s);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) mma_chunk<T>(acc[i][j], fb[j], fa[i]);
     }
+  };
+  fetch(0, 0);
+  if (tiles > 1) fetch(1, 1);
+  for (int64_t t = 0; t < tiles; t += 2) {
+    step(0, t);
+    if (t + 1 < tiles) step(1, t + 1);
   }
 }
 
-// The results through LDS in fp32, so that a row leaves in whole lines: each thread is handed, for kGemmTile * 128 / 8 / 256 = 8
-// places, eight neighbouring columns of a row: use(row, column, values).  SPLIT: column 32 wn + .. of half j is column
-// 64 j + 32 wn + .., and use gets the same eight columns of both halves: use(row, column, first half, second half), for
-// four places.
-template <bool SPLIT, typename Use>
-__device__ __forceinline__ void gemm_results(const f32x16_t (&acc)[2][2], char* lds, Use&& use) {
+// Eight neighbouring elements as they come from memory.
+template <typename T>
+struct EightRaw {
+  static constexpr int N = 16 / (int)sizeof(T);
+  u32x4_t v[8 / N];
+  __device__ __forceinline__ void load(const T* p, int valid) {
+#pragma unroll
+    for (int i = 0; i < 8 / N; ++i) {
+      v[i] = u32x4_t{0, 0, 0, 0};
+      if (valid > i * N) v[i] = load_part<u32x4_t, T>(p + i * N, valid - i * N);
+    }
+  }
+  __device__ __forceinline__ void get(float (&to)[8]) const {
+    typedef T vec __attribute__((ext_vector_type(N)));
+#pragma unroll
+    for (int i = 0; i < 8 / N; ++i) {
+      const vec e = __builtin_bit_cast(vec, v[i]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) to[i * N + j] = (float)e[j];
+    }
+  }
+};
+
+// The results through LDS in fp32, so that a row leaves in whole lines: each thread is handed, for eight places i, eight
+// neighbouring columns of a row: use(i, row, column, values).  SPLIT: column 32 wn + .. of half j is column 64 j + 32 wn + ..,
+// and use gets the same eight columns of both halves, for four places: use(i, row, column, first half, second half).
+// fetch(i, row, column) is called AHEAD places earlier.
+template <bool SPLIT, int AHEAD, typename Fetch, typename Use>
+__device__ __forceinline__ void gemm_results(const f32x16_t (&acc)[2][2], char* lds, Fetch&& fetch, Use&& use) {
+  constexpr int kRow = SPLIT ? 8 : 16, kPlaces = SPLIT ? 4 : 8;
+  auto place = [&](int i, int& r, int& c) {
+    const int id = i * kGemmThreads + (int)threadIdx.x;
+    r = id / kRow;
+    c = id % kRow * 8;
+  };
+  auto ahead = [&](int i) {
+    int r, c;
+    place(i, r, c);
+    fetch(i, r, c);
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD && i < kPlaces; ++i) ahead(i);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
   float* tile = reinterpret_cast<float*>(lds);           // 128 rows of 32 chunks, chunk c of row r at c ^ (r & 31)
   auto chunk = [&](int r, int c) { return reinterpret_cast<f32x4*>(tile + r * 128 + ((c ^ (r & 31)) << 2)); };
@@ -197,24 +239,25 @@ __device__ __forceinline__ void gemm_results(const f32x16_t (&acc)[2][2], char* 
         *chunk(r, n >> 2) = v;
       }
   __syncthreads();
-  constexpr int kRow = SPLIT ? 8 : 16;
 #pragma unroll
-  for (int i = 0; i < (SPLIT ? 4 : 8); ++i) {
-    const int id = i * kGemmThreads + (int)threadIdx.x, r = id / kRow, c = id % kRow;
+  for (int i = 0; i < kPlaces; ++i) {
+    int r, c;
+    place(i, r, c);
     float v[8];
     auto take = [&](int first, float (&to)[8]) {
       const f32x4 x = *chunk(r, first), y = *chunk(r, first + 1);
 #pragma unroll
       for (int e = 0; e < 4; ++e) { to[e] = x[e]; to[4 + e] = y[e]; }
     };
-    take(2 * c, v);
+    take(c / 4, v);
     if constexpr (SPLIT) {
       float u[8];
-      take(16 + 2 * c, u);
-      use(r, c * 8, v, u);
+      take(16 + c / 4, u);
+      use(i, r, c, v, u);
     } else {
-      use(r, c * 8, v);
+      use(i, r, c, v);
     }
+    if (i + AHEAD < kPlaces) ahead(i + AHEAD);
   }
 }
 

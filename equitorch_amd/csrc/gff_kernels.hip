@@ -16,10 +16,11 @@ namespace {
 
 constexpr int kActs = 3;       // CGTP_ACT_SILU, CGTP_ACT_GELU, CGTP_ACT_SIGMOID
 
-// act(g) and its derivative.  16-bit types take the hardware's exponential (1e-6 relative), fp32 the exact one.
+// act(g) and its derivative.  16-bit types take the hardware's exponential and reciprocal (1e-6
+// relative), fp32 the library's.
 template <typename T>
 __device__ __forceinline__ float gff_sigmoid(float g) {
-  if constexpr (sizeof(T) == 2) return 1.f / (1.f + __expf(-g));
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.f + __expf(-g));
   else return 1.f / (1.f + expf(-g));
 }
 template <typename T>
@@ -58,13 +59,13 @@ struct UpArgs {
   const T *x, *wg, *wu;
   T *gate, *up, *mid;            // gate and up may be null (inference)
   int64_t n_rows;
-  int C, H, act, fast;
+  int C, H, act;
 };
 
 __device__ __forceinline__ int rows_left(int64_t n, int64_t from) { return (int)(n - from < kGemmTile ? n - from : kGemmTile); }
 
 // g, u and m.  A tile is 128 rows x 64 hidden channels, of Wg and of Wu.
-template <typename T>
+template <typename T, bool FAST>
 __global__ void __launch_bounds__(kGemmThreads, 2) gff_up_kernel(UpArgs<T> a) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
@@ -75,12 +76,12 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gff_up_kernel(UpArgs<T> a) {
   const GemmOperand<T> x = {{a.x + m0 * a.C, nullptr}, a.C, {rows_left(a.n_rows, m0), 0}};
   const GemmOperand<T> w = {{a.wg + h0, a.wu + h0}, a.H, {a.H - h0, a.H - h0}};
   f32x16_t acc[2][2];
-  gemm_loop<T, true, false, true>(acc, lds, a.fast, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, true, false, true>(acc, lds, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = a.C;
     return x;
   }, [&](int64_t) { return w; });
-  gemm_results<true>(acc, lds, [&](int r, int c, const float (&g)[8], const float (&u)[8]) {
+  gemm_results<true, 4>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&g)[8], const float (&u)[8]) {
     const int left = a.H - h0 - c;
     if (r >= x.rows[0] || left <= 0) return;
     const int64_t to = (m0 + r) * a.H + h0 + c;
@@ -100,11 +101,11 @@ struct MidGradArgs {
   const T *gy, *wd, *gate, *up;
   T *g_gate, *g_up;
   int64_t n_rows;
-  int H, C, act, fast;
+  int H, C, act;
 };
 
 // dg and du from dm = dy Wd^T.
-template <typename T>
+template <typename T, bool FAST>
 __global__ void __launch_bounds__(kGemmThreads, 2) gff_mid_grad_kernel(MidGradArgs<T> a) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
@@ -115,18 +116,28 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gff_mid_grad_kernel(MidGradAr
   const GemmOperand<T> gy = {{a.gy + m0 * a.C, nullptr}, a.C, {rows_left(a.n_rows, m0), 0}};
   const GemmOperand<T> wd = {{a.wd + (int64_t)h0 * a.C, nullptr}, a.C, {rows_left(a.H, h0), 0}};
   f32x16_t acc[2][2];
-  gemm_loop<T, true, true, false>(acc, lds, a.fast, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, true, true, false>(acc, lds, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = a.C;
     return gy;
   }, [&](int64_t) { return wd; });
-  gemm_results<false>(acc, lds, [&](int r, int c, const float (&dm)[8]) {
+  // The projections' part is fetched a few places ahead of its use: one wait for memory in place of one for each place.
+  constexpr int kAhead = sizeof(T) == 2 ? 8 : 4;
+  EightRaw<T> pg[kAhead], pu[kAhead];
+  auto fetch = [&](int i, int r, int c) {
+    const int left = a.H - h0 - c;
+    if (r >= gy.rows[0] || left <= 0) return;
+    const int64_t at = (m0 + r) * a.H + h0 + c;
+    pg[i % kAhead].load(a.gate + at, left);
+    pu[i % kAhead].load(a.up + at, left);
+  };
+  gemm_results<false, kAhead>(acc, lds, fetch, [&](int i, int r, int c, const float (&dm)[8]) {
     const int left = a.H - h0 - c;
     if (r >= gy.rows[0] || left <= 0) return;
     const int64_t to = (m0 + r) * a.H + h0 + c;
     float g[8], u[8];
-    load_eight(g, a.gate + to, left);
-    load_eight(u, a.up + to, left);
+    pg[i % kAhead].get(g);
+    pu[i % kAhead].get(u);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float value;
@@ -145,9 +156,9 @@ struct RowsArgs {
   const T *a[2], *b[2];
   T* out;
   int64_t n_rows, ldb;
-  int segments, K, N, fast;      // K: per segment
+  int segments, K, N;      // K: per segment
 };
-template <typename T, bool KB>
+template <typename T, bool FAST, bool KB>
 __global__ void __launch_bounds__(kGemmThreads, 2) gff_rows_kernel(RowsArgs<T> a) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
@@ -156,7 +167,7 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gff_rows_kernel(RowsArgs<T> a
   if (m0 >= a.n_rows) return;
   const int n0 = at.inner * kGemmTile, tiles = (a.K + D - 1) / D, rows = rows_left(a.n_rows, m0), cols = rows_left(a.N, n0);
   f32x16_t acc[2][2];
-  gemm_loop<T, true, KB, false>(acc, lds, a.fast, (int64_t)tiles * a.segments, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, true, KB, false>(acc, lds, (int64_t)tiles * a.segments, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = (t < tiles ? t : t - tiles) * D;
     depth = a.K;
     return GemmOperand<T>{{(t < tiles ? a.a[0] : a.a[1]) + m0 * a.K, nullptr}, a.K, {rows, 0}};
@@ -165,7 +176,7 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gff_rows_kernel(RowsArgs<T> a
     if (KB) return GemmOperand<T>{{b + n0 * a.ldb, nullptr}, a.ldb, {cols, 0}};
     return GemmOperand<T>{{b + n0, b + n0 + 64}, a.ldb, {cols, cols - 64}};
   });
-  gemm_results<false>(acc, lds, [&](int r, int c, const float (&v)[8]) {
+  gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
     const int left = a.N - n0 - c;
     if (r < rows && left > 0) store_eight(a.out + (m0 + r) * a.N + n0 + c, v, left);
   });
@@ -185,9 +196,9 @@ struct WeightArgs {
   WeightJob<T> job[3];
   float* parts;
   int64_t n_rows, rows_per_split, part_elems;
-  int jobs, tiles, splits, fast;
+  int jobs, tiles, splits;
 };
-template <typename T>
+template <typename T, bool FAST>
 __global__ void __launch_bounds__(kGemmThreads, 2) gff_weight_kernel(WeightArgs<T> w) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
@@ -203,12 +214,12 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gff_weight_kernel(WeightArgs<
   const T *ja = job.a + r0 * job.M + m0, *jb = job.b + r0 * job.N + n0;
   const GemmOperand<T> pa = {{ja, ja + 64}, job.M, {rows, rows - 64}}, pb = {{jb, jb + 64}, job.N, {cols, cols - 64}};
   f32x16_t acc[2][2];
-  gemm_loop<T, false, false, false>(acc, lds, w.fast, (end + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, false, false, false>(acc, lds, (end + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = end;
     return pa;
   }, [&](int64_t) { return pb; });
-  gemm_results<false>(acc, lds, [&](int r, int c, const float (&v)[8]) {
+  gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
     const int left = job.N - n0 - c;
     if (r >= rows || left <= 0) return;
     const int64_t to = (int64_t)(m0 + r) * job.N + n0 + c;
@@ -272,13 +283,14 @@ WeightShape weight_shape(const cgtp_gff_args* a) {
 template <typename T>
 int gff_forward(const cgtp_gff_args* a, hipStream_t s) {
   const int64_t mt = ceil_div(a->n_rows, kGemmTile);
-  UpArgs<T> u = {(const T*)a->x, (const T*)a->w_gate, (const T*)a->w_up, (T*)a->gate, (T*)a->up, (T*)a->mid, a->n_rows,
-                 a->c_in, a->hidden, a->activation, whole_chunks<T>({a->x, a->w_gate, a->w_up}, {a->c_in, a->hidden})};
-  hipLaunchKernelGGL(gff_up_kernel<T>, dim3(tile_grid(mt, ceil_div(a->hidden, 64))), dim3(kGemmThreads), 0, s, u);
-  RowsArgs<T> d = {{(const T*)a->mid, nullptr}, {(const T*)a->w_down, nullptr}, (T*)a->out, a->n_rows, a->c_out, 1, a->hidden,
-                   a->c_out, whole_chunks<T>({a->mid, a->w_down}, {a->hidden, a->c_out})};
-  hipLaunchKernelGGL((gff_rows_kernel<T, false>), dim3(tile_grid(mt, ceil_div(a->c_out, kGemmTile))), dim3(kGemmThreads), 0,
-                     s, d);
+  const UpArgs<T> u = {(const T*)a->x, (const T*)a->w_gate, (const T*)a->w_up, (T*)a->gate, (T*)a->up, (T*)a->mid, a->n_rows,
+                       a->c_in, a->hidden, a->activation};
+  auto up = whole_chunks<T>({u.x, u.wg, u.wu}, {u.C, u.H}) ? gff_up_kernel<T, true> : gff_up_kernel<T, false>;
+  hipLaunchKernelGGL(up, dim3(tile_grid(mt, ceil_div(a->hidden, 64))), dim3(kGemmThreads), 0, s, u);
+  const RowsArgs<T> d = {{(const T*)a->mid, nullptr}, {(const T*)a->w_down, nullptr}, (T*)a->out, a->n_rows, a->c_out, 1, a->hidden,
+                         a->c_out};
+  auto down = whole_chunks<T>({d.a[0], d.b[0]}, {d.K, d.N}) ? gff_rows_kernel<T, true, false> : gff_rows_kernel<T, false, false>;
+  hipLaunchKernelGGL(down, dim3(tile_grid(mt, ceil_div(a->c_out, kGemmTile))), dim3(kGemmThreads), 0, s, d);
   return launch_status();
 }
 
@@ -286,16 +298,17 @@ template <typename T>
 int gff_backward(const cgtp_gff_args* a, hipStream_t s) {
   const int64_t mt = ceil_div(a->n_rows, kGemmTile);
   if (a->n_rows > 0 && (a->grad_x || a->grad_w_gate || a->grad_w_up)) {
-    MidGradArgs<T> m = {(const T*)a->grad_out, (const T*)a->w_down, (const T*)a->gate, (const T*)a->up, (T*)a->grad_gate,
-                        (T*)a->grad_up, a->n_rows, a->hidden, a->c_out, a->activation,
-                        whole_chunks<T>({a->grad_out, a->w_down}, {a->c_out})};
-    hipLaunchKernelGGL(gff_mid_grad_kernel<T>, dim3(tile_grid(mt, ceil_div(a->hidden, kGemmTile))), dim3(kGemmThreads), 0, s, m);
+    const MidGradArgs<T> m = {(const T*)a->grad_out, (const T*)a->w_down, (const T*)a->gate, (const T*)a->up, (T*)a->grad_gate,
+                              (T*)a->grad_up, a->n_rows, a->hidden, a->c_out, a->activation};
+    auto mid = whole_chunks<T>({m.gy, m.wd}, {m.C}) ? gff_mid_grad_kernel<T, true> : gff_mid_grad_kernel<T, false>;
+    hipLaunchKernelGGL(mid, dim3(tile_grid(mt, ceil_div(a->hidden, kGemmTile))), dim3(kGemmThreads), 0, s, m);
   }
   if (a->n_rows > 0 && a->grad_x) {
-    RowsArgs<T> d = {{(const T*)a->grad_gate, (const T*)a->grad_up}, {(const T*)a->w_gate, (const T*)a->w_up}, (T*)a->grad_x,
-                     a->n_rows, a->hidden, 2, a->hidden, a->c_in,
-                     whole_chunks<T>({a->grad_gate, a->grad_up, a->w_gate, a->w_up}, {a->hidden})};
-    hipLaunchKernelGGL((gff_rows_kernel<T, true>), dim3(tile_grid(mt, ceil_div(a->c_in, kGemmTile))), dim3(kGemmThreads), 0, s, d);
+    const RowsArgs<T> d = {{(const T*)a->grad_gate, (const T*)a->grad_up}, {(const T*)a->w_gate, (const T*)a->w_up},
+                           (T*)a->grad_x, a->n_rows, a->hidden, 2, a->hidden, a->c_in};
+    auto back = whole_chunks<T>({d.a[0], d.a[1], d.b[0], d.b[1]}, {d.K}) ? gff_rows_kernel<T, true, true>
+                                                                         : gff_rows_kernel<T, false, true>;
+    hipLaunchKernelGGL(back, dim3(tile_grid(mt, ceil_div(a->c_in, kGemmTile))), dim3(kGemmThreads), 0, s, d);
   }
   const WeightShape shape = weight_shape(a);
   WeightArgs<T> w = {};
@@ -312,9 +325,10 @@ int gff_backward(const cgtp_gff_args* a, hipStream_t s) {
   job(a->x, a->grad_gate, a->grad_w_gate, a->c_in, a->hidden);
   job(a->x, a->grad_up, a->grad_w_up, a->c_in, a->hidden);
   job(a->mid, a->grad_out, a->grad_w_down, a->hidden, a->c_out);
-  w.fast = whole_chunks<T>({a->x, a->grad_gate, a->grad_up, a->mid, a->grad_out}, {a->c_in, a->hidden, a->c_out});
   if (w.jobs) {
-    hipLaunchKernelGGL(gff_weight_kernel<T>, dim3(tile_grid(w.splits, w.tiles)), dim3(kGemmThreads), 0, s, w);
+    auto weight = whole_chunks<T>({a->x, a->grad_gate, a->grad_up, a->mid, a->grad_out}, {a->c_in, a->hidden, a->c_out})
+                      ? gff_weight_kernel<T, true> : gff_weight_kernel<T, false>;
+    hipLaunchKernelGGL(weight, dim3(tile_grid(w.splits, w.tiles)), dim3(kGemmThreads), 0, s, w);
     if (w.splits > 1)
       hipLaunchKernelGGL(gff_add_kernel<T>, dim3((unsigned)ceil_div(w.part_elems, 256)), dim3(256), 0, s, w);
   }
