@@ -1,5 +1,5 @@
 // Matrix products of the gated feed-forward block on the matrix cores: tiles of 128 x 128, four wavefronts of 64 x 64 each,
-// operands brought through registers into two LDS buffers, the next two tiles being loaded while one is worked on.
+// operands brought through registers into two LDS buffers, the next tile loaded while one is worked on.
 //
 // An operand is a matrix whose k or whose rows are contiguous.  In LDS a tile is 1024 chunks of 16 bytes either way:
 //   k contiguous    128 rows of eight chunks along k, chunk c of row r at place c ^ (r & 7);
@@ -133,50 +133,63 @@ struct GemmStage {
 
 // acc[i][j] of wavefront (wm, wn): rows 64 wm + 32 i of the first operand; of the second 64 wn + 32 j, or with SPLIT row 32 wn of
 // half j.  A lane holds row lane % 32 of the first and, at index 4 g + e, row 8 g + 4 (lane / 32) + e of the second.
-// a(t, k0, depth) / b(...): the operands of tile t, and where its k begin and end; tiles: the same for all threads.
-template <typename T, bool FAST, bool KA, bool KB, bool SPLIT, typename A, typename B>
-__device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[2][2], char* lds, int64_t tiles, A&& a, B&& b) {
+//
+// A workgroup works through `results` results of `tiles` tiles of k each, one after the other: the first tile of the next is on
+// its way while done(i) finishes result i.  a(i, t, k0, depth) / b(i, t): the operands of tile t of result i, and where its k
+// begin and end.  All counts are the same for all threads.
+template <typename T, bool FAST, bool KA, bool KB, bool SPLIT, typename A, typename B, typename Done>
+__device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[2][2], char* lds, int results, int64_t tiles, A&& a, B&& b, Done&& done) {
   const int wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
+  auto clear = [&]() {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  if (tiles <= 0) return;
-  GemmStage<T, KA> sa[2];
-  GemmStage<T, KB> sb[2];
-  auto fetch = [&](int which, int64_t t) {
-    int64_t k0, depth;
-    const GemmOperand<T> pa = a(t, k0, depth), pb = b(t);
-    sa[which].template load<FAST>(pa, k0, depth);
-    sb[which].template load<FAST>(pb, k0, depth);
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   };
-  auto step = [&](int which, int64_t t) {
-    char* la = lds + which * 2 * kGemmTileBytes;
-    char* lb = la + kGemmTileBytes;
-    sa[which].store(la);
-    sb[which].store(lb);
-    __syncthreads();
-    if (t + 2 < tiles) fetch(which, t + 2);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      u32x4_t fa[2], fb[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) fa[i] = GemmStage<T, KA>::frag(la, 2 * wm + i, s);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) fb[j] = GemmStage<T, KB>::frag(lb, SPLIT ? 2 * j + wn : 2 * wn + j, s);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) mma_chunk<T>(acc[i][j], fb[j], fa[i]);
-    }
+  clear();
+  if (tiles <= 0) {
+    for (int i = 0; i < results; ++i) done(i);
+    return;
+  }
+  GemmStage<T, KA> sa;
+  GemmStage<T, KB> sb;
+  auto fetch = [&](int i, int64_t t) {
+    int64_t k0, depth;
+    const GemmOperand<T> pa = a(i, t, k0, depth), pb = b(i, t);
+    sa.template load<FAST>(pa, k0, depth);
+    sb.template load<FAST>(pb, k0, depth);
   };
   fetch(0, 0);
-  if (tiles > 1) fetch(1, 1);
-  for (int64_t t = 0; t < tiles; t += 2) {
-    step(0, t);
-    if (t + 1 < tiles) step(1, t + 1);
+  int which = 0;
+  for (int i = 0; i < results; ++i) {
+    for (int64_t t = 0; t < tiles; ++t, which ^= 1) {
+      char* la = lds + which * 2 * kGemmTileBytes;
+      char* lb = la + kGemmTileBytes;
+      sa.store(la);
+      sb.store(lb);
+      __syncthreads();
+      if (t + 1 < tiles) fetch(i, t + 1);
+      else if (i + 1 < results) fetch(i + 1, 0);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        u32x4_t fa[2], fb[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) fa[i] = GemmStage<T, KA>::frag(la, 2 * wm + i, s);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) fb[j] = GemmStage<T, KB>::frag(lb, SPLIT ? 2 * j + wn : 2 * wn + j, s);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mma_chunk<T>(acc[i][j], fb[j], fa[i]);
+      }
+    }
+    done(i);
+    if (i + 1 < results) {
+      clear();
+      __syncthreads();         // done() has used the buffers
+    }
   }
 }
 

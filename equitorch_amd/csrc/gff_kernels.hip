@@ -46,20 +46,23 @@ __device__ __forceinline__ float gff_act_grad(int act, float g, float& value) {
 }
 
 // Workgroups go to the eight XCDs in turn: the tiles of one outer index (which share a panel of an operand) are given to
-// one XCD, whose L2 then reads the panel once.
-struct TilePlace { int64_t outer; int inner; };
-__device__ __forceinline__ TilePlace tile_place(int inner_tiles) {
+// one XCD, whose L2 then reads the panel once.  A workgroup takes `each` inner tiles, one after the other.
+struct TilePlace { int64_t outer; int inner, count; };
+__device__ __forceinline__ TilePlace tile_place(int inner_tiles, int each) {
   const int64_t id = (int64_t)blockIdx.x >> 3;
-  return {id / inner_tiles * 8 + (blockIdx.x & 7), (int)(id % inner_tiles)};
+  const int groups = (inner_tiles + each - 1) / each, first = (int)(id % groups) * each;
+  return {id / groups * 8 + (blockIdx.x & 7), first, std::min(each, inner_tiles - first)};
 }
-unsigned tile_grid(int64_t outer, int64_t inner) { return (unsigned)((outer + 7) / 8 * 8 * inner); }
+unsigned tile_grid(int64_t outer, int64_t inner, int each) { return (unsigned)((outer + 7) / 8 * 8 * ((inner + each - 1) / each)); }
+// Four workgroups for each compute unit, as far as there are tiles.
+int tiles_each(int64_t outer, int64_t inner) { return (int)std::max<int64_t>(1, std::min<int64_t>(inner, outer * inner / 1024)); }
 
 template <typename T>
 struct UpArgs {
   const T *x, *wg, *wu;
   T *gate, *up, *mid;            // gate and up may be null (inference)
   int64_t n_rows;
-  int C, H, act;
+  int C, H, act, each;
 };
 
 __device__ __forceinline__ int rows_left(int64_t n, int64_t from) { return (int)(n - from < kGemmTile ? n - from : kGemmTile); }
@@ -69,30 +72,33 @@ template <typename T, bool FAST>
 __global__ void __launch_bounds__(kGemmThreads, 2) gff_up_kernel(UpArgs<T> a) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place((a.H + 63) / 64);
+  const TilePlace at = tile_place((a.H + 63) / 64, a.each);
   const int64_t m0 = at.outer * kGemmTile;
   if (m0 >= a.n_rows) return;
-  const int h0 = at.inner * 64;
   const GemmOperand<T> x = {{a.x + m0 * a.C, nullptr}, a.C, {rows_left(a.n_rows, m0), 0}};
-  const GemmOperand<T> w = {{a.wg + h0, a.wu + h0}, a.H, {a.H - h0, a.H - h0}};
   f32x16_t acc[2][2];
-  gemm_loop<T, FAST, true, false, true>(acc, lds, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, true, false, true>(acc, lds, at.count, (a.C + D - 1) / D, [&](int, int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = a.C;
     return x;
-  }, [&](int64_t) { return w; });
-  gemm_results<true, 4>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&g)[8], const float (&u)[8]) {
-    const int left = a.H - h0 - c;
-    if (r >= x.rows[0] || left <= 0) return;
-    const int64_t to = (m0 + r) * a.H + h0 + c;
-    float m[8];
+  }, [&](int i, int64_t) {
+    const int h0 = (at.inner + i) * 64;
+    return GemmOperand<T>{{a.wg + h0, a.wu + h0}, a.H, {a.H - h0, a.H - h0}};
+  }, [&](int i) {
+    const int h0 = (at.inner + i) * 64;
+    gemm_results<true, 4>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&g)[8], const float (&u)[8]) {
+      const int left = a.H - h0 - c;
+      if (r >= x.rows[0] || left <= 0) return;
+      const int64_t to = (m0 + r) * a.H + h0 + c;
+      float m[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m[e] = gff_act<T>(a.act, g[e]) * u[e];
-    store_eight(a.mid + to, m, left);
-    if (a.gate) {
-      store_eight(a.gate + to, g, left);
-      store_eight(a.up + to, u, left);
-    }
+      for (int e = 0; e < 8; ++e) m[e] = gff_act<T>(a.act, g[e]) * u[e];
+      store_eight(a.mid + to, m, left);
+      if (a.gate) {
+        store_eight(a.gate + to, g, left);
+        store_eight(a.up + to, u, left);
+      }
+    });
   });
 }
 
@@ -101,7 +107,7 @@ struct MidGradArgs {
   const T *gy, *wd, *gate, *up;
   T *g_gate, *g_up;
   int64_t n_rows;
-  int H, C, act;
+  int H, C, act, each;
 };
 
 // dg and du from dm = dy Wd^T.
@@ -109,44 +115,47 @@ template <typename T, bool FAST>
 __global__ void __launch_bounds__(kGemmThreads, 2) gff_mid_grad_kernel(MidGradArgs<T> a) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place((a.H + kGemmTile - 1) / kGemmTile);
+  const TilePlace at = tile_place((a.H + kGemmTile - 1) / kGemmTile, a.each);
   const int64_t m0 = at.outer * kGemmTile;
   if (m0 >= a.n_rows) return;
-  const int h0 = at.inner * kGemmTile;
   const GemmOperand<T> gy = {{a.gy + m0 * a.C, nullptr}, a.C, {rows_left(a.n_rows, m0), 0}};
-  const GemmOperand<T> wd = {{a.wd + (int64_t)h0 * a.C, nullptr}, a.C, {rows_left(a.H, h0), 0}};
   f32x16_t acc[2][2];
-  gemm_loop<T, FAST, true, true, false>(acc, lds, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, true, true, false>(acc, lds, at.count, (a.C + D - 1) / D, [&](int, int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = a.C;
     return gy;
-  }, [&](int64_t) { return wd; });
-  // The projections' part is fetched a few places ahead of its use: one wait for memory in place of one for each place.
-  constexpr int kAhead = sizeof(T) == 2 ? 8 : 4;
-  EightRaw<T> pg[kAhead], pu[kAhead];
-  auto fetch = [&](int i, int r, int c) {
-    const int left = a.H - h0 - c;
-    if (r >= gy.rows[0] || left <= 0) return;
-    const int64_t at = (m0 + r) * a.H + h0 + c;
-    pg[i % kAhead].load(a.gate + at, left);
-    pu[i % kAhead].load(a.up + at, left);
-  };
-  gemm_results<false, kAhead>(acc, lds, fetch, [&](int i, int r, int c, const float (&dm)[8]) {
-    const int left = a.H - h0 - c;
-    if (r >= gy.rows[0] || left <= 0) return;
-    const int64_t to = (m0 + r) * a.H + h0 + c;
-    float g[8], u[8];
-    pg[i % kAhead].get(g);
-    pu[i % kAhead].get(u);
+  }, [&](int i, int64_t) {
+    const int h0 = (at.inner + i) * kGemmTile;
+    return GemmOperand<T>{{a.wd + (int64_t)h0 * a.C, nullptr}, a.C, {rows_left(a.H, h0), 0}};
+  }, [&](int i) {
+    // The projections' part is fetched a few places ahead of its use: one wait for memory in place of one for each place.
+    constexpr int kAhead = sizeof(T) == 2 ? 8 : 4;
+    EightRaw<T> pg[kAhead], pu[kAhead];
+    const int h0 = (at.inner + i) * kGemmTile;
+    auto fetch = [&](int p, int r, int c) {
+      const int left = a.H - h0 - c;
+      if (r >= gy.rows[0] || left <= 0) return;
+      const int64_t from = (m0 + r) * a.H + h0 + c;
+      pg[p % kAhead].load(a.gate + from, left);
+      pu[p % kAhead].load(a.up + from, left);
+    };
+    gemm_results<false, kAhead>(acc, lds, fetch, [&](int p, int r, int c, const float (&dm)[8]) {
+      const int left = a.H - h0 - c;
+      if (r >= gy.rows[0] || left <= 0) return;
+      const int64_t to = (m0 + r) * a.H + h0 + c;
+      float g[8], u[8];
+      pg[p % kAhead].get(g);
+      pu[p % kAhead].get(u);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float value;
-      const float slope = gff_act_grad<T>(a.act, g[e], value);
-      g[e] = dm[e] * u[e] * slope;
-      u[e] = dm[e] * value;
-    }
-    store_eight(a.g_gate + to, g, left);
-    store_eight(a.g_up + to, u, left);
+      for (int e = 0; e < 8; ++e) {
+        float value;
+        const float slope = gff_act_grad<T>(a.act, g[e], value);
+        g[e] = dm[e] * u[e] * slope;
+        u[e] = dm[e] * value;
+      }
+      store_eight(a.g_gate + to, g, left);
+      store_eight(a.g_up + to, u, left);
+    });
   });
 }
 
@@ -156,29 +165,33 @@ struct RowsArgs {
   const T *a[2], *b[2];
   T* out;
   int64_t n_rows, ldb;
-  int segments, K, N;      // K: per segment
+  int segments, K, N, each;      // K: per segment
 };
 template <typename T, bool FAST, bool KB>
 __global__ void __launch_bounds__(kGemmThreads, 2) gff_rows_kernel(RowsArgs<T> a) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place((a.N + kGemmTile - 1) / kGemmTile);
+  const TilePlace at = tile_place((a.N + kGemmTile - 1) / kGemmTile, a.each);
   const int64_t m0 = at.outer * kGemmTile;
   if (m0 >= a.n_rows) return;
-  const int n0 = at.inner * kGemmTile, tiles = (a.K + D - 1) / D, rows = rows_left(a.n_rows, m0), cols = rows_left(a.N, n0);
+  const int tiles = (a.K + D - 1) / D, rows = rows_left(a.n_rows, m0);
   f32x16_t acc[2][2];
-  gemm_loop<T, FAST, true, KB, false>(acc, lds, (int64_t)tiles * a.segments, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, true, KB, false>(acc, lds, at.count, (int64_t)tiles * a.segments,
+                                      [&](int, int64_t t, int64_t& k0, int64_t& depth) {
     k0 = (t < tiles ? t : t - tiles) * D;
     depth = a.K;
     return GemmOperand<T>{{(t < tiles ? a.a[0] : a.a[1]) + m0 * a.K, nullptr}, a.K, {rows, 0}};
-  }, [&](int64_t t) {
+  }, [&](int i, int64_t t) {
     const T* b = t < tiles ? a.b[0] : a.b[1];
+    const int n0 = (at.inner + i) * kGemmTile, cols = rows_left(a.N, n0);
     if (KB) return GemmOperand<T>{{b + n0 * a.ldb, nullptr}, a.ldb, {cols, 0}};
     return GemmOperand<T>{{b + n0, b + n0 + 64}, a.ldb, {cols, cols - 64}};
-  });
-  gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
-    const int left = a.N - n0 - c;
-    if (r < rows && left > 0) store_eight(a.out + (m0 + r) * a.N + n0 + c, v, left);
+  }, [&](int i) {
+    const int n0 = (at.inner + i) * kGemmTile;
+    gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
+      const int left = a.N - n0 - c;
+      if (r < rows && left > 0) store_eight(a.out + (m0 + r) * a.N + n0 + c, v, left);
+    });
   });
 }
 
@@ -202,7 +215,7 @@ template <typename T, bool FAST>
 __global__ void __launch_bounds__(kGemmThreads, 2) gff_weight_kernel(WeightArgs<T> w) {
   __shared__ alignas(16) char lds[4 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place(w.tiles);
+  const TilePlace at = tile_place(w.tiles, 1);
   if (at.outer >= w.splits) return;
   const int which = w.jobs > 2 && at.inner >= w.job[2].first_tile ? 2 : w.jobs > 1 && at.inner >= w.job[1].first_tile ? 1 : 0;
   const WeightJob<T> job = w.job[which];
@@ -214,17 +227,18 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gff_weight_kernel(WeightArgs<
   const T *ja = job.a + r0 * job.M + m0, *jb = job.b + r0 * job.N + n0;
   const GemmOperand<T> pa = {{ja, ja + 64}, job.M, {rows, rows - 64}}, pb = {{jb, jb + 64}, job.N, {cols, cols - 64}};
   f32x16_t acc[2][2];
-  gemm_loop<T, FAST, false, false, false>(acc, lds, (end + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, false, false, false>(acc, lds, 1, (end + D - 1) / D, [&](int, int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = end;
     return pa;
-  }, [&](int64_t) { return pb; });
-  gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
-    const int left = job.N - n0 - c;
-    if (r >= rows || left <= 0) return;
-    const int64_t to = (int64_t)(m0 + r) * job.N + n0 + c;
-    if (w.splits > 1) store_eight(w.parts + at.outer * w.part_elems + job.first_part + to, v, left);
-    else store_eight(job.out + to, v, left);
+  }, [&](int, int64_t) { return pb; }, [&](int) {
+    gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
+      const int left = job.N - n0 - c;
+      if (r >= rows || left <= 0) return;
+      const int64_t to = (int64_t)(m0 + r) * job.N + n0 + c;
+      if (w.splits > 1) store_eight(w.parts + at.outer * w.part_elems + job.first_part + to, v, left);
+      else store_eight(job.out + to, v, left);
+    });
   });
 }
 template <typename T>
@@ -265,7 +279,7 @@ bool whole_chunks(std::initializer_list<const void*> ptrs, std::initializer_list
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Ranges the rows are cut into for the weight gradients: two workgroups for each compute unit, at least eight k tiles each.
+// Ranges the rows are cut into for the weight gradients: three workgroups for each compute unit, at least eight k tiles each.
 struct WeightShape { int splits; int64_t rows_per_split, part_elems; int tiles; };
 WeightShape weight_shape(const cgtp_gff_args* a) {
   WeightShape s;
@@ -273,8 +287,9 @@ WeightShape weight_shape(const cgtp_gff_args* a) {
   s.tiles = (int)(th * (2 * ti + to));
   s.part_elems = (int64_t)a->hidden * (2 * a->c_in + a->c_out);
   const int depth = a->dtype == CGTP_F32 ? 32 : 64;
-  int64_t splits = std::max<int64_t>(1, 512 / s.tiles);
+  int64_t splits = std::max<int64_t>(1, 768 / s.tiles);
   splits = std::max<int64_t>(1, std::min(splits, ceil_div(a->n_rows, 8 * depth)));
+  if (splits > 8) splits = splits / 8 * 8;           // a range's tiles run on one XCD: as many ranges for each of the eight
   s.rows_per_split = ceil_div(ceil_div(a->n_rows, splits), depth) * depth;
   s.splits = (int)std::max<int64_t>(1, ceil_div(a->n_rows, std::max<int64_t>(1, s.rows_per_split)));
   return s;
@@ -284,13 +299,13 @@ template <typename T>
 int gff_forward(const cgtp_gff_args* a, hipStream_t s) {
   const int64_t mt = ceil_div(a->n_rows, kGemmTile);
   const UpArgs<T> u = {(const T*)a->x, (const T*)a->w_gate, (const T*)a->w_up, (T*)a->gate, (T*)a->up, (T*)a->mid, a->n_rows,
-                       a->c_in, a->hidden, a->activation};
+                       a->c_in, a->hidden, a->activation, tiles_each(mt, ceil_div(a->hidden, 64))};
   auto up = whole_chunks<T>({u.x, u.wg, u.wu}, {u.C, u.H}) ? gff_up_kernel<T, true> : gff_up_kernel<T, false>;
-  hipLaunchKernelGGL(up, dim3(tile_grid(mt, ceil_div(a->hidden, 64))), dim3(kGemmThreads), 0, s, u);
+  hipLaunchKernelGGL(up, dim3(tile_grid(mt, ceil_div(a->hidden, 64), u.each)), dim3(kGemmThreads), 0, s, u);
   const RowsArgs<T> d = {{(const T*)a->mid, nullptr}, {(const T*)a->w_down, nullptr}, (T*)a->out, a->n_rows, a->c_out, 1, a->hidden,
-                         a->c_out};
+                         a->c_out, tiles_each(mt, ceil_div(a->c_out, kGemmTile))};
   auto down = whole_chunks<T>({d.a[0], d.b[0]}, {d.K, d.N}) ? gff_rows_kernel<T, true, false> : gff_rows_kernel<T, false, false>;
-  hipLaunchKernelGGL(down, dim3(tile_grid(mt, ceil_div(a->c_out, kGemmTile))), dim3(kGemmThreads), 0, s, d);
+  hipLaunchKernelGGL(down, dim3(tile_grid(mt, ceil_div(a->c_out, kGemmTile), d.each)), dim3(kGemmThreads), 0, s, d);
   return launch_status();
 }
 
@@ -299,16 +314,18 @@ int gff_backward(const cgtp_gff_args* a, hipStream_t s) {
   const int64_t mt = ceil_div(a->n_rows, kGemmTile);
   if (a->n_rows > 0 && (a->grad_x || a->grad_w_gate || a->grad_w_up)) {
     const MidGradArgs<T> m = {(const T*)a->grad_out, (const T*)a->w_down, (const T*)a->gate, (const T*)a->up, (T*)a->grad_gate,
-                              (T*)a->grad_up, a->n_rows, a->hidden, a->c_out, a->activation};
+                              (T*)a->grad_up, a->n_rows, a->hidden, a->c_out, a->activation,
+                              tiles_each(mt, ceil_div(a->hidden, kGemmTile))};
     auto mid = whole_chunks<T>({m.gy, m.wd}, {m.C}) ? gff_mid_grad_kernel<T, true> : gff_mid_grad_kernel<T, false>;
-    hipLaunchKernelGGL(mid, dim3(tile_grid(mt, ceil_div(a->hidden, kGemmTile))), dim3(kGemmThreads), 0, s, m);
+    hipLaunchKernelGGL(mid, dim3(tile_grid(mt, ceil_div(a->hidden, kGemmTile), m.each)), dim3(kGemmThreads), 0, s, m);
   }
   if (a->n_rows > 0 && a->grad_x) {
     const RowsArgs<T> d = {{(const T*)a->grad_gate, (const T*)a->grad_up}, {(const T*)a->w_gate, (const T*)a->w_up},
-                           (T*)a->grad_x, a->n_rows, a->hidden, 2, a->hidden, a->c_in};
+                           (T*)a->grad_x, a->n_rows, a->hidden, 2, a->hidden, a->c_in,
+                           tiles_each(mt, ceil_div(a->c_in, kGemmTile))};
     auto back = whole_chunks<T>({d.a[0], d.a[1], d.b[0], d.b[1]}, {d.K}) ? gff_rows_kernel<T, true, true>
                                                                          : gff_rows_kernel<T, false, true>;
-    hipLaunchKernelGGL(back, dim3(tile_grid(mt, ceil_div(a->c_in, kGemmTile))), dim3(kGemmThreads), 0, s, d);
+    hipLaunchKernelGGL(back, dim3(tile_grid(mt, ceil_div(a->c_in, kGemmTile), d.each)), dim3(kGemmThreads), 0, s, d);
   }
   const WeightShape shape = weight_shape(a);
   WeightArgs<T> w = {};
@@ -328,7 +345,7 @@ int gff_backward(const cgtp_gff_args* a, hipStream_t s) {
   if (w.jobs) {
     auto weight = whole_chunks<T>({a->x, a->grad_gate, a->grad_up, a->mid, a->grad_out}, {a->c_in, a->hidden, a->c_out})
                       ? gff_weight_kernel<T, true> : gff_weight_kernel<T, false>;
-    hipLaunchKernelGGL(weight, dim3(tile_grid(w.splits, w.tiles)), dim3(kGemmThreads), 0, s, w);
+    hipLaunchKernelGGL(weight, dim3(tile_grid(w.splits, w.tiles, 1)), dim3(kGemmThreads), 0, s, w);
     if (w.splits > 1)
       hipLaunchKernelGGL(gff_add_kernel<T>, dim3((unsigned)ceil_div(w.part_elems, 256)), dim3(256), 0, s, w);
   }
