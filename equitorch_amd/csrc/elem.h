@@ -43,15 +43,16 @@ typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
-// N elements of T from an address aligned to an element only, the ones from `valid` (at least 1) on as zeros.  Vector loads
-// from such addresses are what the hardware does by itself; only a vector that crosses the end is taken apart.
-template <typename T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) Loose { T v[N]; };
+// Vectors at an address aligned to an element only: the hardware reads and writes such by itself.  Their type is an integer
+// vector on purpose: taken as elements, the compiler splits the access.
+template <typename T, typename R> struct LooseOf { typedef R type __attribute__((aligned(sizeof(T)))); };
 
+// N = sizeof(R) / sizeof(T) elements, the ones from `valid` (at least 1) on as zeros.  Only a vector that crosses the end is
+// taken apart.
 template <typename R, typename T>
 __device__ __forceinline__ R load_part(const T* p, int64_t valid) {
   constexpr int N = sizeof(R) / sizeof(T);
-  if (valid >= N) return __builtin_bit_cast(R, *reinterpret_cast<const Loose<T, N>*>(p));
+  if (valid >= N) return *reinterpret_cast<const typename LooseOf<T, R>::type*>(p);
   T e[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -62,14 +63,14 @@ __device__ __forceinline__ R load_part(const T* p, int64_t valid) {
   __builtin_memcpy(&r, e, sizeof(R));
   return r;
 }
-// The first `valid` of N elements to an address aligned to an element only.
+// The first `valid` of N elements.
 template <typename T, int N>
 __device__ __forceinline__ void store_part(T* p, const T (&e)[N], int64_t valid) {
+  typedef unsigned raw_t __attribute__((ext_vector_type(N * sizeof(T) / 4)));
   if (valid >= N) {
-    Loose<T, N> v;
-#pragma unroll
-    for (int i = 0; i < N; ++i) v.v[i] = e[i];
-    *reinterpret_cast<Loose<T, N>*>(p) = v;
+    raw_t r;
+    __builtin_memcpy(&r, e, sizeof(r));
+    *reinterpret_cast<typename LooseOf<T, raw_t>::type*>(p) = r;
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)

@@ -1,5 +1,5 @@
 // Matrix products of the gated feed-forward block on the matrix cores: tiles of 128 x 128, four wavefronts of 64 x 64 each,
-// operands brought through registers into two LDS buffers, the next tile loaded while one is worked on.
+// operands brought through registers into one LDS buffer, the next tile loaded while one is worked on.
 //
 // An operand is a matrix whose k or whose rows are contiguous.  In LDS a tile is 1024 chunks of 16 bytes either way:
 //   k contiguous    128 rows of eight chunks along k, chunk c of row r at place c ^ (r & 7);
@@ -133,62 +133,45 @@ struct GemmStage {
 
 // acc[i][j] of wavefront (wm, wn): rows 64 wm + 32 i of the first operand; of the second 64 wn + 32 j, or with SPLIT row 32 wn of
 // half j.  A lane holds row lane % 32 of the first and, at index 4 g + e, row 8 g + 4 (lane / 32) + e of the second.
-//
-// A workgroup works through `results` results of `tiles` tiles of k each, one after the other: the first tile of the next is on
-// its way while done(i) finishes result i.  a(i, t, k0, depth) / b(i, t): the operands of tile t of result i, and where its k
-// begin and end.  All counts are the same for all threads.
-template <typename T, bool FAST, bool KA, bool KB, bool SPLIT, typename A, typename B, typename Done>
-__device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[2][2], char* lds, int results, int64_t tiles, A&& a, B&& b, Done&& done) {
+// a(t, k0, depth) / b(t): the operands of tile t of k, and where its k begin and end; tiles: the same for all threads.
+template <typename T, bool FAST, bool KA, bool KB, bool SPLIT, typename A, typename B>
+__device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[2][2], char* lds, int64_t tiles, A&& a, B&& b) {
   const int wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
-  auto clear = [&]() {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  };
-  clear();
-  if (tiles <= 0) {
-    for (int i = 0; i < results; ++i) done(i);
-    return;
-  }
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  if (tiles <= 0) return;
   GemmStage<T, KA> sa;
   GemmStage<T, KB> sb;
-  auto fetch = [&](int i, int64_t t) {
+  auto fetch = [&](int64_t t) {
     int64_t k0, depth;
-    const GemmOperand<T> pa = a(i, t, k0, depth), pb = b(i, t);
+    const GemmOperand<T> pa = a(t, k0, depth), pb = b(t);
     sa.template load<FAST>(pa, k0, depth);
     sb.template load<FAST>(pb, k0, depth);
   };
-  fetch(0, 0);
-  int which = 0;
-  for (int i = 0; i < results; ++i) {
-    for (int64_t t = 0; t < tiles; ++t, which ^= 1) {
-      char* la = lds + which * 2 * kGemmTileBytes;
-      char* lb = la + kGemmTileBytes;
-      sa.store(la);
-      sb.store(lb);
-      __syncthreads();
-      if (t + 1 < tiles) fetch(i, t + 1);
-      else if (i + 1 < results) fetch(i + 1, 0);
+  fetch(0);
+  char* la = lds;
+  char* lb = lds + kGemmTileBytes;
+  for (int64_t t = 0; t < tiles; ++t) {
+    if (t) __syncthreads();         // the tile before has used the buffer
+    sa.store(la);
+    sb.store(lb);
+    __syncthreads();
+    if (t + 1 < tiles) fetch(t + 1);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        u32x4_t fa[2], fb[2];
+    for (int s = 0; s < 4; ++s) {
+      u32x4_t fa[2], fb[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) fa[i] = GemmStage<T, KA>::frag(la, 2 * wm + i, s);
+      for (int i = 0; i < 2; ++i) fa[i] = GemmStage<T, KA>::frag(la, 2 * wm + i, s);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) fb[j] = GemmStage<T, KB>::frag(lb, SPLIT ? 2 * j + wn : 2 * wn + j, s);
+      for (int j = 0; j < 2; ++j) fb[j] = GemmStage<T, KB>::frag(lb, SPLIT ? 2 * j + wn : 2 * wn + j, s);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) mma_chunk<T>(acc[i][j], fb[j], fa[i]);
-      }
-    }
-    done(i);
-    if (i + 1 < results) {
-      clear();
-      __syncthreads();         // done() has used the buffers
+        for (int j = 0; j < 2; ++j) mma_chunk<T>(acc[i][j], fb[j], fa[i]);
     }
   }
 }
@@ -224,9 +207,10 @@ template <bool SPLIT, int AHEAD, typename Fetch, typename Use>
 __device__ __forceinline__ void gemm_results(const f32x16_t (&acc)[2][2], char* lds, Fetch&& fetch, Use&& use) {
   constexpr int kRow = SPLIT ? 8 : 16, kPlaces = SPLIT ? 4 : 8;
   auto place = [&](int i, int& r, int& c) {
-    const int id = i * kGemmThreads + (int)threadIdx.x;
-    r = id / kRow;
+    const int id = i % (kPlaces / 2) * kGemmThreads + (int)threadIdx.x, at = id / kRow;     // row of the buffer
+    r = (at >> 5) * 64 + (i / (kPlaces / 2)) * 32 + (at & 31);
     c = id % kRow * 8;
+    return at;
   };
   auto ahead = [&](int i) {
     int r, c;
@@ -236,41 +220,43 @@ __device__ __forceinline__ void gemm_results(const f32x16_t (&acc)[2][2], char* 
 #pragma unroll
   for (int i = 0; i < AHEAD && i < kPlaces; ++i) ahead(i);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
-  float* tile = reinterpret_cast<float*>(lds);           // 128 rows of 32 chunks, chunk c of row r at c ^ (r & 31)
+  float* tile = reinterpret_cast<float*>(lds);           // 64 rows of 32 chunks, chunk c of row r at c ^ (r & 31)
   auto chunk = [&](int r, int c) { return reinterpret_cast<f32x4*>(tile + r * 128 + ((c ^ (r & 31)) << 2)); };
-  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int part = 0; part < 2; ++part) {                 // rows 32 part .. + 31 of both halves
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int r = 64 * wm + 32 * i + (lane & 31), n = (SPLIT ? 64 * j + 32 * wn : 64 * wn + 32 * j) + 8 * g + 4 * (lane >> 5);
+        const int n = (SPLIT ? 64 * j + 32 * wn : 64 * wn + 32 * j) + 8 * g + 4 * (lane >> 5);
         f32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
-        *chunk(r, n >> 2) = v;
+        for (int e = 0; e < 4; ++e) v[e] = acc[part][j][4 * g + e];
+        *chunk(32 * wm + (lane & 31), n >> 2) = v;
       }
-  __syncthreads();
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kPlaces; ++i) {
-    int r, c;
-    place(i, r, c);
-    float v[8];
-    auto take = [&](int first, float (&to)[8]) {
-      const f32x4 x = *chunk(r, first), y = *chunk(r, first + 1);
+    for (int p = 0; p < kPlaces / 2; ++p) {
+      const int i = part * (kPlaces / 2) + p;
+      int r, c;
+      const int at = place(i, r, c);
+      float v[8];
+      auto take = [&](int first, float (&to)[8]) {
+        const f32x4 x = *chunk(at, first), y = *chunk(at, first + 1);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { to[e] = x[e]; to[4 + e] = y[e]; }
-    };
-    take(c / 4, v);
-    if constexpr (SPLIT) {
-      float u[8];
-      take(16 + c / 4, u);
-      use(i, r, c, v, u);
-    } else {
-      use(i, r, c, v);
+        for (int e = 0; e < 4; ++e) { to[e] = x[e]; to[4 + e] = y[e]; }
+      };
+      take(c / 4, v);
+      if constexpr (SPLIT) {
+        float u[8];
+        take(16 + c / 4, u);
+        use(i, r, c, v, u);
+      } else {
+        use(i, r, c, v);
+      }
+      if (i + AHEAD < kPlaces) ahead(i + AHEAD);
     }
-    if (i + AHEAD < kPlaces) ahead(i + AHEAD);
   }
 }
 

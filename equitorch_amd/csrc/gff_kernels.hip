@@ -9,7 +9,7 @@
 #include "gff_gemm.h"
 
 #include <algorithm>
-#include <initializer_list>
+#include <type_traits>
 
 namespace cgtp {
 namespace {
@@ -23,21 +23,21 @@ __device__ __forceinline__ float gff_sigmoid(float g) {
   if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.f + __expf(-g));
   else return 1.f / (1.f + expf(-g));
 }
-template <typename T>
-__device__ __forceinline__ float gff_act(int act, float g) {
-  if (act == CGTP_ACT_GELU) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+template <typename T, int act>
+__device__ __forceinline__ float gff_act(float g) {
+  if constexpr (act == CGTP_ACT_GELU) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
   const float s = gff_sigmoid<T>(g);
   return act == CGTP_ACT_SILU ? g * s : s;
 }
-template <typename T>
-__device__ __forceinline__ float gff_act_grad(int act, float g, float& value) {
-  if (act == CGTP_ACT_GELU) {
+template <typename T, int act>
+__device__ __forceinline__ float gff_act_grad(float g, float& value) {
+  if constexpr (act == CGTP_ACT_GELU) {
     const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
     value = g * cdf;
     return cdf + g * 0.3989422804014327f * expf(-0.5f * g * g);
   }
   const float s = gff_sigmoid<T>(g);
-  if (act == CGTP_ACT_SILU) {
+  if constexpr (act == CGTP_ACT_SILU) {
     value = g * s;
     return s + value * (1.f - s);
   }
@@ -46,59 +46,53 @@ __device__ __forceinline__ float gff_act_grad(int act, float g, float& value) {
 }
 
 // Workgroups go to the eight XCDs in turn: the tiles of one outer index (which share a panel of an operand) are given to
-// one XCD, whose L2 then reads the panel once.  A workgroup takes `each` inner tiles, one after the other.
-struct TilePlace { int64_t outer; int inner, count; };
-__device__ __forceinline__ TilePlace tile_place(int inner_tiles, int each) {
+// one XCD, whose L2 then reads the panel once.
+struct TilePlace { int64_t outer; int inner; };
+__device__ __forceinline__ TilePlace tile_place(int inner_tiles) {
   const int64_t id = (int64_t)blockIdx.x >> 3;
-  const int groups = (inner_tiles + each - 1) / each, first = (int)(id % groups) * each;
-  return {id / groups * 8 + (blockIdx.x & 7), first, std::min(each, inner_tiles - first)};
+  return {id / inner_tiles * 8 + (blockIdx.x & 7), (int)(id % inner_tiles)};
 }
-unsigned tile_grid(int64_t outer, int64_t inner, int each) { return (unsigned)((outer + 7) / 8 * 8 * ((inner + each - 1) / each)); }
-// Four workgroups for each compute unit, as far as there are tiles.
-int tiles_each(int64_t outer, int64_t inner) { return (int)std::max<int64_t>(1, std::min<int64_t>(inner, outer * inner / 1024)); }
+unsigned tile_grid(int64_t outer, int64_t inner) { return (unsigned)((outer + 7) / 8 * 8 * inner); }
 
 template <typename T>
 struct UpArgs {
   const T *x, *wg, *wu;
   T *gate, *up, *mid;            // gate and up may be null (inference)
   int64_t n_rows;
-  int C, H, act, each;
+  int C, H;
 };
 
 __device__ __forceinline__ int rows_left(int64_t n, int64_t from) { return (int)(n - from < kGemmTile ? n - from : kGemmTile); }
 
 // g, u and m.  A tile is 128 rows x 64 hidden channels, of Wg and of Wu.
-template <typename T, bool FAST>
-__global__ void __launch_bounds__(kGemmThreads, 2) gff_up_kernel(UpArgs<T> a) {
-  __shared__ alignas(16) char lds[4 * kGemmTileBytes];
+template <typename T, bool FAST, int ACT>
+__global__ void __launch_bounds__(kGemmThreads, 3) gff_up_kernel(UpArgs<T> a) {
+  __shared__ alignas(16) char lds[2 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place((a.H + 63) / 64, a.each);
+  const TilePlace at = tile_place((a.H + 63) / 64);
   const int64_t m0 = at.outer * kGemmTile;
   if (m0 >= a.n_rows) return;
+  const int h0 = at.inner * 64;
+  const GemmOperand<T> w = {{a.wg + h0, a.wu + h0}, a.H, {a.H - h0, a.H - h0}};
   const GemmOperand<T> x = {{a.x + m0 * a.C, nullptr}, a.C, {rows_left(a.n_rows, m0), 0}};
   f32x16_t acc[2][2];
-  gemm_loop<T, FAST, true, false, true>(acc, lds, at.count, (a.C + D - 1) / D, [&](int, int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, true, false, true>(acc, lds, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = a.C;
     return x;
-  }, [&](int i, int64_t) {
-    const int h0 = (at.inner + i) * 64;
-    return GemmOperand<T>{{a.wg + h0, a.wu + h0}, a.H, {a.H - h0, a.H - h0}};
-  }, [&](int i) {
-    const int h0 = (at.inner + i) * 64;
-    gemm_results<true, 4>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&g)[8], const float (&u)[8]) {
-      const int left = a.H - h0 - c;
-      if (r >= x.rows[0] || left <= 0) return;
-      const int64_t to = (m0 + r) * a.H + h0 + c;
-      float m[8];
+  }, [&](int64_t) { return w; });
+  gemm_results<true, 4>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&g)[8], const float (&u)[8]) {
+    const int left = a.H - h0 - c;
+    if (r >= x.rows[0] || left <= 0) return;
+    const int64_t to = (m0 + r) * a.H + h0 + c;
+    float m[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m[e] = gff_act<T>(a.act, g[e]) * u[e];
-      store_eight(a.mid + to, m, left);
-      if (a.gate) {
-        store_eight(a.gate + to, g, left);
-        store_eight(a.up + to, u, left);
-      }
-    });
+    for (int e = 0; e < 8; ++e) m[e] = gff_act<T, ACT>(g[e]) * u[e];
+    store_eight(a.mid + to, m, FAST ? 8 : left);
+    if (a.gate) {
+      store_eight(a.gate + to, g, FAST ? 8 : left);
+      store_eight(a.up + to, u, FAST ? 8 : left);
+    }
   });
 }
 
@@ -107,55 +101,52 @@ struct MidGradArgs {
   const T *gy, *wd, *gate, *up;
   T *g_gate, *g_up;
   int64_t n_rows;
-  int H, C, act, each;
+  int H, C;
 };
 
 // dg and du from dm = dy Wd^T.
-template <typename T, bool FAST>
-__global__ void __launch_bounds__(kGemmThreads, 2) gff_mid_grad_kernel(MidGradArgs<T> a) {
-  __shared__ alignas(16) char lds[4 * kGemmTileBytes];
+template <typename T, bool FAST, int ACT>
+__global__ void __launch_bounds__(kGemmThreads, 3) gff_mid_grad_kernel(MidGradArgs<T> a) {
+  __shared__ alignas(16) char lds[2 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place((a.H + kGemmTile - 1) / kGemmTile, a.each);
+  const TilePlace at = tile_place((a.H + kGemmTile - 1) / kGemmTile);
   const int64_t m0 = at.outer * kGemmTile;
   if (m0 >= a.n_rows) return;
+  const int h0 = at.inner * kGemmTile;
+  const GemmOperand<T> wd = {{a.wd + (int64_t)h0 * a.C, nullptr}, a.C, {rows_left(a.H, h0), 0}};
   const GemmOperand<T> gy = {{a.gy + m0 * a.C, nullptr}, a.C, {rows_left(a.n_rows, m0), 0}};
   f32x16_t acc[2][2];
-  gemm_loop<T, FAST, true, true, false>(acc, lds, at.count, (a.C + D - 1) / D, [&](int, int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, true, true, false>(acc, lds, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = a.C;
     return gy;
-  }, [&](int i, int64_t) {
-    const int h0 = (at.inner + i) * kGemmTile;
-    return GemmOperand<T>{{a.wd + (int64_t)h0 * a.C, nullptr}, a.C, {rows_left(a.H, h0), 0}};
-  }, [&](int i) {
-    // The projections' part is fetched a few places ahead of its use: one wait for memory in place of one for each place.
-    constexpr int kAhead = sizeof(T) == 2 ? 8 : 4;
-    EightRaw<T> pg[kAhead], pu[kAhead];
-    const int h0 = (at.inner + i) * kGemmTile;
-    auto fetch = [&](int p, int r, int c) {
-      const int left = a.H - h0 - c;
-      if (r >= gy.rows[0] || left <= 0) return;
-      const int64_t from = (m0 + r) * a.H + h0 + c;
-      pg[p % kAhead].load(a.gate + from, left);
-      pu[p % kAhead].load(a.up + from, left);
-    };
-    gemm_results<false, kAhead>(acc, lds, fetch, [&](int p, int r, int c, const float (&dm)[8]) {
-      const int left = a.H - h0 - c;
-      if (r >= gy.rows[0] || left <= 0) return;
-      const int64_t to = (m0 + r) * a.H + h0 + c;
-      float g[8], u[8];
-      pg[p % kAhead].get(g);
-      pu[p % kAhead].get(u);
+  }, [&](int64_t) { return wd; });
+  // The projections' part is fetched a few places ahead of its use: one wait for memory in place of one for each place.
+  constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;
+  EightRaw<T> pg[kAhead], pu[kAhead];
+  auto fetch = [&](int p, int r, int c) {
+    const int left = a.H - h0 - c;
+    if (r >= gy.rows[0] || left <= 0) return;
+    const int64_t from = (m0 + r) * a.H + h0 + c;
+    pg[p % kAhead].load(a.gate + from, FAST ? 8 : left);
+    pu[p % kAhead].load(a.up + from, FAST ? 8 : left);
+  };
+  gemm_results<false, kAhead>(acc, lds, fetch, [&](int p, int r, int c, const float (&dm)[8]) {
+    const int left = a.H - h0 - c;
+    if (r >= gy.rows[0] || left <= 0) return;
+    const int64_t to = (m0 + r) * a.H + h0 + c;
+    float g[8], u[8];
+    pg[p % kAhead].get(g);
+    pu[p % kAhead].get(u);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float value;
-        const float slope = gff_act_grad<T>(a.act, g[e], value);
-        g[e] = dm[e] * u[e] * slope;
-        u[e] = dm[e] * value;
-      }
-      store_eight(a.g_gate + to, g, left);
-      store_eight(a.g_up + to, u, left);
-    });
+    for (int e = 0; e < 8; ++e) {
+      float value;
+      const float slope = gff_act_grad<T, ACT>(g[e], value);
+      g[e] = dm[e] * u[e] * slope;
+      u[e] = dm[e] * value;
+    }
+    store_eight(a.g_gate + to, g, FAST ? 8 : left);
+    store_eight(a.g_up + to, u, FAST ? 8 : left);
   });
 }
 
@@ -165,33 +156,29 @@ struct RowsArgs {
   const T *a[2], *b[2];
   T* out;
   int64_t n_rows, ldb;
-  int segments, K, N, each;      // K: per segment
+  int segments, K, N;      // K: per segment
 };
 template <typename T, bool FAST, bool KB>
-__global__ void __launch_bounds__(kGemmThreads, 2) gff_rows_kernel(RowsArgs<T> a) {
-  __shared__ alignas(16) char lds[4 * kGemmTileBytes];
+__global__ void __launch_bounds__(kGemmThreads, 3) gff_rows_kernel(RowsArgs<T> a) {
+  __shared__ alignas(16) char lds[2 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place((a.N + kGemmTile - 1) / kGemmTile, a.each);
+  const TilePlace at = tile_place((a.N + kGemmTile - 1) / kGemmTile);
   const int64_t m0 = at.outer * kGemmTile;
   if (m0 >= a.n_rows) return;
-  const int tiles = (a.K + D - 1) / D, rows = rows_left(a.n_rows, m0);
+  const int n0 = at.inner * kGemmTile, tiles = (a.K + D - 1) / D, rows = rows_left(a.n_rows, m0), cols = rows_left(a.N, n0);
   f32x16_t acc[2][2];
-  gemm_loop<T, FAST, true, KB, false>(acc, lds, at.count, (int64_t)tiles * a.segments,
-                                      [&](int, int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, true, KB, false>(acc, lds, (int64_t)tiles * a.segments, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = (t < tiles ? t : t - tiles) * D;
     depth = a.K;
     return GemmOperand<T>{{(t < tiles ? a.a[0] : a.a[1]) + m0 * a.K, nullptr}, a.K, {rows, 0}};
-  }, [&](int i, int64_t t) {
+  }, [&](int64_t t) {
     const T* b = t < tiles ? a.b[0] : a.b[1];
-    const int n0 = (at.inner + i) * kGemmTile, cols = rows_left(a.N, n0);
     if (KB) return GemmOperand<T>{{b + n0 * a.ldb, nullptr}, a.ldb, {cols, 0}};
     return GemmOperand<T>{{b + n0, b + n0 + 64}, a.ldb, {cols, cols - 64}};
-  }, [&](int i) {
-    const int n0 = (at.inner + i) * kGemmTile;
-    gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
-      const int left = a.N - n0 - c;
-      if (r < rows && left > 0) store_eight(a.out + (m0 + r) * a.N + n0 + c, v, left);
-    });
+  });
+  gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
+    const int left = a.N - n0 - c;
+    if (r < rows && left > 0) store_eight(a.out + (m0 + r) * a.N + n0 + c, v, FAST ? 8 : left);
   });
 }
 
@@ -212,10 +199,10 @@ struct WeightArgs {
   int jobs, tiles, splits;
 };
 template <typename T, bool FAST>
-__global__ void __launch_bounds__(kGemmThreads, 2) gff_weight_kernel(WeightArgs<T> w) {
-  __shared__ alignas(16) char lds[4 * kGemmTileBytes];
+__global__ void __launch_bounds__(kGemmThreads, 3) gff_weight_kernel(WeightArgs<T> w) {
+  __shared__ alignas(16) char lds[2 * kGemmTileBytes];
   constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place(w.tiles, 1);
+  const TilePlace at = tile_place(w.tiles);
   if (at.outer >= w.splits) return;
   const int which = w.jobs > 2 && at.inner >= w.job[2].first_tile ? 2 : w.jobs > 1 && at.inner >= w.job[1].first_tile ? 1 : 0;
   const WeightJob<T> job = w.job[which];
@@ -227,18 +214,17 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gff_weight_kernel(WeightArgs<
   const T *ja = job.a + r0 * job.M + m0, *jb = job.b + r0 * job.N + n0;
   const GemmOperand<T> pa = {{ja, ja + 64}, job.M, {rows, rows - 64}}, pb = {{jb, jb + 64}, job.N, {cols, cols - 64}};
   f32x16_t acc[2][2];
-  gemm_loop<T, FAST, false, false, false>(acc, lds, 1, (end + D - 1) / D, [&](int, int64_t t, int64_t& k0, int64_t& depth) {
+  gemm_loop<T, FAST, false, false, false>(acc, lds, (end + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = end;
     return pa;
-  }, [&](int, int64_t) { return pb; }, [&](int) {
-    gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
-      const int left = job.N - n0 - c;
-      if (r >= rows || left <= 0) return;
-      const int64_t to = (int64_t)(m0 + r) * job.N + n0 + c;
-      if (w.splits > 1) store_eight(w.parts + at.outer * w.part_elems + job.first_part + to, v, left);
-      else store_eight(job.out + to, v, left);
-    });
+  }, [&](int64_t) { return pb; });
+  gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
+    const int left = job.N - n0 - c;
+    if (r >= rows || left <= 0) return;
+    const int64_t to = (int64_t)(m0 + r) * job.N + n0 + c;
+    if (w.splits > 1) store_eight(w.parts + at.outer * w.part_elems + job.first_part + to, v, FAST ? 8 : left);
+    else store_eight(job.out + to, v, FAST ? 8 : left);
   });
 }
 template <typename T>
@@ -267,14 +253,13 @@ int gff_check(const cgtp_gff_args* a) {
   return CGTP_OK;
 }
 
-// Whether rows of `ld` elements are whole aligned chunks, and a tile's offsets fit 31 bits.
-template <typename T>
-bool whole_chunks(std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> lds) {
+// Whether every row is a number of whole groups of eight elements, aligned, and a tile's offsets fit 31 bits: no access is cut.
+bool whole_groups(const cgtp_gff_args* a) {
+  const void* ptrs[] = {a->x, a->w_gate, a->w_up, a->w_down, a->gate, a->up, a->mid, a->out, a->grad_out, a->grad_gate, a->grad_up,
+                        a->grad_x, a->grad_w_gate, a->grad_w_up, a->grad_w_down, a->workspace};
   for (const void* p : ptrs)
     if (!aligned16(p)) return false;
-  for (int64_t ld : lds)
-    if (ld % (16 / (int)sizeof(T)) || ld * (int64_t)sizeof(T) * kGemmTile > 0x7fffffff) return false;
-  return true;
+  return a->c_in % 8 == 0 && a->hidden % 8 == 0 && a->c_out % 8 == 0;      // hidden < 2^17: 128 rows of it are below 2^26 bytes
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -295,37 +280,49 @@ WeightShape weight_shape(const cgtp_gff_args* a) {
   return s;
 }
 
+// The kernel of an activation: a branch on it for each element costs more than the activation.
+template <typename Kernel, typename Of>
+Kernel for_act(int act, Of&& of) {
+  if (act == CGTP_ACT_SILU) return of(std::integral_constant<int, CGTP_ACT_SILU>{});
+  if (act == CGTP_ACT_GELU) return of(std::integral_constant<int, CGTP_ACT_GELU>{});
+  return of(std::integral_constant<int, CGTP_ACT_SIGMOID>{});
+}
+
 template <typename T>
 int gff_forward(const cgtp_gff_args* a, hipStream_t s) {
+  const bool fast = whole_groups(a);
   const int64_t mt = ceil_div(a->n_rows, kGemmTile);
   const UpArgs<T> u = {(const T*)a->x, (const T*)a->w_gate, (const T*)a->w_up, (T*)a->gate, (T*)a->up, (T*)a->mid, a->n_rows,
-                       a->c_in, a->hidden, a->activation, tiles_each(mt, ceil_div(a->hidden, 64))};
-  auto up = whole_chunks<T>({u.x, u.wg, u.wu}, {u.C, u.H}) ? gff_up_kernel<T, true> : gff_up_kernel<T, false>;
-  hipLaunchKernelGGL(up, dim3(tile_grid(mt, ceil_div(a->hidden, 64), u.each)), dim3(kGemmThreads), 0, s, u);
+                       a->c_in, a->hidden};
+  auto up = for_act<void (*)(UpArgs<T>)>(a->activation, [&](auto act) {
+    return fast ? gff_up_kernel<T, true, decltype(act)::value> : gff_up_kernel<T, false, decltype(act)::value>;
+  });
+  hipLaunchKernelGGL(up, dim3(tile_grid(mt, ceil_div(a->hidden, 64))), dim3(kGemmThreads), 0, s, u);
   const RowsArgs<T> d = {{(const T*)a->mid, nullptr}, {(const T*)a->w_down, nullptr}, (T*)a->out, a->n_rows, a->c_out, 1, a->hidden,
-                         a->c_out, tiles_each(mt, ceil_div(a->c_out, kGemmTile))};
-  auto down = whole_chunks<T>({d.a[0], d.b[0]}, {d.K, d.N}) ? gff_rows_kernel<T, true, false> : gff_rows_kernel<T, false, false>;
-  hipLaunchKernelGGL(down, dim3(tile_grid(mt, ceil_div(a->c_out, kGemmTile), d.each)), dim3(kGemmThreads), 0, s, d);
+                         a->c_out};
+  auto down = fast ? gff_rows_kernel<T, true, false> : gff_rows_kernel<T, false, false>;
+  hipLaunchKernelGGL(down, dim3(tile_grid(mt, ceil_div(a->c_out, kGemmTile))), dim3(kGemmThreads), 0, s, d);
   return launch_status();
 }
 
 template <typename T>
 int gff_backward(const cgtp_gff_args* a, hipStream_t s) {
+  const bool fast = whole_groups(a);
   const int64_t mt = ceil_div(a->n_rows, kGemmTile);
   if (a->n_rows > 0 && (a->grad_x || a->grad_w_gate || a->grad_w_up)) {
     const MidGradArgs<T> m = {(const T*)a->grad_out, (const T*)a->w_down, (const T*)a->gate, (const T*)a->up, (T*)a->grad_gate,
-                              (T*)a->grad_up, a->n_rows, a->hidden, a->c_out, a->activation,
-                              tiles_each(mt, ceil_div(a->hidden, kGemmTile))};
-    auto mid = whole_chunks<T>({m.gy, m.wd}, {m.C}) ? gff_mid_grad_kernel<T, true> : gff_mid_grad_kernel<T, false>;
-    hipLaunchKernelGGL(mid, dim3(tile_grid(mt, ceil_div(a->hidden, kGemmTile), m.each)), dim3(kGemmThreads), 0, s, m);
+                              (T*)a->grad_up, a->n_rows, a->hidden, a->c_out};
+    auto mid = for_act<void (*)(MidGradArgs<T>)>(a->activation, [&](auto act) {
+      return fast ? gff_mid_grad_kernel<T, true, decltype(act)::value> : gff_mid_grad_kernel<T, false, decltype(act)::value>;
+    });
+    hipLaunchKernelGGL(mid, dim3(tile_grid(mt, ceil_div(a->hidden, kGemmTile))), dim3(kGemmThreads), 0, s, m);
   }
   if (a->n_rows > 0 && a->grad_x) {
     const RowsArgs<T> d = {{(const T*)a->grad_gate, (const T*)a->grad_up}, {(const T*)a->w_gate, (const T*)a->w_up},
-                           (T*)a->grad_x, a->n_rows, a->hidden, 2, a->hidden, a->c_in,
-                           tiles_each(mt, ceil_div(a->c_in, kGemmTile))};
-    auto back = whole_chunks<T>({d.a[0], d.a[1], d.b[0], d.b[1]}, {d.K}) ? gff_rows_kernel<T, true, true>
+                           (T*)a->grad_x, a->n_rows, a->hidden, 2, a->hidden, a->c_in};
+    auto back = fast ? gff_rows_kernel<T, true, true>
                                                                          : gff_rows_kernel<T, false, true>;
-    hipLaunchKernelGGL(back, dim3(tile_grid(mt, ceil_div(a->c_in, kGemmTile), d.each)), dim3(kGemmThreads), 0, s, d);
+    hipLaunchKernelGGL(back, dim3(tile_grid(mt, ceil_div(a->c_in, kGemmTile))), dim3(kGemmThreads), 0, s, d);
   }
   const WeightShape shape = weight_shape(a);
   WeightArgs<T> w = {};
@@ -343,9 +340,8 @@ int gff_backward(const cgtp_gff_args* a, hipStream_t s) {
   job(a->x, a->grad_up, a->grad_w_up, a->c_in, a->hidden);
   job(a->mid, a->grad_out, a->grad_w_down, a->hidden, a->c_out);
   if (w.jobs) {
-    auto weight = whole_chunks<T>({a->x, a->grad_gate, a->grad_up, a->mid, a->grad_out}, {a->c_in, a->hidden, a->c_out})
-                      ? gff_weight_kernel<T, true> : gff_weight_kernel<T, false>;
-    hipLaunchKernelGGL(weight, dim3(tile_grid(w.splits, w.tiles, 1)), dim3(kGemmThreads), 0, s, w);
+    auto weight = fast ? gff_weight_kernel<T, true> : gff_weight_kernel<T, false>;
+    hipLaunchKernelGGL(weight, dim3(tile_grid(w.splits, w.tiles)), dim3(kGemmThreads), 0, s, w);
     if (w.splits > 1)
       hipLaunchKernelGGL(gff_add_kernel<T>, dim3((unsigned)ceil_div(w.part_elems, 256)), dim3(256), 0, s, w);
   }
