@@ -297,7 +297,7 @@ def _load():
     for name in ("cgtp_gff", "cgtp_attn"):
         args = C.POINTER(GffArgs if name == "cgtp_gff" else AttnArgs)
         ws = getattr(lib, name + "_workspace_bytes")
-        ws.restype, ws.argtypes = C.c_int64, [args] if name == "cgtp_gff" else [args, C.c_int]
+        ws.restype, ws.argtypes = C.c_int64, [args, C.c_int]
         getattr(lib, name + "_forward").argtypes = [args, C.c_void_p]
         getattr(lib, name + "_backward").argtypes = [args, C.c_void_p]
     lib.cgtp_abi_layout.argtypes = [C.c_int, C.POINTER(C.c_int64), C.c_int]

@@ -54,6 +54,11 @@ __device__ __forceinline__ TilePlace tile_place(int inner_tiles) {
 }
 unsigned tile_grid(int64_t outer, int64_t inner) { return (unsigned)((outer + 7) / 8 * 8 * inner); }
 
+__device__ __forceinline__ int left_of(int64_t n, int64_t from, int most) { return (int)(n - from < most ? n - from : most); }
+
+// LDS of a workgroup: the two operands' tiles, then the results.
+template <int TILE> constexpr int kGemmLds = TILE * 256;
+
 template <typename T>
 struct UpArgs {
   const T *x, *wg, *wu;
@@ -62,26 +67,24 @@ struct UpArgs {
   int C, H;
 };
 
-__device__ __forceinline__ int rows_left(int64_t n, int64_t from) { return (int)(n - from < kGemmTile ? n - from : kGemmTile); }
-
-// g, u and m.  A tile is 128 rows x 64 hidden channels, of Wg and of Wu.
-template <typename T, bool FAST, int ACT>
-__global__ void __launch_bounds__(kGemmThreads, 3) gff_up_kernel(UpArgs<T> a) {
-  __shared__ alignas(16) char lds[2 * kGemmTileBytes];
-  constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place((a.H + 63) / 64);
-  const int64_t m0 = at.outer * kGemmTile;
+// g, u and m.  A tile is TILE rows x TILE / 2 hidden channels, of Wg and of Wu.
+template <typename T, int TILE, bool FAST, int ACT>
+__global__ void __launch_bounds__(kGemmThreads, TILE == 128 ? 3 : 4) gff_up_kernel(UpArgs<T> a) {
+  __shared__ alignas(16) char lds[kGemmLds<TILE>];
+  constexpr int D = GemmType<T>::kDepth, kCols = TILE / 2;
+  const TilePlace at = tile_place((a.H + kCols - 1) / kCols);
+  const int64_t m0 = at.outer * TILE;
   if (m0 >= a.n_rows) return;
-  const int h0 = at.inner * 64;
+  const int h0 = at.inner * kCols;
+  const GemmOperand<T> x = {{a.x + m0 * a.C, nullptr}, a.C, {left_of(a.n_rows, m0, TILE), 0}};
   const GemmOperand<T> w = {{a.wg + h0, a.wu + h0}, a.H, {a.H - h0, a.H - h0}};
-  const GemmOperand<T> x = {{a.x + m0 * a.C, nullptr}, a.C, {rows_left(a.n_rows, m0), 0}};
-  f32x16_t acc[2][2];
-  gemm_loop<T, FAST, true, false, true>(acc, lds, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  GemmAcc<TILE> acc;
+  gemm_loop<T, TILE, FAST, true, false, true>(acc, lds, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = a.C;
     return x;
   }, [&](int64_t) { return w; });
-  gemm_results<true, 4>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&g)[8], const float (&u)[8]) {
+  gemm_results<TILE, true, 4>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&g)[8], const float (&u)[8]) {
     const int left = a.H - h0 - c;
     if (r >= x.rows[0] || left <= 0) return;
     const int64_t to = (m0 + r) * a.H + h0 + c;
@@ -105,18 +108,18 @@ struct MidGradArgs {
 };
 
 // dg and du from dm = dy Wd^T.
-template <typename T, bool FAST, int ACT>
-__global__ void __launch_bounds__(kGemmThreads, 3) gff_mid_grad_kernel(MidGradArgs<T> a) {
-  __shared__ alignas(16) char lds[2 * kGemmTileBytes];
+template <typename T, int TILE, bool FAST, int ACT>
+__global__ void __launch_bounds__(kGemmThreads, TILE == 128 ? 3 : 4) gff_mid_grad_kernel(MidGradArgs<T> a) {
+  __shared__ alignas(16) char lds[kGemmLds<TILE>];
   constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place((a.H + kGemmTile - 1) / kGemmTile);
-  const int64_t m0 = at.outer * kGemmTile;
+  const TilePlace at = tile_place((a.H + TILE - 1) / TILE);
+  const int64_t m0 = at.outer * TILE;
   if (m0 >= a.n_rows) return;
-  const int h0 = at.inner * kGemmTile;
-  const GemmOperand<T> wd = {{a.wd + (int64_t)h0 * a.C, nullptr}, a.C, {rows_left(a.H, h0), 0}};
-  const GemmOperand<T> gy = {{a.gy + m0 * a.C, nullptr}, a.C, {rows_left(a.n_rows, m0), 0}};
-  f32x16_t acc[2][2];
-  gemm_loop<T, FAST, true, true, false>(acc, lds, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  const int h0 = at.inner * TILE;
+  const GemmOperand<T> gy = {{a.gy + m0 * a.C, nullptr}, a.C, {left_of(a.n_rows, m0, TILE), 0}};
+  const GemmOperand<T> wd = {{a.wd + (int64_t)h0 * a.C, nullptr}, a.C, {left_of(a.H, h0, TILE), 0}};
+  GemmAcc<TILE> acc;
+  gemm_loop<T, TILE, FAST, true, true, false>(acc, lds, (a.C + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = a.C;
     return gy;
@@ -131,7 +134,7 @@ __global__ void __launch_bounds__(kGemmThreads, 3) gff_mid_grad_kernel(MidGradAr
     pg[p % kAhead].load(a.gate + from, FAST ? 8 : left);
     pu[p % kAhead].load(a.up + from, FAST ? 8 : left);
   };
-  gemm_results<false, kAhead>(acc, lds, fetch, [&](int p, int r, int c, const float (&dm)[8]) {
+  gemm_results<TILE, false, kAhead>(acc, lds, fetch, [&](int p, int r, int c, const float (&dm)[8]) {
     const int left = a.H - h0 - c;
     if (r >= gy.rows[0] || left <= 0) return;
     const int64_t to = (m0 + r) * a.H + h0 + c;
@@ -150,40 +153,50 @@ __global__ void __launch_bounds__(kGemmThreads, 3) gff_mid_grad_kernel(MidGradAr
   });
 }
 
-// out = sum over segments of A_s B_s: y = m Wd (one segment), dx = dg Wg^T + du Wu^T (two).  A is contiguous along k.
+// out = sum over segments of A_s B_s: y = m Wd (one segment), dx = dg Wg^T + du Wu^T (two).  A is contiguous along k.  The
+// tiles of k are cut into `splits` ranges where the result has few tiles; a range's result is left in fp32 and the ranges
+// are added in order by gff_add_kernel.
 template <typename T>
 struct RowsArgs {
   const T *a[2], *b[2];
   T* out;
+  float* parts;
   int64_t n_rows, ldb;
-  int segments, K, N;      // K: per segment
+  int segments, K, N, splits;      // K: per segment
 };
-template <typename T, bool FAST, bool KB>
-__global__ void __launch_bounds__(kGemmThreads, 3) gff_rows_kernel(RowsArgs<T> a) {
-  __shared__ alignas(16) char lds[2 * kGemmTileBytes];
+template <typename T, int TILE, bool FAST, bool KB>
+__global__ void __launch_bounds__(kGemmThreads, TILE == 128 ? 3 : 4) gff_rows_kernel(RowsArgs<T> a) {
+  __shared__ alignas(16) char lds[kGemmLds<TILE>];
   constexpr int D = GemmType<T>::kDepth;
-  const TilePlace at = tile_place((a.N + kGemmTile - 1) / kGemmTile);
-  const int64_t m0 = at.outer * kGemmTile;
+  const int tiles_n = (a.N + TILE - 1) / TILE;
+  const TilePlace at = tile_place(tiles_n * a.splits);
+  const int64_t m0 = at.outer * TILE;
   if (m0 >= a.n_rows) return;
-  const int n0 = at.inner * kGemmTile, tiles = (a.K + D - 1) / D, rows = rows_left(a.n_rows, m0), cols = rows_left(a.N, n0);
-  f32x16_t acc[2][2];
-  gemm_loop<T, FAST, true, KB, false>(acc, lds, (int64_t)tiles * a.segments, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  const int split = at.inner / tiles_n, n0 = at.inner % tiles_n * TILE;
+  const int tiles = (a.K + D - 1) / D, all = tiles * a.segments, each = (all + a.splits - 1) / a.splits, first = split * each;
+  const int rows = left_of(a.n_rows, m0, TILE), cols = left_of(a.N, n0, TILE);
+  GemmAcc<TILE> acc;
+  gemm_loop<T, TILE, FAST, true, KB, false>(acc, lds, std::min(each, all - first), [&](int64_t t, int64_t& k0, int64_t& depth) {
+    t += first;
     k0 = (t < tiles ? t : t - tiles) * D;
     depth = a.K;
     return GemmOperand<T>{{(t < tiles ? a.a[0] : a.a[1]) + m0 * a.K, nullptr}, a.K, {rows, 0}};
   }, [&](int64_t t) {
-    const T* b = t < tiles ? a.b[0] : a.b[1];
+    const T* b = t + first < tiles ? a.b[0] : a.b[1];
     if (KB) return GemmOperand<T>{{b + n0 * a.ldb, nullptr}, a.ldb, {cols, 0}};
-    return GemmOperand<T>{{b + n0, b + n0 + 64}, a.ldb, {cols, cols - 64}};
+    return GemmOperand<T>{{b + n0, b + n0 + TILE / 2}, a.ldb, {cols, cols - TILE / 2}};
   });
-  gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
+  gemm_results<TILE, false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
     const int left = a.N - n0 - c;
-    if (r < rows && left > 0) store_eight(a.out + (m0 + r) * a.N + n0 + c, v, FAST ? 8 : left);
+    if (r >= rows || left <= 0) return;
+    const int64_t to = (m0 + r) * a.N + n0 + c;
+    if (a.splits > 1) store_eight(a.parts + split * a.n_rows * a.N + to, v, FAST ? 8 : left);
+    else store_eight(a.out + to, v, FAST ? 8 : left);
   });
 }
 
 // Weight gradients out_j = A_j^T B_j over all rows: both operands contiguous along the tile's rows.  The rows are cut
-// into `splits` ranges; a range's result is left in fp32 and the ranges are added in order by gff_add_kernel.
+// into `splits` ranges, as above.
 template <typename T>
 struct WeightJob {
   const T *a, *b;
@@ -198,28 +211,28 @@ struct WeightArgs {
   int64_t n_rows, rows_per_split, part_elems;
   int jobs, tiles, splits;
 };
-template <typename T, bool FAST>
-__global__ void __launch_bounds__(kGemmThreads, 3) gff_weight_kernel(WeightArgs<T> w) {
-  __shared__ alignas(16) char lds[2 * kGemmTileBytes];
-  constexpr int D = GemmType<T>::kDepth;
+template <typename T, int TILE, bool FAST>
+__global__ void __launch_bounds__(kGemmThreads, TILE == 128 ? (FAST ? 3 : 2) : 4) gff_weight_kernel(WeightArgs<T> w) {
+  __shared__ alignas(16) char lds[kGemmLds<TILE>];
+  constexpr int D = GemmType<T>::kDepth, kCut = TILE / 2;
   const TilePlace at = tile_place(w.tiles);
   if (at.outer >= w.splits) return;
   const int which = w.jobs > 2 && at.inner >= w.job[2].first_tile ? 2 : w.jobs > 1 && at.inner >= w.job[1].first_tile ? 1 : 0;
   const WeightJob<T> job = w.job[which];
   const int tile = at.inner - job.first_tile;
-  const int m0 = tile / job.tiles_n * kGemmTile, n0 = tile % job.tiles_n * kGemmTile;
+  const int m0 = tile / job.tiles_n * TILE, n0 = tile % job.tiles_n * TILE;
   const int64_t r0 = at.outer * w.rows_per_split;
   const int64_t end = std::min(w.rows_per_split, w.n_rows - r0);
-  const int rows = rows_left(job.M, m0), cols = rows_left(job.N, n0);
+  const int rows = left_of(job.M, m0, TILE), cols = left_of(job.N, n0, TILE);
   const T *ja = job.a + r0 * job.M + m0, *jb = job.b + r0 * job.N + n0;
-  const GemmOperand<T> pa = {{ja, ja + 64}, job.M, {rows, rows - 64}}, pb = {{jb, jb + 64}, job.N, {cols, cols - 64}};
-  f32x16_t acc[2][2];
-  gemm_loop<T, FAST, false, false, false>(acc, lds, (end + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
+  const GemmOperand<T> pa = {{ja, ja + kCut}, job.M, {rows, rows - kCut}}, pb = {{jb, jb + kCut}, job.N, {cols, cols - kCut}};
+  GemmAcc<TILE> acc;
+  gemm_loop<T, TILE, FAST, false, false, false>(acc, lds, (end + D - 1) / D, [&](int64_t t, int64_t& k0, int64_t& depth) {
     k0 = t * D;
     depth = end;
     return pa;
   }, [&](int64_t) { return pb; });
-  gemm_results<false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
+  gemm_results<TILE, false, 8>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, const float (&v)[8]) {
     const int left = job.N - n0 - c;
     if (r >= rows || left <= 0) return;
     const int64_t to = (int64_t)(m0 + r) * job.N + n0 + c;
@@ -227,15 +240,116 @@ __global__ void __launch_bounds__(kGemmThreads, 3) gff_weight_kernel(WeightArgs<
     else store_eight(job.out + to, v, FAST ? 8 : left);
   });
 }
+
+// out[i] = sum over the ranges of their partial results, in order.  Up to three outputs, one after the other in a range's part.
 template <typename T>
-__global__ void __launch_bounds__(256) gff_add_kernel(WeightArgs<T> w) {
+struct AddArgs {
+  const float* parts;
+  T* out[3];
+  int64_t first[3], elems;
+  int outs, splits;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) gff_add_kernel(AddArgs<T> a) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= w.part_elems) return;
+  if (i >= a.elems) return;
   float s = 0.f;
-  for (int k = 0; k < w.splits; ++k) s += w.parts[k * w.part_elems + i];
-  const int which = w.jobs > 2 && i >= w.job[2].first_part ? 2 : w.jobs > 1 && i >= w.job[1].first_part ? 1 : 0;
-  const WeightJob<T> job = w.job[which];
-  job.out[i - job.first_part] = (T)s;
+#pragma unroll 8
+  for (int k = 0; k < a.splits; ++k) s += a.parts[k * a.elems + i];
+  const int which = a.outs > 2 && i >= a.first[2] ? 2 : a.outs > 1 && i >= a.first[1] ? 1 : 0;
+  a.out[which][i - a.first[which]] = (T)s;
+}
+
+// A handful of rows: the weights are read once for all of them and nothing else counts.  A workgroup takes 32 columns, a
+// thread eight of them at every 64th k, in fp32; the 64 sums of a column are added in LDS in a fixed order.
+// MATS = 2: x against Wg and Wu, then the activation and the product; MATS = 1: m against Wd.
+constexpr int kFewRows = 4, kFewCols = 32, kFewSlices = 64;
+template <typename T>
+struct FewArgs {
+  const T *x, *w[2];
+  T *gate, *up, *out;
+  int n_rows, K, N;
+};
+template <typename T, int ROWS, int MATS, int ACT>
+__global__ void __launch_bounds__(256) gff_few_kernel(FewArgs<T> a) {
+  constexpr int kSums = kFewCols * MATS;
+  __shared__ float sums[kFewSlices][kSums + 4];
+  const int n0 = blockIdx.x * kFewCols, group = threadIdx.x & 3, slice = threadIdx.x >> 2, n = n0 + group * 8, left = a.N - n;
+  float acc[ROWS][MATS][8];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[r][m][e] = 0.f;
+  if (left > 0) {
+    constexpr int kAhead = ROWS == 1 ? 16 / (MATS * (int)sizeof(T) / 2) : 4;      // loads on their way: 16
+    for (int k0 = slice; k0 < a.K; k0 += kFewSlices * kAhead) {
+      EightRaw<T> w[kAhead][MATS];
+      float x[kAhead][ROWS];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int k = k0 + j * kFewSlices;
+        const bool in = k < a.K;
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) w[j][m].load(a.w[m] + (int64_t)(in ? k : k0) * a.N + n, left);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) x[j][r] = r < a.n_rows && in ? (float)a.x[(int64_t)r * a.K + k] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (k0 + j * kFewSlices >= a.K) continue;        // not even 0 times what is read in its place
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+          float v[8];
+          w[j][m].get(v);
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[r][m][e] = fmaf(x[j][r], v[e], acc[r][m][e]);
+        }
+      }
+    }
+  }
+  // 256 / kSums threads for each sum, then one
+  constexpr int kParts = 256 / kSums, kPer = kFewSlices / kParts;
+  __shared__ float last[256];
+  for (int r = 0; r < ROWS && r < a.n_rows; ++r) {
+    __syncthreads();
+#pragma unroll
+    for (int rr = 0; rr < ROWS; ++rr)
+      if (rr == r)
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sums[slice][m * kFewCols + group * 8 + e] = acc[rr][m][e];
+    __syncthreads();
+    const int c = threadIdx.x % kSums, part = threadIdx.x / kSums;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) s += sums[part * kPer + k][c];
+    last[threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.x < kFewCols && n0 + (int)threadIdx.x < a.N) {
+      float t[MATS];
+#pragma unroll
+      for (int m = 0; m < MATS; ++m) {
+        t[m] = 0.f;
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) t[m] += last[p * kSums + m * kFewCols + threadIdx.x];
+      }
+      const int64_t to = (int64_t)r * a.N + n0 + threadIdx.x;
+      if constexpr (MATS == 2) {
+        a.out[to] = (T)(gff_act<T, ACT>(t[0]) * t[1]);
+        if (a.gate) {
+          a.gate[to] = (T)t[0];
+          a.up[to] = (T)t[1];
+        }
+      } else {
+        a.out[to] = (T)t[0];
+      }
+    }
+  }
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
@@ -244,7 +358,7 @@ int gff_check(const cgtp_gff_args* a) {
   if (a->dtype != CGTP_F32 && a->dtype != CGTP_BF16 && a->dtype != CGTP_F16) return CGTP_ERR_DTYPE;
   if (a->n_rows < 0 || a->n_rows > 0x7fffffff || a->c_in <= 0 || a->c_out <= 0 || a->hidden <= 0) return CGTP_ERR_SHAPE;
   // a grid has fewer than 2^32 threads, the weights' partial results an index of 31 bits
-  if (((a->n_rows + 1023) / 1024) * ((a->hidden + 63) / 64) >= (1 << 20)) return CGTP_ERR_SHAPE;
+  if (((a->n_rows + 511) / 512) * ((std::max(std::max(a->hidden, a->c_in), a->c_out) + 31) / 32) >= (1 << 20)) return CGTP_ERR_SHAPE;
   if ((int64_t)a->hidden * (2ll * a->c_in + a->c_out) > 0x7fffffff) return CGTP_ERR_SHAPE;
   if (a->c_in > 0x7fff || a->c_out > 0x7fff || a->hidden > 0x1ffff) return CGTP_ERR_SHAPE;
   if (a->activation < 0 || a->activation >= kActs) return CGTP_ERR_CONFIG;
@@ -264,20 +378,50 @@ bool whole_groups(const cgtp_gff_args* a) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Ranges the rows are cut into for the weight gradients: three workgroups for each compute unit, at least eight k tiles each.
-struct WeightShape { int splits; int64_t rows_per_split, part_elems; int tiles; };
+// Tiles of 128 (fewer bytes from memory and LDS for each product) where they give every compute unit a workgroup, else of 64:
+// 3001 rows of 128 -> 512 channels, fp32, forward and backward 200 us of kernels with tiles of 128 alone, 89 with these.
+bool small_tiles(int64_t tiles_of_128) { return tiles_of_128 < 256; }
+
+// Ranges that k is cut into for a product of `tiles` results: two workgroups for each compute unit, at least four tiles of k.
+int ranges_of(int64_t tiles, int64_t k_tiles) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(tiles < 256 ? 512 / std::max<int64_t>(1, tiles) : 1, k_tiles / 4));
+}
+
+struct RowsShape { int tile, splits; };
+template <typename T>
+RowsShape rows_shape(int64_t n_rows, int N, int64_t k_tiles) {
+  RowsShape s;
+  s.tile = small_tiles(ceil_div(n_rows, 128) * ceil_div(N, 128)) ? 64 : 128;
+  s.splits = s.tile == 64 ? ranges_of(ceil_div(n_rows, 64) * ceil_div(N, 64), k_tiles) : 1;
+  return s;
+}
+
+// The weight gradients' rows: three workgroups for each compute unit, at least eight k tiles each.
+struct WeightShape { int tile, splits; int64_t rows_per_split, part_elems; };
 WeightShape weight_shape(const cgtp_gff_args* a) {
   WeightShape s;
-  const int64_t th = ceil_div(a->hidden, kGemmTile), ti = ceil_div(a->c_in, kGemmTile), to = ceil_div(a->c_out, kGemmTile);
-  s.tiles = (int)(th * (2 * ti + to));
-  s.part_elems = (int64_t)a->hidden * (2 * a->c_in + a->c_out);
+  auto tiles = [&](int t) { return ceil_div(a->hidden, t) * (2 * ceil_div(a->c_in, t) + ceil_div(a->c_out, t)); };
   const int depth = a->dtype == CGTP_F32 ? 32 : 64;
-  int64_t splits = std::max<int64_t>(1, 768 / s.tiles);
-  splits = std::max<int64_t>(1, std::min(splits, ceil_div(a->n_rows, 8 * depth)));
+  const int64_t most = ceil_div(a->n_rows, 8 * depth);
+  s.tile = small_tiles(tiles(128) * most) ? 64 : 128;
+  s.part_elems = (int64_t)a->hidden * (2 * a->c_in + a->c_out);
+  int64_t splits = std::max<int64_t>(1, std::min(std::max<int64_t>(1, 768 / tiles(s.tile)), most));
   if (splits > 8) splits = splits / 8 * 8;           // a range's tiles run on one XCD: as many ranges for each of the eight
   s.rows_per_split = ceil_div(ceil_div(a->n_rows, splits), depth) * depth;
   s.splits = (int)std::max<int64_t>(1, ceil_div(a->n_rows, std::max<int64_t>(1, s.rows_per_split)));
   return s;
+}
+
+int64_t k_tiles_of(const cgtp_gff_args* a) { return ceil_div(a->hidden, a->dtype == CGTP_F32 ? 32 : 64); }
+
+int64_t workspace_of(const cgtp_gff_args* a, bool backward) {
+  auto rows = [&](int N, int64_t k_tiles) {
+    const RowsShape s = rows_shape<float>(a->n_rows, N, k_tiles);
+    return s.splits > 1 ? s.splits * a->n_rows * N * 4 : 0;
+  };
+  if (!backward) return a->n_rows <= kFewRows ? 0 : rows(a->c_out, k_tiles_of(a));
+  const WeightShape w = weight_shape(a);
+  return std::max(rows(a->c_in, 2 * k_tiles_of(a)), w.splits > 1 ? w.splits * w.part_elems * 4 : 0);
 }
 
 // The kernel of an activation: a branch on it for each element costs more than the activation.
@@ -287,63 +431,110 @@ Kernel for_act(int act, Of&& of) {
   if (act == CGTP_ACT_GELU) return of(std::integral_constant<int, CGTP_ACT_GELU>{});
   return of(std::integral_constant<int, CGTP_ACT_SIGMOID>{});
 }
+template <typename Kernel, typename Of>
+Kernel for_tile(int tile, bool fast, Of&& of) {
+  typedef std::integral_constant<int, 64> small;
+  typedef std::integral_constant<int, 128> large;
+  if (tile == 64) return fast ? of(small{}, std::true_type{}) : of(small{}, std::false_type{});
+  return fast ? of(large{}, std::true_type{}) : of(large{}, std::false_type{});
+}
+
+template <typename T>
+void add_launch(const AddArgs<T>& a, hipStream_t s) {
+  hipLaunchKernelGGL(gff_add_kernel<T>, dim3((unsigned)ceil_div(a.elems, 256)), dim3(256), 0, s, a);
+}
+
+template <typename T, bool KB>
+void rows_launch(RowsArgs<T> d, bool fast, void* workspace, hipStream_t s) {
+  const RowsShape shape = rows_shape<T>(d.n_rows, d.N, d.segments * ceil_div(d.K, GemmType<T>::kDepth));
+  d.splits = shape.splits;
+  d.parts = (float*)workspace;
+  auto kern = for_tile<void (*)(RowsArgs<T>)>(shape.tile, fast, [](auto tile, auto is_fast) {
+    return gff_rows_kernel<T, decltype(tile)::value, decltype(is_fast)::value, KB>;
+  });
+  const int64_t mt = ceil_div(d.n_rows, shape.tile), nt = ceil_div(d.N, shape.tile);
+  hipLaunchKernelGGL(kern, dim3(tile_grid(mt, nt * d.splits)), dim3(kGemmThreads), 0, s, d);
+  if (d.splits > 1) add_launch(AddArgs<T>{d.parts, {d.out, nullptr, nullptr}, {0, 0, 0}, d.n_rows * d.N, 1, d.splits}, s);
+}
+
+template <typename T, int ROWS>
+void few_launch(const cgtp_gff_args* a, hipStream_t s) {
+  const FewArgs<T> u = {(const T*)a->x, {(const T*)a->w_gate, (const T*)a->w_up}, (T*)a->gate, (T*)a->up, (T*)a->mid,
+                        (int)a->n_rows, a->c_in, a->hidden};
+  auto up = for_act<void (*)(FewArgs<T>)>(a->activation, [](auto act) { return gff_few_kernel<T, ROWS, 2, decltype(act)::value>; });
+  hipLaunchKernelGGL(up, dim3((unsigned)ceil_div(u.N, kFewCols)), dim3(256), 0, s, u);
+  const FewArgs<T> d = {(const T*)a->mid, {(const T*)a->w_down, nullptr}, nullptr, nullptr, (T*)a->out, (int)a->n_rows, a->hidden,
+                        a->c_out};
+  hipLaunchKernelGGL((gff_few_kernel<T, ROWS, 1, 0>), dim3((unsigned)ceil_div(d.N, kFewCols)), dim3(256), 0, s, d);
+}
 
 template <typename T>
 int gff_forward(const cgtp_gff_args* a, hipStream_t s) {
+  if (a->n_rows == 1) few_launch<T, 1>(a, s);
+  else if (a->n_rows <= kFewRows) few_launch<T, kFewRows>(a, s);
+  if (a->n_rows <= kFewRows) return launch_status();
   const bool fast = whole_groups(a);
-  const int64_t mt = ceil_div(a->n_rows, kGemmTile);
   const UpArgs<T> u = {(const T*)a->x, (const T*)a->w_gate, (const T*)a->w_up, (T*)a->gate, (T*)a->up, (T*)a->mid, a->n_rows,
                        a->c_in, a->hidden};
+  const int tile = small_tiles(ceil_div(a->n_rows, 128) * ceil_div(a->hidden, 64)) ? 64 : 128;
   auto up = for_act<void (*)(UpArgs<T>)>(a->activation, [&](auto act) {
-    return fast ? gff_up_kernel<T, true, decltype(act)::value> : gff_up_kernel<T, false, decltype(act)::value>;
+    return for_tile<void (*)(UpArgs<T>)>(tile, fast, [](auto t, auto is_fast) {
+      return gff_up_kernel<T, decltype(t)::value, decltype(is_fast)::value, decltype(act)::value>;
+    });
   });
-  hipLaunchKernelGGL(up, dim3(tile_grid(mt, ceil_div(a->hidden, 64))), dim3(kGemmThreads), 0, s, u);
-  const RowsArgs<T> d = {{(const T*)a->mid, nullptr}, {(const T*)a->w_down, nullptr}, (T*)a->out, a->n_rows, a->c_out, 1, a->hidden,
-                         a->c_out};
-  auto down = fast ? gff_rows_kernel<T, true, false> : gff_rows_kernel<T, false, false>;
-  hipLaunchKernelGGL(down, dim3(tile_grid(mt, ceil_div(a->c_out, kGemmTile))), dim3(kGemmThreads), 0, s, d);
+  hipLaunchKernelGGL(up, dim3(tile_grid(ceil_div(a->n_rows, tile), ceil_div(a->hidden, tile / 2))), dim3(kGemmThreads), 0, s, u);
+  rows_launch<T, false>(RowsArgs<T>{{(const T*)a->mid, nullptr}, {(const T*)a->w_down, nullptr}, (T*)a->out, nullptr, a->n_rows,
+                                    a->c_out, 1, a->hidden, a->c_out, 1}, fast, a->workspace, s);
   return launch_status();
 }
 
 template <typename T>
 int gff_backward(const cgtp_gff_args* a, hipStream_t s) {
   const bool fast = whole_groups(a);
-  const int64_t mt = ceil_div(a->n_rows, kGemmTile);
   if (a->n_rows > 0 && (a->grad_x || a->grad_w_gate || a->grad_w_up)) {
     const MidGradArgs<T> m = {(const T*)a->grad_out, (const T*)a->w_down, (const T*)a->gate, (const T*)a->up, (T*)a->grad_gate,
                               (T*)a->grad_up, a->n_rows, a->hidden, a->c_out};
+    const int tile = small_tiles(ceil_div(a->n_rows, 128) * ceil_div(a->hidden, 128)) ? 64 : 128;
     auto mid = for_act<void (*)(MidGradArgs<T>)>(a->activation, [&](auto act) {
-      return fast ? gff_mid_grad_kernel<T, true, decltype(act)::value> : gff_mid_grad_kernel<T, false, decltype(act)::value>;
+      return for_tile<void (*)(MidGradArgs<T>)>(tile, fast, [](auto t, auto is_fast) {
+        return gff_mid_grad_kernel<T, decltype(t)::value, decltype(is_fast)::value, decltype(act)::value>;
+      });
     });
-    hipLaunchKernelGGL(mid, dim3(tile_grid(mt, ceil_div(a->hidden, kGemmTile))), dim3(kGemmThreads), 0, s, m);
+    hipLaunchKernelGGL(mid, dim3(tile_grid(ceil_div(a->n_rows, tile), ceil_div(a->hidden, tile))), dim3(kGemmThreads), 0, s, m);
   }
-  if (a->n_rows > 0 && a->grad_x) {
-    const RowsArgs<T> d = {{(const T*)a->grad_gate, (const T*)a->grad_up}, {(const T*)a->w_gate, (const T*)a->w_up},
-                           (T*)a->grad_x, a->n_rows, a->hidden, 2, a->hidden, a->c_in};
-    auto back = fast ? gff_rows_kernel<T, true, true>
-                                                                         : gff_rows_kernel<T, false, true>;
-    hipLaunchKernelGGL(back, dim3(tile_grid(mt, ceil_div(a->c_in, kGemmTile))), dim3(kGemmThreads), 0, s, d);
-  }
+  if (a->n_rows > 0 && a->grad_x)
+    rows_launch<T, true>(RowsArgs<T>{{(const T*)a->grad_gate, (const T*)a->grad_up}, {(const T*)a->w_gate, (const T*)a->w_up},
+                                     (T*)a->grad_x, nullptr, a->n_rows, a->hidden, 2, a->hidden, a->c_in, 1}, fast, a->workspace, s);
   const WeightShape shape = weight_shape(a);
   WeightArgs<T> w = {};
+  AddArgs<T> sum = {};
   w.parts = (float*)a->workspace;
   w.n_rows = a->n_rows;
   w.rows_per_split = shape.rows_per_split;
   w.splits = shape.splits;
   auto job = [&](const void* l, const void* r, void* out, int M, int N) {
     if (!out) return;
-    w.job[w.jobs++] = {(const T*)l, (const T*)r, (T*)out, M, N, w.tiles, (int)ceil_div(N, kGemmTile), w.part_elems};
-    w.tiles += (int)(ceil_div(M, kGemmTile) * ceil_div(N, kGemmTile));
+    sum.out[w.jobs] = (T*)out;
+    sum.first[w.jobs] = w.part_elems;
+    w.job[w.jobs++] = {(const T*)l, (const T*)r, (T*)out, M, N, w.tiles, (int)ceil_div(N, shape.tile), w.part_elems};
+    w.tiles += (int)(ceil_div(M, shape.tile) * ceil_div(N, shape.tile));
     w.part_elems += (int64_t)M * N;
   };
   job(a->x, a->grad_gate, a->grad_w_gate, a->c_in, a->hidden);
   job(a->x, a->grad_up, a->grad_w_up, a->c_in, a->hidden);
   job(a->mid, a->grad_out, a->grad_w_down, a->hidden, a->c_out);
   if (w.jobs) {
-    auto weight = fast ? gff_weight_kernel<T, true> : gff_weight_kernel<T, false>;
+    auto weight = for_tile<void (*)(WeightArgs<T>)>(shape.tile, fast, [](auto t, auto is_fast) {
+      return gff_weight_kernel<T, decltype(t)::value, decltype(is_fast)::value>;
+    });
     hipLaunchKernelGGL(weight, dim3(tile_grid(w.splits, w.tiles)), dim3(kGemmThreads), 0, s, w);
-    if (w.splits > 1)
-      hipLaunchKernelGGL(gff_add_kernel<T>, dim3((unsigned)ceil_div(w.part_elems, 256)), dim3(256), 0, s, w);
+    if (w.splits > 1) {
+      sum.parts = w.parts;
+      sum.elems = w.part_elems;
+      sum.outs = w.jobs;
+      sum.splits = w.splits;
+      add_launch(sum, s);
+    }
   }
   return launch_status();
 }
@@ -353,11 +544,9 @@ int gff_backward(const cgtp_gff_args* a, hipStream_t s) {
 
 extern "C" {
 
-int64_t cgtp_gff_workspace_bytes(const cgtp_gff_args* a) {
+int64_t cgtp_gff_workspace_bytes(const cgtp_gff_args* a, int backward) {
   using namespace cgtp;
-  if (gff_check(a) != CGTP_OK) return 0;
-  const WeightShape s = weight_shape(a);
-  return s.splits > 1 ? s.splits * s.part_elems * 4 : 0;
+  return gff_check(a) == CGTP_OK && a->n_rows > 0 ? workspace_of(a, backward != 0) : 0;
 }
 
 int cgtp_gff_forward(const cgtp_gff_args* a, void* stream) {
@@ -365,6 +554,7 @@ int cgtp_gff_forward(const cgtp_gff_args* a, void* stream) {
   if (int rc = gff_check(a)) return rc;
   if (a->n_rows == 0) return CGTP_OK;
   if (!a->mid || !a->out || (!a->gate) != (!a->up)) return CGTP_ERR_NULL;
+  if (workspace_of(a, false) > 0 && !a->workspace) return CGTP_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   switch (a->dtype) {
     case CGTP_F32: return gff_forward<float>(a, s);
@@ -377,7 +567,7 @@ int cgtp_gff_backward(const cgtp_gff_args* a, void* stream) {
   using namespace cgtp;
   if (int rc = gff_check(a)) return rc;
   if (a->n_rows > 0 && (!a->grad_out || !a->gate || !a->up || !a->mid || !a->grad_gate || !a->grad_up)) return CGTP_ERR_NULL;
-  if (cgtp_gff_workspace_bytes(a) > 0 && !a->workspace) return CGTP_ERR_WORKSPACE;
+  if (cgtp_gff_workspace_bytes(a, 1) > 0 && !a->workspace) return CGTP_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   switch (a->dtype) {
     case CGTP_F32: return gff_backward<float>(a, s);

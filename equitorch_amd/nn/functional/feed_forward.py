@@ -37,6 +37,9 @@ def _forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, act: int, 
         gate, up, mid = None, None, torch.empty((n, h), dtype=x.dtype, device=x.device)
     a = _args(x, w_gate, w_up, w_down, mid, _lib.dtype_code(x.dtype), act)
     a.out, a.gate, a.up = out.data_ptr(), _lib.ptr(gate), _lib.ptr(up)
+    nbytes = _lib.lib.cgtp_gff_workspace_bytes(C.byref(a), 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    a.workspace = _lib.ptr(ws)
     _lib.check(_lib.lib.cgtp_gff_forward(C.byref(a), _lib.stream_ptr(x.device)), "cgtp_gff_forward")
     return out, gate, up, mid
 
@@ -67,7 +70,7 @@ class _GatedFeedForward(Function):
         a.gate, a.up, a.grad_out = gate.data_ptr(), up.data_ptr(), g.data_ptr()
         a.grad_gate, a.grad_up = g_gate.data_ptr(), g_up.data_ptr()
         a.grad_x, a.grad_w_gate, a.grad_w_up, a.grad_w_down = (_lib.ptr(t) for t in grads)
-        ws = torch.empty(_lib.lib.cgtp_gff_workspace_bytes(C.byref(a)), dtype=torch.uint8, device=x.device)
+        ws = torch.empty(_lib.lib.cgtp_gff_workspace_bytes(C.byref(a), 1), dtype=torch.uint8, device=x.device)
         a.workspace = ws.data_ptr()
         _lib.check(_lib.lib.cgtp_gff_backward(C.byref(a), _lib.stream_ptr(x.device)), "cgtp_gff_backward")
         return (*grads, None)

@@ -792,7 +792,7 @@ typedef struct {
   int64_t n_rows;
   int32_t c_in, hidden, c_out, activation, dtype, reserved_;
 } cgtp_gff_args;
-int64_t cgtp_gff_workspace_bytes(const cgtp_gff_args* args);
+int64_t cgtp_gff_workspace_bytes(const cgtp_gff_args* args, int backward);
 int cgtp_gff_forward(const cgtp_gff_args* args, void* stream);
 int cgtp_gff_backward(const cgtp_gff_args* args, void* stream);
 

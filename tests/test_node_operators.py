@@ -62,7 +62,7 @@ def test_feed_forward_codes(changed, forward, backward):
 
 def test_feed_forward_workspace():
     a = _gff(n_rows=100000, grad_w_gate=4096)
-    assert _lib.lib.cgtp_gff_workspace_bytes(C.byref(a)) > 0
+    assert _lib.lib.cgtp_gff_workspace_bytes(C.byref(a), 1) > 0
     assert _lib.lib.cgtp_gff_backward(C.byref(a), None) == WORKSPACE
 
 
