@@ -1,4 +1,4 @@
-// PyTorch C++ extension over the C ABI of libcgtp for the fused edge product (gather, channel-wise tensor product,
+// PyTorch C++ extension over the C ABI of libcgtp for the operators on node features (node_operators.h) and the fused edge product (gather, channel-wise tensor product,
 // segment sum; compiled table): the autograd node, the argument block, output and workspace allocation and the stream
 // lookup of one forward + backward live here instead of in Python, which is what a training step pays per call on the
 // host.  Everything numeric happens behind cgtp_uvu_fwd / cgtp_uvu_bwd (include/cgtp.h); this file holds no kernel.
@@ -284,6 +284,8 @@ at::Tensor opt(const c10::optional<at::Tensor>& t) { return t.has_value() ? *t :
 
 }  // namespace
 
+#include "node_operators.h"
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "torch C++ shim over libcgtp's C ABI for the fused edge tensor product";
   py::class_<EdgeHandle>(m, "EdgeHandle")
@@ -311,5 +313,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     fallbacks().push_back(std::move(fn));
     return (int64_t)fallbacks().size() - 1;
   }, "keeps a callable (grad_out, x, y, w, need_x, need_y, need_w) -> (gx, gy, gw) for gradients of higher order");
+  bind_node_operators(m);
   m.def("abi_version", []() { return cgtp_version(); });
 }

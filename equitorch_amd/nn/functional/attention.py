@@ -13,7 +13,7 @@ import torch
 from torch import Tensor
 from torch.autograd import Function
 
-from ... import _lib
+from ... import _lib, _shim
 from ..._lib import AttnArgs, CgtpError
 from .edge import _higher_order
 
@@ -131,7 +131,7 @@ class AttentionPlan:
         self.num_structures = len(self.len_q)
         self.num_queries, self.num_keys = int(self.len_q.sum()), int(self.len_k.sum())
         self._tables = {}
-        self._buckets = None
+        self._buckets = _Buckets(self.len_q, self.len_k, self.device)
 
     @classmethod
     def from_batch(cls, batch: Tensor, num_structures: Optional[int] = None) -> "AttentionPlan":
@@ -151,10 +151,28 @@ class AttentionPlan:
             self._tables[key] = _Tables(self, group, heads)
         return self._tables[key]
 
-    def buckets(self):
-        """Structures of similar length together, padded to the longest of each bucket, for the tensor expression:
-        ``(rows_q, keep_q, rows_k, keep_k)`` per bucket and the order that sorts the buckets' queries."""
-        if self._buckets is None:
+    def handle(self, mod, group: int, heads: int, scale: float, cap: float):
+        """The extension's copy of the tables, and the tensor expression its node evaluates under gradient mode."""
+        key = (group, heads, scale, cap)
+        if key not in self._tables:
+            t, buckets = self.tables(group, heads), self._buckets
+            h = mod.AttnHandle(t.q_items, t.q_joins, t.k_items, t.k_joins, t.q_slots, t.k_slots, t.wide_q, t.wide_k)
+            # holds the buckets, not the plan: the node keeps it for as long as it lives itself
+            h.set_fallback(lambda g, inputs, need: _higher_order(_of_buckets(buckets, scale, cap), inputs, need, g))
+            self._tables[key] = h
+        return self._tables[key]
+
+
+class _Buckets:
+    """Structures of similar length together, padded to the longest of each bucket, for the tensor expression; made on first
+    use."""
+
+    def __init__(self, len_q: np.ndarray, len_k: np.ndarray, device):
+        self.len_q, self.len_k, self.device, self._made = len_q, len_k, device, None
+
+    def get(self):
+        """``(rows_q, keep_q, rows_k, keep_k)`` per bucket and the order that sorts the buckets' queries."""
+        if self._made is None:
             start_q, start_k = np.cumsum(self.len_q) - self.len_q, np.cumsum(self.len_k) - self.len_k
             groups = {}
             for s in np.flatnonzero(self.len_q):
@@ -170,18 +188,24 @@ class AttentionPlan:
                 order.append(index[0][index[1]])
                 out.append(tuple(torch.from_numpy(i).to(self.device) for i in index))
             order = np.concatenate(order) if order else np.zeros(0, dtype=np.int64)
-            self._buckets = (out, torch.from_numpy(np.argsort(order)).to(self.device))
-        return self._buckets
+            self._made = (out, torch.from_numpy(np.argsort(order)).to(self.device))
+        return self._made
 
 
-def _expression(q, k, v, pos_q, pos_k, slope, plan: AttentionPlan, scale: float, cap: float):
+def _of_buckets(buckets: _Buckets, scale: float, cap: float):
+    def expression(q, k, v, pos_q, pos_k, slope):
+        return _expression(q, k, v, pos_q, pos_q if pos_k is None else pos_k, slope, buckets, scale, cap)
+    return expression
+
+
+def _expression(q, k, v, pos_q, pos_k, slope, padded: _Buckets, scale: float, cap: float):
     """The same result as a tensor expression on padded buckets of structures, which autograd differentiates to any order
     (in 32 bits)."""
     dtype, group = q.dtype, q.shape[1] // k.shape[1]
     if k.shape[0] == 0:                     # no keys at all: something to point at; nothing of it is kept
         k, v = k.new_zeros((1, *k.shape[1:])), v.new_zeros((1, *v.shape[1:]))
         pos_k = None if pos_k is None else pos_k.new_zeros((1, 3))
-    outs, (buckets, order) = [], plan.buckets()
+    outs, (buckets, order) = [], padded.get()
     for rows_q, keep_q, rows_k, keep_k in buckets:
         qb = q[rows_q].float().masked_fill(~keep_q[:, :, None, None], 0.0).transpose(1, 2)
         # padding points at some node: what that holds may not reach a result, not even as a zero times an infinity
@@ -248,8 +272,7 @@ class _SegmentAttention(Function):
         q, k, v, pos_q, pos_k, slope, out, lse = ctx.saved_tensors
         need, plan, scale, cap = ctx.needs_input_grad[:6], ctx.plan, ctx.scale, ctx.cap
         if torch.is_grad_enabled():
-            def expression(q, k, v, pos_q, pos_k, slope):
-                return _expression(q, k, v, pos_q, pos_q if pos_k is None else pos_k, slope, plan, scale, cap)
+            expression = _of_buckets(plan._buckets, scale, cap)
             return (*_higher_order(expression, (q, k, v, pos_q, pos_k, slope), need, g), None, None, None)
         g = g.contiguous()
         a = _args(q, k, v, pos_q, pos_q if pos_k is None else pos_k, slope, plan, scale, cap)
@@ -312,6 +335,11 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, pos:
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
     pos, pos_k, slope = (None if t is None else t.contiguous() for t in (pos, pos_k, slope))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, pos, pos_k, slope)):
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, pos, pos_k, slope))
+    mod = _shim.module()
+    if mod is not None:
+        handle = plan.handle(mod, q.shape[1] // k.shape[1], k.shape[1], scale, cap)
+        return mod.attn(q, k, v, pos, pos_k, slope, handle, scale, cap, keep)
+    if keep:
         return _SegmentAttention.apply(q, k, v, pos, pos_k, slope, plan, scale, cap)
     return _forward(q, k, v, pos, pos if pos_k is None else pos_k, slope, plan, scale, cap, False)[0]

@@ -6,7 +6,7 @@ import torch
 from torch import Tensor
 from torch.autograd import Function
 
-from ... import _lib
+from ... import _lib, _shim
 from ..._lib import CgtpError
 
 
@@ -68,6 +68,9 @@ def embedding(kind: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
         raise CgtpError(f"kind is on {kind.device}, table on {table.device}")
     _lib.dtype_code(table.dtype)
     kind, table = kind.contiguous(), table.contiguous()
+    mod = _shim.module()
+    if mod is not None:
+        return mod.embed(kind, table, float(scale))
     if torch.is_grad_enabled() and table.requires_grad:
         return _Embedding.apply(kind, table, float(scale))
     return _lookup(kind, table, float(scale))

@@ -10,7 +10,7 @@ import torch
 from torch import Tensor
 from torch.autograd import Function
 
-from ... import _lib
+from ... import _lib, _shim
 from ..._lib import CgtpError, GffArgs
 from .edge import _higher_order
 
@@ -44,6 +44,26 @@ def _forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, act: int, 
     return out, gate, up, mid
 
 
+def _expression(act: int):
+    fn = _EXPRESSIONS[act]
+
+    def expression(x, wg, wu, wd):
+        dtype = x.dtype
+        x, wg, wu, wd = (t.float() for t in (x, wg, wu, wd))
+        return ((fn(x @ wg) * (x @ wu)) @ wd).to(dtype)
+    return expression
+
+
+_fallbacks = {}
+
+
+def _fallback(mod, act: int):
+    """The extension's number for the tensor expression of an activation, which a backward under gradient mode evaluates."""
+    if act not in _fallbacks:
+        _fallbacks[act] = mod.Fallback(lambda g, inputs, need: _higher_order(_expression(act), inputs, need, g))
+    return _fallbacks[act]
+
+
 class _GatedFeedForward(Function):
     @staticmethod
     def forward(ctx, x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, act: int):
@@ -57,12 +77,7 @@ class _GatedFeedForward(Function):
         x, w_gate, w_up, w_down, gate, up, mid = ctx.saved_tensors
         need = ctx.needs_input_grad[:4]
         if torch.is_grad_enabled():
-            fn, dtype = _EXPRESSIONS[ctx.act], x.dtype
-
-            def expression(x, wg, wu, wd):
-                x, wg, wu, wd = (t.float() for t in (x, wg, wu, wd))
-                return ((fn(x @ wg) * (x @ wu)) @ wd).to(dtype)
-            return (*_higher_order(expression, (x, w_gate, w_up, w_down), need, g), None)
+            return (*_higher_order(_expression(ctx.act), (x, w_gate, w_up, w_down), need, g), None)
         g = g.contiguous()
         grads = [torch.empty_like(t) if n else None for t, n in zip((x, w_gate, w_up, w_down), need)]
         g_gate, g_up = torch.empty((2, *mid.shape), dtype=x.dtype, device=x.device)
@@ -100,7 +115,11 @@ def gated_feed_forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, 
     flat = x.reshape(-1, c).contiguous()
     weights = [t.contiguous() for t in (w_gate, w_up, w_down)]
     act = _ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    keep = torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    mod = _shim.module()
+    if mod is not None:
+        out = mod.gff(flat, *weights, act, keep, _fallback(mod, act))
+    elif keep:
         out = _GatedFeedForward.apply(flat, *weights, act)
     else:
         out = _forward(flat, *weights, act, False)[0]

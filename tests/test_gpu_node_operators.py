@@ -437,3 +437,41 @@ def test_gated_feed_forward_refuses(device):
                 (x, wg, wu, wd, "relu")):
         with pytest.raises(CgtpError):
             gated_feed_forward(*bad)
+
+
+def test_extension_and_ctypes_issue_the_same_launches(device):
+    """With the C++ extension's autograd nodes and without it: the same bits, and a second order either way, also when nobody
+    holds the plan any more."""
+    from equitorch_amd import _shim
+    from equitorch_amd.nn.functional import AttentionPlan, embedding, gated_feed_forward, segment_attention
+    assert _shim.module() is not None, "the extension is not built"
+    gen = torch.Generator().manual_seed(21)
+    n = 60
+    kind = torch.randint(0, 7, (n,), generator=gen).to(device)
+    data = [_rand(gen, 7, 32), _rand(gen, n, 3), torch.rand(2, generator=gen), _rand(gen, 32, 40, std=0.2), _rand(gen, 32, 40, std=0.2),
+            _rand(gen, 40, 32, std=0.2)]
+    seen = []
+    for use_shim in (True, False):
+        saved = _shim._module
+        if not use_shim:
+            _shim._module = None
+        try:
+            t = [d.to(device).requires_grad_(True) for d in data]
+            x = embedding(kind, t[0], 2.0)
+            assert ("Cpp" in type(x.grad_fn).__name__) == use_shim
+            h = x.view(n, 2, 16)
+            y = segment_attention(h, h, h, AttentionPlan(torch.tensor([0, 25, n], device=device)), pos=t[1], slope=t[2], cap=5.0)
+            y = gated_feed_forward(y.reshape(n, 32), *t[3:])
+            energy = (y * y).sum()
+            first = torch.autograd.grad(energy, t, retain_graph=True)
+            forces = torch.autograd.grad(energy, t[1], create_graph=True)[0]
+            second = torch.autograd.grad((forces * forces).sum(), t)
+            with torch.no_grad():
+                again = gated_feed_forward(y.detach(), *t[3:])
+        finally:
+            _shim._module = saved
+        seen.append([y, *first, again, forces, *second])
+    for a, b in zip(seen[0][:-7], seen[1][:-7]):
+        assert torch.equal(a, b)
+    for a, b in zip(seen[0][-7:], seen[1][-7:]):            # tensor expressions: sums of the library's own order
+        assert torch.allclose(a, b, rtol=1e-4, atol=1e-5 * float(b.abs().max()))

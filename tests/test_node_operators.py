@@ -172,7 +172,7 @@ def test_expression_of_the_attention_is_the_definition():
     pos, pos_k, slope = torch.randn(11, 3, generator=gen), torch.randn(16, 3, generator=gen), torch.rand(4, generator=gen)
     pos_k[15] = pos[10]
     ptr = lambda n: torch.tensor([0] + n).cumsum(0)
-    got = _expression(q, k, v, pos, pos_k, slope, AttentionPlan(ptr(len_q), ptr(len_k)), 0.4, 3.0)
+    got = _expression(q, k, v, pos, pos_k, slope, AttentionPlan(ptr(len_q), ptr(len_k))._buckets, 0.4, 3.0)
     want, a, b = torch.zeros_like(q), 0, 0
     for lq, lk in zip(len_q, len_k):
         for h in range(4):
