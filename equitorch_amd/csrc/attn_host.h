@@ -17,7 +17,7 @@ struct AttnScratch {
   float* delta;        // (n_q, h_q)
   f32x4* row_part;     // (n_q, h_q): a row's part of the gradient of its query's position and of its head's slope
   f32x4* key_part;     // (n_k, h_kv): of the key's position
-  float* slope_part;   // (blocks, h_q)
+  float* slope_part;   // (h_q, blocks)
   float* parts;        // partial results of pieces
 };
 

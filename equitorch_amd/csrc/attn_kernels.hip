@@ -8,36 +8,68 @@
 namespace cgtp {
 namespace {
 
-// Gradient of the positions of 64 nodes: the parts of their rows (as queries) and of their head of keys (as keys, where the
-// positions are one tensor), heads in order; and the 64 queries' part of the gradient of every slope.
-constexpr int kPosNodes = 64;
-__global__ void __launch_bounds__(256) attn_pos_kernel(cgtp_attn_args a, AttnScratch w) {
-  const int64_t i0 = (int64_t)blockIdx.x * kPosNodes;
-  const int n = (int)(a.n_q - i0 < kPosNodes ? a.n_q - i0 : kPosNodes);
-  if (a.grad_pos_q && threadIdx.x < 192) {
-    const int i = threadIdx.x / 3, d = threadIdx.x % 3;
-    if (i < n) {
+// Gradient of the positions of kPosNodes nodes: the parts of their rows (as queries) and of their heads of keys (as keys, where
+// the positions are one tensor); and the queries' part of the gradient of every slope.  Eight lanes for a node, a head each at a
+// time, added in a fixed order.
+constexpr int kPosNodes = 128;
+__device__ __forceinline__ void add_heads(const f32x4* part, int64_t node, int heads, int lane8, bool ok, float (&s)[3]) {
+  for (int h = lane8; h < heads; h += 8) {
+    if (!ok) continue;
+    const f32x4 v = part[node * heads + h];
+#pragma unroll
+    for (int d = 0; d < 3; ++d) s[d] += v[d];
+  }
+}
+__device__ __forceinline__ void write_pos(float* out, int64_t node, int lane8, bool ok, float (&s)[3]) {
+#pragma unroll
+  for (int d = 0; d < 3; ++d) s[d] = group_sum(s[d], 8);
+  if (ok && lane8 < 3) out[node * 3 + lane8] = lane8 == 0 ? s[0] : lane8 == 1 ? s[1] : s[2];
+}
+__global__ void __launch_bounds__(1024) attn_pos_kernel(cgtp_attn_args a, AttnScratch w) {
+  __shared__ float sums[1024];
+  const int lane8 = threadIdx.x & 7, sub = threadIdx.x >> 3;
+  const int64_t node = (int64_t)blockIdx.x * kPosNodes + sub;
+  const bool ok = node < a.n_q;
+  if (a.grad_pos_q) {
+    float s[3] = {};
+    add_heads(w.row_part, node, a.h_q, lane8, ok, s);
+    if (a.same_pos) add_heads(w.key_part, node, a.h_kv, lane8, ok, s);
+    write_pos(a.grad_pos_q, node, lane8, ok, s);
+  }
+  if (!a.grad_slope) return;
+  for (int h0 = 0; h0 < a.h_q; h0 += 8) {
+    const int h = h0 + lane8;
+    __syncthreads();
+    sums[lane8 * kPosNodes + sub] = ok && h < a.h_q ? w.row_part[node * a.h_q + h][3] : 0.f;
+    __syncthreads();
+    // a head's 128 values: 16 lanes take eight each
+    if (threadIdx.x < 128) {
+      const int which = threadIdx.x >> 4, l = threadIdx.x & 15;
       float s = 0.f;
-      for (int h = 0; h < a.h_q; ++h) s += ((const float*)&w.row_part[(i0 + i) * a.h_q + h])[d];
-      if (a.same_pos)
-        for (int h = 0; h < a.h_kv; ++h) s += ((const float*)&w.key_part[(i0 + i) * a.h_kv + h])[d];
-      a.grad_pos_q[(i0 + i) * 3 + d] = s;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += sums[which * kPosNodes + i * 16 + l];
+      s = group_sum(s, 16);
+      if (l == 0 && h0 + which < a.h_q) w.slope_part[(int64_t)(h0 + which) * gridDim.x + blockIdx.x] = s;
     }
   }
-  if (a.grad_slope)
-    for (int h = threadIdx.x; h < a.h_q; h += 256) {
-      float s = 0.f;
-      for (int i = 0; i < n; ++i) s += w.row_part[(i0 + i) * a.h_q + h][3];
-      w.slope_part[(int64_t)blockIdx.x * a.h_q + h] = s;
-    }
 }
-__global__ void __launch_bounds__(192) attn_pos_k_kernel(cgtp_attn_args a, AttnScratch w) {
-  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x / 3;
-  const int d = threadIdx.x % 3;
-  if (i >= a.n_k) return;
+__global__ void __launch_bounds__(1024) attn_pos_k_kernel(cgtp_attn_args a, AttnScratch w) {
+  const int lane8 = threadIdx.x & 7;
+  const int64_t node = (int64_t)blockIdx.x * kPosNodes + (threadIdx.x >> 3);
+  float s[3] = {};
+  add_heads(w.key_part, node, a.h_kv, lane8, node < a.n_k, s);
+  write_pos(a.grad_pos_k, node, lane8, node < a.n_k, s);
+}
+// A workgroup per head: its blocks' parts, each thread every 256th in order, then the threads'.
+__global__ void __launch_bounds__(256) attn_slope_kernel(float* out, const float* __restrict__ part, int blocks) {
+  __shared__ float sums[4];
   float s = 0.f;
-  for (int h = 0; h < a.h_kv; ++h) s += ((const float*)&w.key_part[i * a.h_kv + h])[d];
-  a.grad_pos_k[i * 3 + d] = s;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < blocks; i += 256) s += part[(int64_t)blockIdx.x * blocks + i];
+  s = group_sum(s, 64);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) out[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
 int64_t blocks_of(int64_t n) { return (n + kPosNodes - 1) / kPosNodes; }
@@ -145,10 +177,11 @@ int cgtp_attn_backward(const cgtp_attn_args* a, void* stream) {
   if (a->slope) {
     const unsigned blocks = (unsigned)blocks_of(a->n_q);
     if (blocks && (a->grad_pos_q || a->grad_slope))
-      hipLaunchKernelGGL(attn_pos_kernel, dim3(blocks), dim3(256), 0, s, *a, w);
-    if (a->grad_slope) launch_partial_sum<float>(w.slope_part, a->grad_slope, blocks, a->h_q, s);
+      hipLaunchKernelGGL(attn_pos_kernel, dim3(blocks), dim3(1024), 0, s, *a, w);
+    if (a->grad_slope)
+      hipLaunchKernelGGL(attn_slope_kernel, dim3((unsigned)a->h_q), dim3(256), 0, s, a->grad_slope, (const float*)w.slope_part, (int)blocks);
     if (!a->same_pos && a->grad_pos_k && a->n_k > 0)
-      hipLaunchKernelGGL(attn_pos_k_kernel, dim3((unsigned)blocks_of(a->n_k)), dim3(192), 0, s, *a, w);
+      hipLaunchKernelGGL(attn_pos_k_kernel, dim3((unsigned)blocks_of(a->n_k)), dim3(1024), 0, s, *a, w);
   }
   return hipGetLastError() == hipSuccess ? CGTP_OK : CGTP_ERR_LAUNCH;
 }

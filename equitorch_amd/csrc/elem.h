@@ -39,6 +39,19 @@ __device__ __forceinline__ void store_elems(T* p, const A (&src)[V]) {
   }
 }
 
+// The same past the caches' keep: what is written once should not displace what is read again.
+template <typename T, int V, typename A>
+__device__ __forceinline__ void store_elems_stream(T* p, const A (&src)[V]) {
+  if constexpr (V == 1) {
+    p[0] = (T)src[0];
+  } else {
+    typename ElemVec<T, V>::type v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (T)src[i];
+    __builtin_nontemporal_store(v, reinterpret_cast<typename ElemVec<T, V>::type*>(p));
+  }
+}
+
 typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
