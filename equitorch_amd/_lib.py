@@ -159,6 +159,7 @@ class AttnArgs(C.Structure):
                 ("q_node", C.c_int64), ("q_head", C.c_int64), ("k_node", C.c_int64), ("k_head", C.c_int64),
                 ("v_node", C.c_int64), ("v_head", C.c_int64),
                 ("pos_q", C.c_void_p), ("pos_k", C.c_void_p), ("slope", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+                ("out_low", C.c_void_p),
                 ("q_items", C.c_void_p), ("q_joins", C.c_void_p), ("k_items", C.c_void_p), ("k_joins", C.c_void_p),
                 ("n_q_items", C.c_int32), ("n_q_joins", C.c_int32), ("n_q_slots", C.c_int32),
                 ("n_k_items", C.c_int32), ("n_k_joins", C.c_int32), ("n_k_slots", C.c_int32),
@@ -166,7 +167,7 @@ class AttnArgs(C.Structure):
                 ("grad_pos_q", C.c_void_p), ("grad_pos_k", C.c_void_p), ("grad_slope", C.c_void_p), ("workspace", C.c_void_p),
                 ("n_q", C.c_int64), ("n_k", C.c_int64), ("h_q", C.c_int32), ("h_kv", C.c_int32), ("dim", C.c_int32),
                 ("dtype", C.c_int32), ("wide_q", C.c_int32), ("wide_k", C.c_int32), ("same_pos", C.c_int32),
-                ("reserved_", C.c_int32), ("scale", C.c_float), ("cap", C.c_float)]
+                ("together", C.c_int32), ("scale", C.c_float), ("cap", C.c_float)]
 
 
 def _load():

@@ -230,18 +230,19 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
   }
 }
 
-// Adds the parts of a row: a workgroup for each (tile, head of keys, row), its slots shared out over slices of threads.
+// Adds the parts of a row: a workgroup for each (tile, head, row), its slots shared out over slices of threads.  heads: of keys,
+// each with its group of query heads in the rows, or of queries.
 constexpr int kJoinThreads = 1024;
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) attn_fwd_join_kernel(AttnLaunch a, const float* __restrict__ parts, int rows) {
+__global__ void __launch_bounds__(kJoinThreads) attn_fwd_join_kernel(AttnLaunch a, const float* __restrict__ parts, int rows, int heads) {
   __shared__ float acc[kJoinThreads], red[kJoinThreads / kWave];
-  const int group = a.h_q / a.h_kv, rr = blockIdx.x % rows, hk = blockIdx.x / rows % a.h_kv;
-  const cgtp_attn_item it = a.q_joins[blockIdx.x / rows / a.h_kv];
+  const int group = a.h_q / heads, rr = blockIdx.x % rows, hk = blockIdx.x / rows % heads;
+  const cgtp_attn_item it = a.q_joins[blockIdx.x / rows / heads];
   const Row row = row_of(it, it.row_begin + rr, hk, group);
   if (!row.ok) return;
   const int tid = threadIdx.x, width = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128, slices = kJoinThreads / width;
-  const int64_t step = (int64_t)a.h_kv * rows * (a.dim + 2);
-  const float* p = parts + (((int64_t)it.first * a.h_kv + hk) * rows + rr) * (a.dim + 2);
+  const int64_t step = (int64_t)heads * rows * (a.dim + 2);
+  const float* p = parts + (((int64_t)it.first * heads + hk) * rows + rr) * (a.dim + 2);
   float top = -INFINITY;
   for (int s = tid; s < it.count; s += kJoinThreads) top = fmaxf(top, p[s * step + a.dim]);
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
@@ -272,8 +273,46 @@ __global__ void __launch_bounds__(kJoinThreads) attn_fwd_join_kernel(AttnLaunch 
   for (int s = 0; s < slices; ++s) sum += acc[s * width];
   const bool some = sum > 0.f || sum != sum;
   const int64_t at = (int64_t)row.query * a.h_q + row.head;
-  if (d < a.dim) ((T*)a.out)[at * a.dim + d] = (T)(some ? total / sum : 0.f);
+  if (d < a.dim) {
+    const float o = some ? total / sum : 0.f;
+    ((T*)a.out)[at * a.dim + d] = (T)o;
+    if (sizeof(T) == 2 && a.out_low) ((T*)a.out_low)[at * a.dim + d] = (T)(o - (float)(T)o);
+  }
   if (a.lse && tid == 0) ((float*)a.lse)[at] = some ? top + __log2f(sum) : INFINITY;
+}
+
+// The same where a row has few slots: a workgroup for each (tile, head), an element to a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_fwd_join_few_kernel(AttnLaunch a, const float* __restrict__ parts, int rows, int heads) {
+  const int group = a.h_q / heads, hk = blockIdx.x % heads, width = a.dim + 1;
+  const cgtp_attn_item it = a.q_joins[blockIdx.x / heads];
+  const int here = it.row_end - it.row_begin;
+  const int64_t step = (int64_t)heads * rows * (a.dim + 2);
+  for (int e = blockIdx.y * 256 + threadIdx.x; e < here * width; e += gridDim.y * 256) {
+    const int r = e / width, d = e % width;
+    const float* p = parts + (((int64_t)it.first * heads + hk) * rows + r) * (a.dim + 2);
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int k = 0; k < it.count; ++k) top = fmaxf(top, p[k * step + a.dim]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float o = 0.f, sum = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < it.count; ++k) {
+      const float by = exp2_fast(p[k * step + a.dim] - base);
+      sum += by * p[k * step + a.dim + 1];
+      o += by * p[k * step + d];             // the last element is not used
+    }
+    const bool some = sum > 0.f || sum != sum;
+    const Row row = row_of(it, it.row_begin + r, hk, group);
+    const int64_t at = (int64_t)row.query * a.h_q + row.head;
+    if (d < a.dim) {
+      o = some ? o / sum : 0.f;
+      ((T*)a.out)[at * a.dim + d] = (T)o;
+      if (sizeof(T) == 2 && a.out_low) ((T*)a.out_low)[at * a.dim + d] = (T)(o - (float)(T)o);
+    } else if (a.lse) {
+      ((float*)a.lse)[at] = some ? top + __log2f(sum) : INFINITY;
+    }
+  }
 }
 
 // A row's sums over its keys besides its gradient, and its delta.
@@ -437,6 +476,7 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
   }
 }
 
+// One row to a workgroup: the sums that end with a factor of the row.
 template <typename T>
 __global__ void __launch_bounds__(192) attn_bwd_q_join_kernel(AttnLaunch a, AttnScratch w, int rows) {
   __shared__ float sums[kQSums];
@@ -603,48 +643,95 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(512) attn_bwd_k_join_kernel(AttnLaunch a, AttnScratch w, int rows) {
-  const int kk = blockIdx.x % rows, hk = blockIdx.x / rows % a.h_kv;
-  const cgtp_attn_item it = a.k_joins[blockIdx.x / rows / a.h_kv];
-  const int key = it.k_begin + kk, d = threadIdx.x, width = 2 * a.dim + 4;
-  if (key >= it.k_end || d >= width) return;
-  const int64_t step = (int64_t)a.h_kv * rows * width, at = (int64_t)key * a.h_kv + hk;
-  const float* p = w.parts + (((int64_t)it.first * a.h_kv + hk) * rows + kk) * width + d;
-  float s = 0.f;
-#pragma unroll 8
-  for (int k = 0; k < it.count; ++k) s += p[k * step];
-  if (d < a.dim) {
-    if (a.grad_k) ((T*)a.grad_k)[at * a.dim + d] = (T)s;
-  } else if (d < 2 * a.dim) {
-    if (a.grad_v) ((T*)a.grad_v)[at * a.dim + d - a.dim] = (T)s;
-  } else if (a.slope) {
-    ((float*)&w.key_part[at])[d - 2 * a.dim] = s;
+// Adds the parts of a tile's rows or keys, `width` values for each: a workgroup for each (tile, head), an element of the tile to
+// a thread, its slots in order.  put(row or key, element, sum).
+template <typename Put>
+__device__ __forceinline__ void join_elements(const float* parts, const cgtp_attn_item& it, int head, int heads, int tile, int here,
+                                              int width, Put&& put) {
+  const int64_t step = (int64_t)heads * tile * width;
+  const float* p = parts + ((int64_t)it.first * heads + head) * tile * width;
+  for (int e = blockIdx.y * 256 + threadIdx.x; e < here * width; e += gridDim.y * 256) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < it.count; ++k) s += p[k * step + e];
+    put(e / width, e % width, s);
   }
 }
+template <typename T>
+__global__ void __launch_bounds__(256) attn_bwd_k_join_kernel(cgtp_attn_args a, AttnScratch w, int tile) {
+  const int hk = blockIdx.x % a.h_kv;
+  const cgtp_attn_item it = a.k_joins[blockIdx.x / a.h_kv];
+  join_elements(w.parts, it, hk, a.h_kv, tile, it.k_end - it.k_begin, 2 * a.dim + 4, [&](int key, int d, float s) {
+    const int64_t at = (int64_t)(it.k_begin + key) * a.h_kv + hk;
+    if (d < a.dim) {
+      if (a.grad_k) ((T*)a.grad_k)[at * a.dim + d] = (T)s;
+    } else if (d < 2 * a.dim) {
+      if (a.grad_v) ((T*)a.grad_v)[at * a.dim + d - a.dim] = (T)s;
+    } else if (a.slope) {
+      ((float*)&w.key_part[at])[d - 2 * a.dim] = s;
+    }
+  });
+}
+
+}  // namespace
+}  // namespace cgtp
+
+#include "attn_heads.h"
+
+namespace cgtp {
+namespace {
 
 // ---- launches -----------------------------------------------------------------------------------------------------
+unsigned groups_of(int heads, int each) { return (unsigned)((heads + each - 1) / each); }
+
 template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
 void q_launch(const AttnLaunch& a, const AttnScratch* w, hipStream_t s) {
-  const dim3 grid((unsigned)a.n_q_items * a.h_kv), joins((unsigned)a.n_q_joins * a.h_kv * kRowsOf<NW>);
   float* parts = (float*)a.workspace;
-  if (a.n_q_items) {
-    if (w) hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NW, BIASED, CAPPED>), grid, dim3(64 * NW), 0, s, a, *w);
-    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, BIASED, CAPPED>), grid, dim3(64 * NW), 0, s, a, parts);
+  const bool together = BIASED && DP <= 64 && a.together;
+  const int heads = together ? a.h_q : a.h_kv;
+  const unsigned joins = (unsigned)a.n_q_joins * heads;
+  const dim3 threads(64 * NW);
+  if (a.n_q_items && together) {
+    if constexpr (BIASED && DP <= 64) {
+      const unsigned n = (unsigned)a.n_q_items;
+      if (w)
+        hipLaunchKernelGGL((attn_heads_bwd_q_kernel<T, DP, NW, CAPPED>), dim3(n * groups_of(a.h_q, kHeads)), threads, 0, s, a, *w);
+      else
+        hipLaunchKernelGGL((attn_heads_fwd_kernel<T, DP, NW, CAPPED>), dim3(n * groups_of(a.h_q, kHeads)), threads, 0, s, a, parts);
+    }
+  } else if (a.n_q_items) {
+    const dim3 grid((unsigned)a.n_q_items * a.h_kv);
+    if (w) hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NW, BIASED, CAPPED>), grid, threads, 0, s, a, *w);
+    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, BIASED, CAPPED>), grid, threads, 0, s, a, parts);
   }
-  if (a.n_q_joins) {
-    if (w) hipLaunchKernelGGL((attn_bwd_q_join_kernel<T>), joins, dim3(192), 0, s, a, *w, kRowsOf<NW>);
-    else hipLaunchKernelGGL((attn_fwd_join_kernel<T>), joins, dim3(kJoinThreads), 0, s, a, (const float*)parts, kRowsOf<NW>);
+  if (!joins) return;
+  if (w) {
+    if (together) hipLaunchKernelGGL((attn_heads_bwd_q_join_kernel<T>), dim3(joins, 8), dim3(256), 0, s, a, *w, kRowsOf<NW>);
+    else hipLaunchKernelGGL((attn_bwd_q_join_kernel<T>), dim3(joins * kRowsOf<NW>), dim3(192), 0, s, a, *w, kRowsOf<NW>);
+  } else if (a.n_q_slots > 16 * a.n_q_joins) {
+    // a row's slots are shared out over a workgroup where they are many, else an element's slots are a thread's
+    hipLaunchKernelGGL((attn_fwd_join_kernel<T>), dim3(joins * kRowsOf<NW>), dim3(kJoinThreads), 0, s, a, (const float*)parts,
+                       kRowsOf<NW>, heads);
+  } else {
+    hipLaunchKernelGGL((attn_fwd_join_few_kernel<T>), dim3(joins, 8), dim3(256), 0, s, a, (const float*)parts, kRowsOf<NW>, heads);
   }
 }
 template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
 void k_launch(const AttnLaunch& a, const AttnScratch& w, hipStream_t s) {
-  if (a.n_k_items)
-    hipLaunchKernelGGL((attn_bwd_k_kernel<T, DP, NW, BIASED, CAPPED>), dim3((unsigned)a.n_k_items * a.h_kv), dim3(64 * NW), 0, s,
-                       a, w);
+  const unsigned n = (unsigned)a.n_k_items;
+  const dim3 threads(64 * NW);
+  if (n && BIASED && DP <= 64 && a.together) {
+    if constexpr (BIASED && DP <= 64) {
+      if (a.h_q == a.h_kv)
+        hipLaunchKernelGGL((attn_heads_bwd_k_kernel<T, DP, NW, CAPPED, false>), dim3(n * groups_of(a.h_kv, kHeads)), threads, 0, s, a, w);
+      else
+        hipLaunchKernelGGL((attn_heads_bwd_k_kernel<T, DP, NW, CAPPED, true>), dim3(n * (unsigned)a.h_kv), threads, 0, s, a, w);
+    }
+  } else if (n) {
+    hipLaunchKernelGGL((attn_bwd_k_kernel<T, DP, NW, BIASED, CAPPED>), dim3(n * (unsigned)a.h_kv), threads, 0, s, a, w);
+  }
   if (a.n_k_joins)
-    hipLaunchKernelGGL((attn_bwd_k_join_kernel<T>), dim3((unsigned)a.n_k_joins * a.h_kv * kRowsOf<NW>), dim3(512), 0, s, a, w,
-                       kRowsOf<NW>);
+    hipLaunchKernelGGL((attn_bwd_k_join_kernel<T>), dim3((unsigned)a.n_k_joins * a.h_kv, 8), dim3(256), 0, s, a, w, kRowsOf<NW>);
 }
 template <typename T, int DP, bool BIASED, bool CAPPED>
 void launch_dim(const AttnLaunch& a, const AttnScratch* w, hipStream_t s) {

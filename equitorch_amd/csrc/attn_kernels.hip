@@ -74,6 +74,11 @@ __global__ void __launch_bounds__(256) attn_slope_kernel(float* out, const float
 
 int64_t blocks_of(int64_t n) { return (n + kPosNodes - 1) / kPosNodes; }
 
+// Rows that leave partial results.
+int64_t q_parts(const cgtp_attn_args& a) {
+  return (int64_t)a.n_q_slots * (a.together ? a.h_q : a.h_kv) * cgtp_attn_rows(a.wide_q);
+}
+
 // Workspace of the backward; every buffer starts at a multiple of 256 bytes.  The pieces' results of the two passes share a place.
 struct AttnLayout { int64_t row_part, key_part, slope_part, parts, bytes; };
 AttnLayout attn_layout(const cgtp_attn_args& a) {
@@ -84,9 +89,8 @@ AttnLayout attn_layout(const cgtp_attn_args& a) {
   l.row_part = take(a.slope ? a.n_q * a.h_q * 16 : 0);
   l.key_part = take(a.slope ? a.n_k * a.h_kv * 16 : 0);
   l.slope_part = take(a.slope ? blocks_of(a.n_q) * a.h_q * 4 : 0);
-  const int64_t heads = a.h_kv * 4;
-  l.parts = take(std::max(a.n_q_slots * heads * cgtp_attn_rows(a.wide_q) * (a.dim + kQSums),
-                          a.n_k_slots * heads * cgtp_attn_rows(a.wide_k) * (2 * a.dim + 4)));
+  l.parts = take(std::max(q_parts(a) * (a.dim + kQSums) * 4,
+                          (int64_t)a.n_k_slots * a.h_kv * cgtp_attn_rows(a.wide_k) * (2 * a.dim + 4) * 4));
   l.bytes = at;
   return l;
 }
@@ -100,8 +104,10 @@ int attn_check(const cgtp_attn_args* a) {
   if (a->n_q * (a->h_q / a->h_kv) > 0x7fffffff) return CGTP_ERR_SHAPE;
   if (a->n_q_items < 0 || a->n_q_joins < 0 || a->n_q_slots < 0 || a->n_k_items < 0 || a->n_k_joins < 0 || a->n_k_slots < 0)
     return CGTP_ERR_SHAPE;
-  if ((int64_t)std::max(a->n_q_items, a->n_k_items) * a->h_kv >= (1 << 24)) return CGTP_ERR_SHAPE;
-  if ((int64_t)a->n_q_joins * a->h_kv * cgtp_attn_rows(a->wide_q) >= (1 << 22) ||
+  const int64_t heads = a->together ? a->h_q : a->h_kv, group = a->h_q / a->h_kv;
+  if (a->together && (!a->slope || a->dim > 64 || (group > 2 && group % 4))) return CGTP_ERR_CONFIG;
+  if (a->n_q_items * heads >= (1 << 24) || (int64_t)a->n_k_items * a->h_kv >= (1 << 24)) return CGTP_ERR_SHAPE;
+  if (a->n_q_joins * heads * cgtp_attn_rows(a->wide_q) >= (1 << 22) ||
       (int64_t)a->n_k_joins * a->h_kv * cgtp_attn_rows(a->wide_k) >= (1 << 22))
     return CGTP_ERR_SHAPE;
   if ((a->n_q_items && !a->q_items) || (a->n_q_joins && !a->q_joins)) return CGTP_ERR_NULL;
@@ -150,7 +156,7 @@ int64_t cgtp_attn_workspace_bytes(const cgtp_attn_args* a, int backward) {
   using namespace cgtp;
   if (attn_check(a) != CGTP_OK) return 0;
   if (backward) return attn_layout(*a).bytes;
-  return (int64_t)a->n_q_slots * a->h_kv * cgtp_attn_rows(a->wide_q) * (a->dim + 2) * 4;
+  return q_parts(*a) * (a->dim + 2) * 4;
 }
 
 int cgtp_attn_forward(const cgtp_attn_args* a, void* stream) {
@@ -158,6 +164,7 @@ int cgtp_attn_forward(const cgtp_attn_args* a, void* stream) {
   if (int rc = attn_check(a)) return rc;
   if (a->n_q == 0) return CGTP_OK;
   if (a->n_q_slots > 0 && !a->workspace) return CGTP_ERR_WORKSPACE;
+  if (a->together && (!is_fast(*a, false) || !aligned16(a->out))) return CGTP_ERR_ALIGN;
   launch(*a, nullptr, (hipStream_t)stream);
   return hipGetLastError() == hipSuccess ? CGTP_OK : CGTP_ERR_LAUNCH;
 }
@@ -166,9 +173,12 @@ int cgtp_attn_backward(const cgtp_attn_args* a, void* stream) {
   using namespace cgtp;
   if (int rc = attn_check(a)) return rc;
   if ((a->n_k_items && !a->k_items) || (a->n_k_joins && !a->k_joins)) return CGTP_ERR_NULL;
-  if (a->n_q > 0 && (!a->lse || !a->grad_out)) return CGTP_ERR_NULL;
+  if (a->n_q > 0 && (!a->lse || !a->grad_out || (a->together && a->dtype != CGTP_F32 && !a->out_low))) return CGTP_ERR_NULL;
   const AttnLayout l = attn_layout(*a);
   if (l.bytes > 0 && !a->workspace) return CGTP_ERR_WORKSPACE;
+  if (a->together && (!is_fast(*a, true) || !aligned16(a->out) || !aligned16(a->out_low) || !aligned16(a->grad_q) ||
+                      !aligned16(a->grad_k) || !aligned16(a->grad_v)))
+    return CGTP_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)a->workspace;
   const AttnScratch w = {(float*)ws, (f32x4*)(ws + l.row_part), (f32x4*)(ws + l.key_part), (float*)(ws + l.slope_part),

@@ -65,6 +65,17 @@ struct RowFrag {
       if (p && d < dim) f[s] = load_part<u32x4_t, T>(p + d, dim - d);
     }
   }
+  // Rows of whole aligned chunks.
+  __device__ __forceinline__ void load_fast(const T* p, int dim) {
+    using S = AttnShape<T, DP>;
+    const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s) {
+      const int d = (2 * s + half) * S::kChunk;
+      f[s] = u32x4_t{0, 0, 0, 0};
+      if (p && d < dim) f[s] = *reinterpret_cast<const u32x4_t*>(p + d);
+    }
+  }
 };
 
 // A tile between memory and LDS.  Offset(i): bytes from `base` of row i, kNoRow for none; Pointer(i): the row, null for none.
@@ -74,18 +85,22 @@ struct TileStage {
   static constexpr int kAll = BLOCK * S::kChunks, kEach = (kAll + THREADS - 1) / THREADS;
   u32x4_t reg[kEach];
 
+  template <typename Offset>
+  __device__ __forceinline__ void load_fast(const T* base, int dim, Offset&& offset) {
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kNoRow, 0x00027000);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int id = i * THREADS + (int)threadIdx.x, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
+      if (kAll % THREADS != 0 && id >= kAll) break;
+      const unsigned o = offset(r);
+      reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+          rsrc, o == kNoRow || c * S::kChunk >= dim ? kNoRow : o + c * 16, 0, 0));
+    }
+  }
   template <typename Offset, typename Pointer>
   __device__ __forceinline__ void load(bool fast, const T* base, int dim, Offset&& offset, Pointer&& pointer) {
     if (fast) {
-      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kNoRow, 0x00027000);
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int id = i * THREADS + (int)threadIdx.x, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
-        if (kAll % THREADS != 0 && id >= kAll) break;
-        const unsigned o = offset(r);
-        reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-            rsrc, o == kNoRow || c * S::kChunk >= dim ? kNoRow : o + c * 16, 0, 0));
-      }
+      load_fast(base, dim, offset);
     } else {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
@@ -128,8 +143,21 @@ __device__ __forceinline__ u32x2_t lds_transposed(const char* p) {
   return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)p));
 }
 
-// acc[o] += columns 32 o .. of the tile's 32 rows from `first` on, transposed, times p (rows by lanes' columns).
-template <typename T, int DP>
+// Two values rounded to T, as they lie in a register; `rest`: what that took off them.
+template <typename T>
+__device__ __forceinline__ unsigned round_pair(float a, float b, float (&rest)[2]) {
+  typedef T v2 __attribute__((ext_vector_type(2)));
+  const f32x2 f = {a, b};
+  const v2 h = __builtin_convertvector(f, v2);
+  const f32x2 back = __builtin_convertvector(h, f32x2);
+  rest[0] = a - back[0];
+  rest[1] = b - back[1];
+  return __builtin_bit_cast(unsigned, h);
+}
+
+// acc[o] += columns 32 o .. of the tile's 32 rows from `first` on, transposed, times p (rows by lanes' columns).  BOTH: also
+// times what rounding to a 16-bit type takes off p.
+template <typename T, int DP, bool BOTH = false>
 __device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* lds, int first, const f32x16_t& p) {
   using S = AttnShape<T, DP>;
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -137,17 +165,22 @@ __device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* lds,
     const int r = first + 4 * half + ((lane & 15) >> 2), d = (lane & 16) + 4 * (lane & 3);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      typedef T v8 __attribute__((ext_vector_type(8)));
-      v8 b;
+      u32x4_t hi, lo;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] = (T)p[8 * t + j];
+      for (int j = 0; j < 4; ++j) {
+        float rest[2], none[2];
+        hi[j] = round_pair<T>(p[8 * t + 2 * j], p[8 * t + 2 * j + 1], rest);
+        if constexpr (BOTH) lo[j] = round_pair<T>(rest[0], rest[1], none);
+      }
 #pragma unroll
       for (int o = 0; o < S::kOut; ++o) {
         // DP = 16: the columns 16 .. 31 of the result do not exist; its lanes read the others again
         const int col = DP < 32 ? d & 15 : 32 * o + d;
-        const u32x2_t lo = lds_transposed(lds + S::slot(r + 16 * t, col >> 3) + (col & 7) * 2);
-        const u32x2_t hi = lds_transposed(lds + S::slot(r + 16 * t + 8, col >> 3) + (col & 7) * 2);
-        acc[o] = mma_pair<T>(u32x4_t{lo[0], lo[1], hi[0], hi[1]}, __builtin_bit_cast(u32x4_t, b), acc[o]);
+        const u32x2_t x = lds_transposed(lds + S::slot(r + 16 * t, col >> 3) + (col & 7) * 2);
+        const u32x2_t y = lds_transposed(lds + S::slot(r + 16 * t + 8, col >> 3) + (col & 7) * 2);
+        const u32x4_t a = {x[0], x[1], y[0], y[1]};
+        acc[o] = mma_pair<T>(a, hi, acc[o]);
+        if constexpr (BOTH) acc[o] = mma_pair<T>(a, lo, acc[o]);
       }
     }
   } else {
@@ -164,6 +197,22 @@ __device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* lds,
   }
 }
 
+// Results of a lane's column to a row of whole chunks, aligned to an element's vector of four.
+template <typename T, int DP>
+__device__ __forceinline__ void store_cols_fast(T* p, const AttnAcc<T, DP>& acc, float by, int dim) {
+  const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int o = 0; o < AttnShape<T, DP>::kOut; ++o)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * o + 8 * g + 4 * half;
+      typedef T vec __attribute__((ext_vector_type(4)));
+      vec v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (T)(acc[o][4 * g + e] * by);
+      if (d < dim) *reinterpret_cast<vec*>(p + d) = v;
+    }
+}
 // Results of a lane's column: its elements 32 o + 8 g + 4 (lane / 32) + e of dim, times `by`, to p.
 template <typename T, int DP>
 __device__ __forceinline__ void store_cols(T* p, const AttnAcc<T, DP>& acc, float by, int dim) {

@@ -188,7 +188,7 @@ struct Gff : torch::autograd::Function<Gff> {
 // The kernels' tables of a plan for one number of heads.
 struct AttnHandle {
   at::Tensor q_items, q_joins, k_items, k_joins;
-  int64_t q_slots, k_slots, wide_q, wide_k;
+  int64_t q_slots, k_slots, wide_q, wide_k, together;
   Fallback fallback;
   void set_fallback(py::object fn) { fallback.set(std::move(fn)); }
 };
@@ -232,16 +232,19 @@ cgtp_attn_args attn_args(const AttnOperands& o, const AttnHandle& h, double scal
   a.n_k_slots = (int32_t)h.k_slots;
   a.wide_q = (int32_t)h.wide_q;
   a.wide_k = (int32_t)h.wide_k;
+  a.together = (int32_t)h.together;
   return a;
 }
 
-at::Tensor attn_forward(const AttnOperands& o, const AttnHandle& h, double scale, double cap, at::Tensor* lse) {
+at::Tensor attn_forward(const AttnOperands& o, const AttnHandle& h, double scale, double cap, at::Tensor* lse, at::Tensor* low) {
   c10::hip::HIPGuardMasqueradingAsCUDA guard(o.q.device());
   cgtp_attn_args a = attn_args(o, h, scale, cap);
   at::Tensor out = at::empty(o.q.sizes(), o.q.options());
   if (lse) *lse = at::empty({a.n_q, (int64_t)a.h_q}, o.q.options().dtype(at::kFloat));
+  if (lse && h.together && a.dtype != CGTP_F32) *low = at::empty(o.q.sizes(), o.q.options());
   a.out = out.data_ptr();
   a.lse = lse ? lse->data_ptr() : nullptr;
+  a.out_low = low ? mutable_ptr(*low) : nullptr;
   at::Tensor ws;
   if (a.n_q_slots) {
     ws = bytes_on(o.q, cgtp_attn_workspace_bytes(&a, 0));
@@ -256,11 +259,11 @@ struct Attn : torch::autograd::Function<Attn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Optional& pos_q,
                             const Optional& pos_k, const Optional& slope, const AttnHandle* h, double scale, double cap) {
     const AttnOperands o = {q, k, v, opt(pos_q), opt(pos_k), opt(slope)};
-    at::Tensor lse;
-    at::Tensor out = attn_forward(o, *h, scale, cap, &lse);
-    ctx->save_for_backward({q, k, v, o.pos_q, o.pos_k, o.slope, out, lse, h->q_items, h->q_joins, h->k_items, h->k_joins});
+    at::Tensor lse, low;
+    at::Tensor out = attn_forward(o, *h, scale, cap, &lse, &low);
+    ctx->save_for_backward({q, k, v, o.pos_q, o.pos_k, o.slope, out, lse, h->q_items, h->q_joins, h->k_items, h->k_joins, low});
     auto& d = ctx->saved_data;
-    d["shape"] = std::vector<int64_t>{h->q_slots, h->k_slots, h->wide_q, h->wide_k, h->fallback.id};
+    d["shape"] = std::vector<int64_t>{h->q_slots, h->k_slots, h->wide_q, h->wide_k, h->fallback.id, h->together};
     d["scale"] = scale;
     d["cap"] = cap;
     d["keep"] = c10::IValue::make_capsule(c10::make_intrusive<FallbackHolder>(h->fallback));
@@ -277,11 +280,13 @@ struct Attn : torch::autograd::Function<Attn> {
     if (at::GradMode::is_enabled())
       return call_fallback(shape[4], grad[0], {s[0], s[1], s[2], s[3], s[4], s[5]}, need, 9);
     c10::hip::HIPGuardMasqueradingAsCUDA guard(o.q.device());
-    AttnHandle h{s[8], s[9], s[10], s[11], shape[0], shape[1], shape[2], shape[3], {}};
+    const AttnHandle h{s[8], s[9], s[10], s[11], shape[0], shape[1], shape[2], shape[3], shape[5], {}};
     cgtp_attn_args a = attn_args(o, h, d["scale"].toDouble(), d["cap"].toDouble());
-    const at::Tensor g = grad[0].contiguous();
+    at::Tensor g = grad[0].contiguous();
+    if ((uintptr_t)g.data_ptr() & 15) g = g.clone();
     a.out = s[6].data_ptr();
     a.lse = s[7].data_ptr();
+    a.out_low = mutable_ptr(s[12]);
     a.grad_out = g.data_ptr();
     variable_list out(9);
     for (size_t i = 0; i < 6; ++i)
@@ -315,15 +320,15 @@ void bind_node_operators(py::module& m) {
   }, "gated feed-forward block; with its autograd node where a backward may follow (keep)");
   py::class_<AttnHandle>(m, "AttnHandle")
       .def(py::init([](c10::optional<at::Tensor> q_items, c10::optional<at::Tensor> q_joins, c10::optional<at::Tensor> k_items,
-                       c10::optional<at::Tensor> k_joins, int64_t q_slots, int64_t k_slots, int64_t wide_q, int64_t wide_k) {
-        return AttnHandle{opt(q_items), opt(q_joins), opt(k_items), opt(k_joins), q_slots, k_slots, wide_q, wide_k, {}};
+                       c10::optional<at::Tensor> k_joins, int64_t q_slots, int64_t k_slots, int64_t wide_q, int64_t wide_k, int64_t together) {
+        return AttnHandle{opt(q_items), opt(q_joins), opt(k_items), opt(k_joins), q_slots, k_slots, wide_q, wide_k, together, {}};
       }))
       .def("set_fallback", &AttnHandle::set_fallback, "callable (grad_out, inputs, need) -> gradients, for gradients of higher order");
   m.def("attn", [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& pos_q,
                    const c10::optional<at::Tensor>& pos_k, const c10::optional<at::Tensor>& slope, const AttnHandle& h, double scale,
                    double cap, bool keep) {
     if (keep) return Attn::apply(q, k, v, pos_q, pos_k, slope, &h, scale, cap);
-    return attn_forward({q, k, v, opt(pos_q), opt(pos_k), opt(slope)}, h, scale, cap, nullptr);
+    return attn_forward({q, k, v, opt(pos_q), opt(pos_k), opt(slope)}, h, scale, cap, nullptr, nullptr);
   }, "attention among the nodes of a structure; with its autograd node where a backward may follow (keep)");
 }
 

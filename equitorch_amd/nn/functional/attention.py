@@ -20,7 +20,7 @@ from .edge import _higher_order
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _BLOCK = 64                     # keys (rows) of a tile: pieces of a structure begin at multiples of it
 _PIECE = 256                    # keys (rows) of a piece at least
-_WAVES = 2048                   # wavefronts wanted at least before structures are cut into pieces: two for each SIMD
+_WAVES = 4096                   # wavefronts wanted where structures can be cut into pieces: four for each SIMD
 
 
 def _lengths(ptr: Tensor, name: str) -> np.ndarray:
@@ -72,7 +72,12 @@ def _table(columns, order, device) -> Optional[Tensor]:
 
 
 class _Tables:
-    def __init__(self, plan: "AttentionPlan", group: int, heads: int):
+    def __init__(self, plan: "AttentionPlan", group: int, heads: int, together: bool):
+        # Heads taken together: a row is a query, and a workgroup has two heads of it, else a query with all its heads of a
+        # head of keys.
+        self.together = together
+        if together:
+            group, heads = 1, -(-group * heads // 2)
         rows, cols = plan.len_q * group, plan.len_k
         if rows.sum() >= 2 ** 31:
             raise CgtpError("queries times query heads of a head of keys must stay below 2^31")
@@ -107,6 +112,7 @@ class _Tables:
             setattr(a, name, _lib.ptr(t))
             setattr(a, "n_" + name, 0 if t is None else t.shape[0])
         a.n_q_slots, a.n_k_slots, a.wide_q, a.wide_k = self.q_slots, self.k_slots, self.wide_q, self.wide_k
+        a.together = self.together
 
 
 def _wide(n: np.ndarray) -> bool:
@@ -145,18 +151,23 @@ class AttentionPlan:
         ptr = np.concatenate([[0], np.cumsum(np.bincount(b, minlength=n))]).astype(np.int64)
         return cls(torch.from_numpy(ptr).to(batch.device))
 
-    def tables(self, group: int, heads: int) -> _Tables:
-        key = (group, heads)
+    def tables(self, group: int, heads: int, dim: int, may: bool) -> _Tables:
+        """For ``heads`` heads of keys with ``group`` query heads each.  Distances are formed once for several heads where
+        the operands allow it (``may``: distances, aligned rows) and heads are so narrow that several fit a wavefront's
+        registers, unless the queries are so few that one tile takes all the heads of a structure."""
+        together = may and dim <= 64 and group * heads > 1 and (group <= 2 or group % 4 == 0) \
+            and self.num_queries >= 8 * self.num_structures
+        key = (group, heads, together)
         if key not in self._tables:
-            self._tables[key] = _Tables(self, group, heads)
+            self._tables[key] = _Tables(self, group, heads, together)
         return self._tables[key]
 
-    def handle(self, mod, group: int, heads: int, scale: float, cap: float):
+    def handle(self, mod, group: int, heads: int, dim: int, may: bool, scale: float, cap: float):
         """The extension's copy of the tables, and the tensor expression its node evaluates under gradient mode."""
-        key = (group, heads, scale, cap)
+        key = (group, heads, dim, may, scale, cap)
         if key not in self._tables:
-            t, buckets = self.tables(group, heads), self._buckets
-            h = mod.AttnHandle(t.q_items, t.q_joins, t.k_items, t.k_joins, t.q_slots, t.k_slots, t.wide_q, t.wide_k)
+            t, buckets = self.tables(group, heads, dim, may), self._buckets
+            h = mod.AttnHandle(t.q_items, t.q_joins, t.k_items, t.k_joins, t.q_slots, t.k_slots, t.wide_q, t.wide_k, t.together)
             # holds the buckets, not the plan: the node keeps it for as long as it lives itself
             h.set_fallback(lambda g, inputs, need: _higher_order(_of_buckets(buckets, scale, cap), inputs, need, g))
             self._tables[key] = h
@@ -230,6 +241,15 @@ def _expression(q, k, v, pos_q, pos_k, slope, padded: _Buckets, scale: float, ca
     return torch.cat(outs)[order].to(dtype)
 
 
+def _aligned(*tensors: Tensor) -> bool:
+    """Whether rows are whole vectors of 16 bytes, aligned."""
+    for t in tensors:
+        chunk = 16 // t.element_size()
+        if t.data_ptr() % 16 or t.shape[2] % chunk or t.stride(0) % chunk or t.stride(1) % chunk:
+            return False
+    return True
+
+
 def _args(q, k, v, pos_q, pos_k, slope, plan, scale, cap) -> AttnArgs:
     a = AttnArgs()
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
@@ -239,22 +259,23 @@ def _args(q, k, v, pos_q, pos_k, slope, plan, scale, cap) -> AttnArgs:
     a.pos_q, a.pos_k, a.slope = _lib.ptr(pos_q), _lib.ptr(pos_k), _lib.ptr(slope)
     a.n_q, a.n_k, a.h_q, a.h_kv, a.dim = q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2]
     a.dtype, a.scale, a.cap = _lib.dtype_code(q.dtype), scale, cap
-    plan.tables(a.h_q // a.h_kv, a.h_kv).put(a)
+    plan.tables(a.h_q // a.h_kv, a.h_kv, a.dim, slope is not None and _aligned(q, k, v)).put(a)
     return a
 
 
 def _forward(q, k, v, pos_q, pos_k, slope, plan, scale, cap, keep):
-    """``(out, lse)``; lse, which a backward reads, is None unless ``keep``."""
+    """``(out, lse, out_low)``; the last two, which a backward reads, are None unless ``keep``."""
     a = _args(q, k, v, pos_q, pos_k, slope, plan, scale, cap)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if keep else None
-    a.out, a.lse = out.data_ptr(), _lib.ptr(lse)
+    low = torch.empty(q.shape, dtype=q.dtype, device=q.device) if keep and a.together and q.dtype != torch.float32 else None
+    a.out, a.lse, a.out_low = out.data_ptr(), _lib.ptr(lse), _lib.ptr(low)
     ws = None
     if a.n_q_slots:
         ws = torch.empty(_lib.lib.cgtp_attn_workspace_bytes(C.byref(a), 0), dtype=torch.uint8, device=q.device)
         a.workspace = ws.data_ptr()
     _lib.check(_lib.lib.cgtp_attn_forward(C.byref(a), _lib.stream_ptr(q.device)), "cgtp_attn_forward")
-    return out, lse
+    return out, lse, low
 
 
 class _SegmentAttention(Function):
@@ -262,21 +283,22 @@ class _SegmentAttention(Function):
 
     @staticmethod
     def forward(ctx, q, k, v, pos_q, pos_k, slope, plan, scale, cap):
-        out, lse = _forward(q, k, v, pos_q, pos_q if pos_k is None else pos_k, slope, plan, scale, cap, True)
-        ctx.save_for_backward(q, k, v, pos_q, pos_k, slope, out, lse)
+        out, lse, low = _forward(q, k, v, pos_q, pos_q if pos_k is None else pos_k, slope, plan, scale, cap, True)
+        ctx.save_for_backward(q, k, v, pos_q, pos_k, slope, out, lse, low)
         ctx.plan, ctx.scale, ctx.cap = plan, scale, cap
         return out
 
     @staticmethod
     def backward(ctx, g):
-        q, k, v, pos_q, pos_k, slope, out, lse = ctx.saved_tensors
+        q, k, v, pos_q, pos_k, slope, out, lse, low = ctx.saved_tensors
         need, plan, scale, cap = ctx.needs_input_grad[:6], ctx.plan, ctx.scale, ctx.cap
         if torch.is_grad_enabled():
             expression = _of_buckets(plan._buckets, scale, cap)
             return (*_higher_order(expression, (q, k, v, pos_q, pos_k, slope), need, g), None, None, None)
         g = g.contiguous()
+        g = g if g.data_ptr() % 16 == 0 else g.clone()
         a = _args(q, k, v, pos_q, pos_q if pos_k is None else pos_k, slope, plan, scale, cap)
-        a.out, a.lse, a.grad_out = out.data_ptr(), lse.data_ptr(), g.data_ptr()
+        a.out, a.lse, a.out_low, a.grad_out = out.data_ptr(), lse.data_ptr(), _lib.ptr(low), g.data_ptr()
         grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None
                  for t, n in zip((q, k, v, pos_q, pos_k, slope), need)]
         a.grad_q, a.grad_k, a.grad_v, a.grad_pos_q, a.grad_pos_k, a.grad_slope = (_lib.ptr(t) for t in grads)
@@ -338,7 +360,7 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, pos:
     keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, pos, pos_k, slope))
     mod = _shim.module()
     if mod is not None:
-        handle = plan.handle(mod, q.shape[1] // k.shape[1], k.shape[1], scale, cap)
+        handle = plan.handle(mod, q.shape[1] // k.shape[1], k.shape[1], q.shape[2], slope is not None and _aligned(q, k, v), scale, cap)
         return mod.attn(q, k, v, pos, pos_k, slope, handle, scale, cap, keep)
     if keep:
         return _SegmentAttention.apply(q, k, v, pos, pos_k, slope, plan, scale, cap)

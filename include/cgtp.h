@@ -812,6 +812,10 @@ int cgtp_gff_backward(const cgtp_gff_args* args, void* stream);
  * slot of its own, where it leaves partial results, and first = its place among the pieces of its tile; one entry of q_joins /
  * k_joins adds the slots first .. first + count - 1 of a tile, in that order.  A structure without keys has items with an
  * empty range.  Every query and every key belongs to exactly one tile.
+ * together != 0: with slope, dim <= 64, h_q / h_kv 1, 2 or a multiple of 4, and q, k, v, out, out_low, grad_out, grad_q, grad_k
+ * and grad_v aligned to 16 bytes with dim and strides a multiple of that (else CGTP_ERR_ALIGN), several heads are taken at a time; the rows of
+ * the items are then the queries, each for all heads.  The backward then reads out_low in 16-bit types (NULL in fp32): what
+ * rounding has taken off out, in the same type, which the forward leaves where out_low is not NULL; lse is that call's own.
  * workspace: cgtp_attn_workspace_bytes(args, backward), 16-byte aligned (0: may be NULL).
  * cgtp_attn_backward writes grad_q, grad_k, grad_v and, with slope, grad_slope (h_q) and grad_pos_q (n_q, 3) where they are
  * not NULL; same_pos != 0: the queries' and the keys' positions are one tensor, and grad_pos_q is the whole gradient, else
@@ -825,7 +829,7 @@ typedef struct {
   const void *q, *k, *v;
   int64_t q_node, q_head, k_node, k_head, v_node, v_head;
   const float *pos_q, *pos_k, *slope;
-  void *out, *lse;
+  void *out, *lse, *out_low;
   const cgtp_attn_item *q_items, *q_joins, *k_items, *k_joins;
   int32_t n_q_items, n_q_joins, n_q_slots, n_k_items, n_k_joins, n_k_slots;
   const void* grad_out;
@@ -833,7 +837,7 @@ typedef struct {
   float *grad_pos_q, *grad_pos_k, *grad_slope;
   void* workspace;
   int64_t n_q, n_k;
-  int32_t h_q, h_kv, dim, dtype, wide_q, wide_k, same_pos, reserved_;
+  int32_t h_q, h_kv, dim, dtype, wide_q, wide_k, same_pos, together;
   float scale, cap;
 } cgtp_attn_args;
 int cgtp_attn_rows(int wide);
