@@ -159,7 +159,6 @@ class AttnArgs(C.Structure):
                 ("q_node", C.c_int64), ("q_head", C.c_int64), ("k_node", C.c_int64), ("k_head", C.c_int64),
                 ("v_node", C.c_int64), ("v_head", C.c_int64),
                 ("pos_q", C.c_void_p), ("pos_k", C.c_void_p), ("slope", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
-                ("out_low", C.c_void_p),
                 ("q_items", C.c_void_p), ("q_joins", C.c_void_p), ("k_items", C.c_void_p), ("k_joins", C.c_void_p),
                 ("n_q_items", C.c_int32), ("n_q_joins", C.c_int32), ("n_q_slots", C.c_int32),
                 ("n_k_items", C.c_int32), ("n_k_joins", C.c_int32), ("n_k_slots", C.c_int32),

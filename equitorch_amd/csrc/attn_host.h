@@ -11,7 +11,6 @@ struct AttnLaunch : cgtp_attn_args {
 };
 
 constexpr int kQSums = 10;     // what a piece leaves for each row besides the gradient of q (attn_impl.h, QSums)
-constexpr int kHeadSums = 4;   // and with several heads at a time: the parts of the position's and the slope's gradients
 
 // Buffers of the backward inside its workspace.
 struct AttnScratch {

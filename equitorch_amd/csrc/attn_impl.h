@@ -30,25 +30,33 @@ constexpr float kLog2E = 1.4426950408889634f;
 template <int NW> constexpr int kRowsOf = 32 * NW;
 template <int NW> constexpr int kBlockOf = NW == 1 ? 32 : 64;      // rows of a tile in LDS
 
-// What scores are made of.  A score in units of 1 / unit binary orders: t = q.k where that is all (linear > 0, which then is
-// the unit), else in binary orders: t = linear q.k or outer tanh, less slope |r_i - r_j|.
+// What scores are made of, in binary orders.  Without distances and cap the forward takes t = q.k, in units of `unit` orders (the
+// scale, where that is positive); else t = linear q.k - slope' |r_i - r_j|, or with a cap
+//   t = -2 outer r - slope' |r_i - r_j|,   r = 1 / (2^(inner q.k) + 1),
+// the score without its constant part, which moves lse by as much; 1 - tanh^2 = 4 r (1 - r).
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 template <bool BIASED, bool CAPPED>
-struct ScoreScale {
-  static constexpr bool biased = BIASED, capped = CAPPED;
-  float linear, inner, outer, unit;
-  __device__ __forceinline__ explicit ScoreScale(const AttnLaunch& a) {
+struct Score {
+  float linear, inner, outer2, unit;
+  __device__ __forceinline__ explicit Score(const AttnLaunch& a) {
     linear = a.scale * kLog2E;
-    inner = capped ? 2.f * kLog2E * a.scale / a.cap : 0.f;
-    outer = a.cap * kLog2E;
+    inner = CAPPED ? 2.f * kLog2E * a.scale / a.cap : 0.f;
+    outer2 = -2.f * a.cap * kLog2E;
     unit = plain() ? linear : 1.f;
   }
-  __device__ __forceinline__ bool plain() const { return !capped && !biased && linear > 0.f; }
+  __device__ __forceinline__ bool plain() const { return !CAPPED && !BIASED && linear > 0.f; }
+  // r: what a gradient needs of the cap.
+  __device__ __forceinline__ float operator()(float qk, float slope, float dist, float& r) const {
+    float t;
+    if constexpr (CAPPED) {
+      r = __builtin_amdgcn_rcpf(exp2_fast(inner * qk) + 1.f);
+      t = outer2 * r;
+    } else {
+      t = linear * qk;
+    }
+    return BIASED ? fmaf(-slope, dist, t) : t;
+  }
 };
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// tanh of half of what `inner` makes of q.k.
-__device__ __forceinline__ float capped_tanh(float inner_qk) {
-  return 1.f - 2.f * __builtin_amdgcn_rcpf(exp2_fast(inner_qk) + 1.f);
-}
 __device__ __forceinline__ float half_swap(float x) { return __shfl_xor(x, 32, kWave); }
 
 struct Row {
@@ -101,20 +109,56 @@ struct QueryRows {
 // One tile buffer of LDS where two would not leave room for two workgroups.
 template <int BYTES> constexpr int kBuffers = 2 * BYTES <= 64 * 1024 ? 2 : 1;
 
+// Wavefronts that share out the keys of one tile of rows (KS > 1): each has its own tiles in LDS and waits for nobody, the
+// LDS taking one wavefront's accesses in order; their results are joined at the end.
+template <int KS>
+__device__ __forceinline__ void tile_sync() {
+  if constexpr (KS == 1) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+// Bytes of LDS for the tiles, or for half the wavefronts' results of `sums` values for each lane.
+template <typename T, int DP, int NW, int KS>
+constexpr int attn_lds(int sums) {
+  constexpr int tile = 2 * kBlockOf<NW> * AttnShape<T, DP>::kRow;
+  const int tiles = KS > 1 ? KS * tile : kBuffers<tile> * tile, join = KS > 1 ? KS / 2 * 64 * (16 * AttnShape<T, DP>::kOut + sums) * 4 : 0;
+  return tiles > join ? tiles : join;
+}
+// Halves the number of wavefronts that hold results until one does: give(value place) and take of each value, `n` for a lane.
+template <int KS, typename Give, typename Take>
+__device__ __forceinline__ void join_waves(float* lds, int n, Give&& give, Take&& take) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int s = KS / 2; s >= 1; s >>= 1) {
+    __syncthreads();
+    float* at = lds + (wave % s) * n * 64 + lane;
+    if (wave >= s && wave < 2 * s) give(at);
+    __syncthreads();
+    if (wave < s) take(at);
+  }
+}
+
+
 // ---- forward ----------------------------------------------------------------------------------------------------
-template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
-__global__ void __launch_bounds__(64 * NW, (sizeof(T) == 2 && NW == 4) || DP <= 64 ? 2 : 1)
+template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
+__global__ void __launch_bounds__(64 * NW * KS, (sizeof(T) == 2 && NW == 4) || DP <= 64 ? 2 : 1)
 attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
   using S = AttnShape<T, DP>;
-  constexpr int kBlock = kBlockOf<NW>, kTile = kBlock * S::kRow, kBuf = kBuffers<2 * kTile>;
-  __shared__ alignas(16) char tiles[kBuf][2][kTile];
-  __shared__ alignas(16) float pos[2][3][kBlock];
+  constexpr int kBlock = kBlockOf<NW>, kTile = kBlock * S::kRow, kBuf = KS > 1 ? 1 : kBuffers<2 * kTile>;
+  __shared__ alignas(16) char lds[attn_lds<T, DP, NW, KS>(2)];
+  __shared__ alignas(16) float all_pos[KS][2][3][kBlock];
   const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
   const cgtp_attn_item it = a.q_items[blockIdx.x / a.h_kv];
-  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-  const int r = it.row_begin + wave * 32 + (lane & 31);
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, tid = KS > 1 ? lane : (int)threadIdx.x;
+  const int r = it.row_begin + (KS > 1 ? 0 : wave * 32) + (lane & 31), part = KS > 1 ? wave : 0;
+  char* const tiles = lds + part * 2 * kTile;
+  auto& pos = all_pos[part];
   const Row row = row_of(it, r, hk, group);
-  const ScoreScale<BIASED, CAPPED> sc(a);
+  const Score<BIASED, CAPPED> sc(a);
   RowFrag<T, DP> q;
   q.load(row.ok ? (const T*)a.q + row.query * a.q_node + row.head * a.q_head : nullptr, a.dim);
   float x = 0.f, y = 0.f, z = 0.f, slope = 0.f;
@@ -137,37 +181,32 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
     const KeyRows<T> kr((const T*)a.k, a.k_node, a.k_head, hk, k0, n), vr((const T*)a.v, a.v_node, a.v_head, hk, k0, n);
     ks.load(a.fast, kr.base, a.dim, [&](int i) { return kr.offset(i); }, [&](int i) { return kr.pointer(i); });
     vs.load(a.fast, vr.base, a.dim, [&](int i) { return vr.offset(i); }, [&](int i) { return vr.pointer(i); });
-    if (BIASED && threadIdx.x < kBlock)
+    if (BIASED && tid < kBlock)
 #pragma unroll
-      for (int d = 0; d < 3; ++d) ps[d] = (int)threadIdx.x < n ? a.pos_k[(int64_t)(k0 + threadIdx.x) * 3 + d] : 0.f;
+      for (int d = 0; d < 3; ++d) ps[d] = tid < n ? a.pos_k[(int64_t)(k0 + tid) * 3 + d] : 0.f;
   };
-  if (it.k_begin < it.k_end) fetch(it.k_begin);
+  const int first = it.k_begin + part * kBlock;
+  if (first < it.k_end) fetch(first);
   int buf = 0;
-  for (int k0 = it.k_begin; k0 < it.k_end; k0 += kBlock, buf ^= 1) {
+  for (int k0 = first; k0 < it.k_end; k0 += KS * kBlock, buf ^= 1) {
     const int n = it.k_end - k0;
-    char* const k_tile = tiles[kBuf == 2 ? buf : 0][0];
-    char* const v_tile = tiles[kBuf == 2 ? buf : 0][1];
-    if (kBuf == 1) __syncthreads();
+    char* const k_tile = tiles + (kBuf == 2 ? buf : 0) * 2 * kTile;
+    char* const v_tile = k_tile + kTile;
+    if (kBuf == 1) tile_sync<KS>();
     ks.store(k_tile);
     vs.store(v_tile);
-    if (BIASED && threadIdx.x < kBlock)
+    if (BIASED && tid < kBlock)
 #pragma unroll
-      for (int d = 0; d < 3; ++d) pos[buf][d][threadIdx.x] = ps[d];
-    __syncthreads();
-    if (k0 + kBlock < it.k_end) fetch(k0 + kBlock);
+      for (int d = 0; d < 3; ++d) pos[buf][d][tid] = ps[d];
+    tile_sync<KS>();
+    if (k0 + KS * kBlock < it.k_end) fetch(k0 + KS * kBlock);
     f32x16_t t[kBlock / 32];
     float most = top;
 #pragma unroll
     for (int b = 0; b < kBlock / 32; ++b) {
       if (b * 32 >= n) continue;
       t[b] = rows_times<T, DP>(k_tile, 32 * b, q);
-      if constexpr (CAPPED) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) t[b][e] = sc.outer * capped_tanh(sc.inner * t[b][e]);
-      } else if (BIASED || !sc.plain()) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) t[b][e] *= sc.linear;
-      }
+      float c;
       if constexpr (BIASED) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -178,9 +217,12 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float dx = x - px[e], dy = y - py[e], dz = z - pz[e];
-            t[b][4 * g + e] -= slope * __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz);
+            t[b][4 * g + e] = sc(t[b][4 * g + e], slope, __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz), c);
           }
         }
+      } else if (!sc.plain()) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[b][e] = sc(t[b][e], 0.f, 0.f, c);
       }
       if (n < 32 * b + 32)
 #pragma unroll
@@ -212,6 +254,22 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
     }
   }
   top *= sc.unit;
+  if constexpr (KS > 1) {
+    join_waves<KS>(reinterpret_cast<float*>(lds), 16 * S::kOut + 2, [&](float* at) {
+      at[0] = top;
+      at[64] = sum;
+#pragma unroll
+      for (int i = 0; i < 16 * S::kOut; ++i) at[(2 + i) * 64] = acc[i / 16][i % 16];
+    }, [&](const float* at) {
+      const float top2 = at[0], most = fmaxf(top, top2);
+      const float f1 = top == most ? 1.f : exp2_fast(top - most), f2 = top2 == most ? 1.f : exp2_fast(top2 - most);
+      sum = sum * f1 + at[64] * f2;
+#pragma unroll
+      for (int i = 0; i < 16 * S::kOut; ++i) acc[i / 16][i % 16] = acc[i / 16][i % 16] * f1 + at[(2 + i) * 64] * f2;
+      top = most;
+    });
+    if (wave) return;
+  }
   sum += half_swap(sum);
   if (!row.ok) return;
   if (it.slot < 0) {
@@ -230,11 +288,11 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
   }
 }
 
-// Adds the parts of a row: a workgroup for each (tile, head, row), its slots shared out over slices of threads.  heads: of keys,
-// each with its group of query heads in the rows, or of queries.
+// Adds the parts of a row: a workgroup for each (tile, head of keys, row), its slots shared out over slices of threads.
 constexpr int kJoinThreads = 1024;
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) attn_fwd_join_kernel(AttnLaunch a, const float* __restrict__ parts, int rows, int heads) {
+__global__ void __launch_bounds__(kJoinThreads) attn_fwd_join_kernel(AttnLaunch a, const float* __restrict__ parts, int rows) {
+  const int heads = a.h_kv;
   __shared__ float acc[kJoinThreads], red[kJoinThreads / kWave];
   const int group = a.h_q / heads, rr = blockIdx.x % rows, hk = blockIdx.x / rows % heads;
   const cgtp_attn_item it = a.q_joins[blockIdx.x / rows / heads];
@@ -276,14 +334,14 @@ __global__ void __launch_bounds__(kJoinThreads) attn_fwd_join_kernel(AttnLaunch 
   if (d < a.dim) {
     const float o = some ? total / sum : 0.f;
     ((T*)a.out)[at * a.dim + d] = (T)o;
-    if (sizeof(T) == 2 && a.out_low) ((T*)a.out_low)[at * a.dim + d] = (T)(o - (float)(T)o);
   }
   if (a.lse && tid == 0) ((float*)a.lse)[at] = some ? top + __log2f(sum) : INFINITY;
 }
 
 // The same where a row has few slots: a workgroup for each (tile, head), an element to a thread.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_fwd_join_few_kernel(AttnLaunch a, const float* __restrict__ parts, int rows, int heads) {
+__global__ void __launch_bounds__(256) attn_fwd_join_few_kernel(AttnLaunch a, const float* __restrict__ parts, int rows) {
+  const int heads = a.h_kv;
   const int group = a.h_q / heads, hk = blockIdx.x % heads, width = a.dim + 1;
   const cgtp_attn_item it = a.q_joins[blockIdx.x / heads];
   const int here = it.row_end - it.row_begin;
@@ -308,8 +366,7 @@ __global__ void __launch_bounds__(256) attn_fwd_join_few_kernel(AttnLaunch a, co
     if (d < a.dim) {
       o = some ? o / sum : 0.f;
       ((T*)a.out)[at * a.dim + d] = (T)o;
-      if (sizeof(T) == 2 && a.out_low) ((T*)a.out_low)[at * a.dim + d] = (T)(o - (float)(T)o);
-    } else if (a.lse) {
+      } else if (a.lse) {
       ((float*)a.lse)[at] = some ? top + __log2f(sum) : INFINITY;
     }
   }
@@ -328,20 +385,22 @@ struct QSums {
 };
 
 // ---- gradient with the rows fixed ---------------------------------------------------------------------------------
-template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
-__global__ void __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || DP <= 32 ? 2 : 1)
+template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
+__global__ void __launch_bounds__(64 * NW * KS, (sizeof(T) == 2 && DP <= 64) || DP <= 32 ? 2 : 1)
 attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
   using S = AttnShape<T, DP>;
-  constexpr int kBlock = kBlockOf<NW>, kTile = kBlock * S::kRow, kBuf = kBuffers<2 * kTile>;
-  __shared__ alignas(16) char tiles[kBuf][2][kTile];
-  __shared__ alignas(16) float pos[2][3][kBlock];
+  constexpr int kBlock = kBlockOf<NW>, kTile = kBlock * S::kRow, kBuf = KS > 1 ? 1 : kBuffers<2 * kTile>;
+  __shared__ alignas(16) char lds[attn_lds<T, DP, NW, KS>(9)];
+  __shared__ alignas(16) float all_pos[KS][2][3][kBlock];
   const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
   const cgtp_attn_item it = a.q_items[blockIdx.x / a.h_kv];
-  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-  const int r = it.row_begin + wave * 32 + (lane & 31);
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, tid = KS > 1 ? lane : (int)threadIdx.x;
+  const int r = it.row_begin + (KS > 1 ? 0 : wave * 32) + (lane & 31), part = KS > 1 ? wave : 0;
+  char* const tiles = lds + part * 2 * kTile;
+  auto& pos = all_pos[part];
   const Row row = row_of(it, r, hk, group);
   const int64_t at = (int64_t)row.query * a.h_q + row.head;
-  const ScoreScale<BIASED, CAPPED> sc(a);
+  const Score<BIASED, CAPPED> sc(a);
   RowFrag<T, DP> q, g;
   q.load(row.ok ? (const T*)a.q + row.query * a.q_node + row.head * a.q_head : nullptr, a.dim);
   g.load(row.ok ? (const T*)a.grad_out + at * a.dim : nullptr, a.dim);
@@ -366,6 +425,7 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
     z = a.pos_q[(int64_t)row.query * 3 + 2];
     slope = a.slope[row.head];
   }
+  const float slope2 = slope * kLog2E, grad_scale = CAPPED ? 4.f * a.scale : a.scale;
   AttnAcc<T, DP> acc;
 #pragma unroll
   for (int o = 0; o < S::kOut; ++o)
@@ -383,125 +443,148 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
     const KeyRows<T> kr((const T*)a.k, a.k_node, a.k_head, hk, k0, n), vr((const T*)a.v, a.v_node, a.v_head, hk, k0, n);
     ks.load(a.fast, kr.base, a.dim, [&](int i) { return kr.offset(i); }, [&](int i) { return kr.pointer(i); });
     vs.load(a.fast, vr.base, a.dim, [&](int i) { return vr.offset(i); }, [&](int i) { return vr.pointer(i); });
-    if (BIASED && threadIdx.x < kBlock)
+    if (BIASED && tid < kBlock)
 #pragma unroll
-      for (int d = 0; d < 3; ++d) ps[d] = (int)threadIdx.x < n ? a.pos_k[(int64_t)(k0 + threadIdx.x) * 3 + d] : 0.f;
+      for (int d = 0; d < 3; ++d) ps[d] = tid < n ? a.pos_k[(int64_t)(k0 + tid) * 3 + d] : 0.f;
   };
-  if (it.k_begin < it.k_end) fetch(it.k_begin);
+  const int first = it.k_begin + part * kBlock;
+  if (first < it.k_end) fetch(first);
   int buf = 0;
-  for (int k0 = it.k_begin; k0 < it.k_end; k0 += kBlock, buf ^= 1) {
+  for (int k0 = first; k0 < it.k_end; k0 += KS * kBlock, buf ^= 1) {
     const int n = it.k_end - k0;
-    char* const k_tile = tiles[kBuf == 2 ? buf : 0][0];
-    char* const v_tile = tiles[kBuf == 2 ? buf : 0][1];
-    if (kBuf == 1) __syncthreads();
+    char* const k_tile = tiles + (kBuf == 2 ? buf : 0) * 2 * kTile;
+    char* const v_tile = k_tile + kTile;
+    if (kBuf == 1) tile_sync<KS>();
     ks.store(k_tile);
     vs.store(v_tile);
-    if (BIASED && threadIdx.x < kBlock)
+    if (BIASED && tid < kBlock)
 #pragma unroll
-      for (int d = 0; d < 3; ++d) pos[buf][d][threadIdx.x] = ps[d];
-    __syncthreads();
-    if (k0 + kBlock < it.k_end) fetch(k0 + kBlock);
+      for (int d = 0; d < 3; ++d) pos[buf][d][tid] = ps[d];
+    tile_sync<KS>();
+    if (k0 + KS * kBlock < it.k_end) fetch(k0 + KS * kBlock);
 #pragma unroll 1
     for (int b = 0; b < kBlock / 32; ++b) {
       if (b * 32 >= n) continue;
       f32x16_t t = rows_times<T, DP>(k_tile, 32 * b, q);
       f32x16_t ds = rows_times<T, DP>(v_tile, 32 * b, g);
+      auto turn = [&](bool cut) {
 #pragma unroll
-      for (int gq = 0; gq < 4; ++gq) {
-        const int first = 32 * b + 8 * gq + 4 * half;
-        f32x4 px = {}, py = {}, pz = {};
-        if constexpr (BIASED) {
-          px = *reinterpret_cast<const f32x4*>(&pos[buf][0][first]);
-          py = *reinterpret_cast<const f32x4*>(&pos[buf][1][first]);
-          pz = *reinterpret_cast<const f32x4*>(&pos[buf][2][first]);
-        }
+        for (int gq = 0; gq < 4; ++gq) {
+          const int first = 32 * b + 8 * gq + 4 * half;
+          f32x4 px = {}, py = {}, pz = {};
+          if constexpr (BIASED) {
+            px = *reinterpret_cast<const f32x4*>(&pos[buf][0][first]);
+            py = *reinterpret_cast<const f32x4*>(&pos[buf][1][first]);
+            pz = *reinterpret_cast<const f32x4*>(&pos[buf][2][first]);
+          }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 4 * gq + e;
-          float th = 0.f, s;
-          if constexpr (CAPPED) {
-            th = capped_tanh(sc.inner * t[i]);
-            s = sc.outer * th;
-          } else {
-            s = sc.linear * t[i];
-          }
-          float dx = 0.f, dy = 0.f, dz = 0.f, d2 = 0.f, inv = 0.f;
-          if constexpr (BIASED) {
-            dx = x - px[e];
-            dy = y - py[e];
-            dz = z - pz[e];
-            d2 = dx * dx + dy * dy + dz * dz;
-            inv = __builtin_amdgcn_rsqf(fmaxf(d2, 1e-37f));
-            s -= slope * kLog2E * (d2 * inv);
-          }
-          float p = exp2_fast(s - lse);
-          if (first + e >= n) p = 0.f;
-          float d = p * (ds[i] - delta);
-          if constexpr (BIASED) {
-            const float u = d * inv;
-            m.v[0] = fmaf(u, dx, m.v[0]);
-            m.v[1] = fmaf(u, dy, m.v[1]);
-            m.v[2] = fmaf(u, dz, m.v[2]);
-            m.v[3] = fmaf(u, d2, m.v[3]);
-            if constexpr (kFix) {
-              const float c = p * inv;
-              m.v[4] = fmaf(c, dx, m.v[4]);
-              m.v[5] = fmaf(c, dy, m.v[5]);
-              m.v[6] = fmaf(c, dz, m.v[6]);
-              m.v[7] = fmaf(c, d2, m.v[7]);
-              m.v[8] += d;
+          for (int e = 0; e < 4; ++e) {
+            const int i = 4 * gq + e;
+            float c = 0.f;
+            float dx = 0.f, dy = 0.f, dz = 0.f, d2 = 0.f, inv = 0.f;
+            if constexpr (BIASED) {
+              dx = x - px[e];
+              dy = y - py[e];
+              dz = z - pz[e];
+              d2 = dx * dx + dy * dy + dz * dz;
+              inv = __builtin_amdgcn_rsqf(fmaxf(d2, 1e-37f));
             }
+            float p = exp2_fast(sc(t[i], slope2, d2 * inv, c) - lse);
+            if (cut && first + e >= n) p = 0.f;
+            float d = p * (ds[i] - delta);
+            if constexpr (BIASED) {
+              const float u = d * inv;
+              m.v[0] = fmaf(u, dx, m.v[0]);
+              m.v[1] = fmaf(u, dy, m.v[1]);
+              m.v[2] = fmaf(u, dz, m.v[2]);
+              m.v[3] = fmaf(u, d2, m.v[3]);
+              if constexpr (kFix) {
+                const float near = p * inv;
+                m.v[4] = fmaf(near, dx, m.v[4]);
+                m.v[5] = fmaf(near, dy, m.v[5]);
+                m.v[6] = fmaf(near, dz, m.v[6]);
+                m.v[7] = fmaf(near, d2, m.v[7]);
+                m.v[8] += d;
+              }
+            }
+            if constexpr (CAPPED) d *= fmaf(-c, c, c);
+            ds[i] = d;
           }
-          if constexpr (CAPPED) d *= 1.f - th * th;
-          ds[i] = d;
+          __builtin_amdgcn_sched_barrier(0);      // keeps the next group's reads from LDS out of the registers
         }
-        __builtin_amdgcn_sched_barrier(0);      // keeps the next group's reads from LDS out of the registers
-      }
+      };
+      if (n < 32 * b + 32) turn(true);
+      else turn(false);
       cols_times<T, DP>(acc, k_tile, 32 * b, ds);
     }
+  }
+  if constexpr (KS > 1) {
+    join_waves<KS>(reinterpret_cast<float*>(lds), 16 * S::kOut + 9, [&](float* at) {
+#pragma unroll
+      for (int i = 0; i < 9; ++i) at[i * 64] = m.v[i];
+#pragma unroll
+      for (int i = 0; i < 16 * S::kOut; ++i) at[(9 + i) * 64] = acc[i / 16][i % 16];
+    }, [&](const float* at) {
+#pragma unroll
+      for (int i = 0; i < 9; ++i) m.v[i] += at[i * 64];
+#pragma unroll
+      for (int i = 0; i < 16 * S::kOut; ++i) acc[i / 16][i % 16] += at[(9 + i) * 64];
+    });
+    if (wave) return;
   }
 #pragma unroll
   for (int i = 0; i < (kFix ? 9 : 4); ++i) m.v[i] += half_swap(m.v[i]);
   m.v[9] = delta;
   if (!row.ok) return;
   if (it.slot < 0) {
-    if (a.grad_q) store_cols<T, DP>((T*)a.grad_q + at * a.dim, acc, a.scale, a.dim);
+    if (a.grad_q) store_cols<T, DP>((T*)a.grad_q + at * a.dim, acc, grad_scale, a.dim);
     if (half == 0) m.finish(w, at, slope, BIASED);
   } else {
     float* p = w.parts + (((int64_t)it.slot * a.h_kv + hk) * kRowsOf<NW> + (r - it.row_begin)) * (a.dim + kQSums);
-    store_cols<float, (DP < 32 ? 32 : DP)>(p, acc, a.scale, a.dim);
+    store_cols<float, (DP < 32 ? 32 : DP)>(p, acc, grad_scale, a.dim);
     if (half == 0)
 #pragma unroll
       for (int i = 0; i < kQSums; ++i) p[a.dim + i] = m.v[i];
   }
 }
 
-// One row to a workgroup: the sums that end with a factor of the row.
-template <typename T>
-__global__ void __launch_bounds__(192) attn_bwd_q_join_kernel(AttnLaunch a, AttnScratch w, int rows) {
-  __shared__ float sums[kQSums];
-  const int group = a.h_q / a.h_kv, rr = blockIdx.x % rows, hk = blockIdx.x / rows % a.h_kv;
-  const cgtp_attn_item it = a.q_joins[blockIdx.x / rows / a.h_kv];
-  const Row row = row_of(it, it.row_begin + rr, hk, group);
-  if (!row.ok) return;
-  const int d = threadIdx.x, width = a.dim + kQSums;
-  const int64_t step = (int64_t)a.h_kv * rows * width, at = (int64_t)row.query * a.h_q + row.head;
-  const float* p = w.parts + (((int64_t)it.first * a.h_kv + hk) * rows + rr) * width + d;
-  float s = 0.f;
-  const int count = d == width - 1 ? 1 : d < width ? it.count : 0;       // delta: the same in every piece
-#pragma unroll 8
-  for (int k = 0; k < count; ++k) s += p[k * step];
-  if (d < a.dim) {
-    if (a.grad_q) ((T*)a.grad_q)[at * a.dim + d] = (T)s;
-  } else if (d < width) {
-    sums[d - a.dim] = s;
+// Adds the parts of a tile's rows or keys, `width` values for each, elements from .. from + n - 1 of them: an element of the
+// tile to a thread, its slots in order, the threads of the workgroups y of `ys`.  put(row or key, element, sum).
+template <typename Put>
+__device__ __forceinline__ void join_elements(const float* parts, const cgtp_attn_item& it, int head, int heads, int tile, int here,
+                                              int width, int from, int n, int y, int ys, Put&& put) {
+  const int64_t step = (int64_t)heads * tile * width;
+  const float* p = parts + ((int64_t)it.first * heads + head) * tile * width + from;
+  for (int e = y * 256 + threadIdx.x; e < here * n; e += ys * 256) {
+    const int r = e / n, d = e % n;
+    float s = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < it.count; ++k) s += p[k * step + r * width + d];
+    put(r, d, s);
   }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) attn_bwd_q_join_kernel(AttnLaunch a, AttnScratch w, int tile) {
+  __shared__ float sums[128][kQSums];
+  const int group = a.h_q / a.h_kv, hk = blockIdx.x % a.h_kv, here_width = a.dim + kQSums;
+  const cgtp_attn_item it = a.q_joins[blockIdx.x / a.h_kv];
+  const int here = it.row_end - it.row_begin;
+  if (a.grad_q)
+    join_elements(w.parts, it, hk, a.h_kv, tile, here, here_width, 0, a.dim, blockIdx.y, gridDim.y, [&](int r, int d, float s) {
+      const Row row = row_of(it, it.row_begin + r, hk, group);
+      ((T*)a.grad_q)[((int64_t)row.query * a.h_q + row.head) * a.dim + d] = (T)s;
+    });
+  if (blockIdx.y) return;
+  // one workgroup of a tile: the sums that end with a factor of the row
+  join_elements(w.parts, it, hk, a.h_kv, tile, here, here_width, a.dim, kQSums, 0, 1, [&](int r, int d, float s) { sums[r][d] = s; });
   __syncthreads();
-  if (d != 0) return;
+  if ((int)threadIdx.x >= here) return;
+  const Row row = row_of(it, it.row_begin + threadIdx.x, hk, group);
   QSums m;
 #pragma unroll
-  for (int i = 0; i < kQSums; ++i) m.v[i] = sums[i];
-  m.finish(w, at, a.slope ? a.slope[row.head] : 0.f, a.slope != nullptr);
+  for (int i = 0; i < kQSums; ++i) m.v[i] = sums[threadIdx.x][i];
+  m.v[9] /= (float)it.count;            // delta: the same in every piece
+  m.finish(w, (int64_t)row.query * a.h_q + row.head, a.slope ? a.slope[row.head] : 0.f, a.slope != nullptr);
 }
 
 // ---- gradient with the keys fixed ---------------------------------------------------------------------------------
@@ -517,7 +600,7 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
   const int key = it.k_begin + wave * 32 + (lane & 31);
   const bool ok = key < it.k_end;
-  const ScoreScale<BIASED, CAPPED> sc(a);
+  const Score<BIASED, CAPPED> sc(a);
   RowFrag<T, DP> k, v;
   k.load(ok ? (const T*)a.k + key * a.k_node + hk * a.k_head : nullptr, a.dim);
   v.load(ok ? (const T*)a.v + key * a.v_node + hk * a.v_head : nullptr, a.dim);
@@ -587,23 +670,16 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * g + e;
-          float th = 0.f, s;
-          if constexpr (CAPPED) {
-            th = capped_tanh(sc.inner * t[i]);
-            s = sc.outer * th;
-          } else {
-            s = sc.linear * t[i];
-          }
-          float dx = 0.f, dy = 0.f, dz = 0.f, inv = 0.f;
+          float c = 0.f;
+          float dx = 0.f, dy = 0.f, dz = 0.f, d2 = 0.f, inv = 0.f;
           if constexpr (BIASED) {
             dx = px[e] - x;
             dy = py[e] - y;
             dz = pz[e] - z;
-            const float d2 = dx * dx + dy * dy + dz * dz;
+            d2 = dx * dx + dy * dy + dz * dz;
             inv = __builtin_amdgcn_rsqf(fmaxf(d2, 1e-37f));
-            s -= slope[e] * kLog2E * (d2 * inv);
           }
-          const float p = exp2_fast(s - lse[e]);
+          const float p = exp2_fast(sc(t[i], slope[e] * kLog2E, d2 * inv, c) - lse[e]);
           float d = p * (ds[i] - delta[e]);
           if constexpr (BIASED) {
             const float u = d * inv * slope[e];
@@ -611,7 +687,7 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
             gy = fmaf(u, dy, gy);
             gz = fmaf(u, dz, gz);
           }
-          if constexpr (CAPPED) d *= 1.f - th * th;
+          if constexpr (CAPPED) d *= fmaf(-c, c, c);
           t[i] = p;
           ds[i] = d;
         }
@@ -626,13 +702,14 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
   gz += half_swap(gz);
   if (!ok) return;
   const int64_t at = (int64_t)key * a.h_kv + hk;
+  const float grad_scale = CAPPED ? 4.f * a.scale : a.scale;
   if (it.slot < 0) {
-    if (a.grad_k) store_cols<T, DP>((T*)a.grad_k + at * a.dim, gk, a.scale, a.dim);
+    if (a.grad_k) store_cols<T, DP>((T*)a.grad_k + at * a.dim, gk, grad_scale, a.dim);
     if (a.grad_v) store_cols<T, DP>((T*)a.grad_v + at * a.dim, gv, 1.f, a.dim);
     if (BIASED && half == 0) w.key_part[at] = f32x4{gx, gy, gz, 0.f};
   } else {
     float* p = w.parts + (((int64_t)it.slot * a.h_kv + hk) * kRowsOf<NW> + (key - it.k_begin)) * (2 * a.dim + 4);
-    store_cols<float, (DP < 32 ? 32 : DP)>(p, gk, a.scale, a.dim);
+    store_cols<float, (DP < 32 ? 32 : DP)>(p, gk, grad_scale, a.dim);
     store_cols<float, (DP < 32 ? 32 : DP)>(p + a.dim, gv, 1.f, a.dim);
     if (half == 0) {
       p[2 * a.dim] = gx;
@@ -643,25 +720,12 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
   }
 }
 
-// Adds the parts of a tile's rows or keys, `width` values for each: a workgroup for each (tile, head), an element of the tile to
-// a thread, its slots in order.  put(row or key, element, sum).
-template <typename Put>
-__device__ __forceinline__ void join_elements(const float* parts, const cgtp_attn_item& it, int head, int heads, int tile, int here,
-                                              int width, Put&& put) {
-  const int64_t step = (int64_t)heads * tile * width;
-  const float* p = parts + ((int64_t)it.first * heads + head) * tile * width;
-  for (int e = blockIdx.y * 256 + threadIdx.x; e < here * width; e += gridDim.y * 256) {
-    float s = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < it.count; ++k) s += p[k * step + e];
-    put(e / width, e % width, s);
-  }
-}
 template <typename T>
 __global__ void __launch_bounds__(256) attn_bwd_k_join_kernel(cgtp_attn_args a, AttnScratch w, int tile) {
   const int hk = blockIdx.x % a.h_kv;
   const cgtp_attn_item it = a.k_joins[blockIdx.x / a.h_kv];
-  join_elements(w.parts, it, hk, a.h_kv, tile, it.k_end - it.k_begin, 2 * a.dim + 4, [&](int key, int d, float s) {
+  join_elements(w.parts, it, hk, a.h_kv, tile, it.k_end - it.k_begin, 2 * a.dim + 4, 0, 2 * a.dim + 4, blockIdx.y, gridDim.y,
+                [&](int key, int d, float s) {
     const int64_t at = (int64_t)(it.k_begin + key) * a.h_kv + hk;
     if (d < a.dim) {
       if (a.grad_k) ((T*)a.grad_k)[at * a.dim + d] = (T)s;
@@ -684,36 +748,24 @@ namespace {
 // ---- launches -----------------------------------------------------------------------------------------------------
 unsigned groups_of(int heads, int each) { return (unsigned)((heads + each - 1) / each); }
 
-template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
+template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
 void q_launch(const AttnLaunch& a, const AttnScratch* w, hipStream_t s) {
   float* parts = (float*)a.workspace;
-  const bool together = BIASED && DP <= 64 && a.together;
-  const int heads = together ? a.h_q : a.h_kv;
-  const unsigned joins = (unsigned)a.n_q_joins * heads;
-  const dim3 threads(64 * NW);
-  if (a.n_q_items && together) {
-    if constexpr (BIASED && DP <= 64) {
-      const unsigned n = (unsigned)a.n_q_items;
-      if (w)
-        hipLaunchKernelGGL((attn_heads_bwd_q_kernel<T, DP, NW, CAPPED>), dim3(n * groups_of(a.h_q, kHeads)), threads, 0, s, a, *w);
-      else
-        hipLaunchKernelGGL((attn_heads_fwd_kernel<T, DP, NW, CAPPED>), dim3(n * groups_of(a.h_q, kHeads)), threads, 0, s, a, parts);
-    }
-  } else if (a.n_q_items) {
-    const dim3 grid((unsigned)a.n_q_items * a.h_kv);
-    if (w) hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NW, BIASED, CAPPED>), grid, threads, 0, s, a, *w);
-    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, BIASED, CAPPED>), grid, threads, 0, s, a, parts);
+  const unsigned n = (unsigned)a.n_q_items * a.h_kv, joins = (unsigned)a.n_q_joins * a.h_kv;
+  if (n) {
+    const dim3 threads(64 * NW * KS);
+    if (w) hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NW, KS, BIASED, CAPPED>), dim3(n), threads, 0, s, a, *w);
+    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, KS, BIASED, CAPPED>), dim3(n), threads, 0, s, a, parts);
   }
   if (!joins) return;
   if (w) {
-    if (together) hipLaunchKernelGGL((attn_heads_bwd_q_join_kernel<T>), dim3(joins, 8), dim3(256), 0, s, a, *w, kRowsOf<NW>);
-    else hipLaunchKernelGGL((attn_bwd_q_join_kernel<T>), dim3(joins * kRowsOf<NW>), dim3(192), 0, s, a, *w, kRowsOf<NW>);
+    hipLaunchKernelGGL((attn_bwd_q_join_kernel<T>), dim3(joins, 8), dim3(256), 0, s, a, *w, kRowsOf<NW>);
   } else if (a.n_q_slots > 16 * a.n_q_joins) {
     // a row's slots are shared out over a workgroup where they are many, else an element's slots are a thread's
     hipLaunchKernelGGL((attn_fwd_join_kernel<T>), dim3(joins * kRowsOf<NW>), dim3(kJoinThreads), 0, s, a, (const float*)parts,
-                       kRowsOf<NW>, heads);
+                       kRowsOf<NW>);
   } else {
-    hipLaunchKernelGGL((attn_fwd_join_few_kernel<T>), dim3(joins, 8), dim3(256), 0, s, a, (const float*)parts, kRowsOf<NW>, heads);
+    hipLaunchKernelGGL((attn_fwd_join_few_kernel<T>), dim3(joins, 8), dim3(256), 0, s, a, (const float*)parts, kRowsOf<NW>);
   }
 }
 template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
@@ -735,8 +787,9 @@ void k_launch(const AttnLaunch& a, const AttnScratch& w, hipStream_t s) {
 }
 template <typename T, int DP, bool BIASED, bool CAPPED>
 void launch_dim(const AttnLaunch& a, const AttnScratch* w, hipStream_t s) {
-  if (a.wide_q) q_launch<T, DP, 4, BIASED, CAPPED>(a, w, s);
-  else q_launch<T, DP, 1, BIASED, CAPPED>(a, w, s);
+  if (a.wide_q == 1) q_launch<T, DP, 4, 1, BIASED, CAPPED>(a, w, s);
+  else if (a.wide_q == 2) q_launch<T, DP, 1, 4, BIASED, CAPPED>(a, w, s);
+  else q_launch<T, DP, 1, 1, BIASED, CAPPED>(a, w, s);
   if (!w) return;
   if (a.wide_k) k_launch<T, DP, 4, BIASED, CAPPED>(a, *w, s);
   else k_launch<T, DP, 1, BIASED, CAPPED>(a, *w, s);

@@ -75,9 +75,7 @@ __global__ void __launch_bounds__(256) attn_slope_kernel(float* out, const float
 int64_t blocks_of(int64_t n) { return (n + kPosNodes - 1) / kPosNodes; }
 
 // Rows that leave partial results.
-int64_t q_parts(const cgtp_attn_args& a) {
-  return (int64_t)a.n_q_slots * (a.together ? a.h_q : a.h_kv) * cgtp_attn_rows(a.wide_q);
-}
+int64_t q_parts(const cgtp_attn_args& a) { return (int64_t)a.n_q_slots * a.h_kv * cgtp_attn_rows(a.wide_q); }
 
 // Workspace of the backward; every buffer starts at a multiple of 256 bytes.  The pieces' results of the two passes share a place.
 struct AttnLayout { int64_t row_part, key_part, slope_part, parts, bytes; };
@@ -104,7 +102,8 @@ int attn_check(const cgtp_attn_args* a) {
   if (a->n_q * (a->h_q / a->h_kv) > 0x7fffffff) return CGTP_ERR_SHAPE;
   if (a->n_q_items < 0 || a->n_q_joins < 0 || a->n_q_slots < 0 || a->n_k_items < 0 || a->n_k_joins < 0 || a->n_k_slots < 0)
     return CGTP_ERR_SHAPE;
-  const int64_t heads = a->together ? a->h_q : a->h_kv, group = a->h_q / a->h_kv;
+  const int64_t heads = a->h_kv, group = a->h_q / a->h_kv;
+  if (a->wide_q < 0 || a->wide_q > 2 || a->wide_k < 0 || a->wide_k > 1) return CGTP_ERR_CONFIG;
   if (a->together && (!a->slope || a->dim > 64 || (group > 2 && group % 4))) return CGTP_ERR_CONFIG;
   if (a->n_q_items * heads >= (1 << 24) || (int64_t)a->n_k_items * a->h_kv >= (1 << 24)) return CGTP_ERR_SHAPE;
   if (a->n_q_joins * heads * cgtp_attn_rows(a->wide_q) >= (1 << 22) ||
@@ -150,7 +149,7 @@ void launch(const cgtp_attn_args& args, const AttnScratch* w, hipStream_t s) {
 
 extern "C" {
 
-int cgtp_attn_rows(int wide) { return wide ? 128 : 32; }
+int cgtp_attn_rows(int wide) { return wide == 1 ? 128 : 32; }
 
 int64_t cgtp_attn_workspace_bytes(const cgtp_attn_args* a, int backward) {
   using namespace cgtp;
@@ -164,7 +163,6 @@ int cgtp_attn_forward(const cgtp_attn_args* a, void* stream) {
   if (int rc = attn_check(a)) return rc;
   if (a->n_q == 0) return CGTP_OK;
   if (a->n_q_slots > 0 && !a->workspace) return CGTP_ERR_WORKSPACE;
-  if (a->together && (!is_fast(*a, false) || !aligned16(a->out))) return CGTP_ERR_ALIGN;
   launch(*a, nullptr, (hipStream_t)stream);
   return hipGetLastError() == hipSuccess ? CGTP_OK : CGTP_ERR_LAUNCH;
 }
@@ -173,11 +171,10 @@ int cgtp_attn_backward(const cgtp_attn_args* a, void* stream) {
   using namespace cgtp;
   if (int rc = attn_check(a)) return rc;
   if ((a->n_k_items && !a->k_items) || (a->n_k_joins && !a->k_joins)) return CGTP_ERR_NULL;
-  if (a->n_q > 0 && (!a->lse || !a->grad_out || (a->together && a->dtype != CGTP_F32 && !a->out_low))) return CGTP_ERR_NULL;
+  if (a->n_q > 0 && (!a->lse || !a->grad_out)) return CGTP_ERR_NULL;
   const AttnLayout l = attn_layout(*a);
   if (l.bytes > 0 && !a->workspace) return CGTP_ERR_WORKSPACE;
-  if (a->together && (!is_fast(*a, true) || !aligned16(a->out) || !aligned16(a->out_low) || !aligned16(a->grad_q) ||
-                      !aligned16(a->grad_k) || !aligned16(a->grad_v)))
+  if (a->together && (!is_fast(*a, true) || !aligned16(a->grad_k) || !aligned16(a->grad_v)))
     return CGTP_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)a->workspace;

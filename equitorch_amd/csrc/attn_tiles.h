@@ -78,7 +78,7 @@ struct RowFrag {
   }
 };
 
-// A tile between memory and LDS.  Offset(i): bytes from `base` of row i, kNoRow for none; Pointer(i): the row, null for none.
+// A tile between memory and LDS, moved by THREADS neighbouring threads.  Offset(i): bytes from `base` of row i, kNoRow for none; Pointer(i): the row, null for none.
 template <typename T, int DP, int THREADS, int BLOCK>
 struct TileStage {
   using S = AttnShape<T, DP>;
@@ -90,7 +90,7 @@ struct TileStage {
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kNoRow, 0x00027000);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int id = i * THREADS + (int)threadIdx.x, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
+      const int id = i * THREADS + (int)threadIdx.x % THREADS, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
       if (kAll % THREADS != 0 && id >= kAll) break;
       const unsigned o = offset(r);
       reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
@@ -104,7 +104,7 @@ struct TileStage {
     } else {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        const int id = i * THREADS + (int)threadIdx.x, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
+        const int id = i * THREADS + (int)threadIdx.x % THREADS, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
         if (kAll % THREADS != 0 && id >= kAll) break;
         const T* p = pointer(r);
         reg[i] = u32x4_t{0, 0, 0, 0};
@@ -115,7 +115,7 @@ struct TileStage {
   __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int id = i * THREADS + (int)threadIdx.x;
+      const int id = i * THREADS + (int)threadIdx.x % THREADS;
       if (kAll % THREADS != 0 && id >= kAll) break;
       *reinterpret_cast<u32x4_t*>(lds + id * 16) = reg[i];
     }
@@ -143,21 +143,8 @@ __device__ __forceinline__ u32x2_t lds_transposed(const char* p) {
   return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)p));
 }
 
-// Two values rounded to T, as they lie in a register; `rest`: what that took off them.
-template <typename T>
-__device__ __forceinline__ unsigned round_pair(float a, float b, float (&rest)[2]) {
-  typedef T v2 __attribute__((ext_vector_type(2)));
-  const f32x2 f = {a, b};
-  const v2 h = __builtin_convertvector(f, v2);
-  const f32x2 back = __builtin_convertvector(h, f32x2);
-  rest[0] = a - back[0];
-  rest[1] = b - back[1];
-  return __builtin_bit_cast(unsigned, h);
-}
-
-// acc[o] += columns 32 o .. of the tile's 32 rows from `first` on, transposed, times p (rows by lanes' columns).  BOTH: also
-// times what rounding to a 16-bit type takes off p.
-template <typename T, int DP, bool BOTH = false>
+// acc[o] += columns 32 o .. of the tile's 32 rows from `first` on, transposed, times p (rows by lanes' columns).
+template <typename T, int DP>
 __device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* lds, int first, const f32x16_t& p) {
   using S = AttnShape<T, DP>;
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -165,22 +152,17 @@ __device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* lds,
     const int r = first + 4 * half + ((lane & 15) >> 2), d = (lane & 16) + 4 * (lane & 3);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      u32x4_t hi, lo;
+      typedef T v8 __attribute__((ext_vector_type(8)));
+      v8 b;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float rest[2], none[2];
-        hi[j] = round_pair<T>(p[8 * t + 2 * j], p[8 * t + 2 * j + 1], rest);
-        if constexpr (BOTH) lo[j] = round_pair<T>(rest[0], rest[1], none);
-      }
+      for (int j = 0; j < 8; ++j) b[j] = (T)p[8 * t + j];
 #pragma unroll
       for (int o = 0; o < S::kOut; ++o) {
         // DP = 16: the columns 16 .. 31 of the result do not exist; its lanes read the others again
         const int col = DP < 32 ? d & 15 : 32 * o + d;
         const u32x2_t x = lds_transposed(lds + S::slot(r + 16 * t, col >> 3) + (col & 7) * 2);
         const u32x2_t y = lds_transposed(lds + S::slot(r + 16 * t + 8, col >> 3) + (col & 7) * 2);
-        const u32x4_t a = {x[0], x[1], y[0], y[1]};
-        acc[o] = mma_pair<T>(a, hi, acc[o]);
-        if constexpr (BOTH) acc[o] = mma_pair<T>(a, lo, acc[o]);
+        acc[o] = mma_pair<T>(u32x4_t{x[0], x[1], y[0], y[1]}, __builtin_bit_cast(u32x4_t, b), acc[o]);
       }
     }
   } else {

@@ -236,15 +236,13 @@ cgtp_attn_args attn_args(const AttnOperands& o, const AttnHandle& h, double scal
   return a;
 }
 
-at::Tensor attn_forward(const AttnOperands& o, const AttnHandle& h, double scale, double cap, at::Tensor* lse, at::Tensor* low) {
+at::Tensor attn_forward(const AttnOperands& o, const AttnHandle& h, double scale, double cap, at::Tensor* lse) {
   c10::hip::HIPGuardMasqueradingAsCUDA guard(o.q.device());
   cgtp_attn_args a = attn_args(o, h, scale, cap);
   at::Tensor out = at::empty(o.q.sizes(), o.q.options());
   if (lse) *lse = at::empty({a.n_q, (int64_t)a.h_q}, o.q.options().dtype(at::kFloat));
-  if (lse && h.together && a.dtype != CGTP_F32) *low = at::empty(o.q.sizes(), o.q.options());
   a.out = out.data_ptr();
   a.lse = lse ? lse->data_ptr() : nullptr;
-  a.out_low = low ? mutable_ptr(*low) : nullptr;
   at::Tensor ws;
   if (a.n_q_slots) {
     ws = bytes_on(o.q, cgtp_attn_workspace_bytes(&a, 0));
@@ -259,9 +257,9 @@ struct Attn : torch::autograd::Function<Attn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Optional& pos_q,
                             const Optional& pos_k, const Optional& slope, const AttnHandle* h, double scale, double cap) {
     const AttnOperands o = {q, k, v, opt(pos_q), opt(pos_k), opt(slope)};
-    at::Tensor lse, low;
-    at::Tensor out = attn_forward(o, *h, scale, cap, &lse, &low);
-    ctx->save_for_backward({q, k, v, o.pos_q, o.pos_k, o.slope, out, lse, h->q_items, h->q_joins, h->k_items, h->k_joins, low});
+    at::Tensor lse;
+    at::Tensor out = attn_forward(o, *h, scale, cap, &lse);
+    ctx->save_for_backward({q, k, v, o.pos_q, o.pos_k, o.slope, out, lse, h->q_items, h->q_joins, h->k_items, h->k_joins});
     auto& d = ctx->saved_data;
     d["shape"] = std::vector<int64_t>{h->q_slots, h->k_slots, h->wide_q, h->wide_k, h->fallback.id, h->together};
     d["scale"] = scale;
@@ -286,7 +284,6 @@ struct Attn : torch::autograd::Function<Attn> {
     if ((uintptr_t)g.data_ptr() & 15) g = g.clone();
     a.out = s[6].data_ptr();
     a.lse = s[7].data_ptr();
-    a.out_low = mutable_ptr(s[12]);
     a.grad_out = g.data_ptr();
     variable_list out(9);
     for (size_t i = 0; i < 6; ++i)
@@ -328,7 +325,7 @@ void bind_node_operators(py::module& m) {
                    const c10::optional<at::Tensor>& pos_k, const c10::optional<at::Tensor>& slope, const AttnHandle& h, double scale,
                    double cap, bool keep) {
     if (keep) return Attn::apply(q, k, v, pos_q, pos_k, slope, &h, scale, cap);
-    return attn_forward({q, k, v, opt(pos_q), opt(pos_k), opt(slope)}, h, scale, cap, nullptr, nullptr);
+    return attn_forward({q, k, v, opt(pos_q), opt(pos_k), opt(slope)}, h, scale, cap, nullptr);
   }, "attention among the nodes of a structure; with its autograd node where a backward may follow (keep)");
 }
 

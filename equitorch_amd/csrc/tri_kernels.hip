@@ -685,7 +685,7 @@ int cgtp_abi_layout(int which, int64_t* out, int capacity) {
                                       CGTP_OFF(cgtp_attn_args, k_head), CGTP_OFF(cgtp_attn_args, v_node),
                                       CGTP_OFF(cgtp_attn_args, v_head), CGTP_OFF(cgtp_attn_args, pos_q),
                                       CGTP_OFF(cgtp_attn_args, pos_k), CGTP_OFF(cgtp_attn_args, slope),
-                                      CGTP_OFF(cgtp_attn_args, out), CGTP_OFF(cgtp_attn_args, lse), CGTP_OFF(cgtp_attn_args, out_low),
+                                      CGTP_OFF(cgtp_attn_args, out), CGTP_OFF(cgtp_attn_args, lse),
                                       CGTP_OFF(cgtp_attn_args, q_items), CGTP_OFF(cgtp_attn_args, q_joins),
                                       CGTP_OFF(cgtp_attn_args, k_items), CGTP_OFF(cgtp_attn_args, k_joins),
                                       CGTP_OFF(cgtp_attn_args, n_q_items), CGTP_OFF(cgtp_attn_args, n_q_joins),

@@ -37,13 +37,13 @@ class _Items:
     """Tables of one pass for the kernels: tiles of ``tile`` rows of every structure, each against the columns of its
     structure, or against a piece of them where there are too few tiles to occupy the GPU."""
 
-    def __init__(self, rows: np.ndarray, cols: np.ndarray, tile: int, heads: int):
+    def __init__(self, rows: np.ndarray, cols: np.ndarray, tile: int, heads: int, waves: int):
         tiles = -(-rows // tile)
         s = np.repeat(np.arange(len(rows)), tiles)                             # structure of every tile
         first_tile = np.cumsum(tiles) - tiles
         begin = (np.arange(len(s)) - first_tile[s]) * tile
         end = np.minimum(begin + tile, rows[s])
-        want = -(-_WAVES * 32 // (tile * heads * max(1, len(s))))              # pieces of a tile
+        want = -(-_WAVES // (waves * heads * max(1, len(s))))                  # pieces of a tile
         pieces = np.clip(cols[s] // _PIECE, 1, max(1, want))
         step = -(-(-(-cols[s] // pieces)) // _BLOCK) * _BLOCK                  # columns of a piece
         pieces = np.maximum(1, -(-cols[s] // np.maximum(step, 1)))
@@ -73,19 +73,21 @@ def _table(columns, order, device) -> Optional[Tensor]:
 
 class _Tables:
     def __init__(self, plan: "AttentionPlan", group: int, heads: int, together: bool):
-        # Heads taken together: a row is a query, and a workgroup has two heads of it, else a query with all its heads of a
-        # head of keys.
         self.together = together
-        if together:
-            group, heads = 1, -(-group * heads // 2)
-        rows, cols = plan.len_q * group, plan.len_k
+        cols, rows = plan.len_k, plan.len_q * group
         if rows.sum() >= 2 ** 31:
             raise CgtpError("queries times query heads of a head of keys must stay below 2^31")
         start_q, start_k = np.cumsum(plan.len_q) - plan.len_q, np.cumsum(cols) - cols
-        # Tiles of 128 rows share a tile of keys among four wavefronts; tiles of 32 rows waste less of a short structure.
-        self.wide_q, self.wide_k = _wide(rows), _wide(cols)
-        q = _Items(rows, cols, 128 if self.wide_q else 32, heads)
-        k = _Items(cols, rows, 128 if self.wide_k else 32, heads)
+        # Tiles of 128 rows share a tile of keys among four wavefronts; tiles of 32 rows waste less of a short structure.  Few
+        # rows against many keys (a readout): four wavefronts share out the keys of a tile of 32 rows.
+        self.wide_q, self.wide_k = int(_wide(rows)), int(_wide(cols))
+        if not self.wide_q and int(cols.sum()) >= 96 * int((-(-rows // 32)).sum()):
+            self.wide_q = 2
+        q = _Items(rows, cols, 128 if self.wide_q == 1 else 32, heads, 4 if self.wide_q else 1)
+        # heads taken together: a row is a query for all query heads of a head of keys, and two heads of keys share a workgroup
+        # where each has one
+        k = _Items(cols, plan.len_q if together else rows, 128 if self.wide_k else 32,
+                   -(-heads // 2) if together and group == 1 else heads, 4 if self.wide_k else 1)
         zero = np.zeros_like(q.begin)
         at = start_k[q.structure]
         self.q_items = _table((start_q[q.structure], q.begin, q.end, at + q.col_begin, at + q.col_end, q.slot, q.place, zero),
@@ -152,11 +154,10 @@ class AttentionPlan:
         return cls(torch.from_numpy(ptr).to(batch.device))
 
     def tables(self, group: int, heads: int, dim: int, may: bool) -> _Tables:
-        """For ``heads`` heads of keys with ``group`` query heads each.  Distances are formed once for several heads where
-        the operands allow it (``may``: distances, aligned rows) and heads are so narrow that several fit a wavefront's
-        registers, unless the queries are so few that one tile takes all the heads of a structure."""
-        together = may and dim <= 64 and group * heads > 1 and (group <= 2 or group % 4 == 0) \
-            and self.num_queries >= 8 * self.num_structures
+        """For ``heads`` heads of keys with ``group`` query heads each.  The gradients of keys and values are formed for several
+        heads at a time where the operands allow it (``may``: distances, aligned rows) and heads are so narrow that two fit a
+        wavefront's registers."""
+        together = may and dim <= 64 and group * heads > 1 and (group <= 2 or group % 4 == 0)
         key = (group, heads, together)
         if key not in self._tables:
             self._tables[key] = _Tables(self, group, heads, together)
@@ -264,18 +265,17 @@ def _args(q, k, v, pos_q, pos_k, slope, plan, scale, cap) -> AttnArgs:
 
 
 def _forward(q, k, v, pos_q, pos_k, slope, plan, scale, cap, keep):
-    """``(out, lse, out_low)``; the last two, which a backward reads, are None unless ``keep``."""
+    """``(out, lse)``; lse, which a backward reads, is None unless ``keep``."""
     a = _args(q, k, v, pos_q, pos_k, slope, plan, scale, cap)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if keep else None
-    low = torch.empty(q.shape, dtype=q.dtype, device=q.device) if keep and a.together and q.dtype != torch.float32 else None
-    a.out, a.lse, a.out_low = out.data_ptr(), _lib.ptr(lse), _lib.ptr(low)
+    a.out, a.lse = out.data_ptr(), _lib.ptr(lse)
     ws = None
     if a.n_q_slots:
         ws = torch.empty(_lib.lib.cgtp_attn_workspace_bytes(C.byref(a), 0), dtype=torch.uint8, device=q.device)
         a.workspace = ws.data_ptr()
     _lib.check(_lib.lib.cgtp_attn_forward(C.byref(a), _lib.stream_ptr(q.device)), "cgtp_attn_forward")
-    return out, lse, low
+    return out, lse
 
 
 class _SegmentAttention(Function):
@@ -283,14 +283,14 @@ class _SegmentAttention(Function):
 
     @staticmethod
     def forward(ctx, q, k, v, pos_q, pos_k, slope, plan, scale, cap):
-        out, lse, low = _forward(q, k, v, pos_q, pos_q if pos_k is None else pos_k, slope, plan, scale, cap, True)
-        ctx.save_for_backward(q, k, v, pos_q, pos_k, slope, out, lse, low)
+        out, lse = _forward(q, k, v, pos_q, pos_q if pos_k is None else pos_k, slope, plan, scale, cap, True)
+        ctx.save_for_backward(q, k, v, pos_q, pos_k, slope, out, lse)
         ctx.plan, ctx.scale, ctx.cap = plan, scale, cap
         return out
 
     @staticmethod
     def backward(ctx, g):
-        q, k, v, pos_q, pos_k, slope, out, lse, low = ctx.saved_tensors
+        q, k, v, pos_q, pos_k, slope, out, lse = ctx.saved_tensors
         need, plan, scale, cap = ctx.needs_input_grad[:6], ctx.plan, ctx.scale, ctx.cap
         if torch.is_grad_enabled():
             expression = _of_buckets(plan._buckets, scale, cap)
@@ -298,7 +298,7 @@ class _SegmentAttention(Function):
         g = g.contiguous()
         g = g if g.data_ptr() % 16 == 0 else g.clone()
         a = _args(q, k, v, pos_q, pos_q if pos_k is None else pos_k, slope, plan, scale, cap)
-        a.out, a.lse, a.out_low, a.grad_out = out.data_ptr(), lse.data_ptr(), _lib.ptr(low), g.data_ptr()
+        a.out, a.lse, a.grad_out = out.data_ptr(), lse.data_ptr(), g.data_ptr()
         grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None
                  for t, n in zip((q, k, v, pos_q, pos_k, slope), need)]
         a.grad_q, a.grad_k, a.grad_v, a.grad_pos_q, a.grad_pos_k, a.grad_slope = (_lib.ptr(t) for t in grads)

@@ -799,23 +799,23 @@ int cgtp_gff_backward(const cgtp_gff_args* args, void* stream);
 /* ---- attention among the nodes of a structure ---------------------------------------------------------------------
  * Nodes of many structures lie one after the other; every query of a structure sees all keys of the same structure:
  *   s_ij = cap tanh(scale q_i.k_j / cap) - slope_h |r_i - r_j|     (cap <= 0: scale q_i.k_j;  slope NULL: no distance)
- *   out_i = sum_j softmax_j(s_ij) v_j,  lse_i = log2 of the sum of 2^(s log2 e);  no key, or every score -inf: out_i = 0 and
+ *   out_i = sum_j softmax_j(s_ij) v_j,  lse_i = log2 of the sum of 2^(s log2 e), less cap log2 e where there is a cap;  no key, or every score -inf: out_i = 0 and
  *   lse_i = +inf.
  * q: (n_q, h_q, dim), k and v: (n_k, h_kv, dim), h_q a multiple of h_kv (query head h reads head h / (h_q / h_kv)), with
  * element strides *_node and *_head and contiguous along dim; out, grad_out and the gradients contiguous; lse (n_q, h_q)
  * fp32; pos_q (n_q, 3), pos_k (n_k, 3), slope (h_q) fp32.  lse NULL: not wanted.  Elements may lie anywhere an element may.  dim <= 128.
  *
  * The caller cuts the work into items.  The rows of a structure and a head of keys are its (query, query head) pairs, row =
- * query * (h_q / h_kv) + head.  q_items: tiles of at most cgtp_attn_rows(wide_q) rows against a range of keys, which the
- * forward and the gradient of q walk; k_items: at most cgtp_attn_rows(wide_k) keys against a range of rows.  An item that
+ * query * (h_q / h_kv) + head.  q_items: tiles of at most cgtp_attn_rows(wide_q) rows (wide_q 0: a wavefront, 1: four, for
+ * each tile; 2: four that share out the keys, for few rows against many) against a range of keys, which the forward
+ * and the gradient of q walk; k_items: at most cgtp_attn_rows(wide_k) keys against a range of rows.  An item that
  * covers all keys (rows) of its structure writes its result and has slot -1 and first 0; one that covers a part has a
  * slot of its own, where it leaves partial results, and first = its place among the pieces of its tile; one entry of q_joins /
  * k_joins adds the slots first .. first + count - 1 of a tile, in that order.  A structure without keys has items with an
  * empty range.  Every query and every key belongs to exactly one tile.
- * together != 0: with slope, dim <= 64, h_q / h_kv 1, 2 or a multiple of 4, and q, k, v, out, out_low, grad_out, grad_q, grad_k
- * and grad_v aligned to 16 bytes with dim and strides a multiple of that (else CGTP_ERR_ALIGN), several heads are taken at a time; the rows of
- * the items are then the queries, each for all heads.  The backward then reads out_low in 16-bit types (NULL in fp32): what
- * rounding has taken off out, in the same type, which the forward leaves where out_low is not NULL; lse is that call's own.
+ * together != 0: the pass over the k_items takes several heads at a time, and their rows are queries, each for all query heads
+ * of a head of keys.  It needs slope, dim <= 64, h_q / h_kv 1, 2 or a multiple of 4, and q, k, v, grad_out, grad_k and grad_v
+ * aligned to 16 bytes with dim and strides a multiple of that (else CGTP_ERR_ALIGN).
  * workspace: cgtp_attn_workspace_bytes(args, backward), 16-byte aligned (0: may be NULL).
  * cgtp_attn_backward writes grad_q, grad_k, grad_v and, with slope, grad_slope (h_q) and grad_pos_q (n_q, 3) where they are
  * not NULL; same_pos != 0: the queries' and the keys' positions are one tensor, and grad_pos_q is the whole gradient, else
@@ -829,7 +829,7 @@ typedef struct {
   const void *q, *k, *v;
   int64_t q_node, q_head, k_node, k_head, v_node, v_head;
   const float *pos_q, *pos_k, *slope;
-  void *out, *lse, *out_low;
+  void *out, *lse;
   const cgtp_attn_item *q_items, *q_joins, *k_items, *k_joins;
   int32_t n_q_items, n_q_joins, n_q_slots, n_k_items, n_k_joins, n_k_slots;
   const void* grad_out;

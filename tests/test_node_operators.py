@@ -107,7 +107,7 @@ def test_attention_tables_cover_every_pair_once(len_q, len_k, group, heads):
     len_k = len_q if len_k is None else len_k
     t = plan.tables(group, heads, 32, False)
     start_q, start_k = ptr(len_q).tolist(), ptr(len_k).tolist()
-    for items, joins, slots, tile, keyed in ((t.q_items, t.q_joins, t.q_slots, 128 if t.wide_q else 32, False),
+    for items, joins, slots, tile, keyed in ((t.q_items, t.q_joins, t.q_slots, 128 if t.wide_q == 1 else 32, False),
                                              (t.k_items, t.k_joins, t.k_slots, 128 if t.wide_k else 32, True)):
         seen = {s: np.zeros((len_q[s] * group, len_k[s]), dtype=int) for s in range(len(len_q))}
         fixed = {s: np.zeros(len_k[s] if keyed else len_q[s] * group, dtype=int) for s in range(len(len_q))}
