@@ -8,6 +8,7 @@ from .rotations import AnglesToMatrix
 from .cutoffs import CosineCutoff, MollifierCutoff, PolynomialCutoff
 from .linears import IrrepsLinear, IrrepWiseLinear, SO2Linear, SO3Linear
 from .norm import MeanSquaredNorm, Norm, SquaredNorm
+from .nodes import Embedding, GatedFeedForward, SegmentAttention
 from .normalization import BatchRMSNorm, LayerRMSNorm
 from .radials import BesselBasis
 from .init import initialize_linear, initialize_so3_so2_linear, initialize_tensor_product
@@ -19,4 +20,4 @@ __all__ = ["SO3Linear", "IrrepsLinear", "IrrepWiseLinear", "TensorProduct", "Sph
            "BatchRMSNorm", "LayerRMSNorm", "BesselBasis", "PolynomialCutoff", "CosineCutoff", "MollifierCutoff",
            "SO2Linear", "SinCos", "SparseWignerRotation", "DenseWignerRotation", "WignerD", "AlignToZWignerD",
            "Dropout", "SplitIrreps", "Separable", "AnglesToMatrix", "TensorDot", "XYZToSinCos", "initialize_tensor_product",
-           "initialize_so3_so2_linear", "initialize_linear", "functional"]
+           "initialize_so3_so2_linear", "initialize_linear", "Embedding", "SegmentAttention", "GatedFeedForward", "functional"]
