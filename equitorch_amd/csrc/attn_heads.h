@@ -1,9 +1,9 @@
 // The gradient with the keys fixed for the attention with distances, dim <= 64, two heads at a time: the distance of a pair and
 // what its gradient takes cost as many instructions as the rest of a score, and are the same for all heads.  A row is a query
 // here, and a wavefront holds 32 keys of two heads, or of one head of keys with two of its query heads.  Vector instructions
-// bound it: 34 issue slots for a score with a cap (an exponential, reciprocal or root takes four), 41 with one head at a
-// time; 300 structures of 40 to 250 nodes, 8 heads of 32, bf16: 118 -> 99 us, three of 2000 to 5000, 8 query heads on 4 of
-// 64: 618 -> 486.  With the rows fixed the same saves nothing: two heads' queries, gradients and results leave too few
+// bound it (an exponential, reciprocal or root takes four issue slots): 300 structures of 40 to 250 nodes, 8 heads of 32, bf16:
+// 118 us one head at a time, 102 so, three of 2000 to 5000, 8 query heads on 4 of 64: 618 and 510.  With the
+// rows fixed the same saves nothing: two heads' queries, gradients and results leave too few
 // registers for two wavefronts on a SIMD.
 //
 // The scheduling barriers keep reads from LDS that are needed later out of the registers.  Rows are whole aligned chunks
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_heads_bwd_k_kernel(AttnLaunch
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
   const int key = it.k_begin + wave * 32 + (lane & 31);
   const bool ok = key < it.k_end;
-  const Score<true, CAPPED> score(a);
+  const Score<T, true, CAPPED> score(a);
   RowFrag<T, DP> k[SETS], v[SETS];
   AttnAcc<T, DP> gk[SETS], gv[SETS];
 #pragma unroll
@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_heads_bwd_k_kernel(AttnLaunch
         const char* q_tile = tile + 2 * j * kTile;
         const float slope = a.slope[h0 + j], by = slope * kLog2E;
         f32x16_t t = rows_times<T, DP>(q_tile, 32 * b, k[SHARED ? 0 : j]);
+        score.of(t);
         f32x16_t ds = rows_times<T, DP>(q_tile + kTile, 32 * b, v[SHARED ? 0 : j]);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -164,12 +165,10 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_heads_bwd_k_kernel(AttnLaunch
           const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[buf][4 + 2 * j][first]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float c;
-            const float s = score(t[4 * g + e], by, dist[4 * g + e], c);
-            const float p = exp2_fast(s - lse[e]);
+            const float p = exp2_fast(score.less(t[4 * g + e], by, dist[4 * g + e]) - lse[e]);
             float d = p * (ds[4 * g + e] - delta[e]);
             weight[4 * g + e] = fmaf(slope, d, weight[4 * g + e]);
-            if constexpr (CAPPED) d *= fmaf(-c, c, c);
+            if constexpr (CAPPED) d *= score.through(t[4 * g + e]);
             t[4 * g + e] = p;
             ds[4 * g + e] = d;
           }
@@ -186,7 +185,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_heads_bwd_k_kernel(AttnLaunch
 #pragma unroll
   for (int d = 0; d < 3; ++d) moved[d] += half_swap(moved[d]);
   if (!ok) return;
-  const float scale = CAPPED ? 4.f * a.scale : a.scale;
+  const float scale = a.scale;
 #pragma unroll
   for (int j = 0; j < SETS; ++j) {
     if (j >= sets) continue;
