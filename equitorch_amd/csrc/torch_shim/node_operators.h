@@ -119,9 +119,10 @@ at::Tensor gff_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tens
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   cgtp_gff_args a = gff_args(x, wg, wu, wd, act);
   at::Tensor out = at::empty({a.n_rows, a.c_out}, x.options());
-  *kept = at::empty({keep ? 3 : 1, a.n_rows, a.hidden}, x.options());
+  const int64_t width = (a.hidden + 7) / 8 * 8;
+  *kept = at::empty({keep ? 3 : 1, a.n_rows, width}, x.options());
   char* p = (char*)kept->data_ptr();
-  const int64_t each = a.n_rows * a.hidden * x.element_size();
+  const int64_t each = a.n_rows * width * x.element_size();
   if (keep) {
     a.gate = p;
     a.up = p + each;
@@ -161,8 +162,9 @@ struct Gff : torch::autograd::Function<Gff> {
     variable_list out(6);
     for (size_t i = 0; i < 4; ++i)
       if (need[i]) out[i] = at::empty(s[i].sizes(), s[i].options());
-    const at::Tensor mids = at::empty({2, a.n_rows, a.hidden}, x.options());
-    const int64_t each = a.n_rows * a.hidden * x.element_size();
+    const int64_t width = kept.size(2);
+    const at::Tensor mids = at::empty({2, a.n_rows, width}, x.options());
+    const int64_t each = a.n_rows * width * x.element_size();
     char *p = (char*)kept.data_ptr(), *q = (char*)mids.data_ptr();
     a.gate = p;
     a.up = p + each;

@@ -29,7 +29,7 @@ def _args(x, w_gate, w_up, w_down, mid, code, act) -> GffArgs:
 
 def _forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, act: int, keep: bool):
     """``(out, gate, up, mid)``; gate and up are None unless ``keep``."""
-    n, h = x.shape[0], w_gate.shape[1]
+    n, h = x.shape[0], (w_gate.shape[1] + 7) // 8 * 8
     out = torch.empty((n, w_down.shape[1]), dtype=x.dtype, device=x.device)
     if keep:
         gate, up, mid = torch.empty((3, n, h), dtype=x.dtype, device=x.device)

@@ -777,8 +777,9 @@ int cgtp_embed_backward(const int64_t* kind, const void* grad_out, void* grad_ta
  *   g = x Wg,  u = x Wu,  m = act(g) * u,  out = m Wd
  * x: (n_rows, c_in); w_gate, w_up: (c_in, hidden); w_down: (hidden, c_out); out: (n_rows, c_out), all contiguous, aligned to
  * an element.  Products and the activation in fp32; mid (and gate, up), which the forward leaves for the next product
- * and for the backward, are (n_rows, hidden) in the operands' type.  gate and up NULL: not wanted (inference).
- * cgtp_gff_backward reads gate, up and mid, writes grad_gate and grad_up (buffers of the caller, (n_rows, hidden)) and those
+ * and for the backward, are (n_rows, hidden rounded up to a multiple of eight) in the operands' type, aligned to 16 bytes (else
+ * CGTP_ERR_ALIGN), as are grad_gate and grad_up.  gate and up NULL: not wanted (inference).
+ * cgtp_gff_backward reads gate, up and mid, writes grad_gate and grad_up (buffers of the caller) and those
  * of grad_x, grad_w_gate, grad_w_up, grad_w_down that are not NULL; the weight gradients are summed over rows in a
  * fixed order.  workspace: cgtp_gff_workspace_bytes (0: may be NULL), 16-byte aligned.
  * n_rows < 2^31, c_in and c_out < 2^15, hidden < 2^17.  dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16.

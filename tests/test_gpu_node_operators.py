@@ -475,3 +475,40 @@ def test_extension_and_ctypes_issue_the_same_launches(device):
         assert torch.equal(a, b)
     for a, b in zip(seen[0][-7:], seen[1][-7:]):            # tensor expressions: sums of the library's own order
         assert torch.allclose(a, b, rtol=1e-4, atol=1e-5 * float(b.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,c,h,co,activation", [(17001, 35, 130, 21, "silu"), (2100, 130, 1003, 67, "gelu"),
+                                                    (33001, 9, 15, 13, "sigmoid"), (4001, 64, 520, 33, "silu")])
+def test_gated_feed_forward_of_many_odd_rows(device, dtype, rows, c, h, co, activation):
+    """Rows that are not whole aligned groups in a call large enough that they are copied first."""
+    test_gated_feed_forward(device, dtype, rows, c, h, co, activation)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_gated_feed_forward_of_many_odd_rows_passes_on_what_is_not_finite(device, value):
+    from equitorch_amd.nn.functional import gated_feed_forward
+    gen = torch.Generator().manual_seed(3)
+    x = _rand(gen, 9000, 31).to(device)
+    ws = [_rand(gen, *s, std=0.2).to(device) for s in ((31, 250), (31, 250), (250, 30))]
+    clean = gated_feed_forward(x, *ws)
+    x[777, 30] = value
+    out = gated_feed_forward(x, *ws)
+    keep = torch.arange(9000, device=device) != 777
+    assert torch.equal(out[keep], clean[keep]) and not torch.isfinite(out[777]).any()
+
+
+def test_gated_feed_forward_at_unaligned_addresses(device):
+    """The same numbers at addresses that are multiples of an element only, and in place of aligned ones."""
+    from equitorch_amd.nn.functional import gated_feed_forward
+    gen = torch.Generator().manual_seed(4)
+    shapes = ((8192, 32), (32, 256), (32, 256), (256, 32))
+    data = [_rand(gen, *s, dtype=BF16, std=0.3).to(device) for s in shapes]
+    loose = [torch.empty(t.numel() + 1, dtype=BF16, device=device)[1:].view(t.shape).copy_(t) for t in data]
+    results = []
+    for given in (data, loose):
+        leaves = [t.detach().requires_grad_(True) for t in given]
+        out = gated_feed_forward(*leaves)
+        results.append((out, *torch.autograd.grad(out.float().sum(), leaves)))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)

@@ -9,7 +9,7 @@ import torch
 from equitorch_amd import _lib
 from equitorch_amd._lib import AttnArgs, CgtpError, GffArgs
 
-NULL, SHAPE, DTYPE, CONFIG, WORKSPACE = 1, 2, 4, 5, 8
+NULL, SHAPE, DTYPE, CONFIG, ALIGN, WORKSPACE = 1, 2, 4, 5, 6, 8
 
 
 class _Item(C.Structure):
@@ -64,6 +64,20 @@ def test_feed_forward_workspace():
     a = _gff(n_rows=100000, grad_w_gate=4096)
     assert _lib.lib.cgtp_gff_workspace_bytes(C.byref(a), 1) > 0
     assert _lib.lib.cgtp_gff_backward(C.byref(a), None) == WORKSPACE
+
+
+def test_feed_forward_copies_rows_of_large_calls():
+    def need(n_rows, c, backward):
+        a = _gff(n_rows=n_rows, c_in=c, hidden=250, c_out=8, dtype=2, grad_x=4096)
+        return _lib.lib.cgtp_gff_workspace_bytes(C.byref(a), backward)
+    rows, weights = 20000, (15 + 15) * 256 + 250 * 8
+    assert need(rows, 15, 0) == 2 * (rows * 16 + weights)
+    assert need(rows, 15, 1) >= 2 * (rows * 16 + weights + rows * 8)
+    assert need(100, 15, 0) == 0
+    for name in ("mid", "gate"):
+        assert _lib.lib.cgtp_gff_forward(C.byref(_gff(**{name: 4098})), None) == ALIGN
+    for name in ("mid", "up", "grad_gate", "grad_up"):
+        assert _lib.lib.cgtp_gff_backward(C.byref(_gff(**{name: 4098})), None) == ALIGN
 
 
 def _attn(**changed):
