@@ -9,7 +9,7 @@ import torch
 from equitorch_amd import _lib
 from equitorch_amd._lib import AttnArgs, CgtpError, GffArgs
 
-NULL, SHAPE, DTYPE, CONFIG, ALIGN, WORKSPACE = 1, 2, 4, 5, 6, 8
+NULL, SHAPE, ALIGN, DTYPE, CONFIG, WORKSPACE = 1, 2, 3, 4, 5, 8
 
 
 class _Item(C.Structure):
