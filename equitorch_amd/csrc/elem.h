@@ -16,42 +16,6 @@ template <> struct AccOf<double> { using type = double; };
 template <typename T, int V> struct ElemVec { typedef T type __attribute__((ext_vector_type(V))); };
 template <typename T> struct ElemVec<T, 1> { typedef T type; };
 
-// V consecutive elements, widened to the accumulation type.
-template <typename T, int V, typename A>
-__device__ __forceinline__ void load_elems(A (&dst)[V], const T* p) {
-  if constexpr (V == 1) {
-    dst[0] = (A)p[0];
-  } else {
-    const typename ElemVec<T, V>::type v = *reinterpret_cast<const typename ElemVec<T, V>::type*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) dst[i] = (A)v[i];
-  }
-}
-template <typename T, int V, typename A>
-__device__ __forceinline__ void store_elems(T* p, const A (&src)[V]) {
-  if constexpr (V == 1) {
-    p[0] = (T)src[0];
-  } else {
-    typename ElemVec<T, V>::type v;
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (T)src[i];
-    *reinterpret_cast<typename ElemVec<T, V>::type*>(p) = v;
-  }
-}
-
-// The same past the caches' keep: what is written once should not displace what is read again.
-template <typename T, int V, typename A>
-__device__ __forceinline__ void store_elems_stream(T* p, const A (&src)[V]) {
-  if constexpr (V == 1) {
-    p[0] = (T)src[0];
-  } else {
-    typename ElemVec<T, V>::type v;
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (T)src[i];
-    __builtin_nontemporal_store(v, reinterpret_cast<typename ElemVec<T, V>::type*>(p));
-  }
-}
-
 typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -59,6 +23,33 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 // Vectors at an address aligned to an element only: the hardware reads and writes such by itself.  Their type is an integer
 // vector on purpose: taken as elements, the compiler splits the access.
 template <typename T, typename R> struct LooseOf { typedef R type __attribute__((aligned(sizeof(T)))); };
+
+// V elements, 16 bytes of them or one, widened to the accumulation type.
+template <typename T, int V, typename A>
+__device__ __forceinline__ void load_elems(A (&dst)[V], const T* p) {
+  if constexpr (V == 1) {
+    dst[0] = (A)p[0];
+  } else {
+    static_assert(V * sizeof(T) == 16);
+    const typename ElemVec<T, V>::type v = __builtin_bit_cast(typename ElemVec<T, V>::type, *reinterpret_cast<const typename LooseOf<T, u32x4_t>::type*>(p));
+#pragma unroll
+    for (int i = 0; i < V; ++i) dst[i] = (A)v[i];
+  }
+}
+// STREAM: past the caches' keep: what is written once should not displace what is read again.
+template <typename T, int V, bool STREAM = false, typename A>
+__device__ __forceinline__ void store_elems(T* p, const A (&src)[V]) {
+  if constexpr (V == 1) {
+    p[0] = (T)src[0];
+  } else {
+    typename ElemVec<T, V>::type v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (T)src[i];
+    const u32x4_t r = __builtin_bit_cast(u32x4_t, v);
+    if constexpr (STREAM) __builtin_nontemporal_store(r, reinterpret_cast<typename LooseOf<T, u32x4_t>::type*>(p));
+    else *reinterpret_cast<typename LooseOf<T, u32x4_t>::type*>(p) = r;
+  }
+}
 
 // N = sizeof(R) / sizeof(T) elements, the ones from `valid` (at least 1) on as zeros.  Only a vector that crosses the end is
 // taken apart.

@@ -11,6 +11,10 @@
 // a few kinds may hold most rows (elements), or most kinds a row or two (environments), and neither leaves compute
 // units idle.  A run of equal kinds inside a chunk goes straight to the table; the run a chunk begins with and the one it
 // ends with are left as fp32 partial sums (fp64 for fp64) and joined by the workgroup of the chunk where the run begins.
+//
+// A lane takes 16 bytes of a row, wherever it starts; where a row is not whole vectors its last one is taken from its end, and
+// the columns that this vector shares with the one before are computed and written twice, with the same bits.
+// Lookup and gradient of 1000003 rows of 201 channels, 30000 kinds, bf16: 605 us an element at a time, 290 so, 200 channels 265.
 #include "elem.h"
 
 #include <algorithm>
@@ -35,7 +39,8 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const int64_t* __restric
     int64_t k[kRows];
 #pragma unroll
     for (int j = 0; j < kRows; ++j) k[j] = row + j * stride < n_rows ? kind[row + j * stride] : -1;
-    for (int c = sub * V; c < C; c += step) {
+    for (int at = sub * V; at < C; at += step) {
+      const int c = min(at, C - V);
       A v[kRows][V];
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
@@ -46,7 +51,7 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const int64_t* __restric
       }
 #pragma unroll
       for (int j = 0; j < kRows; ++j)
-        if (row + j * stride < n_rows) store_elems_stream<T, V>(out + (row + j * stride) * C + c, v[j]);
+        if (row + j * stride < n_rows) store_elems<T, V, true>(out + (row + j * stride) * C + c, v[j]);
     }
   }
 }
@@ -177,11 +182,10 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const T* __restrict__ gr
   __shared__ int head_key[256], tail_key[256];           // tail_key -1: the group's part is one run; head_key -1: it is empty
   const int groups = 256 >> lpr_log2, lpr = 1 << lpr_log2;
   const int sub = threadIdx.x & (lpr - 1), g = threadIdx.x >> lpr_log2;
-  const int c = (blockIdx.y * lpr + sub) * V;
-  const bool col_ok = c < C;
+  const int at_c = (blockIdx.y * lpr + sub) * V, c = min(at_c, C - V);
+  const bool col_ok = at_c < C;
   const int64_t p0 = ((int64_t)blockIdx.x * groups + g) * per_group;
   const int64_t p1 = p0 + per_group < n_rows ? p0 + per_group : n_rows;
-  const int cc = col_ok ? c : 0;
   auto put = [&](int key, const A (&s)[V]) {
     if (!col_ok || key >= n_kinds) return;
     A o[V];
@@ -211,7 +215,7 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const T* __restrict__ gr
     for (int j = 0; j < kAhead; ++j) {
       const int64_t at = p + j < p1 ? p + j : p1 - 1;
       key[j] = keys[at];
-      load_elems<T, V>(v[j], grad_out + (int64_t)rows[at] * C + cc);
+      load_elems<T, V>(v[j], grad_out + (int64_t)rows[at] * C + c);
     }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
@@ -346,11 +350,11 @@ struct EmbedPlan {
 };
 
 template <typename T>
-EmbedPlan embed_plan(int64_t n_rows, int64_t n_kinds, int C, bool aligned) {
+EmbedPlan embed_plan(int64_t n_rows, int64_t n_kinds, int C) {
   using A = typename AccOf<T>::type;
   EmbedPlan p;
   constexpr int VW = 16 / sizeof(T);
-  p.v = aligned && C % VW == 0 ? VW : 1;
+  p.v = C >= VW ? VW : 1;
   p.lpr_log2 = log2_up((C + p.v - 1) / p.v, 6);
   p.groups = 256 >> p.lpr_log2;
   p.per_group = sum_per_group(n_rows, p.groups);
@@ -385,8 +389,8 @@ template <typename T>
 int embed_forward(const int64_t* kind, const void* table, void* out, int64_t n_rows, int64_t n_kinds, int C, double scale,
                   hipStream_t stream) {
   constexpr int VW = 16 / sizeof(T);
-  const bool vec = aligned16(table) && aligned16(out) && C % VW == 0;
-  const int lpr_log2 = log2_up(vec ? C / VW : C, 8);
+  const bool vec = C >= VW;
+  const int lpr_log2 = log2_up(vec ? (C + VW - 1) / VW : C, 8);
   // a row for each group while that leaves compute units idle, else four
   const int64_t threads = n_rows << lpr_log2;
   const int64_t blocks = std::min<int64_t>(threads < 2048 * 256 ? (threads + 255) / 256 : (threads + 1023) / 1024, kMaxBlocks);
@@ -400,7 +404,7 @@ template <typename T>
 int embed_backward(const int64_t* kind, const void* grad_out, void* grad_table, void* workspace, int64_t n_rows,
                    int64_t n_kinds, int C, double scale, hipStream_t stream) {
   using A = typename AccOf<T>::type;
-  const EmbedPlan p = embed_plan<T>(n_rows, n_kinds, C, aligned16(grad_out) && aligned16(grad_table));
+  const EmbedPlan p = embed_plan<T>(n_rows, n_kinds, C);
   char* ws = (char*)workspace;
   int32_t* digits = (int32_t*)(ws + p.digits);
   for (int pass = 0; pass < p.passes; ++pass) {
@@ -439,15 +443,9 @@ extern "C" {
 int64_t cgtp_embed_workspace_bytes(int64_t n_rows, int64_t n_kinds, int C, int dtype) {
   using namespace cgtp;
   if (embed_check(n_rows, n_kinds, C, dtype) != CGTP_OK || n_rows == 0) return 0;
-  // the same for aligned and unaligned tensors: the larger of the two
-  int64_t most = 0;
-  for (int aligned = 0; aligned < 2; ++aligned) {
-    const int64_t n = dtype == CGTP_F64 ? embed_plan<double>(n_rows, n_kinds, C, aligned).bytes
-                      : dtype == CGTP_F32 ? embed_plan<float>(n_rows, n_kinds, C, aligned).bytes
-                                          : embed_plan<bf16_t>(n_rows, n_kinds, C, aligned).bytes;
-    most = n > most ? n : most;
-  }
-  return most;
+  return dtype == CGTP_F64 ? embed_plan<double>(n_rows, n_kinds, C).bytes
+         : dtype == CGTP_F32 ? embed_plan<float>(n_rows, n_kinds, C).bytes
+                             : embed_plan<bf16_t>(n_rows, n_kinds, C).bytes;
 }
 
 int cgtp_embed_forward(const int64_t* kind, const void* table, void* out, int64_t n_rows, int64_t n_kinds, int C,
