@@ -166,7 +166,7 @@ class AttnArgs(C.Structure):
                 ("grad_pos_q", C.c_void_p), ("grad_pos_k", C.c_void_p), ("grad_slope", C.c_void_p), ("workspace", C.c_void_p),
                 ("n_q", C.c_int64), ("n_k", C.c_int64), ("h_q", C.c_int32), ("h_kv", C.c_int32), ("dim", C.c_int32),
                 ("dtype", C.c_int32), ("wide_q", C.c_int32), ("wide_k", C.c_int32), ("same_pos", C.c_int32),
-                ("together", C.c_int32), ("scale", C.c_float), ("cap", C.c_float)]
+                ("reserved_", C.c_int32), ("scale", C.c_float), ("cap", C.c_float)]
 
 
 def _load():

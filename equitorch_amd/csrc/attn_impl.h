@@ -773,17 +773,7 @@ __global__ void __launch_bounds__(256) attn_bwd_k_join_kernel(cgtp_attn_args a, 
   });
 }
 
-}  // namespace
-}  // namespace cgtp
-
-#include "attn_heads.h"
-
-namespace cgtp {
-namespace {
-
 // ---- launches -----------------------------------------------------------------------------------------------------
-unsigned groups_of(int heads, int each) { return (unsigned)((heads + each - 1) / each); }
-
 template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
 void q_launch(const AttnLaunch& a, const AttnScratch* w, hipStream_t s) {
   float* parts = (float*)a.workspace;
@@ -808,14 +798,7 @@ template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
 void k_launch(const AttnLaunch& a, const AttnScratch& w, hipStream_t s) {
   const unsigned n = (unsigned)a.n_k_items;
   const dim3 threads(64 * NW);
-  if (n && BIASED && DP <= 64 && a.together) {
-    if constexpr (BIASED && DP <= 64) {
-      if (a.h_q == a.h_kv)
-        hipLaunchKernelGGL((attn_heads_bwd_k_kernel<T, DP, NW, CAPPED, false>), dim3(n * groups_of(a.h_kv, kHeads)), threads, 0, s, a, w);
-      else
-        hipLaunchKernelGGL((attn_heads_bwd_k_kernel<T, DP, NW, CAPPED, true>), dim3(n * (unsigned)a.h_kv), threads, 0, s, a, w);
-    }
-  } else if (n) {
+  if (n) {
     hipLaunchKernelGGL((attn_bwd_k_kernel<T, DP, NW, BIASED, CAPPED>), dim3(n * (unsigned)a.h_kv), threads, 0, s, a, w);
   }
   if (a.n_k_joins)

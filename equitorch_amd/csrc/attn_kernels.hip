@@ -104,7 +104,6 @@ int attn_check(const cgtp_attn_args* a) {
     return CGTP_ERR_SHAPE;
   const int64_t heads = a->h_kv, group = a->h_q / a->h_kv;
   if (a->wide_q < 0 || a->wide_q > 2 || a->wide_k < 0 || a->wide_k > 1) return CGTP_ERR_CONFIG;
-  if (a->together && (!a->slope || a->dim > 64 || (group > 2 && group % 4))) return CGTP_ERR_CONFIG;
   if (a->n_q_items * heads >= (1 << 24) || (int64_t)a->n_k_items * a->h_kv >= (1 << 24)) return CGTP_ERR_SHAPE;
   if (a->n_q_joins * heads * cgtp_attn_rows(a->wide_q) >= (1 << 22) ||
       (int64_t)a->n_k_joins * a->h_kv * cgtp_attn_rows(a->wide_k) >= (1 << 22))
@@ -174,8 +173,6 @@ int cgtp_attn_backward(const cgtp_attn_args* a, void* stream) {
   if (a->n_q > 0 && (!a->lse || !a->grad_out)) return CGTP_ERR_NULL;
   const AttnLayout l = attn_layout(*a);
   if (l.bytes > 0 && !a->workspace) return CGTP_ERR_WORKSPACE;
-  if (a->together && (!is_fast(*a, true) || !aligned16(a->grad_k) || !aligned16(a->grad_v)))
-    return CGTP_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)a->workspace;
   const AttnScratch w = {(float*)ws, (f32x4*)(ws + l.row_part), (f32x4*)(ws + l.key_part), (float*)(ws + l.slope_part),

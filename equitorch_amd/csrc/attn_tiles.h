@@ -65,42 +65,28 @@ struct RowFrag {
       if (p && d < dim) f[s] = load_part<u32x4_t, T>(p + d, dim - d);
     }
   }
-  // Rows of whole aligned chunks.
-  __device__ __forceinline__ void load_fast(const T* p, int dim) {
-    using S = AttnShape<T, DP>;
-    const int half = (threadIdx.x & 63) >> 5;
-#pragma unroll
-    for (int s = 0; s < S::kSteps; ++s) {
-      const int d = (2 * s + half) * S::kChunk;
-      f[s] = u32x4_t{0, 0, 0, 0};
-      if (p && d < dim) f[s] = *reinterpret_cast<const u32x4_t*>(p + d);
-    }
-  }
 };
 
-// A tile between memory and LDS, moved by THREADS neighbouring threads.  Offset(i): bytes from `base` of row i, kNoRow for none; Pointer(i): the row, null for none.
+// A tile between memory and LDS, moved by THREADS neighbouring threads.  Offset(i): bytes from `base` of row i, kNoRow for none;
+// Pointer(i): the row, null for none.
 template <typename T, int DP, int THREADS, int BLOCK>
 struct TileStage {
   using S = AttnShape<T, DP>;
   static constexpr int kAll = BLOCK * S::kChunks, kEach = (kAll + THREADS - 1) / THREADS;
   u32x4_t reg[kEach];
 
-  template <typename Offset>
-  __device__ __forceinline__ void load_fast(const T* base, int dim, Offset&& offset) {
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kNoRow, 0x00027000);
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int id = i * THREADS + (int)threadIdx.x % THREADS, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
-      if (kAll % THREADS != 0 && id >= kAll) break;
-      const unsigned o = offset(r);
-      reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-          rsrc, o == kNoRow || c * S::kChunk >= dim ? kNoRow : o + c * 16, 0, 0));
-    }
-  }
   template <typename Offset, typename Pointer>
   __device__ __forceinline__ void load(bool fast, const T* base, int dim, Offset&& offset, Pointer&& pointer) {
     if (fast) {
-      load_fast(base, dim, offset);
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kNoRow, 0x00027000);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int id = i * THREADS + (int)threadIdx.x % THREADS, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
+        if (kAll % THREADS != 0 && id >= kAll) break;
+        const unsigned o = offset(r);
+        reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+            rsrc, o == kNoRow || c * S::kChunk >= dim ? kNoRow : o + c * 16, 0, 0));
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
@@ -179,22 +165,6 @@ __device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* lds,
   }
 }
 
-// Results of a lane's column to a row of whole chunks, aligned to an element's vector of four.
-template <typename T, int DP>
-__device__ __forceinline__ void store_cols_fast(T* p, const AttnAcc<T, DP>& acc, float by, int dim) {
-  const int half = (threadIdx.x & 63) >> 5;
-#pragma unroll
-  for (int o = 0; o < AttnShape<T, DP>::kOut; ++o)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * o + 8 * g + 4 * half;
-      typedef T vec __attribute__((ext_vector_type(4)));
-      vec v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (T)(acc[o][4 * g + e] * by);
-      if (d < dim) *reinterpret_cast<vec*>(p + d) = v;
-    }
-}
 // Results of a lane's column: its elements 32 o + 8 g + 4 (lane / 32) + e of dim, times `by`, to p.
 template <typename T, int DP>
 __device__ __forceinline__ void store_cols(T* p, const AttnAcc<T, DP>& acc, float by, int dim) {

@@ -190,7 +190,7 @@ struct Gff : torch::autograd::Function<Gff> {
 // The kernels' tables of a plan for one number of heads.
 struct AttnHandle {
   at::Tensor q_items, q_joins, k_items, k_joins;
-  int64_t q_slots, k_slots, wide_q, wide_k, together;
+  int64_t q_slots, k_slots, wide_q, wide_k;
   Fallback fallback;
   void set_fallback(py::object fn) { fallback.set(std::move(fn)); }
 };
@@ -234,7 +234,6 @@ cgtp_attn_args attn_args(const AttnOperands& o, const AttnHandle& h, double scal
   a.n_k_slots = (int32_t)h.k_slots;
   a.wide_q = (int32_t)h.wide_q;
   a.wide_k = (int32_t)h.wide_k;
-  a.together = (int32_t)h.together;
   return a;
 }
 
@@ -263,7 +262,7 @@ struct Attn : torch::autograd::Function<Attn> {
     at::Tensor out = attn_forward(o, *h, scale, cap, &lse);
     ctx->save_for_backward({q, k, v, o.pos_q, o.pos_k, o.slope, out, lse, h->q_items, h->q_joins, h->k_items, h->k_joins});
     auto& d = ctx->saved_data;
-    d["shape"] = std::vector<int64_t>{h->q_slots, h->k_slots, h->wide_q, h->wide_k, h->fallback.id, h->together};
+    d["shape"] = std::vector<int64_t>{h->q_slots, h->k_slots, h->wide_q, h->wide_k, h->fallback.id};
     d["scale"] = scale;
     d["cap"] = cap;
     d["keep"] = c10::IValue::make_capsule(c10::make_intrusive<FallbackHolder>(h->fallback));
@@ -280,7 +279,7 @@ struct Attn : torch::autograd::Function<Attn> {
     if (at::GradMode::is_enabled())
       return call_fallback(shape[4], grad[0], {s[0], s[1], s[2], s[3], s[4], s[5]}, need, 9);
     c10::hip::HIPGuardMasqueradingAsCUDA guard(o.q.device());
-    const AttnHandle h{s[8], s[9], s[10], s[11], shape[0], shape[1], shape[2], shape[3], shape[5], {}};
+    const AttnHandle h{s[8], s[9], s[10], s[11], shape[0], shape[1], shape[2], shape[3], {}};
     cgtp_attn_args a = attn_args(o, h, d["scale"].toDouble(), d["cap"].toDouble());
     at::Tensor g = grad[0].contiguous();
     if ((uintptr_t)g.data_ptr() & 15) g = g.clone();
@@ -319,8 +318,8 @@ void bind_node_operators(py::module& m) {
   }, "gated feed-forward block; with its autograd node where a backward may follow (keep)");
   py::class_<AttnHandle>(m, "AttnHandle")
       .def(py::init([](c10::optional<at::Tensor> q_items, c10::optional<at::Tensor> q_joins, c10::optional<at::Tensor> k_items,
-                       c10::optional<at::Tensor> k_joins, int64_t q_slots, int64_t k_slots, int64_t wide_q, int64_t wide_k, int64_t together) {
-        return AttnHandle{opt(q_items), opt(q_joins), opt(k_items), opt(k_joins), q_slots, k_slots, wide_q, wide_k, together, {}};
+                       c10::optional<at::Tensor> k_joins, int64_t q_slots, int64_t k_slots, int64_t wide_q, int64_t wide_k) {
+        return AttnHandle{opt(q_items), opt(q_joins), opt(k_items), opt(k_joins), q_slots, k_slots, wide_q, wide_k, {}};
       }))
       .def("set_fallback", &AttnHandle::set_fallback, "callable (grad_out, inputs, need) -> gradients, for gradients of higher order");
   m.def("attn", [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& pos_q,

@@ -699,7 +699,7 @@ int cgtp_abi_layout(int which, int64_t* out, int capacity) {
                                       CGTP_OFF(cgtp_attn_args, h_q), CGTP_OFF(cgtp_attn_args, h_kv),
                                       CGTP_OFF(cgtp_attn_args, dim), CGTP_OFF(cgtp_attn_args, dtype),
                                       CGTP_OFF(cgtp_attn_args, wide_q), CGTP_OFF(cgtp_attn_args, wide_k),
-                                      CGTP_OFF(cgtp_attn_args, same_pos), CGTP_OFF(cgtp_attn_args, together),
+                                      CGTP_OFF(cgtp_attn_args, same_pos), CGTP_OFF(cgtp_attn_args, reserved_),
                                       CGTP_OFF(cgtp_attn_args, scale), CGTP_OFF(cgtp_attn_args, cap)};
   static const int64_t attn_item[] = {sizeof(cgtp_attn_item), CGTP_OFF(cgtp_attn_item, node),
                                       CGTP_OFF(cgtp_attn_item, row_begin), CGTP_OFF(cgtp_attn_item, row_end),

@@ -72,8 +72,7 @@ def _table(columns, order, device) -> Optional[Tensor]:
 
 
 class _Tables:
-    def __init__(self, plan: "AttentionPlan", group: int, heads: int, together: bool):
-        self.together = together
+    def __init__(self, plan: "AttentionPlan", group: int, heads: int):
         cols, rows = plan.len_k, plan.len_q * group
         if rows.sum() >= 2 ** 31:
             raise CgtpError("queries times query heads of a head of keys must stay below 2^31")
@@ -84,10 +83,7 @@ class _Tables:
         if not self.wide_q and int(cols.sum()) >= 96 * int((-(-rows // 32)).sum()):
             self.wide_q = 2
         q = _Items(rows, cols, 128 if self.wide_q == 1 else 32, heads, 4 if self.wide_q else 1)
-        # heads taken together: a row is a query for all query heads of a head of keys, and two heads of keys share a workgroup
-        # where each has one
-        k = _Items(cols, plan.len_q if together else rows, 128 if self.wide_k else 32,
-                   -(-heads // 2) if together and group == 1 else heads, 4 if self.wide_k else 1)
+        k = _Items(cols, rows, 128 if self.wide_k else 32, heads, 4 if self.wide_k else 1)
         zero = np.zeros_like(q.begin)
         at = start_k[q.structure]
         self.q_items = _table((start_q[q.structure], q.begin, q.end, at + q.col_begin, at + q.col_end, q.slot, q.place, zero),
@@ -114,7 +110,6 @@ class _Tables:
             setattr(a, name, _lib.ptr(t))
             setattr(a, "n_" + name, 0 if t is None else t.shape[0])
         a.n_q_slots, a.n_k_slots, a.wide_q, a.wide_k = self.q_slots, self.k_slots, self.wide_q, self.wide_k
-        a.together = self.together
 
 
 def _wide(n: np.ndarray) -> bool:
@@ -153,22 +148,19 @@ class AttentionPlan:
         ptr = np.concatenate([[0], np.cumsum(np.bincount(b, minlength=n))]).astype(np.int64)
         return cls(torch.from_numpy(ptr).to(batch.device))
 
-    def tables(self, group: int, heads: int, dim: int, may: bool) -> _Tables:
-        """For ``heads`` heads of keys with ``group`` query heads each.  The gradients of keys and values are formed for several
-        heads at a time where the operands allow it (``may``: distances, aligned rows) and heads are so narrow that two fit a
-        wavefront's registers."""
-        together = may and dim <= 64 and group * heads > 1 and (group <= 2 or group % 4 == 0)
-        key = (group, heads, together)
+    def tables(self, group: int, heads: int) -> _Tables:
+        """For ``heads`` heads of keys with ``group`` query heads each."""
+        key = (group, heads)
         if key not in self._tables:
-            self._tables[key] = _Tables(self, group, heads, together)
+            self._tables[key] = _Tables(self, group, heads)
         return self._tables[key]
 
-    def handle(self, mod, group: int, heads: int, dim: int, may: bool, scale: float, cap: float):
+    def handle(self, mod, group: int, heads: int, scale: float, cap: float):
         """The extension's copy of the tables, and the tensor expression its node evaluates under gradient mode."""
-        key = (group, heads, dim, may, scale, cap)
+        key = (group, heads, scale, cap)
         if key not in self._tables:
-            t, buckets = self.tables(group, heads, dim, may), self._buckets
-            h = mod.AttnHandle(t.q_items, t.q_joins, t.k_items, t.k_joins, t.q_slots, t.k_slots, t.wide_q, t.wide_k, t.together)
+            t, buckets = self.tables(group, heads), self._buckets
+            h = mod.AttnHandle(t.q_items, t.q_joins, t.k_items, t.k_joins, t.q_slots, t.k_slots, t.wide_q, t.wide_k)
             # holds the buckets, not the plan: the node keeps it for as long as it lives itself
             h.set_fallback(lambda g, inputs, need: _higher_order(_of_buckets(buckets, scale, cap), inputs, need, g))
             self._tables[key] = h
@@ -242,15 +234,6 @@ def _expression(q, k, v, pos_q, pos_k, slope, padded: _Buckets, scale: float, ca
     return torch.cat(outs)[order].to(dtype)
 
 
-def _aligned(*tensors: Tensor) -> bool:
-    """Whether rows are whole vectors of 16 bytes, aligned."""
-    for t in tensors:
-        chunk = 16 // t.element_size()
-        if t.data_ptr() % 16 or t.shape[2] % chunk or t.stride(0) % chunk or t.stride(1) % chunk:
-            return False
-    return True
-
-
 def _args(q, k, v, pos_q, pos_k, slope, plan, scale, cap) -> AttnArgs:
     a = AttnArgs()
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
@@ -260,7 +243,7 @@ def _args(q, k, v, pos_q, pos_k, slope, plan, scale, cap) -> AttnArgs:
     a.pos_q, a.pos_k, a.slope = _lib.ptr(pos_q), _lib.ptr(pos_k), _lib.ptr(slope)
     a.n_q, a.n_k, a.h_q, a.h_kv, a.dim = q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2]
     a.dtype, a.scale, a.cap = _lib.dtype_code(q.dtype), scale, cap
-    plan.tables(a.h_q // a.h_kv, a.h_kv, a.dim, slope is not None and _aligned(q, k, v)).put(a)
+    plan.tables(a.h_q // a.h_kv, a.h_kv).put(a)
     return a
 
 
@@ -360,7 +343,7 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, pos:
     keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, pos, pos_k, slope))
     mod = _shim.module()
     if mod is not None:
-        handle = plan.handle(mod, q.shape[1] // k.shape[1], k.shape[1], q.shape[2], slope is not None and _aligned(q, k, v), scale, cap)
+        handle = plan.handle(mod, q.shape[1] // k.shape[1], k.shape[1], scale, cap)
         return mod.attn(q, k, v, pos, pos_k, slope, handle, scale, cap, keep)
     if keep:
         return _SegmentAttention.apply(q, k, v, pos, pos_k, slope, plan, scale, cap)

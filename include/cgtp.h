@@ -814,9 +814,6 @@ int cgtp_gff_backward(const cgtp_gff_args* args, void* stream);
  * slot of its own, where it leaves partial results, and first = its place among the pieces of its tile; one entry of q_joins /
  * k_joins adds the slots first .. first + count - 1 of a tile, in that order.  A structure without keys has items with an
  * empty range.  Every query and every key belongs to exactly one tile.
- * together != 0: the pass over the k_items takes several heads at a time, and their rows are queries, each for all query heads
- * of a head of keys.  It needs slope, dim <= 64, h_q / h_kv 1, 2 or a multiple of 4, and q, k, v, grad_out, grad_k and grad_v
- * aligned to 16 bytes with dim and strides a multiple of that (else CGTP_ERR_ALIGN).
  * workspace: cgtp_attn_workspace_bytes(args, backward), 16-byte aligned (0: may be NULL).
  * cgtp_attn_backward writes grad_q, grad_k, grad_v and, with slope, grad_slope (h_q) and grad_pos_q (n_q, 3) where they are
  * not NULL; same_pos != 0: the queries' and the keys' positions are one tensor, and grad_pos_q is the whole gradient, else
@@ -838,7 +835,7 @@ typedef struct {
   float *grad_pos_q, *grad_pos_k, *grad_slope;
   void* workspace;
   int64_t n_q, n_k;
-  int32_t h_q, h_kv, dim, dtype, wide_q, wide_k, same_pos, together;
+  int32_t h_q, h_kv, dim, dtype, wide_q, wide_k, same_pos, reserved_;
   float scale, cap;
 } cgtp_attn_args;
 int cgtp_attn_rows(int wide);

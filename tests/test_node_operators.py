@@ -119,7 +119,7 @@ def test_attention_tables_cover_every_pair_once(len_q, len_k, group, heads):
     ptr = lambda n: torch.tensor([0] + list(n)).cumsum(0)
     plan = AttentionPlan(ptr(len_q)) if len_k is None else AttentionPlan(ptr(len_q), ptr(len_k))
     len_k = len_q if len_k is None else len_k
-    t = plan.tables(group, heads, 32, False)
+    t = plan.tables(group, heads)
     start_q, start_k = ptr(len_q).tolist(), ptr(len_k).tolist()
     for items, joins, slots, tile, keyed in ((t.q_items, t.q_joins, t.q_slots, 128 if t.wide_q == 1 else 32, False),
                                              (t.k_items, t.k_joins, t.k_slots, 128 if t.wide_k else 32, True)):
