@@ -5,9 +5,10 @@
 
 namespace cgtp {
 
-// A call's arguments and what follows from them.
+// A call's arguments: rows of q, k, v and the gradient of the output start at multiples of 16 bytes, what a row has beyond dim in
+// its last 16 bytes is zeros, and a tile's offsets fit 31 bits (a copy has been made of those that were not so).
 struct AttnLaunch : cgtp_attn_args {
-  int fast;            // rows are whole 16-byte chunks, aligned, and a tile's offsets fit 31 bits
+  int64_t g_node, g_head;      // elements between nodes and heads of the gradient of the output
 };
 
 constexpr int kQSums = 10;     // what a piece leaves for each row besides the gradient of q (attn_impl.h, QSums)

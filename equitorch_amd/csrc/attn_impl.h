@@ -28,7 +28,10 @@ namespace {
 constexpr float kLog2E = 1.4426950408889634f;
 
 template <int NW> constexpr int kRowsOf = 32 * NW;
-template <int NW> constexpr int kBlockOf = NW == 1 ? 32 : 64;      // rows of a tile in LDS
+// Rows of a tile in LDS: 64 where four wavefronts move them, half of that for rows beyond 256 bytes, whose tiles on their way
+// leave registers for one wavefront on a SIMD else (20 structures of 1000 nodes, 4 heads of 96, fp32: forward 364 -> 334 us,
+// gradient of keys and values 738 -> 649).
+template <typename T, int DP, int NW> constexpr int kBlockOf = NW == 1 || DP * sizeof(T) > 256 ? 32 : 64;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -120,7 +123,6 @@ struct KeyRows {
   __device__ __forceinline__ KeyRows(const T* p, int64_t node, int64_t head, int hk, int k0, int n)
       : base(p + (int64_t)k0 * node + hk * head), node(node), n(n) {}
   __device__ __forceinline__ unsigned offset(int i) const { return i < n ? (unsigned)i * (unsigned)(node * sizeof(T)) : kNoRow; }
-  __device__ __forceinline__ const T* pointer(int i) const { return i < n ? base + i * node : nullptr; }
 };
 // The rows of a tile, from r0 on, n of them: query0 + (at + i) / group, head (at + i) % group of the kv head's.
 template <typename T>
@@ -139,10 +141,6 @@ struct QueryRows {
     const int q = query(i), h = at + i - q * group;
     return i < n ? (unsigned)q * (unsigned)(node * sizeof(T)) + (unsigned)h * (unsigned)(head * sizeof(T)) : kNoRow;
   }
-  __device__ __forceinline__ const T* pointer(int i) const {
-    const int q = query(i), h = at + i - q * group;
-    return i < n ? base + q * node + h * head : nullptr;
-  }
 };
 
 // One tile buffer of LDS where two would not leave room for two workgroups.
@@ -160,11 +158,18 @@ __device__ __forceinline__ void tile_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 }
-// Bytes of LDS for the tiles, or for half the wavefronts' results of `sums` values for each lane.
+// A wavefront that moves its own tiles of long rows: both tiles of a step on their way at once would take half its registers, and
+// two buffers of both the LDS of most wavefronts that a compute unit has room for.  One tile is fetched while the other
+// one is worked on, into the same registers, and in the forward into the same place.  2000 structures of up to 20 nodes, 8 query
+// heads on 2 of 128, fp32: forward 137 -> 92 us, step 546 -> 350; of 64: 60 -> 44 and 343 -> 186.
+template <typename T, int DP, int NW> constexpr bool kLean = NW == 1 && DP * sizeof(T) > 128;
+
+// Bytes of LDS for the tiles of a step (`lean`: how many of the two are there at a time), or for half the wavefronts' results of
+// `sums` values for each lane.
 template <typename T, int DP, int NW, int KS>
-constexpr int attn_lds(int sums) {
-  constexpr int tile = 2 * kBlockOf<NW> * AttnShape<T, DP>::kRow;
-  const int tiles = KS > 1 ? KS * tile : kBuffers<tile> * tile, join = KS > 1 ? KS / 2 * 64 * (16 * AttnShape<T, DP>::kOut + sums) * 4 : 0;
+constexpr int attn_lds(int lean, int sums) {
+  constexpr int one = kBlockOf<T, DP, NW> * AttnShape<T, DP>::kRow, tile = 2 * one;
+  const int tiles = kLean<T, DP, NW> ? KS * lean * one : KS > 1 ? KS * tile : kBuffers<tile> * tile, join = KS > 1 ? KS / 2 * 64 * (16 * AttnShape<T, DP>::kOut + sums) * 4 : 0;
   return tiles > join ? tiles : join;
 }
 // Halves the number of wavefronts that hold results until one does: give(value place) and take of each value, `n` for a lane.
@@ -184,17 +189,18 @@ __device__ __forceinline__ void join_waves(float* lds, int n, Give&& give, Take&
 
 // ---- forward ----------------------------------------------------------------------------------------------------
 template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
-__global__ void __launch_bounds__(64 * NW * KS, (sizeof(T) == 2 && NW == 4) || DP <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(64 * NW * KS, NW == 4 || DP * sizeof(T) <= 256 ? 2 : 1)
 attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
   using S = AttnShape<T, DP>;
-  constexpr int kBlock = kBlockOf<NW>, kTile = kBlock * S::kRow, kBuf = KS > 1 ? 1 : kBuffers<2 * kTile>;
-  __shared__ alignas(16) char lds[attn_lds<T, DP, NW, KS>(2)];
+  constexpr int kBlock = kBlockOf<T, DP, NW>, kTile = kBlock * S::kRow, kBuf = KS > 1 || kLean<T, DP, NW> ? 1 : kBuffers<2 * kTile>;
+  constexpr bool LEAN = kLean<T, DP, NW>;
+  __shared__ alignas(16) char lds[attn_lds<T, DP, NW, KS>(1, 2)];
   __shared__ alignas(16) float all_pos[KS][2][3][kBlock];
   const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
   const cgtp_attn_item it = a.q_items[blockIdx.x / a.h_kv];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, tid = KS > 1 ? lane : (int)threadIdx.x;
   const int r = it.row_begin + (KS > 1 ? 0 : wave * 32) + (lane & 31), part = KS > 1 ? wave : 0;
-  char* const tiles = lds + part * 2 * kTile;
+  char* const tiles = lds + part * (LEAN ? 1 : 2) * kTile;
   auto& pos = all_pos[part];
   const Row row = row_of(it, r, hk, group);
   const Score<T, BIASED, CAPPED> sc(a);
@@ -213,13 +219,19 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[o][e] = 0.f;
   float top = -INFINITY, sum = 0.f;           // of the row's keys (top), of this lane's (sum)
-  TileStage<T, DP, 64 * NW, kBlock> ks, vs;
+  TileStage<T, DP, 64 * NW, kBlock> ks, other;
+  auto& vs = LEAN ? ks : other;
   float ps[3] = {};
+  auto fetch_v = [&](int k0) {
+    const int n = it.k_end - k0;
+    const KeyRows<T> vr((const T*)a.v, a.v_node, a.v_head, hk, k0, n);
+    vs.load(vr.base, a.dim, [&](int i) { return vr.offset(i); });
+  };
   auto fetch = [&](int k0) {
     const int n = it.k_end - k0;
-    const KeyRows<T> kr((const T*)a.k, a.k_node, a.k_head, hk, k0, n), vr((const T*)a.v, a.v_node, a.v_head, hk, k0, n);
-    ks.load(a.fast, kr.base, a.dim, [&](int i) { return kr.offset(i); }, [&](int i) { return kr.pointer(i); });
-    vs.load(a.fast, vr.base, a.dim, [&](int i) { return vr.offset(i); }, [&](int i) { return vr.pointer(i); });
+    const KeyRows<T> kr((const T*)a.k, a.k_node, a.k_head, hk, k0, n);
+    ks.load(kr.base, a.dim, [&](int i) { return kr.offset(i); });
+    if (!LEAN) fetch_v(k0);
     if (BIASED && tid < kBlock)
 #pragma unroll
       for (int d = 0; d < 3; ++d) ps[d] = tid < n ? a.pos_k[(int64_t)(k0 + tid) * 3 + d] : 0.f;
@@ -230,15 +242,16 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
   for (int k0 = first; k0 < it.k_end; k0 += KS * kBlock, buf ^= 1) {
     const int n = it.k_end - k0;
     char* const k_tile = tiles + (kBuf == 2 ? buf : 0) * 2 * kTile;
-    char* const v_tile = k_tile + kTile;
+    char* const v_tile = LEAN ? k_tile : k_tile + kTile;
     if (kBuf == 1) tile_sync<KS>();
     ks.store(k_tile);
-    vs.store(v_tile);
+    if (!LEAN) vs.store(v_tile);
     if (BIASED && tid < kBlock)
 #pragma unroll
       for (int d = 0; d < 3; ++d) pos[buf][d][tid] = ps[d];
     tile_sync<KS>();
-    if (k0 + KS * kBlock < it.k_end) fetch(k0 + KS * kBlock);
+    if (LEAN) fetch_v(k0);
+    else if (k0 + KS * kBlock < it.k_end) fetch(k0 + KS * kBlock);
     f32x16_t t[kBlock / 32];
     float most = top;
 #pragma unroll
@@ -258,6 +271,7 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
             const float dx = x - px[e], dy = y - py[e], dz = z - pz[e];
             t[b][4 * g + e] = sc.less(t[b][4 * g + e], slope, __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz));
           }
+          if (LEAN) __builtin_amdgcn_sched_barrier(0);
         }
       }
       if (n < 32 * b + 32)
@@ -285,6 +299,12 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
       for (int e = 0; e < 16; ++e) {
         t[b][e] = exp2_fast(fmaf(t[b][e], sc.unit, base));
         sum += t[b][e];
+      }
+      if (LEAN) {
+        tile_sync<KS>();
+        vs.store(v_tile);
+        tile_sync<KS>();
+        if (k0 + KS * kBlock < it.k_end) fetch(k0 + KS * kBlock);
       }
       cols_times<T, DP>(acc, v_tile, 32 * b, t[b]);
     }
@@ -422,11 +442,12 @@ struct QSums {
 
 // ---- gradient with the rows fixed ---------------------------------------------------------------------------------
 template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
-__global__ void __launch_bounds__(64 * NW * KS, (sizeof(T) == 2 && DP <= 64) || DP <= 32 ? 2 : 1)
+__global__ void __launch_bounds__(64 * NW * KS, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
 attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
   using S = AttnShape<T, DP>;
-  constexpr int kBlock = kBlockOf<NW>, kTile = kBlock * S::kRow, kBuf = KS > 1 ? 1 : kBuffers<2 * kTile>;
-  __shared__ alignas(16) char lds[attn_lds<T, DP, NW, KS>(9)];
+  constexpr int kBlock = kBlockOf<T, DP, NW>, kTile = kBlock * S::kRow, kBuf = KS > 1 || kLean<T, DP, NW> ? 1 : kBuffers<2 * kTile>;
+  constexpr bool LEAN = kLean<T, DP, NW>;
+  __shared__ alignas(16) char lds[attn_lds<T, DP, NW, KS>(2, 9)];
   __shared__ alignas(16) float all_pos[KS][2][3][kBlock];
   const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
   const cgtp_attn_item it = a.q_items[blockIdx.x / a.h_kv];
@@ -439,11 +460,11 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
   const Score<T, BIASED, CAPPED> sc(a);
   RowFrag<T, DP> q, g;
   q.load(row.ok ? (const T*)a.q + row.query * a.q_node + row.head * a.q_head : nullptr, a.dim);
-  g.load(row.ok ? (const T*)a.grad_out + at * a.dim : nullptr, a.dim);
+  g.load(row.ok ? (const T*)a.grad_out + row.query * a.g_node + row.head * a.g_head : nullptr, a.dim);
   float delta = 0.f;
   {
     RowFrag<T, DP> o;
-    o.load(row.ok ? (const T*)a.out + at * a.dim : nullptr, a.dim);
+    o.template load<false>(row.ok ? (const T*)a.out + at * a.dim : nullptr, a.dim);
 #pragma unroll
     for (int s = 0; s < S::kSteps; ++s) {
       typedef T vec __attribute__((ext_vector_type(S::kChunk)));
@@ -472,13 +493,19 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
   // exact one is delta + sum ds, and with it the gradients of positions and slopes, which are fp32, err as in fp32.
   constexpr bool kFix = sizeof(T) == 2;
   QSums m = {};
-  TileStage<T, DP, 64 * NW, kBlock> ks, vs;
+  TileStage<T, DP, 64 * NW, kBlock> ks, other;
+  auto& vs = LEAN ? ks : other;
   float ps[3] = {};
+  auto fetch_v = [&](int k0) {
+    const int n = it.k_end - k0;
+    const KeyRows<T> vr((const T*)a.v, a.v_node, a.v_head, hk, k0, n);
+    vs.load(vr.base, a.dim, [&](int i) { return vr.offset(i); });
+  };
   auto fetch = [&](int k0) {
     const int n = it.k_end - k0;
-    const KeyRows<T> kr((const T*)a.k, a.k_node, a.k_head, hk, k0, n), vr((const T*)a.v, a.v_node, a.v_head, hk, k0, n);
-    ks.load(a.fast, kr.base, a.dim, [&](int i) { return kr.offset(i); }, [&](int i) { return kr.pointer(i); });
-    vs.load(a.fast, vr.base, a.dim, [&](int i) { return vr.offset(i); }, [&](int i) { return vr.pointer(i); });
+    const KeyRows<T> kr((const T*)a.k, a.k_node, a.k_head, hk, k0, n);
+    ks.load(kr.base, a.dim, [&](int i) { return kr.offset(i); });
+    if (!LEAN) fetch_v(k0);
     if (BIASED && tid < kBlock)
 #pragma unroll
       for (int d = 0; d < 3; ++d) ps[d] = tid < n ? a.pos_k[(int64_t)(k0 + tid) * 3 + d] : 0.f;
@@ -492,17 +519,23 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
     char* const v_tile = k_tile + kTile;
     if (kBuf == 1) tile_sync<KS>();
     ks.store(k_tile);
-    vs.store(v_tile);
+    if (!LEAN) vs.store(v_tile);
     if (BIASED && tid < kBlock)
 #pragma unroll
       for (int d = 0; d < 3; ++d) pos[buf][d][tid] = ps[d];
     tile_sync<KS>();
-    if (k0 + KS * kBlock < it.k_end) fetch(k0 + KS * kBlock);
+    if (LEAN) fetch_v(k0);
+    else if (k0 + KS * kBlock < it.k_end) fetch(k0 + KS * kBlock);
 #pragma unroll 1
     for (int b = 0; b < kBlock / 32; ++b) {
       if (b * 32 >= n) continue;
       f32x16_t t = rows_times<T, DP>(k_tile, 32 * b, q);
       sc.of(t);
+      if (LEAN) {
+        vs.store(v_tile);
+        tile_sync<KS>();
+        if (k0 + KS * kBlock < it.k_end) fetch(k0 + KS * kBlock);
+      }
       f32x16_t ds = rows_times<T, DP>(v_tile, 32 * b, g);
       auto turn = [&](bool cut) {
 #pragma unroll
@@ -625,10 +658,11 @@ __global__ void __launch_bounds__(256) attn_bwd_q_join_kernel(AttnLaunch a, Attn
 
 // ---- gradient with the keys fixed ---------------------------------------------------------------------------------
 template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
-__global__ void __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || DP <= 32 ? 2 : 1)
+__global__ void __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1)
 attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
   using S = AttnShape<T, DP>;
-  constexpr int kBlock = kBlockOf<NW>, kTile = kBlock * S::kRow, kBuf = kBuffers<2 * kTile>;
+  constexpr int kBlock = kBlockOf<T, DP, NW>, kTile = kBlock * S::kRow, kBuf = kLean<T, DP, NW> ? 1 : kBuffers<2 * kTile>;
+  constexpr bool LEAN = kLean<T, DP, NW>;
   __shared__ alignas(16) char tiles[kBuf][2][kTile];
   __shared__ alignas(16) float stat[2][6][kBlock];       // lse, delta, slope, position
   const int hk = blockIdx.x % a.h_kv, group = a.h_q / a.h_kv;
@@ -652,14 +686,17 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) gk[o][e] = gv[o][e] = 0.f;
   float gx = 0.f, gy = 0.f, gz = 0.f;
-  TileStage<T, DP, 64 * NW, kBlock> qs, gs;
+  TileStage<T, DP, 64 * NW, kBlock> qs, other;
+  auto& gs = LEAN ? qs : other;
   float st[6] = {};
+  auto fetch_g = [&](int r0) {
+    const QueryRows<T> gr((const T*)a.grad_out, a.g_node, a.g_head, it.node, hk, group, r0, it.row_end - r0);
+    gs.load(gr.base, a.dim, [&](int i) { return gr.offset(i); });
+  };
   auto fetch = [&](int r0) {
-    const int n = it.row_end - r0;
-    const QueryRows<T> qr((const T*)a.q, a.q_node, a.q_head, it.node, hk, group, r0, n),
-        gr((const T*)a.grad_out, (int64_t)a.h_q * a.dim, a.dim, it.node, hk, group, r0, n);
-    qs.load(a.fast, qr.base, a.dim, [&](int i) { return qr.offset(i); }, [&](int i) { return qr.pointer(i); });
-    gs.load(a.fast, gr.base, a.dim, [&](int i) { return gr.offset(i); }, [&](int i) { return gr.pointer(i); });
+    const QueryRows<T> qr((const T*)a.q, a.q_node, a.q_head, it.node, hk, group, r0, it.row_end - r0);
+    qs.load(qr.base, a.dim, [&](int i) { return qr.offset(i); });
+    if (!LEAN) fetch_g(r0);
     if (threadIdx.x < kBlock) {
       const Row o = row_of(it, r0 + threadIdx.x, hk, group);
       const int64_t at = (int64_t)o.query * a.h_q + o.head;
@@ -680,17 +717,23 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
     char* const g_tile = tiles[kBuf == 2 ? buf : 0][1];
     if (kBuf == 1) __syncthreads();
     qs.store(q_tile);
-    gs.store(g_tile);
+    if (!LEAN) gs.store(g_tile);
     if (threadIdx.x < kBlock)
 #pragma unroll
       for (int d = 0; d < 6; ++d) stat[buf][d][threadIdx.x] = st[d];
     __syncthreads();
-    if (r0 + kBlock < it.row_end) fetch(r0 + kBlock);
+    if (LEAN) fetch_g(r0);
+    else if (r0 + kBlock < it.row_end) fetch(r0 + kBlock);
 #pragma unroll 1
     for (int b = 0; b < kBlock / 32; ++b) {
       if (b * 32 >= n) continue;
       f32x16_t t = rows_times<T, DP>(q_tile, 32 * b, k);
       sc.of(t);
+      if (LEAN) {
+        gs.store(g_tile);
+        __syncthreads();
+        if (r0 + kBlock < it.row_end) fetch(r0 + kBlock);
+      }
       f32x16_t ds = rows_times<T, DP>(g_tile, 32 * b, v);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {

@@ -55,6 +55,7 @@ template <typename T, int DP> using AttnAcc = f32x16_t[AttnShape<T, DP>::kOut];
 template <typename T, int DP>
 struct RowFrag {
   u32x4_t f[AttnShape<T, DP>::kSteps];
+  template <bool WHOLE = true>      // 16 bytes at a time, aligned
   __device__ __forceinline__ void load(const T* p, int dim) {
     using S = AttnShape<T, DP>;
     const int half = (threadIdx.x & 63) >> 5;
@@ -62,40 +63,28 @@ struct RowFrag {
     for (int s = 0; s < S::kSteps; ++s) {
       const int d = (2 * s + half) * S::kChunk;
       f[s] = u32x4_t{0, 0, 0, 0};
-      if (p && d < dim) f[s] = load_part<u32x4_t, T>(p + d, dim - d);
+      if (p && d < dim) f[s] = WHOLE ? *reinterpret_cast<const u32x4_t*>(p + d) : load_part<u32x4_t, T>(p + d, dim - d);
     }
   }
 };
 
-// A tile between memory and LDS, moved by THREADS neighbouring threads.  Offset(i): bytes from `base` of row i, kNoRow for none;
-// Pointer(i): the row, null for none.
+// A tile between memory and LDS, moved by THREADS neighbouring threads.  Offset(i): bytes from `base` of row i, kNoRow for none.
 template <typename T, int DP, int THREADS, int BLOCK>
 struct TileStage {
   using S = AttnShape<T, DP>;
   static constexpr int kAll = BLOCK * S::kChunks, kEach = (kAll + THREADS - 1) / THREADS;
   u32x4_t reg[kEach];
 
-  template <typename Offset, typename Pointer>
-  __device__ __forceinline__ void load(bool fast, const T* base, int dim, Offset&& offset, Pointer&& pointer) {
-    if (fast) {
-      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kNoRow, 0x00027000);
+  template <typename Offset>
+  __device__ __forceinline__ void load(const T* base, int dim, Offset&& offset) {
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kNoRow, 0x00027000);
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int id = i * THREADS + (int)threadIdx.x % THREADS, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
-        if (kAll % THREADS != 0 && id >= kAll) break;
-        const unsigned o = offset(r);
-        reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-            rsrc, o == kNoRow || c * S::kChunk >= dim ? kNoRow : o + c * 16, 0, 0));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int id = i * THREADS + (int)threadIdx.x % THREADS, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
-        if (kAll % THREADS != 0 && id >= kAll) break;
-        const T* p = pointer(r);
-        reg[i] = u32x4_t{0, 0, 0, 0};
-        if (p && c * S::kChunk < dim) reg[i] = load_part<u32x4_t, T>(p + c * S::kChunk, dim - c * S::kChunk);
-      }
+    for (int i = 0; i < kEach; ++i) {
+      const int id = i * THREADS + (int)threadIdx.x % THREADS, r = id / S::kChunks, c = S::mixed(r, id % S::kChunks);
+      if (kAll % THREADS != 0 && id >= kAll) break;
+      const unsigned o = offset(r);
+      reg[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+          rsrc, o == kNoRow || c * S::kChunk >= dim ? kNoRow : o + c * 16, 0, 0));
     }
   }
   __device__ __forceinline__ void store(char* lds) const {
@@ -117,8 +106,10 @@ __device__ __forceinline__ f32x16_t rows_times(const char* lds, int first, const
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = 0.f;
 #pragma unroll
-  for (int s = 0; s < S::kSteps; ++s)
+  for (int s = 0; s < S::kSteps; ++s) {
     acc = mma_pair<T>(*reinterpret_cast<const u32x4_t*>(lds + S::slot(r, 2 * s + half)), b.f[s], acc);
+    if (sizeof(T) == 4 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // not all of a row's reads at once in registers
+  }
   return acc;
 }
 
@@ -161,6 +152,7 @@ __device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* lds,
         const float v = *reinterpret_cast<const float*>(lds + S::slot(r, d >> 2) + ((d & 3) << 2));
         acc[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[e], acc[o], 0, 0, 0);
       }
+      if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
 }

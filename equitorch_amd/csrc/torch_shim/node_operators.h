@@ -245,8 +245,8 @@ at::Tensor attn_forward(const AttnOperands& o, const AttnHandle& h, double scale
   a.out = out.data_ptr();
   a.lse = lse ? lse->data_ptr() : nullptr;
   at::Tensor ws;
-  if (a.n_q_slots) {
-    ws = bytes_on(o.q, cgtp_attn_workspace_bytes(&a, 0));
+  if (const int64_t n = cgtp_attn_workspace_bytes(&a, 0)) {
+    ws = bytes_on(o.q, n);
     a.workspace = ws.data_ptr();
   }
   check_status(cgtp_attn_forward(&a, current_stream(o.q)), "cgtp_attn_forward");

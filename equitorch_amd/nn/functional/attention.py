@@ -253,10 +253,9 @@ def _forward(q, k, v, pos_q, pos_k, slope, plan, scale, cap, keep):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if keep else None
     a.out, a.lse = out.data_ptr(), _lib.ptr(lse)
-    ws = None
-    if a.n_q_slots:
-        ws = torch.empty(_lib.lib.cgtp_attn_workspace_bytes(C.byref(a), 0), dtype=torch.uint8, device=q.device)
-        a.workspace = ws.data_ptr()
+    nbytes = _lib.lib.cgtp_attn_workspace_bytes(C.byref(a), 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    a.workspace = _lib.ptr(ws)
     _lib.check(_lib.lib.cgtp_attn_forward(C.byref(a), _lib.stream_ptr(q.device)), "cgtp_attn_forward")
     return out, lse
 

@@ -800,7 +800,7 @@ int cgtp_gff_backward(const cgtp_gff_args* args, void* stream);
 /* ---- attention among the nodes of a structure ---------------------------------------------------------------------
  * Nodes of many structures lie one after the other; every query of a structure sees all keys of the same structure:
  *   s_ij = cap tanh(scale q_i.k_j / cap) - slope_h |r_i - r_j|     (cap <= 0: scale q_i.k_j;  slope NULL: no distance)
- *   out_i = sum_j softmax_j(s_ij) v_j,  lse_i = log2 of the sum of 2^(s log2 e), less cap log2 e where there is a cap;  no key, or every score -inf: out_i = 0 and
+ *   out_i = sum_j softmax_j(s_ij) v_j,  lse_i = log2 sum_j 2^(s_ij log2 e);  no key, or every score -inf: out_i = 0 and
  *   lse_i = +inf.
  * q: (n_q, h_q, dim), k and v: (n_k, h_kv, dim), h_q a multiple of h_kv (query head h reads head h / (h_q / h_kv)), with
  * element strides *_node and *_head and contiguous along dim; out, grad_out and the gradients contiguous; lse (n_q, h_q)
@@ -814,7 +814,8 @@ int cgtp_gff_backward(const cgtp_gff_args* args, void* stream);
  * slot of its own, where it leaves partial results, and first = its place among the pieces of its tile; one entry of q_joins /
  * k_joins adds the slots first .. first + count - 1 of a tile, in that order.  A structure without keys has items with an
  * empty range.  Every query and every key belongs to exactly one tile.
- * workspace: cgtp_attn_workspace_bytes(args, backward), 16-byte aligned (0: may be NULL).
+ * workspace: cgtp_attn_workspace_bytes(args, backward), aligned to 16 bytes, else CGTP_ERR_ALIGN (0: may be NULL); it holds the
+ * pieces' results and a copy of those operands whose rows are not whole aligned 16 bytes.
  * cgtp_attn_backward writes grad_q, grad_k, grad_v and, with slope, grad_slope (h_q) and grad_pos_q (n_q, 3) where they are
  * not NULL; same_pos != 0: the queries' and the keys' positions are one tensor, and grad_pos_q is the whole gradient, else
  * grad_pos_k (n_k, 3) is that of pos_k.  All sums have an order that the arguments alone determine.

@@ -109,6 +109,24 @@ def test_attention_codes_of_one_direction():
     assert lib.cgtp_attn_backward(C.byref(_attn(workspace=None)), None) == WORKSPACE
     assert lib.cgtp_attn_backward(C.byref(_attn(lse=None)), None) == NULL
     assert lib.cgtp_attn_backward(C.byref(_attn(k_items=None)), None) == NULL
+    assert lib.cgtp_attn_forward(C.byref(_attn(workspace=4100)), None) == ALIGN
+    assert lib.cgtp_attn_backward(C.byref(_attn(workspace=4100)), None) == ALIGN
+
+
+def test_attention_copies_rows_that_are_not_whole():
+    strides = dict(q_node=32, q_head=16, k_node=16, k_head=16, v_node=16, v_head=16)
+
+    def need(backward=0, **changed):
+        return _lib.lib.cgtp_attn_workspace_bytes(C.byref(_attn(**{**strides, "dtype": 2, **changed})), backward)
+    kept = need(backward=1)
+    assert need() == 0
+    assert need(q=4098) == 256                               # 4 x 2 rows of 32 bytes
+    assert need(k=4098) == need(v_node=17) == 256            # 4 rows
+    assert need(q_node=-32) == need(q_node=1 << 30) == 256
+    assert need(dim=15) == 3 * 256 and need(backward=1, dim=15) == kept + 4 * 256
+    assert need(backward=1, grad_out=4098) == kept + 256
+    for backward, launch in ((0, _lib.lib.cgtp_attn_forward), (1, _lib.lib.cgtp_attn_backward)):
+        assert launch(C.byref(_attn(**{**strides, "dtype": 2, "q": 4098, "workspace": None})), None) == WORKSPACE
 
 
 @pytest.mark.parametrize("len_q,len_k,group,heads", [
