@@ -1,11 +1,13 @@
 // Matrix products of the gated feed-forward block on the matrix cores: tiles of 128 x 128, four wavefronts of 64 x 64 each, or
-// of 64 x 64 where there would be too few of the others (TILE), operands brought through registers into one LDS buffer, the next tile loaded while one is worked on.
+// of 64 x 64 where there would be too few of the others (TILE), operands brought through registers into one LDS buffer, the
+// next tile loaded while one is worked on.
 //
 // An operand is a matrix whose k or whose rows are contiguous.  In LDS a tile is 8 TILE chunks of 16 bytes either way:
-//   k contiguous    TILE rows of eight chunks along k, chunk c of row r at place c ^ (r & 7);
+//   k contiguous    TILE rows of eight chunks along k, chunk c of row r at place c ^ (r / 2 & 7);
 //   rows contiguous two halves of TILE / 2 rows, in each the rows of one k after the other, chunks exchanged by
-//                   (k & 3) | (k >> 1 & 4) where there are eight of them, which the transposing loads of 16-bit types (four
-//                   k of 16 rows for each 16 lanes, k and k + 8 in one instruction) find in different groups of banks.
+//                   (k & 1) | (k << 1 & 4) | (k >> 2 & 2) where there are eight of them, which the transposing loads of
+//                   16-bit types (four k of 32 rows for 32 lanes, k + 8 for the others) find in different banks.
+// Neither has bank conflicts; with c ^ (r & 7) and (k & 3) | (k >> 1 & 4) they took 10 to 17 % of the cycles.
 // 16-bit types use 32 x 32 x 16 instructions, fp32 32 x 32 x 2 ones, four for a pair of chunks, whose k are taken in the order
 // that lets a lane read its four in one access.
 //
@@ -55,7 +57,7 @@ struct GemmStage {
   static constexpr int kHalf = TILE / 2, kRow = kHalf / CH;       // rows contiguous: rows of a half, chunks of one k in it
   u32x4_t reg[kEach];
 
-  __device__ static __forceinline__ int mix(int k) { return kRow >= 8 ? (k & 3) | ((k >> 1) & 4) : 0; }
+  __device__ static __forceinline__ int mix(int k) { return kRow >= 8 ? (k & 1) | ((k << 1) & 4) | ((k >> 2) & 2) : 0; }
 
   // k0: first k of the tile, depth: end of k.
   template <bool FAST>
@@ -66,7 +68,7 @@ struct GemmStage {
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kOutside, 0x00027000);
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        const int id = i * kGemmThreads + tid, r = id >> 3, c = (id & 7) ^ (r & 7);
+        const int id = i * kGemmThreads + tid, r = id >> 3, c = (id & 7) ^ ((r >> 1) & 7);
         const bool in = r < p.rows[0] && c * CH < left;
         if constexpr (FAST) {
           const unsigned at = (unsigned)r * (unsigned)(p.ld * sizeof(T)) + c * 16;
@@ -102,7 +104,7 @@ struct GemmStage {
     const int lane = threadIdx.x & 63, half = lane >> 5;
     if constexpr (K_CONTIGUOUS) {
       const int r = block * 32 + (lane & 31);
-      return *reinterpret_cast<const u32x4_t*>(lds + r * 128 + (((2 * s + half) ^ (r & 7)) << 4));
+      return *reinterpret_cast<const u32x4_t*>(lds + r * 128 + (((2 * s + half) ^ ((r >> 1) & 7)) << 4));
     } else if constexpr (sizeof(T) == 2) {
       const char* h = lds + block * 32 / kHalf * (TILE * 64);
       const int k = 16 * s + 8 * half + ((lane & 15) >> 2), m = block * 32 % kHalf + (lane & 16) + 4 * (lane & 3);
