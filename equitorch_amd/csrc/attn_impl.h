@@ -189,9 +189,9 @@ __device__ __forceinline__ void join_waves(float* lds, int n, Give&& give, Take&
 
 // ---- forward ----------------------------------------------------------------------------------------------------
 // Vector instructions bound it with distances: some 25 issue slots for a score (a root and an exponential take four each), 79 %
-// of all slots used, the matrix cores 14 %.  300 structures of 40 to 250 nodes, 8 heads of 32, bf16, cap: 64 us; three of
-// 2000 to 5000, 8 query heads on 4 of 64: 324 us.  Without distances and cap the matrix cores and LDS do: one of 12007, 16 query
-// heads on 4 of 128, fp16: 1.46 ms, 810 TFLOP/s, 0.72 of what a large library product reaches.
+// of all slots used, the matrix cores 14 %.  300 structures of 40 to 250 nodes, 8 heads of 32, bf16, cap: 62 us; three of
+// 2000 to 5000, 8 query heads on 4 of 64: 321 us.  Without distances and cap the matrix cores and LDS do: one of 12007, 16 query
+// heads on 4 of 128, fp16: 1.35 ms, 877 TFLOP/s, 0.78 of what a large library product reaches.
 //
 // NW wavefronts of 32 rows share the tiles of keys (wide_q 1), or KS share out the keys of one tile of rows and join their
 // results in LDS (wide_q 2: 64 readouts of one query over up to 400 keys, fp32, 30 us with one wavefront each, 15 so; one query
@@ -452,7 +452,7 @@ struct QSums {
 
 // ---- gradient with the rows fixed ---------------------------------------------------------------------------------
 // Bound by vector instructions as the forward is (84 % of the slots): the score again, and the sums for positions and slopes.
-// The two workloads above: 111 and 528 us.
+// The two workloads above: 108 and 527 us.
 template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
 __global__ void __launch_bounds__(64 * NW * KS, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
 attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
@@ -670,7 +670,7 @@ __global__ void __launch_bounds__(256) attn_bwd_q_join_kernel(AttnLaunch a, Attn
 
 // ---- gradient with the keys fixed ---------------------------------------------------------------------------------
 // Bound by vector instructions; four sums of 32 x dim for a wavefront leave room for two of them on a SIMD up to dim 64.  The
-// two workloads above: 100 and 570 us.  Taking two heads at a time, whose distances are the same, was within 5 % of
+// two workloads above: 98 and 567 us.  Taking two heads at a time, whose distances are the same, was within 5 % of
 // this for short rows and slower for others (their sums spilled).
 template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
 __global__ void __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1)
