@@ -74,21 +74,28 @@ struct SortInput {
   }
 };
 
-// Digits of every block's part; the first pass also clears the gradient (kinds without a row keep the zeros).
+// Zeros, by threads `at` of `stride`.
+__device__ __forceinline__ void clear_by(char* p, int64_t bytes, int64_t at, int64_t stride) {
+  const int64_t words = (reinterpret_cast<uintptr_t>(p) & 15u) ? 0 : bytes / 16;
+  for (int64_t i = at; i < words; i += stride) reinterpret_cast<uint4*>(p)[i] = uint4{0, 0, 0, 0};
+  for (int64_t i = words * 16 + at; i < bytes; i += stride) p[i] = 0;
+}
+
+// Digits of every block's part; the first pass also clears the gradient (kinds without a row keep the zeros), with blocks that do
+// nothing else where the table is large for the rows (300 rows of 30000 kinds, 256 channels fp32: 227 us without them).
 __global__ void __launch_bounds__(kSortThreads) embed_digits_kernel(SortInput in, int32_t* __restrict__ digits,
                                                                     int64_t n_rows, int64_t per_block, int shift,
                                                                     char* __restrict__ clear, int64_t clear_bytes) {
+  if (clear_bytes) clear_by(clear, clear_bytes, (int64_t)blockIdx.x * kSortThreads + threadIdx.x, (int64_t)gridDim.x * kSortThreads);
+  const int64_t i0 = blockIdx.x * per_block;
+  if (i0 >= n_rows) return;
   __shared__ int count[kDigits];
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) count[d] = 0;
   __syncthreads();
-  const int64_t i0 = blockIdx.x * per_block, i1 = i0 + per_block < n_rows ? i0 + per_block : n_rows;
+  const int64_t i1 = i0 + per_block < n_rows ? i0 + per_block : n_rows;
   for (int64_t i = i0 + threadIdx.x; i < i1; i += kSortThreads) atomicAdd(&count[(in.key(i) >> shift) & 255], 1);
   __syncthreads();
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) digits[(int64_t)blockIdx.x * kDigits + d] = count[d];
-  const int64_t words = (reinterpret_cast<uintptr_t>(clear) & 15u) ? 0 : clear_bytes / 16, stride = (int64_t)gridDim.x * kSortThreads;
-  const int64_t at = (int64_t)blockIdx.x * kSortThreads + threadIdx.x;
-  for (int64_t i = at; i < words; i += stride) reinterpret_cast<uint4*>(clear)[i] = uint4{0, 0, 0, 0};
-  for (int64_t i = words * 16 + at; i < clear_bytes; i += stride) clear[i] = 0;
 }
 
 // Each block works out where its part's digits begin from the counts of all blocks, then moves its part in order: the rank of
@@ -326,9 +333,61 @@ __global__ void __launch_bounds__(THREADS) embed_join_kernel(const typename AccO
   grad_table[(int64_t)me.last * C + c] = (T)(s * scale);
 }
 
+// Few rows: one launch in place of the sort, the sums and the join.  Every wavefront holds all the kinds, takes a row of the table
+// at a time, finds who has its kind and sums them in ascending order, eight on their way.  256 rows of 100 kinds, 64 channels
+// fp32, 5 us against 16 in four launches, all of one kind 17 against 13; of 30000 kinds, 256 channels, 8.5.
+constexpr int kFewRows = 256;
+template <typename T, int V>
+__global__ void __launch_bounds__(256) embed_few_kernel(const int64_t* __restrict__ kind, const T* __restrict__ grad_out,
+                                                        T* __restrict__ grad_table, int n_rows, int n_kinds, int C,
+                                                        typename AccOf<T>::type scale) {
+  using A = typename AccOf<T>::type;
+  constexpr int kGroups = kFewRows / kWave, kAhead = 8;
+  const int lane = threadIdx.x & (kWave - 1), waves = gridDim.x * (256 / kWave);
+  int mine[kGroups];
+#pragma unroll
+  for (int q = 0; q < kGroups; ++q) {
+    const int i = q * kWave + lane;
+    const int64_t k = i < n_rows ? kind[i] : -1;
+    mine[q] = (uint64_t)k < (uint64_t)n_kinds ? (int)k : -1;
+  }
+  for (int64_t t = (blockIdx.x * 256 + (int)threadIdx.x) / kWave; t < n_kinds; t += waves) {
+    uint64_t who[kGroups];
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) who[q] = __ballot(mine[q] == (int)t);
+    for (int at = lane * V; at < C; at += kWave * V) {
+      const int c = min(at, C - V);
+      A acc[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = A(0);
+#pragma unroll
+      for (int q = 0; q < kGroups; ++q) {
+        for (uint64_t m = who[q]; m;) {
+          A v[kAhead][V];
+          const int n = min(kAhead, __popcll(m));
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) {
+            if (j >= n) continue;
+            load_elems<T, V>(v[j], grad_out + (int64_t)(q * kWave + __ffsll((unsigned long long)m) - 1) * C + c);
+            m &= m - 1;
+          }
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) {
+            if (j >= n) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += v[j][e];
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] *= scale;
+      store_elems<T, V>(grad_table + t * C + c, acc);
+    }
+  }
+}
+
 __global__ void __launch_bounds__(256) embed_clear_kernel(char* __restrict__ p, int64_t bytes) {
-  const int64_t stride = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < bytes; i += stride) p[i] = 0;
+  clear_by(p, bytes, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
@@ -407,6 +466,13 @@ template <typename T>
 int embed_backward(const int64_t* kind, const void* grad_out, void* grad_table, void* workspace, int64_t n_rows,
                    int64_t n_kinds, int C, double scale, hipStream_t stream) {
   using A = typename AccOf<T>::type;
+  if (n_rows <= kFewRows) {
+    constexpr int VW = 16 / sizeof(T);
+    auto few = C >= VW ? embed_few_kernel<T, VW> : embed_few_kernel<T, 1>;
+    hipLaunchKernelGGL(few, dim3((unsigned)std::min<int64_t>((n_kinds + 3) / 4, 2048)), dim3(256), 0, stream, kind, (const T*)grad_out,
+                       (T*)grad_table, (int)n_rows, (int)n_kinds, C, (A)scale);
+    return launch_status();
+  }
   const EmbedPlan p = embed_plan<T>(n_rows, n_kinds, C);
   char* ws = (char*)workspace;
   int32_t* digits = (int32_t*)(ws + p.digits);
@@ -414,8 +480,10 @@ int embed_backward(const int64_t* kind, const void* grad_out, void* grad_table, 
     const int from = (pass + 1) & 1, to = pass & 1;
     const SortInput in = {kind, pass ? (const int32_t*)(ws + p.keys[from]) : nullptr,
                           pass ? (const int32_t*)(ws + p.rows[from]) : nullptr, n_kinds};
-    hipLaunchKernelGGL(embed_digits_kernel, dim3((unsigned)p.blocks), dim3(kSortThreads), 0, stream, in, digits, n_rows,
-                       p.per_block, 8 * pass, (char*)grad_table, pass ? (int64_t)0 : n_kinds * C * (int64_t)sizeof(T));
+    const int64_t clear = pass ? 0 : n_kinds * C * (int64_t)sizeof(T);
+    const int64_t grid = std::max(p.blocks, std::min<int64_t>(512, clear >> 16));
+    hipLaunchKernelGGL(embed_digits_kernel, dim3((unsigned)grid), dim3(kSortThreads), 0, stream, in, digits, n_rows, p.per_block,
+                       8 * pass, (char*)grad_table, clear);
     hipLaunchKernelGGL(embed_scatter_kernel, dim3((unsigned)p.blocks), dim3(kSortThreads), 0, stream, in, digits,
                        (int32_t*)(ws + p.keys[to]), (int32_t*)(ws + p.rows[to]), n_rows, p.per_block, 8 * pass);
   }
@@ -474,7 +542,7 @@ int cgtp_embed_backward(const int64_t* kind, const void* grad_out, void* grad_ta
   hipStream_t s = (hipStream_t)stream;
   if (n_rows == 0) {
     const int64_t bytes = n_kinds * C * elem_size(dtype);
-    hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)std::min<int64_t>((bytes + 255) / 256, kMaxBlocks)), dim3(256), 0, s, (char*)grad_table, bytes);
+    hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)std::min<int64_t>((bytes + 4095) / 4096, kMaxBlocks)), dim3(256), 0, s, (char*)grad_table, bytes);
     return launch_status();
   }
   if (!kind || !grad_out) return CGTP_ERR_NULL;

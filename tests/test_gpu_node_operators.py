@@ -512,3 +512,10 @@ def test_gated_feed_forward_at_unaligned_addresses(device):
         results.append((out, *torch.autograd.grad(out.float().sum(), leaves)))
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, F64, BF16])
+@pytest.mark.parametrize("rows,kinds,channels", [(1, 9000, 5), (64, 1, 70), (200, 40, 513), (255, 7, 33), (256, 300, 8), (257, 5000, 200)])
+def test_embedding_of_few_rows(device, dtype, rows, kinds, channels):
+    """Where the gradient takes one launch, and just beyond: many rows of one kind, and a table much larger than the rows."""
+    test_embedding(device, dtype, rows, kinds, channels)
