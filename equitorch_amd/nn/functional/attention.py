@@ -20,6 +20,7 @@ from .edge import _higher_order
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _BLOCK = 64                     # keys (rows) of a tile: pieces of a structure begin at multiples of it
 _PIECE = 256                    # keys (rows) of a piece at least
+_SMALL = 256                    # tiles of 32 rows that leave wavefronts idle: four for each make one for each SIMD
 _WAVES = 4096                   # wavefronts wanted where structures can be cut into pieces: four for each SIMD
 
 
@@ -78,9 +79,12 @@ class _Tables:
             raise CgtpError("queries times query heads of a head of keys must stay below 2^31")
         start_q, start_k = np.cumsum(plan.len_q) - plan.len_q, np.cumsum(cols) - cols
         # Tiles of 128 rows share a tile of keys among four wavefronts; tiles of 32 rows waste less of a short structure.  Few
-        # rows against many keys (a readout): four wavefronts share out the keys of a tile of 32 rows.
+        # rows against many keys (a readout), or so few tiles that the GPU is idle otherwise: four wavefronts share out the
+        # keys of a tile of 32 rows (8 structures of 510 nodes, a head of 48, fp32: forward 48 -> 22 us; but 376 tiles of 2
+        # structures of 3000 nodes 144 so, 127 by 128).
         self.wide_q, self.wide_k = int(_wide(rows)), int(_wide(cols))
-        if not self.wide_q and int(cols.sum()) >= 96 * int((-(-rows // 32)).sum()):
+        tiles = int((-(-rows // 32)).sum())
+        if not self.wide_q and int(cols.sum()) >= 96 * tiles or 0 < tiles * heads <= _SMALL and int(cols.max()) > 32:
             self.wide_q = 2
         q = _Items(rows, cols, 128 if self.wide_q == 1 else 32, heads, 4 if self.wide_q else 1)
         k = _Items(cols, rows, 128 if self.wide_k else 32, heads, 4 if self.wide_k else 1)
