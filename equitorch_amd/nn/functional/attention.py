@@ -20,6 +20,7 @@ from .edge import _higher_order
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _BLOCK = 64                     # keys (rows) of a tile: pieces of a structure begin at multiples of it
 _PIECE = 256                    # keys (rows) of a piece at least
+_LEAST = 64                     # the same where tiles are few
 _SMALL = 256                    # tiles of 32 rows that leave wavefronts idle: four for each make one for each SIMD
 _WAVES = 4096                   # wavefronts wanted where structures can be cut into pieces: four for each SIMD
 
@@ -38,14 +39,14 @@ class _Items:
     """Tables of one pass for the kernels: tiles of ``tile`` rows of every structure, each against the columns of its
     structure, or against a piece of them where there are too few tiles to occupy the GPU."""
 
-    def __init__(self, rows: np.ndarray, cols: np.ndarray, tile: int, heads: int, waves: int):
+    def __init__(self, rows: np.ndarray, cols: np.ndarray, tile: int, heads: int, waves: int, least: int = _PIECE):
         tiles = -(-rows // tile)
         s = np.repeat(np.arange(len(rows)), tiles)                             # structure of every tile
         first_tile = np.cumsum(tiles) - tiles
         begin = (np.arange(len(s)) - first_tile[s]) * tile
         end = np.minimum(begin + tile, rows[s])
         want = -(-_WAVES // (waves * heads * max(1, len(s))))                  # pieces of a tile
-        pieces = np.clip(cols[s] // _PIECE, 1, max(1, want))
+        pieces = np.clip(cols[s] // least, 1, max(1, want))
         step = -(-(-(-cols[s] // pieces)) // _BLOCK) * _BLOCK                  # columns of a piece
         pieces = np.maximum(1, -(-cols[s] // np.maximum(step, 1)))
         t = np.repeat(np.arange(len(s)), pieces)                               # tile of every piece
@@ -87,7 +88,11 @@ class _Tables:
         if not self.wide_q and int(cols.sum()) >= 96 * tiles or 0 < tiles * heads <= _SMALL and int(cols.max()) > 32:
             self.wide_q = 2
         q = _Items(rows, cols, 128 if self.wide_q == 1 else 32, heads, 4 if self.wide_q else 1)
-        k = _Items(cols, rows, 128 if self.wide_k else 32, heads, 4 if self.wide_k else 1)
+        # The gradient of keys and values likewise, by short pieces of the rows (151 nodes, 4 query heads on one of 128, fp32: step
+        # 203 -> 116 us, 8 structures of 510 nodes, a head of 48, 211 -> 104).
+        few = int((-(-cols // 32)).sum()) * heads <= _SMALL
+        self.wide_k = int(self.wide_k and not few)
+        k = _Items(cols, rows, 128 if self.wide_k else 32, heads, 4 if self.wide_k else 1, _LEAST if few else _PIECE)
         zero = np.zeros_like(q.begin)
         at = start_k[q.structure]
         self.q_items = _table((start_q[q.structure], q.begin, q.end, at + q.col_begin, at + q.col_end, q.slot, q.place, zero),
