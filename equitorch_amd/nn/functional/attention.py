@@ -39,13 +39,13 @@ class _Items:
     """Tables of one pass for the kernels: tiles of ``tile`` rows of every structure, each against the columns of its
     structure, or against a piece of them where there are too few tiles to occupy the GPU."""
 
-    def __init__(self, rows: np.ndarray, cols: np.ndarray, tile: int, heads: int, waves: int, least: int = _PIECE):
+    def __init__(self, rows: np.ndarray, cols: np.ndarray, tile: int, heads: int, waves: int, least: int = _PIECE, wanted: int = _WAVES):
         tiles = -(-rows // tile)
         s = np.repeat(np.arange(len(rows)), tiles)                             # structure of every tile
         first_tile = np.cumsum(tiles) - tiles
         begin = (np.arange(len(s)) - first_tile[s]) * tile
         end = np.minimum(begin + tile, rows[s])
-        want = -(-_WAVES // (waves * heads * max(1, len(s))))                  # pieces of a tile
+        want = -(-wanted // (waves * heads * max(1, len(s))))                  # pieces of a tile
         pieces = np.clip(cols[s] // least, 1, max(1, want))
         step = -(-(-(-cols[s] // pieces)) // _BLOCK) * _BLOCK                  # columns of a piece
         pieces = np.maximum(1, -(-cols[s] // np.maximum(step, 1)))
@@ -87,7 +87,10 @@ class _Tables:
         tiles = int((-(-rows // 32)).sum())
         if not self.wide_q and int(cols.sum()) >= 96 * tiles or 0 < tiles * heads <= _SMALL and int(cols.max()) > 32:
             self.wide_q = 2
-        q = _Items(rows, cols, 128 if self.wide_q == 1 else 32, heads, 4 if self.wide_q else 1)
+        # Two for each SIMD, all at once, where there are few rows: more pieces take another turn and a longer join (one query of 8
+        # heads on 2 over 200003 keys, bf16: 38 us with four, 31 so).
+        q = _Items(rows, cols, 128 if self.wide_q == 1 else 32, heads, 4 if self.wide_q else 1,
+                   wanted=_WAVES // 2 if self.wide_q == 2 else _WAVES)
         # The gradient of keys and values likewise, by short pieces of the rows (151 nodes, 4 query heads on one of 128, fp32: step
         # 203 -> 116 us, 8 structures of 510 nodes, a head of 48, 211 -> 104).
         few = int((-(-cols // 32)).sum()) * heads <= _SMALL
