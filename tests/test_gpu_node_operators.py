@@ -519,3 +519,15 @@ def test_gated_feed_forward_at_unaligned_addresses(device):
 def test_embedding_of_few_rows(device, dtype, rows, kinds, channels):
     """Where the gradient takes one launch, and just beyond: many rows of one kind, and a table much larger than the rows."""
     test_embedding(device, dtype, rows, kinds, channels)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,biased,cap", [
+    ("short", 8, 8, 16, True, 0.0), ("short", 8, 4, 128, True, 0.0), ("short", 4, 4, 96, True, 5.0), ("short", 2, 2, 64, False, 0.0),
+    ("odd", 4, 4, 32, True, 4.0), ("odd", 4, 1, 64, False, 0.0), ("odd", 2, 2, 128, True, 0.0), ("long", 2, 1, 72, True, 3.0),
+    ("long", 2, 2, 128, False, 0.0), ("few_keys", 4, 2, 24, True, 0.0), ("mixed", 3, 3, 96, True, 6.0), ("mixed", 4, 4, 8, False, 0.0)])
+def test_attention_as_in_a_large_batch(device, monkeypatch, dtype, lengths, heads, kv_heads, dim, biased, cap):
+    """The tiles that a batch gets which fills the GPU: a wavefront for each, or four for 128 rows, and long pieces."""
+    from equitorch_amd.nn.functional import attention
+    monkeypatch.setattr(attention, "_SMALL", 0)
+    test_attention(device, dtype, lengths, heads, kv_heads, dim, biased, cap)
