@@ -48,7 +48,10 @@ __global__ void __launch_bounds__(1024) attn_pos_kernel(cgtp_attn_args a, AttnSc
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += sums[which * kPosNodes + i * 16 + l];
       s = group_sum(s, 16);
-      if (l == 0 && h0 + which < a.h_q) w.slope_part[(int64_t)(h0 + which) * gridDim.x + blockIdx.x] = s;
+      if (l == 0 && h0 + which < a.h_q) {
+        if (gridDim.x == 1) a.grad_slope[h0 + which] = s;          // nothing to add it to
+        else w.slope_part[(int64_t)(h0 + which) * gridDim.x + blockIdx.x] = s;
+      }
     }
   }
 }
@@ -227,7 +230,7 @@ int cgtp_attn_backward(const cgtp_attn_args* a, void* stream) {
     const unsigned blocks = (unsigned)blocks_of(a->n_q);
     if (blocks && (a->grad_pos_q || a->grad_slope))
       hipLaunchKernelGGL(attn_pos_kernel, dim3(blocks), dim3(1024), 0, s, *a, w);
-    if (a->grad_slope)
+    if (a->grad_slope && blocks != 1)
       hipLaunchKernelGGL(attn_slope_kernel, dim3((unsigned)a->h_q), dim3(256), 0, s, a->grad_slope, (const float*)w.slope_part, (int)blocks);
     if (!a->same_pos && a->grad_pos_k && a->n_k > 0)
       hipLaunchKernelGGL(attn_pos_k_kernel, dim3((unsigned)blocks_of(a->n_k)), dim3(1024), 0, s, *a, w);
