@@ -196,8 +196,10 @@ __device__ __forceinline__ void join_waves(float* lds, int n, Give&& give, Take&
 // NW wavefronts of 32 rows share the tiles of keys (wide_q 1), or KS share out the keys of one tile of rows and join their
 // results in LDS (wide_q 2: 64 readouts of one query over up to 400 keys, fp32, 30 us with one wavefront each, 15 so; one query
 // of 8 heads on 2 of 64 over 200003 keys, bf16: 30 us, 3.4 TB/s of keys and values).
+// Four wavefronts on a SIMD where a row is short and they wait for each other (20 structures of 1000 nodes, 4 heads of 32, bf16:
+// 59 us with three, 50 so).
 template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
-__global__ void __launch_bounds__(64 * NW * KS, NW == 4 || DP * sizeof(T) <= 256 ? 2 : 1)
+__global__ void __launch_bounds__(64 * NW * KS, sizeof(T) == 2 && DP <= 32 ? 4 : NW == 4 || DP * sizeof(T) <= 256 ? 2 : 1)
 attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
   using S = AttnShape<T, DP>;
   constexpr int kBlock = kBlockOf<T, DP, NW>, kTile = kBlock * S::kRow, kBuf = KS > 1 || kLean<T, DP, NW> ? 1 : kBuffers<2 * kTile>;
