@@ -195,7 +195,7 @@ __device__ __forceinline__ void join_waves(float* lds, int n, Give&& give, Take&
 //
 // NW wavefronts of 32 rows share the tiles of keys (wide_q 1), or KS share out the keys of one tile of rows and join their
 // results in LDS (wide_q 2: 64 readouts of one query over up to 400 keys, fp32, 30 us with one wavefront each, 15 so; one query
-// of 8 heads on 2 of 64 over 200003 keys, bf16: 30 us, 3.4 TB/s of keys and values).
+// of 8 heads on 2 of 64 over 200003 keys, bf16: 25 us, 4.1 TB/s of keys and values).
 // Four wavefronts on a SIMD where a row is short and they wait for each other (20 structures of 1000 nodes, 4 heads of 32, bf16:
 // 59 us with three, 50 so).
 template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
@@ -355,7 +355,7 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
 }
 
 // Adds the parts of a row: a workgroup for each (tile, head of keys, row), its slots shared out over slices of threads.  A few
-// slots in flight for each thread: bound by latency, 8.5 us for that query.
+// slots in flight for each thread: bound by latency, 6 us for that query.
 constexpr int kJoinThreads = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) attn_fwd_join_kernel(AttnLaunch a, const float* __restrict__ parts, int rows) {
