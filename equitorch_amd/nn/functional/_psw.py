@@ -21,6 +21,7 @@ from torch.autograd import Function
 
 from ... import _lib
 from ...ops import kernels
+from ._higher_order import higher_order
 
 _END_ROW = 1 << 24
 _NO_TERM = 1 << 25       # the path has no term for this row: the entry only closes the (zero) row
@@ -171,10 +172,7 @@ class _Product(Function):
         x, y, w = ctx.saved_tensors
         need = ctx.needs_input_grad[:3]
         if torch.is_grad_enabled():
-            with torch.enable_grad():
-                inputs = [t for t, n in zip((x, y, w), need) if n]
-                grads = iter(torch.autograd.grad(ctx.fallback(x, y, w), inputs, g, create_graph=True))
-            return tuple(next(grads) if n else None for n in need) + (None, None)
+            return (*higher_order(ctx.fallback, (x, y, w), need, g), None, None)
         g = g.contiguous()
         if g.data_ptr() % 16:
             g = g.clone()

@@ -10,6 +10,7 @@ from torch import Tensor
 from torch.autograd import Function
 
 from ... import _lib
+from ._higher_order import higher_order
 
 POLYNOMIAL, COSINE, MOLLIFIER = 0, 1, 2
 
@@ -36,10 +37,7 @@ class _Bessel(Function):
         r, freq = ctx.saved_tensors
         need = ctx.needs_input_grad[:2]
         if torch.is_grad_enabled():
-            with torch.enable_grad():
-                inputs = [t for t, n in zip((r, freq), need) if n]
-                grads = iter(torch.autograd.grad(ctx.expression(r, freq), inputs, g, create_graph=True))
-            return tuple(next(grads) if n else None for n in need) + (None, None)
+            return (*higher_order(ctx.expression, (r, freq), need, g), None, None)
         g = g.contiguous()
         gr = torch.empty_like(r) if need[0] else None
         rows = torch.empty_like(g) if need[1] else None
@@ -73,9 +71,7 @@ class _Cutoff(Function):
         if not ctx.needs_input_grad[0]:
             return (None,) * 6
         if torch.is_grad_enabled():
-            with torch.enable_grad():
-                (gr,) = torch.autograd.grad(ctx.expression(r), (r,), g, create_graph=True)
-            return (gr,) + (None,) * 5
+            return (*higher_order(ctx.expression, (r,), (True,), g),) + (None,) * 5
         g = g.contiguous()
         gr = torch.empty_like(r)
         kind, r_min, span, param = ctx.args

@@ -23,6 +23,7 @@ from torch.autograd import Function
 from ... import _lib
 from ..._tables import TpCoo
 from ...ops import kernels
+from ._higher_order import higher_order
 
 FIRST, LAST = 1, 2
 
@@ -743,11 +744,8 @@ class _U1vNative(Function):
         tp_info = ctx.tp_info
         higher = torch.is_grad_enabled()  # higher-order derivative: the differentiable route throughout
         if higher or (isinstance(tp_info, CooTable) and tp_info.algebra and _observed(g)):
-            with torch.enable_grad():
-                out = tp_info.fallback(x, y, w) if isinstance(tp_info, CooTable) else _uv_gemm.u1v(x, y, w, tp_info)
-                wanted = [t for t, n in zip((x, y, w), need) if n]
-                got = iter(torch.autograd.grad(out, wanted, g, create_graph=higher, allow_unused=True))
-            return tuple(next(got) if n else None for n in need) + (None,)
+            plain = tp_info.fallback if isinstance(tp_info, CooTable) else lambda *t: _uv_gemm.u1v(*t, tp_info)
+            return (*higher_order(plain, (x, y, w), need, g, create_graph=higher), None)
         c = _coo(tp_info)
         p, u, wc = w.shape
         gx = gy = gw = None
@@ -833,11 +831,7 @@ class _Vu1Native(Function):
         x, y, w = ctx.saved_tensors
         need = ctx.needs_input_grad[:3]
         if torch.is_grad_enabled():       # higher-order derivative: the differentiable route throughout
-            with torch.enable_grad():
-                out = _uv_gemm.vu1(x, y, w, ctx.tp_info)
-                wanted = [v for v, n in zip((x, y, w), need) if n]
-                got = iter(torch.autograd.grad(out, wanted, g, create_graph=True, allow_unused=True))
-            return tuple(next(got) if n else None for n in need) + (None,)
+            return (*higher_order(lambda *t: _uv_gemm.vu1(*t, ctx.tp_info), (x, y, w), need, g), None)
         t = _swapped(ctx.tp_info)
         c = t.coo
         p, u, wc = w.shape
@@ -887,11 +881,7 @@ class _UvwNative(Function):
         need = ctx.needs_input_grad[:3]
         tp_info = ctx.tp_info
         if torch.is_grad_enabled():
-            with torch.enable_grad():
-                out = _uvw_gemm.uvw(x, y, w, tp_info)
-                wanted = [t for t, n in zip((x, y, w), need) if n]
-                got = iter(torch.autograd.grad(out, wanted, g, create_graph=True, allow_unused=True))
-            return tuple(next(got) if n else None for n in need) + (None,)
+            return (*higher_order(lambda *t: _uvw_gemm.uvw(*t, tp_info), (x, y, w), need, g), None)
         c = _coo(tp_info)
         p, u, v, wc = w.shape
         g = _aligned(g)

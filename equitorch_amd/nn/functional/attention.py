@@ -15,7 +15,7 @@ from torch.autograd import Function
 
 from ... import _lib, _shim
 from ..._lib import AttnArgs, CgtpError
-from .edge import _higher_order
+from ._higher_order import higher_order
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _BLOCK = 64                     # keys (rows) of a tile: pieces of a structure begin at multiples of it
@@ -174,7 +174,7 @@ class AttentionPlan:
             t, buckets = self.tables(group, heads), self._buckets
             h = mod.AttnHandle(t.q_items, t.q_joins, t.k_items, t.k_joins, t.q_slots, t.k_slots, t.wide_q, t.wide_k)
             # holds the buckets, not the plan: the node keeps it for as long as it lives itself
-            h.set_fallback(lambda g, inputs, need: _higher_order(_of_buckets(buckets, scale, cap), inputs, need, g))
+            h.set_fallback(lambda g, inputs, need: higher_order(_of_buckets(buckets, scale, cap), inputs, need, g))
             self._tables[key] = h
         return self._tables[key]
 
@@ -288,7 +288,7 @@ class _SegmentAttention(Function):
         need, plan, scale, cap = ctx.needs_input_grad[:6], ctx.plan, ctx.scale, ctx.cap
         if torch.is_grad_enabled():
             expression = _of_buckets(plan._buckets, scale, cap)
-            return (*_higher_order(expression, (q, k, v, pos_q, pos_k, slope), need, g), None, None, None)
+            return (*higher_order(expression, (q, k, v, pos_q, pos_k, slope), need, g), None, None, None)
         g = g.contiguous()
         g = g if g.data_ptr() % 16 == 0 else g.clone()
         a = _args(q, k, v, pos_q, pos_q if pos_k is None else pos_k, slope, plan, scale, cap)

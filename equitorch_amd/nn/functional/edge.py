@@ -19,6 +19,7 @@ from torch.autograd import Function
 from ... import _lib
 from ...ops import kernels
 from ...structs import TensorProductInfo
+from ._higher_order import higher_order
 from .linears import tensor_product_u1u
 from .sparse_scale import sparse_scale
 from ...structs import SparseScaleInfo
@@ -107,14 +108,6 @@ def _unfused(plan: EdgePlan, tp_info: TensorProductInfo, y_vec: int = 0):
     return expression
 
 
-def _higher_order(expression, inputs, need, g: Tensor):
-    """Gradients of ``expression(*inputs)`` for the inputs ``need`` marks, themselves differentiable."""
-    with torch.enable_grad():
-        wanted = [t for t, n in zip(inputs, need) if n]
-        grads = iter(torch.autograd.grad(expression(*inputs), wanted, g, create_graph=True, allow_unused=True))
-    return tuple(next(grads) if n else None for n in need)
-
-
 def _shim_handle(plan: EdgePlan, cfg, x: Tensor, y_vec: int, tp_info: TensorProductInfo):
     """The C++ extension's handle of this plan for one compiled table, dtype and channel count (it holds the sorted
     views and the range tables of both directions), or None when the extension is not there or the table needs the
@@ -135,7 +128,7 @@ def _shim_handle(plan: EdgePlan, cfg, x: Tensor, y_vec: int, tp_info: TensorProd
             views += [seg.ptr, seg.perm, seg.seg_ids, seg.gather, wave_seg, wave_pos]
         handles[key] = mod.EdgeHandle(int(cfg), int(kernels.uvu_dims(cfg)[2]), int(y_vec), scale, *views)
         expression = _unfused(plan, tp_info, y_vec)
-        handles[key].set_fallback(lambda g, x_, y_, w_, *need: _higher_order(expression, (x_, y_, w_), need, g))
+        handles[key].set_fallback(lambda g, x_, y_, w_, *need: higher_order(expression, (x_, y_, w_), need, g))
     return handles[key]
 
 
@@ -153,7 +146,7 @@ class _EdgeUvuCompiled(Function):
         x, sh, w = ctx.saved_tensors
         plan = ctx.plan
         if torch.is_grad_enabled():
-            return (*_higher_order(_unfused(plan, ctx.tp_info), (x, sh, w), ctx.needs_input_grad[:3], g), None, None, None)
+            return (*higher_order(_unfused(plan, ctx.tp_info), (x, sh, w), ctx.needs_input_grad[:3], g), None, None, None)
         res = kernels.uvu_backward(ctx.cfg, ctx.dims, x, sh, w, g.contiguous(), ctx.needs_input_grad[:3],
                                    seg=plan.bwd_index)
         return (*res, None, None, None)
@@ -175,7 +168,7 @@ class _EdgeUvuVectors(Function):
         x, vec, w = ctx.saved_tensors
         if torch.is_grad_enabled():
             expression = _unfused(ctx.plan, ctx.tp_info, ctx.y_vec)
-            return (*_higher_order(expression, (x, vec, w), ctx.needs_input_grad[:3], g), None, None, None, None)
+            return (*higher_order(expression, (x, vec, w), ctx.needs_input_grad[:3], g), None, None, None, None)
         res = kernels.uvu_backward(ctx.cfg, ctx.dims, x, vec, w, g.contiguous(), ctx.needs_input_grad[:3],
                                    seg=ctx.plan.bwd_index, y_vec=ctx.y_vec)
         return (*res, None, None, None, None)
@@ -204,7 +197,7 @@ class _EdgeUvuRadial(Function):
 
             def expression(x_, y_, h_, w_):
                 return plain(x_, y_, (h_ @ w_.reshape(w_.shape[0], -1)).view(h_.shape[0], *w_.shape[1:]))
-            return (*_higher_order(expression, (x, y, h, w_last), need, g), None, None, None, None)
+            return (*higher_order(expression, (x, y, h, w_last), need, g), None, None, None, None)
         gx, gy, gh, gwe = kernels.uvu_radial_backward(ctx.cfg, ctx.dims, x, y, h, w_eff, g.contiguous(), need,
                                                       ctx.plan.bwd_index, ctx.y_vec)
         gwl = None
@@ -233,7 +226,7 @@ class _EdgeUvuTable(Function):
     def backward(ctx, g):
         x, sh, w = ctx.saved_tensors
         if torch.is_grad_enabled():
-            return (*_higher_order(_unfused(ctx.plan, ctx.tp_info), (x, sh, w), ctx.needs_input_grad[:3], g), None, None, None, None)
+            return (*higher_order(_unfused(ctx.plan, ctx.tp_info), (x, sh, w), ctx.needs_input_grad[:3], g), None, None, None, None)
         res = kernels.uvu_tab_backward(ctx.tab, x, sh, w, g.contiguous(), ctx.needs_input_grad[:3], ctx.plan.bwd_index,
                                        ctx.as_it_is)
         return (*res, None, None, None, None)
@@ -260,7 +253,7 @@ class _EdgeUvuRows(Function):
         plan = ctx.plan
         need = ctx.needs_input_grad[:3]
         if torch.is_grad_enabled():
-            return (*_higher_order(_unfused(plan, ctx.tp_info), (x, sh, w), need, g), None, None, None)
+            return (*higher_order(_unfused(plan, ctx.tp_info), (x, sh, w), need, g), None, None, None)
         gxe, gy, gw = kernels.uvu_backward(ctx.cfg, ctx.dims, x, sh, w, g.contiguous(), need, gather=plan.dst,
                                            x_gather=plan.src)
         gx = None

@@ -12,7 +12,7 @@ from torch.autograd import Function
 
 from ... import _lib, _shim
 from ..._lib import CgtpError, GffArgs
-from .edge import _higher_order
+from ._higher_order import higher_order
 
 _ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
 _EXPRESSIONS = (torch.nn.functional.silu, torch.nn.functional.gelu, torch.sigmoid)
@@ -60,7 +60,7 @@ _fallbacks = {}
 def _fallback(mod, act: int):
     """The extension's number for the tensor expression of an activation, which a backward under gradient mode evaluates."""
     if act not in _fallbacks:
-        _fallbacks[act] = mod.Fallback(lambda g, inputs, need: _higher_order(_expression(act), inputs, need, g))
+        _fallbacks[act] = mod.Fallback(lambda g, inputs, need: higher_order(_expression(act), inputs, need, g))
     return _fallbacks[act]
 
 
@@ -77,7 +77,7 @@ class _GatedFeedForward(Function):
         x, w_gate, w_up, w_down, gate, up, mid = ctx.saved_tensors
         need = ctx.needs_input_grad[:4]
         if torch.is_grad_enabled():
-            return (*_higher_order(_expression(ctx.act), (x, w_gate, w_up, w_down), need, g), None)
+            return (*higher_order(_expression(ctx.act), (x, w_gate, w_up, w_down), need, g), None)
         g = g.contiguous()
         grads = [torch.empty_like(t) if n else None for t, n in zip((x, w_gate, w_up, w_down), need)]
         g_gate, g_up = torch.empty((2, *mid.shape), dtype=x.dtype, device=x.device)

@@ -5,6 +5,7 @@ from torch.autograd import Function
 
 from ...ops import kernels
 from ...structs import IrrepsInfo
+from ._higher_order import higher_order
 from .activations import _broadcast_infos
 from .norm import batch_mean_squared_norm, channel_mean_squared_norm
 from .sparse_product import sparse_mul, sparse_vecsca
@@ -53,12 +54,8 @@ class _LayerRMSFused(Function):
         x, weight, rsigma = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[0], weight is not None and ctx.needs_input_grad[1]
         if torch.is_grad_enabled():
-            with torch.enable_grad():
-                out = _layer_rms_composed(x, ctx.irreps_info, weight, ctx.scaled, ctx.eps)
-                wanted = [t for t, n in ((x, need_x), (weight, need_w)) if n]
-                grads = list(torch.autograd.grad(out, wanted, g, create_graph=True))
-            gx = grads.pop(0) if need_x else None
-            gw = grads.pop(0) if need_w else None
+            gx, gw = higher_order(lambda x_, w_: _layer_rms_composed(x_, ctx.irreps_info, w_, ctx.scaled, ctx.eps), (x, weight),
+                                  (need_x, need_w), g)
             return gx, gw, None, None, None
         gx, gw = kernels.layer_rms_backward(x, weight, rsigma, g.contiguous(), ctx.irreps_info.irrep_seg,
                                             ctx.irreps_info.rdims, ctx.scaled,

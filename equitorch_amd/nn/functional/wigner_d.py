@@ -12,6 +12,7 @@ from torch.autograd import Function
 
 from ...ops import kernels
 from ...structs import WignerRotationInfo
+from ._higher_order import higher_order
 from .angular import sincos
 from .sparse_product import sparse_vecsca
 from .sparse_scale import sparse_scale
@@ -52,14 +53,8 @@ class _FusedRotation(Function):
         x, sa, sb, sg = ctx.saved_tensors
         need_cs = [t is not None and ctx.needs_input_grad[1 + i] for i, t in enumerate((sa, sb, sg))]
         if torch.is_grad_enabled():          # a gradient of this gradient is wanted
-            with torch.enable_grad():
-                out = _composed_rotation(x, sa, sb, sg, ctx.info)
-                wanted = [(i, t) for i, t in enumerate((x, sa, sb, sg)) if t is not None and ctx.needs_input_grad[i]]
-                grads = torch.autograd.grad(out, [t for _, t in wanted], g, create_graph=True)
-            res = [None] * 4
-            for (i, _), gr in zip(wanted, grads):
-                res[i] = gr
-            return (*res, None, None)
+            return (*higher_order(lambda *t: _composed_rotation(*t, ctx.info), (x, sa, sb, sg),
+                                  (ctx.needs_input_grad[0], *need_cs), g), None, None)
         if not any(need_cs):                 # the transposed rotation; nothing to recompute
             return kernels.wigner_rotate(g.contiguous(), sa, sb, sg, ctx.layout, transposed=True), None, None, None, None, None
         gx, gcs = kernels.wigner_rotate_backward(x, g.contiguous(), (sa, sb, sg), ctx.layout, ctx.needs_input_grad[0],
