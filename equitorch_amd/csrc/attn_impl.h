@@ -60,6 +60,8 @@ struct Score {
       c[1] = linear * z * z * (2.f / 15.f);
       c[2] = linear * z * z * z * (-17.f / 315.f);
       c[3] = linear * z * z * z * z * (62.f / 2835.f);
+      // A cap far below the scale takes them past fp32.  The other form serves alone then: what it errs by is 2^-24 of that cap.
+      if (!(fabsf(c[0]) + fabsf(c[1]) + fabsf(c[2]) + fabsf(c[3]) <= 1e38f)) near = -1.f;
     }
   }
   __device__ __forceinline__ bool plain() const { return !CAPPED && !BIASED && linear > 0.f; }

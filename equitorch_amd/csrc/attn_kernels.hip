@@ -3,6 +3,7 @@
 #include "attn_host.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace cgtp {
 namespace {
@@ -180,9 +181,16 @@ void launch_type(const AttnLaunch& a, const AttnScratch* w, hipStream_t s) {
   if (a.slope) a.cap > 0.f ? attn_launch<T, true, true>(a, w, s) : attn_launch<T, true, false>(a, w, s);
   else a.cap > 0.f ? attn_launch<T, false, true>(a, w, s) : attn_launch<T, false, false>(a, w, s);
 }
+// A cap that the kernels can form scale / cap and its square with.  Smaller ones are as good as this: scores all but equal.  Larger
+// ones do not show before products q.k of 2^52, in scores that differ by more than any softmax tells apart.
+float usable_cap(float scale, float cap) {
+  if (!(cap > 0.f) || cap > std::fabs(scale) * 0x1p64f) return 0.f;
+  return std::max(cap, std::max(std::fabs(scale), 1.f) * 0x1p-100f);
+}
 // copies: where they start in the workspace.
 void launch(const cgtp_attn_args& args, const AttnScratch* w, int64_t copies, hipStream_t s) {
   AttnLaunch a = launch_of(args);
+  a.cap = usable_cap(a.scale, a.cap);
   pack(a, w != nullptr, copies, true, s);
   if (a.dtype == CGTP_F32) launch_type<float>(a, w, s);
   else if (a.dtype == CGTP_BF16) launch_type<bf16_t>(a, w, s);

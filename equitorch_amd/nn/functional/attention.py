@@ -348,6 +348,8 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, pos:
     cap = 0.0 if cap is None else float(cap)
     if not 0.0 <= cap < float("inf"):
         raise CgtpError(f"cap must be positive and finite (or None), got {cap}")
+    if cap > 0.0:
+        cap = min(max(cap, 2.0 ** -100), 2.0 ** 127)      # as a float neither zero, which is no cap, nor infinite
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
     pos, pos_k, slope = (None if t is None else t.contiguous() for t in (pos, pos_k, slope))

@@ -531,3 +531,25 @@ def test_attention_as_in_a_large_batch(device, monkeypatch, dtype, lengths, head
     from equitorch_amd.nn.functional import attention
     monkeypatch.setattr(attention, "_SMALL", 0)
     test_attention(device, dtype, lengths, heads, kv_heads, dim, biased, cap)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("scale,cap", [(1.0, 1e-5), (0.125, 1e-6), (0.125, 1e-9), (1.0, 1e-30), (1.0, 1e-44), (1.0, 1e-60), (1e-3, 1e-6),
+                                       (64.0, 1e-3), (1.0, 1e25), (1.0, 3e38), (1.0, 1e300), (0.0, 5.0)])
+def test_attention_caps_of_every_size(device, dtype, scale, cap):
+    """Scores within 1e-3 of one another at most, or as good as uncapped, in lengths that leave rows and keys of a tile empty."""
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    gen = torch.Generator().manual_seed(31)
+    lengths, heads, dim = [1, 40, 33], 2, 24
+    n = sum(lengths)
+    q, k, v, ct = (_rand(gen, n, heads, dim, dtype=dtype) for _ in range(4))
+    q[7] = 0.0                                             # scores of exactly zero
+    val, mag, top = _reference(q, k, v, lengths, lengths, None, None, None, scale, cap, ct)
+    plan = AttentionPlan(torch.tensor([0] + lengths, device=device).cumsum(0))
+    leaves = [t.to(device).requires_grad_(True) for t in (q, k, v)]
+    out = segment_attention(*leaves, plan, cap=cap, scale=scale)
+    grads = torch.autograd.grad(out, leaves, ct.to(device))
+    # as for other caps (test_attention); `top` bounds the products, not the scores, where these are within the cap
+    unit = 4 * EPS[dtype] + EPS[F32] * (32 + dim + 16 * top) if dtype != F32 else EPS[F32] * (32 + dim + 16 * top)
+    for name, got in zip(("out", "q", "k", "v"), (out, *grads)):
+        _within(got, val[name], EPS[dtype] * val[name].abs() + unit * mag[name] + 64 * TINY[dtype], name)
