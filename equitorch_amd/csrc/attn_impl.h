@@ -303,7 +303,7 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
         for (int e = 0; e < 16; ++e) acc[o][e] *= by;
       top = most;
     }
-    const float base = top == -INFINITY ? 0.f : -top * sc.unit;
+    const float base = top == -INFINITY ? 0.f : fmaf(-top, sc.unit, (float)kUp<T>);
 #pragma unroll
     for (int b = 0; b < kBlock / 32; ++b) {
       if (b * 32 >= n) continue;
@@ -321,7 +321,7 @@ attn_fwd_kernel(AttnLaunch a, float* __restrict__ parts) {
       cols_times<T, DP>(acc, v_tile, 32 * b, t[b]);
     }
   }
-  top *= sc.unit;
+  top = fmaf(top, sc.unit, (float)-kUp<T>);
   if constexpr (KS > 1) {
     join_waves<KS>(reinterpret_cast<float*>(lds), 16 * S::kOut + 2, [&](float* at) {
       at[0] = top;
@@ -498,7 +498,7 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
     z = a.pos_q[(int64_t)row.query * 3 + 2];
     slope = a.slope[row.head];
   }
-  const float slope2 = slope * kLog2E, grad_scale = a.scale;
+  const float slope2 = slope * kLog2E;
   AttnAcc<T, DP> acc;
 #pragma unroll
   for (int o = 0; o < S::kOut; ++o)
@@ -509,6 +509,7 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
   // exact one is delta + sum ds, and with it the gradients of positions and slopes, which are fp32, err as in fp32.
   constexpr bool kFix = sizeof(T) == 2;
   QSums m = {};
+  ColumnFit<T, DP> fit;
   TileStage<T, DP, 64 * NW, kBlock> ks, other;
   auto& vs = LEAN ? ks : other;
   float ps[3] = {};
@@ -600,10 +601,12 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
       };
       if (n < 32 * b + 32) turn(true);
       else turn(false);
+      fit.fit(ds, acc);
       cols_times<T, DP>(acc, k_tile, 32 * b, ds);
     }
   }
   if constexpr (KS > 1) {
+    fit.settle(acc);
     join_waves<KS>(reinterpret_cast<float*>(lds), 16 * S::kOut + 9, [&](float* at) {
 #pragma unroll
       for (int i = 0; i < 9; ++i) at[i * 64] = m.v[i];
@@ -621,6 +624,7 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
   for (int i = 0; i < (kFix ? 9 : 4); ++i) m.v[i] += half_swap(m.v[i]);
   m.v[9] = delta;
   if (!row.ok) return;
+  const float grad_scale = fit.undo(a.scale);
   if (it.slot < 0) {
     if (a.grad_q) store_cols<T, DP>((T*)a.grad_q + at * a.dim, acc, grad_scale, a.dim);
     if (half == 0) m.finish(w, at, slope, BIASED);
@@ -705,6 +709,7 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) gk[o][e] = gv[o][e] = 0.f;
   float gx = 0.f, gy = 0.f, gz = 0.f;
+  ColumnFit<T, DP> fit;
   TileStage<T, DP, 64 * NW, kBlock> qs, other;
   auto& gs = LEAN ? qs : other;
   float st[6] = {};
@@ -719,7 +724,7 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
     if (threadIdx.x < kBlock) {
       const Row o = row_of(it, r0 + threadIdx.x, hk, group);
       const int64_t at = (int64_t)o.query * a.h_q + o.head;
-      st[0] = o.ok ? ((const float*)a.lse)[at] : INFINITY;        // +inf: probability zero
+      st[0] = o.ok ? ((const float*)a.lse)[at] - kUp<T> : INFINITY;        // +inf: probability zero
       st[1] = o.ok ? w.delta[at] : 0.f;
       if constexpr (BIASED) {
         st[2] = o.ok ? a.slope[o.head] : 0.f;
@@ -791,6 +796,7 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+      fit.fit(ds, gk);
       cols_times<T, DP>(gv, g_tile, 32 * b, t);
       cols_times<T, DP>(gk, q_tile, 32 * b, ds);
     }
@@ -800,19 +806,21 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
   gz += half_swap(gz);
   if (!ok) return;
   const int64_t at = (int64_t)key * a.h_kv + hk;
-  const float grad_scale = a.scale;
+  // p and ds were formed 2^kUp times as large
+  constexpr float kDown = 1.f / (1 << kUp<T>);
+  const float grad_scale = fit.undo(a.scale * kDown);
   if (it.slot < 0) {
     if (a.grad_k) store_cols<T, DP>((T*)a.grad_k + at * a.dim, gk, grad_scale, a.dim);
-    if (a.grad_v) store_cols<T, DP>((T*)a.grad_v + at * a.dim, gv, 1.f, a.dim);
-    if (BIASED && half == 0) w.key_part[at] = f32x4{gx, gy, gz, 0.f};
+    if (a.grad_v) store_cols<T, DP>((T*)a.grad_v + at * a.dim, gv, kDown, a.dim);
+    if (BIASED && half == 0) w.key_part[at] = f32x4{gx * kDown, gy * kDown, gz * kDown, 0.f};
   } else {
     float* p = w.parts + (((int64_t)it.slot * a.h_kv + hk) * kRowsOf<NW> + (key - it.k_begin)) * (2 * a.dim + 4);
     store_cols<float, (DP < 32 ? 32 : DP)>(p, gk, grad_scale, a.dim);
-    store_cols<float, (DP < 32 ? 32 : DP)>(p + a.dim, gv, 1.f, a.dim);
+    store_cols<float, (DP < 32 ? 32 : DP)>(p + a.dim, gv, kDown, a.dim);
     if (half == 0) {
-      p[2 * a.dim] = gx;
-      p[2 * a.dim + 1] = gy;
-      p[2 * a.dim + 2] = gz;
+      p[2 * a.dim] = gx * kDown;
+      p[2 * a.dim + 1] = gy * kDown;
+      p[2 * a.dim + 2] = gz * kDown;
       p[2 * a.dim + 3] = 0.f;
     }
   }

@@ -162,6 +162,50 @@ __device__ __forceinline__ void cols_times(AttnAcc<T, DP>& acc, const char* lds,
   }
 }
 
+// fp16 operands.  Its normal numbers end at 2^-14 and 65504, and a probability is 1 / keys, a score's gradient as much of the incoming
+// gradient, whatever that was scaled by.  So probabilities are 2^kUp times as large where they enter a product, and the
+// gradients of a column's scores `by` times, a power of two that falls as larger ones come, along with the sum so far.  6000 keys
+// and a gradient of 1e-3: dq and dk err 4e-4 of their norm in place of 8e-3.  It costs 5 to 15 % of a step (three structures of
+// 2000 to 5000 nodes, 8 query heads on 4 of 64, fp16: 1330 us without it, 1400 so); the sum is multiplied every time, as a branch
+// about it takes the gradient of keys and values 80 registers.  bf16 has fp32's range.
+template <typename T> constexpr int kUp = __is_same(T, f16_t) ? 10 : 0;
+template <typename T, int DP>
+struct ColumnFit {
+  static constexpr bool kOn = __is_same(T, f16_t);
+  float by = kOn ? 0x1p100f : 1.f;
+  // acc: the column's sum of such products so far.
+  __device__ __forceinline__ void fit(f32x16_t& d, AttnAcc<T, DP>& acc) {
+    if constexpr (kOn) {
+      float most = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(d[e]));
+      most = fmaxf(most, __shfl_xor(most, 32, kWave));
+      // an infinity has the exponent 0, and no factor becomes larger
+      const float now = most * by > 0x1p15f ? fminf(by, ldexpf(1.f, 13 - __builtin_amdgcn_frexp_expf(most))) : by;
+      scale(acc, now * inverse(by));
+      by = now;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) d[e] *= by;
+    }
+  }
+  __device__ __forceinline__ float undo(float x) const { return kOn ? x * inverse(by) : x; }
+  __device__ __forceinline__ void settle(AttnAcc<T, DP>& acc) {
+    if constexpr (kOn) {
+      scale(acc, inverse(by));
+      by = 1.f;
+    }
+  }
+
+ private:
+  __device__ static __forceinline__ float inverse(float power) { return ldexpf(1.f, 1 - __builtin_amdgcn_frexp_expf(power)); }
+  __device__ static __forceinline__ void scale(AttnAcc<T, DP>& acc, float f) {
+#pragma unroll
+    for (int o = 0; o < AttnShape<T, DP>::kOut; ++o)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[o][e] *= f;
+  }
+};
+
 // Results of a lane's column: its elements 32 o + 8 g + 4 (lane / 32) + e of dim, times `by`, to p.
 template <typename T, int DP>
 __device__ __forceinline__ void store_cols(T* p, const AttnAcc<T, DP>& acc, float by, int dim) {

@@ -553,3 +553,70 @@ def test_attention_caps_of_every_size(device, dtype, scale, cap):
     unit = 4 * EPS[dtype] + EPS[F32] * (32 + dim + 16 * top) if dtype != F32 else EPS[F32] * (32 + dim + 16 * top)
     for name, got in zip(("out", "q", "k", "v"), (out, *grads)):
         _within(got, val[name], EPS[dtype] * val[name].abs() + unit * mag[name] + 64 * TINY[dtype], name)
+
+
+def _attention_of_one_structure(q, k, v, ct, scale):
+    """Result and gradients in 64 bits, one head after the other."""
+    got = [torch.zeros_like(t) for t in (q, q, k, v)]
+    for h in range(q.shape[1]):
+        p = torch.softmax(q[:, h] @ k[:, h].T * scale, 1)
+        dp = ct[:, h] @ v[:, h].T
+        got[0][:, h], got[3][:, h] = p @ v[:, h], p.T @ ct[:, h]
+        ds = p * (dp - (p * dp).sum(1, keepdim=True)) * scale
+        got[1][:, h], got[2][:, h] = ds @ k[:, h], ds.T @ q[:, h]
+    return got
+
+
+@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("n_q,n_k,heads,dim,size,scale", [
+    (4000, 4000, 1, 64, 1e-3, None), (4000, 4000, 1, 64, 1.0, None), (4000, 4000, 1, 64, 1e4, None), (16, 100003, 2, 32, 1e4, None),
+    (1, 200003, 2, 16, 1e4, None), (300, 7001, 2, 96, 1e-2, None), (4, 5, 2, 128, 3e4, 2.0 ** -9), (6, 4, 1, 128, 3e4, 2.0 ** -9)])
+def test_attention_fp16_gradients_of_any_size(device, monkeypatch, wide, n_q, n_k, heads, dim, size, scale):
+    """Probabilities below fp16's normal range, and gradients of the scores below or beyond it where the results are within.  Each term of a
+    sum is rounded by 2^-11 at most, in either direction, and so is the result: of its norm 2^-10 together, and half a
+    subnormal step for each element."""
+    from equitorch_amd.nn.functional import AttentionPlan, attention, segment_attention
+    if not wide:
+        monkeypatch.setattr(attention, "_SMALL", 0)
+    gen = torch.Generator(device=device).manual_seed(41)
+    draw = lambda n: torch.randn(n, heads, dim, generator=gen, device=device)
+    q, k, v, ct = draw(n_q), draw(n_k), draw(n_k), draw(n_q).clamp(-1, 1) * size
+    q, k, v, ct = (t.half() for t in (q, k, v, ct))
+    plan = AttentionPlan(torch.tensor([0, n_q], device=device), torch.tensor([0, n_k], device=device))
+    scale = dim ** -0.5 if scale is None else scale
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = segment_attention(*leaves, plan, scale=scale)
+    grads = torch.autograd.grad(out, leaves, ct)
+    want = _attention_of_one_structure(*(t.double() for t in (q, k, v, ct)), scale)
+    for name, a, b in zip(("out", "q", "k", "v"), (out, *grads), want):
+        err, most = float((a.double() - b).norm()), 2.0 ** -10 * float(b.norm()) + 2.0 ** -25 * b.numel() ** 0.5
+        assert err <= most, f"{name}: {err:.3e} beyond {most:.3e}"
+
+
+def test_attention_fp16_gradients_of_rows_of_different_size(device):
+    """A column's factor is its own, falls as larger gradients come, and zeros, infinities and NaN stay theirs."""
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    gen = torch.Generator(device=device).manual_seed(42)
+    n, dim = 600, 32
+    q, k, v, ct = (torch.randn(n, 1, dim, generator=gen, device=device) for _ in range(4))
+    ct = ct * torch.logspace(-6, 3, n, device=device)[:, None, None]
+    ct[100:140] = 0.0
+    q, k, v, ct = (t.half() for t in (q, k, v, ct))
+    plan = AttentionPlan(torch.tensor([0, n], device=device))
+
+    def gradients(ct):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(segment_attention(*leaves, plan), leaves, ct)
+    got = gradients(ct)
+    want = _attention_of_one_structure(*(t.double() for t in (q, k, v, ct)), dim ** -0.5)[1:]
+    for row in range(n):                                   # dq: each row by its own size
+        err, most = float((got[0][row].double() - want[0][row]).norm()), 2.0 ** -9 * float(want[0][row].norm()) + 2.0 ** -24 * dim ** 0.5
+        assert err <= most, f"row {row}: {err:.3e} beyond {most:.3e}"
+    assert torch.equal(got[0][100:140], torch.zeros_like(got[0][100:140]))
+    for a, b in zip(got[1:], want[1:]):
+        assert float((a.double() - b).norm()) <= 2.0 ** -10 * float(b.norm())
+    ct[300] = float("inf")
+    bad = gradients(ct)
+    keep = torch.arange(n, device=device) != 300
+    assert torch.equal(bad[0][keep], got[0][keep]) and not torch.isfinite(bad[0][300]).any()
+    assert not torch.isfinite(bad[1]).any() and not torch.isfinite(bad[2]).any()
