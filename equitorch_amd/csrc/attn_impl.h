@@ -26,6 +26,9 @@ namespace cgtp {
 namespace {
 
 constexpr float kLog2E = 1.4426950408889634f;
+// Bounds of a squared distance in the backward, whose distance is d2 / sqrt(d2): a distance of zero gives 3e-19 and no direction, and a
+// node so far off that d2 is infinite (-inf for its score in the forward, taking it out) the probability 0, not inf * 0.
+constexpr float kNear2 = 1e-37f, kFar2 = 3e38f;
 
 template <int NW> constexpr int kRowsOf = 32 * NW;
 // Rows of a tile in LDS: 64 where four wavefronts move them, half of that for rows beyond 256 bytes, whose tiles on their way
@@ -572,8 +575,8 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
               dx = x - px[e];
               dy = y - py[e];
               dz = z - pz[e];
-              d2 = dx * dx + dy * dy + dz * dz;
-              inv = __builtin_amdgcn_rsqf(fmaxf(d2, 1e-37f));
+              d2 = __builtin_amdgcn_fmed3f(dx * dx + dy * dy + dz * dz, kNear2, kFar2);
+              inv = __builtin_amdgcn_rsqf(d2);
             }
             float p = exp2_fast(sc.less(t[i], slope2, d2 * inv) - lse);
             if (cut && first + e >= n) p = 0.f;
@@ -779,8 +782,8 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
             dx = px[e] - x;
             dy = py[e] - y;
             dz = pz[e] - z;
-            d2 = dx * dx + dy * dy + dz * dz;
-            inv = __builtin_amdgcn_rsqf(fmaxf(d2, 1e-37f));
+            d2 = __builtin_amdgcn_fmed3f(dx * dx + dy * dy + dz * dz, kNear2, kFar2);
+            inv = __builtin_amdgcn_rsqf(d2);
           }
           const float p = exp2_fast(sc.less(t[i], slope[e] * kLog2E, d2 * inv) - lse[e]);
           float d = p * (ds[i] - delta[e]);

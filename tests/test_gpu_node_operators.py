@@ -620,3 +620,35 @@ def test_attention_fp16_gradients_of_rows_of_different_size(device):
     keep = torch.arange(n, device=device) != 300
     assert torch.equal(bad[0][keep], got[0][keep]) and not torch.isfinite(bad[0][300]).any()
     assert not torch.isfinite(bad[1]).any() and not torch.isfinite(bad[2]).any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("small", [256, 0])
+@pytest.mark.parametrize("readout", [False, True])
+def test_attention_nodes_beyond_any_distance(device, monkeypatch, dtype, small, readout):
+    """A node so far off that its squared distance is infinite in fp32 takes no part: results and gradients stay finite."""
+    from equitorch_amd.nn.functional import AttentionPlan, attention, segment_attention
+    monkeypatch.setattr(attention, "_SMALL", small)
+    gen = torch.Generator().manual_seed(51)
+    len_k, heads, dim = [40, 150], 2, 16
+    len_q = [2, 3] if readout else len_k
+    nq, nk = sum(len_q), sum(len_k)
+    q, ct = (_rand(gen, nq, heads, dim, dtype=dtype) for _ in range(2))
+    k, v = (_rand(gen, nk, heads, dim, dtype=dtype) for _ in range(2))
+    pos_k, slope = _rand(gen, nk, 3), torch.rand(heads, generator=gen) + 0.1
+    pos_k[[3, 39, 77]] = torch.tensor([[1e20, 0.0, 0.0], [0.0, -3e19, 1e19], [2e25, 2e25, 2e25]])
+    pos = _rand(gen, nq, 3) if readout else pos_k
+    val, mag, top = _reference(q, k, v, len_q, len_k, pos, pos_k, slope, dim ** -0.5, 0.0, ct)
+    ptr = lambda n: torch.tensor([0] + n, device=device).cumsum(0)
+    plan = AttentionPlan(ptr(len_q), ptr(len_k)) if readout else AttentionPlan(ptr(len_k))
+    leaves = [t.to(device).requires_grad_(True) for t in (q, k, v, pos, slope)]
+    more = [pos_k.to(device).requires_grad_(True)] if readout else []
+    out = segment_attention(*leaves[:3], plan, pos=leaves[3], slope=leaves[4], pos_k=more[0] if more else None)
+    grads = torch.autograd.grad(out, leaves + more, ct.to(device))
+    if not readout:
+        val["pos"], mag["pos"] = val["pos"] + val["pos_k"], mag["pos"] + mag["pos_k"]
+    # as in test_attention, for the scores of nodes that take part: 40 at most
+    unit = 4 * EPS[dtype] + EPS[F32] * (32 + dim + 16 * 40) if dtype != F32 else EPS[F32] * (32 + dim + 16 * 40)
+    for name, got in zip(("out", "q", "k", "v", "pos", "slope", "pos_k"), (out, *grads)):
+        own_type = EPS[F32] if name in ("pos", "pos_k", "slope") else EPS[dtype]
+        _within(got, val[name], own_type * val[name].abs() + unit * mag[name] + 64 * TINY[dtype], name)
