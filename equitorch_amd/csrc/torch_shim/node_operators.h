@@ -30,15 +30,17 @@ struct FallbackHolder : torch::CustomClassHolder {
   Fallback fallback;
   explicit FallbackHolder(const Fallback& f) : fallback(f) {}
 };
-// fn(grad_out, inputs, need) -> gradients, into the first places of `places`.
-variable_list call_fallback(int64_t id, const at::Tensor& g, const variable_list& inputs, const std::vector<bool>& need, size_t places) {
+// fn(grad_out, inputs, need, *more) -> gradients, into the first places of `places`.
+template <typename... More>
+variable_list call_fallback(int64_t id, const at::Tensor& g, const variable_list& inputs, const std::vector<bool>& need, size_t places,
+                            More... more) {
   py::gil_scoped_acquire gil;
   const auto it = edge_fallbacks().find(id);
   TORCH_CHECK(it != edge_fallbacks().end(), "cgtp: no tensor expression for a gradient of higher order");
   py::list in, wanted;
   for (const auto& t : inputs) in.append(t.defined() ? py::cast(t) : py::none());
   for (bool n : need) wanted.append(n);
-  const py::tuple r = it->second(g, in, wanted);
+  const py::tuple r = it->second(g, in, wanted, more...);
   variable_list out(places);
   for (size_t i = 0; i < inputs.size(); ++i)
     if (!r[i].is_none()) out[i] = r[i].cast<at::Tensor>();
@@ -277,7 +279,8 @@ struct Attn : torch::autograd::Function<Attn> {
     size_t edge = 0;                    // the node has an edge for each operand that is there
     for (size_t i = 0; i < 6; ++i) need.push_back(s[i].defined() && ctx->needs_input_grad(edge++));
     if (at::GradMode::is_enabled())
-      return call_fallback(shape[4], grad[0], {s[0], s[1], s[2], s[3], s[4], s[5]}, need, 9);
+      return call_fallback(shape[4], grad[0], {s[0], s[1], s[2], s[3], s[4], s[5]}, need, 9, d["scale"].toDouble(),
+                           d["cap"].toDouble());
     c10::hip::HIPGuardMasqueradingAsCUDA guard(o.q.device());
     const AttnHandle h{s[8], s[9], s[10], s[11], shape[0], shape[1], shape[2], shape[3], {}};
     cgtp_attn_args a = attn_args(o, h, d["scale"].toDouble(), d["cap"].toDouble());
@@ -321,7 +324,7 @@ void bind_node_operators(py::module& m) {
                        c10::optional<at::Tensor> k_joins, int64_t q_slots, int64_t k_slots, int64_t wide_q, int64_t wide_k) {
         return AttnHandle{opt(q_items), opt(q_joins), opt(k_items), opt(k_joins), q_slots, k_slots, wide_q, wide_k, {}};
       }))
-      .def("set_fallback", &AttnHandle::set_fallback, "callable (grad_out, inputs, need) -> gradients, for gradients of higher order");
+      .def("set_fallback", &AttnHandle::set_fallback, "callable (grad_out, inputs, need, scale, cap) -> gradients, for gradients of higher order");
   m.def("attn", [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& pos_q,
                    const c10::optional<at::Tensor>& pos_k, const c10::optional<at::Tensor>& slope, const AttnHandle& h, double scale,
                    double cap, bool keep) {

@@ -145,7 +145,7 @@ class AttentionPlan:
             raise CgtpError(f"ptr is on {ptr.device}, ptr_k on {ptr_k.device}")
         self.num_structures = len(self.len_q)
         self.num_queries, self.num_keys = int(self.len_q.sum()), int(self.len_k.sum())
-        self._tables = {}
+        self._tables, self._handles = {}, {}
         self._buckets = _Buckets(self.len_q, self.len_k, self.device)
 
     @classmethod
@@ -167,16 +167,16 @@ class AttentionPlan:
             self._tables[key] = _Tables(self, group, heads)
         return self._tables[key]
 
-    def handle(self, mod, group: int, heads: int, scale: float, cap: float):
+    def handle(self, mod, group: int, heads: int):
         """The extension's copy of the tables, and the tensor expression its node evaluates under gradient mode."""
-        key = (group, heads, scale, cap)
-        if key not in self._tables:
+        key = (group, heads)
+        if key not in self._handles:
             t, buckets = self.tables(group, heads), self._buckets
             h = mod.AttnHandle(t.q_items, t.q_joins, t.k_items, t.k_joins, t.q_slots, t.k_slots, t.wide_q, t.wide_k)
             # holds the buckets, not the plan: the node keeps it for as long as it lives itself
-            h.set_fallback(lambda g, inputs, need: higher_order(_of_buckets(buckets, scale, cap), inputs, need, g))
-            self._tables[key] = h
-        return self._tables[key]
+            h.set_fallback(lambda g, inputs, need, scale, cap: higher_order(_of_buckets(buckets, scale, cap), inputs, need, g))
+            self._handles[key] = h
+        return self._handles[key]
 
 
 class _Buckets:
@@ -356,7 +356,7 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, pos:
     keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, pos, pos_k, slope))
     mod = _shim.module()
     if mod is not None:
-        handle = plan.handle(mod, q.shape[1] // k.shape[1], k.shape[1], scale, cap)
+        handle = plan.handle(mod, q.shape[1] // k.shape[1], k.shape[1])
         return mod.attn(q, k, v, pos, pos_k, slope, handle, scale, cap, keep)
     if keep:
         return _SegmentAttention.apply(q, k, v, pos, pos_k, slope, plan, scale, cap)

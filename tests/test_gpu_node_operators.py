@@ -652,3 +652,29 @@ def test_attention_nodes_beyond_any_distance(device, monkeypatch, dtype, small, 
     for name, got in zip(("out", "q", "k", "v", "pos", "slope", "pos_k"), (out, *grads)):
         own_type = EPS[F32] if name in ("pos", "pos_k", "slope") else EPS[dtype]
         _within(got, val[name], own_type * val[name].abs() + unit * mag[name] + 64 * TINY[dtype], name)
+
+
+def test_attention_plan_does_not_grow_with_scales_and_caps(device):
+    """A scale or a cap that changes every step leaves nothing behind on a lasting plan; the second order knows it all the same."""
+    from equitorch_amd import _shim
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    gen = torch.Generator().manual_seed(61)
+    plan = AttentionPlan(torch.tensor([0, 12, 30], device=device))
+    data = [_rand(gen, 30, 2, 8) for _ in range(4)]
+    seen = []
+    for step in range(5):
+        scale, cap = 0.3 + 0.1 * step, 2.0 + step
+        q, k, v, ct = (t.to(device).requires_grad_(True) for t in data)
+        out = segment_attention(q, k, v, plan, cap=cap, scale=scale)
+        (gq,) = torch.autograd.grad(out, q, ct, create_graph=True)
+        (gk,) = torch.autograd.grad(gq.square().sum(), k)
+        wide = [t.double().requires_grad_(True) for t in data]
+        want = torch.cat([torch.einsum("hij,jhd->ihd", torch.softmax(cap * torch.tanh(torch.einsum("ihd,jhd->hij", wide[0][s], wide[1][s])
+                                                                                      * scale / cap), -1), wide[2][s])
+                          for s in (slice(0, 12), slice(12, 30))])
+        (rq,) = torch.autograd.grad(want, wide[0], wide[3], create_graph=True)
+        (rk,) = torch.autograd.grad(rq.square().sum(), wide[1])
+        for a, b in ((out, want), (gq, rq), (gk, rk)):     # fp32, sums of some hundred terms
+            assert float((a.detach().cpu().double() - b.detach()).abs().max()) <= 1e-4 * max(1.0, float(b.abs().max()))
+        seen.append(len(plan._tables) + len(plan._handles))
+    assert _shim.module() is not None and seen == [2] * 5
