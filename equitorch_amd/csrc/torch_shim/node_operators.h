@@ -192,10 +192,19 @@ struct Gff : torch::autograd::Function<Gff> {
 // The kernels' tables of a plan for one number of heads.
 struct AttnHandle {
   at::Tensor q_items, q_joins, k_items, k_joins;
-  int64_t q_slots, k_slots, wide_q, wide_k;
+  int64_t q_slots, k_slots, wide_q, wide_k, stream;      // stream: what the tables were allocated on
   Fallback fallback;
   void set_fallback(py::object fn) { fallback.set(std::move(fn)); }
 };
+
+// The tables are read on the current stream: where that is not the stream of their memory, the memory is not handed out again
+// before what is queued here is done, whatever becomes of the plan.
+void record_tables(const AttnHandle& h, const at::Tensor& like) {
+  const auto s = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(like.device().index());
+  if ((int64_t)s.stream() == h.stream) return;
+  for (const at::Tensor& t : {h.q_items, h.q_joins, h.k_items, h.k_joins})
+    if (t.defined()) t.record_stream(s.unwrap());
+}
 
 struct AttnOperands {
   at::Tensor q, k, v, pos_q, pos_k, slope;      // pos_k undefined: the queries' positions are the keys' too
@@ -251,6 +260,7 @@ at::Tensor attn_forward(const AttnOperands& o, const AttnHandle& h, double scale
     ws = bytes_on(o.q, n);
     a.workspace = ws.data_ptr();
   }
+  record_tables(h, o.q);
   check_status(cgtp_attn_forward(&a, current_stream(o.q)), "cgtp_attn_forward");
   return out;
 }
@@ -264,7 +274,7 @@ struct Attn : torch::autograd::Function<Attn> {
     at::Tensor out = attn_forward(o, *h, scale, cap, &lse);
     ctx->save_for_backward({q, k, v, o.pos_q, o.pos_k, o.slope, out, lse, h->q_items, h->q_joins, h->k_items, h->k_joins});
     auto& d = ctx->saved_data;
-    d["shape"] = std::vector<int64_t>{h->q_slots, h->k_slots, h->wide_q, h->wide_k, h->fallback.id};
+    d["shape"] = std::vector<int64_t>{h->q_slots, h->k_slots, h->wide_q, h->wide_k, h->stream, h->fallback.id};
     d["scale"] = scale;
     d["cap"] = cap;
     d["keep"] = c10::IValue::make_capsule(c10::make_intrusive<FallbackHolder>(h->fallback));
@@ -279,10 +289,10 @@ struct Attn : torch::autograd::Function<Attn> {
     size_t edge = 0;                    // the node has an edge for each operand that is there
     for (size_t i = 0; i < 6; ++i) need.push_back(s[i].defined() && ctx->needs_input_grad(edge++));
     if (at::GradMode::is_enabled())
-      return call_fallback(shape[4], grad[0], {s[0], s[1], s[2], s[3], s[4], s[5]}, need, 9, d["scale"].toDouble(),
+      return call_fallback(shape[5], grad[0], {s[0], s[1], s[2], s[3], s[4], s[5]}, need, 9, d["scale"].toDouble(),
                            d["cap"].toDouble());
     c10::hip::HIPGuardMasqueradingAsCUDA guard(o.q.device());
-    const AttnHandle h{s[8], s[9], s[10], s[11], shape[0], shape[1], shape[2], shape[3], {}};
+    const AttnHandle h{s[8], s[9], s[10], s[11], shape[0], shape[1], shape[2], shape[3], shape[4], {}};
     cgtp_attn_args a = attn_args(o, h, d["scale"].toDouble(), d["cap"].toDouble());
     at::Tensor g = grad[0].contiguous();
     if ((uintptr_t)g.data_ptr() & 15) g = g.clone();
@@ -300,6 +310,7 @@ struct Attn : torch::autograd::Function<Attn> {
     a.grad_slope = (float*)mutable_ptr(out[5]);
     const at::Tensor ws = bytes_on(o.q, cgtp_attn_workspace_bytes(&a, 1));
     a.workspace = ws.data_ptr();
+    record_tables(h, o.q);
     check_status(cgtp_attn_backward(&a, current_stream(o.q)), "cgtp_attn_backward");
     return out;
   }
@@ -321,8 +332,8 @@ void bind_node_operators(py::module& m) {
   }, "gated feed-forward block; with its autograd node where a backward may follow (keep)");
   py::class_<AttnHandle>(m, "AttnHandle")
       .def(py::init([](c10::optional<at::Tensor> q_items, c10::optional<at::Tensor> q_joins, c10::optional<at::Tensor> k_items,
-                       c10::optional<at::Tensor> k_joins, int64_t q_slots, int64_t k_slots, int64_t wide_q, int64_t wide_k) {
-        return AttnHandle{opt(q_items), opt(q_joins), opt(k_items), opt(k_joins), q_slots, k_slots, wide_q, wide_k, {}};
+                       c10::optional<at::Tensor> k_joins, int64_t q_slots, int64_t k_slots, int64_t wide_q, int64_t wide_k, int64_t stream) {
+        return AttnHandle{opt(q_items), opt(q_joins), opt(k_items), opt(k_joins), q_slots, k_slots, wide_q, wide_k, stream, {}};
       }))
       .def("set_fallback", &AttnHandle::set_fallback, "callable (grad_out, inputs, need, scale, cap) -> gradients, for gradients of higher order");
   m.def("attn", [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& pos_q,

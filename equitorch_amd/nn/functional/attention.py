@@ -115,13 +115,27 @@ class _Tables:
         self.k_joins = _table((start_q[s], zero, zero, start_k[s] + k.tile_begin[cut], start_k[s] + k.tile_end[cut], zero,
                                k.first_slot[cut], k.pieces[cut]), None, plan.device)
         self.q_slots, self.k_slots = q.slots, k.slots
+        self.stream = _stream_of(plan.device)
 
     def put(self, a: AttnArgs) -> None:
+        _record(self.stream, self.q_items, self.q_joins, self.k_items, self.k_joins)
         for name in ("q_items", "q_joins", "k_items", "k_joins"):
             t = getattr(self, name)
             setattr(a, name, _lib.ptr(t))
             setattr(a, "n_" + name, 0 if t is None else t.shape[0])
         a.n_q_slots, a.n_k_slots, a.wide_q, a.wide_k = self.q_slots, self.k_slots, self.wide_q, self.wide_k
+
+
+def _stream_of(device) -> int:
+    return _lib.stream_ptr(device) if device.type == "cuda" else 0
+
+
+def _record(stream: int, *tensors: Optional[Tensor]) -> None:
+    """What a plan holds is read on the current stream: where that is not the stream of its memory, ``stream``, the memory is not
+    handed out again before what is queued here is done."""
+    for t in tensors:
+        if t is not None and t.is_cuda and _stream_of(t.device) != stream:
+            t.record_stream(torch.cuda.current_stream(t.device))
 
 
 def _wide(n: np.ndarray) -> bool:
@@ -133,7 +147,8 @@ class AttentionPlan:
     """Where the structures of a batch begin: ``ptr`` int64 ``(S + 1,)``, ``ptr[s] .. ptr[s + 1]`` the nodes of structure
     ``s``, and ``ptr_k`` the same for the keys where queries and keys are different nodes (a readout: one query for each
     structure).  Structures may be empty, on either side.  Built once for a batch (it reads ``ptr`` on the host), used by
-    every layer; the kernels' tables are made on first use for each number of heads and kept with it."""
+    every layer; the kernels' tables are made on first use for each number of heads and kept with it (a graph is captured after
+    that).  A plan may be used on any stream."""
 
     def __init__(self, ptr: Tensor, ptr_k: Optional[Tensor] = None):
         self.device = ptr.device
@@ -172,7 +187,7 @@ class AttentionPlan:
         key = (group, heads)
         if key not in self._handles:
             t, buckets = self.tables(group, heads), self._buckets
-            h = mod.AttnHandle(t.q_items, t.q_joins, t.k_items, t.k_joins, t.q_slots, t.k_slots, t.wide_q, t.wide_k)
+            h = mod.AttnHandle(t.q_items, t.q_joins, t.k_items, t.k_joins, t.q_slots, t.k_slots, t.wide_q, t.wide_k, t.stream)
             # holds the buckets, not the plan: the node keeps it for as long as it lives itself
             h.set_fallback(lambda g, inputs, need, scale, cap: higher_order(_of_buckets(buckets, scale, cap), inputs, need, g))
             self._handles[key] = h
@@ -205,6 +220,8 @@ class _Buckets:
                 out.append(tuple(torch.from_numpy(i).to(self.device) for i in index))
             order = np.concatenate(order) if order else np.zeros(0, dtype=np.int64)
             self._made = (out, torch.from_numpy(np.argsort(order)).to(self.device))
+            self._stream = _stream_of(self.device)
+        _record(self._stream, self._made[1], *(t for bucket in self._made[0] for t in bucket))
         return self._made
 
 

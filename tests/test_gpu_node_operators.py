@@ -678,3 +678,30 @@ def test_attention_plan_does_not_grow_with_scales_and_caps(device):
             assert float((a.detach().cpu().double() - b.detach()).abs().max()) <= 1e-4 * max(1.0, float(b.abs().max()))
         seen.append(len(plan._tables) + len(plan._handles))
     assert _shim.module() is not None and seen == [2] * 5
+
+
+@pytest.mark.parametrize("use_extension", [True, False])
+def test_attention_plan_dropped_while_another_stream_reads_it(device, monkeypatch, use_extension):
+    """The tables' memory is not handed out again before the work that another stream has queued with them is done."""
+    from equitorch_amd import _shim
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    if not use_extension:
+        monkeypatch.setattr(_shim, "_module", None)
+    n, count = 21, 4000                                    # tables of a size of their own, 128 kB
+    ptr = torch.arange(count + 1, device=device) * n
+    q = torch.randn(n * count, 1, 16, device=device)
+    want = segment_attention(q, q, q, AttentionPlan(ptr))
+    plan = AttentionPlan(ptr)
+    table = plan.tables(1, 1).q_items
+    place, size = table.data_ptr(), table.numel() * table.element_size()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)                     # a bounded wait, some 50 ms
+        out = segment_attention(q, q, q, plan)
+    del plan, table
+    ours = [torch.empty(size, dtype=torch.uint8, device=device) for _ in range(20)]
+    assert not side.query(), "the other stream was done too early to tell"
+    assert place not in {t.data_ptr() for t in ours}
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
