@@ -409,10 +409,11 @@ int gff_check(const cgtp_gff_args* a) {
   if (!a) return CGTP_ERR_NULL;
   if (a->dtype != CGTP_F32 && a->dtype != CGTP_BF16 && a->dtype != CGTP_F16) return CGTP_ERR_DTYPE;
   if (a->n_rows < 0 || a->n_rows > 0x7fffffff || a->c_in <= 0 || a->c_out <= 0 || a->hidden <= 0) return CGTP_ERR_SHAPE;
-  // a grid has fewer than 2^32 threads, the weights' partial results an index of 31 bits
-  if (((a->n_rows + 511) / 512) * ((std::max(std::max(a->hidden, a->c_in), a->c_out) + 31) / 32) >= (1 << 20)) return CGTP_ERR_SHAPE;
-  if ((int64_t)a->hidden * (2ll * a->c_in + a->c_out) > 0x7fffffff) return CGTP_ERR_SHAPE;
   if (a->c_in > 0x7fff || a->c_out > 0x7fff || a->hidden > 0x1ffff) return CGTP_ERR_SHAPE;
+  // A grid has fewer than 2^32 threads, 2^24 workgroups.  That many tiles are of 128 rows (those of 64 are for results of fewer than 256
+  // tiles of 128), by 64 hidden channels or 128 of x or out, and their rows are rounded up to eight tiles.
+  const int64_t cols = std::max({(a->hidden + 63) / 64, (a->c_in + 127) / 128, (a->c_out + 127) / 128});
+  if ((a->n_rows + 1023) / 1024 * 8 * cols >= (1 << 24)) return CGTP_ERR_SHAPE;
   if (a->activation < 0 || a->activation >= kActs) return CGTP_ERR_CONFIG;
   if (!a->w_gate || !a->w_up || !a->w_down) return CGTP_ERR_NULL;
   if (a->n_rows > 0 && !a->x) return CGTP_ERR_NULL;

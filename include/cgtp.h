@@ -782,7 +782,8 @@ int cgtp_embed_backward(const int64_t* kind, const void* grad_out, void* grad_ta
  * cgtp_gff_backward reads gate, up and mid, writes grad_gate and grad_up (buffers of the caller) and those
  * of grad_x, grad_w_gate, grad_w_up, grad_w_down that are not NULL; the weight gradients are summed over rows in a
  * fixed order.  workspace: cgtp_gff_workspace_bytes (0: may be NULL), 16-byte aligned.
- * n_rows < 2^31, c_in and c_out < 2^15, hidden < 2^17.  dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16.
+ * c_in and c_out < 2^15, hidden < 2^17, and ceil(n_rows / 1024) * max(ceil(hidden / 64), ceil(c_in / 128), ceil(c_out / 128)) <
+ * 2^21 (workgroups of one launch; 1.3e8 rows of 1024 hidden channels), else CGTP_ERR_SHAPE.  dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16.
  */
 enum { CGTP_ACT_SILU = 0, CGTP_ACT_GELU = 1 /* with the error function */, CGTP_ACT_SIGMOID = 2 };
 typedef struct {
@@ -804,7 +805,9 @@ int cgtp_gff_backward(const cgtp_gff_args* args, void* stream);
  *   lse_i = +inf.
  * q: (n_q, h_q, dim), k and v: (n_k, h_kv, dim), h_q a multiple of h_kv (query head h reads head h / (h_q / h_kv)), with
  * element strides *_node and *_head and contiguous along dim; out, grad_out and the gradients contiguous; lse (n_q, h_q)
- * fp32; pos_q (n_q, 3), pos_k (n_k, 3), slope (h_q) fp32.  lse NULL: not wanted.  Elements may lie anywhere an element may.  dim <= 128.
+ * fp32; pos_q (n_q, 3), pos_k (n_k, 3), slope (h_q) fp32.  lse NULL: not wanted.  Elements may lie anywhere an element may.  dim <= 128,
+ * h_q < 2^14; n_k, n_q and n_q * (h_q / h_kv) < 2^31; items times h_kv < 2^24 either way, and joins times h_kv times the
+ * rows of a tile < 2^22 (workgroups of one launch), else CGTP_ERR_SHAPE.
  *
  * The caller cuts the work into items.  The rows of a structure and a head of keys are its (query, query head) pairs, row =
  * query * (h_q / h_kv) + head.  q_items: tiles of at most cgtp_attn_rows(wide_q) rows (wide_q 0: a wavefront, 1: four, for

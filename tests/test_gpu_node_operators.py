@@ -705,3 +705,54 @@ def test_attention_plan_dropped_while_another_stream_reads_it(device, monkeypatc
     assert place not in {t.data_ptr() for t in ours}
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def test_gated_feed_forward_of_millions_of_wide_rows(device):
+    """More rows than fit 2^31 elements of what is kept: rows here and there against 64 bits."""
+    from equitorch_amd.nn.functional import gated_feed_forward
+    gen = torch.Generator(device=device).manual_seed(71)
+    rows, c, hidden = 2200001, 8, 8192
+    draw = lambda *s, std=1.0: (torch.randn(*s, generator=gen, device=device) * std).bfloat16()
+    x, wg, wu, wd = draw(rows, c), draw(c, hidden, std=c ** -0.5), draw(c, hidden, std=c ** -0.5), draw(hidden, c, std=hidden ** -0.5)
+    with torch.no_grad():
+        out = gated_feed_forward(x, wg, wu, wd)
+    at = torch.cat([torch.randint(0, rows, (60,), generator=gen, device=device), torch.tensor([0, 262143, 262144, rows - 1], device=device)])
+    g, u, w = (t.double() for t in (x[at].double() @ wg.double(), x[at].double() @ wu.double(), wd))
+    mid = g * torch.sigmoid(g) * u
+    # the products' sums in fp32, mid and the result rounded to bf16
+    bound = EPS[BF16] * ((mid @ w).abs() + 1.1 * mid.abs() @ w.abs()) + 1e-5
+    _within(out[at], (mid @ w).cpu(), bound.cpu(), "out")
+
+
+def test_gated_feed_forward_of_weights_beyond_31_bits(device):
+    """Weights with more than 2^31 elements together: results, and their gradients at places here and there, against 64 bits."""
+    from equitorch_amd.nn.functional import gated_feed_forward
+    gen = torch.Generator(device=device).manual_seed(72)
+    rows, c, hidden = 5, 12000, 65000
+    draw = lambda *s, std=1.0: (torch.randn(*s, generator=gen, device=device) * std).bfloat16()
+    t = [draw(rows, c), draw(c, hidden, std=c ** -0.5), draw(c, hidden, std=c ** -0.5), draw(hidden, c, std=hidden ** -0.5)]
+    t = [a.requires_grad_(True) for a in t]
+    ct = draw(rows, c)
+    out = gated_feed_forward(*t)
+    got = torch.autograd.grad(out, t, ct)
+    x, wg, wu, wd = (a.detach() for a in t)
+    want, size, gx, size_x = (torch.zeros(rows, c, dtype=F64, device=device) for _ in range(4))
+    cols = torch.tensor([0, 1, 32767, 32768, 64999], device=device)
+    xd, cd = x.double(), ct.double()
+    for h in range(0, hidden, 5000):
+        s = slice(h, h + 5000)
+        g, u, gm = xd @ wg[:, s].double(), xd @ wu[:, s].double(), cd @ wd[s].double().T
+        sig = torch.sigmoid(g)
+        mid, dg, du = g * sig * u, gm * u * (sig + g * sig * (1 - sig)), gm * g * sig
+        want += mid @ wd[s].double()
+        size += mid.abs() @ wd[s].double().abs()
+        gx += dg @ wg[:, s].double().T + du @ wu[:, s].double().T
+        # dg and du are rounded, as are g and u that they are formed from: four roundings of terms of this size
+        size_x += (gm * u).abs() @ wg[:, s].double().abs().T + (gm * g).abs() @ wu[:, s].double().abs().T
+        here = cols[(cols >= h) & (cols < h + 5000)] - h
+        for name, a, b, m in (("w_gate", got[1][:, here + h], xd.T @ dg[:, here], xd.abs().T @ (gm * u).abs()[:, here]),
+                              ("w_up", got[2][:, here + h], xd.T @ du[:, here], xd.abs().T @ (gm * g).abs()[:, here]),
+                              ("w_down", got[3][here + h], mid[:, here].T @ cd, mid.abs()[:, here].T @ cd.abs())):
+            _within(a, b.cpu(), (EPS[BF16] * (b.abs() + 6 * m) + 1e-4 * m).cpu(), name)
+    _within(out, want.cpu(), (EPS[BF16] * (want.abs() + 1.1 * size) + 1e-4 * size).cpu(), "out")
+    _within(got[0], gx.cpu(), (EPS[BF16] * (gx.abs() + 6 * size_x) + 1e-4 * size_x).cpu(), "x")

@@ -214,3 +214,18 @@ def test_expression_of_the_attention_is_the_definition():
                 want[a:a + lq, h] = torch.softmax(s, 1) @ v[b:b + lk, h // 2]
         a, b = a + lq, b + lk
     assert torch.allclose(got, want, rtol=0, atol=3e-6)
+
+
+def test_feed_forward_limits_are_those_of_its_launches():
+    """Refused from 2^21 tiles of 1024 rows by 64 hidden channels (128 of x and out) on, and by the widths; accepted below (the call then
+    misses a buffer: nothing is launched)."""
+    def code(n_rows, hidden, c_in=256, c_out=256):
+        a = _gff(n_rows=n_rows, c_in=c_in, hidden=hidden, c_out=c_out, mid=None)
+        codes = {_lib.lib.cgtp_gff_forward(C.byref(a), None), _lib.lib.cgtp_gff_backward(C.byref(a), None)}
+        assert len(codes) == 1
+        return codes.pop()
+    assert code(1 << 24, 1024) == code(3 << 20, 8192) == code((1 << 27) - 1024, 1024) == NULL
+    assert code(1 << 27, 1024) == code(1 << 24, 8192) == SHAPE
+    assert code((1 << 31) - 1, 64, 128, 129) == SHAPE and code((1 << 30), 64, 128, 129) == SHAPE and code(1 << 30, 64, 128, 128) == NULL
+    assert code(5, (1 << 17) - 1, (1 << 15) - 1, (1 << 15) - 1) == NULL
+    assert code(5, 1 << 17) == code(5, 64, 1 << 15) == code(5, 64, 8, 1 << 15) == SHAPE
