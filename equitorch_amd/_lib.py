@@ -322,6 +322,12 @@ def dtype_code(dtype: torch.dtype) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def forward_mode() -> bool:
+    """Whether a level of forward-mode differentiation is open: tensors may carry tangents, which an autograd node refuses and a
+    launch without one would drop."""
+    return torch.autograd.forward_ad._current_level >= 0
+
+
 def stream_ptr(device) -> int:
     """The current stream of ``device`` as a raw handle.  Asked from torch directly where it offers that (a tenth of the
     time of building a ``torch.cuda.Stream`` object per launch)."""

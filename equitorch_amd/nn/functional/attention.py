@@ -370,7 +370,8 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, pos:
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
     pos, pos_k, slope = (None if t is None else t.contiguous() for t in (pos, pos_k, slope))
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, pos, pos_k, slope))
+    keep = (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, pos, pos_k, slope))) \
+        or _lib.forward_mode()
     mod = _shim.module()
     if mod is not None:
         handle = plan.handle(mod, q.shape[1] // k.shape[1], k.shape[1])

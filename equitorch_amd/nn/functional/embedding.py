@@ -71,6 +71,6 @@ def embedding(kind: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
     mod = _shim.module()
     if mod is not None:
         return mod.embed(kind, table, float(scale))
-    if torch.is_grad_enabled() and table.requires_grad:
+    if (torch.is_grad_enabled() and table.requires_grad) or _lib.forward_mode():
         return _Embedding.apply(kind, table, float(scale))
     return _lookup(kind, table, float(scale))

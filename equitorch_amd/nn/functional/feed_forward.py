@@ -115,7 +115,7 @@ def gated_feed_forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, 
     flat = x.reshape(-1, c).contiguous()
     weights = [t.contiguous() for t in (w_gate, w_up, w_down)]
     act = _ACTIVATIONS[activation]
-    keep = torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    keep = (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or _lib.forward_mode()
     mod = _shim.module()
     if mod is not None:
         out = mod.gff(flat, *weights, act, keep, _fallback(mod, act))

@@ -756,3 +756,26 @@ def test_gated_feed_forward_of_weights_beyond_31_bits(device):
             _within(a, b.cpu(), (EPS[BF16] * (b.abs() + 6 * m) + 1e-4 * m).cpu(), name)
     _within(out, want.cpu(), (EPS[BF16] * (want.abs() + 1.1 * size) + 1e-4 * size).cpu(), "out")
     _within(got[0], gx.cpu(), (EPS[BF16] * (gx.abs() + 6 * size_x) + 1e-4 * size_x).cpu(), "x")
+
+
+@pytest.mark.parametrize("use_extension", [True, False])
+@pytest.mark.parametrize("operator", ["embedding", "attention", "feed_forward"])
+def test_tangents_are_refused_not_dropped(device, monkeypatch, use_extension, operator):
+    """Forward-mode differentiation is not served: an operand with a tangent raises, one without gives the usual result."""
+    import torch.autograd.forward_ad as forward_ad
+    from equitorch_amd import _shim
+    from equitorch_amd.nn.functional import AttentionPlan, embedding, gated_feed_forward, segment_attention
+    if not use_extension:
+        monkeypatch.setattr(_shim, "_module", None)
+    gen = torch.Generator().manual_seed(81)
+    plan, kind = AttentionPlan(torch.tensor([0, 9], device=device)), torch.arange(9, device=device)
+    x, w = _rand(gen, 9, 8).to(device), _rand(gen, 8, 8).to(device)
+    run = {"embedding": lambda x: embedding(kind, x), "feed_forward": lambda x: gated_feed_forward(x, w, w, w),
+           "attention": lambda x: segment_attention(*[x.view(9, 2, 4)] * 3, plan)}[operator]
+    want = run(x)
+    with forward_ad.dual_level():
+        assert torch.equal(run(x), want)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            run(forward_ad.make_dual(x, torch.ones_like(x)))
+        with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
+            run(forward_ad.make_dual(x, torch.ones_like(x)))
