@@ -322,6 +322,16 @@ def dtype_code(dtype: torch.dtype) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def of_one_type(*tensors):
+    """Under autocast, operands of different types (16-bit features, fp32 weights) in autocast's type, as torch's products take
+    them; else as they are."""
+    first = tensors[0].dtype
+    if all(t.dtype == first for t in tensors) or not torch.is_autocast_enabled("cuda") \
+            or any(t.dtype not in (torch.float32, torch.bfloat16, torch.float16) for t in tensors):
+        return tensors
+    return tuple(t.to(torch.get_autocast_dtype("cuda")) for t in tensors)
+
+
 def forward_mode() -> bool:
     """Whether a level of forward-mode differentiation is open: tensors may carry tangents, which an autograd node refuses and a
     launch without one would drop."""

@@ -361,6 +361,7 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, pos:
     Statistics and sums are in 32 bits; in 16-bit types the probabilities and the scores' gradients are rounded to the type
     as operands of the next product.  Results do not depend on timing; differentiable to any order, beyond the first
     through a tensor expression that holds the scores of every structure in memory."""
+    q, k, v = _lib.of_one_type(q, k, v)
     _check(q, k, v, plan, pos, slope, pos_k)
     cap = 0.0 if cap is None else float(cap)
     if not 0.0 <= cap < float("inf"):

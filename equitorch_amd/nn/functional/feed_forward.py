@@ -93,13 +93,13 @@ class _GatedFeedForward(Function):
 
 def gated_feed_forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activation: str = "silu") -> Tensor:
     """``(act(x w_gate) * (x w_up)) w_down`` over the last axis of ``x``: ``x`` ``(..., C_in)``, ``w_gate`` and ``w_up``
-    ``(C_in, H)``, ``w_down`` ``(H, C_out)``, all fp32, bf16 or fp16; ``activation`` ``"silu"``, ``"gelu"`` (with the error
+    ``(C_in, H)``, ``w_down`` ``(H, C_out)``, all fp32, bf16 or fp16 (under autocast also mixed: autocast's type); ``activation`` ``"silu"``, ``"gelu"`` (with the error
     function) or ``"sigmoid"``.
 
     Products and activation are computed in 32 bits.  What is kept between the products — ``act(x w_gate) * (x w_up)``,
     and for a backward pass the two projections and their gradients — is rounded to the operands' type, so in fp16 it has
     fp16's range.  Gradients of the weights are summed over the rows in a fixed order."""
-    tensors = (x, w_gate, w_up, w_down)
+    tensors = x, w_gate, w_up, w_down = _lib.of_one_type(x, w_gate, w_up, w_down)
     _lib.require_gpu(*tensors)
     if activation not in _ACTIVATIONS:
         raise CgtpError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")

@@ -779,3 +779,37 @@ def test_tangents_are_refused_not_dropped(device, monkeypatch, use_extension, op
             run(forward_ad.make_dual(x, torch.ones_like(x)))
         with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
             run(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_operands_of_different_types_under_autocast(device, dtype):
+    """16-bit features and fp32 weights: as with every operand rounded to autocast's type; gradients in the operands' own types.
+    Without autocast they are refused."""
+    from equitorch_amd.nn import GatedFeedForward, SegmentAttention
+    from equitorch_amd.nn.functional import AttentionPlan, gated_feed_forward, segment_attention
+    gen = torch.Generator().manual_seed(91)
+    x = _rand(gen, 30, 16, dtype=dtype).to(device)
+    ws = [_rand(gen, *s, std=0.3).to(device).requires_grad_(True) for s in ((16, 24), (16, 24), (24, 16))]
+    rounded = [w.detach().to(dtype).requires_grad_(True) for w in ws]
+    want = gated_feed_forward(x, *rounded)
+    grads = torch.autograd.grad(want.float().sum(), rounded)
+    with torch.autocast("cuda", dtype=dtype):
+        out = gated_feed_forward(x, *ws)
+    got = torch.autograd.grad(out.float().sum(), ws)
+    assert out.dtype == dtype and torch.equal(out, want)
+    for a, b in zip(got, grads):
+        assert a.dtype == F32 and torch.equal(a, b.float())
+    plan = AttentionPlan(torch.tensor([0, 11, 30], device=device))
+    q = x.view(30, 2, 8)
+    with torch.autocast("cuda", dtype=dtype):
+        assert torch.equal(segment_attention(q, q.float(), q, plan), segment_attention(q, q, q, plan))
+        for bad in ((x.double(), *ws), (x, ws[0].double(), *ws[1:])):
+            with pytest.raises(CgtpError):
+                gated_feed_forward(*bad)
+        attention, block = SegmentAttention(16, 2).to(device), GatedFeedForward(16, 24).to(device)
+        y = block(attention(x, plan, torch.zeros(30, 3, device=device)))
+    assert y.dtype == dtype and torch.isfinite(y).all()
+    with pytest.raises(CgtpError):
+        gated_feed_forward(x, *ws)
+    with pytest.raises(CgtpError):
+        segment_attention(q, q.float(), q, plan)
