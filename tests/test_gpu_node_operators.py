@@ -813,3 +813,13 @@ def test_operands_of_different_types_under_autocast(device, dtype):
         gated_feed_forward(x, *ws)
     with pytest.raises(CgtpError):
         segment_attention(q, q.float(), q, plan)
+
+
+LENGTHS["one long among many short"] = ([1] * 200, [5, 0, 33, 64] * 25 + [30011] + [7] * 99)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim,biased,cap", [(8, 8, 32, True, 0.0), (4, 1, 20, False, 3.0)])
+def test_attention_of_one_long_structure_among_many(device, dtype, heads, kv_heads, dim, biased, cap):
+    """Where the keys of one structure are cut and all others' are not."""
+    test_attention(device, dtype, "one long among many short", heads, kv_heads, dim, biased, cap)

@@ -229,3 +229,16 @@ def test_feed_forward_limits_are_those_of_its_launches():
     assert code((1 << 31) - 1, 64, 128, 129) == SHAPE and code((1 << 30), 64, 128, 129) == SHAPE and code(1 << 30, 64, 128, 128) == NULL
     assert code(5, (1 << 17) - 1, (1 << 15) - 1, (1 << 15) - 1) == NULL
     assert code(5, 1 << 17) == code(5, 64, 1 << 15) == code(5, 64, 8, 1 << 15) == SHAPE
+
+
+@pytest.mark.parametrize("len_q,len_k,group,heads,longest", [
+    ([1] * 64, [100000] + [300] * 63, 1, 8, 8192), ([1] * 600, [300] * 300 + [100000] + [300] * 299, 2, 8, 20000),
+    ([20] * 500 + [6000], None, 1, 2, 2048), ([0] * 40 + [2] * 40 + [1], [7] * 80 + [50000], 4, 1, 4096)])
+def test_attention_tables_of_one_long_structure_among_many(len_q, len_k, group, heads, longest):
+    """The long one's keys (rows) are cut by its own length, however many short ones there are, and every pair is still covered."""
+    from equitorch_amd.nn.functional import AttentionPlan
+    test_attention_tables_cover_every_pair_once(len_q, len_k, group, heads)
+    ptr = lambda n: torch.tensor([0] + list(n)).cumsum(0)
+    t = (AttentionPlan(ptr(len_q)) if len_k is None else AttentionPlan(ptr(len_q), ptr(len_k))).tables(group, heads)
+    items = t.q_items
+    assert int((items[:, 4] - items[:, 3]).max()) <= longest
