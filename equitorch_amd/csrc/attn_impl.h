@@ -15,8 +15,8 @@
 // single query of a structure brings all its heads to one tile.  A wavefront owns 32 rows (or 32 keys) and forms the scores with
 // the other operand's rows down the registers, so that a row's statistics take one exchange between the halves of the
 // wavefront and the probabilities are the next product's operand as they lie.  Tiles never cross structures: what another
-// structure holds, infinities and NaN included, is never read.  A key or row of a tile beyond its range is a zero in LDS and
-// its score -inf.
+// structure holds, infinities and NaN included, is never read.  A key or row of a tile beyond its range is a zero in LDS (in
+// the backward's scores the last one once more) and its probability zero.
 #pragma once
 
 #include "attn_tiles.h"
@@ -128,6 +128,8 @@ struct KeyRows {
   __device__ __forceinline__ KeyRows(const T* p, int64_t node, int64_t head, int hk, int k0, int n)
       : base(p + (int64_t)k0 * node + hk * head), node(node), n(n) {}
   __device__ __forceinline__ unsigned offset(int i) const { return i < n ? (unsigned)i * (unsigned)(node * sizeof(T)) : kNoRow; }
+  // The last row again for those beyond: what has no part in a sum is a score like the others, not a zero times an infinity.
+  __device__ __forceinline__ unsigned offset_again(int i) const { return offset(min(i, n - 1)); }
 };
 // The rows of a tile, from r0 on, n of them: query0 + (at + i) / group, head (at + i) % group of the kv head's.
 template <typename T>
@@ -146,6 +148,7 @@ struct QueryRows {
     const int q = query(i), h = at + i - q * group;
     return i < n ? (unsigned)q * (unsigned)(node * sizeof(T)) + (unsigned)h * (unsigned)(head * sizeof(T)) : kNoRow;
   }
+  __device__ __forceinline__ unsigned offset_again(int i) const { return offset(min(i, n - 1)); }
 };
 
 // One tile buffer of LDS where two would not leave room for two workgroups.
@@ -524,7 +527,7 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
   auto fetch = [&](int k0) {
     const int n = it.k_end - k0;
     const KeyRows<T> kr((const T*)a.k, a.k_node, a.k_head, hk, k0, n);
-    ks.load(kr.base, a.dim, [&](int i) { return kr.offset(i); });
+    ks.load(kr.base, a.dim, [&](int i) { return kr.offset_again(i); });
     if (!LEAN) fetch_v(k0);
     if (BIASED && tid < kBlock)
 #pragma unroll
@@ -627,6 +630,12 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
   for (int i = 0; i < (kFix ? 9 : 4); ++i) m.v[i] += half_swap(m.v[i]);
   m.v[9] = delta;
   if (!row.ok) return;
+  if (lse == INFINITY) {                  // no key, or every score -inf: a key of infinities times a gradient of zero is none
+#pragma unroll
+    for (int i = 0; i < 9; ++i) m.v[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16 * S::kOut; ++i) acc[i / 16][i % 16] = 0.f;
+  }
   const float grad_scale = fit.undo(a.scale);
   if (it.slot < 0) {
     if (a.grad_q) store_cols<T, DP>((T*)a.grad_q + at * a.dim, acc, grad_scale, a.dim);
@@ -722,7 +731,7 @@ attn_bwd_k_kernel(AttnLaunch a, AttnScratch w) {
   };
   auto fetch = [&](int r0) {
     const QueryRows<T> qr((const T*)a.q, a.q_node, a.q_head, it.node, hk, group, r0, it.row_end - r0);
-    qs.load(qr.base, a.dim, [&](int i) { return qr.offset(i); });
+    qs.load(qr.base, a.dim, [&](int i) { return qr.offset_again(i); });
     if (!LEAN) fetch_g(r0);
     if (threadIdx.x < kBlock) {
       const Row o = row_of(it, r0 + threadIdx.x, hk, group);

@@ -361,7 +361,8 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, pos:
 
     ``cap``: scores are ``cap * tanh(score / cap)``.  ``slope`` fp32 ``(H_q,)`` and ``pos`` fp32 ``(N_q, 3)`` (``pos_k``
     ``(N_k, 3)`` where the keys are other nodes): ``slope_h`` times the distance is taken off the score.  The gradient of a
-    distance of zero is zero.  A query without keys gets zeros.
+    distance of zero is zero.  A query without keys, or whose scores are all -inf, gets zeros, and so do its gradients; where only
+    some are, because of infinities in those keys, its own gradient is a sum with 0 * inf in it.
 
     Statistics and sums are in 32 bits; in 16-bit types the probabilities and the scores' gradients are rounded to the type
     as operands of the next product.  Results do not depend on timing; differentiable to any order, beyond the first

@@ -823,3 +823,27 @@ LENGTHS["one long among many short"] = ([1] * 200, [5, 0, 33, 64] * 25 + [30011]
 def test_attention_of_one_long_structure_among_many(device, dtype, heads, kv_heads, dim, biased, cap):
     """Where the keys of one structure are cut and all others' are not."""
     test_attention(device, dtype, "one long among many short", heads, kv_heads, dim, biased, cap)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("keys", [1, 40, 700])
+@pytest.mark.parametrize("biased", [False, True])
+def test_attention_gradients_of_a_row_of_nothing(device, dtype, keys, biased):
+    """Every score of a structure -inf: its results and gradients are zeros, in one piece or several; another structure's are as without
+    it."""
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    gen = torch.Generator().manual_seed(101)
+    n = keys + 9
+    q, k, v, ct = (_rand(gen, n, 2, 16, dtype=dtype).abs().to(device) for _ in range(4))
+    pos, slope = _rand(gen, n, 3).to(device), torch.rand(2, generator=gen).to(device)
+    k[:keys] = -torch.inf
+
+    def run(rows, lengths):
+        t = [a[rows].clone().requires_grad_(True) for a in (q, k, v, pos)]
+        out = segment_attention(*t[:3], AttentionPlan(torch.tensor([0] + lengths, device=device).cumsum(0)),
+                                pos=t[3] if biased else None, slope=slope if biased else None)
+        return (out, *torch.autograd.grad(out, t if biased else t[:3], ct[rows]))
+    both, alone = run(slice(0, n), [keys, 9]), run(slice(keys, n), [9])
+    for a, b in zip(both, alone):
+        assert torch.equal(a[:keys], torch.zeros_like(a[:keys]))
+        assert float((a[keys:].float() - b.float()).abs().max()) <= 2 * EPS[dtype] * max(1.0, float(b.float().abs().max()))
