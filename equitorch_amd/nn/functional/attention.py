@@ -240,6 +240,9 @@ def _expression(q, k, v, pos_q, pos_k, slope, padded: _Buckets, scale: float, ca
     """The same result as a tensor expression on padded buckets of structures, which autograd differentiates to any order
     (in 32 bits)."""
     dtype, group = q.dtype, q.shape[1] // k.shape[1]
+    nothing = None
+    if k.shape[0] == 0 or not padded.len_q.any():          # some operands are not read: their gradients are zeros all the same
+        nothing = sum(t[:0].float().sum() for t in (q, k, v, pos_q, pos_k, slope) if t is not None)
     if k.shape[0] == 0:                     # no keys at all: something to point at; nothing of it is kept
         k, v = k.new_zeros((1, *k.shape[1:])), v.new_zeros((1, *v.shape[1:]))
         pos_k = None if pos_k is None else pos_k.new_zeros((1, 3))
@@ -263,9 +266,8 @@ def _expression(q, k, v, pos_q, pos_k, slope, padded: _Buckets, scale: float, ca
         total = p.sum(-1, keepdim=True)
         out = torch.matmul(p, vb) / torch.where(total > 0, total, torch.ones_like(total))
         outs.append(out.transpose(1, 2)[keep_q])
-    if not outs:
-        return q * 0.0
-    return torch.cat(outs)[order].to(dtype)
+    out = torch.cat(outs)[order].to(dtype) if outs else q * 0.0
+    return out if nothing is None else out + nothing
 
 
 def _args(q, k, v, pos_q, pos_k, slope, plan, scale, cap) -> AttnArgs:

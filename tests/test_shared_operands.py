@@ -231,3 +231,34 @@ def test_example_forces_in_the_loss(device):
             continue
         worst = float((a.detach().cpu().double() - b.detach()).abs().max())
         assert worst <= 2e-3 * max(1.0, float(b.abs().max())), f"{name}: {worst:.3e}"
+
+
+LENGTHS_OF_NOTHING = [([], []), ([0, 0], [0, 0]), ([0, 0], [3, 40]), ([2, 40], [0, 0])]
+
+
+@pytest.mark.parametrize("len_q,len_k", LENGTHS_OF_NOTHING)
+def test_expression_of_the_attention_of_nothing(len_q, len_k):
+    """No queries, or no keys: gradients of zeros, not none."""
+    from equitorch_amd.nn.functional import AttentionPlan
+    from equitorch_amd.nn.functional.attention import _of_buckets
+    ptr = lambda n: torch.tensor([0] + n).cumsum(0)
+    t = [torch.ones(sum(n), h, 4, requires_grad=True) for n, h in ((len_q, 2), (len_k, 1), (len_k, 1))]
+    t += [torch.ones(sum(n), 3, requires_grad=True) for n in (len_q, len_k)] + [torch.ones(2, requires_grad=True)]
+    got = higher_order(_of_buckets(AttentionPlan(ptr(len_q), ptr(len_k))._buckets, 1.0, 0.0), t, [True] * 6, torch.ones_like(t[0]))
+    for a, b in zip(got, t):
+        assert torch.equal(a, torch.zeros_like(b))
+
+
+@gpu
+@pytest.mark.parametrize("len_q,len_k", LENGTHS_OF_NOTHING)
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_attention_of_nothing(device, extension, len_q, len_k, create_graph):
+    from equitorch_amd.nn.functional import AttentionPlan, segment_attention
+    ptr = lambda n: torch.tensor([0] + n, device=device).cumsum(0)
+    t = [torch.ones(sum(n), h, 4, device=device, requires_grad=True) for n, h in ((len_q, 2), (len_k, 1), (len_k, 1))]
+    pos, pos_k = (torch.ones(sum(n), 3, device=device, requires_grad=True) for n in (len_q, len_k))
+    t += [pos, pos_k, torch.ones(2, device=device, requires_grad=True)]
+    out = segment_attention(*t[:3], AttentionPlan(ptr(len_q), ptr(len_k)), pos=pos, slope=t[5], pos_k=pos_k)
+    assert torch.equal(out, torch.zeros_like(t[0]))
+    for a, b in zip(torch.autograd.grad(out.sum(), t, create_graph=create_graph), t):
+        assert torch.equal(a, torch.zeros_like(b))
