@@ -257,7 +257,7 @@ def _expression(q, k, v, pos_q, pos_k, slope, padded: _Buckets, scale: float, ca
             s = cap * torch.tanh(s / cap)
         if slope is not None:
             diff = pos_q[rows_q].masked_fill(~keep_q[:, :, None], 0.0)[:, :, None] - pos_k[rows_k].masked_fill(~keep_k[:, :, None], 0.0)[:, None]
-            d2 = (diff * diff).sum(-1)
+            d2 = (diff * diff).sum(-1).clamp(max=3e38)       # where fp32 ends: -1e19 times the slope for its score, and no inf * 0
             s = s - slope[:, None, None] * torch.where(d2 > 0, torch.where(d2 > 0, d2, torch.ones_like(d2)).sqrt(),
                                                        torch.zeros_like(d2))[:, None]
         s = s.masked_fill(~keep_k[:, None, None], -torch.inf)
@@ -364,7 +364,7 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, pos:
     ``cap``: scores are ``cap * tanh(score / cap)``.  ``slope`` fp32 ``(H_q,)`` and ``pos`` fp32 ``(N_q, 3)`` (``pos_k``
     ``(N_k, 3)`` where the keys are other nodes): ``slope_h`` times the distance is taken off the score.  The gradient of a
     distance of zero is zero.  A query without keys, or whose scores are all -inf, gets zeros, and so do its gradients; where only
-    some are, because of infinities in those keys, its own gradient is a sum with 0 * inf in it.
+    some are, because of infinities in those keys, its own gradient is a sum with 0 * inf in it (in gradient mode in either case).
 
     Statistics and sums are in 32 bits; in 16-bit types the probabilities and the scores' gradients are rounded to the type
     as operands of the next product.  Results do not depend on timing; differentiable to any order, beyond the first

@@ -262,3 +262,26 @@ def test_attention_of_nothing(device, extension, len_q, len_k, create_graph):
     assert torch.equal(out, torch.zeros_like(t[0]))
     for a, b in zip(torch.autograd.grad(out.sum(), t, create_graph=create_graph), t):
         assert torch.equal(a, torch.zeros_like(b))
+
+
+def test_expression_of_the_attention_with_nodes_beyond_any_distance():
+    """A squared distance beyond fp32: that node takes no part, in the gradients either, of first and second order."""
+    from equitorch_amd.nn.functional import AttentionPlan
+    from equitorch_amd.nn.functional.attention import _of_buckets
+    gen = torch.Generator().manual_seed(11)
+    near = slice(0, 9)
+    data = [_rand(gen, 10, 2, 4, dtype=F32) for _ in range(3)] + [_rand(gen, 10, 3, dtype=F32), torch.rand(2, generator=gen) + 0.1]
+    data[3][9] = torch.tensor([1e20, 0.0, -2e20])
+    ct, cf = _rand(gen, 10, 2, 4, dtype=F32), _rand(gen, 10, 3, dtype=F32)
+    seen = []
+    for n in (10, 9):
+        t = [a[:n].clone().requires_grad_(True) for a in data[:4]] + [data[4].clone().requires_grad_(True)]
+        q, k, v, pos, slope = t
+        out = _as_operator(_of_buckets(AttentionPlan(torch.tensor([0, n]))._buckets, 0.5, 0.0), (q, k, v, pos, None, slope))
+        first = torch.autograd.grad(out[near], t, ct[near], create_graph=True)
+        second = torch.autograd.grad((first[3][near] * cf[near]).sum(), t)
+        seen.append([out, *first, *second])
+    for a, b in zip(*seen):                                # the nine others: sums of ten terms in another order
+        assert torch.isfinite(a).all()
+        a = a[near] if a.shape[0] == 10 else a
+        assert float((a - b).detach().abs().max()) <= 1e-5 * max(1.0, float(b.detach().abs().max()))
