@@ -38,22 +38,6 @@ struct AttnShape {
   __device__ static __forceinline__ int slot(int row, int c) { return (row * kChunks + mixed(row, c)) << 4; }
 };
 
-template <typename T>
-__device__ __forceinline__ f32x16_t mma_pair(const u32x4_t& a, const u32x4_t& b, f32x16_t acc) {
-  if constexpr (sizeof(T) == 4) {
-    const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[j], fb[j], acc, 0, 0, 0);
-  } else if constexpr (__is_same(T, f16_t)) {
-    typedef f16_t v8 __attribute__((ext_vector_type(8)));
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), acc, 0, 0, 0);
-  } else {
-    typedef bf16_t v8 __attribute__((ext_vector_type(8)));
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), acc, 0, 0, 0);
-  }
-  return acc;
-}
-
 template <typename T, int DP> using AttnAcc = f32x16_t[AttnShape<T, DP>::kOut];
 
 // A lane's part of one row as the B operand: chunk 2 s + lane / 32 at step s.  p null: zeros.

@@ -96,6 +96,23 @@ __device__ __forceinline__ void store_eight(T* p, const float (&src)[8], int64_t
   }
 }
 
+// acc + a b with 32 x 32 results: a pair of chunks of 16 bytes along k, one for each half of the wavefront.
+template <typename T>
+__device__ __forceinline__ f32x16_t mma_pair(const u32x4_t& a, const u32x4_t& b, f32x16_t acc) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[j], fb[j], acc, 0, 0, 0);
+  } else if constexpr (__is_same(T, f16_t)) {
+    typedef f16_t v8 __attribute__((ext_vector_type(8)));
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), acc, 0, 0, 0);
+  } else {
+    typedef bf16_t v8 __attribute__((ext_vector_type(8)));
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), acc, 0, 0, 0);
+  }
+  return acc;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int launch_status() { return hipGetLastError() == hipSuccess ? CGTP_OK : CGTP_ERR_LAUNCH; }
 

@@ -26,21 +26,6 @@ template <typename T> struct GemmType {
   static constexpr int kChunk = 16 / (int)sizeof(T), kDepth = 8 * kChunk;     // elements of a chunk; k of a tile
 };
 
-template <typename T>
-__device__ __forceinline__ void mma_chunk(f32x16_t& acc, const u32x4_t& a, const u32x4_t& b) {
-  if constexpr (sizeof(T) == 4) {
-    const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[j], fb[j], acc, 0, 0, 0);
-  } else if constexpr (__is_same(T, f16_t)) {
-    typedef f16_t v8 __attribute__((ext_vector_type(8)));
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), acc, 0, 0, 0);
-  } else {
-    typedef bf16_t v8 __attribute__((ext_vector_type(8)));
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), acc, 0, 0, 0);
-  }
-}
-
 // An operand's tile.  k contiguous: `base` at the tile's first row, `ld` elements between rows, `rows` of them left.  Rows
 // contiguous: base[i] at the first row of half i at k = 0, ld between k, rows[i] left.  The second half of a k-contiguous
 // operand is not used.
@@ -177,7 +162,7 @@ __device__ __forceinline__ void gemm_loop(GemmAcc<TILE>& acc, char* lds, int64_t
 #pragma unroll
       for (int i = 0; i < kB; ++i)
 #pragma unroll
-        for (int j = 0; j < kB; ++j) mma_chunk<T>(acc[i][j], fb[j], fa[i]);
+        for (int j = 0; j < kB; ++j) acc[i][j] = mma_pair<T>(fb[j], fa[i], acc[i][j]);
     }
   }
 }
