@@ -285,3 +285,34 @@ def test_expression_of_the_attention_with_nodes_beyond_any_distance():
         assert torch.isfinite(a).all()
         a = a[near] if a.shape[0] == 10 else a
         assert float((a - b).detach().abs().max()) <= 1e-5 * max(1.0, float(b.detach().abs().max()))
+
+
+@gpu
+@pytest.mark.parametrize("fused", [False, True])
+def test_layer_whose_weights_come_from_the_edge_vectors(device, extension, fused):
+    """A message-passing layer as models have it: radial functions of the edge vectors make the weights of a product that takes
+    the vectors too, twice over."""
+    from equitorch_amd import nn as enn
+    from equitorch_amd.nn.functional import EdgePlan, edge_tensor_product_uu_radial, edge_tensor_product_uu_vectors
+    irr, n, e, c = "0e+1o+2e", 30, 300, 64
+    torch.manual_seed(12)
+    gen = torch.Generator().manual_seed(12)
+    tp = enn.SO3Linear(irr, irr, irr, c, c, internal_weights=False, feature_mode="uu").to(device)
+    basis, cutoff = enn.BesselBasis(3.0, 8).to(device), enn.PolynomialCutoff(3.0)
+    hidden = torch.nn.Sequential(torch.nn.Linear(8, 16), torch.nn.SiLU()).to(device)
+    mix, gate_lin, gate, norm = (m.to(device) for m in (enn.IrrepsLinear(irr, irr, c, c), enn.IrrepsLinear(irr, "0e+0e+0e", c, c),
+                                                        enn.Gate(irr, activation=torch.nn.Sigmoid()), enn.LayerRMSNorm(irr, c)))
+    plan = EdgePlan(*(torch.randint(0, n, (e,), generator=gen).to(device) for _ in range(2)), n)
+    x, vec, last = (_rand(gen, *s, dtype=F32, std=0.5).to(device).requires_grad_(True) for s in ((n, 9, c), (e, 3), (16, tp.num_paths, c)))
+
+    def layer(x, vec, last):
+        r = vec.norm(dim=-1)
+        feat = hidden(basis(r) * cutoff(r)[:, None])
+        if fused:
+            msg = edge_tensor_product_uu_radial(x, vec, feat, last, plan, tp.tp_info_forward, edge_vectors=True)
+        else:
+            msg = edge_tensor_product_uu_vectors(x, vec, (feat @ last.reshape(16, -1)).view(e, -1, c), plan, tp.tp_info_forward)
+        h = mix(msg)
+        return norm(gate(h, gate_lin(h)))
+    # fp32 through two layers; gradients of a length near zero are large
+    _both_ways(lambda x, vec, last: layer(layer(x, vec, last) + x, vec, last), [x, vec, last], gen, 1e-3)
