@@ -197,13 +197,13 @@ __device__ __forceinline__ void join_waves(float* lds, int n, Give&& give, Take&
 
 // ---- forward ----------------------------------------------------------------------------------------------------
 // Vector instructions bound it with distances: some 25 issue slots for a score (a root and an exponential take four each), 79 %
-// of all slots used, the matrix cores 14 %.  300 structures of 40 to 250 nodes, 8 heads of 32, bf16, cap: 62 us; three of
-// 2000 to 5000, 8 query heads on 4 of 64: 321 us.  Without distances and cap the matrix cores and LDS do: one of 12007, 16 query
-// heads on 4 of 128, fp16: 1.35 ms, 877 TFLOP/s, 0.78 of what a large library product reaches.
+// of all slots used, the matrix cores 14 %.  300 structures of 40 to 250 nodes, 8 heads of 32, bf16, cap: 59 us; three of
+// 2000 to 5000, 8 query heads on 4 of 64: 311 us.  Without distances and cap the matrix cores and LDS do: one of 12007, 16 query
+// heads on 4 of 128, fp16: 1.35 to 1.43 ms, 830 to 877 TFLOP/s, 0.75 of what a large library product reaches.
 //
 // NW wavefronts of 32 rows share the tiles of keys (wide_q 1), or KS share out the keys of one tile of rows and join their
 // results in LDS (wide_q 2: 64 readouts of one query over up to 400 keys, fp32, 30 us with one wavefront each, 15 so; one query
-// of 8 heads on 2 of 64 over 200003 keys, bf16: 25 us, 4.1 TB/s of keys and values).
+// of 8 heads on 2 of 64 over 200003 keys, bf16: 24 us, 4.3 TB/s of keys and values).
 // Four wavefronts on a SIMD where a row is short and they wait for each other (20 structures of 1000 nodes, 4 heads of 32, bf16:
 // 59 us with three, 50 so).
 template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
@@ -462,7 +462,7 @@ struct QSums {
 
 // ---- gradient with the rows fixed ---------------------------------------------------------------------------------
 // Bound by vector instructions as the forward is (84 % of the slots): the score again, and the sums for positions and slopes.
-// The two workloads above: 108 and 527 us.
+// The two workloads above: 109 and 511 us.
 template <typename T, int DP, int NW, int KS, bool BIASED, bool CAPPED>
 __global__ void __launch_bounds__(64 * NW * KS, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
 attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
@@ -512,7 +512,8 @@ attn_bwd_q_kernel(AttnLaunch a, AttnScratch w) {
     for (int e = 0; e < 16; ++e) acc[o][e] = 0.f;
   // Sums over the keys of ds (r_i - r_j) / |r_i - r_j| and of ds |r_i - r_j|; in 16-bit types also of ds, and of the others with
   // p for ds (kFix).  delta is against an output that was summed from rounded probabilities and rounded itself: the
-  // exact one is delta + sum ds, and with it the gradients of positions and slopes, which are fp32, err as in fp32.
+  // exact one is delta + sum ds, and with it the gradients of positions and slopes, which are fp32, err as in fp32.  It is known
+  // when the row is done: the row's own dq, rounded to 16 bits anyway, goes without.
   constexpr bool kFix = sizeof(T) == 2;
   QSums m = {};
   ColumnFit<T, DP> fit;
@@ -690,7 +691,7 @@ __global__ void __launch_bounds__(256) attn_bwd_q_join_kernel(AttnLaunch a, Attn
 
 // ---- gradient with the keys fixed ---------------------------------------------------------------------------------
 // Bound by vector instructions; four sums of 32 x dim for a wavefront leave room for two of them on a SIMD up to dim 64.  The
-// two workloads above: 98 and 567 us.  Taking two heads at a time, whose distances are the same, was within 5 % of
+// two workloads above: 111 and 549 us.  Taking two heads at a time, whose distances are the same, was within 5 % of
 // this for short rows and slower for others (their sums spilled).
 template <typename T, int DP, int NW, bool BIASED, bool CAPPED>
 __global__ void __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1)

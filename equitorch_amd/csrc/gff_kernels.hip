@@ -7,7 +7,8 @@
 // x (rows, C_in), Wg, Wu (C_in, H), Wd (H, C_out).  Every product is formed in fp32; m, g, u, dg and du are rounded to the
 // operands' type where they are stored, as operands of the next product: the same rounding the inputs have.
 //
-// 65536 rows of 256 -> 1024 -> 256 channels, bf16, forward and backward: 565 us.  No pipe is full: the products use a third of the
+// 65536 rows of 256 -> 1024 -> 256 channels, bf16, forward and backward: 566 us (the kernels' own figures below are from a trace, one
+// after the other, and come to 657).  No pipe is full: the products use a third of the
 // matrix cores' cycles at most, LDS a third; with three workgroups on a compute unit a product's short run over k (four tiles
 // of 256 channels) and its results alternate.  Two products at a time in one kernel, with 128 rows' operands and results in
 // registers, were measured too: 504 us here, but 391 against 362 at 40000 rows, where the last of its few large
@@ -87,7 +88,7 @@ __device__ __forceinline__ void store_kept(T* to, const float (&v)[8], int left)
   }
 }
 
-// 65536 rows as above: 155 us, 2.6 TB/s written.
+// 65536 rows as above: 162 us, 2.5 TB/s written.
 // g, u and m.  A tile is TILE rows x TILE / 2 hidden channels, of Wg and of Wu.
 template <typename T, int TILE, bool FAST, int ACT>
 __global__ void __launch_bounds__(kGemmThreads, TILE == 128 ? 3 : 4) gff_up_kernel(UpArgs<T> a) {
@@ -128,7 +129,7 @@ struct MidGradArgs {
   int H, C, ldg, ldw, ldh;
 };
 
-// dg and du from dm = dy Wd^T.  136 us, 4.1 TB/s: bound by memory, the projections read and their gradients written.
+// dg and du from dm = dy Wd^T.  139 us, 4.0 TB/s: bound by memory, the projections read and their gradients written.
 template <typename T, int TILE, bool FAST, int ACT>
 __global__ void __launch_bounds__(kGemmThreads, TILE == 128 ? 3 : 4) gff_mid_grad_kernel(MidGradArgs<T> a) {
   __shared__ alignas(16) char lds[kGemmLds<TILE>];
@@ -179,7 +180,7 @@ enum { kWhole, kPacked, kLoose };
 
 // out = sum over segments of A_s B_s: y = m Wd (one segment), dx = dg Wg^T + du Wu^T (two).  A is contiguous along k.  The
 // tiles of k are cut into `splits` ranges where the result has few tiles; a range's result is left in fp32 and the ranges
-// are added in order by gff_add_kernel.  y 61 us, dx 112 us (560 and 610 TFLOP/s).
+// are added in order by gff_add_kernel.  y 63 us, dx 116 us (545 and 590 TFLOP/s).
 template <typename T>
 struct RowsArgs {
   const T *a[2], *b[2];
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kGemmThreads, TILE == 128 ? 3 : 4) gff_rows_ke
 }
 
 // Weight gradients out_j = A_j^T B_j over all rows: both operands contiguous along the tile's rows.  The rows are cut
-// into `splits` ranges, as above.  157 us, 660 TFLOP/s, where the library's product takes 272.
+// into `splits` ranges, as above.  167 us, 620 TFLOP/s, where the library's product takes 272.
 template <typename T>
 struct WeightJob {
   const T *a, *b;
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(256) gff_pack_kernel(PackArgs<T> a) {
 // A handful of rows: the weights are read once for all of them and nothing else counts.  A workgroup takes 32 columns, a
 // thread eight of them at every 64th k, in fp32; the 64 sums of a column are added in LDS in a fixed order.
 // MATS = 2: x against Wg and Wu, then the activation and the product; MATS = 1: m against Wd.  Bound by latency: one row of
-// 256 -> 1024 -> 256 channels, bf16, 4.6 and 7.8 us.
+// 256 -> 1024 -> 256 channels, bf16, 4.4 and 7.7 us.
 constexpr int kFewRows = 4, kFewCols = 32, kFewSlices = 64;
 template <typename T>
 struct FewArgs {

@@ -153,7 +153,7 @@ class AttentionPlan:
     ``s``, and ``ptr_k`` the same for the keys where queries and keys are different nodes (a readout: one query for each
     structure).  Structures may be empty, on either side.  Built once for a batch (it reads ``ptr`` on the host), used by
     every layer; the kernels' tables are made on first use for each number of heads and kept with it (a graph is captured after
-    that).  A plan may be used on any stream."""
+    that, and reads them for as long as it is replayed).  A plan may be used, and dropped, on any stream."""
 
     def __init__(self, ptr: Tensor, ptr_k: Optional[Tensor] = None):
         self.device = ptr.device
@@ -367,7 +367,7 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, pos:
     some are, because of infinities in those keys, its own gradient is a sum with 0 * inf in it (in gradient mode in either case).
 
     Statistics and sums are in 32 bits; in 16-bit types the probabilities and the scores' gradients are rounded to the type
-    as operands of the next product.  Results do not depend on timing; differentiable to any order, beyond the first
+    as operands of the next product (in fp16 scaled into its range first).  Results do not depend on timing; differentiable to any order, beyond the first
     through a tensor expression that holds the scores of every structure in memory."""
     q, k, v = _lib.of_one_type(q, k, v)
     _check(q, k, v, plan, pos, slope, pos_k)

@@ -32,7 +32,8 @@ class EdgePlan:
     (``ptr_dst[v] .. ptr_dst[v+1]`` are the sorted positions whose edges end at ``v``) — bit for bit the
     ``index`` and ``seg_out`` of ``sparse_scale_info(index=range(E), index_out=dst, out_size=num_nodes)``
     (``equitorch/utils/_structs.py:22-71``; a tuple sort on ``(dst, e)`` is a stable sort on ``dst``).
-    ``perm_src`` / ``ptr_src`` are the same for ``src``.  All tensors are int64 on ``src.device``.
+    ``perm_src`` / ``ptr_src`` are the same for ``src``.  All tensors are int64 on ``src.device``.  Used on another stream than
+    the one it was made on, a plan is kept until the work there is done.
     """
 
     def __init__(self, src: Tensor, dst: Tensor, num_nodes: int, num_src_nodes: Optional[int] = None):
