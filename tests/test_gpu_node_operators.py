@@ -847,3 +847,22 @@ def test_attention_gradients_of_a_row_of_nothing(device, dtype, keys, biased):
     for a, b in zip(both, alone):
         assert torch.equal(a[:keys], torch.zeros_like(a[:keys]))
         assert float((a[keys:].float() - b.float()).abs().max()) <= 2 * EPS[dtype] * max(1.0, float(b.float().abs().max()))
+
+
+@pytest.mark.parametrize("use_extension", [True, False])
+@pytest.mark.parametrize("operator", ["embedding", "attention", "feed_forward"])
+def test_batched_gradients_are_refused(device, monkeypatch, use_extension, operator):
+    """A gradient that a transform has batched has no memory of its own to read: an error, no launch."""
+    from equitorch_amd import _shim
+    from equitorch_amd.nn.functional import AttentionPlan, embedding, gated_feed_forward, segment_attention
+    if not use_extension:
+        monkeypatch.setattr(_shim, "_module", None)
+    gen = torch.Generator().manual_seed(111)
+    plan, kind = AttentionPlan(torch.tensor([0, 9], device=device)), torch.arange(9, device=device)
+    x, w = _rand(gen, 9, 8).to(device).requires_grad_(True), _rand(gen, 8, 8).to(device)
+    out = {"embedding": lambda: embedding(kind, x), "feed_forward": lambda: gated_feed_forward(x, w, w, w),
+           "attention": lambda: segment_attention(*[x.view(9, 2, 4)] * 3, plan).reshape(9, 8)}[operator]()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, x, torch.ones(3, 9, 8, device=device), is_grads_batched=True)
+    (g,) = torch.autograd.grad(out, x, torch.ones(9, 8, device=device))
+    assert torch.isfinite(g).all()
