@@ -101,10 +101,12 @@ int64_t forward_bytes(const cgtp_attn_args& a) { return (q_parts(a) * (a.dim + 2
 int attn_check(const cgtp_attn_args* a) {
   if (!a) return CGTP_ERR_NULL;
   if (a->dtype != CGTP_F32 && a->dtype != CGTP_BF16 && a->dtype != CGTP_F16) return CGTP_ERR_DTYPE;
-  if (a->n_q < 0 || a->n_k < 0 || a->n_q > 0x7fffffff || a->n_k > 0x7fffffff) return CGTP_ERR_SHAPE;
+  // keys and rows are counted in 32 bits, up to four tiles of 64 beyond the last one
+  constexpr int64_t kMost = 0x7fffffff - 1024;
+  if (a->n_q < 0 || a->n_k < 0 || a->n_q > kMost || a->n_k > kMost) return CGTP_ERR_SHAPE;
   if (a->dim <= 0 || a->dim > 128 || a->h_kv <= 0 || a->h_q <= 0 || a->h_q % a->h_kv || a->h_q > 0x3fff) return CGTP_ERR_SHAPE;
-  // rows are counted in 32 bits, and a grid has fewer than 2^32 threads
-  if (a->n_q * (a->h_q / a->h_kv) > 0x7fffffff) return CGTP_ERR_SHAPE;
+  if (a->n_q * (a->h_q / a->h_kv) > kMost) return CGTP_ERR_SHAPE;
+  // a grid has fewer than 2^32 threads
   if (a->n_q_items < 0 || a->n_q_joins < 0 || a->n_q_slots < 0 || a->n_k_items < 0 || a->n_k_joins < 0 || a->n_k_slots < 0)
     return CGTP_ERR_SHAPE;
   const int64_t heads = a->h_kv, group = a->h_q / a->h_kv;

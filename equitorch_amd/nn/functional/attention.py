@@ -18,6 +18,7 @@ from ..._lib import AttnArgs, CgtpError
 from ._higher_order import higher_order
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_MOST = 2 ** 31 - 1024          # the kernels count keys and rows in 32 bits, up to four tiles beyond the last one
 _BLOCK = 64                     # keys (rows) of a tile: pieces of a structure begin at multiples of it
 _PIECE = 256                    # keys (rows) of a piece at least
 _LEAST = 64                     # the same where tiles are few
@@ -30,8 +31,8 @@ def _lengths(ptr: Tensor, name: str) -> np.ndarray:
         raise CgtpError(f"{name} must be a 1-d int64 tensor of S + 1 offsets, got {ptr.dtype} {tuple(ptr.shape)}")
     p = ptr.detach().cpu().numpy()
     lengths = np.diff(p)
-    if p[0] != 0 or (lengths < 0).any() or p[-1] >= 2 ** 31:
-        raise CgtpError(f"{name} must start at 0, never descend and stay below 2^31")
+    if p[0] != 0 or (lengths < 0).any() or p[-1] >= _MOST:
+        raise CgtpError(f"{name} must start at 0, never descend and stay below 2^31 - 1024")
     return lengths
 
 
@@ -81,8 +82,8 @@ def _table(columns, order, device) -> Optional[Tensor]:
 class _Tables:
     def __init__(self, plan: "AttentionPlan", group: int, heads: int):
         cols, rows = plan.len_k, plan.len_q * group
-        if rows.sum() >= 2 ** 31:
-            raise CgtpError("queries times query heads of a head of keys must stay below 2^31")
+        if rows.sum() >= _MOST:
+            raise CgtpError("queries times query heads of a head of keys must stay below 2^31 - 1024")
         start_q, start_k = np.cumsum(plan.len_q) - plan.len_q, np.cumsum(cols) - cols
         # Tiles of 128 rows share a tile of keys among four wavefronts; tiles of 32 rows waste less of a short structure.  Few
         # rows against many keys (a readout), or so few tiles that the GPU is idle otherwise: four wavefronts share out the

@@ -806,7 +806,7 @@ int cgtp_gff_backward(const cgtp_gff_args* args, void* stream);
  * q: (n_q, h_q, dim), k and v: (n_k, h_kv, dim), h_q a multiple of h_kv (query head h reads head h / (h_q / h_kv)), with
  * element strides *_node and *_head and contiguous along dim; out, grad_out and the gradients contiguous; lse (n_q, h_q)
  * fp32; pos_q (n_q, 3), pos_k (n_k, 3), slope (h_q) fp32.  lse NULL: not wanted.  Elements may lie anywhere an element may.  dim <= 128,
- * h_q < 2^14; n_k, n_q and n_q * (h_q / h_kv) < 2^31; items times h_kv < 2^24 either way, and joins times h_kv times the
+ * h_q < 2^14; n_k, n_q and n_q * (h_q / h_kv) < 2^31 - 1024; items times h_kv < 2^24 either way, and joins times h_kv times the
  * rows of a tile < 2^22 (workgroups of one launch), else CGTP_ERR_SHAPE.
  *
  * The caller cuts the work into items.  The rows of a structure and a head of keys are its (query, query head) pairs, row =

@@ -242,3 +242,21 @@ def test_attention_tables_of_one_long_structure_among_many(len_q, len_k, group, 
     t = (AttentionPlan(ptr(len_q)) if len_k is None else AttentionPlan(ptr(len_q), ptr(len_k))).tables(group, heads)
     items = t.q_items
     assert int((items[:, 4] - items[:, 3]).max()) <= longest
+
+
+@pytest.mark.parametrize("most", [2 ** 31 - 1024])
+def test_attention_counts_stay_within_32_bits(most):
+    """Kernels step through keys and rows by up to 256 at a time in 32 bits: the last ones that would step past the end are refused."""
+    from equitorch_amd.nn.functional import AttentionPlan
+    lib, steps = _lib.lib, 256
+    assert most - 1 + 4 * steps < 2 ** 31
+    # one more than the largest count is refused, the largest itself only misses a buffer (nothing is launched)
+    for name in ("n_k", "n_q"):
+        assert lib.cgtp_attn_forward(C.byref(_attn(**{name: most, "h_q": 1, "q_items": None})), None) == SHAPE
+        assert lib.cgtp_attn_forward(C.byref(_attn(**{name: most - 1, "h_q": 1, "q_items": None})), None) == NULL
+    assert lib.cgtp_attn_forward(C.byref(_attn(n_q=most // 2, h_q=2, q_items=None)), None) == SHAPE
+    for bad in (most, 2 ** 31 - 1):
+        with pytest.raises(CgtpError):
+            AttentionPlan(torch.tensor([0, bad]))
+    with pytest.raises(CgtpError):
+        AttentionPlan(torch.tensor([0, most // 2]), torch.tensor([0, 4])).tables(2, 1)
