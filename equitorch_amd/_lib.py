@@ -169,6 +169,14 @@ class AttnArgs(C.Structure):
                 ("reserved_", C.c_int32), ("scale", C.c_float), ("cap", C.c_float)]
 
 
+class AddRmsArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("out", C.c_void_p), ("total", C.c_void_p),
+                ("rstd", C.c_void_p), ("scale", C.c_void_p), ("grad_out", C.c_void_p), ("grad_total", C.c_void_p),
+                ("grad_x", C.c_void_p), ("grad_residual", C.c_void_p), ("grad_weight", C.c_void_p), ("workspace", C.c_void_p),
+                ("n_rows", C.c_int64), ("eps", C.c_double), ("channels", C.c_int32), ("dtype", C.c_int32),
+                ("residual_dtype", C.c_int32), ("weight_dtype", C.c_int32)]
+
+
 def _load():
     if not os.path.exists(_LIB_PATH):
         raise ImportError(
@@ -300,6 +308,9 @@ def _load():
         ws.restype, ws.argtypes = C.c_int64, [args, C.c_int]
         getattr(lib, name + "_forward").argtypes = [args, C.c_void_p]
         getattr(lib, name + "_backward").argtypes = [args, C.c_void_p]
+    lib.cgtp_add_rms_workspace_bytes.restype = C.c_int64
+    lib.cgtp_add_rms_workspace_bytes.argtypes = [C.POINTER(AddRmsArgs)]
+    lib.cgtp_add_rms_forward.argtypes = lib.cgtp_add_rms_backward.argtypes = [C.POINTER(AddRmsArgs), C.c_void_p]
     lib.cgtp_abi_layout.argtypes = [C.c_int, C.POINTER(C.c_int64), C.c_int]
     return lib
 

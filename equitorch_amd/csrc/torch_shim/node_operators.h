@@ -1,5 +1,5 @@
 // Autograd nodes of the operators on invariant node features over the C ABI: embedding of node kinds, attention among the nodes of
-// a structure, gated feed-forward block.  Operands are checked by the Python layer, which also holds the same launches
+// a structure, gated feed-forward block, norm after a residual's addition.  Operands are checked by the Python layer, which also holds the same launches
 // through ctypes for when this extension is not there; a backward under gradient mode hands over to a Python callable.
 #pragma once
 
@@ -316,7 +316,109 @@ struct Attn : torch::autograd::Function<Attn> {
   }
 };
 
+// ---- root-mean-square norm after a residual's addition ------------------------------------------------------------------
+cgtp_add_rms_args add_rms_args(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& total, double eps) {
+  cgtp_add_rms_args a{};
+  a.weight = ptr_or_null(weight);
+  a.total = mutable_ptr(total);
+  a.n_rows = x.size(0);
+  a.channels = (int32_t)x.size(1);
+  a.eps = eps;
+  a.dtype = code_of(x);
+  a.residual_dtype = code_of(total);
+  a.weight_dtype = weight.defined() ? code_of(weight) : a.dtype;
+  return a;
+}
+
+struct AddRmsOut {
+  at::Tensor out, total, rstd, scale;      // total: x itself without a residual
+};
+AddRmsOut add_rms_forward(const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight, double eps, bool keep, bool eight) {
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  AddRmsOut r;
+  r.total = residual.defined() ? at::empty(residual.sizes(), residual.options()) : x;
+  r.out = at::empty(x.sizes(), eight ? x.options().dtype(at::kFloat8_e4m3fn) : x.options());
+  const auto wide = x.options().dtype(at::kFloat);
+  if (keep) r.rstd = at::empty({x.size(0)}, wide);
+  if (eight) r.scale = at::empty({x.size(0)}, wide);
+  cgtp_add_rms_args a = add_rms_args(x, weight, r.total, eps);
+  a.x = x.data_ptr();
+  a.residual = ptr_or_null(residual);
+  a.out = r.out.data_ptr();
+  a.rstd = (float*)mutable_ptr(r.rstd);
+  a.scale = (float*)mutable_ptr(r.scale);
+  check_status(cgtp_add_rms_forward(&a, current_stream(x)), "cgtp_add_rms_forward");
+  return r;
+}
+
+struct AddRms : torch::autograd::Function<AddRms> {
+  typedef c10::optional<at::Tensor> Optional;
+  // out and, with a residual, total
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const Optional& residual, const Optional& weight, double eps,
+                               int64_t fallback) {
+    AddRmsOut r = add_rms_forward(x, opt(residual), opt(weight), eps, true, false);
+    ctx->save_for_backward({x, opt(residual), opt(weight), r.total, r.rstd});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["fallback"] = fallback;
+    ctx->set_materialize_grads(false);
+    if (residual.has_value()) return {r.out, r.total};
+    return {r.out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    const variable_list s = ctx->get_saved_variables();
+    const at::Tensor &x = s[0], &residual = s[1], &weight = s[2], &total = s[3];
+    const at::Tensor g_total = grad.size() > 1 ? grad[1] : at::Tensor();
+    std::vector<bool> need;
+    size_t edge = 0;                    // the node has an edge for each operand that is there
+    for (size_t i = 0; i < 3; ++i) need.push_back(s[i].defined() && ctx->needs_input_grad(edge++));
+    variable_list out(5);
+    if (!grad[0].defined() && !g_total.defined()) return out;
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    const at::Tensor g_out = grad[0].defined() ? grad[0] : at::zeros(x.sizes(), x.options());
+    if (at::GradMode::is_enabled())
+      return call_fallback(ctx->saved_data["fallback"].toInt(), g_out, {x, residual, weight}, need, 5,
+                           g_total.defined() ? Optional(g_total) : Optional());
+    const at::Tensor g = g_out.contiguous(), gt = g_total.defined() ? g_total.contiguous() : g_total;
+    cgtp_add_rms_args a = add_rms_args(x, weight, total, ctx->saved_data["eps"].toDouble());
+    a.rstd = (float*)s[4].data_ptr();
+    a.grad_out = g.data_ptr();
+    a.grad_total = ptr_or_null(gt);
+    // of one type: one tensor is the gradient of both
+    const bool same = residual.defined() && residual.scalar_type() == x.scalar_type();
+    at::Tensor gx, gr;
+    if (need[0] || (same && need[1])) gx = at::empty(x.sizes(), x.options());
+    if (same) gr = gx;
+    else if (need[1]) gr = at::empty(residual.sizes(), residual.options());
+    if (need[0]) out[0] = gx;
+    if (need[1]) out[1] = gr;
+    if (need[2]) out[2] = at::empty(weight.sizes(), weight.options());
+    a.grad_x = mutable_ptr(gx);
+    a.grad_residual = same ? nullptr : mutable_ptr(gr);
+    a.grad_weight = mutable_ptr(out[2]);
+    at::Tensor ws;
+    if (const int64_t n = cgtp_add_rms_workspace_bytes(&a)) {
+      ws = bytes_on(x, n);
+      a.workspace = ws.data_ptr();
+    }
+    check_status(cgtp_add_rms_backward(&a, current_stream(x)), "cgtp_add_rms_backward");
+    return out;
+  }
+};
+
 void bind_node_operators(py::module& m) {
+  typedef c10::optional<at::Tensor> Optional;
+  m.def("add_rms", [](const at::Tensor& x, const Optional& residual, const Optional& weight, double eps, bool keep, const Fallback& fallback) {
+    if (keep) {
+      variable_list r = AddRms::apply(x, residual, weight, eps, fallback.id);
+      return std::make_pair(r[0], r.size() > 1 ? r[1] : x);
+    }
+    AddRmsOut r = add_rms_forward(x, opt(residual), opt(weight), eps, false, false);
+    return std::make_pair(r.out, r.total);
+  }, "norm after a residual's addition: (out, total); with its autograd node where a backward may follow (keep)");
+  m.def("add_rms_8bit", [](const at::Tensor& x, const Optional& residual, const Optional& weight, double eps) {
+    AddRmsOut r = add_rms_forward(x, opt(residual), opt(weight), eps, false, true);
+    return std::make_tuple(r.out, r.scale, r.total);
+  }, "the same in 8 bits: (values, scale, total)");
   m.def("embed", [](const at::Tensor& kind, const at::Tensor& table, double scale) { return Embed::apply(kind, table, scale); },
         "embedding of node kinds with its autograd node");
   py::class_<Fallback>(m, "Fallback").def(py::init([](py::object fn) {

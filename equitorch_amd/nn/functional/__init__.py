@@ -1,5 +1,6 @@
 """Functional layer (``equitorch.nn.functional``) of the sparse tensor-product path."""
 from .activations import gating
+from .add_rms_norm import add_rms_norm, add_rms_norm_8bit
 from .angular import sincos
 from .attention import AttentionPlan, segment_attention
 from .cutoffs import cosine_cutoff, mollifier_cutoff, polynomial_cutoff, radial_standarize
@@ -29,5 +30,5 @@ __all__ = [
     "batch_mean_squared_norm", "batch_rms_norm", "layer_rms_norm", "radial_standarize", "polynomial_cutoff",
     "cosine_cutoff", "mollifier_cutoff", "sincos", "xyz_to_sincos", "sparse_wigner_rotation",
     "dense_wigner_rotation", "wigner_d_matrix", "align_to_z_wigner_d", "irrep_wise_dropout", "angles_to_matrix", "so2_linear_uu", "so2_linear_uv", "tensor_dot_uu", "tensor_dot_uv",
-    "embedding", "AttentionPlan", "segment_attention", "gated_feed_forward",
+    "embedding", "AttentionPlan", "segment_attention", "gated_feed_forward", "add_rms_norm", "add_rms_norm_8bit",
 ]

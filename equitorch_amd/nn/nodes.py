@@ -1,10 +1,11 @@
 """Layers on the invariant channels of nodes: ``Embedding`` of their kinds, ``SegmentAttention`` among the nodes of a
-structure and the ``GatedFeedForward`` block."""
-from typing import Optional
+structure, the ``GatedFeedForward`` block and the ``AddRMSNorm`` between blocks."""
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor, nn
 
+from .functional.add_rms_norm import add_rms_norm
 from .functional.attention import AttentionPlan, segment_attention
 from .functional.embedding import embedding
 from .functional.feed_forward import _ACTIVATIONS, gated_feed_forward
@@ -112,3 +113,32 @@ class GatedFeedForward(nn.Module):
     def extra_repr(self) -> str:
         return (f"channels={self.channels}, hidden={self.hidden}, channels_out={self.channels_out}, "
                 f"activation='{self.activation}'")
+
+
+class AddRMSNorm(nn.Module):
+    """``(x, residual) -> (out, total)``: ``total = x + residual`` (``x`` without one) and its root-mean-square norm over the
+    last axis times a learnable ``(channels,)`` weight (``affine``).  ``total``, in the residual's type, is the next block's residual."""
+
+    def __init__(self, channels: int, eps: float = 1e-5, affine: bool = True):
+        super().__init__()
+        if channels < 1:
+            raise ValueError(f"channels must be positive, got {channels}")
+        if not 0.0 <= eps < float("inf"):
+            raise ValueError(f"eps must be finite and not negative, got {eps}")
+        self.channels, self.eps, self.affine = channels, eps, affine
+        if affine:
+            self.weight = nn.Parameter(torch.ones(channels))
+        else:
+            self.register_parameter("weight", None)
+
+    def reset_parameters(self) -> None:
+        if self.weight is not None:
+            nn.init.ones_(self.weight)
+
+    def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+        if x.shape[-1:] != (self.channels,):
+            raise ValueError(f"Input tensor's channel dimension does not match expected channels ({self.channels}): {tuple(x.shape)}")
+        return add_rms_norm(x, residual, self.weight, self.eps)
+
+    def extra_repr(self) -> str:
+        return f"channels={self.channels}, eps={self.eps}, affine={self.affine}"

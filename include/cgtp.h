@@ -43,7 +43,7 @@ int cgtp_version(void);
 enum { CGTP_LAYOUT_OPERAND = 0, CGTP_LAYOUT_TRI_ARGS = 1, CGTP_LAYOUT_GEN_OPERAND = 2, CGTP_LAYOUT_GEN_ARGS = 3,
        CGTP_LAYOUT_UVU_ARGS = 4, CGTP_LAYOUT_UVT_ITEM = 5, CGTP_LAYOUT_UVT_ARGS = 6, CGTP_LAYOUT_UVT_GW_ARGS = 7,
        CGTP_LAYOUT_UVT_GY_ARGS = 8, CGTP_LAYOUT_UVU_TABLE = 9, CGTP_LAYOUT_PSW_TABLE = 10, CGTP_LAYOUT_PSW_ARGS = 11,
-       CGTP_LAYOUT_GFF_ARGS = 17, CGTP_LAYOUT_ATTN_ARGS = 18, CGTP_LAYOUT_ATTN_ITEM = 19 };   /* 16: none */
+       CGTP_LAYOUT_GFF_ARGS = 17, CGTP_LAYOUT_ATTN_ARGS = 18, CGTP_LAYOUT_ATTN_ITEM = 19, CGTP_LAYOUT_ADD_RMS_ARGS = 20 };   /* 16: none */
 int cgtp_abi_layout(int which, int64_t* out, int capacity);
 
 /* ---- generic sparse trilinear contraction -------------------------------------------------------------
@@ -846,6 +846,32 @@ int cgtp_attn_rows(int wide);
 int64_t cgtp_attn_workspace_bytes(const cgtp_attn_args* args, int backward);
 int cgtp_attn_forward(const cgtp_attn_args* args, void* stream);
 int cgtp_attn_backward(const cgtp_attn_args* args, void* stream);
+
+/* ---- root-mean-square norm after a residual's addition ------------------------------------------------------------
+ *   t = x + residual, rounded to residual_dtype (residual NULL: t = x),  r = 1 / sqrt(mean_c t^2 + eps),  out = t r weight
+ * x, out: (n_rows, channels) of dtype; residual, total (receives t; NULL: not wanted, and not written without a residual): the same of
+ * residual_dtype; weight (channels) of weight_dtype, NULL: ones; rstd (n_rows) receives r, NULL: not wanted; all contiguous,
+ * aligned to an element.  scale not NULL: 8 bits; scale (n_rows) receives s = max_c |out| / 448 (0 for a row of zeros, at least 2^-126
+ * else, NaN for a row with an infinity or a NaN) and out, one byte an element, out / s in e4m3, to nearest.
+ * cgtp_add_rms_backward reads weight, total (t; x where there is no residual), rstd, grad_out and grad_total (the gradient of t
+ * apart from out's, NULL: none) and writes those of grad_x, grad_residual (the same values in residual_dtype) and grad_weight
+ * (weight_dtype) that are not NULL.  The sums over rows have an order that the sizes alone determine.
+ * workspace: cgtp_add_rms_workspace_bytes (backward; 0: may be NULL).  channels < 2^15, n_rows < 2^31.
+ * dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16; residual_dtype and weight_dtype: dtype or CGTP_F32.
+ */
+typedef struct {
+  const void *x, *residual, *weight;
+  void *out, *total;
+  float *rstd, *scale;
+  const void *grad_out, *grad_total;
+  void *grad_x, *grad_residual, *grad_weight, *workspace;
+  int64_t n_rows;
+  double eps;
+  int32_t channels, dtype, residual_dtype, weight_dtype;
+} cgtp_add_rms_args;
+int64_t cgtp_add_rms_workspace_bytes(const cgtp_add_rms_args* args);
+int cgtp_add_rms_forward(const cgtp_add_rms_args* args, void* stream);
+int cgtp_add_rms_backward(const cgtp_add_rms_args* args, void* stream);
 
 #ifdef __cplusplus
 }
