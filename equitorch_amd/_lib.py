@@ -177,6 +177,13 @@ class AddRmsArgs(C.Structure):
                 ("residual_dtype", C.c_int32), ("weight_dtype", C.c_int32)]
 
 
+class KindLossArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("table", C.c_void_p), ("kind", C.c_void_p), ("loss", C.c_void_p), ("lse", C.c_void_p),
+                ("grad_loss", C.c_void_p), ("grad_x", C.c_void_p), ("grad_table", C.c_void_p), ("workspace", C.c_void_p),
+                ("n_rows", C.c_int64), ("n_kinds", C.c_int64), ("channels", C.c_int32), ("dtype", C.c_int32),
+                ("scale", C.c_float), ("cap", C.c_float)]
+
+
 def _load():
     if not os.path.exists(_LIB_PATH):
         raise ImportError(
@@ -302,8 +309,8 @@ def _load():
     lib.cgtp_embed_workspace_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int, C.c_int]
     lib.cgtp_embed_forward.argtypes = [C.c_void_p] * 3 + [C.c_int64, C.c_int64, C.c_int, C.c_double, C.c_int, C.c_void_p]
     lib.cgtp_embed_backward.argtypes = [C.c_void_p] * 4 + [C.c_int64, C.c_int64, C.c_int, C.c_double, C.c_int, C.c_void_p]
-    for name in ("cgtp_gff", "cgtp_attn"):
-        args = C.POINTER(GffArgs if name == "cgtp_gff" else AttnArgs)
+    for name, args in (("cgtp_gff", GffArgs), ("cgtp_attn", AttnArgs), ("cgtp_kind_loss", KindLossArgs)):
+        args = C.POINTER(args)
         ws = getattr(lib, name + "_workspace_bytes")
         ws.restype, ws.argtypes = C.c_int64, [args, C.c_int]
         getattr(lib, name + "_forward").argtypes = [args, C.c_void_p]

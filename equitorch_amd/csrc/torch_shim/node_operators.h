@@ -1,5 +1,6 @@
 // Autograd nodes of the operators on invariant node features over the C ABI: embedding of node kinds, attention among the nodes of
-// a structure, gated feed-forward block, norm after a residual's addition.  Operands are checked by the Python layer, which also holds the same launches
+// a structure, gated feed-forward block, norm after a residual's addition, cross
+// entropy over kinds.  Operands are checked by the Python layer, which also holds the same launches
 // through ctypes for when this extension is not there; a backward under gradient mode hands over to a Python callable.
 #pragma once
 
@@ -405,7 +406,77 @@ struct AddRms : torch::autograd::Function<AddRms> {
   }
 };
 
+// ---- softmax cross entropy over kinds -------------------------------------------------------------------------------------
+cgtp_kind_loss_args kind_loss_args(const at::Tensor& x, const at::Tensor& table, const at::Tensor& kind, double scale, double cap) {
+  cgtp_kind_loss_args a{};
+  a.x = x.data_ptr();
+  a.table = table.data_ptr();
+  a.kind = kind.data_ptr<int64_t>();
+  a.n_rows = x.size(0);
+  a.n_kinds = table.size(0);
+  a.channels = (int32_t)x.size(1);
+  a.dtype = code_of(x);
+  a.scale = (float)scale;
+  a.cap = (float)cap;
+  return a;
+}
+
+at::Tensor kind_loss_forward(const at::Tensor& x, const at::Tensor& table, const at::Tensor& kind, double scale, double cap, at::Tensor* lse) {
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  cgtp_kind_loss_args a = kind_loss_args(x, table, kind, scale, cap);
+  const auto wide = x.options().dtype(at::kFloat);
+  at::Tensor loss = at::empty({a.n_rows}, wide);
+  if (lse) *lse = at::empty({a.n_rows}, wide);
+  a.loss = (float*)loss.data_ptr();
+  a.lse = lse ? (float*)lse->data_ptr() : nullptr;
+  const at::Tensor ws = bytes_on(x, cgtp_kind_loss_workspace_bytes(&a, 0));
+  a.workspace = ws.data_ptr();
+  check_status(cgtp_kind_loss_forward(&a, current_stream(x)), "cgtp_kind_loss_forward");
+  return loss;
+}
+
+struct KindLoss : torch::autograd::Function<KindLoss> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& table, const at::Tensor& kind, double scale,
+                            double cap, const Fallback* fallback) {
+    at::Tensor lse;
+    at::Tensor loss = kind_loss_forward(x, table, kind, scale, cap, &lse);
+    ctx->save_for_backward({x, table, kind, lse});
+    auto& d = ctx->saved_data;
+    d["scale"] = scale;
+    d["cap"] = cap;
+    d["fallback"] = fallback->id;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    const variable_list s = ctx->get_saved_variables();
+    const at::Tensor &x = s[0], &table = s[1], &kind = s[2];
+    auto& d = ctx->saved_data;
+    const std::vector<bool> need = {ctx->needs_input_grad(0), ctx->needs_input_grad(1)};
+    if (at::GradMode::is_enabled())
+      return call_fallback(d["fallback"].toInt(), grad[0], {x, table}, need, 6, kind, d["scale"].toDouble(), d["cap"].toDouble());
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    cgtp_kind_loss_args a = kind_loss_args(x, table, kind, d["scale"].toDouble(), d["cap"].toDouble());
+    const at::Tensor g = grad[0].contiguous();
+    variable_list out(6);
+    for (size_t i = 0; i < 2; ++i)
+      if (need[i]) out[i] = at::empty(s[i].sizes(), s[i].options());
+    a.lse = (float*)s[3].data_ptr();
+    a.grad_loss = (const float*)g.data_ptr();
+    a.grad_x = mutable_ptr(out[0]);
+    a.grad_table = mutable_ptr(out[1]);
+    const at::Tensor ws = bytes_on(x, cgtp_kind_loss_workspace_bytes(&a, 1));
+    a.workspace = ws.data_ptr();
+    check_status(cgtp_kind_loss_backward(&a, current_stream(x)), "cgtp_kind_loss_backward");
+    return out;
+  }
+};
+
 void bind_node_operators(py::module& m) {
+  m.def("kind_loss", [](const at::Tensor& x, const at::Tensor& table, const at::Tensor& kind, double scale, double cap, bool keep,
+                        const Fallback& fallback) {
+    if (keep) return KindLoss::apply(x, table, kind, scale, cap, &fallback);
+    return kind_loss_forward(x, table, kind, scale, cap, nullptr);
+  }, "softmax cross entropy over kinds; with its autograd node where a backward may follow (keep)");
   typedef c10::optional<at::Tensor> Optional;
   m.def("add_rms", [](const at::Tensor& x, const Optional& residual, const Optional& weight, double eps, bool keep, const Fallback& fallback) {
     if (keep) {

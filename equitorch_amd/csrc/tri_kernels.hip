@@ -716,17 +716,26 @@ int cgtp_abi_layout(int which, int64_t* out, int capacity) {
                                          CGTP_OFF(cgtp_add_rms_args, n_rows), CGTP_OFF(cgtp_add_rms_args, eps),
                                          CGTP_OFF(cgtp_add_rms_args, channels), CGTP_OFF(cgtp_add_rms_args, dtype),
                                          CGTP_OFF(cgtp_add_rms_args, residual_dtype), CGTP_OFF(cgtp_add_rms_args, weight_dtype)};
+  static const int64_t kind_loss_args[] = {sizeof(cgtp_kind_loss_args), CGTP_OFF(cgtp_kind_loss_args, x), CGTP_OFF(cgtp_kind_loss_args, table),
+                                           CGTP_OFF(cgtp_kind_loss_args, kind), CGTP_OFF(cgtp_kind_loss_args, loss),
+                                           CGTP_OFF(cgtp_kind_loss_args, lse), CGTP_OFF(cgtp_kind_loss_args, grad_loss),
+                                           CGTP_OFF(cgtp_kind_loss_args, grad_x), CGTP_OFF(cgtp_kind_loss_args, grad_table),
+                                           CGTP_OFF(cgtp_kind_loss_args, workspace), CGTP_OFF(cgtp_kind_loss_args, n_rows),
+                                           CGTP_OFF(cgtp_kind_loss_args, n_kinds), CGTP_OFF(cgtp_kind_loss_args, channels),
+                                           CGTP_OFF(cgtp_kind_loss_args, dtype), CGTP_OFF(cgtp_kind_loss_args, scale),
+                                           CGTP_OFF(cgtp_kind_loss_args, cap)};
 #undef CGTP_OFF
   const int64_t* tabs[] = {operand, tri, gen_operand, gen, uvu, uvt_item, uvt, uvt_gw, uvt_gy, uvu_tab, psw_table,
-                           psw_args, uvu_mx, uvl_args, uvg_args, uvl_gw_args, nullptr, gff_args, attn_args, attn_item, add_rms_args};
+                           psw_args, uvu_mx, uvl_args, uvg_args, uvl_gw_args, nullptr, gff_args, attn_args, attn_item, add_rms_args, kind_loss_args};
   const int counts[] = {(int)(sizeof(operand) / 8), (int)(sizeof(tri) / 8), (int)(sizeof(gen_operand) / 8),
                         (int)(sizeof(gen) / 8), (int)(sizeof(uvu) / 8), (int)(sizeof(uvt_item) / 8),
                         (int)(sizeof(uvt) / 8), (int)(sizeof(uvt_gw) / 8), (int)(sizeof(uvt_gy) / 8),
                         (int)(sizeof(uvu_tab) / 8), (int)(sizeof(psw_table) / 8), (int)(sizeof(psw_args) / 8), (int)(sizeof(uvu_mx) / 8),
                         (int)(sizeof(uvl_args) / 8), (int)(sizeof(uvg_args) / 8),
                         (int)(sizeof(uvl_gw_args) / 8), 0, (int)(sizeof(gff_args) / 8),
-                        (int)(sizeof(attn_args) / 8), (int)(sizeof(attn_item) / 8), (int)(sizeof(add_rms_args) / 8)};
-  if (which < 0 || which > CGTP_LAYOUT_ADD_RMS_ARGS || !tabs[which]) return -1;
+                        (int)(sizeof(attn_args) / 8), (int)(sizeof(attn_item) / 8), (int)(sizeof(add_rms_args) / 8),
+                        (int)(sizeof(kind_loss_args) / 8)};
+  if (which < 0 || which > CGTP_LAYOUT_KIND_LOSS_ARGS || !tabs[which]) return -1;
   for (int i = 0; out && i < counts[which] && i < capacity; ++i) out[i] = tabs[which][i];
   return counts[which];
 }

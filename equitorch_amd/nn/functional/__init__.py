@@ -8,6 +8,7 @@ from .dropout import irrep_wise_dropout
 from .rotations import angles_to_matrix
 from .embedding import embedding
 from .feed_forward import gated_feed_forward
+from .kind_cross_entropy import kind_cross_entropy
 from .edge import (EdgePlan, edge_tensor_product_uu, edge_tensor_product_uu_radial,
                    edge_tensor_product_uu_vectors)
 from .linears import (irrep_wise_linear, irreps_linear, so2_linear_uu, so2_linear_uv, so3_linear_uu, so3_linear_uv, tensor_product_1uu, tensor_product_1vu, tensor_product_u1u,
@@ -30,5 +31,5 @@ __all__ = [
     "batch_mean_squared_norm", "batch_rms_norm", "layer_rms_norm", "radial_standarize", "polynomial_cutoff",
     "cosine_cutoff", "mollifier_cutoff", "sincos", "xyz_to_sincos", "sparse_wigner_rotation",
     "dense_wigner_rotation", "wigner_d_matrix", "align_to_z_wigner_d", "irrep_wise_dropout", "angles_to_matrix", "so2_linear_uu", "so2_linear_uv", "tensor_dot_uu", "tensor_dot_uv",
-    "embedding", "AttentionPlan", "segment_attention", "gated_feed_forward", "add_rms_norm", "add_rms_norm_8bit",
+    "embedding", "AttentionPlan", "segment_attention", "gated_feed_forward", "add_rms_norm", "add_rms_norm_8bit", "kind_cross_entropy",
 ]

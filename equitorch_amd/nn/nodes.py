@@ -1,5 +1,5 @@
 """Layers on the invariant channels of nodes: ``Embedding`` of their kinds, ``SegmentAttention`` among the nodes of a
-structure, the ``GatedFeedForward`` block and the ``AddRMSNorm`` between blocks."""
+structure, the ``GatedFeedForward`` block, the ``AddRMSNorm`` between blocks and the ``KindCrossEntropy`` of pretraining."""
 from typing import Optional, Tuple
 
 import torch
@@ -9,6 +9,7 @@ from .functional.add_rms_norm import add_rms_norm
 from .functional.attention import AttentionPlan, segment_attention
 from .functional.embedding import embedding
 from .functional.feed_forward import _ACTIVATIONS, gated_feed_forward
+from .functional.kind_cross_entropy import kind_cross_entropy
 from .init import initialize_linear
 
 
@@ -142,3 +143,29 @@ class AddRMSNorm(nn.Module):
 
     def extra_repr(self) -> str:
         return f"channels={self.channels}, eps={self.eps}, affine={self.affine}"
+
+
+class KindCrossEntropy(nn.Module):
+    """``(x (..., channels), kind (...)) -> loss (...)``: cross entropy of ``softmax(scale * x @ weight.T)`` over the rows of a
+    learnable ``(kinds, channels)`` table, 0 where ``kind`` is outside it.  ``weight`` may be an :class:`Embedding`'s
+    (``loss.weight = embedding.weight``); ``scale`` is ``channels ** -0.5`` unless given, ``cap`` bounds the logits."""
+
+    def __init__(self, kinds: int, channels: int, scale: Optional[float] = None, cap: Optional[float] = None):
+        super().__init__()
+        if kinds < 1 or channels < 1:
+            raise ValueError(f"kinds and channels must be positive, got {kinds} and {channels}")
+        if cap is not None and not cap > 0:
+            raise ValueError(f"cap must be positive or None, got {cap}")
+        self.kinds, self.channels, self.cap = kinds, channels, cap
+        self.scale = channels ** -0.5 if scale is None else scale
+        self.weight = nn.Parameter(torch.empty(kinds, channels))
+        self.reset_parameters()
+
+    def reset_parameters(self) -> None:
+        nn.init.normal_(self.weight)
+
+    def forward(self, x: Tensor, kind: Tensor) -> Tensor:
+        return kind_cross_entropy(x, self.weight, kind, self.scale, self.cap)
+
+    def extra_repr(self) -> str:
+        return f"kinds={self.kinds}, channels={self.channels}, scale={self.scale}, cap={self.cap}"

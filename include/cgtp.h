@@ -43,7 +43,8 @@ int cgtp_version(void);
 enum { CGTP_LAYOUT_OPERAND = 0, CGTP_LAYOUT_TRI_ARGS = 1, CGTP_LAYOUT_GEN_OPERAND = 2, CGTP_LAYOUT_GEN_ARGS = 3,
        CGTP_LAYOUT_UVU_ARGS = 4, CGTP_LAYOUT_UVT_ITEM = 5, CGTP_LAYOUT_UVT_ARGS = 6, CGTP_LAYOUT_UVT_GW_ARGS = 7,
        CGTP_LAYOUT_UVT_GY_ARGS = 8, CGTP_LAYOUT_UVU_TABLE = 9, CGTP_LAYOUT_PSW_TABLE = 10, CGTP_LAYOUT_PSW_ARGS = 11,
-       CGTP_LAYOUT_GFF_ARGS = 17, CGTP_LAYOUT_ATTN_ARGS = 18, CGTP_LAYOUT_ATTN_ITEM = 19, CGTP_LAYOUT_ADD_RMS_ARGS = 20 };   /* 16: none */
+       CGTP_LAYOUT_GFF_ARGS = 17, CGTP_LAYOUT_ATTN_ARGS = 18, CGTP_LAYOUT_ATTN_ITEM = 19, CGTP_LAYOUT_ADD_RMS_ARGS = 20,
+       CGTP_LAYOUT_KIND_LOSS_ARGS = 21 };   /* 16: none */
 int cgtp_abi_layout(int which, int64_t* out, int capacity);
 
 /* ---- generic sparse trilinear contraction -------------------------------------------------------------
@@ -872,6 +873,32 @@ typedef struct {
 int64_t cgtp_add_rms_workspace_bytes(const cgtp_add_rms_args* args);
 int cgtp_add_rms_forward(const cgtp_add_rms_args* args, void* stream);
 int cgtp_add_rms_backward(const cgtp_add_rms_args* args, void* stream);
+
+/* ---- softmax cross entropy over the kinds of a table ---------------------------------------------------------------
+ *   z_ik = scale x_i . table_k  (cap > 0: cap tanh(scale x_i . table_k / cap)),  loss_i = log sum_k exp z_ik - z_i,kind(i)
+ * x: (n_rows, channels), table: (n_kinds, channels), contiguous, aligned to an element; kind: (n_rows); loss (n_rows); lse (n_rows)
+ * receives log2 sum_k 2^(z_ik log2 e), for the backward (NULL: not wanted).  A row whose kind is outside 0 .. n_kinds - 1 has loss 0 and no
+ * gradient, whatever it holds, and costs nothing but its zeros.
+ * cgtp_kind_loss_backward reads lse and grad_loss (n_rows) and writes those of grad_x and grad_table that are not NULL, every row
+ * of them.  Products and statistics in fp32; the operand of the gradients' products, softmax less one at the row's kind, is rounded to
+ * dtype, and for grad_table the rows of x times grad_loss over its largest magnitude.  All sums have an order that the sizes and the
+ * rows with a kind determine.  The logits are never kept: workspace (cgtp_kind_loss_workspace_bytes, 16-byte aligned) holds a
+ * copy of the rows that have a kind, statistics, and for the backward up to 64 million logits' gradients at a time and sums in fp32.
+ * n_rows and n_kinds <= 2^30, channels < 2^15, else CGTP_ERR_SHAPE.  dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16.
+ */
+typedef struct {
+  const void *x, *table;
+  const int64_t* kind;
+  float *loss, *lse;
+  const float* grad_loss;
+  void *grad_x, *grad_table, *workspace;
+  int64_t n_rows, n_kinds;
+  int32_t channels, dtype;
+  float scale, cap;
+} cgtp_kind_loss_args;
+int64_t cgtp_kind_loss_workspace_bytes(const cgtp_kind_loss_args* args, int backward);
+int cgtp_kind_loss_forward(const cgtp_kind_loss_args* args, void* stream);
+int cgtp_kind_loss_backward(const cgtp_kind_loss_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,305 @@
+"""Cross entropy over kinds against its definition in 64 bits.
+
+Tolerances are bounds on rounding, element by element: the result's own rounding, plus the roundings of what is held in 32
+bits or in the operands' type times the magnitudes that enter the element."""
+import pytest
+import torch
+
+from equitorch_amd._lib import CgtpError
+from helpers import stable_seed
+
+pytestmark = pytest.mark.gpu
+
+F32, F64, BF16, F16 = torch.float32, torch.float64, torch.bfloat16, torch.float16
+EPS = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}
+U = 2.0 ** -24
+
+
+def _rand(gen, *shape, dtype=F32, std=1.0):
+    return (torch.randn(*shape, generator=gen, dtype=F64) * std).to(dtype)
+
+
+def _within(got, want, bound, what):
+    got, want = got.detach().to(want.device).double(), want.double()
+    assert got.shape == want.shape, f"{what}: {tuple(got.shape)} vs {tuple(want.shape)}"
+    excess = ((got - want).abs() - bound).max() if want.numel() else torch.tensor(-1.0)
+    assert float(excess) <= 0 and torch.isfinite(got).all(), f"{what}: {float(excess):.3e} over the bound"
+
+
+def _check(got, x, table, kind, scale, cap, g, dtype):
+    """(loss, grad_x, grad_table) against the formulas, row by row those that have a kind."""
+    n, c = x.shape
+    k = table.shape[0]
+    asked = ((kind >= 0) & (kind < k)).nonzero()[:, 0]
+    y = kind[asked]
+    w, xs, gs = table.double(), x[asked].double(), g[asked].double()[:, None]
+    raw = xs @ w.T * scale
+    err = (c + 4) * U * (xs.abs() @ w.abs().T) * abs(scale)              # of a product over C and the scale
+    th = torch.tanh(raw / cap) if cap else torch.zeros_like(raw)
+    z = cap * th if cap else raw
+    if cap:
+        err = err + 12 * U * cap                                         # a hyperbolic tangent in 32 bits: some roundings of 1
+    err = err + 4 * U * z.abs().amax(1, keepdim=True)                    # to the base 2, less the maximum
+    most = err.amax(1, keepdim=True)
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    delta = most + (k / 4 + 40) * U                                      # of lse: its terms' errors, and a sum in chains of K / 4
+    loss = torch.zeros(n, dtype=F64, device=x.device)
+    bound = torch.zeros_like(loss)
+    loss[asked] = (lse - z.gather(1, y[:, None]))[:, 0]
+    bound[asked] = (delta + err.gather(1, y[:, None]) + 4 * U * (lse.abs() + loss[asked][:, None].abs()))[:, 0]
+    _within(got[0], loss, bound, "loss")
+    if got[1] is None and got[2] is None:
+        return
+    one = torch.zeros_like(z).scatter_(1, y[:, None], 1.0)
+    p = (z - lse).exp()
+    slope = 1 - th * th
+    dz = (p - one) * slope
+    off = 2 * p * (err + delta + 2 * U * (z - lse).abs()) + 2 * U * one + (8 * U if cap else 0) * (p + one)
+    off = off + EPS[dtype] * (dz.abs() + off) + (2.0 ** -40 if dtype == F16 else 2.0 ** -120)
+    if got[1] is not None:
+        want, size = torch.zeros(n, c, dtype=F64, device=x.device), torch.zeros(n, c, dtype=F64, device=x.device)
+        want[asked] = gs * scale * (dz @ w)
+        size[asked] = gs.abs() * abs(scale) * ((off + (k + 4) * U * dz.abs()) @ w.abs())
+        _within(got[1], want, EPS[dtype] * (want.abs() + size) + size + (2.0 ** -25 if dtype == F16 else 0), "grad_x")
+    if got[2] is not None:
+        top = float(gs.abs().max()) if len(asked) else 0.0
+        xg, rounding = gs * xs, EPS[dtype] * (gs * xs).abs() + (top * 2.0 ** -25 if dtype == F16 else 0)
+        want = scale * (dz.T @ xg)
+        size = abs(scale) * ((off + (n + 8) * U * dz.abs()).T @ (xg.abs() + rounding) + dz.abs().T @ rounding)
+        _within(got[2], want, EPS[dtype] * (want.abs() + size) + size + (2.0 ** -25 if dtype == F16 else 0), "grad_table")
+
+
+def _inputs(seed, rows, kinds, channels, dtype, masked):
+    gen = torch.Generator().manual_seed(seed)
+    x, table = _rand(gen, rows, channels, dtype=dtype), _rand(gen, kinds, channels, dtype=dtype)
+    kind = torch.randint(0, kinds, (rows,), generator=gen)
+    hidden = torch.rand(rows, generator=gen) < masked
+    kind[hidden] = torch.where(torch.arange(int(hidden.sum())) % 2 == 0, -1, kinds)
+    x[hidden] = float("nan")                                             # what is not asked for is not read
+    g = _rand(gen, rows) if rows % 2 else torch.full((rows,), 1.0 / rows)
+    g[hidden] = float("nan")
+    return x, table, kind, g
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,kinds,channels,masked,cap", [
+    (1, 1, 1, 0.0, None), (1, 2, 8, 0.0, None), (30, 100, 64, 0.0, None), (31, 100, 64, 0.3, 5.0), (129, 257, 40, 0.0, 20.0), (64, 128, 32, 0.0, None),
+    (65, 129, 33, 0.5, None), (301, 1000, 33, 0.85, 3.0), (1001, 3000, 100, 0.1, None), (130, 129, 512, 0.0, None), (5, 20011, 16, 0.0, None),
+    (2001, 10, 7, 0.7, None), (3, 40, 1003, 0.0, 30.0), (70, 5, 20, 1.0, None)])
+def test_kind_cross_entropy(device, dtype, rows, kinds, channels, masked, cap):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    x, table, kind, g = _inputs(stable_seed(rows, kinds, channels), rows, kinds, channels, dtype, masked)
+    scale = 1.5 * channels ** -0.5
+    leaves = [t.to(device).requires_grad_(True) for t in (x, table)]
+    loss = kind_cross_entropy(*leaves, kind.to(device), scale, cap)
+    assert loss.dtype == F32 and loss.shape == (rows,)
+    grads = torch.autograd.grad(loss, leaves, g.to(device), retain_graph=True)
+    _check((loss, *grads), x, table, kind, scale, cap, g, dtype)
+    assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(loss, leaves, g.to(device))))
+    with torch.no_grad():
+        assert torch.equal(kind_cross_entropy(*leaves, kind.to(device), scale, cap), loss)
+
+
+@pytest.mark.parametrize("rows,kinds,channels,dtype", [(33001, 2300, 16, BF16), (66001, 1100, 8, F32), (300, 300011, 8, F16)])
+def test_pieces(device, rows, kinds, channels, dtype):
+    """More rows and kinds than the backward takes at a time."""
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    x, table, kind, g = (t.to(device) for t in _inputs(stable_seed(rows, kinds), rows, kinds, channels, dtype, 0.02))
+    leaves = [t.clone().requires_grad_(True) for t in (x, table)]
+    loss = kind_cross_entropy(*leaves, kind, 0.3)
+    grads = torch.autograd.grad(loss, leaves, g)
+    _check((loss, *grads), x, table, kind, 0.3, None, g, dtype)
+
+
+def test_one_gradient_at_a_time(device):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    x, table, kind, g = _inputs(3, 301, 700, 24, BF16, 0.2)
+    leaves = [t.to(device).requires_grad_(True) for t in (x, table)]
+    both = torch.autograd.grad(kind_cross_entropy(*leaves, kind.to(device)), leaves, g.to(device))
+    for i in (0, 1):
+        one = [t.detach().requires_grad_(i == j) for j, t in enumerate(leaves)]
+        (grad,) = torch.autograd.grad(kind_cross_entropy(*one, kind.to(device)), one[i], g.to(device))
+        assert torch.equal(grad, both[i])
+
+
+def test_large_logits(device):
+    """Probabilities of one and of nothing: no overflow, no NaN."""
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    for dtype in (F32, BF16, F16):
+        x, table, kind, g = _inputs(4, 201, 333, 16, dtype, 0.0)
+        leaves = [t.to(device).requires_grad_(True) for t in (x, table)]
+        loss = kind_cross_entropy(*leaves, kind.to(device), 300.0)
+        _check((loss, *torch.autograd.grad(loss, leaves, g.to(device))), x, table, kind, 300.0, None, g, dtype)
+        loss = kind_cross_entropy(*leaves, kind.to(device), 1e4, 2.0)
+        assert torch.isfinite(loss).all() and all(torch.isfinite(t).all() for t in torch.autograd.grad(loss, leaves, g.to(device)))
+
+
+def test_small_incoming_gradients_in_fp16(device):
+    """Gradients of one row and of the mean over many, whose products with probabilities are below fp16's range."""
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    x, table, kind, g = _inputs(5, 201, 5000, 16, F16, 0.0)
+    for size in (1e-3, 1.0):
+        leaves = [t.to(device).requires_grad_(True) for t in (x, table)]
+        weights = torch.full_like(g, size)
+        weights[7] = size * 2.0 ** -12
+        loss = kind_cross_entropy(*leaves, kind.to(device), 0.25)
+        _check((loss, *torch.autograd.grad(loss, leaves, weights.to(device))), x, table, kind, 0.25, None, weights, F16)
+
+
+def test_no_gradient_comes_in(device):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    x, table, kind, _ = _inputs(6, 77, 50, 16, F32, 0.1)
+    leaves = [t.to(device).requires_grad_(True) for t in (x, table)]
+    loss = kind_cross_entropy(*leaves, kind.to(device))
+    for grad in torch.autograd.grad(loss, leaves, torch.zeros(77, device=device)):
+        assert torch.equal(grad, torch.zeros_like(grad))
+
+
+def test_shapes_strides_and_streams(device):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    gen = torch.Generator().manual_seed(7)
+    x, table = _rand(gen, 4, 25, 19).to(device), _rand(gen, 60, 19).to(device)
+    kind = torch.randint(-1, 60, (4, 25), generator=gen).to(device)
+    want = kind_cross_entropy(x.reshape(100, 19), table, kind.reshape(100)).reshape(4, 25)
+    assert torch.equal(kind_cross_entropy(x, table, kind), want)
+    assert torch.equal(kind_cross_entropy(x.transpose(0, 1), table.T.contiguous().T, kind.T), want.T)
+    loose = torch.empty(60 * 19 + 1, device=device)[1:].view(60, 19).copy_(table)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = kind_cross_entropy(x, loose, kind)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    assert torch.equal(kind_cross_entropy(x[0, 0], table, kind[0, 0]), want[0, 0])
+    none = table.clone().requires_grad_(True)
+    empty = kind_cross_entropy(x[:0], none, kind[:0])
+    assert empty.shape == (0, 25)
+    (grad,) = torch.autograd.grad(empty.sum(), none)
+    assert torch.equal(grad, torch.zeros_like(grad))
+
+
+def test_tied_to_an_embedding(device):
+    """One table is looked up and scored against: its gradient is the sum of both."""
+    from equitorch_amd.nn.functional import embedding, kind_cross_entropy
+    gen = torch.Generator().manual_seed(8)
+    table = _rand(gen, 30, 12).to(device).requires_grad_(True)
+    seen, asked = (torch.randint(0, 30, (50,), generator=gen).to(device) for _ in range(2))
+    (got,) = torch.autograd.grad(kind_cross_entropy(embedding(seen, table), table, asked, 0.5).mean(), table)
+    wide = table.detach().double().requires_grad_(True)
+    loss = torch.nn.functional.cross_entropy(wide[seen] @ wide.T * 0.5, asked)
+    (want,) = torch.autograd.grad(loss, wide)
+    _within(got, want, 1e-5 * want.abs().max(), "table")      # some hundred roundings of 2^-24 of the largest
+
+
+def test_higher_order_and_differences(device):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    gen = torch.Generator().manual_seed(9)
+    x, table = _rand(gen, 15, 9).to(device).requires_grad_(True), _rand(gen, 21, 9).to(device).requires_grad_(True)
+    kind = torch.randint(-1, 21, (15,), generator=gen).to(device)
+    for cap in (None, 3.0):
+        def plain(x, w):
+            z = x @ w.T * 0.7
+            z = cap * torch.tanh(z / cap) if cap else z
+            ok = kind >= 0
+            return torch.nn.functional.cross_entropy(z[ok], kind[ok], reduction="sum")
+        got = torch.autograd.grad(kind_cross_entropy(x, table, kind, 0.7, cap).sum(), (x, table), create_graph=True)
+        twice = torch.autograd.grad(sum(t.square().sum() for t in got), (x, table))
+        wide = [t.detach().double().requires_grad_(True) for t in (x, table)]
+        want = torch.autograd.grad(plain(*wide), wide, create_graph=True)
+        more = torch.autograd.grad(sum(t.square().sum() for t in want), wide)
+        for a, b in zip((*got, *twice), (*want, *more)):
+            _within(a, b.detach(), 1e-4 * b.detach().abs().max(), "gradient")
+        first = torch.autograd.grad(kind_cross_entropy(x, table, kind, 0.7, cap).sum(), (x, table))
+        for i in (0, 1):
+            v = _rand(gen, *(x, table)[i].shape).to(device)
+            ends = [float(kind_cross_entropy(*[t.detach() + (s * 1e-2 * v if j == i else 0) for j, t in enumerate((x, table))], kind, 0.7, cap)
+                          .double().sum()) for s in (1, -1)]
+            along = float((first[i] * v).sum())
+            assert abs((ends[0] - ends[1]) / 2e-2 - along) <= 2e-2 * (1 + abs(along))
+
+
+def test_logits_are_not_kept(device):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    rows, kinds = 20000, 50000
+    x = torch.randn(rows, 32, device=device, dtype=BF16, requires_grad=True)
+    table = torch.randn(kinds, 32, device=device, dtype=BF16, requires_grad=True)
+    kind = torch.randint(0, kinds, (rows,), device=device)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    loss = kind_cross_entropy(x, table, kind)
+    assert torch.cuda.max_memory_allocated() - before < rows * kinds * 2 / 20
+    torch.autograd.grad(loss.mean(), (x, table))
+    assert torch.cuda.max_memory_allocated() - before < rows * kinds * 2 / 4
+
+
+def test_graph_replays(device):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    x = torch.randn(700, 96, device=device, dtype=BF16, requires_grad=True)
+    table = torch.randn(3000, 96, device=device, dtype=BF16, requires_grad=True)
+    kind = torch.randint(0, 3000, (700,), device=device)
+    g = torch.rand(700, device=device)
+
+    def step():
+        loss = kind_cross_entropy(x, table, kind, 0.1)
+        return (loss, *torch.autograd.grad(loss, (x, table), g))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = step()
+    for seed in range(3):
+        torch.manual_seed(seed)
+        with torch.no_grad():
+            x.copy_(torch.randn(700, 96, device=device))
+            kind.copy_(torch.randint(-1000, 3000, (700,), device=device))       # another number of rows with a kind
+            g.copy_(torch.rand(700, device=device))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(kept, step()):
+            assert torch.equal(a, b)
+
+
+def test_autocast(device):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    x = torch.randn(20, 16, device=device, dtype=BF16)
+    table = torch.randn(9, 16, device=device, requires_grad=True)
+    kind = torch.arange(20, device=device) % 9
+    with torch.autocast("cuda", dtype=BF16):
+        loss = kind_cross_entropy(x, table, kind)
+    assert torch.equal(loss, kind_cross_entropy(x, table.to(BF16), kind))
+    assert torch.autograd.grad(loss.sum(), table)[0].dtype == F32
+    with pytest.raises(CgtpError):
+        kind_cross_entropy(x, table, kind)
+
+
+def test_refusals(device):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    x, w, k = torch.zeros(3, 8, device=device), torch.ones(5, 8, device=device), torch.zeros(3, dtype=torch.int64, device=device)
+    for bad in ((x.double(), w.double(), k), (x, w.half(), k), (x, w, k.int()), (x, w[:, :4], k), (x, w[0], k), (x, w[:0], k), (x, w, k[:2]),
+                (x, w, k[:, None]), (x[:, :0], w[:, :0], k), (x.cpu(), w, k), (x, w.cpu(), k), (x, w, k.cpu())):
+        with pytest.raises(CgtpError):
+            kind_cross_entropy(*bad)
+    for scale, cap in ((float("nan"), None), (float("inf"), None), (1e39, None), (1.0, 0.0), (1.0, -1.0), (1.0, float("nan")), (1.0, float("inf")), (1.0, 1e-40),
+                       (1e20, 1e-30)):
+        with pytest.raises(CgtpError):
+            kind_cross_entropy(x, w, k, scale, cap)
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        kind_cross_entropy(fwd.make_dual(x, torch.ones_like(x)), w, k)
+
+
+def test_layer(device):
+    from equitorch_amd import nn as en
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    table = en.Embedding(11, 8).to(device)
+    m = en.KindCrossEntropy(11, 8).to(device)
+    m.weight = table.weight
+    x, kind = torch.randn(2, 9, 8, device=device), torch.arange(18, device=device).view(2, 9) - 3
+    loss = m(x, kind)
+    assert torch.equal(loss, kind_cross_entropy(x, table.weight, kind, 8 ** -0.5)) and float(loss[0, :3].detach().abs().max()) == 0
+    loss.sum().backward()
+    assert torch.isfinite(table.weight.grad).all()

@@ -6,12 +6,12 @@ import pytest
 import torch
 
 from equitorch_amd import _lib
-from equitorch_amd._lib import AddRmsArgs, CgtpError
+from equitorch_amd._lib import AddRmsArgs, CgtpError, KindLossArgs
 
 NULL, SHAPE, ALIGN, DTYPE, CONFIG, WORKSPACE = 1, 2, 3, 4, 5, 8
 
 
-@pytest.mark.parametrize("which,cls", [(20, AddRmsArgs)])
+@pytest.mark.parametrize("which,cls", [(20, AddRmsArgs), (21, KindLossArgs)])
 def test_struct_layouts(which, cls):
     n = _lib.lib.cgtp_abi_layout(which, None, 0)
     assert n == 1 + len(cls._fields_)
@@ -69,5 +69,64 @@ def test_add_rms_layer():
     m = en.AddRMSNorm(12, eps=1e-6)
     assert m.weight.shape == (12,) and "channels=12" in repr(m) and en.AddRMSNorm(3, affine=False).weight is None
     for make in (lambda: en.AddRMSNorm(0), lambda: en.AddRMSNorm(4, eps=-1.0), lambda: en.AddRMSNorm(4, eps=float("inf")), lambda: m(torch.zeros(3, 4))):
+        with pytest.raises(ValueError):
+            make()
+
+
+# ---- cross entropy over kinds ------------------------------------------------------------------------------------
+def _loss(**changed):
+    a = KindLossArgs()
+    for name in ("x", "table", "kind", "loss", "lse", "grad_loss", "grad_x", "grad_table", "workspace"):
+        setattr(a, name, 4096)
+    a.n_rows, a.n_kinds, a.channels, a.scale = 5, 7, 8, 1.0
+    for name, value in changed.items():
+        setattr(a, name, value)
+    return a
+
+
+@pytest.mark.parametrize("changed,forward,backward", [
+    ({"dtype": 1}, DTYPE, DTYPE), ({"channels": 0}, SHAPE, SHAPE), ({"channels": 1 << 15}, SHAPE, SHAPE), ({"n_rows": -1}, SHAPE, SHAPE),
+    ({"n_rows": (1 << 30) + 1}, SHAPE, SHAPE), ({"n_kinds": 0}, SHAPE, SHAPE), ({"n_kinds": (1 << 30) + 1}, SHAPE, SHAPE), ({"x": None}, NULL, NULL),
+    ({"table": None}, NULL, NULL), ({"kind": None}, NULL, NULL), ({"loss": None}, NULL, None), ({"lse": None}, None, NULL),
+    ({"grad_loss": None}, None, NULL), ({"workspace": None}, WORKSPACE, WORKSPACE), ({"workspace": 4104}, ALIGN, ALIGN)])
+def test_kind_loss_codes(changed, forward, backward):
+    a = _loss(**changed)
+    if forward is not None:
+        assert _lib.lib.cgtp_kind_loss_forward(C.byref(a), None) == forward
+    if backward is not None:
+        assert _lib.lib.cgtp_kind_loss_backward(C.byref(a), None) == backward
+    assert _lib.lib.cgtp_kind_loss_forward(None, None) == _lib.lib.cgtp_kind_loss_backward(None, None) == NULL
+
+
+def test_kind_loss_without_work():
+    assert _lib.lib.cgtp_kind_loss_forward(C.byref(_loss(n_rows=0, x=None, kind=None, workspace=None)), None) == 0
+    assert _lib.lib.cgtp_kind_loss_backward(C.byref(_loss(n_rows=0, grad_table=None)), None) == 0
+    assert _lib.lib.cgtp_kind_loss_backward(C.byref(_loss(grad_x=None, grad_table=None)), None) == 0
+
+
+def test_kind_loss_workspace():
+    need = lambda backward, **changed: _lib.lib.cgtp_kind_loss_workspace_bytes(C.byref(_loss(**changed)), backward)
+    assert need(0, n_rows=0) == need(1, n_rows=0) == need(1, channels=0) == 0
+    large = dict(n_rows=16384, n_kinds=30000, channels=256, dtype=2)
+    logits = 2 * 16384 * 30000
+    assert 2 * 16384 * 256 < need(0, **large) < logits / 16 and need(1, **large) < logits / 2
+    assert need(1, **{**large, "grad_table": None}) < need(1, **large)
+    # a table whose rows are not whole aligned chunks is copied
+    assert need(0, **{**large, "table": 4098}) - need(0, **large) == 2 * 30000 * 256
+    # the most rows and kinds there may be: no overflow
+    assert need(1, n_rows=1 << 30, n_kinds=1 << 30, channels=(1 << 15) - 1) > 1 << 45
+
+
+def test_kind_cross_entropy_takes_gpu_tensors_only():
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    with pytest.raises(CgtpError):
+        kind_cross_entropy(torch.zeros(3, 4), torch.zeros(5, 4), torch.zeros(3, dtype=torch.int64))
+
+
+def test_kind_cross_entropy_layer():
+    from equitorch_amd import nn as en
+    m = en.KindCrossEntropy(5, 16, cap=3.0)
+    assert m.weight.shape == (5, 16) and m.scale == 0.25 and "cap=3.0" in repr(m)
+    for make in (lambda: en.KindCrossEntropy(0, 4), lambda: en.KindCrossEntropy(4, 0), lambda: en.KindCrossEntropy(4, 4, cap=0.0)):
         with pytest.raises(ValueError):
             make()
