@@ -184,6 +184,18 @@ class KindLossArgs(C.Structure):
                 ("scale", C.c_float), ("cap", C.c_float)]
 
 
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p), ("master", C.c_void_p), ("step", C.c_void_p),
+                ("n", C.c_int64), ("number", C.c_int64)]
+
+
+class AdamwArgs(C.Structure):
+    _fields_ = [("tensors", C.POINTER(AdamwTensor)), ("n_tensors", C.c_int64), ("lr_ptr", C.c_void_p), ("lr", C.c_double),
+                ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double), ("dtype", C.c_int32),
+                ("state_bits", C.c_int32), ("master", C.c_int32), ("maximize", C.c_int32), ("seed", C.c_uint32), ("reserved_", C.c_int32)]
+
+
 def _load():
     if not os.path.exists(_LIB_PATH):
         raise ImportError(
@@ -318,6 +330,7 @@ def _load():
     lib.cgtp_add_rms_workspace_bytes.restype = C.c_int64
     lib.cgtp_add_rms_workspace_bytes.argtypes = [C.POINTER(AddRmsArgs)]
     lib.cgtp_add_rms_forward.argtypes = lib.cgtp_add_rms_backward.argtypes = [C.POINTER(AddRmsArgs), C.c_void_p]
+    lib.cgtp_adamw_step.argtypes = [C.POINTER(AdamwArgs), C.c_void_p]
     lib.cgtp_abi_layout.argtypes = [C.c_int, C.POINTER(C.c_int64), C.c_int]
     return lib
 

@@ -1,0 +1,322 @@
+// AdamW step over many tensors at once (cgtp_adamw_step):
+//
+//   m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2,
+//   p <- p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Bound by memory: 28 bytes an element in fp32 with states in 32 bits, 16 with states in 8.  The tensors' addresses are kernel
+// arguments, so that a launch takes dozens of tensors and nothing has to reach the GPU before it; a workgroup takes a chunk of one
+// tensor.  The step's number is on the GPU (a recorded graph counts on when it is replayed): every workgroup reads it and
+// works its factors out, and a launch behind them adds one.
+//
+// 8 bits: m and r = sqrt(v) in e4m3 with a scale for each 256 elements of a tensor, the largest magnitude / 448.  A wavefront has
+// such a block in registers, four elements a lane.  m is rounded to nearest.  r is rounded up or down at random, in
+// proportion: b2 = 0.999 changes v by a thousandth a step, a sixteenth of the way to the next value of three
+// mantissa bits at most, and to nearest it would stay where it is for ever.  Above zero it never becomes zero, which m would
+// be divided by.  The random bits are a hash of seed, tensor, step and element: the same in every run.  The step itself is taken on m and v
+// before they are rounded.
+#include "elem.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace cgtp {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64, kBlock = CGTP_ADAMW_BLOCK, kAtOnce = 48;
+static_assert(kBlock == 256, "four elements for each lane");
+
+struct Entry {
+  void* p;
+  const void* g;
+  void *m, *v;
+  float *m_scale, *v_scale, *master;
+  const float* step;
+  unsigned n, first, number;      // first: its first chunk among the launch's; number: the tensor's, for the random bits
+};
+struct StepArgs {
+  Entry entry[kAtOnce];
+  double log_b1, log_b2, lr, decay;
+  const float* lr_ptr;            // null: lr
+  float b1, b1_rest, b2, b2_rest, eps, sign;
+  unsigned seed;
+  int entries, blocks;            // blocks: of 256 elements, in a chunk
+};
+static_assert(sizeof(StepArgs) <= 4096);
+
+struct Factors {
+  float keep, size, root;         // 1 - lr decay, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  unsigned key;
+};
+
+__device__ __forceinline__ unsigned mix(unsigned h) {
+  h = (h ^ (h >> 16)) * 0x9C8F2D35u;
+  h = (h ^ (h >> 15)) * 0xB5297A4Du;
+  return h ^ (h >> 16);
+}
+
+// Four elements of a block from `left` on; WHOLE: all are there.
+template <typename U, bool WHOLE>
+__device__ __forceinline__ void load4(float (&d)[4], const U* p, int left) {
+  typedef U vec __attribute__((ext_vector_type(4)));
+  typedef unsigned raw_t __attribute__((ext_vector_type(sizeof(U))));
+  if constexpr (WHOLE) {
+    const vec v = __builtin_bit_cast(vec, *reinterpret_cast<const typename LooseOf<U, raw_t>::type*>(p));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[e] = (float)v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[e] = e < left ? (float)p[e] : 0.f;
+  }
+}
+template <typename U, bool WHOLE>
+__device__ __forceinline__ void store4(U* p, const float (&s)[4], int left) {
+  typedef U vec __attribute__((ext_vector_type(4)));
+  typedef unsigned raw_t __attribute__((ext_vector_type(sizeof(U))));
+  if constexpr (WHOLE) {
+    vec v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (U)s[e];
+    *reinterpret_cast<typename LooseOf<U, raw_t>::type*>(p) = __builtin_bit_cast(raw_t, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) p[e] = (U)s[e];
+  }
+}
+typedef unsigned loose_u32 __attribute__((aligned(1)));
+template <bool WHOLE>
+__device__ __forceinline__ unsigned load_codes(const uint8_t* p, int left) {
+  if constexpr (WHOLE) return *reinterpret_cast<const loose_u32*>(p);
+  unsigned r = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < left) r |= (unsigned)p[e] << (8 * e);
+  return r;
+}
+template <bool WHOLE>
+__device__ __forceinline__ void store_codes(uint8_t* p, unsigned codes, int left) {
+  if constexpr (WHOLE) {
+    *reinterpret_cast<loose_u32*>(p) = codes;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) p[e] = (uint8_t)(codes >> (8 * e));
+  }
+}
+__device__ __forceinline__ void decode(float (&d)[4], unsigned codes, float scale) {
+  d[0] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 0) * scale;
+  d[1] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 1) * scale;
+  d[2] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 2) * scale;
+  d[3] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 3) * scale;
+}
+__device__ __forceinline__ unsigned encode(const float (&s)[4]) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], r, true);
+}
+
+// The scale of a block: its largest magnitude / 448, 0 for zeros, a normal number else (whose inverse is finite), NaN where an
+// element is not finite.  The order of the bit patterns is that of the magnitudes, NaN above infinity.
+__device__ __forceinline__ float block_scale(const float (&s)[4], float& inverse) {
+  unsigned top = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = std::max(top, __float_as_uint(s[e]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) top = std::max(top, (unsigned)__shfl_xor((int)top, o));
+  const float most = __uint_as_float(top);
+  const float scale = most == 0.f ? 0.f : most < INFINITY ? std::max(most / 448.f, 0x1p-126f) : NAN;
+  inverse = most == 0.f ? 0.f : 1.f / scale;
+  return scale;
+}
+__device__ __forceinline__ float within_448(float q) { return q > 448.f ? 448.f : q < -448.f ? -448.f : q; }
+
+// A value of 0 .. 448 up or down to one of e4m3, by 20 random bits: added below the last bit that stays, which is then cut; below
+// 2^-6 the values are the multiples of 2^-9.
+__device__ __forceinline__ float at_random(float q, unsigned bits) {
+  const float normal = __uint_as_float((__float_as_uint(q) + bits) & 0xfff00000u);
+  const float small = floorf(q * 512.f + (float)bits * 0x1p-20f) * 0x1p-9f;
+  const float r = q < 0x1p-6f ? std::max(small, 0x1p-9f) : std::min(normal, 448.f);
+  return q > 0.f ? r : 0.f;
+}
+
+// A value rounded to fp32 here: neither a product that a sum takes unrounded nor a result that goes on to 16 bits unrounded, so
+// that what is stored in 16 and in 8 bits is the rounding of the number in 32 that the formula says.
+__device__ __forceinline__ float rounded(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+
+// Four elements of one lane.
+template <typename T, bool MASTER, bool EIGHT, bool WHOLE>
+__device__ __forceinline__ void step_block(const StepArgs& a, const Entry& t, const Factors& f, unsigned at, unsigned block) {
+  const int left = (int)(t.n - at);
+  float p[4], g[4], m[4], v[4];
+  float* master = t.master + at;
+  T* param = (T*)t.p + at;
+  if constexpr (MASTER) load4<float, WHOLE>(p, master, left);
+  else load4<T, WHOLE>(p, param, left);
+  load4<T, WHOLE>(g, (const T*)t.g + at, left);
+  if constexpr (EIGHT) {
+    const unsigned cm = load_codes<WHOLE>((const uint8_t*)t.m + at, left), cv = load_codes<WHOLE>((const uint8_t*)t.v + at, left);
+    decode(m, cm, t.m_scale[block]);
+    decode(v, cv, t.v_scale[block]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = rounded(v[e] * v[e]);
+  } else {
+    load4<float, WHOLE>(m, (const float*)t.m + at, left);
+    load4<float, WHOLE>(v, (const float*)t.v + at, left);
+  }
+  float r[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float ge = g[e] * a.sign;
+    m[e] = rounded(m[e] * a.b1) + rounded(ge * a.b1_rest);
+    v[e] = rounded(v[e] * a.b2) + rounded(ge * ge * a.b2_rest);
+    r[e] = sqrtf(v[e]);
+    p[e] = rounded(rounded(p[e] * f.keep) - rounded(f.size * (m[e] / (rounded(r[e] * f.root) + a.eps))));
+  }
+  if constexpr (MASTER) store4<float, WHOLE>(master, p, left);
+  store4<T, WHOLE>(param, p, left);
+  if constexpr (EIGHT) {
+    float inverse, q[4];
+    const float m_scale = block_scale(m, inverse);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = within_448(m[e] * inverse);
+    store_codes<WHOLE>((uint8_t*)t.m + at, encode(q), left);
+    const float v_scale = block_scale(r, inverse);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = at_random(std::min(r[e] * inverse, 448.f), mix(f.key + (at + e) * 0x9E3779B1u) >> 12);
+    store_codes<WHOLE>((uint8_t*)t.v + at, encode(q), left);
+    if ((threadIdx.x & 63) == 0) {
+      t.m_scale[block] = m_scale;
+      t.v_scale[block] = v_scale;
+    }
+  } else {
+    store4<float, WHOLE>((float*)t.m + at, m, left);
+    store4<float, WHOLE>((float*)t.v + at, v, left);
+  }
+}
+
+template <typename T, bool MASTER, bool EIGHT>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(StepArgs a) {
+  int lo = 0, hi = a.entries - 1;      // the last tensor whose first chunk is not behind this one
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.entry[mid].first <= blockIdx.x) lo = mid;
+    else hi = mid - 1;
+  }
+  const Entry& t = a.entry[lo];
+  Factors f;
+  {
+    const float now = *t.step + 1.f;
+    const double lr = a.lr_ptr ? (double)*a.lr_ptr : a.lr;
+    f.keep = (float)(1.0 - lr * a.decay);
+    f.size = (float)(lr / -expm1((double)now * a.log_b1));
+    f.root = (float)(1.0 / sqrt(-expm1((double)now * a.log_b2)));
+    f.key = mix(a.seed * 0x85157AF5u + t.number * 0x9E3779B1u + (unsigned)now * 0xC2B2AE63u);
+  }
+  const int lane = threadIdx.x & 63;
+  const unsigned first = (blockIdx.x - t.first) * (unsigned)a.blocks, all = (t.n + kBlock - 1) / kBlock, end = std::min(first + a.blocks, all);
+  for (unsigned b = first + (threadIdx.x >> 6); b < end; b += kWaves) {
+    const unsigned at = b * kBlock + lane * 4;
+    if ((b + 1) * (int64_t)kBlock <= t.n) {
+      step_block<T, MASTER, EIGHT, true>(a, t, f, at, b);
+    } else {
+      // lanes beyond the end have nothing, but take part in the block's scale
+      step_block<T, MASTER, EIGHT, false>(a, t, f, std::min(at, t.n), b);
+    }
+  }
+}
+
+constexpr int kSteps = 480;
+struct CountArgs {
+  float* step[kSteps];
+  int n;
+};
+__global__ void __launch_bounds__(kSteps) adamw_count_kernel(CountArgs a) {
+  if ((int)threadIdx.x < a.n) *a.step[threadIdx.x] += 1.f;
+}
+
+int adamw_check(const cgtp_adamw_args* a) {
+  if (!a) return CGTP_ERR_NULL;
+  if (a->dtype != CGTP_F32 && a->dtype != CGTP_BF16 && a->dtype != CGTP_F16) return CGTP_ERR_DTYPE;
+  if (a->state_bits != 8 && a->state_bits != 32) return CGTP_ERR_CONFIG;
+  if (a->n_tensors < 0) return CGTP_ERR_SHAPE;
+  if (!(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1)) return CGTP_ERR_CONFIG;
+  if (a->n_tensors > 0 && !a->tensors) return CGTP_ERR_NULL;
+  for (int64_t i = 0; i < a->n_tensors; ++i) {
+    const cgtp_adamw_tensor& t = a->tensors[i];
+    if (t.n < 0 || t.n > 0x7fffffff) return CGTP_ERR_SHAPE;
+    if (!t.step) return CGTP_ERR_NULL;
+    if (t.n == 0) continue;
+    if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return CGTP_ERR_NULL;
+    if (a->state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return CGTP_ERR_NULL;
+    if (a->master && !t.master) return CGTP_ERR_NULL;
+  }
+  if (a->master && a->dtype == CGTP_F32) return CGTP_ERR_CONFIG;
+  return CGTP_OK;
+}
+
+typedef void (*Kernel)(StepArgs);
+template <typename T>
+Kernel kernel_of(bool master, bool eight) {
+  if constexpr (sizeof(T) == 2)
+    if (master) return eight ? adamw_kernel<T, true, true> : adamw_kernel<T, true, false>;
+  return eight ? adamw_kernel<T, false, true> : adamw_kernel<T, false, false>;
+}
+
+}  // namespace
+}  // namespace cgtp
+
+extern "C" {
+
+int cgtp_adamw_step(const cgtp_adamw_args* a, void* stream) {
+  using namespace cgtp;
+  if (int rc = adamw_check(a)) return rc;
+  if (a->n_tensors == 0) return CGTP_OK;
+  const bool eight = a->state_bits == 8, master = a->master != 0;
+  const Kernel kernel = a->dtype == CGTP_F32 ? kernel_of<float>(master, eight)
+                        : a->dtype == CGTP_BF16 ? kernel_of<bf16_t>(master, eight) : kernel_of<f16_t>(master, eight);
+  StepArgs s = {};
+  s.log_b1 = std::log(a->beta1);
+  s.log_b2 = std::log(a->beta2);
+  s.lr = a->lr;
+  s.lr_ptr = a->lr_ptr;
+  s.decay = a->weight_decay;
+  s.b1 = (float)a->beta1;
+  s.b1_rest = (float)(1.0 - a->beta1);
+  s.b2 = (float)a->beta2;
+  s.b2_rest = (float)(1.0 - a->beta2);
+  s.eps = (float)a->eps;
+  s.sign = a->maximize ? -1.f : 1.f;
+  s.seed = a->seed;
+  int64_t all = 0;
+  for (int64_t i = 0; i < a->n_tensors; ++i) all += (a->tensors[i].n + kBlock - 1) / kBlock;
+  // Blocks of a chunk: eight for each wavefront of a workgroup, fewer where that leaves compute units idle.
+  s.blocks = kWaves * (int)std::max<int64_t>(1, std::min<int64_t>(8, all / (kWaves * 1024)));
+  hipStream_t q = (hipStream_t)stream;
+  unsigned chunks = 0;
+  auto launch = [&] {
+    if (s.entries) hipLaunchKernelGGL(kernel, dim3(chunks), dim3(kThreads), 0, q, s);
+    s.entries = 0;
+    chunks = 0;
+  };
+  for (int64_t i = 0; i < a->n_tensors; ++i) {
+    const cgtp_adamw_tensor& t = a->tensors[i];
+    if (t.n == 0) continue;
+    // a grid has fewer than 2^32 threads
+    const unsigned each = (unsigned)((t.n + kBlock * s.blocks - 1) / (kBlock * s.blocks));
+    if (s.entries == kAtOnce || chunks + each >= (1u << 24)) launch();
+    s.entry[s.entries++] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.master, t.step,
+                            (unsigned)t.n, chunks, (unsigned)t.number};
+    chunks += each;
+  }
+  launch();
+  CountArgs c;
+  for (int64_t i = 0; i < a->n_tensors;) {
+    for (c.n = 0; c.n < kSteps && i < a->n_tensors; ++i) c.step[c.n++] = a->tensors[i].step;
+    hipLaunchKernelGGL(adamw_count_kernel, dim3(1), dim3(kSteps), 0, q, c);
+  }
+  return launch_status();
+}
+
+}  // extern "C"

@@ -1,6 +1,6 @@
 // Autograd nodes of the operators on invariant node features over the C ABI: embedding of node kinds, attention among the nodes of
 // a structure, gated feed-forward block, norm after a residual's addition, cross
-// entropy over kinds.  Operands are checked by the Python layer, which also holds the same launches
+// entropy over kinds; and the AdamW step.  Operands are checked by the Python layer, which also holds the same launches
 // through ctypes for when this extension is not there; a backward under gradient mode hands over to a Python callable.
 #pragma once
 
@@ -471,7 +471,87 @@ struct KindLoss : torch::autograd::Function<KindLoss> {
   }
 };
 
+// ---- AdamW step -------------------------------------------------------------------------------------------------------------
+// The step of a group of parameters where every operand is as the kernels take it.  False, with nothing launched, where one is
+// not (a state that is not there yet, another layout or type): the Python layer then makes, copies or refuses.  `args`: the
+// address of a cgtp_adamw_args with the group's numbers.
+bool adamw_step(const py::list& params, const py::dict& states, bool master, const c10::optional<at::Tensor>& lr, int64_t args, int64_t number) {
+  static PyObject* const names[] = {PyUnicode_InternFromString("exp_avg"), PyUnicode_InternFromString("exp_avg_sq"),
+                                    PyUnicode_InternFromString("root_avg_sq"), PyUnicode_InternFromString("exp_avg_scale"),
+                                    PyUnicode_InternFromString("root_avg_sq_scale"), PyUnicode_InternFromString("master"),
+                                    PyUnicode_InternFromString("step")};
+  enum { kAvg, kSq, kRoot, kAvgScale, kRootScale, kMaster, kStep };
+  cgtp_adamw_args a = *(const cgtp_adamw_args*)args;
+  const bool eight = a.state_bits == 8;
+  std::vector<cgtp_adamw_tensor> tensors;
+  std::vector<at::Tensor> stepped;
+  tensors.reserve(params.size());
+  stepped.reserve(params.size());
+  at::Tensor like;
+  int64_t i = number - 1;
+  for (py::handle h : params) {
+    ++i;
+    if (!THPVariable_Check(h.ptr())) return false;
+    const at::Tensor& p = THPVariable_Unpack(h.ptr());
+    const at::Tensor& g = p.grad();
+    if (!g.defined()) continue;
+    if (!like.defined()) {
+      like = p;
+      const auto type = p.scalar_type();
+      if (!p.is_cuda() || (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf)) return false;
+      if (lr.has_value() && lr->device() != p.device()) return false;
+      a.dtype = code_of(p);
+      a.master = master && type != at::kFloat;
+    }
+    if (p.scalar_type() != like.scalar_type() || p.device() != like.device() || !p.is_contiguous() || p.numel() >= (int64_t)1 << 31) return false;
+    if (g.layout() != at::kStrided || g.scalar_type() != p.scalar_type() || g.device() != p.device() || !g.is_contiguous() ||
+        g.sizes() != p.sizes())
+      return false;
+    PyObject* const state = PyDict_GetItemWithError(states.ptr(), h.ptr());
+    if (!state || !PyDict_Check(state)) {
+      if (PyErr_Occurred()) throw py::error_already_set();
+      return false;
+    }
+    bool good = true;
+    auto pointer = [&](int name, at::ScalarType type, at::IntArrayRef shape) -> void* {
+      PyObject* const o = PyDict_GetItemWithError(state, names[name]);
+      if (!o && PyErr_Occurred()) throw py::error_already_set();
+      if (!o || !THPVariable_Check(o)) return good = false, nullptr;
+      const at::Tensor& t = THPVariable_Unpack(o);
+      if (t.layout() != at::kStrided || t.scalar_type() != type || t.device() != p.device() || t.sizes() != shape || !t.is_contiguous())
+        return good = false, nullptr;
+      return t.data_ptr();
+    };
+    cgtp_adamw_tensor t{};
+    t.n = p.numel();
+    t.number = i;
+    const int64_t blocks[] = {(t.n + CGTP_ADAMW_BLOCK - 1) / CGTP_ADAMW_BLOCK};
+    const auto wide = eight ? at::kFloat8_e4m3fn : at::kFloat;
+    t.param = p.data_ptr();
+    t.grad = g.data_ptr();
+    t.exp_avg = pointer(kAvg, wide, p.sizes());
+    t.exp_avg_sq = pointer(eight ? kRoot : kSq, wide, p.sizes());
+    if (eight) {
+      t.exp_avg_scale = (float*)pointer(kAvgScale, at::kFloat, blocks);
+      t.exp_avg_sq_scale = (float*)pointer(kRootScale, at::kFloat, blocks);
+    }
+    if (a.master) t.master = (float*)pointer(kMaster, at::kFloat, p.sizes());
+    t.step = (float*)pointer(kStep, at::kFloat, {});
+    if (!good) return false;
+    tensors.push_back(t);
+    stepped.push_back(p);
+  }
+  if (tensors.empty()) return true;
+  a.tensors = tensors.data();
+  a.n_tensors = (int64_t)tensors.size();
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(like.device());
+  check_status(cgtp_adamw_step(&a, current_stream(like)), "cgtp_adamw_step");
+  for (const at::Tensor& p : stepped) p.unsafeGetTensorImpl()->bump_version();
+  return true;
+}
+
 void bind_node_operators(py::module& m) {
+  m.def("adamw", &adamw_step, "AdamW step of a group of parameters; false where an operand is not as the kernels take it");
   m.def("kind_loss", [](const at::Tensor& x, const at::Tensor& table, const at::Tensor& kind, double scale, double cap, bool keep,
                         const Fallback& fallback) {
     if (keep) return KindLoss::apply(x, table, kind, scale, cap, &fallback);

@@ -724,9 +724,19 @@ int cgtp_abi_layout(int which, int64_t* out, int capacity) {
                                            CGTP_OFF(cgtp_kind_loss_args, n_kinds), CGTP_OFF(cgtp_kind_loss_args, channels),
                                            CGTP_OFF(cgtp_kind_loss_args, dtype), CGTP_OFF(cgtp_kind_loss_args, scale),
                                            CGTP_OFF(cgtp_kind_loss_args, cap)};
+  static const int64_t adamw_tensor[] = {sizeof(cgtp_adamw_tensor), CGTP_OFF(cgtp_adamw_tensor, param), CGTP_OFF(cgtp_adamw_tensor, grad), CGTP_OFF(cgtp_adamw_tensor, exp_avg),
+      CGTP_OFF(cgtp_adamw_tensor, exp_avg_sq), CGTP_OFF(cgtp_adamw_tensor, exp_avg_scale), CGTP_OFF(cgtp_adamw_tensor, exp_avg_sq_scale),
+      CGTP_OFF(cgtp_adamw_tensor, master), CGTP_OFF(cgtp_adamw_tensor, step), CGTP_OFF(cgtp_adamw_tensor, n),
+      CGTP_OFF(cgtp_adamw_tensor, number)};
+  static const int64_t adamw_args[] = {sizeof(cgtp_adamw_args), CGTP_OFF(cgtp_adamw_args, tensors), CGTP_OFF(cgtp_adamw_args, n_tensors), CGTP_OFF(cgtp_adamw_args, lr_ptr),
+      CGTP_OFF(cgtp_adamw_args, lr), CGTP_OFF(cgtp_adamw_args, beta1), CGTP_OFF(cgtp_adamw_args, beta2),
+      CGTP_OFF(cgtp_adamw_args, eps), CGTP_OFF(cgtp_adamw_args, weight_decay), CGTP_OFF(cgtp_adamw_args, dtype),
+      CGTP_OFF(cgtp_adamw_args, state_bits), CGTP_OFF(cgtp_adamw_args, master), CGTP_OFF(cgtp_adamw_args, maximize),
+      CGTP_OFF(cgtp_adamw_args, seed), CGTP_OFF(cgtp_adamw_args, reserved_)};
 #undef CGTP_OFF
   const int64_t* tabs[] = {operand, tri, gen_operand, gen, uvu, uvt_item, uvt, uvt_gw, uvt_gy, uvu_tab, psw_table,
-                           psw_args, uvu_mx, uvl_args, uvg_args, uvl_gw_args, nullptr, gff_args, attn_args, attn_item, add_rms_args, kind_loss_args};
+                           psw_args, uvu_mx, uvl_args, uvg_args, uvl_gw_args, nullptr, gff_args, attn_args, attn_item, add_rms_args, kind_loss_args,
+                           adamw_tensor, adamw_args};
   const int counts[] = {(int)(sizeof(operand) / 8), (int)(sizeof(tri) / 8), (int)(sizeof(gen_operand) / 8),
                         (int)(sizeof(gen) / 8), (int)(sizeof(uvu) / 8), (int)(sizeof(uvt_item) / 8),
                         (int)(sizeof(uvt) / 8), (int)(sizeof(uvt_gw) / 8), (int)(sizeof(uvt_gy) / 8),
@@ -734,8 +744,8 @@ int cgtp_abi_layout(int which, int64_t* out, int capacity) {
                         (int)(sizeof(uvl_args) / 8), (int)(sizeof(uvg_args) / 8),
                         (int)(sizeof(uvl_gw_args) / 8), 0, (int)(sizeof(gff_args) / 8),
                         (int)(sizeof(attn_args) / 8), (int)(sizeof(attn_item) / 8), (int)(sizeof(add_rms_args) / 8),
-                        (int)(sizeof(kind_loss_args) / 8)};
-  if (which < 0 || which > CGTP_LAYOUT_KIND_LOSS_ARGS || !tabs[which]) return -1;
+                        (int)(sizeof(kind_loss_args) / 8), (int)(sizeof(adamw_tensor) / 8), (int)(sizeof(adamw_args) / 8)};
+  if (which < 0 || which > CGTP_LAYOUT_ADAMW_ARGS || !tabs[which]) return -1;
   for (int i = 0; out && i < counts[which] && i < capacity; ++i) out[i] = tabs[which][i];
   return counts[which];
 }

@@ -44,7 +44,7 @@ enum { CGTP_LAYOUT_OPERAND = 0, CGTP_LAYOUT_TRI_ARGS = 1, CGTP_LAYOUT_GEN_OPERAN
        CGTP_LAYOUT_UVU_ARGS = 4, CGTP_LAYOUT_UVT_ITEM = 5, CGTP_LAYOUT_UVT_ARGS = 6, CGTP_LAYOUT_UVT_GW_ARGS = 7,
        CGTP_LAYOUT_UVT_GY_ARGS = 8, CGTP_LAYOUT_UVU_TABLE = 9, CGTP_LAYOUT_PSW_TABLE = 10, CGTP_LAYOUT_PSW_ARGS = 11,
        CGTP_LAYOUT_GFF_ARGS = 17, CGTP_LAYOUT_ATTN_ARGS = 18, CGTP_LAYOUT_ATTN_ITEM = 19, CGTP_LAYOUT_ADD_RMS_ARGS = 20,
-       CGTP_LAYOUT_KIND_LOSS_ARGS = 21 };   /* 16: none */
+       CGTP_LAYOUT_KIND_LOSS_ARGS = 21, CGTP_LAYOUT_ADAMW_TENSOR = 22, CGTP_LAYOUT_ADAMW_ARGS = 23 };   /* 16: none */
 int cgtp_abi_layout(int which, int64_t* out, int capacity);
 
 /* ---- generic sparse trilinear contraction -------------------------------------------------------------
@@ -899,6 +899,39 @@ typedef struct {
 int64_t cgtp_kind_loss_workspace_bytes(const cgtp_kind_loss_args* args, int backward);
 int cgtp_kind_loss_forward(const cgtp_kind_loss_args* args, void* stream);
 int cgtp_kind_loss_backward(const cgtp_kind_loss_args* args, void* stream);
+
+/* ---- AdamW step over many tensors ------------------------------------------------------------------------------------
+ * t = *step + 1 of each tensor, g its gradient (its negative: maximize):
+ *   m <- beta1 m + (1 - beta1) g,  v <- beta2 v + (1 - beta2) g^2,
+ *   p <- p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps),  *step <- t
+ * tensors: HOST array, read before the call returns.  n elements one after the other (any order that all of a tensor's
+ * arrays share): param and grad of dtype; master (fp32, where args->master: the step is taken on it and param receives it rounded;
+ * 16-bit types only); step: one fp32 number in device memory, the tensor's own.  Elements may lie anywhere an element may.
+ * state_bits 32: exp_avg (m) and exp_avg_sq (v) fp32.  8: exp_avg (m) and exp_avg_sq (sqrt(v)) one byte an element in e4m3, times exp_avg_scale and
+ * exp_avg_sq_scale, fp32, one for each CGTP_ADAMW_BLOCK elements: the block's largest magnitude / 448.  m is rounded to nearest, sqrt(v) up
+ * or down in proportion by 20 random bits, a hash of seed, number, t and the element's place, and not to zero from above it;
+ * a block with an infinity or a NaN becomes NaN.  p is computed from m and v before they are rounded.
+ * lr_ptr: lr in device memory (fp32), read when the kernels run; NULL: lr.  0 <= beta < 1 and known state_bits, else CGTP_ERR_CONFIG.
+ * n < 2^31.  Arrays of different tensors may not overlap.  dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16, of all tensors.
+ */
+enum { CGTP_ADAMW_BLOCK = 256 };
+typedef struct {
+  void* param;
+  const void* grad;
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale, *master, *step;
+  int64_t n, number;
+} cgtp_adamw_tensor;
+typedef struct {
+  const cgtp_adamw_tensor* tensors;
+  int64_t n_tensors;
+  const float* lr_ptr;
+  double lr, beta1, beta2, eps, weight_decay;
+  int32_t dtype, state_bits, master, maximize;
+  uint32_t seed;
+  int32_t reserved_;
+} cgtp_adamw_args;
+int cgtp_adamw_step(const cgtp_adamw_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -6,12 +6,12 @@ import pytest
 import torch
 
 from equitorch_amd import _lib
-from equitorch_amd._lib import AddRmsArgs, CgtpError, KindLossArgs
+from equitorch_amd._lib import AdamwArgs, AdamwTensor, AddRmsArgs, CgtpError, KindLossArgs
 
 NULL, SHAPE, ALIGN, DTYPE, CONFIG, WORKSPACE = 1, 2, 3, 4, 5, 8
 
 
-@pytest.mark.parametrize("which,cls", [(20, AddRmsArgs), (21, KindLossArgs)])
+@pytest.mark.parametrize("which,cls", [(20, AddRmsArgs), (21, KindLossArgs), (22, AdamwTensor), (23, AdamwArgs)])
 def test_struct_layouts(which, cls):
     n = _lib.lib.cgtp_abi_layout(which, None, 0)
     assert n == 1 + len(cls._fields_)
@@ -130,3 +130,47 @@ def test_kind_cross_entropy_layer():
     for make in (lambda: en.KindCrossEntropy(0, 4), lambda: en.KindCrossEntropy(4, 0), lambda: en.KindCrossEntropy(4, 4, cap=0.0)):
         with pytest.raises(ValueError):
             make()
+
+
+# ---- AdamW ---------------------------------------------------------------------------------------------------------
+def _adamw(tensor=None, **changed):
+    t = (AdamwTensor * 1)()
+    for name in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master", "step"):
+        setattr(t[0], name, 4096)
+    t[0].n = 10
+    for name, value in (tensor or {}).items():
+        setattr(t[0], name, value)
+    a = AdamwArgs()
+    a.tensors, a.n_tensors, a.beta1, a.beta2, a.state_bits = t, 1, 0.9, 0.999, 32
+    for name, value in changed.items():
+        setattr(a, name, value)
+    return a, t
+
+
+@pytest.mark.parametrize("tensor,changed,status", [
+    ({}, {"dtype": 1}, DTYPE), ({}, {"state_bits": 16}, CONFIG), ({}, {"n_tensors": -1}, SHAPE), ({}, {"beta1": 1.0}, CONFIG), ({}, {"beta2": -0.1}, CONFIG),
+    ({}, {"beta1": float("nan")}, CONFIG), ({}, {"tensors": None}, NULL), ({"n": -1}, {}, SHAPE), ({"n": 1 << 31}, {}, SHAPE), ({"param": None}, {}, NULL),
+    ({"grad": None}, {}, NULL), ({"exp_avg": None}, {}, NULL), ({"exp_avg_sq": None}, {}, NULL), ({"step": None}, {}, NULL),
+    ({"exp_avg_scale": None}, {"state_bits": 8}, NULL), ({"exp_avg_sq_scale": None}, {"state_bits": 8}, NULL), ({"master": None}, {"master": 1, "dtype": 2}, NULL),
+    ({}, {"master": 1}, CONFIG)])
+def test_adamw_codes(tensor, changed, status):
+    a, _ = _adamw(tensor, **changed)
+    assert _lib.lib.cgtp_adamw_step(C.byref(a), None) == status
+    assert _lib.lib.cgtp_adamw_step(None, None) == NULL
+
+
+def test_adamw_without_work():
+    a, _ = _adamw(n_tensors=0, tensors=None)
+    assert _lib.lib.cgtp_adamw_step(C.byref(a), None) == 0
+
+
+def test_adamw_takes_gpu_tensors_only():
+    from equitorch_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    with pytest.raises(CgtpError):
+        AdamW([p]).step()
+    p.grad = None
+    AdamW([p]).step()
+    with pytest.raises(ValueError):
+        AdamW([p], state_bits=4)
