@@ -13,6 +13,7 @@
 #include "gff_gemm.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cgtp {
 namespace {
@@ -176,7 +177,9 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const T* from, T* to, in
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n * chunks; i += step) {
     const int64_t r = i / chunks;
     const int k = (int)(i - r * chunks) * CH;
-    *reinterpret_cast<u32x4_t*>(to + r * ld + k) = load_part<u32x4_t, T>(from + r * c + k, c - k);
+    u32x4_t v = {0, 0, 0, 0};
+    if (k < c) v = load_part<u32x4_t, T>(from + r * c + k, c - k);
+    *reinterpret_cast<u32x4_t*>(to + r * ld + k) = v;
   }
 }
 
@@ -338,6 +341,253 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_dz_kernel(LogitArgs<T> a
   });
 }
 
+// ---- logits in 16-bit types, up to 512 channels -----------------------------------------------------------------------------
+// A wavefront keeps its rows of x in registers, RB blocks of 32 of them over KS steps of 16 channels, and the table's rows go by
+// in LDS, 32 kinds (a stage) at a time, for all four wavefronts: read twice as seldom as where both operands come from LDS, and
+// the next stage is on its way throughout.  A lane holds one row of x and sixteen neighbouring kinds of a stage: statistics need no
+// exchange before the end, and gradients leave as whole chunks.
+//
+// In LDS a stage is 32 rows of 2 KS chunks, chunk c of row i at c ^ chunk_mix(i): sixteen lanes that read one chunk of
+// neighbouring rows find it in different banks.  Row i is that of kind 16 (i >> 2 & 1) + 4 (i >> 3) + (i & 3): what the matrix
+// instruction gives a lane is then in order.
+constexpr int kStage = 32, kWalkThreads = 256, kWalkGrid = 512, kLeastKinds = 128;      // the grid: two workgroups for each compute unit
+
+template <int KS> struct Walk {
+  static constexpr int RB = KS <= 16 ? 2 : 1, ROWS = 4 * 32 * RB, NC = 2 * KS, PER = kStage * NC / kWalkThreads;
+  static constexpr int BYTES = kStage * NC * 16;
+  __device__ static __forceinline__ int chunk_mix(int i) { return NC % 16 == 0 ? i & 15 : (i >> 1) & 7; }
+};
+
+// How the rows (tiles of them) and the kinds are shared out, by the number of rows with a kind: `splits` ranges of the kinds, so
+// that the tiles' ranges fill the grid some whole number of times.  The host asks for the most there can be.
+struct Share { int tiles, splits, each; };
+__host__ __device__ inline Share share_out(int64_t rows, int rows_of_tile, int64_t kinds) {
+  Share s;
+  s.tiles = (int)((rows + rows_of_tile - 1) / rows_of_tile);
+  if (s.tiles < 1) s.tiles = 1;
+  const int most = (int)((kinds + kLeastKinds - 1) / kLeastKinds), rounds = (s.tiles + kWalkGrid - 1) / kWalkGrid;
+  int64_t best = 0;                // cost of a split: rounds of the grid, and a fiftieth of one for each beyond the fewest
+  s.splits = 0;
+  for (int j = rounds; j < rounds + 4; ++j) {
+    int n = (int)((int64_t)j * kWalkGrid / s.tiles);
+    n = n < most ? n : most;
+    const int64_t cost = 50 * ((s.tiles * (int64_t)n + kWalkGrid - 1) / kWalkGrid) + j - rounds;
+    if (!s.splits || cost * s.splits < best * n) { best = cost; s.splits = n; }
+  }
+  s.each = (int)((kinds + s.splits - 1) / s.splits + kStage - 1) / kStage * kStage;
+  s.splits = (int)((kinds + s.each - 1) / s.each);
+  return s;
+}
+// The most results (a tile's rows for each split) that any number of rows up to `rows` leaves.
+inline int64_t most_results(int64_t rows, int rows_of_tile, int64_t kinds) {
+  const int64_t tiles = std::max<int64_t>(1, ceil_div(rows, rows_of_tile));
+  return rows_of_tile * std::min(tiles * ceil_div(kinds, kLeastKinds), (ceil_div(tiles, kWalkGrid) + 3) * kWalkGrid);
+}
+
+// DZ: the gradients of a piece, else statistics, stats[(tile * splits + split) * ROWS + row].
+template <typename T, int KS, bool DZ, bool CAP>
+__global__ void __launch_bounds__(kWalkThreads, 2) loss_walk_kernel(LogitArgs<T> a) {
+  typedef Walk<KS> W;
+  constexpr int RB = W::RB;
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  __shared__ alignas(16) char lds[2][W::BYTES];
+  const int64_t all = *a.count, rows = DZ ? std::min(all, a.r0 + a.r_most) : all;
+  if (rows <= a.r0) return;
+  const Share share = share_out(rows - a.r0, W::ROWS, a.k_end - a.k0);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, li = lane & 31;
+  const float scale = fabsf(a.scale);
+  const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
+  // where this thread's chunks of a stage come from
+  int from_row[W::PER], from_chunk[W::PER];
+#pragma unroll
+  for (int p = 0; p < W::PER; ++p) {
+    const int q = p * kWalkThreads + tid, i = q / W::NC;
+    from_row[p] = 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3);
+    from_chunk[p] = (q % W::NC ^ W::chunk_mix(i)) * 8;
+  }
+  const int read = li * W::NC, mixed = W::chunk_mix(li);
+  for (int64_t item = blockIdx.x; item < (int64_t)share.tiles * share.splits; item += gridDim.x) {
+    const int64_t m0 = a.r0 + item / share.splits * W::ROWS + wave * 32 * RB;
+    const int64_t first = a.k0 + item % share.splits * share.each, end = std::min(first + share.each, a.k_end);
+    const int stages = (int)((end - first + kStage - 1) / kStage);
+    u32x4_t x[RB][KS];
+    int own[RB];
+    float top[RB], sum[RB], lse[RB];
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      const int64_t row = std::min(m0 + 32 * i + li, rows - 1);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        x[i][s] = *reinterpret_cast<const u32x4_t*>(a.x + row * a.ld + (2 * s + half) * 8);
+        x[i][s] ^= flip;
+      }
+      own[i] = a.target[row];
+      if constexpr (DZ) lse[i] = a.lse[row];
+      else top[i] = -INFINITY, sum[i] = 0.f;
+    }
+    u32x4_t next[W::PER];
+    auto fetch = [&](int t) {
+      const int64_t k = first + (int64_t)t * kStage;
+      const T* base = a.table + k * a.ld;
+      const int last = (int)std::min<int64_t>(kStage, a.k_end - k) - 1;       // rows beyond the table: the last one again
+#pragma unroll
+      for (int p = 0; p < W::PER; ++p)
+        next[p] = *reinterpret_cast<const u32x4_t*>(base + (int64_t)std::min(from_row[p], last) * a.ld + from_chunk[p]);
+    };
+    auto store = [&](int t) {
+#pragma unroll
+      for (int p = 0; p < W::PER; ++p) *reinterpret_cast<u32x4_t*>(lds[t & 1] + (p * kWalkThreads + tid) * 16) = next[p];
+    };
+    __syncthreads();               // the item before has read its last stage
+    fetch(0);
+    store(0);
+    if (stages > 1) fetch(1);
+    for (int t = 0; t < stages; ++t) {
+      __syncthreads();             // stage t is there, stage t - 1 has been read
+      if (t + 1 < stages) store(t + 1);
+      if (t + 2 < stages) fetch(t + 2);
+      const char* at = lds[t & 1];
+      f32x16_t acc[RB];
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(at + (read + ((2 * s + half) ^ mixed)) * 16);
+#pragma unroll
+        for (int i = 0; i < RB; ++i) acc[i] = mma_pair<T>(w, x[i][s], acc[i]);
+      }
+      const int64_t k0 = first + (int64_t)t * kStage;
+      const int mine = (int)std::min<int64_t>(end - k0 - 16 * half, 16);      // of this lane's sixteen kinds
+      const bool cut = end - k0 < kStage;
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        const int at_own = (int)std::max<int64_t>(-1, std::min<int64_t>(own[i] - k0 - 16 * half, 16));
+        const bool has_own = at_own >= 0 && at_own < mine;
+        if constexpr (DZ) {
+          float v[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float slope = 1.f, z = acc[i][e];
+            if constexpr (CAP) v[e] = __builtin_amdgcn_exp2f(capped<T>(z, scale, a.cap, slope) - lse[i]);
+            else v[e] = __builtin_amdgcn_exp2f(fmaf(z, scale, -lse[i]));
+            if constexpr (CAP) acc[i][e] = slope;
+          }
+          if (__any(has_own))
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (e == at_own) v[e] -= 1.f;
+          vec8 out[2];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if constexpr (CAP) v[e] *= acc[i][e];
+            out[e >> 3][e & 7] = (T)(kRaise<T> == 1.f ? v[e] : v[e] * kRaise<T>);
+          }
+          if (cut)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (e >= mine) out[e >> 3][e & 7] = T(0);
+          const int64_t row = m0 + 32 * i + li;
+          if (row < rows) {
+            T* to = a.dz + (row - a.r0) * a.ld_dz + (k0 - a.k0) + 16 * half;
+            *reinterpret_cast<vec8*>(to) = out[0];
+            *reinterpret_cast<vec8*>(to + 8) = out[1];
+          }
+        } else {
+          if constexpr (CAP)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float slope;
+              acc[i][e] = capped<T>(acc[i][e], scale, a.cap, slope);
+            }
+          const float factor = CAP ? 1.f : scale;
+          if (__any(has_own))
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (e == at_own && has_own && m0 + 32 * i + li < rows) a.at[m0 + 32 * i + li] = acc[i][e] * factor;
+          if (cut)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (e >= mine) acc[i][e] = -INFINITY;
+          float most = acc[i][0];
+#pragma unroll
+          for (int e = 1; e < 16; ++e) most = fmaxf(most, acc[i][e]);
+          most = most == -INFINITY ? most : most * factor;      // a factor of zero
+          const float now = fmaxf(top[i], most), base = now == -INFINITY ? 0.f : now;
+          float s = sum[i] * __builtin_amdgcn_exp2f(top[i] - base);
+          if (cut) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (e < mine) s += __builtin_amdgcn_exp2f(fmaf(acc[i][e], factor, -base));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(fmaf(acc[i][e], factor, -base));
+          }
+          top[i] = now;
+          sum[i] = s;
+        }
+      }
+    }
+    if constexpr (!DZ) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        const float other = __shfl_xor(top[i], 32), more = __shfl_xor(sum[i], 32);
+        const float now = fmaxf(top[i], other), base = now == -INFINITY ? 0.f : now;
+        const float s = sum[i] * __builtin_amdgcn_exp2f(top[i] - base) + more * __builtin_amdgcn_exp2f(other - base);
+        if (half == 0) a.stats[item * W::ROWS + (wave * RB + i) * 32 + li] = {now, s};
+      }
+    }
+  }
+}
+
+// loss and the logarithm of the sum from the shares' statistics.
+__global__ void __launch_bounds__(256) loss_walk_join_kernel(const float2* stats, const float* at, const int* rows, const int* count, int rows_of_tile,
+                                                             int64_t kinds, float* loss, float* lse) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = *count;
+  if (i >= n) return;
+  const Share share = share_out(n, rows_of_tile, kinds);
+  const float2* mine = stats + i / rows_of_tile * share.splits * rows_of_tile + i % rows_of_tile;
+  float most = -INFINITY;
+  for (int s = 0; s < share.splits; ++s) most = fmaxf(most, mine[(int64_t)s * rows_of_tile].x);
+  const float base = most == -INFINITY ? 0.f : most;
+  float sum = 0.f;
+  for (int s = 0; s < share.splits; ++s) {
+    const float2 v = mine[(int64_t)s * rows_of_tile];
+    sum += v.y * __builtin_amdgcn_exp2f(v.x - base);
+  }
+  const float total = base + __builtin_amdgcn_logf(sum);
+  loss[rows[i]] = (total - at[i]) * kLn2;
+  if (lse) lse[rows[i]] = total;
+}
+
+// Steps of 16 channels of the kernels above for a width, 0: not theirs.
+int walk_steps(int channels, int size) {
+  if (size == 4 || channels > 512) return 0;
+  const int steps = (channels + 15) / 16;
+  for (int s : {4, 8, 12, 16, 24, 32})
+    if (steps <= s) return s;
+  return 0;
+}
+template <bool DZ, typename T>
+void walk_launch(int steps, const LogitArgs<T>& l, unsigned grid, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    auto go = [&](auto ks) {
+      constexpr int KS = decltype(ks)::value;
+      if (l.cap > 0.f) hipLaunchKernelGGL((loss_walk_kernel<T, KS, DZ, true>), dim3(grid), dim3(kWalkThreads), 0, s, l);
+      else hipLaunchKernelGGL((loss_walk_kernel<T, KS, DZ, false>), dim3(grid), dim3(kWalkThreads), 0, s, l);
+    };
+    switch (steps) {
+      case 4: return go(std::integral_constant<int, 4>{});
+      case 8: return go(std::integral_constant<int, 8>{});
+      case 12: return go(std::integral_constant<int, 12>{});
+      case 16: return go(std::integral_constant<int, 16>{});
+      case 24: return go(std::integral_constant<int, 24>{});
+      default: return go(std::integral_constant<int, 32>{});
+    }
+  }
+}
+
 // ---- gradients ----------------------------------------------------------------------------------------------------------
 // Planes of fp32 results, one for each range of k, added up over the launches of a sum (first: it begins).
 template <typename T>
@@ -449,14 +699,16 @@ int loss_check(const cgtp_kind_loss_args* a) {
 
 // What a call's workspace holds, in bytes from its start.
 struct Plan {
-  int ld, splits, each, blocks, dx_splits, dw_splits;
+  int ld, splits, each, blocks, dx_splits, dw_splits, steps, tile_rows;      // steps: of the kernels for 16-bit types, 0: the others
   int64_t row_each, chunk, piece;          // rows of a workgroup of loss_rows_kernel; rows and kinds of dz
   int64_t counts, tops, rows, target, row_g, at, stats, x, xg, table, dz, dx, dw, sums, all;
 };
 Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
   Plan p = {};
   const int64_t size = a->dtype == CGTP_F32 ? 4 : 2, n = a->n_rows, k = a->n_kinds, c = a->channels;
-  p.ld = (int)up_to(c, 16 / size);
+  p.steps = walk_steps(a->channels, (int)size);
+  p.tile_rows = p.steps && p.steps <= 16 ? 256 : 128;
+  p.ld = (int)(p.steps ? 16 * p.steps : up_to(c, 16 / size));
   p.row_each = up_to(std::max<int64_t>(64, ceil_div(n, kRowBlocks)), 64);
   p.blocks = (int)std::max<int64_t>(1, ceil_div(n, p.row_each));
   auto take = [&](int64_t bytes) {
@@ -477,7 +729,7 @@ Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
     p.each = (int)(ceil_div(k_tiles, splits) * kTile);
     p.splits = (int)ceil_div(k, p.each);
     p.at = take(4 * n);
-    p.stats = take(8 * n * p.splits);
+    p.stats = take(8 * (p.steps ? most_results(n, p.tile_rows, k) : n * p.splits));
     return p;
   }
   p.row_g = take(4 * n);
@@ -564,6 +816,13 @@ int loss_forward(const cgtp_kind_loss_args* a, hipStream_t s) {
   l.each = p.each;
   l.stats = (float2*)(ws + p.stats);
   l.at = (float*)(ws + p.at);
+  if (p.steps) {
+    const unsigned grid = (unsigned)std::min<int64_t>(kWalkGrid, most_results(a->n_rows, p.tile_rows, a->n_kinds) / p.tile_rows);
+    walk_launch<false>(p.steps, l, grid, s);
+    hipLaunchKernelGGL(loss_walk_join_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count,
+                       p.tile_rows, a->n_kinds, a->loss, a->lse);
+    return launch_status();
+  }
   hipLaunchKernelGGL(loss_stats_kernel<T>, dim3((unsigned)(ceil_div(a->n_rows, kTile) * p.splits)), dim3(kGemmThreads), 0, s, l);
   hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count, a->n_rows,
                      p.splits, a->loss, a->lse);
@@ -599,7 +858,8 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
       l.k_end = std::min(a->n_kinds, k0 + p.piece);
       d.kinds = l.k_end - k0;
       const int64_t k_tiles = ceil_div(d.kinds, kTile);
-      hipLaunchKernelGGL(loss_dz_kernel<T>, dim3((unsigned)(row_tiles * k_tiles)), dim3(kGemmThreads), 0, s, l);
+      if (p.steps) walk_launch<true>(p.steps, l, (unsigned)std::min<int64_t>(kWalkGrid, most_results(p.chunk, p.tile_rows, d.kinds) / p.tile_rows), s);
+      else hipLaunchKernelGGL(loss_dz_kernel<T>, dim3((unsigned)(row_tiles * k_tiles)), dim3(kGemmThreads), 0, s, l);
       if (a->grad_x) {
         d.b = l.table + k0 * p.ld;
         d.planes = (float*)(ws + p.dx);
