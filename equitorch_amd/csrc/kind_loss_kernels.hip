@@ -198,6 +198,9 @@ struct LogitArgs {
   const float* lse;               // backward, of the rows of the copy
   T* dz;                          // backward: (r_most, ld_dz)
   int64_t ld_dz;
+  float* planes;                  // dx, see kDx
+  int64_t piece;
+  int first;
 };
 
 // Logits in log2 units; slope: 1 - tanh^2.
@@ -347,31 +350,76 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_dz_kernel(LogitArgs<T> a
 // the next stage is on its way throughout.  A lane holds one row of x and sixteen neighbouring kinds of a stage: statistics need no
 // exchange before the end, and gradients leave as whole chunks.
 //
+// The gradients' products, up to 256 channels, are of the same kind.  Where x has a gradient one kernel forms dz and adds up dx: a
+// lane's sixteen kinds of dz are the next product's operand as they lie, and the stage in LDS, read through the transposing
+// loads, the other.  For the table's gradient dz is kept in blocks of 32 rows x 32 kinds in the order in which that product's operand lies in
+// a wavefront (turned over in LDS), so that it comes straight to registers while rows of x go by in LDS.
+//
 // In LDS a stage is 32 rows of 2 KS chunks, chunk c of row i at c ^ chunk_mix(i): sixteen lanes that read one chunk of
-// neighbouring rows find it in different banks.  Row i is that of kind 16 (i >> 2 & 1) + 4 (i >> 3) + (i & 3): what the matrix
-// instruction gives a lane is then in order.
-constexpr int kStage = 32, kWalkThreads = 256, kWalkGrid = 512, kLeastKinds = 128;      // the grid: two workgroups for each compute unit
+// neighbouring rows find it in different banks, and so do the transposing loads, of a pair of chunks of four rows.  Row i is that of kind
+// 16 (i >> 2 & 1) + 4 (i >> 3) + (i & 3): what the matrix instruction gives a lane is then in order.
+constexpr int kStage = 32, kLeastKinds = 128;
+enum { kStats, kDz, kDx };
 
-template <int KS> struct Walk {
-  static constexpr int RB = KS <= 16 ? 2 : 1, ROWS = 4 * 32 * RB, NC = 2 * KS, PER = kStage * NC / kWalkThreads;
-  static constexpr int BYTES = kStage * NC * 16;
-  __device__ static __forceinline__ int chunk_mix(int i) { return NC % 16 == 0 ? i & 15 : (i >> 1) & 7; }
+template <int KS, int MODE> struct Walk {
+  static constexpr int THREADS = 256, RB = KS <= 16 && MODE != kDx ? 2 : 1, ROWS = THREADS / 2 * RB;
+  static constexpr int NC = 2 * KS, PER = kStage * NC / THREADS, BYTES = kStage * NC * 16;
+  static constexpr int BUFFERS = 3 * BYTES <= 80 * 1024 ? 3 : 2;
+  static constexpr bool BLOCKS = KS <= 16 && MODE != kStats;         // dz in blocks, turned over in 2 KB of LDS a wavefront and block of rows
+  static constexpr int LDS = BUFFERS * BYTES + (BLOCKS ? 4 * RB * 2048 : 0);
+  static_assert(PER * THREADS == kStage * NC);
+  __device__ static __forceinline__ int chunk_mix(int i) {
+    return NC % 16 == 0 ? ((i & 7) << 1) | ((i >> 3) & 1) : (((i >> 1) & 3) << 1) | ((i >> 3) & 1);
+  }
 };
+// Four elements of one column for each lane, from four rows that its sixteen lanes' addresses lie in.
+__device__ __forceinline__ u32x2_t read_turned(const char* p) {
+  typedef short v4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4 lds_v4;
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)p));
+}
+// Sixteen bytes for each lane from base + at (base the same in all lanes) to LDS, one lane's after the other's.  As assembly, since
+// the compiler would wait for all that is on its way to LDS before every transposing load from there: what has to be there is what
+// wait_and_meet counts.
+struct LdsSource {
+  u32x4_t words;
+  __device__ __forceinline__ explicit LdsSource(const void* base) {
+    const uint64_t p = (uint64_t)base;
+    words[0] = __builtin_amdgcn_readfirstlane((unsigned)p);
+    words[1] = __builtin_amdgcn_readfirstlane((unsigned)(p >> 32) & 0xffffu);
+    words[2] = kOutside;
+    words[3] = 0x00027000;
+  }
+  __device__ __forceinline__ void load(const char* lds, unsigned at) const {
+    typedef __attribute__((address_space(3))) const char lds_char;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 ::"s"(__builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_char*)lds)), "v"(at), "s"(words) : "memory", "m0");
+  }
+};
+// All of a workgroup's wavefronts have read what they asked of LDS, and all but the last COUNT of each one's accesses to memory are done.
+template <int COUNT>
+__device__ __forceinline__ void wait_and_meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(COUNT) : "memory");
+}
+constexpr int walk_rows(int steps, int mode) { return steps <= 16 && mode != kDx ? 256 : 128; }
+constexpr int walk_grid(int) { return 512; }      // eight wavefronts for each compute unit
 
 // How the rows (tiles of them) and the kinds are shared out, by the number of rows with a kind: `splits` ranges of the kinds, so
 // that the tiles' ranges fill the grid some whole number of times.  The host asks for the most there can be.
 struct Share { int tiles, splits, each; };
-__host__ __device__ inline Share share_out(int64_t rows, int rows_of_tile, int64_t kinds) {
+constexpr int more_rounds(int mode) { return mode == kDx ? 1 : 3; }        // of the grid than the fewest
+__host__ __device__ inline Share share_out(int mode, int64_t rows, int rows_of_tile, int64_t kinds) {
+  const int grid = walk_grid(mode);
   Share s;
   s.tiles = (int)((rows + rows_of_tile - 1) / rows_of_tile);
   if (s.tiles < 1) s.tiles = 1;
-  const int most = (int)((kinds + kLeastKinds - 1) / kLeastKinds), rounds = (s.tiles + kWalkGrid - 1) / kWalkGrid;
+  const int most = (int)((kinds + kLeastKinds - 1) / kLeastKinds), rounds = (s.tiles + grid - 1) / grid;
   int64_t best = 0;                // cost of a split: rounds of the grid, and a fiftieth of one for each beyond the fewest
   s.splits = 0;
-  for (int j = rounds; j < rounds + 4; ++j) {
-    int n = (int)((int64_t)j * kWalkGrid / s.tiles);
+  for (int j = rounds; j <= rounds + more_rounds(mode); ++j) {
+    int n = (int)((int64_t)j * grid / s.tiles);
     n = n < most ? n : most;
-    const int64_t cost = 50 * ((s.tiles * (int64_t)n + kWalkGrid - 1) / kWalkGrid) + j - rounds;
+    const int64_t cost = 50 * ((s.tiles * (int64_t)n + grid - 1) / grid) + j - rounds;
     if (!s.splits || cost * s.splits < best * n) { best = cost; s.splits = n; }
   }
   s.each = (int)((kinds + s.splits - 1) / s.splits + kStage - 1) / kStage * kStage;
@@ -379,39 +427,54 @@ __host__ __device__ inline Share share_out(int64_t rows, int rows_of_tile, int64
   return s;
 }
 // The most results (a tile's rows for each split) that any number of rows up to `rows` leaves.
-inline int64_t most_results(int64_t rows, int rows_of_tile, int64_t kinds) {
+inline int64_t most_results(int mode, int64_t rows, int rows_of_tile, int64_t kinds) {
   const int64_t tiles = std::max<int64_t>(1, ceil_div(rows, rows_of_tile));
-  return rows_of_tile * std::min(tiles * ceil_div(kinds, kLeastKinds), (ceil_div(tiles, kWalkGrid) + 3) * kWalkGrid);
+  return rows_of_tile * std::min(tiles * ceil_div(kinds, kLeastKinds), (ceil_div(tiles, walk_grid(mode)) + more_rounds(mode)) * walk_grid(mode));
 }
 
-// DZ: the gradients of a piece, else statistics, stats[(tile * splits + split) * ROWS + row].
-template <typename T, int KS, bool DZ, bool CAP>
-__global__ void __launch_bounds__(kWalkThreads, 2) loss_walk_kernel(LogitArgs<T> a) {
-  typedef Walk<KS> W;
-  constexpr int RB = W::RB;
+// kStats: statistics, stats[(tile * splits + split) * ROWS + row].  kDz: the gradients of a piece's logits.  kDx: them too (dz null: not
+// wanted) and planes[(tile * splits + split) * ROWS + row][c] of dx, which `first` begins and other pieces add to.
+template <typename T, int KS, int MODE, bool CAP>
+__global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
+  typedef Walk<KS, MODE> W;
+  constexpr int RB = W::RB, CB = MODE == kDx ? KS / 2 : 1;       // blocks of 32 channels of dx
+  constexpr bool DZ = MODE != kStats;
   typedef T vec8 __attribute__((ext_vector_type(8)));
-  __shared__ alignas(16) char lds[2][W::BYTES];
+  __shared__ alignas(16) char lds[W::LDS];
   const int64_t all = *a.count, rows = DZ ? std::min(all, a.r0 + a.r_most) : all;
   if (rows <= a.r0) return;
-  const Share share = share_out(rows - a.r0, W::ROWS, a.k_end - a.k0);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, li = lane & 31;
+  // pieces whose dx is added up are all shared out alike
+  const Share share = share_out(MODE, rows - a.r0, W::ROWS, MODE == kDx ? a.piece : a.k_end - a.k0);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, li = lane & 31;
   const float scale = fabsf(a.scale);
   const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
-  // where this thread's chunks of a stage come from
-  int from_row[W::PER], from_chunk[W::PER];
+  // this thread's chunks of a stage: the row, bytes from the row's start and from the stage's
+  auto place = [&](int p, int& row, unsigned& chunk) {
+    const int q = p * W::THREADS + tid, i = q / W::NC;
+    row = 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3);
+    chunk = (unsigned)((q % W::NC ^ W::chunk_mix(i)) * 16);
+  };
+  const unsigned row_bytes = (unsigned)(a.ld * sizeof(T));
+  unsigned from[W::PER];
 #pragma unroll
   for (int p = 0; p < W::PER; ++p) {
-    const int q = p * kWalkThreads + tid, i = q / W::NC;
-    from_row[p] = 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3);
-    from_chunk[p] = (q % W::NC ^ W::chunk_mix(i)) * 8;
+    int row;
+    place(p, row, from[p]);
+    from[p] += row * row_bytes;
   }
-  const int read = li * W::NC, mixed = W::chunk_mix(li);
+  // Where a lane reads: chunk c ^ mix of a row is at (place of c = 0) ^ c for the mixed bits of c, plus the others.  q: a row of
+  // four for the transposing loads.
+  constexpr int MIXED = W::NC % 16 == 0 ? 15 : 7;
+  const int q = 4 * half + ((lane & 15) >> 2);
+  const int read_rows = (li * W::NC + (half ^ W::chunk_mix(li))) * 16;
+  const int read_cols = (q * W::NC + ((((lane & 16) >> 3) + ((lane & 3) >> 1)) ^ W::chunk_mix(q))) * 16 + (lane & 1) * 8;
   for (int64_t item = blockIdx.x; item < (int64_t)share.tiles * share.splits; item += gridDim.x) {
     const int64_t m0 = a.r0 + item / share.splits * W::ROWS + wave * 32 * RB;
     const int64_t first = a.k0 + item % share.splits * share.each, end = std::min(first + share.each, a.k_end);
-    const int stages = (int)((end - first + kStage - 1) / kStage);
+    const int kinds = (int)std::max<int64_t>(0, end - first), stages = (kinds + kStage - 1) / kStage;
+    const int have = (int)std::min<int64_t>(32 * RB, rows - m0) - li;            // rows of the wavefront from this lane's on
     u32x4_t x[RB][KS];
-    int own[RB];
+    int own[RB];                   // the row's kind, from this lane's first of a stage on
     float top[RB], sum[RB], lse[RB];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
@@ -421,32 +484,72 @@ __global__ void __launch_bounds__(kWalkThreads, 2) loss_walk_kernel(LogitArgs<T>
         x[i][s] = *reinterpret_cast<const u32x4_t*>(a.x + row * a.ld + (2 * s + half) * 8);
         x[i][s] ^= flip;
       }
-      own[i] = a.target[row];
-      if constexpr (DZ) lse[i] = a.lse[row];
-      else top[i] = -INFINITY, sum[i] = 0.f;
+      own[i] = a.target[row] - (int)first - 16 * half;
+      if constexpr (DZ) {
+        lse[i] = a.lse[row];
+        if (32 * i >= have) {      // no row: its dz is zero
+          lse[i] = INFINITY;
+          own[i] = -(1 << 29);
+        }
+      } else {
+        top[i] = -INFINITY;
+        sum[i] = 0.f;
+      }
     }
-    u32x4_t next[W::PER];
-    auto fetch = [&](int t) {
-      const int64_t k = first + (int64_t)t * kStage;
-      const T* base = a.table + k * a.ld;
-      const int last = (int)std::min<int64_t>(kStage, a.k_end - k) - 1;       // rows beyond the table: the last one again
+    f32x16_t dx[RB][CB];
+    if constexpr (MODE == kDx)
 #pragma unroll
-      for (int p = 0; p < W::PER; ++p)
-        next[p] = *reinterpret_cast<const u32x4_t*>(base + (int64_t)std::min(from_row[p], last) * a.ld + from_chunk[p]);
-    };
-    auto store = [&](int t) {
+      for (int i = 0; i < RB; ++i)
 #pragma unroll
-      for (int p = 0; p < W::PER; ++p) *reinterpret_cast<u32x4_t*>(lds[t & 1] + (p * kWalkThreads + tid) * 16) = next[p];
+        for (int j = 0; j < CB; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) dx[i][j][e] = 0.f;
+    // Stages go from memory to LDS without passing through registers, a wavefront's 64 chunks one after the other.  Three buffers:
+    // stage t + 2 is on its way while t is worked on (two where three do not fit: t + 1).
+    auto fetch = [&](int t, int buffer) {
+      const int64_t k = first + (int64_t)t * kStage, left = a.k_end - k;
+      const LdsSource source(a.table + k * a.ld);
+#pragma unroll
+      for (int p = 0; p < W::PER; ++p) {
+        unsigned at = from[p];
+        if (left < kStage) {       // rows beyond the last kind: that kind's again
+          int row;
+          place(p, row, at);
+          at += std::min<int>(row, (int)left - 1) * row_bytes;
+        }
+        source.load(lds + buffer + (p * W::THREADS + wave * 64) * 16, at);
+      }
     };
-    __syncthreads();               // the item before has read its last stage
-    fetch(0);
-    store(0);
-    if (stages > 1) fetch(1);
+    constexpr int AHEAD = W::BUFFERS - 1;
+    wait_and_meet<0>();            // the item before has read its last stage
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t)
+      if (t < stages) fetch(t, t * W::BYTES);
+    // Where dz goes: blocks (kinds / 32, rows / 32), each in two parts of 64 lanes' sixteen bytes, or rows; what is not there, or not wanted,
+    // beyond the end of the buffer, where it is dropped.
+    unsigned to[RB];
+    const int64_t stage_bytes = W::BLOCKS ? a.ld_dz * 64 : 64;
+    const char* dz_base = nullptr;
+    if constexpr (DZ) {
+      dz_base = (const char*)a.dz + (W::BLOCKS ? (first - a.k0) / kStage * stage_bytes + (m0 - a.r0) * 64
+                                               : ((m0 - a.r0) * a.ld_dz + (first - a.k0)) * (int64_t)sizeof(T));
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        if constexpr (W::BLOCKS) to[i] = a.dz && m0 + 32 * i < rows ? (unsigned)(i * 2048 + lane * 16) : kOutside;
+        else to[i] = a.dz && 32 * i < have ? (unsigned)(((32 * i + li) * a.ld_dz + 16 * half) * (int)sizeof(T)) : kOutside;
+      }
+    }
+    int now_at = 0, next_at = AHEAD * W::BYTES;      // the buffers of stages t and t + AHEAD
     for (int t = 0; t < stages; ++t) {
-      __syncthreads();             // stage t is there, stage t - 1 has been read
-      if (t + 1 < stages) store(t + 1);
-      if (t + 2 < stages) fetch(t + 2);
-      const char* at = lds[t & 1];
+      // stage t is there (at least the PER loads of the next one have been asked for since), stage t - 1 has been read
+      if (AHEAD > 1 && t + 1 < stages) wait_and_meet<W::PER>();
+      else wait_and_meet<0>();
+      if (t + AHEAD < stages) fetch(t + AHEAD, next_at);
+      // places for this stage: not kept over the stages, which would take a register for each
+      int at_rows = read_rows + now_at, at_cols = read_cols + now_at;
+      now_at = now_at == AHEAD * W::BYTES ? 0 : now_at + W::BYTES;
+      next_at = next_at == AHEAD * W::BYTES ? 0 : next_at + W::BYTES;
+      asm volatile("" : "+v"(at_rows), "+v"(at_cols));
       f32x16_t acc[RB];
 #pragma unroll
       for (int i = 0; i < RB; ++i)
@@ -454,47 +557,85 @@ __global__ void __launch_bounds__(kWalkThreads, 2) loss_walk_kernel(LogitArgs<T>
         for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(at + (read + ((2 * s + half) ^ mixed)) * 16);
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(lds + (at_rows ^ ((2 * s & MIXED) << 4)) + ((2 * s & ~MIXED) << 4));
 #pragma unroll
         for (int i = 0; i < RB; ++i) acc[i] = mma_pair<T>(w, x[i][s], acc[i]);
       }
-      const int64_t k0 = first + (int64_t)t * kStage;
-      const int mine = (int)std::min<int64_t>(end - k0 - 16 * half, 16);      // of this lane's sixteen kinds
-      const bool cut = end - k0 < kStage;
+      const int k0 = t * kStage, mine = kinds - k0 - 16 * half;                 // of this lane's sixteen kinds, where not all
+      const bool cut = kinds - k0 < kStage;
+      if constexpr (DZ) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(dz_base + t * stage_bytes), 0, kOutside, 0x00027000);
+        bool some = cut;
 #pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        const int at_own = (int)std::max<int64_t>(-1, std::min<int64_t>(own[i] - k0 - 16 * half, 16));
-        const bool has_own = at_own >= 0 && at_own < mine;
-        if constexpr (DZ) {
-          float v[16];
+        for (int i = 0; i < RB; ++i) some = some || __any((unsigned)(own[i] - k0) < 16u);
+        vec8 out[RB][2];
+        auto gradients = [&](auto odd) {            // odd: a row's own kind is among them, or the kinds end here
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float slope = 1.f, z = acc[i][e];
-            if constexpr (CAP) v[e] = __builtin_amdgcn_exp2f(capped<T>(z, scale, a.cap, slope) - lse[i]);
-            else v[e] = __builtin_amdgcn_exp2f(fmaf(z, scale, -lse[i]));
-            if constexpr (CAP) acc[i][e] = slope;
-          }
-          if (__any(has_own))
+          for (int i = 0; i < RB; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (e == at_own) v[e] -= 1.f;
-          vec8 out[2];
+            for (int e = 0; e < 16; ++e) {
+              const float z = acc[i][e];
+              float slope = 1.f, v;
+              if constexpr (CAP) v = __builtin_amdgcn_exp2f(capped<T>(z, scale, a.cap, slope) - lse[i]);
+              else v = __builtin_amdgcn_exp2f(fmaf(z, scale, -lse[i]));
+              if (decltype(odd)::value && e == own[i] - k0) v -= 1.f;
+              if constexpr (CAP) v *= slope;
+              if constexpr (kRaise<T> != 1.f) v *= kRaise<T>;
+              out[i][e >> 3][e & 7] = (T)(decltype(odd)::value && e >= mine ? 0.f : v);
+            }
+        };
+        if (some) gradients(std::true_type{});
+        else gradients(std::false_type{});
+        if constexpr (W::BLOCKS) {
+          // row li of a block is 64 bytes, chunk c at c ^ (li >> 2 & 3)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            if constexpr (CAP) v[e] *= acc[i][e];
-            out[e >> 3][e & 7] = (T)(kRaise<T> == 1.f ? v[e] : v[e] * kRaise<T>);
-          }
-          if (cut)
+          for (int i = 0; i < RB; ++i) {
+            char* turn = lds + W::BUFFERS * W::BYTES + (wave * RB + i) * 2048;
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (e >= mine) out[e >> 3][e & 7] = T(0);
-          const int64_t row = m0 + 32 * i + li;
-          if (row < rows) {
-            T* to = a.dz + (row - a.r0) * a.ld_dz + (k0 - a.k0) + 16 * half;
-            *reinterpret_cast<vec8*>(to) = out[0];
-            *reinterpret_cast<vec8*>(to + 8) = out[1];
+            for (int s = 0; s < 2; ++s)
+              *reinterpret_cast<vec8*>(turn + li * 64 + (((2 * half + s) ^ ((li >> 2) & 3)) << 4)) = out[i][s];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              u32x4_t f;
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const int r = 16 * s + 8 * half + 4 * u + ((lane & 15) >> 2), c = ((lane & 16) >> 3) + ((lane & 3) >> 1);
+                const u32x2_t v2 = read_turned(turn + r * 64 + ((c ^ ((2 * half + u) & 3)) << 4) + (lane & 1) * 8);
+                f[2 * u] = v2[0];
+                f[2 * u + 1] = v2[1];
+              }
+              __builtin_amdgcn_raw_buffer_store_b128(f, rsrc, to[i] + 1024 * s, 0, 0);
+            }
           }
         } else {
+#pragma unroll
+          for (int i = 0; i < RB; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, out[i][s]), rsrc, to[i] + 16 * s, 0, 0);
+        }
+        // dx^T += W^T dz^T: k = 8 s + .. of this half's kinds are rows 16 s + 4 half + 0 .. 3 and 8 more of the stage
+        if constexpr (MODE == kDx)
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < CB; ++j) {
+              u32x4_t f;
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const u32x2_t v2 = read_turned(lds + (at_cols ^ (((4 * j & MIXED) ^ u) << 4)) + ((4 * j & ~MIXED) << 4) +
+                                               (16 * s + 8 * u) * W::NC * 16);
+                f[2 * u] = v2[0];
+                f[2 * u + 1] = v2[1];
+              }
+#pragma unroll
+              for (int i = 0; i < RB; ++i) dx[i][j] = mma_pair<T>(f, __builtin_bit_cast(u32x4_t, out[i][s]), dx[i][j]);
+            }
+      } else {
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+          const int at_own = own[i] - k0;
+          const bool has_own = (unsigned)at_own < 16u && at_own < mine;
           if constexpr (CAP)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -505,7 +646,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) loss_walk_kernel(LogitArgs<T>
           if (__any(has_own))
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              if (e == at_own && has_own && m0 + 32 * i + li < rows) a.at[m0 + 32 * i + li] = acc[i][e] * factor;
+              if (e == at_own && has_own && 32 * i < have) a.at[m0 + 32 * i + li] = acc[i][e] * factor;
           if (cut)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -538,7 +679,130 @@ __global__ void __launch_bounds__(kWalkThreads, 2) loss_walk_kernel(LogitArgs<T>
         if (half == 0) a.stats[item * W::ROWS + (wave * RB + i) * 32 + li] = {now, s};
       }
     }
+    if constexpr (MODE == kDx) {
+      // as a wavefront holds them: four channels 32 j + 8 g + 4 half + .. of a lane's row, 64 lanes one after the other
+      f32x4* to_plane = reinterpret_cast<f32x4*>(a.planes) + (item * 4 + wave) * (RB * CB * 4 * 64) + lane;
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int j = 0; j < CB; ++j) {
+          f32x4 old[4] = {};
+          if (!a.first)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) old[g] = to_plane[((i * CB + j) * 4 + g) * 64];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) old[g][e] += dx[i][j][4 * g + e];
+            to_plane[((i * CB + j) * 4 + g) * 64] = old[g];
+          }
+        }
+    }
   }
+}
+
+// Planes of the table's gradient: kinds of a piece, 32 to a wavefront, by ranges of the rows; x: the rows of xg from the chunk's first
+// on, a stage of 32 of them at a time in LDS; dz in blocks.  planes[(tile * splits + split) * 4 + wavefront], as a wavefront holds them.
+template <typename T>
+struct TableArgs {
+  const T *x, *dz;
+  float* planes;
+  const int* count;
+  int64_t r0, r_most, kinds;      // rows of the chunk (of dz's blocks), kinds of the piece
+  int ld, splits;
+};
+template <typename T, int KS>
+__global__ void __launch_bounds__(256, 2) loss_table_kernel(TableArgs<T> a) {
+  typedef Walk<KS, kStats> W;
+  constexpr int CB = KS / 2, MIXED = W::NC % 16 == 0 ? 15 : 7, TURN = W::NC % 16 == 0 ? 8 : 4, DEEP = 4;
+  __shared__ alignas(16) char lds[3 * W::BYTES + 4 * DEEP * 2048];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int rows = (int)std::max<int64_t>(0, std::min<int64_t>(*a.count - a.r0, a.r_most));
+  const int all = (rows + kStage - 1) / kStage, each = (all + a.splits - 1) / a.splits, split = blockIdx.x % a.splits;
+  const int begin = split * each, stages = std::max(0, std::min(each, all - begin));
+  const int64_t block = (int64_t)(blockIdx.x / a.splits) * 4 + wave;            // of 32 kinds
+  auto place = [&](int p, int& row, unsigned& chunk) {
+    const int q = p * W::THREADS + tid;
+    row = q / W::NC;
+    chunk = (unsigned)((q % W::NC ^ W::chunk_mix(row)) * 16);
+  };
+  const unsigned row_bytes = (unsigned)(a.ld * sizeof(T));
+  auto fetch = [&](int t, int buffer) {
+    const int first = (begin + t) * kStage, left = rows - first;
+    const LdsSource source(a.x + (int64_t)first * a.ld);
+#pragma unroll
+    for (int p = 0; p < W::PER; ++p) {
+      int row;
+      unsigned at;
+      place(p, row, at);
+      at += std::min(row, left - 1) * row_bytes;            // rows beyond the last: that one again, against zeros of dz
+      source.load(lds + buffer + (p * W::THREADS + wave * 64) * 16, at);
+    }
+  };
+  // blocks beyond the piece's kinds: the last one again, not written
+  const int64_t last = (a.kinds + kStage - 1) / kStage - 1;
+  const char* dz = (const char*)a.dz + std::min(block, last) * (a.r_most * 64) + (int64_t)begin * 2048;
+  const int q = (lane & 15) >> 2, cl = ((lane & 16) >> 3) + ((lane & 3) >> 1);
+  const int read = ((8 * half + q) * W::NC + (cl ^ W::chunk_mix(8 * half + q))) * 16 + (lane & 1) * 8;
+  f32x16_t acc[CB];
+#pragma unroll
+  for (int j = 0; j < CB; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+  // Stages of x are asked for two ahead, blocks of dz, which come from further away, three, into 2 KB a wavefront and stage; in this
+  // order throughout, so that where stage t begins PER + 2 accesses younger than its own may be outstanding.
+  char* const blocks = lds + 3 * W::BYTES + wave * (DEEP * 2048);
+  auto fetch_dz = [&](int t) {
+    const LdsSource source(dz + (int64_t)std::min(t, stages - 1) * 2048);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) source.load(blocks + t % DEEP * 2048 + s * 1024, s * 1024 + lane * 16);
+  };
+  if (stages > 0) {
+    fetch_dz(0);
+    fetch_dz(1);
+    fetch(0, 0);
+    fetch_dz(2);
+    if (stages > 1) fetch(1, W::BYTES);
+  }
+  int now_at = 0, next_at = 2 * W::BYTES;
+  for (int t = 0; t < stages; ++t) {
+    if (t + 1 < stages) wait_and_meet<W::PER + 2>();
+    else wait_and_meet<0>();
+    fetch_dz(t + 3);
+    if (t + 2 < stages) fetch(t + 2, next_at);
+    int at = read + now_at;
+    now_at = now_at == 2 * W::BYTES ? 0 : now_at + W::BYTES;
+    next_at = next_at == 2 * W::BYTES ? 0 : next_at + W::BYTES;
+    asm volatile("" : "+v"(at));
+    const char* mine = blocks + t % DEEP * 2048 + lane * 16;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const u32x4_t now = *reinterpret_cast<const u32x4_t*>(mine + s * 1024);
+#pragma unroll
+      for (int j = 0; j < CB; ++j) {
+        u32x4_t f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const u32x2_t v2 =
+              read_turned(lds + (at ^ (((4 * j & MIXED) ^ (TURN * u)) << 4)) + ((4 * j & ~MIXED) << 4) + (16 * s + 4 * u) * W::NC * 16);
+          f[2 * u] = v2[0];
+          f[2 * u + 1] = v2[1];
+        }
+        acc[j] = mma_pair<T>(f, now, acc[j]);
+      }
+    }
+  }
+  wait_and_meet<0>();              // what was asked for beyond the end
+  f32x4* to_plane = reinterpret_cast<f32x4*>(a.planes) + ((int64_t)blockIdx.x * 4 + wave) * (CB * 4 * 64) + lane;
+#pragma unroll
+  for (int j = 0; j < CB; ++j)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[j][4 * g + e];
+      to_plane[(j * 4 + g) * 64] = v;
+    }
 }
 
 // loss and the logarithm of the sum from the shares' statistics.
@@ -546,7 +810,7 @@ __global__ void __launch_bounds__(256) loss_walk_join_kernel(const float2* stats
                                                              int64_t kinds, float* loss, float* lse) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = *count;
   if (i >= n) return;
-  const Share share = share_out(n, rows_of_tile, kinds);
+  const Share share = share_out(kStats, n, rows_of_tile, kinds);
   const float2* mine = stats + i / rows_of_tile * share.splits * rows_of_tile + i % rows_of_tile;
   float most = -INFINITY;
   for (int s = 0; s < share.splits; ++s) most = fmaxf(most, mine[(int64_t)s * rows_of_tile].x);
@@ -569,13 +833,18 @@ int walk_steps(int channels, int size) {
     if (steps <= s) return s;
   return 0;
 }
-template <bool DZ, typename T>
-void walk_launch(int steps, const LogitArgs<T>& l, unsigned grid, hipStream_t s) {
+template <int MODE, typename T>
+void walk_launch(int steps, const LogitArgs<T>& l, int64_t rows, int64_t kinds, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
+    const int of_tile = walk_rows(steps, MODE);
+    const unsigned grid = (unsigned)std::min<int64_t>(walk_grid(MODE), most_results(MODE, rows, of_tile, kinds) / of_tile);
+    const dim3 threads(256);
     auto go = [&](auto ks) {
       constexpr int KS = decltype(ks)::value;
-      if (l.cap > 0.f) hipLaunchKernelGGL((loss_walk_kernel<T, KS, DZ, true>), dim3(grid), dim3(kWalkThreads), 0, s, l);
-      else hipLaunchKernelGGL((loss_walk_kernel<T, KS, DZ, false>), dim3(grid), dim3(kWalkThreads), 0, s, l);
+      if constexpr (KS <= 16 || MODE != kDx) {
+        if (l.cap > 0.f) hipLaunchKernelGGL((loss_walk_kernel<T, KS, MODE, true>), dim3(grid), threads, 0, s, l);
+        else hipLaunchKernelGGL((loss_walk_kernel<T, KS, MODE, false>), dim3(grid), threads, 0, s, l);
+      }
     };
     switch (steps) {
       case 4: return go(std::integral_constant<int, 4>{});
@@ -669,6 +938,60 @@ __global__ void __launch_bounds__(256) loss_dx_join_kernel(const float* planes, 
   grad_x[(int64_t)rows[r0 + row] * c + (i - row * c)] = (T)(s * (g[r0 + row] * scale));
 }
 
+// The same from the planes of the kernel that forms dz too; steps: of 16 channels.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_walk_dx_kernel(const float* planes, const int* rows, const float* g, const int* count, int64_t r0,
+                                                           int64_t r_most, int64_t piece, int rows_of_tile, int steps, int c, float scale,
+                                                           T* grad_x) {
+  const int64_t n = std::min<int64_t>(*count - r0, r_most);
+  if (n <= 0) return;
+  const Share share = share_out(kDx, n, rows_of_tile, piece);
+  // a thread for four channels of a row, in the order of the planes
+  const int each = rows_of_tile * 16 * steps / 4, part = each / 4, blocks = steps * 2;       // of a tile, a wavefront; of 8 channels
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, tile = i / each;
+  if (tile >= share.tiles) return;
+  const int at = (int)(i - tile * each), wave = at / part, of_wave = at % part, lane = of_wave & 63, block = of_wave >> 6;
+  const int64_t row = tile * rows_of_tile + (wave * (rows_of_tile / 128) + block / blocks) * 32 + (lane & 31);
+  const int ch = block % blocks * 8 + 4 * (lane >> 5), left = c - ch;
+  if (row >= n || left <= 0) return;
+  const f32x4* p = reinterpret_cast<const f32x4*>(planes) + tile * share.splits * each + at;
+  f32x4 s = {};
+  for (int k = 0; k < share.splits; ++k) s += p[(int64_t)k * each];
+  T out[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = (T)(s[e] * (g[r0 + row] * scale));
+  store_part<T, 4>(grad_x + (int64_t)rows[r0 + row] * c + ch, out, left);
+}
+
+// The table's from the planes of loss_table_kernel, over the chunks of rows as below.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_table_join_kernel(const float* planes, int splits, int64_t kinds, int steps, int c, const unsigned* top,
+                                                              float scale, int first, int last, float* sums, T* out) {
+  const int part = 32 * 16 * steps / 4, blocks = steps * 2;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, wave = i / part;
+  const int of_wave = (int)(i - wave * part), lane = of_wave & 63, ch = (of_wave >> 6) % blocks * 8 + 4 * (lane >> 5), left = c - ch;
+  const int64_t kind = wave * 32 + (lane & 31);
+  if (kind >= kinds || left <= 0) return;
+  const f32x4* p = reinterpret_cast<const f32x4*>(planes) + (wave / 4 * splits * 4 + wave % 4) * part + of_wave;
+  f32x4 s = {};
+  for (int k = 0; k < splits; ++k) s += p[(int64_t)k * 4 * part];
+  const int64_t to = kind * c + ch;
+  if (!first)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) s[e] += sums[to + e];
+  if (last) {
+    T v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (T)(s[e] * (__uint_as_float(*top) * scale));
+    store_part<T, 4>(out + to, v, left);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) sums[to + e] = s[e];
+  }
+}
+
 // The planes of a piece's kinds, over the chunks of rows: sums[i] += them, or the result in the last chunk.
 template <typename T>
 __global__ void __launch_bounds__(256) loss_dw_join_kernel(const float* planes, int splits, int64_t elems, const unsigned* top, float scale,
@@ -697,9 +1020,12 @@ int loss_check(const cgtp_kind_loss_args* a) {
   return CGTP_OK;
 }
 
+constexpr int64_t kDzBytes = 256 << 20;
+
 // What a call's workspace holds, in bytes from its start.
 struct Plan {
-  int ld, splits, each, blocks, dx_splits, dw_splits, steps, tile_rows;      // steps: of the kernels for 16-bit types, 0: the others
+  int ld, splits, each, blocks, dx_splits, dw_splits, steps;      // steps: of the kernels for 16-bit types, 0: the others
+  bool blocks_of_dz, fused;                      // dz in blocks of 32 x 32; dz and dx in one kernel
   int64_t row_each, chunk, piece;          // rows of a workgroup of loss_rows_kernel; rows and kinds of dz
   int64_t counts, tops, rows, target, row_g, at, stats, x, xg, table, dz, dx, dw, sums, all;
 };
@@ -707,7 +1033,6 @@ Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
   Plan p = {};
   const int64_t size = a->dtype == CGTP_F32 ? 4 : 2, n = a->n_rows, k = a->n_kinds, c = a->channels;
   p.steps = walk_steps(a->channels, (int)size);
-  p.tile_rows = p.steps && p.steps <= 16 ? 256 : 128;
   p.ld = (int)(p.steps ? 16 * p.steps : up_to(c, 16 / size));
   p.row_each = up_to(std::max<int64_t>(64, ceil_div(n, kRowBlocks)), 64);
   p.blocks = (int)std::max<int64_t>(1, ceil_div(n, p.row_each));
@@ -729,27 +1054,38 @@ Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
     p.each = (int)(ceil_div(k_tiles, splits) * kTile);
     p.splits = (int)ceil_div(k, p.each);
     p.at = take(4 * n);
-    p.stats = take(8 * (p.steps ? most_results(n, p.tile_rows, k) : n * p.splits));
+    p.stats = take(8 * (p.steps ? most_results(kStats, n, walk_rows(p.steps, kStats), k) : n * p.splits));
     return p;
   }
   p.row_g = take(4 * n);
   p.at = take(4 * n);                    // lse of the rows of the copy
   p.xg = a->grad_table ? take(n * p.ld * size) : -1;
-  // dz: up to 64 million values; a piece's planes of up to 128 million
+  // dz: up to kDzBytes, in pieces of about one size; a piece's planes of up to 128 million values
+  p.blocks_of_dz = p.steps && p.steps <= 16;
+  p.fused = p.blocks_of_dz && a->grad_x;
   p.chunk = std::min<int64_t>(up_to(n, kTile), 32768);
-  p.piece = std::min<int64_t>(up_to(k, kTile), std::max<int64_t>(1024, std::min((1 << 26) / p.chunk, (1 << 27) / c) / kTile * kTile));
-  p.dz = take(p.chunk * p.piece * size);
+  const int64_t most = std::max<int64_t>(1024, std::min(kDzBytes / size / p.chunk, (1 << 27) / c) / kTile * kTile);
+  p.piece = up_to(ceil_div(k, ceil_div(k, most)), kTile);
+  if (p.fused && !a->grad_table) p.piece = up_to(k, kTile);      // no dz
+  else p.dz = take(p.chunk * p.piece * size);
   const int64_t tiles_c = ceil_div(c, kTile), depth = 128 / size;
   auto ranges = [&](int64_t tiles, int64_t k_tiles) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, std::max<int64_t>(1, tiles)), k_tiles / 8));
   };
-  if (a->grad_x) {
+  if (p.fused) {
+    p.dx = take(most_results(kDx, p.chunk, walk_rows(p.steps, kDx), p.piece) * p.ld * 4);
+  } else if (a->grad_x) {
     p.dx_splits = ranges(p.chunk / kTile * tiles_c, p.piece / depth);
     p.dx = take(p.dx_splits * p.chunk * c * 4);
   }
   if (a->grad_table) {
-    p.dw_splits = ranges(p.piece / kTile * tiles_c, p.chunk / depth);
-    p.dw = take(p.dw_splits * p.piece * c * 4);
+    if (p.blocks_of_dz) {        // ranges of at least eight stages of rows
+      p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / (p.piece / kTile), p.chunk / kStage / 8));
+      p.dw = take(p.dw_splits * p.piece * p.ld * 4);
+    } else {
+      p.dw_splits = ranges(p.piece / kTile * tiles_c, p.chunk / depth);
+      p.dw = take(p.dw_splits * p.piece * c * 4);
+    }
     if (n > p.chunk) p.sums = take(k * c * 4);
   }
   return p;
@@ -817,10 +1153,9 @@ int loss_forward(const cgtp_kind_loss_args* a, hipStream_t s) {
   l.stats = (float2*)(ws + p.stats);
   l.at = (float*)(ws + p.at);
   if (p.steps) {
-    const unsigned grid = (unsigned)std::min<int64_t>(kWalkGrid, most_results(a->n_rows, p.tile_rows, a->n_kinds) / p.tile_rows);
-    walk_launch<false>(p.steps, l, grid, s);
+    walk_launch<kStats>(p.steps, l, a->n_rows, a->n_kinds, s);
     hipLaunchKernelGGL(loss_walk_join_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count,
-                       p.tile_rows, a->n_kinds, a->loss, a->lse);
+                       walk_rows(p.steps, kStats), a->n_kinds, a->loss, a->lse);
     return launch_status();
   }
   hipLaunchKernelGGL(loss_stats_kernel<T>, dim3((unsigned)(ceil_div(a->n_rows, kTile) * p.splits)), dim3(kGemmThreads), 0, s, l);
@@ -838,8 +1173,10 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
   float* lse = (float*)(ws + p.at);
   hipLaunchKernelGGL(loss_take_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, a->lse, r.rows, r.count, lse);
   l.lse = lse;
-  l.dz = (T*)(ws + p.dz);
-  l.ld_dz = p.piece;
+  l.dz = p.fused && !a->grad_table ? nullptr : (T*)(ws + p.dz);
+  l.planes = (float*)(ws + p.dx);
+  l.piece = p.piece;
+  l.ld_dz = p.blocks_of_dz ? p.chunk : p.piece;
   const int64_t c = a->channels, tiles_c = ceil_div(c, kTile);
   const float scale = a->scale / kRaise<T>;
   ProductArgs<T> d = {};
@@ -858,16 +1195,32 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
       l.k_end = std::min(a->n_kinds, k0 + p.piece);
       d.kinds = l.k_end - k0;
       const int64_t k_tiles = ceil_div(d.kinds, kTile);
-      if (p.steps) walk_launch<true>(p.steps, l, (unsigned)std::min<int64_t>(kWalkGrid, most_results(p.chunk, p.tile_rows, d.kinds) / p.tile_rows), s);
+      l.first = k0 == 0;
+      if (p.fused) walk_launch<kDx>(p.steps, l, p.chunk, p.piece, s);
+      else if (p.steps) walk_launch<kDz>(p.steps, l, p.chunk, d.kinds, s);
       else hipLaunchKernelGGL(loss_dz_kernel<T>, dim3((unsigned)(row_tiles * k_tiles)), dim3(kGemmThreads), 0, s, l);
-      if (a->grad_x) {
+      if (a->grad_x && !p.fused) {
         d.b = l.table + k0 * p.ld;
         d.planes = (float*)(ws + p.dx);
         d.splits = p.dx_splits;
         d.first = k0 == 0;
         hipLaunchKernelGGL(loss_dx_kernel<T>, dim3((unsigned)(row_tiles * tiles_c * d.splits)), dim3(kGemmThreads), 0, s, d);
       }
-      if (a->grad_table) {
+      if (a->grad_table && p.blocks_of_dz) {
+        if constexpr (sizeof(T) == 2) {
+          const TableArgs<T> w = {r.to_g + r0 * p.ld, l.dz, (float*)(ws + p.dw), r.count, r0, p.chunk, d.kinds, p.ld, p.dw_splits};
+          const dim3 grid((unsigned)(k_tiles * w.splits));
+          switch (p.steps) {
+            case 4: hipLaunchKernelGGL((loss_table_kernel<T, 4>), grid, dim3(256), 0, s, w); break;
+            case 8: hipLaunchKernelGGL((loss_table_kernel<T, 8>), grid, dim3(256), 0, s, w); break;
+            case 12: hipLaunchKernelGGL((loss_table_kernel<T, 12>), grid, dim3(256), 0, s, w); break;
+            default: hipLaunchKernelGGL((loss_table_kernel<T, 16>), grid, dim3(256), 0, s, w);
+          }
+          hipLaunchKernelGGL(loss_table_join_kernel<T>, dim3((unsigned)(k_tiles * kTile * p.ld / 4 / 256)), dim3(256), 0, s, w.planes, w.splits,
+                             d.kinds, p.steps, a->channels, r.tops + p.blocks, scale, r0 == 0, last, (float*)(ws + p.sums) + k0 * c,
+                             (T*)a->grad_table + k0 * c);
+        }
+      } else if (a->grad_table) {
         d.b = r.to_g + r0 * p.ld;
         d.planes = (float*)(ws + p.dw);
         d.splits = p.dw_splits;
@@ -876,9 +1229,13 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
                            r.tops + p.blocks, scale, r0 == 0, last, (float*)(ws + p.sums) + k0 * c, (T*)a->grad_table + k0 * c);
       }
     }
-    if (a->grad_x)
-      hipLaunchKernelGGL(loss_dx_join_kernel<T>, dim3((unsigned)ceil_div(std::min(p.chunk, a->n_rows - r0) * c, 256)), dim3(256), 0, s,
-                         (const float*)(ws + p.dx), p.dx_splits, r.rows, r.row_g, r.count, r0, p.chunk, a->channels, scale, (T*)a->grad_x);
+    const int64_t rows_now = std::min(p.chunk, a->n_rows - r0);
+    if (p.fused)
+      hipLaunchKernelGGL(loss_walk_dx_kernel<T>, dim3((unsigned)ceil_div(up_to(rows_now, walk_rows(p.steps, kDx)) * p.ld / 4, 256)), dim3(256), 0, s,
+                         l.planes, r.rows, r.row_g, r.count, r0, p.chunk, p.piece, walk_rows(p.steps, kDx), p.steps, a->channels, scale, (T*)a->grad_x);
+    else if (a->grad_x)
+      hipLaunchKernelGGL(loss_dx_join_kernel<T>, dim3((unsigned)ceil_div(rows_now * c, 256)), dim3(256), 0, s, (const float*)(ws + p.dx), p.dx_splits,
+                         r.rows, r.row_g, r.count, r0, p.chunk, a->channels, scale, (T*)a->grad_x);
   }
   return launch_status();
 }
