@@ -390,12 +390,35 @@ struct LdsSource {
     words[2] = kOutside;
     words[3] = 0x00027000;
   }
-  __device__ __forceinline__ void load(const char* lds, unsigned at) const {
-    typedef __attribute__((address_space(3))) const char lds_char;
+  // to: the place in LDS, the same in all lanes
+  __device__ __forceinline__ void load(unsigned to, unsigned at) const {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 ::"s"(__builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_char*)lds)), "v"(at), "s"(words) : "memory", "m0");
+                 ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(at), "s"(words) : "memory", "m0");
   }
 };
+__device__ __forceinline__ unsigned place_in_lds(const char* p) {
+  typedef __attribute__((address_space(3))) const char lds_char;
+  return (unsigned)(uintptr_t)(lds_char*)p;
+}
+// The chunks of a stage that a thread brings, THREADS / NC rows apart: row << 16 | bytes from the row's start, where row i of LDS is
+// row of(i) of the stage.
+template <typename W, typename Of>
+__device__ __forceinline__ void stage_places(unsigned (&place)[W::PER], Of&& of) {
+#pragma unroll
+  for (int p = 0; p < W::PER; ++p) {
+    const int q = p * W::THREADS + (int)threadIdx.x, i = q / W::NC;
+    place[p] = (unsigned)(of(i) << 16 | (q % W::NC ^ W::chunk_mix(i)) << 4);
+  }
+}
+// Brings a stage whose rows from `left` on are not there: the last one again.
+template <typename W>
+__device__ __forceinline__ void fetch_stage(const void* base, unsigned row_bytes, int left, const unsigned (&place)[W::PER], unsigned to, int wave) {
+  const LdsSource source(base);
+  const unsigned last = (unsigned)std::min(left, kStage) - 1;
+#pragma unroll
+  for (int p = 0; p < W::PER; ++p)
+    source.load(to + (p * W::THREADS + wave * 64) * 16, std::min(place[p] >> 16, last) * row_bytes + (place[p] & 0xffffu));
+}
 // All of a workgroup's wavefronts have read what they asked of LDS, and all but the last COUNT of each one's accesses to memory are done.
 template <int COUNT>
 __device__ __forceinline__ void wait_and_meet() {
@@ -439,6 +462,7 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
   typedef Walk<KS, MODE> W;
   constexpr int RB = W::RB, CB = MODE == kDx ? KS / 2 : 1;       // blocks of 32 channels of dx
   constexpr bool DZ = MODE != kStats;
+  constexpr int AHEAD_READS = 4;
   typedef T vec8 __attribute__((ext_vector_type(8)));
   __shared__ alignas(16) char lds[W::LDS];
   const int64_t all = *a.count, rows = DZ ? std::min(all, a.r0 + a.r_most) : all;
@@ -448,29 +472,22 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, li = lane & 31;
   const float scale = fabsf(a.scale);
   const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
-  // this thread's chunks of a stage: the row, bytes from the row's start and from the stage's
-  auto place = [&](int p, int& row, unsigned& chunk) {
-    const int q = p * W::THREADS + tid, i = q / W::NC;
-    row = 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3);
-    chunk = (unsigned)((q % W::NC ^ W::chunk_mix(i)) * 16);
-  };
-  const unsigned row_bytes = (unsigned)(a.ld * sizeof(T));
-  unsigned from[W::PER];
-#pragma unroll
-  for (int p = 0; p < W::PER; ++p) {
-    int row;
-    place(p, row, from[p]);
-    from[p] += row * row_bytes;
-  }
+  const unsigned row_bytes = (unsigned)(a.ld * sizeof(T)), lds_at = place_in_lds(lds);
+  unsigned place[W::PER];
+  stage_places<W>(place, [](int i) { return 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3); });
   // Where a lane reads: chunk c ^ mix of a row is at (place of c = 0) ^ c for the mixed bits of c, plus the others.  q: a row of
   // four for the transposing loads.
   constexpr int MIXED = W::NC % 16 == 0 ? 15 : 7;
   const int q = 4 * half + ((lane & 15) >> 2);
   const int read_rows = (li * W::NC + (half ^ W::chunk_mix(li))) * 16;
   const int read_cols = (q * W::NC + ((((lane & 16) >> 3) + ((lane & 3) >> 1)) ^ W::chunk_mix(q))) * 16 + (lane & 1) * 8;
-  for (int64_t item = blockIdx.x; item < (int64_t)share.tiles * share.splits; item += gridDim.x) {
-    const int64_t m0 = a.r0 + item / share.splits * W::ROWS + wave * 32 * RB;
-    const int64_t first = a.k0 + item % share.splits * share.each, end = std::min(first + share.each, a.k_end);
+  const int items = __builtin_amdgcn_readfirstlane(share.tiles * share.splits), splits = __builtin_amdgcn_readfirstlane(share.splits),
+            each = __builtin_amdgcn_readfirstlane(share.each);
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    // the same in all lanes, but divided by vector instructions: back to scalar registers
+    const int tile = __builtin_amdgcn_readfirstlane(item / splits), split = item - tile * splits;
+    const int64_t m0 = a.r0 + (int64_t)tile * W::ROWS + wave * 32 * RB;
+    const int64_t first = a.k0 + (int64_t)split * each, end = std::min(first + each, a.k_end);
     const int kinds = (int)std::max<int64_t>(0, end - first), stages = (kinds + kStage - 1) / kStage;
     const int have = (int)std::min<int64_t>(32 * RB, rows - m0) - li;            // rows of the wavefront from this lane's on
     u32x4_t x[RB][KS];
@@ -506,19 +523,10 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
           for (int e = 0; e < 16; ++e) dx[i][j][e] = 0.f;
     // Stages go from memory to LDS without passing through registers, a wavefront's 64 chunks one after the other.  Three buffers:
     // stage t + 2 is on its way while t is worked on (two where three do not fit: t + 1).
+    const int left_of_all = (int)(a.k_end - first);
+    const char* table = (const char*)(a.table + first * a.ld);
     auto fetch = [&](int t, int buffer) {
-      const int64_t k = first + (int64_t)t * kStage, left = a.k_end - k;
-      const LdsSource source(a.table + k * a.ld);
-#pragma unroll
-      for (int p = 0; p < W::PER; ++p) {
-        unsigned at = from[p];
-        if (left < kStage) {       // rows beyond the last kind: that kind's again
-          int row;
-          place(p, row, at);
-          at += std::min<int>(row, (int)left - 1) * row_bytes;
-        }
-        source.load(lds + buffer + (p * W::THREADS + wave * 64) * 16, at);
-      }
+      fetch_stage<W>(table + (int64_t)t * kStage * row_bytes, row_bytes, left_of_all - t * kStage, place, lds_at + buffer, wave);
     };
     constexpr int AHEAD = W::BUFFERS - 1;
     wait_and_meet<0>();            // the item before has read its last stage
@@ -561,6 +569,15 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
 #pragma unroll
         for (int i = 0; i < RB; ++i) acc[i] = mma_pair<T>(w, x[i][s], acc[i]);
       }
+      if constexpr (MODE == kDx) {
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD_READS, 0);
+#pragma unroll
+        for (int s = 0; s < KS - AHEAD_READS; ++s) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, AHEAD_READS, 0);
+      }
       const int k0 = t * kStage, mine = kinds - k0 - 16 * half;                 // of this lane's sixteen kinds, where not all
       const bool cut = kinds - k0 < kStage;
       if constexpr (DZ) {
@@ -573,15 +590,23 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
 #pragma unroll
           for (int i = 0; i < RB; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float z = acc[i][e];
-              float slope = 1.f, v;
-              if constexpr (CAP) v = __builtin_amdgcn_exp2f(capped<T>(z, scale, a.cap, slope) - lse[i]);
-              else v = __builtin_amdgcn_exp2f(fmaf(z, scale, -lse[i]));
-              if (decltype(odd)::value && e == own[i] - k0) v -= 1.f;
-              if constexpr (CAP) v *= slope;
-              if constexpr (kRaise<T> != 1.f) v *= kRaise<T>;
-              out[i][e >> 3][e & 7] = (T)(decltype(odd)::value && e >= mine ? 0.f : v);
+            for (int e = 0; e < 16; e += 2) {
+              f32x2 v;
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float z = acc[i][e + k];
+                float slope = 1.f;
+                if constexpr (CAP) v[k] = __builtin_amdgcn_exp2f(capped<T>(z, scale, a.cap, slope) - lse[i]);
+                else v[k] = __builtin_amdgcn_exp2f(fmaf(z, scale, -lse[i]));
+                if (decltype(odd)::value && e + k == own[i] - k0) v[k] -= 1.f;
+                if constexpr (CAP) v[k] *= slope;
+                if constexpr (kRaise<T> != 1.f) v[k] *= kRaise<T>;
+                if (decltype(odd)::value && e + k >= mine) v[k] = 0.f;
+              }
+              typedef T vec2 __attribute__((ext_vector_type(2)));
+              const vec2 r = __builtin_convertvector(v, vec2);
+              out[i][e >> 3][e & 7] = r[0];
+              out[i][e >> 3][(e & 7) + 1] = r[1];
             }
         };
         if (some) gradients(std::true_type{});
@@ -631,6 +656,15 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
 #pragma unroll
               for (int i = 0; i < RB; ++i) dx[i][j] = mma_pair<T>(f, __builtin_bit_cast(u32x4_t, out[i][s]), dx[i][j]);
             }
+        if constexpr (MODE == kDx) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD_READS, 1);
+#pragma unroll
+          for (int s = 0; s < 2 * CB - AHEAD_READS; ++s) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x8, AHEAD_READS, 1);
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < RB; ++i) {
@@ -676,12 +710,12 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
         const float other = __shfl_xor(top[i], 32), more = __shfl_xor(sum[i], 32);
         const float now = fmaxf(top[i], other), base = now == -INFINITY ? 0.f : now;
         const float s = sum[i] * __builtin_amdgcn_exp2f(top[i] - base) + more * __builtin_amdgcn_exp2f(other - base);
-        if (half == 0) a.stats[item * W::ROWS + (wave * RB + i) * 32 + li] = {now, s};
+        if (half == 0) a.stats[(int64_t)item * W::ROWS + (wave * RB + i) * 32 + li] = {now, s};
       }
     }
     if constexpr (MODE == kDx) {
       // as a wavefront holds them: four channels 32 j + 8 g + 4 half + .. of a lane's row, 64 lanes one after the other
-      f32x4* to_plane = reinterpret_cast<f32x4*>(a.planes) + (item * 4 + wave) * (RB * CB * 4 * 64) + lane;
+      f32x4* to_plane = reinterpret_cast<f32x4*>(a.planes) + ((int64_t)item * 4 + wave) * (RB * CB * 4 * 64) + lane;
 #pragma unroll
       for (int i = 0; i < RB; ++i)
 #pragma unroll
@@ -701,8 +735,10 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
   }
 }
 
-// Planes of the table's gradient: kinds of a piece, 32 to a wavefront, by ranges of the rows; x: the rows of xg from the chunk's first
-// on, a stage of 32 of them at a time in LDS; dz in blocks.  planes[(tile * splits + split) * 4 + wavefront], as a wavefront holds them.
+// Planes of the table's gradient: 128 kinds of a piece to a workgroup, by ranges of the rows; x: the rows of xg from the chunk's first
+// on, a stage of 32 of them at a time in LDS, and with it the stage's blocks of dz.  A wavefront has 64 kinds and half the channels, so that
+// three quarters of an operand are read from LDS for each product, where 32 kinds and all channels take nine eighths.
+// planes[(tile * splits + split) * 4 + wavefront], as a wavefront holds them.
 template <typename T>
 struct TableArgs {
   const T *x, *dz;
@@ -714,48 +750,40 @@ struct TableArgs {
 template <typename T, int KS>
 __global__ void __launch_bounds__(256, 2) loss_table_kernel(TableArgs<T> a) {
   typedef Walk<KS, kStats> W;
-  constexpr int CB = KS / 2, MIXED = W::NC % 16 == 0 ? 15 : 7, TURN = W::NC % 16 == 0 ? 8 : 4, DEEP = 4;
+  constexpr int CB = KS / 4, MIXED = W::NC % 16 == 0 ? 15 : 7, TURN = W::NC % 16 == 0 ? 8 : 4, DEEP = 4;
   __shared__ alignas(16) char lds[3 * W::BYTES + 4 * DEEP * 2048];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int rows = (int)std::max<int64_t>(0, std::min<int64_t>(*a.count - a.r0, a.r_most));
   const int all = (rows + kStage - 1) / kStage, each = (all + a.splits - 1) / a.splits, split = blockIdx.x % a.splits;
   const int begin = split * each, stages = std::max(0, std::min(each, all - begin));
-  const int64_t block = (int64_t)(blockIdx.x / a.splits) * 4 + wave;            // of 32 kinds
-  auto place = [&](int p, int& row, unsigned& chunk) {
-    const int q = p * W::THREADS + tid;
-    row = q / W::NC;
-    chunk = (unsigned)((q % W::NC ^ W::chunk_mix(row)) * 16);
-  };
-  const unsigned row_bytes = (unsigned)(a.ld * sizeof(T));
-  auto fetch = [&](int t, int buffer) {
-    const int first = (begin + t) * kStage, left = rows - first;
-    const LdsSource source(a.x + (int64_t)first * a.ld);
-#pragma unroll
-    for (int p = 0; p < W::PER; ++p) {
-      int row;
-      unsigned at;
-      place(p, row, at);
-      at += std::min(row, left - 1) * row_bytes;            // rows beyond the last: that one again, against zeros of dz
-      source.load(lds + buffer + (p * W::THREADS + wave * 64) * 16, at);
-    }
+  const int64_t block = (int64_t)(blockIdx.x / a.splits) * 4 + wave;            // of 32 kinds, which this wavefront brings
+  const unsigned row_bytes = (unsigned)(a.ld * sizeof(T)), lds_at = place_in_lds(lds);
+  unsigned place[W::PER];
+  stage_places<W>(place, [](int i) { return i; });
+  auto fetch = [&](int t, int buffer) {            // rows beyond the last: that one again, against zeros of dz
+    const int first = (begin + t) * kStage;
+    fetch_stage<W>(a.x + (int64_t)first * a.ld, row_bytes, rows - first, place, lds_at + buffer, wave);
   };
   // blocks beyond the piece's kinds: the last one again, not written
   const int64_t last = (a.kinds + kStage - 1) / kStage - 1;
   const char* dz = (const char*)a.dz + std::min(block, last) * (a.r_most * 64) + (int64_t)begin * 2048;
   const int q = (lane & 15) >> 2, cl = ((lane & 16) >> 3) + ((lane & 3) >> 1);
-  const int read = ((8 * half + q) * W::NC + (cl ^ W::chunk_mix(8 * half + q))) * 16 + (lane & 1) * 8;
-  f32x16_t acc[CB];
+  // chunks of this half of the channels: 4 (j + CB * part) ^ .., the part's bits among the mixed ones or above them
+  const int part = wave & 1, from = 4 * CB * part, pair = wave >> 1;
+  const int read = ((8 * half + q) * W::NC + ((cl ^ W::chunk_mix(8 * half + q)))) * 16 + (lane & 1) * 8;
+  f32x16_t acc[2][CB];
 #pragma unroll
-  for (int j = 0; j < CB; ++j)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+    for (int j = 0; j < CB; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   // Stages of x are asked for two ahead, blocks of dz, which come from further away, three, into 2 KB a wavefront and stage; in this
   // order throughout, so that where stage t begins PER + 2 accesses younger than its own may be outstanding.
-  char* const blocks = lds + 3 * W::BYTES + wave * (DEEP * 2048);
   auto fetch_dz = [&](int t) {
     const LdsSource source(dz + (int64_t)std::min(t, stages - 1) * 2048);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) source.load(blocks + t % DEEP * 2048 + s * 1024, s * 1024 + lane * 16);
+    for (int s = 0; s < 2; ++s) source.load(lds_at + 3 * W::BYTES + (t % DEEP * 4 + wave) * 2048 + s * 1024, s * 1024 + lane * 16);
   };
   if (stages > 0) {
     fetch_dz(0);
@@ -774,35 +802,41 @@ __global__ void __launch_bounds__(256, 2) loss_table_kernel(TableArgs<T> a) {
     now_at = now_at == 2 * W::BYTES ? 0 : now_at + W::BYTES;
     next_at = next_at == 2 * W::BYTES ? 0 : next_at + W::BYTES;
     asm volatile("" : "+v"(at));
-    const char* mine = blocks + t % DEEP * 2048 + lane * 16;
+    const char* mine = lds + 3 * W::BYTES + (t % DEEP * 4 + pair * 2) * 2048 + lane * 16;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const u32x4_t now = *reinterpret_cast<const u32x4_t*>(mine + s * 1024);
+      u32x4_t now[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) now[i] = *reinterpret_cast<const u32x4_t*>(mine + i * 2048 + s * 1024);
 #pragma unroll
       for (int j = 0; j < CB; ++j) {
         u32x4_t f;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const u32x2_t v2 =
-              read_turned(lds + (at ^ (((4 * j & MIXED) ^ (TURN * u)) << 4)) + ((4 * j & ~MIXED) << 4) + (16 * s + 4 * u) * W::NC * 16);
+          const int c = 4 * j + from;
+          const u32x2_t v2 = read_turned(lds + (at ^ (((c & MIXED) ^ (TURN * u)) << 4)) + ((c & ~MIXED) << 4) + (16 * s + 4 * u) * W::NC * 16);
           f[2 * u] = v2[0];
           f[2 * u + 1] = v2[1];
         }
-        acc[j] = mma_pair<T>(f, now, acc[j]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][j] = mma_pair<T>(f, now[i], acc[i][j]);
       }
     }
   }
   wait_and_meet<0>();              // what was asked for beyond the end
-  f32x4* to_plane = reinterpret_cast<f32x4*>(a.planes) + ((int64_t)blockIdx.x * 4 + wave) * (CB * 4 * 64) + lane;
+  // planes of 32 kinds and all channels, this half's behind the other's
+  f32x4* to_plane = reinterpret_cast<f32x4*>(a.planes) + (((int64_t)blockIdx.x * 4 + pair * 2) * 2 + part) * (CB * 4 * 64) + lane;
 #pragma unroll
-  for (int j = 0; j < CB; ++j)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      f32x4 v;
+    for (int j = 0; j < CB; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = acc[j][4 * g + e];
-      to_plane[(j * 4 + g) * 64] = v;
-    }
+      for (int g = 0; g < 4; ++g) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
+        to_plane[(i * 2 * CB + j) * 4 * 64 + g * 64] = v;
+      }
 }
 
 // loss and the logarithm of the sum from the shares' statistics.
@@ -1020,7 +1054,9 @@ int loss_check(const cgtp_kind_loss_args* a) {
   return CGTP_OK;
 }
 
-constexpr int64_t kDzBytes = 256 << 20;
+// What a piece of dz may take.  Each piece adds to the planes of dx and has planes of the table's gradient joined: 16384 rows, 30011 kinds,
+// 256 bf16 channels, kernels of a step 1620 us with 128 MB, 1453 with 256, 1365 with 512 and 1317 with the 1 GB of all of it.
+constexpr int64_t kDzBytes = 512 << 20;
 
 // What a call's workspace holds, in bytes from its start.
 struct Plan {

@@ -229,8 +229,10 @@ def test_logits_are_not_kept(device):
     before = torch.cuda.memory_allocated()
     loss = kind_cross_entropy(x, table, kind)
     assert torch.cuda.max_memory_allocated() - before < rows * kinds * 2 / 20
+    # a backward takes 512 MB of the logits' gradients at a time; with it two planes of 512 x 128 rows x 64 fp32 channels, as many
+    # of kinds, copies of x and the results: 100 MB
     torch.autograd.grad(loss.mean(), (x, table))
-    assert torch.cuda.max_memory_allocated() - before < rows * kinds * 2 / 4
+    assert torch.cuda.max_memory_allocated() - before < (612 << 20) < rows * kinds * 2 / 3
 
 
 def test_graph_replays(device):

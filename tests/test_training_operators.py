@@ -108,11 +108,12 @@ def test_kind_loss_workspace():
     need = lambda backward, **changed: _lib.lib.cgtp_kind_loss_workspace_bytes(C.byref(_loss(**changed)), backward)
     assert need(0, n_rows=0) == need(1, n_rows=0) == need(1, channels=0) == 0
     large = dict(n_rows=16384, n_kinds=30000, channels=256, dtype=2)
-    logits = 2 * 16384 * 30000
-    assert 2 * 16384 * 256 < need(0, **large) < logits / 16 and need(1, **large) < logits / 2
+    logits = 2 * 65536 * 60000
+    large.update(n_rows=65536, n_kinds=60000)
+    assert 2 * 65536 * 256 < need(0, **large) < logits / 16 and need(1, **large) < logits / 6
     assert need(1, **{**large, "grad_table": None}) < need(1, **large)
     # a table whose rows are not whole aligned chunks is copied
-    assert need(0, **{**large, "table": 4098}) - need(0, **large) == 2 * 30000 * 256
+    assert need(0, **{**large, "table": 4098}) - need(0, **large) == 2 * 60000 * 256
     # the most rows and kinds there may be: no overflow
     assert need(1, n_rows=1 << 30, n_kinds=1 << 30, channels=(1 << 15) - 1) > 1 << 45
 
