@@ -37,6 +37,8 @@ struct RowsOf {
   int *counts, *rows, *target, *count;     // counts: rows with a kind, of each workgroup; count: of all
   unsigned* tops;                 // the largest |g| of each workgroup
   float* row_g;                   // g of the rows with a kind
+  const float* lse_of;            // backward: of all rows, and of those with a kind
+  float* row_lse;
   T *to, *to_g;                   // the copy, and the copy times g / max |g| (null: not wanted)
   float *loss, *lse;              // forward: zeros for the rows without a kind
   T* grad_x;                      // backward: likewise (null: not wanted)
@@ -131,7 +133,10 @@ __global__ void __launch_bounds__(kRowThreads) loss_rows_kernel(RowsOf<T> a) {
     if (has) {
       a.rows[place] = (int)row;
       a.target[place] = (int)kind;
-      if (a.g) a.row_g[place] = a.g[row];
+      if (a.g) {
+        a.row_g[place] = a.g[row];
+        a.row_lse[place] = a.lse_of[row];
+      }
     } else if (row < end && a.loss) {
       a.loss[row] = 0.f;
       if (a.lse) a.lse[row] = 0.f;
@@ -997,51 +1002,78 @@ __global__ void __launch_bounds__(256) loss_walk_dx_kernel(const float* planes, 
   store_part<T, 4>(grad_x + (int64_t)rows[r0 + row] * c + ch, out, left);
 }
 
-// The table's from the planes of loss_table_kernel, over the chunks of rows as below.
+// The planes of a piece's kinds, over the chunks of rows: sums += them, or the result in the last chunk.  Four values to a thread; where
+// there are many planes of few values, `slices` threads share out the planes and their sums are added in order.  blocks: planes as
+// loss_table_kernel leaves them (steps: of 16 channels), else rows of c channels.
 template <typename T>
-__global__ void __launch_bounds__(256) loss_table_join_kernel(const float* planes, int splits, int64_t kinds, int steps, int c, const unsigned* top,
-                                                              float scale, int first, int last, float* sums, T* out) {
-  const int part = 32 * 16 * steps / 4, blocks = steps * 2;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, wave = i / part;
-  const int of_wave = (int)(i - wave * part), lane = of_wave & 63, ch = (of_wave >> 6) % blocks * 8 + 4 * (lane >> 5), left = c - ch;
-  const int64_t kind = wave * 32 + (lane & 31);
-  if (kind >= kinds || left <= 0) return;
-  const f32x4* p = reinterpret_cast<const f32x4*>(planes) + (wave / 4 * splits * 4 + wave % 4) * part + of_wave;
+struct TableJoin {
+  const float* planes;
+  const unsigned* top;
+  float* sums;
+  T* out;
+  int64_t kinds, stride;            // stride: four values, between planes
+  int splits, slices, steps, c, first, last, blocks;
+  float scale;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) loss_table_join_kernel(TableJoin<T> a) {
+  __shared__ f32x4 shared[256];
+  const int per = 256 / a.slices, lane = threadIdx.x % per, slice = threadIdx.x / per;
+  const int64_t i = (int64_t)blockIdx.x * per + lane;
+  int64_t kind, at;                 // at: of the first plane, four values
+  int ch;
+  if (a.blocks) {
+    const int part = 32 * 16 * a.steps / 4;
+    const int64_t wave = i / part;
+    const int of_wave = (int)(i - wave * part);
+    ch = (of_wave >> 6) % (2 * a.steps) * 8 + 4 * ((of_wave & 63) >> 5);
+    kind = wave * 32 + (of_wave & 31);
+    at = (wave / 4 * a.splits * 4 + wave % 4) * part + of_wave;
+  } else {
+    const int groups = (a.c + 3) / 4;
+    kind = i / groups;
+    ch = (int)(i - kind * groups) * 4;
+    at = 0;
+  }
+  const int left = a.c - ch;
+  const bool in = kind < a.kinds && left > 0;
   f32x4 s = {};
-  for (int k = 0; k < splits; ++k) s += p[(int64_t)k * 4 * part];
-  const int64_t to = kind * c + ch;
-  if (!first)
+  if (in) {
+    if (a.blocks) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(a.planes) + at;
+#pragma unroll 4
+      for (int k = slice; k < a.splits; k += a.slices) s += p[(int64_t)k * a.stride];
+    } else {
+      const float* p = a.planes + kind * a.c + ch;
+#pragma unroll 4
+      for (int k = slice; k < a.splits; k += a.slices)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < left) s[e] += p[(int64_t)k * a.stride + e];
+    }
+  }
+  if (a.slices > 1) {
+    shared[threadIdx.x] = s;
+    __syncthreads();
+    if (slice) return;
+    for (int k = 1; k < a.slices; ++k) s += shared[k * per + lane];
+  }
+  if (!in) return;
+  const int64_t to = kind * a.c + ch;
+  if (!a.first)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (e < left) s[e] += sums[to + e];
-  if (last) {
+      if (e < left) s[e] += a.sums[to + e];
+  if (a.last) {
     T v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (T)(s[e] * (__uint_as_float(*top) * scale));
-    store_part<T, 4>(out + to, v, left);
+    for (int e = 0; e < 4; ++e) v[e] = (T)(s[e] * (__uint_as_float(*a.top) * a.scale));
+    store_part<T, 4>(a.out + to, v, left);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (e < left) sums[to + e] = s[e];
+      if (e < left) a.sums[to + e] = s[e];
   }
-}
-
-// The planes of a piece's kinds, over the chunks of rows: sums[i] += them, or the result in the last chunk.
-template <typename T>
-__global__ void __launch_bounds__(256) loss_dw_join_kernel(const float* planes, int splits, int64_t elems, const unsigned* top, float scale,
-                                                           int first, int last, float* sums, T* out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= elems) return;
-  float s = first ? 0.f : sums[i];
-  for (int k = 0; k < splits; ++k) s += planes[k * elems + i];
-  if (last) out[i] = (T)(s * (__uint_as_float(*top) * scale));
-  else sums[i] = s;
-}
-
-// lse of the rows of the copy.
-__global__ void __launch_bounds__(256) loss_take_kernel(const float* from, const int* rows, const int* count, float* to) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < *count) to[i] = from[rows[i]];
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------
@@ -1099,7 +1131,10 @@ Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
   // dz: up to kDzBytes, in pieces of about one size; a piece's planes of up to 128 million values
   p.blocks_of_dz = p.steps && p.steps <= 16;
   p.fused = p.blocks_of_dz && a->grad_x;
-  p.chunk = std::min<int64_t>(up_to(n, kTile), 32768);
+  // rows at a time: all of them where their dz is one piece, as far as planes of their dx go; else 32768
+  const int64_t rows_of_planes = std::max<int64_t>(4096, std::min<int64_t>((1 << 25) / c / kTile * kTile, 131072));
+  const int64_t of_one_piece = kDzBytes / size / up_to(k, kTile) / kTile * kTile;
+  p.chunk = std::min(up_to(n, kTile), std::min(rows_of_planes, std::max<int64_t>(32768, of_one_piece)));
   const int64_t most = std::max<int64_t>(1024, std::min(kDzBytes / size / p.chunk, (1 << 27) / c) / kTile * kTile);
   p.piece = up_to(ceil_div(k, ceil_div(k, most)), kTile);
   if (p.fused && !a->grad_table) p.piece = up_to(k, kTile);      // no dz
@@ -1148,6 +1183,8 @@ RowsOf<T> gather(const cgtp_kind_loss_args* a, const Plan& p, bool backward, hip
   r.blocks = p.blocks;
   if (backward) {
     r.row_g = (float*)(ws + p.row_g);
+    r.lse_of = a->lse;
+    r.row_lse = (float*)(ws + p.at);
     r.to_g = p.xg < 0 ? nullptr : (T*)(ws + p.xg);
     r.grad_x = (T*)a->grad_x;
   } else {
@@ -1206,9 +1243,7 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
   char* ws = (char*)a->workspace;
   const RowsOf<T> r = gather<T>(a, p, true, s);
   LogitArgs<T> l = logit_args<T>(a, p, r);
-  float* lse = (float*)(ws + p.at);
-  hipLaunchKernelGGL(loss_take_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, a->lse, r.rows, r.count, lse);
-  l.lse = lse;
+  l.lse = r.row_lse;
   l.dz = p.fused && !a->grad_table ? nullptr : (T*)(ws + p.dz);
   l.planes = (float*)(ws + p.dx);
   l.piece = p.piece;
@@ -1221,6 +1256,14 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
   d.ld_dz = p.piece;
   d.c = a->channels;
   d.ld = p.ld;
+  auto join = [&](bool blocks, int64_t kinds, bool first, bool last, int64_t k0) {
+    TableJoin<T> j = {(const float*)(ws + p.dw), r.tops + p.blocks, (float*)(ws + p.sums) + k0 * c, (T*)a->grad_table + k0 * c, kinds,
+                      blocks ? 4 * (32 * 16 * p.steps / 4) : kinds * c, p.dw_splits, 1, p.steps, a->channels, first, last, blocks, scale};
+    const int64_t threads = blocks ? up_to(kinds, kTile) * p.ld / 4 : kinds * ceil_div(c, 4);
+    // 1024 workgroups' worth of threads, at least eight planes each
+    while (j.slices < 32 && threads * j.slices < 256 * 1024 && p.dw_splits >= 16 * j.slices) j.slices *= 2;
+    hipLaunchKernelGGL(loss_table_join_kernel<T>, dim3((unsigned)ceil_div(threads * j.slices, 256)), dim3(256), 0, s, j);
+  };
   for (int64_t r0 = 0; r0 < a->n_rows; r0 += p.chunk) {
     const int64_t row_tiles = ceil_div(std::min(p.chunk, a->n_rows - r0), kTile);
     const bool last = r0 + p.chunk >= a->n_rows;
@@ -1252,17 +1295,14 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
             case 12: hipLaunchKernelGGL((loss_table_kernel<T, 12>), grid, dim3(256), 0, s, w); break;
             default: hipLaunchKernelGGL((loss_table_kernel<T, 16>), grid, dim3(256), 0, s, w);
           }
-          hipLaunchKernelGGL(loss_table_join_kernel<T>, dim3((unsigned)(k_tiles * kTile * p.ld / 4 / 256)), dim3(256), 0, s, w.planes, w.splits,
-                             d.kinds, p.steps, a->channels, r.tops + p.blocks, scale, r0 == 0, last, (float*)(ws + p.sums) + k0 * c,
-                             (T*)a->grad_table + k0 * c);
+          join(true, d.kinds, r0 == 0, last, k0);
         }
       } else if (a->grad_table) {
         d.b = r.to_g + r0 * p.ld;
         d.planes = (float*)(ws + p.dw);
         d.splits = p.dw_splits;
         hipLaunchKernelGGL(loss_dw_kernel<T>, dim3((unsigned)(k_tiles * tiles_c * d.splits)), dim3(kGemmThreads), 0, s, d);
-        hipLaunchKernelGGL(loss_dw_join_kernel<T>, dim3((unsigned)ceil_div(d.kinds * c, 256)), dim3(256), 0, s, d.planes, d.splits, d.kinds * c,
-                           r.tops + p.blocks, scale, r0 == 0, last, (float*)(ws + p.sums) + k0 * c, (T*)a->grad_table + k0 * c);
+        join(false, d.kinds, r0 == 0, last, k0);
       }
     }
     const int64_t rows_now = std::min(p.chunk, a->n_rows - r0);
