@@ -18,7 +18,11 @@
 namespace cgtp {
 namespace {
 
-constexpr int kTile = 128, kLds = kTile * 256, kRowBlocks = 1024, kRowThreads = 256;
+constexpr int kTile = 128, kRowBlocks = 1024, kRowThreads = 256;
+// Tiles of the products of both operands from LDS: in fp32, whose matrix instructions are slow, small ones cost nothing and keep more of the
+// GPU busy (9000 rows, 100 kinds, 128 channels: logits 17 us with tiles of 128, 7 with these).
+template <typename T> constexpr int kTileOf = sizeof(T) == 4 ? 64 : kTile;
+template <typename T> constexpr int kLds = kTileOf<T> * 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <typename T> constexpr float kRaise = __is_same(T, f16_t) ? 32768.f : 1.f;
@@ -198,7 +202,9 @@ struct LogitArgs {
   int64_t n;                      // rows of the arrays below
   int c, ld, splits, each;        // each: kinds of a split, whole tiles
   float scale, cap;               // scale: to log2 units without a cap, else over the cap; cap: in log2 units, 0: none
-  float2* stats;                  // forward: maximum and sum of each split and row
+  float *loss, *lse_of;           // forward, of all rows
+  const int* rows;
+  float2* stats;                  // forward, several splits: maximum and sum of each split and row
   float* at;                      // forward: the logit of the row's own kind
   const float* lse;               // backward, of the rows of the copy
   T* dz;                          // backward: (r_most, ld_dz)
@@ -225,49 +231,67 @@ __device__ __forceinline__ float capped(float z, float scale, float cap, float& 
 
 template <typename T>
 __device__ __forceinline__ GemmOperand<T> k_rows(const T* p, int64_t row, int64_t ld, int64_t left) {
-  return {{p + row * ld, nullptr}, ld, {(int)std::min<int64_t>(left, kTile), 0}};
+  return {{p + row * ld, nullptr}, ld, {(int)std::min<int64_t>(left, kTileOf<T>), 0}};
 }
 
 template <typename T>
-__device__ __forceinline__ void logits_tile(GemmAcc<kTile>& acc, char* lds, const LogitArgs<T>& a, int64_t m0, int64_t rows, int64_t k0) {
+__device__ __forceinline__ void logits_tile(GemmAcc<kTileOf<T>>& acc, char* lds, const LogitArgs<T>& a, int64_t m0, int64_t rows, int64_t k0) {
   constexpr int D = GemmType<T>::kDepth;
   const GemmOperand<T> x = k_rows(a.x, m0, a.ld, rows - m0), w = k_rows(a.table, k0, a.ld, a.k_end - k0);
-  gemm_loop<T, kTile, true, true, true, false>(acc, lds, (a.ld + D - 1) / D, [&](int64_t t, int64_t& k, int64_t& depth) {
+  gemm_loop<T, kTileOf<T>, true, true, true, false>(acc, lds, (a.ld + D - 1) / D, [&](int64_t t, int64_t& k, int64_t& depth) {
     k = t * D;
     depth = a.ld;
     return x;
   }, [&](int64_t) { return w; });
 }
 
+// The loss and the logarithm of the sum (log2 units) of a row from its own kind's logit, a maximum and a sum.
+__device__ __forceinline__ void give_loss(float* loss, float* lse, int row, float at, float top, float sum) {
+  const float total = (top == -INFINITY ? 0.f : top) + __builtin_amdgcn_logf(sum);
+  loss[row] = (total - at) * kLn2;
+  if (lse) lse[row] = total;
+}
+template <typename T>
+__device__ __forceinline__ void give_loss(const LogitArgs<T>& a, int64_t row, float at, float top, float sum) {
+  give_loss(a.loss, a.lse_of, a.rows[row], at, top, sum);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kGemmThreads, 2) loss_stats_kernel(LogitArgs<T> a) {
-  __shared__ alignas(16) char lds[kLds];
-  const int64_t rows = *a.count, m0 = (int64_t)(blockIdx.x / a.splits) * kTile;
+  __shared__ alignas(16) char lds[kLds<T>];
+  const int64_t rows = *a.count, m0 = (int64_t)(blockIdx.x / a.splits) * kTileOf<T>;
   if (m0 >= rows) return;
   const int split = blockIdx.x % a.splits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
   const int64_t first = (int64_t)split * a.each, end = std::min(first + a.each, a.k_end);
-  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-  int own[2];
+  constexpr int B = kTileOf<T> / 64;      // blocks of 32 for a wavefront, each way
+  float top[B], sum[B];
+  int own[B];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t row = m0 + 32 * (2 * wm + i) + (lane & 31);
+  for (int i = 0; i < B; ++i) {
+    const int64_t row = m0 + 32 * (B * wm + i) + (lane & 31);
     own[i] = row < rows ? a.target[row] : -1;
+    top[i] = -INFINITY;
+    sum[i] = 0.f;
   }
-  GemmAcc<kTile> acc;
-  for (int64_t k0 = first; k0 < end; k0 += kTile) {
+  __shared__ float own_places[kTileOf<T>];
+  GemmAcc<kTileOf<T>> acc;
+  for (int64_t k0 = first; k0 < end; k0 += kTileOf<T>) {
     logits_tile(acc, lds, a, m0, rows, k0);
     __syncthreads();               // the next tile's operands
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < B; ++i) {
       float most = top[i];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < B; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int64_t kind = k0 + 32 * (2 * wn + j) + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+          const int64_t kind = k0 + 32 * (B * wn + j) + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
           float slope, z = acc[i][j][e];
           z = a.cap > 0.f ? capped<T>(z, a.scale, a.cap, slope) : z * a.scale;
-          if (kind == own[i]) a.at[m0 + 32 * (2 * wm + i) + (lane & 31)] = z;
+          if (kind == own[i]) {
+            if (a.splits > 1) a.at[m0 + 32 * (B * wm + i) + (lane & 31)] = z;
+            else own_places[32 * (B * wm + i) + (lane & 31)] = z;
+          }
           z = kind < end ? z : -INFINITY;
           acc[i][j][e] = z;
           most = fmaxf(most, z);
@@ -275,7 +299,7 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_stats_kernel(LogitArgs<T
       const float base = most == -INFINITY ? 0.f : most;
       float s = sum[i] * __builtin_amdgcn_exp2f(top[i] - base);
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < B; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(acc[i][j][e] - base);
       top[i] = most;
@@ -283,7 +307,7 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_stats_kernel(LogitArgs<T
     }
   }
   // the two halves of a wavefront, then the two wavefronts that share rows
-  float2* shared = reinterpret_cast<float2*>(lds);
+  float2* shared = reinterpret_cast<float2*>(lds);      // one for each row of the tile
   auto join = [](float& m, float& s, float m2, float s2) {
     const float most = fmaxf(m, m2), base = most == -INFINITY ? 0.f : most;
     s = s * __builtin_amdgcn_exp2f(m - base) + s2 * __builtin_amdgcn_exp2f(m2 - base);
@@ -291,22 +315,24 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_stats_kernel(LogitArgs<T
   };
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < B; ++i) {
     join(top[i], sum[i], __shfl_xor(top[i], 32), __shfl_xor(sum[i], 32));
-    if (wn == 1 && lane < 32) shared[32 * (2 * wm + i) + lane] = {top[i], sum[i]};
+    if (wn == 1 && lane < 32) shared[32 * (B * wm + i) + lane] = {top[i], sum[i]};
   }
   __syncthreads();
   if (wn == 1 || lane >= 32) return;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 32 * (2 * wm + i) + lane;
+  for (int i = 0; i < B; ++i) {
+    const int r = 32 * (B * wm + i) + lane;
     const float2 other = shared[r];
     join(top[i], sum[i], other.x, other.y);
-    if (m0 + r < rows) a.stats[split * a.n + m0 + r] = {top[i], sum[i]};
+    if (m0 + r >= rows) continue;
+    if (a.splits > 1) a.stats[split * a.n + m0 + r] = {top[i], sum[i]};
+    else give_loss(a, m0 + r, own_places[r], top[i], sum[i]);
   }
 }
 
-// loss and the logarithm of the sum (log2 units) from the splits' statistics.
+// The same from the statistics of several splits.
 __global__ void __launch_bounds__(256) loss_join_kernel(const float2* stats, const float* at, const int* rows, const int* count, int64_t n,
                                                         int splits, float* loss, float* lse) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -319,22 +345,20 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const float2* stats, con
     const float2 v = stats[s * n + i];
     sum += v.y * __builtin_amdgcn_exp2f(v.x - base);
   }
-  const float total = base + __builtin_amdgcn_logf(sum);
-  loss[rows[i]] = (total - at[i]) * kLn2;
-  if (lse) lse[rows[i]] = total;
+  give_loss(loss, lse, rows[i], at[i], base, sum);
 }
 
 // (p - [k = y]) (1 - tanh^2) of a tile of rows x kinds.
 template <typename T>
 __global__ void __launch_bounds__(kGemmThreads, 2) loss_dz_kernel(LogitArgs<T> a) {
-  __shared__ alignas(16) char lds[kLds];
+  __shared__ alignas(16) char lds[kLds<T>];
   const int64_t rows = std::min<int64_t>(*a.count, a.r0 + a.r_most);
-  const int tiles_k = (int)((a.k_end - a.k0 + kTile - 1) / kTile);
-  const int64_t m0 = a.r0 + (int64_t)(blockIdx.x / tiles_k) * kTile, k0 = a.k0 + (int64_t)(blockIdx.x % tiles_k) * kTile;
+  const int tiles_k = (int)((a.k_end - a.k0 + kTileOf<T> - 1) / kTileOf<T>);
+  const int64_t m0 = a.r0 + (int64_t)(blockIdx.x / tiles_k) * kTileOf<T>, k0 = a.k0 + (int64_t)(blockIdx.x % tiles_k) * kTileOf<T>;
   if (m0 >= rows) return;
-  GemmAcc<kTile> acc;
+  GemmAcc<kTileOf<T>> acc;
   logits_tile(acc, lds, a, m0, rows, k0);
-  gemm_results<kTile, false, 1>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, float (&v)[8]) {
+  gemm_results<kTileOf<T>, false, 1>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, float (&v)[8]) {
     if (m0 + r >= rows) return;
     const float lse = a.lse[m0 + r];
     const int own = a.target[m0 + r];
@@ -497,7 +521,7 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
     const int have = (int)std::min<int64_t>(32 * RB, rows - m0) - li;            // rows of the wavefront from this lane's on
     u32x4_t x[RB][KS];
     int own[RB];                   // the row's kind, from this lane's first of a stage on
-    float top[RB], sum[RB], lse[RB];
+    float top[RB], sum[RB], lse[RB], own_z[RB];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
       const int64_t row = std::min(m0 + 32 * i + li, rows - 1);
@@ -516,6 +540,7 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
       } else {
         top[i] = -INFINITY;
         sum[i] = 0.f;
+        own_z[i] = 0.f;
       }
     }
     f32x16_t dx[RB][CB];
@@ -685,7 +710,7 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
           if (__any(has_own))
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              if (e == at_own && has_own && 32 * i < have) a.at[m0 + 32 * i + li] = acc[i][e] * factor;
+              if (e == at_own && has_own) own_z[i] = acc[i][e] * factor;
           if (cut)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -715,7 +740,14 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
         const float other = __shfl_xor(top[i], 32), more = __shfl_xor(sum[i], 32);
         const float now = fmaxf(top[i], other), base = now == -INFINITY ? 0.f : now;
         const float s = sum[i] * __builtin_amdgcn_exp2f(top[i] - base) + more * __builtin_amdgcn_exp2f(other - base);
-        if (half == 0) a.stats[(int64_t)item * W::ROWS + (wave * RB + i) * 32 + li] = {now, s};
+        const bool in = 32 * i < have, has_own = (unsigned)own[i] < (unsigned)((stages - 1) * kStage + 16) && !(own[i] & 16);
+        if (splits > 1) {
+          if (half == 0) a.stats[(int64_t)item * W::ROWS + (wave * RB + i) * 32 + li] = {now, s};
+          if (in && has_own) a.at[m0 + 32 * i + li] = own_z[i];
+        } else {
+          const float there = __shfl_xor(own_z[i], 32);
+          if (in && half == 0) give_loss(a, m0 + 32 * i + li, has_own ? own_z[i] : there, now, s);
+        }
       }
     }
     if constexpr (MODE == kDx) {
@@ -850,6 +882,7 @@ __global__ void __launch_bounds__(256) loss_walk_join_kernel(const float2* stats
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = *count;
   if (i >= n) return;
   const Share share = share_out(kStats, n, rows_of_tile, kinds);
+  if (share.splits == 1) return;   // given already
   const float2* mine = stats + i / rows_of_tile * share.splits * rows_of_tile + i % rows_of_tile;
   float most = -INFINITY;
   for (int s = 0; s < share.splits; ++s) most = fmaxf(most, mine[(int64_t)s * rows_of_tile].x);
@@ -859,9 +892,7 @@ __global__ void __launch_bounds__(256) loss_walk_join_kernel(const float2* stats
     const float2 v = mine[(int64_t)s * rows_of_tile];
     sum += v.y * __builtin_amdgcn_exp2f(v.x - base);
   }
-  const float total = base + __builtin_amdgcn_logf(sum);
-  loss[rows[i]] = (total - at[i]) * kLn2;
-  if (lse) lse[rows[i]] = total;
+  give_loss(loss, lse, rows[i], at[i], base, sum);
 }
 
 // Steps of 16 channels of the kernels above for a width, 0: not theirs.
@@ -910,24 +941,24 @@ struct ProductArgs {
 // planes[s][row][c] += sum over range s of the piece's kinds of dz[row][k] table[k][c]
 template <typename T>
 __global__ void __launch_bounds__(kGemmThreads, 2) loss_dx_kernel(ProductArgs<T> a) {
-  __shared__ alignas(16) char lds[kLds];
+  __shared__ alignas(16) char lds[kLds<T>];
   constexpr int D = GemmType<T>::kDepth;
   const int64_t rows = std::min<int64_t>(*a.count - a.r0, a.r_most);
-  const int tiles_c = (a.c + kTile - 1) / kTile, inner = tiles_c * a.splits;
-  const int64_t m0 = (int64_t)(blockIdx.x / inner) * kTile;
+  const int tiles_c = (a.c + kTileOf<T> - 1) / kTileOf<T>, inner = tiles_c * a.splits;
+  const int64_t m0 = (int64_t)(blockIdx.x / inner) * kTileOf<T>;
   if (m0 >= rows) return;
-  const int split = blockIdx.x % inner / tiles_c, c0 = blockIdx.x % tiles_c * kTile;
+  const int split = blockIdx.x % inner / tiles_c, c0 = blockIdx.x % tiles_c * kTileOf<T>;
   const int64_t all = (a.kinds + D - 1) / D, each = (all + a.splits - 1) / a.splits, from = split * each;
   const GemmOperand<T> dz = k_rows(a.dz, m0, a.ld_dz, rows - m0);
-  const GemmOperand<T> w = {{a.b + c0, a.b + c0 + kTile / 2}, a.ld, {a.ld - c0, a.ld - c0 - kTile / 2}};
-  GemmAcc<kTile> acc;
-  gemm_loop<T, kTile, true, true, false, false>(acc, lds, std::min(each, all - from), [&](int64_t t, int64_t& k, int64_t& depth) {
+  const GemmOperand<T> w = {{a.b + c0, a.b + c0 + kTileOf<T> / 2}, a.ld, {a.ld - c0, a.ld - c0 - kTileOf<T> / 2}};
+  GemmAcc<kTileOf<T>> acc;
+  gemm_loop<T, kTileOf<T>, true, true, false, false>(acc, lds, std::min(each, all - from), [&](int64_t t, int64_t& k, int64_t& depth) {
     k = (t + from) * D;
     depth = a.kinds;
     return dz;
   }, [&](int64_t) { return w; });
   float* plane = a.planes + split * a.r_most * a.c;
-  gemm_results<kTile, false, 1>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, float (&v)[8]) {
+  gemm_results<kTileOf<T>, false, 1>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, float (&v)[8]) {
     const int left = a.c - c0 - c;
     if (m0 + r >= rows || left <= 0) return;
     float* to = plane + (m0 + r) * a.c + c0 + c;
@@ -941,24 +972,24 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_dx_kernel(ProductArgs<T>
 // planes[s][kind][c] = sum over range s of the rows of dz[row][kind] xg[row][c]
 template <typename T>
 __global__ void __launch_bounds__(kGemmThreads, 2) loss_dw_kernel(ProductArgs<T> a) {
-  __shared__ alignas(16) char lds[kLds];
+  __shared__ alignas(16) char lds[kLds<T>];
   constexpr int D = GemmType<T>::kDepth;
   const int64_t rows = std::max<int64_t>(0, std::min<int64_t>(*a.count - a.r0, a.r_most));
-  const int tiles_c = (a.c + kTile - 1) / kTile, inner = tiles_c * a.splits;
-  const int64_t m0 = (int64_t)(blockIdx.x / inner) * kTile;
-  const int split = blockIdx.x % inner / tiles_c, c0 = blockIdx.x % tiles_c * kTile;
+  const int tiles_c = (a.c + kTileOf<T> - 1) / kTileOf<T>, inner = tiles_c * a.splits;
+  const int64_t m0 = (int64_t)(blockIdx.x / inner) * kTileOf<T>;
+  const int split = blockIdx.x % inner / tiles_c, c0 = blockIdx.x % tiles_c * kTileOf<T>;
   const int64_t all = (rows + D - 1) / D, each = (all + a.splits - 1) / a.splits, from = std::min(split * each, all);
   const int left_k = (int)(a.ld_dz - m0);
-  const GemmOperand<T> dz = {{a.dz + m0, a.dz + m0 + kTile / 2}, a.ld_dz, {left_k, left_k - kTile / 2}};
-  const GemmOperand<T> x = {{a.b + c0, a.b + c0 + kTile / 2}, a.ld, {a.ld - c0, a.ld - c0 - kTile / 2}};
-  GemmAcc<kTile> acc;
-  gemm_loop<T, kTile, true, false, false, false>(acc, lds, std::min(each, all - from), [&](int64_t t, int64_t& k, int64_t& depth) {
+  const GemmOperand<T> dz = {{a.dz + m0, a.dz + m0 + kTileOf<T> / 2}, a.ld_dz, {left_k, left_k - kTileOf<T> / 2}};
+  const GemmOperand<T> x = {{a.b + c0, a.b + c0 + kTileOf<T> / 2}, a.ld, {a.ld - c0, a.ld - c0 - kTileOf<T> / 2}};
+  GemmAcc<kTileOf<T>> acc;
+  gemm_loop<T, kTileOf<T>, true, false, false, false>(acc, lds, std::min(each, all - from), [&](int64_t t, int64_t& k, int64_t& depth) {
     k = (t + from) * D;
     depth = rows;
     return dz;
   }, [&](int64_t) { return x; });
   float* plane = a.planes + split * a.kinds * a.c;
-  gemm_results<kTile, false, 1>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, float (&v)[8]) {
+  gemm_results<kTileOf<T>, false, 1>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, float (&v)[8]) {
     const int left = a.c - c0 - c;
     if (m0 + r >= a.kinds || left <= 0) return;
     store_eight(plane + (m0 + r) * a.c + c0 + c, v, left);
@@ -1092,7 +1123,7 @@ constexpr int64_t kDzBytes = 512 << 20;
 
 // What a call's workspace holds, in bytes from its start.
 struct Plan {
-  int ld, splits, each, blocks, dx_splits, dw_splits, steps;      // steps: of the kernels for 16-bit types, 0: the others
+  int ld, tile, splits, each, blocks, dx_splits, dw_splits, steps;      // steps: of the kernels for 16-bit types, 0: the others
   bool blocks_of_dz, fused;                      // dz in blocks of 32 x 32; dz and dx in one kernel
   int64_t row_each, chunk, piece;          // rows of a workgroup of loss_rows_kernel; rows and kinds of dz
   int64_t counts, tops, rows, target, row_g, at, stats, x, xg, table, dz, dx, dw, sums, all;
@@ -1101,6 +1132,7 @@ Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
   Plan p = {};
   const int64_t size = a->dtype == CGTP_F32 ? 4 : 2, n = a->n_rows, k = a->n_kinds, c = a->channels;
   p.steps = walk_steps(a->channels, (int)size);
+  p.tile = size == 4 ? kTileOf<float> : kTile;
   p.ld = (int)(p.steps ? 16 * p.steps : up_to(c, 16 / size));
   p.row_each = up_to(std::max<int64_t>(64, ceil_div(n, kRowBlocks)), 64);
   p.blocks = (int)std::max<int64_t>(1, ceil_div(n, p.row_each));
@@ -1116,10 +1148,10 @@ Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
   p.x = take(n * p.ld * size);
   p.table = p.ld == c && aligned16(a->table) ? -1 : take(k * p.ld * size);
   if (!backward) {
-    // 1024 workgroups where the table has that many tiles for them; a split is whole tiles
-    const int64_t tiles = ceil_div(n, kTile), k_tiles = ceil_div(k, kTile);
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(k_tiles, 1024 / std::max<int64_t>(1, tiles)));
-    p.each = (int)(ceil_div(k_tiles, splits) * kTile);
+    // 1024 workgroups where the table has 256 kinds for each; a split is whole tiles
+    const int64_t tiles = ceil_div(n, p.tile), k_tiles = ceil_div(k, p.tile);
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(ceil_div(k, 256), 1024 / std::max<int64_t>(1, tiles)));
+    p.each = (int)(ceil_div(k_tiles, splits) * p.tile);
     p.splits = (int)ceil_div(k, p.each);
     p.at = take(4 * n);
     p.stats = take(8 * (p.steps ? most_results(kStats, n, walk_rows(p.steps, kStats), k) : n * p.splits));
@@ -1139,14 +1171,14 @@ Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
   p.piece = up_to(ceil_div(k, ceil_div(k, most)), kTile);
   if (p.fused && !a->grad_table) p.piece = up_to(k, kTile);      // no dz
   else p.dz = take(p.chunk * p.piece * size);
-  const int64_t tiles_c = ceil_div(c, kTile), depth = 128 / size;
+  const int64_t tiles_c = ceil_div(c, p.tile), depth = 128 / size;
   auto ranges = [&](int64_t tiles, int64_t k_tiles) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, std::max<int64_t>(1, tiles)), k_tiles / 8));
   };
   if (p.fused) {
     p.dx = take(most_results(kDx, p.chunk, walk_rows(p.steps, kDx), p.piece) * p.ld * 4);
   } else if (a->grad_x) {
-    p.dx_splits = ranges(p.chunk / kTile * tiles_c, p.piece / depth);
+    p.dx_splits = ranges(p.chunk / p.tile * tiles_c, p.piece / depth);
     p.dx = take(p.dx_splits * p.chunk * c * 4);
   }
   if (a->grad_table) {
@@ -1154,7 +1186,7 @@ Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
       p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / (p.piece / kTile), p.chunk / kStage / 8));
       p.dw = take(p.dw_splits * p.piece * p.ld * 4);
     } else {
-      p.dw_splits = ranges(p.piece / kTile * tiles_c, p.chunk / depth);
+      p.dw_splits = ranges(p.piece / p.tile * tiles_c, p.chunk / depth);
       p.dw = take(p.dw_splits * p.piece * c * 4);
     }
     if (n > p.chunk) p.sums = take(k * c * 4);
@@ -1223,16 +1255,19 @@ int loss_forward(const cgtp_kind_loss_args* a, hipStream_t s) {
   l.k_end = a->n_kinds;
   l.splits = p.splits;
   l.each = p.each;
+  l.loss = a->loss;
+  l.lse_of = a->lse;
+  l.rows = r.rows;
   l.stats = (float2*)(ws + p.stats);
   l.at = (float*)(ws + p.at);
   if (p.steps) {
     walk_launch<kStats>(p.steps, l, a->n_rows, a->n_kinds, s);
-    hipLaunchKernelGGL(loss_walk_join_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count,
+    if (a->n_kinds > kLeastKinds) hipLaunchKernelGGL(loss_walk_join_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count,
                        walk_rows(p.steps, kStats), a->n_kinds, a->loss, a->lse);
     return launch_status();
   }
-  hipLaunchKernelGGL(loss_stats_kernel<T>, dim3((unsigned)(ceil_div(a->n_rows, kTile) * p.splits)), dim3(kGemmThreads), 0, s, l);
-  hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count, a->n_rows,
+  hipLaunchKernelGGL(loss_stats_kernel<T>, dim3((unsigned)(ceil_div(a->n_rows, p.tile) * p.splits)), dim3(kGemmThreads), 0, s, l);
+  if (p.splits > 1) hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count, a->n_rows,
                      p.splits, a->loss, a->lse);
   return launch_status();
 }
@@ -1248,7 +1283,7 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
   l.planes = (float*)(ws + p.dx);
   l.piece = p.piece;
   l.ld_dz = p.blocks_of_dz ? p.chunk : p.piece;
-  const int64_t c = a->channels, tiles_c = ceil_div(c, kTile);
+  const int64_t c = a->channels, tiles_c = ceil_div(c, p.tile);
   const float scale = a->scale / kRaise<T>;
   ProductArgs<T> d = {};
   d.dz = l.dz;
@@ -1265,7 +1300,7 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
     hipLaunchKernelGGL(loss_table_join_kernel<T>, dim3((unsigned)ceil_div(threads * j.slices, 256)), dim3(256), 0, s, j);
   };
   for (int64_t r0 = 0; r0 < a->n_rows; r0 += p.chunk) {
-    const int64_t row_tiles = ceil_div(std::min(p.chunk, a->n_rows - r0), kTile);
+    const int64_t row_tiles = ceil_div(std::min(p.chunk, a->n_rows - r0), p.tile);
     const bool last = r0 + p.chunk >= a->n_rows;
     l.r0 = d.r0 = r0;
     l.r_most = d.r_most = p.chunk;
@@ -1273,7 +1308,7 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
       l.k0 = k0;
       l.k_end = std::min(a->n_kinds, k0 + p.piece);
       d.kinds = l.k_end - k0;
-      const int64_t k_tiles = ceil_div(d.kinds, kTile);
+      const int64_t k_tiles = ceil_div(d.kinds, p.tile);
       l.first = k0 == 0;
       if (p.fused) walk_launch<kDx>(p.steps, l, p.chunk, p.piece, s);
       else if (p.steps) walk_launch<kDz>(p.steps, l, p.chunk, d.kinds, s);
@@ -1288,7 +1323,7 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
       if (a->grad_table && p.blocks_of_dz) {
         if constexpr (sizeof(T) == 2) {
           const TableArgs<T> w = {r.to_g + r0 * p.ld, l.dz, (float*)(ws + p.dw), r.count, r0, p.chunk, d.kinds, p.ld, p.dw_splits};
-          const dim3 grid((unsigned)(k_tiles * w.splits));
+          const dim3 grid((unsigned)(k_tiles * w.splits));      // tiles of 128 kinds
           switch (p.steps) {
             case 4: hipLaunchKernelGGL((loss_table_kernel<T, 4>), grid, dim3(256), 0, s, w); break;
             case 8: hipLaunchKernelGGL((loss_table_kernel<T, 8>), grid, dim3(256), 0, s, w); break;

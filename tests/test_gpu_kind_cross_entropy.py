@@ -100,9 +100,10 @@ def test_kind_cross_entropy(device, dtype, rows, kinds, channels, masked, cap):
         assert torch.equal(kind_cross_entropy(*leaves, kind.to(device), scale, cap), loss)
 
 
-@pytest.mark.parametrize("rows,kinds,channels,dtype", [(33001, 2300, 16, BF16), (66001, 1100, 8, F32), (300, 300011, 8, F16)])
+@pytest.mark.parametrize("rows,kinds,channels,dtype", [(40003, 10007, 16, BF16), (35001, 5003, 8, F32), (33001, 9001, 264, F16), (140001, 300, 8, F16),
+                                                       (300, 300011, 8, F16), (20011, 130, 100, BF16)])
 def test_pieces(device, rows, kinds, channels, dtype):
-    """More rows and kinds than the backward takes at a time."""
+    """More rows, or kinds, or both, than the backward takes at a time; many of one and few of the other."""
     from equitorch_amd.nn.functional import kind_cross_entropy
     x, table, kind, g = (t.to(device) for t in _inputs(stable_seed(rows, kinds), rows, kinds, channels, dtype, 0.02))
     leaves = [t.clone().requires_grad_(True) for t in (x, table)]
