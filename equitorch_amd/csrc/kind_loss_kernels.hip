@@ -212,6 +212,9 @@ struct LogitArgs {
   float* planes;                  // dx, see kDx
   int64_t piece;
   int first;
+  T* grad_x;                      // kDx with one piece: where one range of kinds leaves dx, times g and scale_dx (null: planes)
+  const float* g;
+  float scale_dx;
 };
 
 // Logits in log2 units; slope: 1 - tanh^2.
@@ -751,6 +754,27 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
       }
     }
     if constexpr (MODE == kDx) {
+      if (a.grad_x && splits == 1) {
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+          if (32 * i >= have) continue;
+          const int64_t row = m0 + 32 * i + li;
+          const float by = a.g[row] * a.scale_dx;
+          T* to_row = a.grad_x + (int64_t)a.rows[row] * a.c;
+#pragma unroll
+          for (int j = 0; j < CB; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int c = 32 * j + 8 * g + 4 * half, left = a.c - c;
+              if (left <= 0) continue;
+              T v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = (T)(dx[i][j][4 * g + e] * by);
+              store_part<T, 4>(to_row + c, v, left);
+            }
+        }
+        continue;
+      }
       // as a wavefront holds them: four channels 32 j + 8 g + 4 half + .. of a lane's row, 64 lanes one after the other
       f32x4* to_plane = reinterpret_cast<f32x4*>(a.planes) + ((int64_t)item * 4 + wave) * (RB * CB * 4 * 64) + lane;
 #pragma unroll
@@ -936,6 +960,11 @@ struct ProductArgs {
   const int* count;
   int64_t r0, r_most, ld_dz, kinds;      // kinds of the piece
   int c, ld, splits, first;
+  // dx of one range of one piece goes where it belongs: row rows[i], times g[i] scale
+  T* grad_x;                      // null: planes
+  const int* rows;
+  const float* g;
+  float scale;
 };
 
 // planes[s][row][c] += sum over range s of the piece's kinds of dz[row][k] table[k][c]
@@ -961,6 +990,13 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_dx_kernel(ProductArgs<T>
   gemm_results<kTileOf<T>, false, 1>(acc, lds, [](int, int, int) {}, [&](int, int r, int c, float (&v)[8]) {
     const int left = a.c - c0 - c;
     if (m0 + r >= rows || left <= 0) return;
+    if (a.grad_x) {
+      const float by = a.g[a.r0 + m0 + r] * a.scale;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= by;
+      store_eight(a.grad_x + (int64_t)a.rows[a.r0 + m0 + r] * a.c + c0 + c, v, left);
+      return;
+    }
     float* to = plane + (m0 + r) * a.c + c0 + c;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -1012,10 +1048,11 @@ __global__ void __launch_bounds__(256) loss_dx_join_kernel(const float* planes, 
 template <typename T>
 __global__ void __launch_bounds__(256) loss_walk_dx_kernel(const float* planes, const int* rows, const float* g, const int* count, int64_t r0,
                                                            int64_t r_most, int64_t piece, int rows_of_tile, int steps, int c, float scale,
-                                                           T* grad_x) {
+                                                           int one_piece, T* grad_x) {
   const int64_t n = std::min<int64_t>(*count - r0, r_most);
   if (n <= 0) return;
   const Share share = share_out(kDx, n, rows_of_tile, piece);
+  if (one_piece && share.splits == 1) return;      // there already
   // a thread for four channels of a row, in the order of the planes
   const int each = rows_of_tile * 16 * steps / 4, part = each / 4, blocks = steps * 2;       // of a tile, a wavefront; of 8 channels
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, tile = i / each;
@@ -1291,6 +1328,12 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
   d.ld_dz = p.piece;
   d.c = a->channels;
   d.ld = p.ld;
+  d.rows = l.rows = r.rows;
+  d.g = l.g = r.row_g;
+  d.scale = l.scale_dx = scale;
+  const bool one_piece = p.piece >= a->n_kinds;
+  if (one_piece) l.grad_x = (T*)a->grad_x;
+  if (one_piece && p.dx_splits == 1) d.grad_x = (T*)a->grad_x;
   auto join = [&](bool blocks, int64_t kinds, bool first, bool last, int64_t k0) {
     TableJoin<T> j = {(const float*)(ws + p.dw), r.tops + p.blocks, (float*)(ws + p.sums) + k0 * c, (T*)a->grad_table + k0 * c, kinds,
                       blocks ? 4 * (32 * 16 * p.steps / 4) : kinds * c, p.dw_splits, 1, p.steps, a->channels, first, last, blocks, scale};
@@ -1341,10 +1384,10 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
       }
     }
     const int64_t rows_now = std::min(p.chunk, a->n_rows - r0);
-    if (p.fused)
+    if (p.fused && (!one_piece || p.piece > kLeastKinds))
       hipLaunchKernelGGL(loss_walk_dx_kernel<T>, dim3((unsigned)ceil_div(up_to(rows_now, walk_rows(p.steps, kDx)) * p.ld / 4, 256)), dim3(256), 0, s,
-                         l.planes, r.rows, r.row_g, r.count, r0, p.chunk, p.piece, walk_rows(p.steps, kDx), p.steps, a->channels, scale, (T*)a->grad_x);
-    else if (a->grad_x)
+                         l.planes, r.rows, r.row_g, r.count, r0, p.chunk, p.piece, walk_rows(p.steps, kDx), p.steps, a->channels, scale, one_piece, (T*)a->grad_x);
+    else if (a->grad_x && !p.fused && !d.grad_x)
       hipLaunchKernelGGL(loss_dx_join_kernel<T>, dim3((unsigned)ceil_div(rows_now * c, 256)), dim3(256), 0, s, (const float*)(ws + p.dx), p.dx_splits,
                          r.rows, r.row_g, r.count, r0, p.chunk, a->channels, scale, (T*)a->grad_x);
   }
