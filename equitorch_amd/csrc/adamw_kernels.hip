@@ -35,9 +35,9 @@ struct Entry {
 };
 struct StepArgs {
   Entry entry[kAtOnce];
-  double log_b1, log_b2, lr, decay;
+  double lr, decay;
   const float* lr_ptr;            // null: lr
-  float b1, b1_rest, b2, b2_rest, eps, sign;
+  float b1, b1_rest, log_b1, b2, b2_rest, log_b2, eps;      // b1_rest: with the sign of the step
   unsigned seed;
   int entries, blocks;            // blocks: of 256 elements, in a chunk
 };
@@ -114,28 +114,39 @@ __device__ __forceinline__ unsigned encode(const float (&s)[4]) {
   return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], r, true);
 }
 
+// The largest of all lanes' values, by moves within rows of sixteen and from row to row, in a scalar register.
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+  v = std::max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));      // from the lane before
+  v = std::max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));      // two before
+  v = std::max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));      // four
+  v = std::max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));      // eight
+  v = std::max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));      // rows 0 and 2 to the next
+  v = std::max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));      // row 1 to rows 2 and 3
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
 // The scale of a block: its largest magnitude / 448, 0 for zeros, a normal number else (whose inverse is finite), NaN where an
 // element is not finite.  The order of the bit patterns is that of the magnitudes, NaN above infinity.
 __device__ __forceinline__ float block_scale(const float (&s)[4], float& inverse) {
   unsigned top = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) top = std::max(top, __float_as_uint(s[e]) & 0x7fffffffu);
-#pragma unroll
-  for (int o = 32; o; o >>= 1) top = std::max(top, (unsigned)__shfl_xor((int)top, o));
-  const float most = __uint_as_float(top);
-  const float scale = most == 0.f ? 0.f : most < INFINITY ? std::max(most / 448.f, 0x1p-126f) : NAN;
-  inverse = most == 0.f ? 0.f : 1.f / scale;
+  const float most = __uint_as_float(wave_max(top));
+  const float scale = most == 0.f ? 0.f : most < INFINITY ? std::max(most * (1.f / 448.f), 0x1p-126f) : NAN;
+  inverse = most == 0.f ? 0.f : __builtin_amdgcn_rcpf(scale);
   return scale;
 }
-__device__ __forceinline__ float within_448(float q) { return q > 448.f ? 448.f : q < -448.f ? -448.f : q; }
 
-// A value of 0 .. 448 up or down to one of e4m3, by 20 random bits: added below the last bit that stays, which is then cut; below
-// 2^-6 the values are the multiples of 2^-9.
+// A value of 0 .. 448 up or down to one of e4m3, by 20 random bits: added below the last bit that stays, which is then cut.  Below
+// 2^-6 the values are the multiples of 2^-9, as they are between 2^-6 and 2^-5: those are rounded there.
 __device__ __forceinline__ float at_random(float q, unsigned bits) {
-  const float normal = __uint_as_float((__float_as_uint(q) + bits) & 0xfff00000u);
-  const float small = floorf(q * 512.f + (float)bits * 0x1p-20f) * 0x1p-9f;
-  const float r = q < 0x1p-6f ? std::max(small, 0x1p-9f) : std::min(normal, 448.f);
-  return q > 0.f ? r : 0.f;
+  const float lift = q < 0x1p-6f ? 0x1p-6f : 0.f;
+  const float r = __uint_as_float((__float_as_uint(q + lift) + bits) & 0xfff00000u) - lift;
+  return q > 0.f ? std::max(r, 0x1p-9f) : 0.f;
+}
+// The root to a unit in the last place, small numbers brought among the normal ones first.
+__device__ __forceinline__ float root(float v) {
+  const bool small = v < 0x1p-96f;
+  return __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v) * (small ? 0x1p-32f : 1.f);
 }
 
 // A value rounded to fp32 here: neither a product that a sum takes unrounded nor a result that goes on to 16 bits unrounded, so
@@ -150,10 +161,8 @@ template <typename T, bool MASTER, bool EIGHT, bool WHOLE>
 __device__ __forceinline__ void step_block(const StepArgs& a, const Entry& t, const Factors& f, unsigned at, unsigned block) {
   const int left = (int)(t.n - at);
   float p[4], g[4], m[4], v[4];
-  float* master = t.master + at;
-  T* param = (T*)t.p + at;
-  if constexpr (MASTER) load4<float, WHOLE>(p, master, left);
-  else load4<T, WHOLE>(p, param, left);
+  if constexpr (MASTER) load4<float, WHOLE>(p, t.master + at, left);
+  else load4<T, WHOLE>(p, (const T*)t.p + at, left);
   load4<T, WHOLE>(g, (const T*)t.g + at, left);
   if constexpr (EIGHT) {
     const unsigned cm = load_codes<WHOLE>((const uint8_t*)t.m + at, left), cv = load_codes<WHOLE>((const uint8_t*)t.v + at, left);
@@ -168,19 +177,19 @@ __device__ __forceinline__ void step_block(const StepArgs& a, const Entry& t, co
   float r[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float ge = g[e] * a.sign;
-    m[e] = rounded(m[e] * a.b1) + rounded(ge * a.b1_rest);
-    v[e] = rounded(v[e] * a.b2) + rounded(ge * ge * a.b2_rest);
-    r[e] = sqrtf(v[e]);
-    p[e] = rounded(rounded(p[e] * f.keep) - rounded(f.size * (m[e] / (rounded(r[e] * f.root) + a.eps))));
+    m[e] = rounded(m[e] * a.b1) + rounded(g[e] * a.b1_rest);
+    v[e] = rounded(v[e] * a.b2) + rounded(g[e] * g[e] * a.b2_rest);
+    r[e] = root(v[e]);
+    // the reciprocal errs a unit in the last place
+    p[e] = rounded(rounded(p[e] * f.keep) - rounded(f.size * (m[e] * __builtin_amdgcn_rcpf(rounded(r[e] * f.root) + a.eps))));
   }
-  if constexpr (MASTER) store4<float, WHOLE>(master, p, left);
-  store4<T, WHOLE>(param, p, left);
+  if constexpr (MASTER) store4<float, WHOLE>(t.master + at, p, left);
+  store4<T, WHOLE>((T*)t.p + at, p, left);
   if constexpr (EIGHT) {
     float inverse, q[4];
     const float m_scale = block_scale(m, inverse);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = within_448(m[e] * inverse);
+    for (int e = 0; e < 4; ++e) q[e] = __builtin_amdgcn_fmed3f(m[e] * inverse, -448.f, 448.f);
     store_codes<WHOLE>((uint8_t*)t.m + at, encode(q), left);
     const float v_scale = block_scale(r, inverse);
 #pragma unroll
@@ -204,26 +213,23 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(StepArgs a) {
     if (a.entry[mid].first <= blockIdx.x) lo = mid;
     else hi = mid - 1;
   }
-  const Entry& t = a.entry[lo];
+  const Entry t = a.entry[lo];
   Factors f;
   {
     const float now = *t.step + 1.f;
     const double lr = a.lr_ptr ? (double)*a.lr_ptr : a.lr;
     f.keep = (float)(1.0 - lr * a.decay);
-    f.size = (float)(lr / -expm1((double)now * a.log_b1));
-    f.root = (float)(1.0 / sqrt(-expm1((double)now * a.log_b2)));
+    // 1 - b^t for b near 1 without the difference; in fp32: in 64 bits it took a chunk's wavefronts as long as its memory
+    f.size = (float)lr / -expm1f(now * a.log_b1);
+    f.root = 1.f / sqrtf(-expm1f(now * a.log_b2));
     f.key = mix(a.seed * 0x85157AF5u + t.number * 0x9E3779B1u + (unsigned)now * 0xC2B2AE63u);
   }
   const int lane = threadIdx.x & 63;
   const unsigned first = (blockIdx.x - t.first) * (unsigned)a.blocks, all = (t.n + kBlock - 1) / kBlock, end = std::min(first + a.blocks, all);
-  for (unsigned b = first + (threadIdx.x >> 6); b < end; b += kWaves) {
+  for (unsigned b = __builtin_amdgcn_readfirstlane(first + (threadIdx.x >> 6)); b < end; b += kWaves) {
     const unsigned at = b * kBlock + lane * 4;
-    if ((b + 1) * (int64_t)kBlock <= t.n) {
-      step_block<T, MASTER, EIGHT, true>(a, t, f, at, b);
-    } else {
-      // lanes beyond the end have nothing, but take part in the block's scale
-      step_block<T, MASTER, EIGHT, false>(a, t, f, std::min(at, t.n), b);
-    }
+    if (b < t.n / kBlock) step_block<T, MASTER, EIGHT, true>(a, t, f, at, b);
+    else step_block<T, MASTER, EIGHT, false>(a, t, f, std::min(at, t.n), b);      // lanes beyond the end take part in the block's scale
   }
 }
 
@@ -277,17 +283,16 @@ int cgtp_adamw_step(const cgtp_adamw_args* a, void* stream) {
   const Kernel kernel = a->dtype == CGTP_F32 ? kernel_of<float>(master, eight)
                         : a->dtype == CGTP_BF16 ? kernel_of<bf16_t>(master, eight) : kernel_of<f16_t>(master, eight);
   StepArgs s = {};
-  s.log_b1 = std::log(a->beta1);
-  s.log_b2 = std::log(a->beta2);
+  s.log_b1 = (float)std::log(a->beta1);
+  s.log_b2 = (float)std::log(a->beta2);
   s.lr = a->lr;
   s.lr_ptr = a->lr_ptr;
   s.decay = a->weight_decay;
   s.b1 = (float)a->beta1;
-  s.b1_rest = (float)(1.0 - a->beta1);
+  s.b1_rest = (float)(1.0 - a->beta1) * (a->maximize ? -1.f : 1.f);
   s.b2 = (float)a->beta2;
   s.b2_rest = (float)(1.0 - a->beta2);
   s.eps = (float)a->eps;
-  s.sign = a->maximize ? -1.f : 1.f;
   s.seed = a->seed;
   int64_t all = 0;
   for (int64_t i = 0; i < a->n_tensors; ++i) all += (a->tensors[i].n + kBlock - 1) / kBlock;
