@@ -146,28 +146,39 @@ __global__ void __launch_bounds__(kRowThreads) loss_rows_kernel(RowsOf<T> a) {
       if (a.lse) a.lse[row] = 0.f;
     }
     __syncthreads();
-    const int rows = (int)std::min<int64_t>(kRowThreads, end - r0);
-    for (int64_t i = threadIdx.x; i < (int64_t)rows * chunks; i += kRowThreads) {
-      const int r = (int)(i / chunks), c = (int)(i % chunks) * CH, to = places[r], left = a.c - c;
-      if (to < 0) {
-        if (a.grad_x && left > 0) {
+    // chunks of all rows, four of a thread on their way at a time
+    const unsigned all = (unsigned)std::min<int64_t>(kRowThreads, end - r0) * (unsigned)chunks;
+    for (unsigned i0 = threadIdx.x; i0 < all; i0 += 4 * kRowThreads) {
+      u32x4_t v[4];
+      int row_at[4], chunk_at[4], to[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned i = i0 + k * kRowThreads;
+        row_at[k] = (int)(i / (unsigned)chunks);
+        chunk_at[k] = (int)(i - (unsigned)row_at[k] * (unsigned)chunks) * CH;
+        to[k] = i < all ? places[row_at[k]] : -2;
+        v[k] = u32x4_t{0, 0, 0, 0};
+        if (to[k] >= 0 && chunk_at[k] < a.c) v[k] = load_part<u32x4_t, T>(a.x + (r0 + row_at[k]) * a.c + chunk_at[k], a.c - chunk_at[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = chunk_at[k];
+        if (to[k] >= 0) {
+          *reinterpret_cast<u32x4_t*>(a.to + (int64_t)to[k] * a.ld + c) = v[k];
+          if (a.to_g) {
+            typedef T vec __attribute__((ext_vector_type(CH)));
+            vec e = __builtin_bit_cast(vec, v[k]);
+            const float share = most == 0.f ? 0.f : a.g[r0 + row_at[k]] / most;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) e[j] = (T)((float)e[j] * share);
+            *reinterpret_cast<vec*>(a.to_g + (int64_t)to[k] * a.ld + c) = e;
+          }
+        } else if (to[k] == -1 && a.grad_x && c < a.c) {
           T zero[CH];
 #pragma unroll
           for (int e = 0; e < CH; ++e) zero[e] = T(0);
-          store_part<T, CH>(a.grad_x + (r0 + r) * a.c + c, zero, left);
+          store_part<T, CH>(a.grad_x + (r0 + row_at[k]) * a.c + c, zero, a.c - c);
         }
-        continue;
-      }
-      u32x4_t v = {0, 0, 0, 0};
-      if (left > 0) v = load_part<u32x4_t, T>(a.x + (r0 + r) * a.c + c, left);
-      *reinterpret_cast<u32x4_t*>(a.to + (int64_t)to * a.ld + c) = v;
-      if (a.to_g) {
-        typedef T vec __attribute__((ext_vector_type(CH)));
-        vec e = __builtin_bit_cast(vec, v);
-        const float share = most == 0.f ? 0.f : a.g[r0 + r] / most;
-#pragma unroll
-        for (int j = 0; j < CH; ++j) e[j] = (T)((float)e[j] * share);
-        *reinterpret_cast<vec*>(a.to_g + (int64_t)to * a.ld + c) = e;
       }
     }
   }
@@ -248,6 +259,25 @@ __device__ __forceinline__ void logits_tile(GemmAcc<kTileOf<T>>& acc, char* lds,
   }, [&](int64_t) { return w; });
 }
 
+// Maximum and sum of `splits` statistics `each` places apart, eight of them on their way at a time; base: the maximum, 0 where it is -inf.
+__device__ __forceinline__ void join_stats(const float2* p, int64_t each, int splits, float& base, float& sum) {
+  float most = -INFINITY;
+  base = sum = 0.f;
+  for (int s0 = 0; s0 < splits; s0 += 8) {
+    float2 v[8];
+    float now = most;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[k] = s0 + k < splits ? p[(s0 + k) * each] : float2{-INFINITY, 0.f};
+      now = fmaxf(now, v[k].x);
+    }
+    base = now == -INFINITY ? 0.f : now;
+    sum *= __builtin_amdgcn_exp2f(most - base);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += v[k].y * __builtin_amdgcn_exp2f(v[k].x - base);
+    most = now;
+  }
+}
 // The loss and the logarithm of the sum (log2 units) of a row from its own kind's logit, a maximum and a sum.
 __device__ __forceinline__ void give_loss(float* loss, float* lse, int row, float at, float top, float sum) {
   const float total = (top == -INFINITY ? 0.f : top) + __builtin_amdgcn_logf(sum);
@@ -340,14 +370,8 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const float2* stats, con
                                                         int splits, float* loss, float* lse) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= *count) return;
-  float most = -INFINITY;
-  for (int s = 0; s < splits; ++s) most = fmaxf(most, stats[s * n + i].x);
-  const float base = most == -INFINITY ? 0.f : most;
-  float sum = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float2 v = stats[s * n + i];
-    sum += v.y * __builtin_amdgcn_exp2f(v.x - base);
-  }
+  float base, sum;
+  join_stats(stats + i, n, splits, base, sum);
   give_loss(loss, lse, rows[i], at[i], base, sum);
 }
 
@@ -585,11 +609,8 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
       // stage t is there (at least the PER loads of the next one have been asked for since), stage t - 1 has been read
       if (AHEAD > 1 && t + 1 < stages) wait_and_meet<W::PER>();
       else wait_and_meet<0>();
-      if (t + AHEAD < stages) fetch(t + AHEAD, next_at);
       // places for this stage: not kept over the stages, which would take a register for each
       int at_rows = read_rows + now_at, at_cols = read_cols + now_at;
-      now_at = now_at == AHEAD * W::BYTES ? 0 : now_at + W::BYTES;
-      next_at = next_at == AHEAD * W::BYTES ? 0 : next_at + W::BYTES;
       asm volatile("" : "+v"(at_rows), "+v"(at_cols));
       f32x16_t acc[RB];
 #pragma unroll
@@ -611,6 +632,9 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
         }
         __builtin_amdgcn_sched_group_barrier(0x8, AHEAD_READS, 0);
       }
+      if (t + AHEAD < stages) fetch(t + AHEAD, next_at);        // while the matrix cores are busy
+      now_at = now_at == AHEAD * W::BYTES ? 0 : now_at + W::BYTES;
+      next_at = next_at == AHEAD * W::BYTES ? 0 : next_at + W::BYTES;
       const int k0 = t * kStage, mine = kinds - k0 - 16 * half;                 // of this lane's sixteen kinds, where not all
       const bool cut = kinds - k0 < kStage;
       if constexpr (DZ) {
@@ -857,11 +881,7 @@ __global__ void __launch_bounds__(256, 2) loss_table_kernel(TableArgs<T> a) {
   for (int t = 0; t < stages; ++t) {
     if (t + 1 < stages) wait_and_meet<W::PER + 2>();
     else wait_and_meet<0>();
-    fetch_dz(t + 3);
-    if (t + 2 < stages) fetch(t + 2, next_at);
     int at = read + now_at;
-    now_at = now_at == 2 * W::BYTES ? 0 : now_at + W::BYTES;
-    next_at = next_at == 2 * W::BYTES ? 0 : next_at + W::BYTES;
     asm volatile("" : "+v"(at));
     const char* mine = lds + 3 * W::BYTES + (t % DEEP * 4 + pair * 2) * 2048 + lane * 16;
 #pragma unroll
@@ -882,7 +902,13 @@ __global__ void __launch_bounds__(256, 2) loss_table_kernel(TableArgs<T> a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) acc[i][j] = mma_pair<T>(f, now[i], acc[i][j]);
       }
+      if (s == 0) {                // while the matrix cores are busy
+        fetch_dz(t + 3);
+        if (t + 2 < stages) fetch(t + 2, next_at);
+      }
     }
+    now_at = now_at == 2 * W::BYTES ? 0 : now_at + W::BYTES;
+    next_at = next_at == 2 * W::BYTES ? 0 : next_at + W::BYTES;
   }
   wait_and_meet<0>();              // what was asked for beyond the end
   // planes of 32 kinds and all channels, this half's behind the other's
@@ -907,15 +933,8 @@ __global__ void __launch_bounds__(256) loss_walk_join_kernel(const float2* stats
   if (i >= n) return;
   const Share share = share_out(kStats, n, rows_of_tile, kinds);
   if (share.splits == 1) return;   // given already
-  const float2* mine = stats + i / rows_of_tile * share.splits * rows_of_tile + i % rows_of_tile;
-  float most = -INFINITY;
-  for (int s = 0; s < share.splits; ++s) most = fmaxf(most, mine[(int64_t)s * rows_of_tile].x);
-  const float base = most == -INFINITY ? 0.f : most;
-  float sum = 0.f;
-  for (int s = 0; s < share.splits; ++s) {
-    const float2 v = mine[(int64_t)s * rows_of_tile];
-    sum += v.y * __builtin_amdgcn_exp2f(v.x - base);
-  }
+  float base, sum;
+  join_stats(stats + i / rows_of_tile * share.splits * rows_of_tile + i % rows_of_tile, rows_of_tile, share.splits, base, sum);
   give_loss(loss, lse, rows[i], at[i], base, sum);
 }
 
@@ -1171,7 +1190,7 @@ Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
   p.steps = walk_steps(a->channels, (int)size);
   p.tile = size == 4 ? kTileOf<float> : kTile;
   p.ld = (int)(p.steps ? 16 * p.steps : up_to(c, 16 / size));
-  p.row_each = up_to(std::max<int64_t>(64, ceil_div(n, kRowBlocks)), 64);
+  p.row_each = n <= 64 ? 64 : std::max<int64_t>(16, ceil_div(n, kRowBlocks));      // 64: one workgroup needs no other's count
   p.blocks = (int)std::max<int64_t>(1, ceil_div(n, p.row_each));
   auto take = [&](int64_t bytes) {
     const int64_t at = p.all;
