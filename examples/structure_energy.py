@@ -1,36 +1,41 @@
 """Energies and forces of structures from an attention model over their nodes.
 
-    python examples/structure_energy.py [--structures 64] [--steps 20] [--bf16]
+    python examples/structure_energy.py [--structures 64] [--pretrain 0] [--steps 20] [--bf16]
 
 Kinds are embedded, a few layers of attention (with distances) and gated feed-forward blocks mix the nodes of each structure,
 one learnable query for each structure reads the energy out, and the forces are its gradient with respect to the positions.
+``--pretrain`` first takes that many steps on hidden kinds: some nodes' kinds are not shown, and the model is asked for them.
 Training fits energies and forces of a pair potential, so a step differentiates the attention twice; ``--bf16`` then evaluates
 the energies once more with 16-bit operands."""
 import argparse
 import os
 import sys
+from typing import Optional
 
 import torch
 from torch import Tensor, nn
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."))
-from equitorch_amd.nn import Embedding, GatedFeedForward, LayerRMSNorm, SegmentAttention  # noqa: E402
+from equitorch_amd.nn import AddRMSNorm, Embedding, GatedFeedForward, KindCrossEntropy, SegmentAttention  # noqa: E402
 from equitorch_amd.nn.functional import AttentionPlan  # noqa: E402
+from equitorch_amd.optim import AdamW  # noqa: E402
 
 
 class Layer(nn.Module):
-    """Norm, attention, norm, feed-forward; the sum of the layers' results stays in fp32."""
+    """Norm, attention, norm, feed-forward.  ``(update, x)``: what the layer before adds to ``x`` and ``x``, the sum of the layers'
+    results, which stays in fp32; a norm adds the one to the other."""
 
     def __init__(self, channels: int, heads: int, kv_heads: int, hidden: int):
         super().__init__()
-        self.norm1, self.norm2 = LayerRMSNorm("0e", channels), LayerRMSNorm("0e", channels)
+        self.norm1, self.norm2 = AddRMSNorm(channels), AddRMSNorm(channels)
         self.attention = SegmentAttention(channels, heads, kv_heads, cap=30.0)
         self.feed_forward = GatedFeedForward(channels, hidden)
 
-    def forward(self, x: Tensor, plan: AttentionPlan, pos: Tensor) -> Tensor:
+    def forward(self, update: Tensor, x: Optional[Tensor], plan: AttentionPlan, pos: Tensor):
         dtype = self.attention.weight_in.dtype
-        x = x + self.attention(self.norm1(x[:, None])[:, 0].to(dtype), plan, pos).float()
-        return x + self.feed_forward(self.norm2(x[:, None])[:, 0].to(dtype)).float()
+        out, x = self.norm1(update, x)
+        out, x = self.norm2(self.attention(out.to(dtype), plan, pos), x)
+        return self.feed_forward(out.to(dtype)), x
 
 
 class StructureEnergy(nn.Module):
@@ -40,7 +45,7 @@ class StructureEnergy(nn.Module):
         super().__init__()
         self.embedding = Embedding(kinds, channels)
         self.layers = nn.ModuleList(Layer(channels, heads, kv_heads, hidden) for _ in range(layers))
-        self.norm = LayerRMSNorm("0e", channels)
+        self.norm = AddRMSNorm(channels)
         self.query = nn.Parameter(torch.randn(1, channels))
         self.readout = SegmentAttention(channels, heads, kv_heads, distances=False)
         self.head = nn.Linear(channels, 1)
@@ -52,15 +57,19 @@ class StructureEnergy(nn.Module):
                 module.to(dtype)
         return self
 
-    def forward(self, kind: Tensor, pos: Tensor, ptr: Tensor) -> Tensor:
+    def nodes(self, kind: Tensor, pos: Tensor, ptr: Tensor) -> Tensor:
+        """Features of every node, the sum of the layers' results after a norm; a kind of -1 is embedded as zeros."""
         plan = AttentionPlan(ptr)
-        each = AttentionPlan(torch.arange(len(ptr), device=ptr.device), ptr)       # one query for each structure
-        x = self.embedding(kind)
+        update, x = self.embedding(kind), None
         for layer in self.layers:
-            x = layer(x, plan, pos)
+            update, x = layer(update, x, plan, pos)
+        return self.norm(update, x)[0]
+
+    def forward(self, kind: Tensor, pos: Tensor, ptr: Tensor) -> Tensor:
+        each = AttentionPlan(torch.arange(len(ptr), device=ptr.device), ptr)       # one query for each structure
         dtype = self.readout.weight_in.dtype
         query = self.query.expand(len(ptr) - 1, -1).to(dtype)
-        out = self.readout(query, each, x_k=self.norm(x[:, None])[:, 0].to(dtype))
+        out = self.readout(query, each, x_k=self.nodes(kind, pos, ptr).to(dtype))
         return self.head(out.float())[:, 0] * torch.diff(ptr)
 
     def energy_and_forces(self, kind: Tensor, pos: Tensor, ptr: Tensor, create_graph: bool = False):
@@ -92,11 +101,37 @@ def make_structures(structures: int, generator: torch.Generator, device):
     return kind.to(device), pos.to(device), ptr.to(device)
 
 
+def hidden_kinds_loss(model: StructureEnergy, loss: KindCrossEntropy, data, hidden: Tensor) -> Tensor:
+    """Mean cross entropy of the kinds of the ``hidden`` nodes, which the model does not see."""
+    kind, pos, ptr = data
+    shown, asked = kind.masked_fill(hidden, -1), kind.masked_fill(~hidden, -1)
+    return loss(model.nodes(shown, pos, ptr).to(loss.weight.dtype), asked).sum() / hidden.sum().clamp(min=1)
+
+
+def pretrain(model: StructureEnergy, data, steps: int, share: float = 0.15, report=None):
+    """Asks for the kinds of a share of the nodes, another in every step, scored against the embedding's own table; states of the
+    optimizer in 8 bits.  Returns the loss of every step."""
+    table = model.embedding.weight
+    loss = KindCrossEntropy(*table.shape).to(table.device)
+    loss.weight = table
+    optimizer = AdamW([p for n, p in model.named_parameters() if not n.startswith(("query", "readout", "head"))], lr=2e-3, state_bits=8)
+    losses = []
+    for step in range(steps):
+        value = hidden_kinds_loss(model, loss, data, torch.rand(len(data[0]), device=table.device) < share)
+        optimizer.zero_grad()
+        value.backward()
+        optimizer.step()
+        losses.append(value.detach())
+        if report is not None:
+            report(step, float(losses[-1]))
+    return torch.stack(losses)
+
+
 def train(model: StructureEnergy, data, steps: int, report=None):
     """Fits energies (a node) and forces; returns the loss of every step."""
     kind, pos, ptr = data
     energy, forces = pair_potential(*data)
-    optimizer = torch.optim.Adam(model.parameters(), lr=2e-3)
+    optimizer = AdamW(model.parameters(), lr=2e-3, weight_decay=0.0)
     losses = []
     for step in range(steps):
         e, f = model.energy_and_forces(kind, pos, ptr, create_graph=True)
@@ -113,6 +148,7 @@ def train(model: StructureEnergy, data, steps: int, report=None):
 def main():
     parser = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     parser.add_argument("--structures", type=int, default=64)
+    parser.add_argument("--pretrain", type=int, default=0)
     parser.add_argument("--steps", type=int, default=20)
     parser.add_argument("--bf16", action="store_true")
     args = parser.parse_args()
@@ -120,6 +156,8 @@ def main():
     torch.manual_seed(0)
     data = make_structures(args.structures, torch.Generator().manual_seed(0), device)
     model = StructureEnergy().to(device)
+    if args.pretrain:
+        pretrain(model, data, args.pretrain, report=lambda step, loss: print(f"pretraining step {step}: loss {loss:.5f}", flush=True))
     train(model, data, args.steps, lambda step, loss: print(f"step {step}: loss {loss:.5f}", flush=True))
     with torch.no_grad():
         energy = model(*data)
