@@ -28,6 +28,11 @@ def _dense(t: Tensor) -> bool:
     return True
 
 
+def _same_order(a: Tensor, b: Tensor) -> bool:
+    """Whether the elements of two tensors of one shape lie in the same order (the stride of an axis of one says nothing)."""
+    return all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
 def _like(p: Tensor, dtype: torch.dtype) -> Tensor:
     """Zeros in the order of p's elements."""
     if dtype == _E4M3:
@@ -137,7 +142,7 @@ class AdamW(torch.optim.Optimizer):
             raise CgtpError(f"a parameter's elements must lie one after the other, got strides {p.stride()} of {tuple(p.shape)}")
         if p.numel() >= 1 << 31:
             raise CgtpError(f"a parameter must have fewer than 2^31 elements, got {p.numel()}")
-        if g.stride() != p.stride():
+        if not _same_order(g, p):
             g = torch.empty_like(p).copy_(g)
         state = self.state[p] or self._init_state(p, bits, master)
         wide, blocks = (torch.float32, _E4M3)[bits == 8], (-(-p.numel() // BLOCK),)
@@ -148,7 +153,7 @@ class AdamW(torch.optim.Optimizer):
         for name, dtype, shape in wanted + [("step", torch.float32, ())]:
             t = state.get(name)
             if not isinstance(t, Tensor) or t.dtype != dtype or t.shape != shape or t.device != p.device \
-                    or (t.stride() != p.stride() if shape == p.shape else not t.is_contiguous()):
+                    or not (_same_order(t, p) if shape == p.shape else t.is_contiguous()):
                 raise CgtpError(f"state {name!r} of a parameter {tuple(p.shape)} must be {dtype} {tuple(shape)} on {p.device}, in the order "
                                 f"of the parameter's elements: it is missing or another (state_bits or master of another run?)")
         scales = [state[n + "_scale"] for n in names] if bits == 8 else [None, None]

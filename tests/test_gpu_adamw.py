@@ -142,7 +142,8 @@ def test_layouts(device, route, bits):
     gen = torch.Generator().manual_seed(1)
     flat = torch.randn(4000, generator=gen).to(device)
     params = [flat[1:1025].view(32, 32), flat[1031:1031 + 777], flat[2003:2003 + 600].view(20, 30).T, torch.randn(2, 3, 5, 7, generator=gen).to(device).permute(0, 3, 1, 2),
-              torch.randn(40, 50, generator=gen).to(device), torch.zeros((), device=device), torch.zeros(0, 3, device=device)]
+              torch.randn(40, 50, generator=gen).to(device), torch.zeros((), device=device), torch.zeros(0, 3, device=device),
+              torch.randn(6, generator=gen).to(device).as_strided((6, 1, 1), (1, 17, 3))]
     params = [torch.nn.Parameter(p) for p in params]
     assert params[2].data_ptr() == flat.data_ptr() + 4 * 2003
     opt = AdamW(params, lr=1e-2, state_bits=bits)
