@@ -446,9 +446,10 @@ struct LdsSource {
     words[2] = kOutside;
     words[3] = 0x00027000;
   }
-  // to: the place in LDS, the same in all lanes
+  // to: the place in LDS, the same in all lanes.  The compiler does not see an access to memory here: the wait states between a vector
+  // instruction that wrote one of the scalar operands and the access, five, stand in the assembly.
   __device__ __forceinline__ void load(unsigned to, unsigned at) const {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(at), "s"(words) : "memory", "m0");
   }
 };

@@ -101,7 +101,7 @@ def test_kind_cross_entropy(device, dtype, rows, kinds, channels, masked, cap):
 
 
 @pytest.mark.parametrize("rows,kinds,channels,dtype", [(40003, 10007, 16, BF16), (35001, 5003, 8, F32), (33001, 9001, 264, F16), (140001, 300, 8, F16),
-                                                       (300, 300011, 8, F16), (20011, 130, 100, BF16)])
+                                                       (300, 300011, 8, F16), (20011, 130, 100, BF16), (300001, 20, 8, F32), (270001, 140, 24, F16)])
 def test_pieces(device, rows, kinds, channels, dtype):
     """More rows, or kinds, or both, than the backward takes at a time; many of one and few of the other."""
     from equitorch_amd.nn.functional import kind_cross_entropy
@@ -133,6 +133,40 @@ def test_large_logits(device):
         _check((loss, *torch.autograd.grad(loss, leaves, g.to(device))), x, table, kind, 300.0, None, g, dtype)
         loss = kind_cross_entropy(*leaves, kind.to(device), 1e4, 2.0)
         assert torch.isfinite(loss).all() and all(torch.isfinite(t).all() for t in torch.autograd.grad(loss, leaves, g.to(device)))
+
+
+@pytest.mark.parametrize("scale,cap", [(-0.4, None), (-0.4, 2.0), (0.0, None), (0.0, 2.0)])
+def test_scales_of_either_sign(device, scale, cap):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    for dtype in (F32, BF16):
+        x, table, kind, g = _inputs(11, 77, 150, 24, dtype, 0.1)
+        leaves = [t.to(device).requires_grad_(True) for t in (x, table)]
+        loss = kind_cross_entropy(*leaves, kind.to(device), scale, cap)
+        _check((loss, *torch.autograd.grad(loss, leaves, g.to(device))), x, table, kind, scale, cap, g, dtype)
+
+
+def test_what_is_not_finite_stays_in_its_row(device):
+    """An infinity in a row that is asked for makes its loss and its gradient NaN and, through the table's gradient, all of that; the other
+    rows' losses and gradients are theirs."""
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    for dtype, channels in ((F32, 24), (BF16, 24), (F16, 300)):
+        x, table, kind, _ = _inputs(12, 90, 70, channels, dtype, 0.0)
+        good = kind_cross_entropy(x.to(device), table.to(device), kind.to(device), 0.1)
+        x[17, 3] = float("inf")
+        leaves = [t.to(device).requires_grad_(True) for t in (x, table)]
+        loss = kind_cross_entropy(*leaves, kind.to(device), 0.1)
+        others = torch.arange(90, device=device) != 17
+        assert torch.isnan(loss[17]) and torch.equal(loss[others], good[others])
+        gx, gw = torch.autograd.grad(loss, leaves, torch.ones_like(loss))
+        assert torch.isnan(gx[17]).any() and torch.isfinite(gx[others]).all() and torch.isnan(gw).any()
+
+
+def test_batched_gradients_are_refused(device):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    x = torch.randn(5, 8, device=device, requires_grad=True)
+    loss = kind_cross_entropy(x, torch.randn(7, 8, device=device), torch.arange(5, device=device))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, x, torch.ones(3, 5, device=device), is_grads_batched=True)
 
 
 def test_small_incoming_gradients_in_fp16(device):
