@@ -264,3 +264,22 @@ def test_layer(device):
     _within(total, (x.double() + r.double()).cpu(), 2 * EPS[F32] * (x.abs().double() + r.abs().double()).cpu(), "total")
     out.float().sum().backward()
     assert m.weight.grad.shape == (30,) and torch.isfinite(m.weight.grad).all()
+
+
+def test_batched_gradients_are_refused(device):
+    from equitorch_amd.nn.functional import add_rms_norm
+    x = torch.randn(5, 8, device=device, requires_grad=True)
+    out, _ = add_rms_norm(x, torch.randn(5, 8, device=device))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, x, torch.ones(3, 5, 8, device=device), is_grads_batched=True)
+
+
+def test_total_is_kept_from_changes(device):
+    """The backward reads total: a change of it in place is noticed."""
+    from equitorch_amd.nn.functional import add_rms_norm
+    x, r = torch.randn(5, 8, device=device, requires_grad=True), torch.randn(5, 8, device=device)
+    out, total = add_rms_norm(x, r)
+    with torch.no_grad():
+        total.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
