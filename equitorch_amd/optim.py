@@ -47,7 +47,7 @@ class AdamW(torch.optim.Optimizer):
     ``torch.float8_e4m3fn``, each with a ``..._scale`` in fp32 for every 256 elements in the order of memory.  ``root_avg_sq`` is rounded up or
     down at random in proportion, since a step's change of it is far below the distance of two such values; the random bits are
     a hash of ``seed``, the parameter's place among all of the optimizer's, the step and the element, so runs repeat.  A block of 256
-    with a gradient that is not finite becomes NaN.
+    with a gradient that is not finite, or whose square is not, becomes NaN.
 
     ``master``: parameters in 16 bits have a copy in fp32 (``master``) that the steps are taken on, and receive it rounded.  Without it
     a step below half a unit of a 16-bit weight is lost.
@@ -70,15 +70,17 @@ class AdamW(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
 
-    def _check_group(self, group: dict) -> None:
+    @staticmethod
+    def _check_numbers(group: dict) -> None:
         lr = group["lr"]
         if isinstance(lr, Tensor):
             if lr.numel() != 1 or (lr.is_cuda and lr.dtype != torch.float32):
                 raise ValueError(f"lr must be a number or one fp32 number on the GPU, got {lr.dtype} {tuple(lr.shape)}")
         elif not 0.0 <= lr < float("inf"):
             raise ValueError(f"lr must be finite and not negative, got {lr}")
-        if len(group["betas"]) != 2 or not all(0.0 <= b < 1.0 for b in group["betas"]):
-            raise ValueError(f"betas must be two numbers of 0 <= beta < 1, got {group['betas']}")
+        betas = group["betas"]
+        if len(betas) != 2 or not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"betas must be two numbers of 0 <= beta < 1, got {betas}")
         for name in ("eps", "weight_decay"):
             if not 0.0 <= group[name] < float("inf"):
                 raise ValueError(f"{name} must be finite and not negative, got {group[name]}")
@@ -86,6 +88,9 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
         if not 0 <= group["seed"] < 1 << 32:
             raise ValueError(f"seed must be 0 <= seed < 2^32, got {group['seed']}")
+
+    def _check_group(self, group: dict) -> None:
+        self._check_numbers(group)
         taken = []
         for p in (p for g in self.param_groups for p in g["params"]):
             if p.numel():
@@ -165,6 +170,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        for group in self.param_groups:          # a schedule or a user may have changed them; nothing is stepped if one is refused
+            self._check_numbers(group)
         mod, number = _shim.module(), 0
         for group in self.param_groups:
             params, lr, (b1, b2) = group["params"], group["lr"], group["betas"]
@@ -184,9 +191,10 @@ class AdamW(torch.optim.Optimizer):
         for i, p in enumerate(params):
             if p.grad is not None:
                 calls.setdefault((p.device, p.dtype), []).append((i, p, self._operands(p, a.state_bits, master)))
-        for (device, dtype), items in calls.items():
+        for device, _ in calls:
             if lr is not None and lr.device != device:
                 raise CgtpError(f"lr is on {lr.device}, parameters on {device}")
+        for (device, dtype), items in calls.items():
             tensors = (AdamwTensor * len(items))()
             for t, (i, p, (g, m, v, m_scale, v_scale, wide, step)) in zip(tensors, items):
                 t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.step = (x.data_ptr() for x in (p, g, m, v, step))

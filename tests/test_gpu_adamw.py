@@ -428,3 +428,47 @@ def test_refusals(device, route):
     opt.param_groups[0]["state_bits"] = 8
     with pytest.raises(CgtpError):
         opt.step()
+
+
+def test_options_changed_later_are_checked(device, route):
+    """A number that a schedule or a user sets after the optimizer was made is looked at by the step, before any group's is taken."""
+    first, second = (torch.nn.Parameter(torch.ones(6, 4, device=device)) for _ in range(2))
+    opt = AdamW([{"params": [first]}, {"params": [second]}])
+    first.grad, second.grad = torch.ones_like(first), torch.ones_like(second)
+    opt.step()
+    group = opt.param_groups[1]
+    for name, value in (("lr", -1.0), ("lr", float("nan")), ("lr", torch.ones((), device=device, dtype=F64)), ("lr", torch.ones(2, device=device)),
+                        ("betas", (1.0, 0.9)), ("eps", -1e-8), ("weight_decay", float("inf")), ("state_bits", 4), ("seed", 1 << 32)):
+        kept, before = group[name], [p.detach().clone() for p in (first, second)]
+        group[name] = value
+        with pytest.raises(ValueError):
+            opt.step()
+        group[name] = kept
+        assert torch.equal(first, before[0]) and torch.equal(second, before[1])
+    group["lr"] = torch.full((), 1e-3, device=device)
+    opt.step()
+    assert not torch.equal(second, before[1])
+
+
+def test_the_largest_tensor(device):
+    """The end of a tensor whose offsets in bytes pass 32 bits, against the same elements as a tensor of their own."""
+    n, tail = (1 << 31) - 100, 256 * 20 + 156      # whole blocks of 256 before the tail, which ends inside one
+    assert (n - tail) % 256 == 0
+    gen = torch.Generator(device=device).manual_seed(3)
+    for bits in (8, 32):
+        large = torch.nn.Parameter(torch.zeros(n, device=device, dtype=BF16))
+        large.grad = torch.zeros_like(large)
+        small = torch.nn.Parameter(torch.randn(tail, device=device, generator=gen).to(BF16))
+        small.grad = torch.randn(tail, device=device, generator=gen).to(BF16)
+        with torch.no_grad():
+            large[n - tail:] = small
+            large.grad[n - tail:] = small.grad
+        opts = [AdamW([p], lr=1e-1, state_bits=bits) for p in (large, small)]
+        for opt in opts:
+            opt.step()
+        assert torch.equal(large[n - tail:], small) and not large[:n - tail].any()
+        a, b = (opt.state[p] for opt, p in zip(opts, (large, small)))
+        for name in b:
+            if name == "root_avg_sq":
+                continue                             # rounded at random by the element's place
+            assert torch.equal(a[name].reshape(-1)[-b[name].numel():].float(), b[name].reshape(-1).float()), name
