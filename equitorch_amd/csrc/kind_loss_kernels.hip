@@ -1168,7 +1168,8 @@ __global__ void __launch_bounds__(256) loss_table_join_kernel(TableJoin<T> a) {
 int loss_check(const cgtp_kind_loss_args* a) {
   if (!a) return CGTP_ERR_NULL;
   if (a->dtype != CGTP_F32 && a->dtype != CGTP_BF16 && a->dtype != CGTP_F16) return CGTP_ERR_DTYPE;
-  if (a->n_rows < 0 || a->n_rows > (1 << 30) || a->n_kinds < 1 || a->n_kinds > (1 << 30) || a->channels < 1 || a->channels > 0x7fff)
+  // 2^29 rows are 2^23 workgroups for tiles of 64: a grid has fewer than 2^32 threads
+  if (a->n_rows < 0 || a->n_rows > (1 << 29) || a->n_kinds < 1 || a->n_kinds > (1 << 30) || a->channels < 1 || a->channels > 0x7fff)
     return CGTP_ERR_SHAPE;
   if (a->n_rows > 0 && (!a->x || !a->table || !a->kind)) return CGTP_ERR_NULL;
   return CGTP_OK;

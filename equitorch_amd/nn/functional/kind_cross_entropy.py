@@ -114,8 +114,8 @@ def kind_cross_entropy(x: Tensor, table: Tensor, kind: Tensor, scale: float = 1.
     # the kernels take scale * log2 e, or scale / cap and cap * log2 e, as fp32
     if not abs(scale) <= 1e38 or (bounded and not (1e-37 <= cap <= 1e38 and abs(scale) / cap <= 1e38)):
         raise CgtpError(f"scale, cap (above zero, or None) and their quotient must be in fp32's range, got {scale} and {cap}")
-    if (x.numel() and kind.numel() > 1 << 30) or table.shape[0] > 1 << 30:
-        raise CgtpError(f"at most 2^30 rows and kinds, got {kind.numel()} and {table.shape[0]}")
+    if (x.numel() and kind.numel() > 1 << 29) or table.shape[0] > 1 << 30:
+        raise CgtpError(f"at most 2^29 rows and 2^30 kinds, got {kind.numel()} and {table.shape[0]}")
     flat, table, kinds = x.reshape(-1, c).contiguous(), table.contiguous(), kind.reshape(-1).contiguous()
     keep = (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or _lib.forward_mode()
     mod = _shim.module()

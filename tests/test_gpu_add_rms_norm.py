@@ -283,3 +283,31 @@ def test_total_is_kept_from_changes(device):
         total.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+def test_offsets_beyond_32_bits(device):
+    """The last rows of an array of more than 2^31 elements, against the same rows alone; the weight's gradient has terms of those only."""
+    from equitorch_amd.nn.functional import add_rms_norm, add_rms_norm_8bit
+    n, c, tail = (1 << 24) + 5003, 129, 3000
+    gen = torch.Generator(device=device).manual_seed(1)
+    x, r = (torch.zeros(n, c, device=device, dtype=torch.bfloat16) for _ in range(2))
+    for t in (x, r):
+        t[:7] = t[-tail:] = 1.0
+        t[-tail:] *= torch.randn(tail, c, device=device, generator=gen).to(t.dtype)
+    weight = torch.randn(c, device=device, generator=gen, requires_grad=True)
+    g = torch.zeros_like(x)
+    g[-tail:] = torch.randn(tail, c, device=device, generator=gen).to(g.dtype)
+    results = []
+    for rows in (slice(None), slice(n - tail, None)):
+        leaf = x[rows].detach().requires_grad_(True)
+        out, total = add_rms_norm(leaf, r[rows], weight)
+        gx, gw = torch.autograd.grad(out, (leaf, weight), g[rows])
+        values, scale, _ = add_rms_norm_8bit(leaf.detach(), r[rows], weight.detach())
+        results.append([t.detach()[-tail:].clone() for t in (out, total, gx, values.view(torch.uint8), scale)] + [gw])
+        del out, total, gx, values, leaf
+    for a, b in zip(*(t[:5] for t in results)):
+        assert torch.equal(a, b)
+    t = results[1][1].double()
+    size = (g[-tail:].double() * t * (t.square().mean(1, keepdim=True) + 1e-6).rsqrt()).abs().sum(0)
+    # two sums of the same 3000 terms in other orders: each at most one rounding of the partial sum a term
+    assert ((results[0][5] - results[1][5]).abs().double() <= 2 * 3000 * 2.0 ** -24 * size).all()

@@ -169,6 +169,82 @@ def test_batched_gradients_are_refused(device):
         torch.autograd.grad(loss, x, torch.ones(3, 5, device=device), is_grads_batched=True)
 
 
+def test_rows_and_table_of_one_leaf(device):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    for dtype in (F32, BF16):
+        table = _inputs(13, 5, 60, 40, dtype, 0.0)[1].to(device)
+        kind, g = (torch.arange(60, device=device) + 7) % 61 - 1, torch.rand(60, device=device)
+        one = table.clone().requires_grad_(True)
+        two = [table.clone().requires_grad_(True) for _ in range(2)]
+        got, = torch.autograd.grad(kind_cross_entropy(one, one, kind, 0.2), one, g)
+        gx, gw = torch.autograd.grad(kind_cross_entropy(*two, kind, 0.2), two, g)
+        assert torch.equal(got, gx + gw)
+
+
+@pytest.mark.parametrize("dtype,k,c", [(BF16, (1 << 23) + 77, 256), (F32, (1 << 21) + 1011, 1024)])
+def test_offsets_beyond_32_bits_in_the_table(device, dtype, k, c):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    n, gen = 20, torch.Generator(device=device).manual_seed(5)
+    x = torch.randn(n, c, device=device, generator=gen).to(dtype)
+    table = torch.randn(k, c, device=device, generator=gen, dtype=dtype)
+    kind = k - 1 - 37 * torch.arange(n, device=device)
+    kind[3], kind[4] = 0, -1
+    g = torch.rand(n, device=device, generator=gen)
+    leaves = [t.requires_grad_(True) for t in (x, table)]
+    loss = kind_cross_entropy(*leaves, kind, 0.1)
+    gx, gw = torch.autograd.grad(loss, leaves, g)
+    x, table = x.detach(), table.detach()
+    with torch.no_grad():
+        # the logits in 64 bits, and what the gradients have of the rows near both ends of the table
+        z = torch.cat([x.double() @ part.double().T for part in table.split(1 << 18)], 1) * 0.1
+        p = (z - torch.logsumexp(z, 1, keepdim=True)).exp()
+        asked = torch.arange(n, device=device) != 4
+        want = (torch.logsumexp(z, 1) - z.gather(1, kind.clamp(min=0)[:, None])[:, 0]) * asked
+        # of a logit: the product over C and the scale; of the sum's logarithm: chains of no more than all terms of a range
+        err = (c + 8) * U * 0.1 * (x.double().norm(dim=1) * table[::997].double().norm(dim=1).max() * 1.2) + 8 * U * z.abs().amax(1)
+        assert ((loss - want).abs() <= 2 * err + (k / 4 + 40) * U).all()
+        p[torch.arange(n, device=device)[asked], kind[asked]] -= 1
+        dz = p * (g * asked).double()[:, None] * 0.1
+        size = dz.abs()
+        off = 3 * EPS[dtype] + 4 * float(err.max()) + (k / 4 + 40) * U         # of dz, of x over the largest g, and of a product's result
+        for rows in (slice(0, 300), slice(k - 1100, k)):
+            _within(gw[rows], dz[:, rows].T @ x.double(), off * (size[:, rows].T @ x.double().abs()) + 2.0 ** -60, "grad table")
+        want, bound = torch.zeros(n, c, dtype=F64, device=device), torch.zeros(n, c, dtype=F64, device=device)
+        at = 0
+        for part in table.split(1 << 18):
+            d = dz[:, at:at + len(part)]
+            want += d @ part.double()
+            bound += d.abs() @ part.double().abs()
+            at += len(part)
+        _within(gx, want, (off + (k / 4 + 40) * U) * bound, "grad x")
+
+
+def test_offsets_beyond_32_bits_in_the_rows(device):
+    """Every row's results are those of the rows alone; the table's gradient has terms of the last ones only."""
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    n, c, k, tail = (1 << 23) + 5003, 256, 40, 3000
+    gen = torch.Generator(device=device).manual_seed(6)
+    x = torch.randn(n, c, device=device, generator=gen, dtype=BF16)
+    table = torch.randn(k, c, device=device, generator=gen, dtype=BF16).requires_grad_(True)
+    kind = torch.randint(0, k, (n,), device=device, generator=gen)
+    g = torch.zeros(n, device=device)
+    g[-tail:] = torch.rand(tail, device=device, generator=gen)
+    results = []
+    for rows in (slice(None), slice(n - tail, None)):
+        leaf = x[rows].detach().requires_grad_(True)
+        loss = kind_cross_entropy(leaf, table, kind[rows], 0.1)
+        gx, gw = torch.autograd.grad(loss, (leaf, table), g[rows])
+        results.append((loss.detach()[-tail:].clone(), gx[-tail:].clone(), gw))
+        if loss.numel() == n:
+            assert not gx[:-tail].any()
+    for a, b in zip(results[0][:2], results[1][:2]):
+        assert torch.equal(a, b)
+    # two sums of the same terms, of at most |x| 0.1 g each, in other orders, and each rounded once
+    size = 0.1 * (g[-tail:, None] * x[-tail:].abs().float()).sum(0).double()
+    gap = (results[0][2].double() - results[1][2].double()).abs()
+    assert (gap <= 2 * 3000 * U * size + 2 * EPS[BF16] * results[1][2].double().abs()).all()
+
+
 def test_small_incoming_gradients_in_fp16(device):
     """Gradients of one row and of the mean over many, whose products with probabilities are below fp16's range."""
     from equitorch_amd.nn.functional import kind_cross_entropy

@@ -86,7 +86,7 @@ def _loss(**changed):
 
 @pytest.mark.parametrize("changed,forward,backward", [
     ({"dtype": 1}, DTYPE, DTYPE), ({"channels": 0}, SHAPE, SHAPE), ({"channels": 1 << 15}, SHAPE, SHAPE), ({"n_rows": -1}, SHAPE, SHAPE),
-    ({"n_rows": (1 << 30) + 1}, SHAPE, SHAPE), ({"n_kinds": 0}, SHAPE, SHAPE), ({"n_kinds": (1 << 30) + 1}, SHAPE, SHAPE), ({"x": None}, NULL, NULL),
+    ({"n_rows": (1 << 29) + 1}, SHAPE, SHAPE), ({"n_kinds": 0}, SHAPE, SHAPE), ({"n_kinds": (1 << 30) + 1}, SHAPE, SHAPE), ({"x": None}, NULL, NULL),
     ({"table": None}, NULL, NULL), ({"kind": None}, NULL, NULL), ({"loss": None}, NULL, None), ({"lse": None}, None, NULL),
     ({"grad_loss": None}, None, NULL), ({"workspace": None}, WORKSPACE, WORKSPACE), ({"workspace": 4104}, ALIGN, ALIGN)])
 def test_kind_loss_codes(changed, forward, backward):
@@ -115,7 +115,7 @@ def test_kind_loss_workspace():
     # a table whose rows are not whole aligned chunks is copied
     assert need(0, **{**large, "table": 4098}) - need(0, **large) == 2 * 60000 * 256
     # the most rows and kinds there may be: no overflow
-    assert need(1, n_rows=1 << 30, n_kinds=1 << 30, channels=(1 << 15) - 1) > 1 << 45
+    assert need(1, n_rows=1 << 29, n_kinds=1 << 30, channels=(1 << 15) - 1) > 1 << 45
 
 
 def test_kind_cross_entropy_takes_gpu_tensors_only():
