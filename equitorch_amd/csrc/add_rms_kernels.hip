@@ -7,9 +7,12 @@
 // the forward's values.  8 bits: s = max_c |out| / 448 for each row, and out / s in e4m3.
 //
 // Bound by memory: every row is read once and stays in registers, eight elements (a chunk) a lane at a time.  A row of up to
-// 64 chunks has the power of two of lanes that holds it, one chunk each, so that short rows share a wavefront; up to 4096
-// channels a wavefront with up to eight chunks a lane; longer ones a workgroup.  Loads need no alignment but the
-// element's.
+// 64 chunks has the power of two of lanes that holds it, one chunk each, so that short rows share a wavefront; up to 1024
+// channels a wavefront with two chunks a lane; longer ones a workgroup, with 256 threads of one to four chunks, or 512 of four or eight
+// (which spill, above 16384 channels).  More chunks a lane leave too few wavefronts to hide the memory behind: 9765 rows of 4096 fp16
+// channels, backward: 158 us with a wavefront and eight chunks, 71 with a workgroup and two; 26666 of 1500: 91 us with a wavefront and four, 76
+// with a workgroup and one.  Loads need no alignment but the element's.  65536 rows of 256 channels, bf16 on an fp32 residual: forward
+// 38.7 us (5.2 TB/s), backward 47.0 (5.4); 200003 rows of 512 in bf16 to 8 bits: 140 us (5.1 TB/s).
 #include "elem.h"
 
 #include <algorithm>
@@ -17,7 +20,7 @@
 namespace cgtp {
 namespace {
 
-constexpr int kThreads = 256, kMaxChunks = 8;
+constexpr int kThreads = 256, kWaveChunks = 2;
 
 template <typename U>
 struct Chunk {
@@ -73,14 +76,23 @@ __device__ __forceinline__ unsigned row_max(unsigned v, int group, float* shared
   return v;
 }
 
+// Where a lane's chunk of a row is.  A last chunk that the row does not fill is taken from the row's end: the columns that it shares with the
+// chunk before are computed twice with the same bits, and only the sums leave the first `twice` of its elements out.  One by one
+// its elements took as many accesses as a row of 1001 has altogether.
+struct Place { int c, valid, twice; };
+__device__ __forceinline__ Place place_of(int channels, int chunk) {
+  Place p = {chunk * 8, channels - chunk * 8, 0};
+  if (p.valid > 0 && p.valid < 8 && channels >= 8) p = {channels - 8, 8, 8 - p.valid};
+  return p;
+}
+
 template <typename T>
-__device__ __forceinline__ void load_weight(float (&w)[8], const RmsArgs& a, int c) {
-  const int valid = a.c - c;
+__device__ __forceinline__ void load_weight(float (&w)[8], const RmsArgs& a, const Place& p) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) w[e] = 1.f;
-  if (!a.weight || valid <= 0) return;
-  if (a.weight_f32) Chunk<float>::load(w, (const float*)a.weight + c, valid);
-  else Chunk<T>::load(w, (const T*)a.weight + c, valid);
+  if (!a.weight || p.valid <= 0) return;
+  if (a.weight_f32) Chunk<float>::load(w, (const float*)a.weight + p.c, p.valid);
+  else Chunk<T>::load(w, (const T*)a.weight + p.c, p.valid);
 }
 
 // Eight values of magnitude up to 448 in e4m3, to nearest.
@@ -103,8 +115,12 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) add_rms_kernel(RmsArgs
   const T* x = (const T*)a.x;
   const R* residual = (const R*)a.residual;
   float w[CHUNKS][8];
+  Place place[CHUNKS];
 #pragma unroll
-  for (int k = 0; k < CHUNKS; ++k) load_weight<T>(w[k], a, (k * lanes + lane) * 8);
+  for (int k = 0; k < CHUNKS; ++k) {
+    place[k] = place_of(a.c, k * lanes + lane);
+    load_weight<T>(w[k], a, place[k]);
+  }
   const float inv_c = 1.f / (float)a.c;
   for (int64_t first = (int64_t)blockIdx.x * per_block; first < a.n_rows; first += (int64_t)gridDim.x * per_block) {
     const int64_t row = first + (BLOCK ? 0 : (int)threadIdx.x / lanes);
@@ -113,30 +129,31 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) add_rms_kernel(RmsArgs
     float t[CHUNKS][8], sum = 0.f;
 #pragma unroll
     for (int k = 0; k < CHUNKS; ++k) {
-      const int c = (k * lanes + lane) * 8, valid = in ? a.c - c : 0;
+      const int c = place[k].c, valid = in ? place[k].valid : 0;
       Chunk<T>::load(t[k], x + at + c, valid);
       if (residual) {
         float r[8];
         Chunk<R>::load(r, residual + at + c, valid);
 #pragma unroll
         for (int e = 0; e < 8; ++e) t[k][e] = (float)(R)(t[k][e] + r[e]);
-        if (a.total) store_eight((R*)a.total + at + c, t[k], valid);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(t[k][e], t[k][e], sum);
+      for (int e = 0; e < 8; ++e) {
+        const float v = e < place[k].twice ? 0.f : t[k][e];
+        sum = fmaf(v, v, sum);
+      }
     }
     const float rstd = rsqrtf(row_sum<BLOCK>(sum, lanes, shared) * inv_c + a.eps);
     if (a.rstd && in && lane == 0) a.rstd[row] = rstd;
 #pragma unroll
-    for (int k = 0; k < CHUNKS; ++k)
+    for (int k = 0; k < CHUNKS; ++k) {
+      if (residual && a.total) store_eight((R*)a.total + at + place[k].c, t[k], in ? place[k].valid : 0);
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[k][e] = t[k][e] * rstd * w[k][e];
+    }
     if (!a.scale) {
 #pragma unroll
-      for (int k = 0; k < CHUNKS; ++k) {
-        const int c = (k * lanes + lane) * 8;
-        store_eight((T*)a.out + at + c, t[k], in ? a.c - c : 0);
-      }
+      for (int k = 0; k < CHUNKS; ++k) store_eight((T*)a.out + at + place[k].c, t[k], in ? place[k].valid : 0);
     } else {
       unsigned top = 0;
 #pragma unroll
@@ -151,13 +168,13 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) add_rms_kernel(RmsArgs
       if (in && lane == 0) a.scale[row] = scale;
 #pragma unroll
       for (int k = 0; k < CHUNKS; ++k) {
-        const int c = (k * lanes + lane) * 8, valid = in ? a.c - c : 0;
+        const int valid = in ? place[k].valid : 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float q = t[k][e] * inverse;
           t[k][e] = q > 448.f ? 448.f : q < -448.f ? -448.f : q;
         }
-        if (valid > 0) store_e4m3((uint8_t*)a.out + at + c, t[k], valid);
+        if (valid > 0) store_e4m3((uint8_t*)a.out + at + place[k].c, t[k], valid);
       }
     }
   }
@@ -174,9 +191,11 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) add_rms_grad_kernel(Rm
   const int per_block = BLOCK ? 1 : kThreads / lanes;
   const R* total = (const R*)a.total;
   float w[CHUNKS][8], gw[CHUNKS][8];
+  Place place[CHUNKS];
 #pragma unroll
   for (int k = 0; k < CHUNKS; ++k) {
-    load_weight<T>(w[k], a, (k * lanes + lane) * 8);
+    place[k] = place_of(a.c, k * lanes + lane);
+    load_weight<T>(w[k], a, place[k]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) gw[k][e] = 0.f;
   }
@@ -189,22 +208,22 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) add_rms_grad_kernel(Rm
     float t[CHUNKS][8], u[CHUNKS][8], dot = 0.f;
 #pragma unroll
     for (int k = 0; k < CHUNKS; ++k) {
-      const int c = (k * lanes + lane) * 8, valid = in ? a.c - c : 0;
+      const int c = place[k].c, valid = in ? place[k].valid : 0;
       Chunk<R>::load(t[k], total + at + c, valid);
       Chunk<T>::load(u[k], (const T*)a.grad_out + at + c, valid);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         t[k][e] *= rstd;
-        gw[k][e] = fmaf(u[k][e], t[k][e], gw[k][e]);
+        gw[k][e] = fmaf(u[k][e], t[k][e], gw[k][e]);        // of columns that are there twice: not taken below
         u[k][e] *= w[k][e];
-        dot = fmaf(u[k][e], t[k][e], dot);
+        dot = fmaf(e < place[k].twice ? 0.f : u[k][e], t[k][e], dot);
       }
     }
     if (!a.grad_x && !a.grad_residual) continue;
     const float mean = row_sum<BLOCK>(dot, lanes, shared) * inv_c;
 #pragma unroll
     for (int k = 0; k < CHUNKS; ++k) {
-      const int c = (k * lanes + lane) * 8, valid = in ? a.c - c : 0;
+      const int c = place[k].c, valid = in ? place[k].valid : 0;
       if (a.grad_total) {
         float g[8];
         Chunk<R>::load(g, (const R*)a.grad_total + at + c, valid);
@@ -230,8 +249,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) add_rms_grad_kernel(Rm
     for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int c = (k * lanes + lane) * 8 + e;
-        if (c < a.c) give(c, gw[k][e]);
+        if (e >= place[k].twice && e < place[k].valid) give(place[k].c + e, gw[k][e]);
       }
   } else {
 #pragma unroll
@@ -253,9 +271,9 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) add_rms_grad_kernel(Rm
       __syncthreads();
     }
     for (int i = threadIdx.x; i < CHUNKS * lanes * 8; i += kThreads) {
-      const int c = i;                                          // channel: chunk (c / 8), element c % 8
-      const int k = c / 8 / lanes, l = c / 8 % lanes, e = c & 7;
-      if (c < a.c) give(c, sums[(k * 8 + e) * lanes + l]);
+      if (i >= a.c) continue;                                   // channel i: element i % 8 of chunk i / 8, the last one's behind the others
+      const int k = i / 8 / lanes, l = i / 8 % lanes, e = (i & 7) + place_of(a.c, i / 8).twice;
+      give(i, sums[(k * 8 + e) * lanes + l]);
     }
   }
 }
@@ -280,17 +298,19 @@ __global__ void __launch_bounds__(kJoin * kJoin) add_rms_join_kernel(const float
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-struct RmsShape { int group, chunks, threads, rows; };      // rows of a workgroup at a time
+struct RmsShape { int group, chunks, threads, rows; bool block; };      // rows of a workgroup at a time; block: the workgroup has one
 RmsShape shape_of(int c) {
   const int chunks = (c + 7) / 8;
-  RmsShape s = {64, 1, kThreads, 1};
+  RmsShape s = {64, 1, kThreads, 1, false};
   if (chunks <= 64) {
     for (s.group = 1; s.group < chunks;) s.group *= 2;
-  } else if (chunks <= 64 * kMaxChunks) {
+  } else if (chunks <= 64 * kWaveChunks) {
     while (64 * s.chunks < chunks) s.chunks *= 2;
   } else {
-    s.threads = s.group = chunks <= 256 * kMaxChunks ? 256 : 512;
-    s.chunks = kMaxChunks;
+    s.block = true;
+    if (chunks > 4 * kThreads) s.threads = 512;
+    while (s.threads * s.chunks < chunks) s.chunks *= 2;
+    s.group = s.threads;
     return s;
   }
   s.rows = kThreads / s.group;
@@ -335,11 +355,13 @@ void launch(const RmsArgs& k, const RmsShape& s, hipStream_t stream) {
 }
 template <typename T, typename R, bool BACKWARD>
 void launch_of(const RmsArgs& k, const RmsShape& s, hipStream_t stream) {
-  if (s.rows == 1 && s.threads == s.group) launch<T, R, BACKWARD, kMaxChunks, true>(k, s, stream);
-  else if (s.chunks == 1) launch<T, R, BACKWARD, 1, false>(k, s, stream);
-  else if (s.chunks == 2) launch<T, R, BACKWARD, 2, false>(k, s, stream);
-  else if (s.chunks == 4) launch<T, R, BACKWARD, 4, false>(k, s, stream);
-  else launch<T, R, BACKWARD, 8, false>(k, s, stream);
+  if (!s.block && s.chunks == 1) launch<T, R, BACKWARD, 1, false>(k, s, stream);
+  else if (!s.block && s.chunks == 2) launch<T, R, BACKWARD, 2, false>(k, s, stream);
+  else if (!s.block) launch<T, R, BACKWARD, 4, false>(k, s, stream);
+  else if (s.chunks == 1) launch<T, R, BACKWARD, 1, true>(k, s, stream);
+  else if (s.chunks == 2) launch<T, R, BACKWARD, 2, true>(k, s, stream);
+  else if (s.chunks == 4) launch<T, R, BACKWARD, 4, true>(k, s, stream);
+  else launch<T, R, BACKWARD, 8, true>(k, s, stream);
 }
 template <bool BACKWARD>
 void launch_types(const cgtp_add_rms_args* a, const RmsArgs& k, const RmsShape& s, hipStream_t stream) {
