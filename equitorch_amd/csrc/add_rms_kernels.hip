@@ -143,14 +143,20 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) add_rms_kernel(RmsArgs
         sum = fmaf(v, v, sum);
       }
     }
+    // total may be x or the residual: all of a row is read first, by all wavefronts that share it
+    auto store_total = [&] {
+#pragma unroll
+      for (int k = 0; k < CHUNKS; ++k)
+        if (residual && a.total) store_eight((R*)a.total + at + place[k].c, t[k], in ? place[k].valid : 0);
+    };
+    if constexpr (!BLOCK) store_total();
     const float rstd = rsqrtf(row_sum<BLOCK>(sum, lanes, shared) * inv_c + a.eps);
+    if constexpr (BLOCK) store_total();
     if (a.rstd && in && lane == 0) a.rstd[row] = rstd;
 #pragma unroll
-    for (int k = 0; k < CHUNKS; ++k) {
-      if (residual && a.total) store_eight((R*)a.total + at + place[k].c, t[k], in ? place[k].valid : 0);
+    for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[k][e] = t[k][e] * rstd * w[k][e];
-    }
     if (!a.scale) {
 #pragma unroll
       for (int k = 0; k < CHUNKS; ++k) store_eight((T*)a.out + at + place[k].c, t[k], in ? place[k].valid : 0);

@@ -851,8 +851,8 @@ int cgtp_attn_backward(const cgtp_attn_args* args, void* stream);
 /* ---- root-mean-square norm after a residual's addition ------------------------------------------------------------
  *   t = x + residual, rounded to residual_dtype (residual NULL: t = x),  r = 1 / sqrt(mean_c t^2 + eps),  out = t r weight
  * x, out: (n_rows, channels) of dtype; residual, total (receives t; NULL: not wanted, and not written without a residual): the same of
- * residual_dtype; weight (channels) of weight_dtype, NULL: ones; rstd (n_rows) receives r, NULL: not wanted; all contiguous,
- * aligned to an element.  scale not NULL: 8 bits; scale (n_rows) receives s = max_c |out| / 448 (0 for a row of zeros, at least 2^-126
+ * residual_dtype, which may be the residual itself; weight (channels) of weight_dtype, NULL: ones; rstd (n_rows) receives r, NULL: not
+ * wanted; all contiguous, aligned to an element.  scale not NULL: 8 bits; scale (n_rows) receives s = max_c |out| / 448 (0 for a row of zeros, at least 2^-126
  * else, NaN for a row with an infinity or a NaN) and out, one byte an element, out / s in e4m3, to nearest.
  * cgtp_add_rms_backward reads weight, total (t; x where there is no residual), rstd, grad_out and grad_total (the gradient of t
  * apart from out's, NULL: none) and writes those of grad_x, grad_residual (the same values in residual_dtype) and grad_weight

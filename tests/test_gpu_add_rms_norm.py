@@ -38,7 +38,8 @@ TYPES = [(F32, F32, F32), (BF16, BF16, F32), (BF16, F32, BF16), (F16, F16, F16),
 
 @pytest.mark.parametrize("dtype,residual_type,weight_type", TYPES)
 @pytest.mark.parametrize("rows,channels", [(1, 1), (3, 7), (1000, 8), (257, 9), (30, 64), (5000, 100), (70, 256), (33, 513), (20, 1001),
-                                           (3, 2049), (9, 4096), (5, 4097), (2, 16391), (3, 32767), (20000, 40)])
+                                           (3, 2049), (9, 4096), (5, 4097), (2, 16391), (3, 32767), (20000, 40), (1500, 1025), (7, 1995), (6, 6001),
+                                           (3, 8200)])
 def test_add_rms_norm(device, dtype, residual_type, weight_type, rows, channels):
     from equitorch_amd.nn.functional import add_rms_norm
     gen = torch.Generator().manual_seed(stable_seed(rows, channels, str(dtype)))
@@ -311,3 +312,21 @@ def test_offsets_beyond_32_bits(device):
     size = (g[-tail:].double() * t * (t.square().mean(1, keepdim=True) + 1e-6).rsqrt()).abs().sum(0)
     # two sums of the same 3000 terms in other orders: each at most one rounding of the partial sum a term
     assert ((results[0][5] - results[1][5]).abs().double() <= 2 * 3000 * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.parametrize("n,c", [(70, 9), (50, 77), (40, 1001), (30, 1501), (20, 3003), (9, 9001), (3, 20003)])
+def test_total_in_the_residuals_place(device, n, c):
+    import ctypes as C
+    from equitorch_amd import _lib
+    from equitorch_amd.nn.functional import add_rms_norm
+    gen = torch.Generator().manual_seed(n)
+    for dtype in (torch.float32, torch.bfloat16):
+        x, r = (torch.randn(n, c, generator=gen).to(device, dtype) for _ in range(2))
+        out, total = add_rms_norm(x, r, eps=1e-6)
+        got = torch.empty_like(x)
+        a = _lib.AddRmsArgs()
+        a.x, a.residual, a.total, a.out = x.data_ptr(), r.data_ptr(), r.data_ptr(), got.data_ptr()
+        a.n_rows, a.channels, a.eps = n, c, 1e-6
+        a.dtype = a.residual_dtype = a.weight_dtype = _lib.dtype_code(dtype)
+        _lib.check(_lib.lib.cgtp_add_rms_forward(C.byref(a), _lib.stream_ptr(x.device)), "cgtp_add_rms_forward")
+        assert torch.equal(r, total) and torch.equal(got, out)
