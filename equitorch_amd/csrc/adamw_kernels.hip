@@ -4,7 +4,7 @@
 //   p <- p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Bound by memory: 28 bytes an element in fp32 with states in 32 bits, 16 with states in 8.  The tensors' addresses are kernel
-// arguments, so that a launch takes dozens of tensors and nothing has to reach the GPU before it; a workgroup takes a chunk of one
+// arguments, so that a launch takes 52 to 64 tensors and nothing has to reach the GPU before it; a workgroup takes a chunk of one
 // tensor.  The step's number is on the GPU (a recorded graph counts on when it is replayed): every workgroup reads it and
 // works its factors out, and a launch behind them adds one.
 //
@@ -22,26 +22,35 @@
 namespace cgtp {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / 64, kBlock = CGTP_ADAMW_BLOCK, kAtOnce = 48;
+constexpr int kThreads = 256, kWaves = kThreads / 64, kBlock = CGTP_ADAMW_BLOCK;
 static_assert(kBlock == 256, "four elements for each lane");
 
+template <bool MASTER, bool EIGHT>
 struct Entry {
   void* p;
   const void* g;
   void *m, *v;
-  float *m_scale, *v_scale, *master;
   const float* step;
-  unsigned n, first, number;      // first: its first chunk among the launch's; number: the tensor's, for the random bits
+  void* more[2 * EIGHT + MASTER > 0 ? 2 * EIGHT + MASTER : 1];      // scales of m and v, then the copy in 32 bits
+  unsigned n, number;             // number: the tensor's, for the random bits
+  __device__ __forceinline__ float* m_scale() const { return (float*)more[0]; }
+  __device__ __forceinline__ float* v_scale() const { return (float*)more[1]; }
+  __device__ __forceinline__ float* master() const { return (float*)more[2 * EIGHT]; }
 };
+// As many tensors as 4 KB of arguments hold, no more than a wavefront finds its own among at once.
+template <bool MASTER, bool EIGHT> constexpr int kAtOnce = std::min<int>(64, (4096 - 72) / (sizeof(Entry<MASTER, EIGHT>) + 4));
+template <bool MASTER, bool EIGHT>
 struct StepArgs {
-  Entry entry[kAtOnce];
+  Entry<MASTER, EIGHT> entry[kAtOnce<MASTER, EIGHT>];
+  unsigned first[kAtOnce<MASTER, EIGHT>];      // each one's first chunk among the launch's
   double lr, decay;
   const float* lr_ptr;            // null: lr
   float b1, b1_rest, log_b1, b2, b2_rest, log_b2, eps;      // b1_rest: with the sign of the step
   unsigned seed;
   int entries, blocks;            // blocks: of 256 elements, in a chunk
 };
-static_assert(sizeof(StepArgs) <= 4096);
+static_assert(sizeof(StepArgs<false, false>) <= 4096 && sizeof(StepArgs<false, true>) <= 4096 && sizeof(StepArgs<true, false>) <= 4096 &&
+              sizeof(StepArgs<true, true>) <= 4096);
 
 struct Factors {
   float keep, size, root;         // 1 - lr decay, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
@@ -132,7 +141,8 @@ __device__ __forceinline__ float block_scale(const float (&s)[4], float& inverse
   for (int e = 0; e < 4; ++e) top = std::max(top, __float_as_uint(s[e]) & 0x7fffffffu);
   const float most = __uint_as_float(wave_max(top));
   const float scale = most == 0.f ? 0.f : most < INFINITY ? std::max(most * (1.f / 448.f), 0x1p-126f) : NAN;
-  inverse = most == 0.f ? 0.f : __builtin_amdgcn_rcpf(scale);
+  inverse = __builtin_amdgcn_rcpf(scale);      // to nearest: by what is left over
+  inverse = most == 0.f ? 0.f : fmaf(fmaf(inverse, -scale, 1.f), inverse, inverse);
   return scale;
 }
 
@@ -149,6 +159,15 @@ __device__ __forceinline__ float root(float v) {
   return __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v) * (small ? 0x1p-32f : 1.f);
 }
 
+// The same to nearest, as the reciprocal of a scale: the states in 8 bits are then, bit for bit, those of the formulas in elementary operations
+// of 32 bits.  A last place of a root decides some roundings of it, and a block whose largest root is kept one value lower has that scale in all
+// steps after.  115 million elements, bf16 with copies: 405 us, 401 with roots that err a unit in the last place.
+__device__ __forceinline__ float near_root(float v) {
+  const bool small = v < 0x1p-96f;
+  const float w = small ? v * 0x1p64f : v, y = __builtin_amdgcn_rsqf(std::max(w, 0x1p-120f)), s = w * y;
+  return fmaf(fmaf(-s, s, w) * 0.5f, y, s) * (small ? 0x1p-32f : 1.f);
+}
+
 // A value rounded to fp32 here: neither a product that a sum takes unrounded nor a result that goes on to 16 bits unrounded, so
 // that what is stored in 16 and in 8 bits is the rounding of the number in 32 that the formula says.
 __device__ __forceinline__ float rounded(float v) {
@@ -156,34 +175,50 @@ __device__ __forceinline__ float rounded(float v) {
   return v;
 }
 
-// Four elements of one lane.
-template <typename T, bool MASTER, bool EIGHT, bool WHOLE>
-__device__ __forceinline__ void step_block(const StepArgs& a, const Entry& t, const Factors& f, unsigned at, unsigned block) {
-  const int left = (int)(t.n - at);
+// Four elements of one lane, as they are in memory.
+template <typename T, bool MASTER, bool EIGHT>
+struct Elements {
   float p[4], g[4], m[4], v[4];
-  if constexpr (MASTER) load4<float, WHOLE>(p, t.master + at, left);
-  else load4<T, WHOLE>(p, (const T*)t.p + at, left);
-  load4<T, WHOLE>(g, (const T*)t.g + at, left);
+  unsigned cm, cv;
+  float sm, sv;
+};
+template <typename T, bool MASTER, bool EIGHT, bool WHOLE>
+__device__ __forceinline__ void load_block(Elements<T, MASTER, EIGHT>& x, const Entry<MASTER, EIGHT>& t, unsigned at, unsigned block) {
+  const int left = (int)(t.n - at);
+  if constexpr (MASTER) load4<float, WHOLE>(x.p, t.master() + at, left);
+  else load4<T, WHOLE>(x.p, (const T*)t.p + at, left);
+  load4<T, WHOLE>(x.g, (const T*)t.g + at, left);
   if constexpr (EIGHT) {
-    const unsigned cm = load_codes<WHOLE>((const uint8_t*)t.m + at, left), cv = load_codes<WHOLE>((const uint8_t*)t.v + at, left);
-    decode(m, cm, t.m_scale[block]);
-    decode(v, cv, t.v_scale[block]);
+    x.cm = load_codes<WHOLE>((const uint8_t*)t.m + at, left);
+    x.cv = load_codes<WHOLE>((const uint8_t*)t.v + at, left);
+    x.sm = t.m_scale()[block];
+    x.sv = t.v_scale()[block];
+  } else {
+    load4<float, WHOLE>(x.m, (const float*)t.m + at, left);
+    load4<float, WHOLE>(x.v, (const float*)t.v + at, left);
+  }
+}
+template <typename T, bool MASTER, bool EIGHT, bool WHOLE>
+__device__ __forceinline__ void step_block(Elements<T, MASTER, EIGHT>& x, const StepArgs<MASTER, EIGHT>& a, const Entry<MASTER, EIGHT>& t, const Factors& f,
+                                           unsigned at, unsigned block) {
+  const int left = (int)(t.n - at);
+  float (&p)[4] = x.p, (&g)[4] = x.g, (&m)[4] = x.m, (&v)[4] = x.v;
+  if constexpr (EIGHT) {
+    decode(m, x.cm, x.sm);
+    decode(v, x.cv, x.sv);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = rounded(v[e] * v[e]);
-  } else {
-    load4<float, WHOLE>(m, (const float*)t.m + at, left);
-    load4<float, WHOLE>(v, (const float*)t.v + at, left);
   }
   float r[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     m[e] = rounded(m[e] * a.b1) + rounded(g[e] * a.b1_rest);
     v[e] = rounded(v[e] * a.b2) + rounded(g[e] * g[e] * a.b2_rest);
-    r[e] = root(v[e]);
+    r[e] = EIGHT ? near_root(v[e]) : root(v[e]);
     // the reciprocal errs a unit in the last place
     p[e] = rounded(rounded(p[e] * f.keep) - rounded(f.size * (m[e] * __builtin_amdgcn_rcpf(rounded(r[e] * f.root) + a.eps))));
   }
-  if constexpr (MASTER) store4<float, WHOLE>(t.master + at, p, left);
+  if constexpr (MASTER) store4<float, WHOLE>(t.master() + at, p, left);
   store4<T, WHOLE>((T*)t.p + at, p, left);
   if constexpr (EIGHT) {
     float inverse, q[4];
@@ -196,8 +231,8 @@ __device__ __forceinline__ void step_block(const StepArgs& a, const Entry& t, co
     for (int e = 0; e < 4; ++e) q[e] = at_random(std::min(r[e] * inverse, 448.f), mix(f.key + (at + e) * 0x9E3779B1u) >> 12);
     store_codes<WHOLE>((uint8_t*)t.v + at, encode(q), left);
     if ((threadIdx.x & 63) == 0) {
-      t.m_scale[block] = m_scale;
-      t.v_scale[block] = v_scale;
+      t.m_scale()[block] = m_scale;
+      t.v_scale()[block] = v_scale;
     }
   } else {
     store4<float, WHOLE>((float*)t.m + at, m, left);
@@ -206,14 +241,23 @@ __device__ __forceinline__ void step_block(const StepArgs& a, const Entry& t, co
 }
 
 template <typename T, bool MASTER, bool EIGHT>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(StepArgs a) {
-  int lo = 0, hi = a.entries - 1;      // the last tensor whose first chunk is not behind this one
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.entry[mid].first <= blockIdx.x) lo = mid;
-    else hi = mid - 1;
-  }
-  const Entry t = a.entry[lo];
+__global__ void __launch_bounds__(kThreads) adamw_kernel(StepArgs<MASTER, EIGHT> a) {
+  const int lane = threadIdx.x & 63;
+  // the last tensor whose first chunk is not behind this one: every lane asks for one
+  const unsigned long long before = __ballot(lane < a.entries && a.first[std::min(lane, kAtOnce<MASTER, EIGHT> - 1)] <= blockIdx.x);
+  const int own = __popcll(before) - 1;
+  const Entry<MASTER, EIGHT> t = a.entry[own];
+  const unsigned first = (blockIdx.x - a.first[own]) * (unsigned)a.blocks, all = (t.n + kBlock - 1) / kBlock, end = std::min(first + a.blocks, all);
+  unsigned b = __builtin_amdgcn_readfirstlane(first + (threadIdx.x >> 6));
+  if (b >= end) return;
+  // lanes beyond the end take part in the block's scale
+  auto place = [&] { return b < t.n / kBlock ? b * kBlock + lane * 4 : std::min(b * kBlock + lane * 4, t.n); };
+  Elements<T, MASTER, EIGHT> x;
+  auto load = [&] {
+    if (b < t.n / kBlock) load_block<T, MASTER, EIGHT, true>(x, t, place(), b);
+    else load_block<T, MASTER, EIGHT, false>(x, t, place(), b);
+  };
+  load();                          // on its way while the factors are worked out (55 tensors of 3 million elements: 20 us -> 15 with one launch for two)
   Factors f;
   {
     const float now = *t.step + 1.f;
@@ -224,12 +268,11 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(StepArgs a) {
     f.root = 1.f / sqrtf(-expm1f(now * a.log_b2));
     f.key = mix(a.seed * 0x85157AF5u + t.number * 0x9E3779B1u + (unsigned)now * 0xC2B2AE63u);
   }
-  const int lane = threadIdx.x & 63;
-  const unsigned first = (blockIdx.x - t.first) * (unsigned)a.blocks, all = (t.n + kBlock - 1) / kBlock, end = std::min(first + a.blocks, all);
-  for (unsigned b = __builtin_amdgcn_readfirstlane(first + (threadIdx.x >> 6)); b < end; b += kWaves) {
-    const unsigned at = b * kBlock + lane * 4;
-    if (b < t.n / kBlock) step_block<T, MASTER, EIGHT, true>(a, t, f, at, b);
-    else step_block<T, MASTER, EIGHT, false>(a, t, f, std::min(at, t.n), b);      // lanes beyond the end take part in the block's scale
+  for (;;) {
+    if (b < t.n / kBlock) step_block<T, MASTER, EIGHT, true>(x, a, t, f, place(), b);
+    else step_block<T, MASTER, EIGHT, false>(x, a, t, f, place(), b);
+    if ((b += kWaves) >= end) return;
+    load();
   }
 }
 
@@ -262,27 +305,9 @@ int adamw_check(const cgtp_adamw_args* a) {
   return CGTP_OK;
 }
 
-typedef void (*Kernel)(StepArgs);
-template <typename T>
-Kernel kernel_of(bool master, bool eight) {
-  if constexpr (sizeof(T) == 2)
-    if (master) return eight ? adamw_kernel<T, true, true> : adamw_kernel<T, true, false>;
-  return eight ? adamw_kernel<T, false, true> : adamw_kernel<T, false, false>;
-}
-
-}  // namespace
-}  // namespace cgtp
-
-extern "C" {
-
-int cgtp_adamw_step(const cgtp_adamw_args* a, void* stream) {
-  using namespace cgtp;
-  if (int rc = adamw_check(a)) return rc;
-  if (a->n_tensors == 0) return CGTP_OK;
-  const bool eight = a->state_bits == 8, master = a->master != 0;
-  const Kernel kernel = a->dtype == CGTP_F32 ? kernel_of<float>(master, eight)
-                        : a->dtype == CGTP_BF16 ? kernel_of<bf16_t>(master, eight) : kernel_of<f16_t>(master, eight);
-  StepArgs s = {};
+template <typename T, bool MASTER, bool EIGHT>
+void adamw_launch(const cgtp_adamw_args* a, hipStream_t q) {
+  StepArgs<MASTER, EIGHT> s = {};
   s.log_b1 = (float)std::log(a->beta1);
   s.log_b2 = (float)std::log(a->beta2);
   s.lr = a->lr;
@@ -298,10 +323,9 @@ int cgtp_adamw_step(const cgtp_adamw_args* a, void* stream) {
   for (int64_t i = 0; i < a->n_tensors; ++i) all += (a->tensors[i].n + kBlock - 1) / kBlock;
   // Blocks of a chunk: eight for each wavefront of a workgroup, fewer where that leaves compute units idle.
   s.blocks = kWaves * (int)std::max<int64_t>(1, std::min<int64_t>(8, all / (kWaves * 1024)));
-  hipStream_t q = (hipStream_t)stream;
   unsigned chunks = 0;
   auto launch = [&] {
-    if (s.entries) hipLaunchKernelGGL(kernel, dim3(chunks), dim3(kThreads), 0, q, s);
+    if (s.entries) hipLaunchKernelGGL((adamw_kernel<T, MASTER, EIGHT>), dim3(chunks), dim3(kThreads), 0, q, s);
     s.entries = 0;
     chunks = 0;
   };
@@ -310,12 +334,40 @@ int cgtp_adamw_step(const cgtp_adamw_args* a, void* stream) {
     if (t.n == 0) continue;
     // a grid has fewer than 2^32 threads
     const unsigned each = (unsigned)((t.n + kBlock * s.blocks - 1) / (kBlock * s.blocks));
-    if (s.entries == kAtOnce || chunks + each >= (1u << 24)) launch();
-    s.entry[s.entries++] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.master, t.step,
-                            (unsigned)t.n, chunks, (unsigned)t.number};
+    if (s.entries == kAtOnce<MASTER, EIGHT> || chunks + each >= (1u << 24)) launch();
+    Entry<MASTER, EIGHT>& e = s.entry[s.entries];
+    e = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.step, {}, (unsigned)t.n, (unsigned)t.number};
+    if constexpr (EIGHT) {
+      e.more[0] = t.exp_avg_scale;
+      e.more[1] = t.exp_avg_sq_scale;
+    }
+    if constexpr (MASTER) e.more[2 * EIGHT] = t.master;
+    s.first[s.entries++] = chunks;
     chunks += each;
   }
   launch();
+}
+template <typename T>
+void adamw_launch(const cgtp_adamw_args* a, hipStream_t q) {
+  const bool eight = a->state_bits == 8;
+  if constexpr (sizeof(T) == 2)
+    if (a->master) return eight ? adamw_launch<T, true, true>(a, q) : adamw_launch<T, true, false>(a, q);
+  eight ? adamw_launch<T, false, true>(a, q) : adamw_launch<T, false, false>(a, q);
+}
+
+}  // namespace
+}  // namespace cgtp
+
+extern "C" {
+
+int cgtp_adamw_step(const cgtp_adamw_args* a, void* stream) {
+  using namespace cgtp;
+  if (int rc = adamw_check(a)) return rc;
+  if (a->n_tensors == 0) return CGTP_OK;
+  hipStream_t q = (hipStream_t)stream;
+  if (a->dtype == CGTP_F32) adamw_launch<float>(a, q);
+  else if (a->dtype == CGTP_BF16) adamw_launch<bf16_t>(a, q);
+  else adamw_launch<f16_t>(a, q);
   CountArgs c;
   for (int64_t i = 0; i < a->n_tensors;) {
     for (c.n = 0; c.n < kSteps && i < a->n_tensors; ++i) c.step[c.n++] = a->tensors[i].step;

@@ -472,3 +472,45 @@ def test_the_largest_tensor(device):
             if name == "root_avg_sq":
                 continue                             # rounded at random by the element's place
             assert torch.equal(a[name].reshape(-1)[-b[name].numel():].float(), b[name].reshape(-1).float()), name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_eight_bit_states_are_those_of_elementary_operations(device, dtype):
+    """Every step's states, bit for bit, by the formulas in operations of 32 bits, each rounded once; roots of 2^-6 and more in units
+    of their scale, below which the random bits are added at another place."""
+    n, seed, number, (b1, b2) = 256 * 500, 77, 1, (0.9, 0.99)
+    gen = torch.Generator().manual_seed(4)
+    other, p = (torch.nn.Parameter(torch.randn(k, generator=gen).to(device, dtype)) for k in (5, n))
+    opt = AdamW([other, p], lr=1e-3, betas=(b1, b2), state_bits=8, seed=seed)
+    m = v = torch.zeros(500, 256, device=device)
+
+    def mixed(h):
+        h = (h ^ (h >> 16)) * 0x9C8F2D35 & 0xFFFFFFFF
+        h = (h ^ (h >> 15)) * 0xB5297A4D & 0xFFFFFFFF
+        return h ^ (h >> 16)
+
+    def scales(x):
+        scale = (x.abs().amax(1) * (1 / 448)).clamp(min=2.0 ** -126)
+        return scale, (1.0 / scale)[:, None]
+    element = torch.arange(n, device=device).view(500, 256)
+    for step in range(1, 6):
+        g = torch.randn(n, generator=gen).mul(torch.rand(n, generator=gen) + 0.1).to(device, dtype)
+        p.grad = g
+        opt.step()
+        g = g.float().view(500, 256)
+        m, v = m * b1 + g * (1 - b1), v * b2 + g * g * (1 - b2)
+        state = opt.state[p]
+        scale, inverse = scales(m)
+        codes = (m * inverse).clamp(-448, 448).to(torch.float8_e4m3fn)
+        assert torch.equal(state["exp_avg_scale"], scale) and torch.equal(state["exp_avg"].view(500, 256).view(torch.uint8), codes.view(torch.uint8))
+        m = codes.float() * scale[:, None]
+        r = v.sqrt()
+        scale, inverse = scales(r)
+        q = (r * inverse).clamp(max=448.0)
+        key = mixed(torch.tensor(seed * 0x85157AF5 + number * 0x9E3779B1 + step * 0xC2B2AE63, device=device) & 0xFFFFFFFF)
+        bits = (mixed((key + element * 0x9E3779B1) & 0xFFFFFFFF) >> 12).int()
+        want = ((q.view(torch.int32) + bits) & -(1 << 20)).view(torch.float32)
+        got = state["root_avg_sq"].view(500, 256).float()
+        normal = q >= 2.0 ** -6
+        assert torch.equal(state["root_avg_sq_scale"], scale) and torch.equal(got[normal], want[normal]) and normal.float().mean() > 0.99
+        v = (got * scale[:, None]).square()
