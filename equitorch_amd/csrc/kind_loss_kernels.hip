@@ -6,10 +6,14 @@
 // Rows with a kind are taken together first (the others cost nothing and are not read, whatever they hold): their numbers in
 // order, and a copy of them with rows of whole aligned chunks.  The forward forms the logits tile by tile and keeps a running
 // maximum and sum for each row; the kinds are cut into `splits` ranges where there are few rows, whose statistics are joined in order.
-// The backward forms the logits again, a piece of the kinds at a time: (p - [k = y]) (1 - tanh^2) is rounded to the operands'
-// type as the operand of the two products it enters, small enough to stay in the caches between them.  g_i multiplies dx
-// afterwards; for dW it multiplies the rows of x, divided by the largest |g| (exact where all are equal).  In fp16 the
-// probabilities are scaled by 2^15 into its range.
+// The backward forms the logits again, a piece of the kinds at a time (of rows and kinds up to 512 MB): (p - [k = y]) (1 - tanh^2) is rounded
+// to the operands' type as the operand of the two products it enters.  g_i multiplies dx afterwards; for dW it multiplies the rows of x,
+// divided by the largest |g| (exact where all are equal).  In fp16 the probabilities are scaled by 2^15 into its range.
+//
+// Bound by the matrix cores: 2 N K C operations forward, 6 N K C backward, where a calculation that kept all logits would do 4.
+// 16384 rows, 30011 kinds, 256 bf16 channels: statistics 250-290 us (870-1000 TFLOP/s), logits again and dx 500-580 (870-1000), the
+// table's gradient 320 (785), joins and copies of rows 75; 4253 rows with a kind, 50021 kinds, 500 fp16 channels, capped: 255-290 us (730-830).
+// Small calls: the launches, three forward and up to eight backward.
 #include "gff_gemm.h"
 
 #include <algorithm>
@@ -20,7 +24,7 @@ namespace {
 
 constexpr int kTile = 128, kRowBlocks = 1024, kRowThreads = 256;
 // Tiles of the products of both operands from LDS: in fp32, whose matrix instructions are slow, small ones cost nothing and keep more of the
-// GPU busy (9000 rows, 100 kinds, 128 channels: logits 17 us with tiles of 128, 7 with these).
+// GPU busy (9000 rows, 100 kinds, 128 channels: statistics 17 us with tiles of 128, 12 with these, the logits' gradients 18 and 11).
 template <typename T> constexpr int kTileOf = sizeof(T) == 4 ? 64 : kTile;
 template <typename T> constexpr int kLds = kTileOf<T> * 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -259,10 +263,10 @@ __device__ __forceinline__ void logits_tile(GemmAcc<kTileOf<T>>& acc, char* lds,
   }, [&](int64_t) { return w; });
 }
 
-// Maximum and sum of `splits` statistics `each` places apart, eight of them on their way at a time; base: the maximum, 0 where it is -inf.
-__device__ __forceinline__ void join_stats(const float2* p, int64_t each, int splits, float& base, float& sum) {
-  float most = -INFINITY;
-  base = sum = 0.f;
+// Maximum and sum of `splits` statistics `each` places apart, eight of them on their way at a time.
+__device__ __forceinline__ void join_stats(const float2* p, int64_t each, int splits, float& most, float& sum) {
+  most = -INFINITY;
+  sum = 0.f;
   for (int s0 = 0; s0 < splits; s0 += 8) {
     float2 v[8];
     float now = most;
@@ -271,12 +275,29 @@ __device__ __forceinline__ void join_stats(const float2* p, int64_t each, int sp
       v[k] = s0 + k < splits ? p[(s0 + k) * each] : float2{-INFINITY, 0.f};
       now = fmaxf(now, v[k].x);
     }
-    base = now == -INFINITY ? 0.f : now;
+    const float base = now == -INFINITY ? 0.f : now;
     sum *= __builtin_amdgcn_exp2f(most - base);
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum += v[k].y * __builtin_amdgcn_exp2f(v[k].x - base);
     most = now;
   }
+}
+// The same by `slices` threads of a workgroup, 256 / slices apart, that have every slices-th statistic each; the first of them has the
+// result.  478 rows with statistics of up to 192 ranges each: 17 us with a thread for a row, 5 with sixteen.
+__device__ __forceinline__ void join_stats(const float2* p, int64_t each, int splits, int slices, float& most, float& sum) {
+  __shared__ float2 shared[256];
+  const int per = 256 / slices, slice = threadIdx.x / per;
+  join_stats(p + slice * each, each * slices, splits > slice ? (splits - slice + slices - 1) / slices : 0, most, sum);
+  if (slices == 1) return;
+  shared[threadIdx.x] = {most, sum};
+  __syncthreads();
+  if (slice == 0) join_stats(shared + threadIdx.x, per, slices, most, sum);
+}
+// Threads that share a sum of up to `terms` for each of n results: at least eight terms each, and no more than some 64 K threads.
+int slices_of(int64_t n, int64_t terms) {
+  int slices = 1;
+  while (slices < 32 && n * slices < 32 * 1024 && terms >= 16 * slices) slices *= 2;
+  return slices;
 }
 // The loss and the logarithm of the sum (log2 units) of a row from its own kind's logit, a maximum and a sum.
 __device__ __forceinline__ void give_loss(float* loss, float* lse, int row, float at, float top, float sum) {
@@ -367,12 +388,12 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_stats_kernel(LogitArgs<T
 
 // The same from the statistics of several splits.
 __global__ void __launch_bounds__(256) loss_join_kernel(const float2* stats, const float* at, const int* rows, const int* count, int64_t n,
-                                                        int splits, float* loss, float* lse) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= *count) return;
-  float base, sum;
-  join_stats(stats + i, n, splits, base, sum);
-  give_loss(loss, lse, rows[i], at[i], base, sum);
+                                                        int splits, int slices, float* loss, float* lse) {
+  const int per = 256 / slices;
+  const int64_t i = (int64_t)blockIdx.x * per + threadIdx.x % per, have = *count;
+  float top, sum;
+  join_stats(stats + i, n, i < have ? splits : 0, slices, top, sum);
+  if (i < have && (int)threadIdx.x < per) give_loss(loss, lse, rows[i], at[i], top, sum);
 }
 
 // (p - [k = y]) (1 - tanh^2) of a tile of rows x kinds.
@@ -409,7 +430,7 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_dz_kernel(LogitArgs<T> a
 // The gradients' products, up to 256 channels, are of the same kind.  Where x has a gradient one kernel forms dz and adds up dx: a
 // lane's sixteen kinds of dz are the next product's operand as they lie, and the stage in LDS, read through the transposing
 // loads, the other.  For the table's gradient dz is kept in blocks of 32 rows x 32 kinds in the order in which that product's operand lies in
-// a wavefront (turned over in LDS), so that it comes straight to registers while rows of x go by in LDS.
+// a wavefront (turned over in LDS), so that it passes through LDS as it lies while rows of x go by beside it.
 //
 // In LDS a stage is 32 rows of 2 KS chunks, chunk c of row i at c ^ chunk_mix(i): sixteen lanes that read one chunk of
 // neighbouring rows find it in different banks, and so do the transposing loads, of a pair of chunks of four rows.  Row i is that of kind
@@ -929,14 +950,14 @@ __global__ void __launch_bounds__(256, 2) loss_table_kernel(TableArgs<T> a) {
 
 // loss and the logarithm of the sum from the shares' statistics.
 __global__ void __launch_bounds__(256) loss_walk_join_kernel(const float2* stats, const float* at, const int* rows, const int* count, int rows_of_tile,
-                                                             int64_t kinds, float* loss, float* lse) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = *count;
-  if (i >= n) return;
+                                                             int64_t kinds, int slices, float* loss, float* lse) {
+  const int per = 256 / slices;
+  const int64_t i = (int64_t)blockIdx.x * per + threadIdx.x % per, n = *count;
   const Share share = share_out(kStats, n, rows_of_tile, kinds);
   if (share.splits == 1) return;   // given already
-  float base, sum;
-  join_stats(stats + i / rows_of_tile * share.splits * rows_of_tile + i % rows_of_tile, rows_of_tile, share.splits, base, sum);
-  give_loss(loss, lse, rows[i], at[i], base, sum);
+  float top, sum;
+  join_stats(stats + i / rows_of_tile * share.splits * rows_of_tile + i % rows_of_tile, rows_of_tile, i < n ? share.splits : 0, slices, top, sum);
+  if (i < n && (int)threadIdx.x < per) give_loss(loss, lse, rows[i], at[i], top, sum);
 }
 
 // Steps of 16 channels of the kernels above for a width, 0: not theirs.
@@ -1060,30 +1081,43 @@ __global__ void __launch_bounds__(256) loss_dx_join_kernel(const float* planes, 
   const int64_t row = i / c;
   if (row >= n) return;
   float s = 0.f;
+#pragma unroll 4
   for (int k = 0; k < splits; ++k) s += planes[k * r_most * c + i];
   grad_x[(int64_t)rows[r0 + row] * c + (i - row * c)] = (T)(s * (g[r0 + row] * scale));
 }
 
-// The same from the planes of the kernel that forms dz too; steps: of 16 channels.
+// The same from the planes of the kernel that forms dz too; steps: of 16 channels.  `slices` threads of a workgroup share out the planes
+// (21 rows, 23215 kinds, 106 channels: 55 us with one thread, 6 with sixteen).
 template <typename T>
 __global__ void __launch_bounds__(256) loss_walk_dx_kernel(const float* planes, const int* rows, const float* g, const int* count, int64_t r0,
                                                            int64_t r_most, int64_t piece, int rows_of_tile, int steps, int c, float scale,
-                                                           int one_piece, T* grad_x) {
+                                                           int one_piece, int slices, T* grad_x) {
+  __shared__ f32x4 shared[256];
   const int64_t n = std::min<int64_t>(*count - r0, r_most);
   if (n <= 0) return;
   const Share share = share_out(kDx, n, rows_of_tile, piece);
   if (one_piece && share.splits == 1) return;      // there already
   // a thread for four channels of a row, in the order of the planes
   const int each = rows_of_tile * 16 * steps / 4, part = each / 4, blocks = steps * 2;       // of a tile, a wavefront; of 8 channels
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, tile = i / each;
-  if (tile >= share.tiles) return;
+  const int per = 256 / slices, slice = threadIdx.x / per;
+  const int64_t i = (int64_t)blockIdx.x * per + threadIdx.x % per, tile = i / each;
   const int at = (int)(i - tile * each), wave = at / part, of_wave = at % part, lane = of_wave & 63, block = of_wave >> 6;
   const int64_t row = tile * rows_of_tile + (wave * (rows_of_tile / 128) + block / blocks) * 32 + (lane & 31);
   const int ch = block % blocks * 8 + 4 * (lane >> 5), left = c - ch;
-  if (row >= n || left <= 0) return;
-  const f32x4* p = reinterpret_cast<const f32x4*>(planes) + tile * share.splits * each + at;
+  const bool in = tile < share.tiles && row < n && left > 0;
   f32x4 s = {};
-  for (int k = 0; k < share.splits; ++k) s += p[(int64_t)k * each];
+  if (in) {
+    const f32x4* p = reinterpret_cast<const f32x4*>(planes) + tile * share.splits * each + at;
+#pragma unroll 4
+    for (int k = slice; k < share.splits; k += slices) s += p[(int64_t)k * each];
+  }
+  if (slices > 1) {
+    shared[threadIdx.x] = s;
+    __syncthreads();
+    if (slice) return;
+    for (int k = 1; k < slices; ++k) s += shared[k * per + threadIdx.x];
+  }
+  if (!in) return;
   T out[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) out[e] = (T)(s[e] * (g[r0 + row] * scale));
@@ -1206,9 +1240,10 @@ Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
   p.x = take(n * p.ld * size);
   p.table = p.ld == c && aligned16(a->table) ? -1 : take(k * p.ld * size);
   if (!backward) {
-    // 1024 workgroups where the table has 256 kinds for each; a split is whole tiles
+    // up to 1024 workgroups of whole tiles, of which two go one after the other rather than be joined: 26 rows, 4216 kinds, 401 fp32
+    // channels 42 us with 256 kinds to a workgroup, 12.5 with 64
     const int64_t tiles = ceil_div(n, p.tile), k_tiles = ceil_div(k, p.tile);
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(ceil_div(k, 256), 1024 / std::max<int64_t>(1, tiles)));
+    const int64_t splits = k_tiles <= 2 ? 1 : std::max<int64_t>(1, std::min<int64_t>(k_tiles, 1024 / std::max<int64_t>(1, tiles)));
     p.each = (int)(ceil_div(k_tiles, splits) * p.tile);
     p.splits = (int)ceil_div(k, p.each);
     p.at = take(4 * n);
@@ -1320,13 +1355,17 @@ int loss_forward(const cgtp_kind_loss_args* a, hipStream_t s) {
   l.at = (float*)(ws + p.at);
   if (p.steps) {
     walk_launch<kStats>(p.steps, l, a->n_rows, a->n_kinds, s);
-    if (a->n_kinds > kLeastKinds) hipLaunchKernelGGL(loss_walk_join_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count,
-                       walk_rows(p.steps, kStats), a->n_kinds, a->loss, a->lse);
+    const int slices = slices_of(a->n_rows, ceil_div(a->n_kinds, kLeastKinds));
+    if (a->n_kinds > kLeastKinds)
+      hipLaunchKernelGGL(loss_walk_join_kernel, dim3((unsigned)ceil_div(a->n_rows * slices, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count,
+                         walk_rows(p.steps, kStats), a->n_kinds, slices, a->loss, a->lse);
     return launch_status();
   }
   hipLaunchKernelGGL(loss_stats_kernel<T>, dim3((unsigned)(ceil_div(a->n_rows, p.tile) * p.splits)), dim3(kGemmThreads), 0, s, l);
-  if (p.splits > 1) hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)ceil_div(a->n_rows, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count, a->n_rows,
-                     p.splits, a->loss, a->lse);
+  const int slices = slices_of(a->n_rows, p.splits);
+  if (p.splits > 1)
+    hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)ceil_div(a->n_rows * slices, 256)), dim3(256), 0, s, l.stats, l.at, r.rows, r.count, a->n_rows,
+                       p.splits, slices, a->loss, a->lse);
   return launch_status();
 }
 
@@ -1405,12 +1444,15 @@ int loss_backward(const cgtp_kind_loss_args* a, hipStream_t s) {
       }
     }
     const int64_t rows_now = std::min(p.chunk, a->n_rows - r0);
-    if (p.fused && (!one_piece || p.piece > kLeastKinds))
-      hipLaunchKernelGGL(loss_walk_dx_kernel<T>, dim3((unsigned)ceil_div(up_to(rows_now, walk_rows(p.steps, kDx)) * p.ld / 4, 256)), dim3(256), 0, s,
-                         l.planes, r.rows, r.row_g, r.count, r0, p.chunk, p.piece, walk_rows(p.steps, kDx), p.steps, a->channels, scale, one_piece, (T*)a->grad_x);
-    else if (a->grad_x && !p.fused && !d.grad_x)
+    if (p.fused && (!one_piece || p.piece > kLeastKinds)) {
+      const int64_t threads = up_to(rows_now, walk_rows(p.steps, kDx)) * p.ld / 4;
+      const int slices = slices_of(threads, ceil_div(p.piece, kLeastKinds));
+      hipLaunchKernelGGL(loss_walk_dx_kernel<T>, dim3((unsigned)ceil_div(threads * slices, 256)), dim3(256), 0, s, l.planes, r.rows, r.row_g, r.count, r0,
+                         p.chunk, p.piece, walk_rows(p.steps, kDx), p.steps, a->channels, scale, one_piece, slices, (T*)a->grad_x);
+    } else if (a->grad_x && !p.fused && !d.grad_x) {
       hipLaunchKernelGGL(loss_dx_join_kernel<T>, dim3((unsigned)ceil_div(rows_now * c, 256)), dim3(256), 0, s, (const float*)(ws + p.dx), p.dx_splits,
                          r.rows, r.row_g, r.count, r0, p.chunk, a->channels, scale, (T*)a->grad_x);
+    }
   }
   return launch_status();
 }
