@@ -1,6 +1,7 @@
 """Loader of the PyTorch C++ extension over the C ABI (``equitorch_amd/lib/_cgtp_torch.so``, built from
 ``csrc/torch_shim/cgtp_torch.cpp``): the autograd nodes and per-call marshalling of the fused edge product, of the embedding, of
-the attention among the nodes of a structure and of the gated feed-forward block in C++.
+the attention among the nodes of a structure, of the gated feed-forward block, of the norm after a residual and of the cross
+entropy over kinds, and the gathering of an AdamW step's tensors, in C++.
 The extension is an accelerator of the host side only — every launch still goes through ``libcgtp.so``; without it
 (not built, or ``CGTP_TORCH_SHIM=0``) the same launches are issued through ``ctypes``."""
 import importlib.util
