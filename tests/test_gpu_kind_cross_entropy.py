@@ -169,6 +169,25 @@ def test_batched_gradients_are_refused(device):
         torch.autograd.grad(loss, x, torch.ones(3, 5, device=device), is_grads_batched=True)
 
 
+@pytest.mark.parametrize("n,k,c,cap", [(700, 900, 300, None), (130, 2001, 384, 3.0), (40, 5003, 512, None), (3000, 170, 449, None), (1, 129, 257, 2.0),
+                                       (20000, 130, 390, None), (500, 33, 500, None)])
+def test_gradients_of_more_than_256_channels(device, n, k, c, cap):
+    from equitorch_amd.nn.functional import kind_cross_entropy
+    for dtype, wanted in ((BF16, (True, True)), (F16, (True, True)), (BF16, (False, True)), (F16, (True, False))):
+        x, table, kind, g = _inputs(stable_seed(n, k, c), n, k, c, dtype, 0.3)
+        leaves = [t.to(device).requires_grad_(w) for t, w in zip((x, table), wanted)]
+        loss = kind_cross_entropy(*leaves, kind.to(device), 0.06, cap)
+        grads = iter(torch.autograd.grad(loss, [t for t in leaves if t.requires_grad], g.to(device)))
+        got = [loss] + [next(grads) if w else None for w in wanted]
+        if all(wanted):
+            _check(got, x, table, kind, 0.06, cap, g, dtype)
+            both = {dtype: got} if dtype == BF16 else {**both, dtype: got}
+        else:                       # one alone: from another kernel or without the other's, of the same numbers
+            _check((loss, None, None), x, table, kind, 0.06, cap, g, dtype)
+            for one, two in zip(got[1:], both[dtype][1:]):
+                assert one is None or float((one - two).abs().max()) <= 8 * EPS[dtype] * float(two.abs().max())
+
+
 def test_rows_and_table_of_one_leaf(device):
     from equitorch_amd.nn.functional import kind_cross_entropy
     for dtype in (F32, BF16):
