@@ -354,54 +354,65 @@ AddRmsOut add_rms_forward(const at::Tensor& x, const at::Tensor& residual, const
 
 struct AddRms : torch::autograd::Function<AddRms> {
   typedef c10::optional<at::Tensor> Optional;
-  // out and, with a residual, total
+  // out and, with a residual, total: the backward needs neither x nor the residual beside it
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const Optional& residual, const Optional& weight, double eps,
                                int64_t fallback) {
     AddRmsOut r = add_rms_forward(x, opt(residual), opt(weight), eps, true, false);
-    ctx->save_for_backward({x, opt(residual), opt(weight), r.total, r.rstd});
-    ctx->saved_data["eps"] = eps;
-    ctx->saved_data["fallback"] = fallback;
+    ctx->save_for_backward({r.total, opt(weight), r.rstd});
+    auto& d = ctx->saved_data;
+    d["eps"] = eps;
+    d["fallback"] = fallback;
+    d["type"] = (int64_t)x.scalar_type();
+    d["residual"] = residual.has_value();
     ctx->set_materialize_grads(false);
     if (residual.has_value()) return {r.out, r.total};
     return {r.out};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     const variable_list s = ctx->get_saved_variables();
-    const at::Tensor &x = s[0], &residual = s[1], &weight = s[2], &total = s[3];
+    const at::Tensor &total = s[0], &weight = s[1];
+    auto& d = ctx->saved_data;
+    const bool residual = d["residual"].toBool();
+    const auto type = (at::ScalarType)d["type"].toInt();
     const at::Tensor g_total = grad.size() > 1 ? grad[1] : at::Tensor();
-    std::vector<bool> need;
-    size_t edge = 0;                    // the node has an edge for each operand that is there
-    for (size_t i = 0; i < 3; ++i) need.push_back(s[i].defined() && ctx->needs_input_grad(edge++));
+    // the node has an edge for each operand that is there
+    const bool need_x = ctx->needs_input_grad(0), need_residual = residual && ctx->needs_input_grad(1),
+               need_weight = weight.defined() && ctx->needs_input_grad(residual ? 2 : 1);
     variable_list out(5);
     if (!grad[0].defined() && !g_total.defined()) return out;
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
-    const at::Tensor g_out = grad[0].defined() ? grad[0] : at::zeros(x.sizes(), x.options());
-    if (at::GradMode::is_enabled())
-      return call_fallback(ctx->saved_data["fallback"].toInt(), g_out, {x, residual, weight}, need, 5,
-                           g_total.defined() ? Optional(g_total) : Optional());
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(total.device());
+    const at::Tensor g_out = grad[0].defined() ? grad[0] : at::zeros(total.sizes(), total.options().dtype(type));
+    if (at::GradMode::is_enabled()) {
+      const variable_list g = call_fallback(d["fallback"].toInt(), g_out, {total, weight}, {need_x || need_residual, need_weight}, 2,
+                                            g_total.defined() ? Optional(g_total) : Optional(), type);
+      if (need_x) out[0] = g[0].to(type);
+      if (need_residual) out[1] = g[0];
+      out[2] = g[1];
+      return out;
+    }
     const at::Tensor g = g_out.contiguous(), gt = g_total.defined() ? g_total.contiguous() : g_total;
-    cgtp_add_rms_args a = add_rms_args(x, weight, total, ctx->saved_data["eps"].toDouble());
-    a.rstd = (float*)s[4].data_ptr();
+    cgtp_add_rms_args a = add_rms_args(g, weight, total, d["eps"].toDouble());
+    a.rstd = (float*)s[2].data_ptr();
     a.grad_out = g.data_ptr();
     a.grad_total = ptr_or_null(gt);
     // of one type: one tensor is the gradient of both
-    const bool same = residual.defined() && residual.scalar_type() == x.scalar_type();
+    const bool same = residual && total.scalar_type() == type;
     at::Tensor gx, gr;
-    if (need[0] || (same && need[1])) gx = at::empty(x.sizes(), x.options());
+    if (need_x || (same && need_residual)) gx = at::empty(g.sizes(), g.options());
     if (same) gr = gx;
-    else if (need[1]) gr = at::empty(residual.sizes(), residual.options());
-    if (need[0]) out[0] = gx;
-    if (need[1]) out[1] = gr;
-    if (need[2]) out[2] = at::empty(weight.sizes(), weight.options());
+    else if (need_residual) gr = at::empty(total.sizes(), total.options());
+    if (need_x) out[0] = gx;
+    if (need_residual) out[1] = gr;
+    if (need_weight) out[2] = at::empty(weight.sizes(), weight.options());
     a.grad_x = mutable_ptr(gx);
     a.grad_residual = same ? nullptr : mutable_ptr(gr);
     a.grad_weight = mutable_ptr(out[2]);
     at::Tensor ws;
     if (const int64_t n = cgtp_add_rms_workspace_bytes(&a)) {
-      ws = bytes_on(x, n);
+      ws = bytes_on(total, n);
       a.workspace = ws.data_ptr();
     }
-    check_status(cgtp_add_rms_backward(&a, current_stream(x)), "cgtp_add_rms_backward");
+    check_status(cgtp_add_rms_backward(&a, current_stream(total)), "cgtp_add_rms_backward");
     return out;
   }
 };

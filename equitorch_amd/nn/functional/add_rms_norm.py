@@ -40,23 +40,18 @@ def _forward(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], ep
     return out, total, rstd, scale
 
 
-def _expression(eps: float, both: bool):
-    """``(x, residual, weight) -> out``, and the total where a gradient of it came in."""
-    def expression(x, residual, weight):
-        total = x if residual is None else (x.float() + residual.float()).to(residual.dtype)
+def _higher(g_out, g_total, inputs, need, eps: float, dtype: torch.dtype):
+    """Gradients of ``(total, weight)`` through the tensor expression of ``out``, of type ``dtype``; what has come in for the total is added."""
+    def expression(total, weight):
         t = total.float()
         out = t * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps)
         if weight is not None:
             out = out * weight.float()
-        return (out.to(x.dtype), total) if both else out.to(x.dtype)
-    return expression
-
-
-def _higher(g_out, g_total, inputs, need, eps: float):
-    if g_out is None:
-        g_out = torch.zeros(inputs[0].shape, dtype=inputs[0].dtype, device=inputs[0].device)
-    both = g_total is not None and (need[0] or need[1])           # the weight has no part in the total
-    return higher_order(_expression(eps, both), inputs, need, (g_out, g_total) if both else g_out)
+        return out.to(dtype)
+    grads = (None, None) if g_out is None else higher_order(expression, inputs, need, g_out)
+    if g_total is None or not need[0]:
+        return grads
+    return g_total if grads[0] is None else grads[0] + g_total, grads[1]
 
 
 _fallbacks = {}
@@ -65,45 +60,46 @@ _fallbacks = {}
 def _fallback(mod, eps: float):
     """The extension's number for the tensor expression, which a backward under gradient mode evaluates."""
     if eps not in _fallbacks:
-        def grads(g_out, inputs, need, g_total):
-            return _higher(g_out, g_total, inputs, need, eps)
+        def grads(g_out, inputs, need, g_total, dtype):
+            return _higher(g_out, g_total, inputs, need, eps, dtype)
         _fallbacks[eps] = mod.Fallback(grads)
     return _fallbacks[eps]
 
 
 class _AddRmsNorm(Function):
-    """Outputs ``out`` and, with a residual, ``total``."""
+    """Outputs ``out`` and, with a residual, ``total``: the backward needs neither x nor the residual beside it."""
 
     @staticmethod
     def forward(ctx, x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float):
         out, total, rstd, _ = _forward(x, residual, weight, eps, True)
-        ctx.save_for_backward(x, residual, weight, total, rstd)
-        ctx.eps = eps
+        ctx.save_for_backward(total, weight, rstd)
+        ctx.eps, ctx.dtype = eps, x.dtype
         ctx.set_materialize_grads(False)
         return out if residual is None else (out, total)
 
     @staticmethod
     def backward(ctx, g_out, g_total=None):
-        x, residual, weight, total, rstd = ctx.saved_tensors
-        need = [t is not None and n for t, n in zip((x, residual, weight), ctx.needs_input_grad)]
+        total, weight, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad[:3]
         if g_out is None and g_total is None:
             return None, None, None, None
         if torch.is_grad_enabled():
-            return (*_higher(g_out, g_total, (x, residual, weight), need, ctx.eps), None)
-        g_out = torch.zeros_like(x) if g_out is None else g_out.contiguous()
+            g, gw = _higher(g_out, g_total, (total, weight), (need[0] or need[1], need[2]), ctx.eps, ctx.dtype)
+            return g.to(ctx.dtype) if need[0] else None, g if need[1] else None, gw, None
+        same = total.dtype == ctx.dtype                       # then one tensor is the gradient of x and of the residual
+        g_out = torch.zeros_like(total, dtype=ctx.dtype) if g_out is None else g_out.contiguous()
         g_total = None if g_total is None else g_total.contiguous()
-        a = _args(x, weight, total.dtype, ctx.eps)
+        a = _args(g_out, weight, total.dtype, ctx.eps)
         a.total, a.rstd, a.grad_out, a.grad_total = total.data_ptr(), rstd.data_ptr(), g_out.data_ptr(), _lib.ptr(g_total)
-        same = residual is not None and residual.dtype == x.dtype           # then one tensor is the gradient of both
-        gx = torch.empty_like(x) if need[0] or (same and need[1]) else None
-        gr = gx if same else torch.empty_like(residual) if need[1] else None
+        gx = torch.empty_like(g_out) if need[0] or (same and need[1]) else None
+        gr = gx if same else torch.empty_like(total) if need[1] else None
         gw = torch.empty_like(weight) if need[2] else None
         a.grad_x, a.grad_residual, a.grad_weight = _lib.ptr(gx), 0 if same else _lib.ptr(gr), _lib.ptr(gw)
         nbytes = _lib.lib.cgtp_add_rms_workspace_bytes(C.byref(a))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=total.device) if nbytes else None
         a.workspace = _lib.ptr(ws)
-        with torch.cuda.device(x.device):
-            _lib.check(_lib.lib.cgtp_add_rms_backward(C.byref(a), _lib.stream_ptr(x.device)), "cgtp_add_rms_backward")
+        with torch.cuda.device(total.device):
+            _lib.check(_lib.lib.cgtp_add_rms_backward(C.byref(a), _lib.stream_ptr(total.device)), "cgtp_add_rms_backward")
         return gx if need[0] else None, gr if need[1] else None, gw, None
 
 

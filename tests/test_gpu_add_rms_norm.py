@@ -330,3 +330,39 @@ def test_total_in_the_residuals_place(device, n, c):
         a.dtype = a.residual_dtype = a.weight_dtype = _lib.dtype_code(dtype)
         _lib.check(_lib.lib.cgtp_add_rms_forward(C.byref(a), _lib.stream_ptr(x.device)), "cgtp_add_rms_forward")
         assert torch.equal(r, total) and torch.equal(got, out)
+
+
+@pytest.mark.parametrize("route", ["extension", "ctypes"])
+def test_what_a_backward_keeps(device, route, monkeypatch):
+    """total and a number for each row: x and the residual may be freed or written over; gradients of either order are those of them as they were."""
+    import gc
+    from equitorch_amd import _shim
+    from equitorch_amd.nn.functional import add_rms_norm
+    if route == "ctypes":
+        monkeypatch.setattr(_shim, "module", lambda: None)
+    n, c = 5000, 256
+    for residual_type in (BF16, F32):
+        leaf = torch.randn(n, c, device=device, dtype=BF16, requires_grad=True)
+        weight = torch.randn(c, device=device, requires_grad=True)
+        gc.collect()
+        before = torch.cuda.memory_allocated()
+        x, r = leaf * 2, (leaf * 3).to(residual_type)
+        out, total = add_rms_norm(x, r, weight)
+        del x, r
+        kept = torch.cuda.memory_allocated() - before
+        # out and total, rstd; the products keep nothing of this size, and allocations are whole blocks of 512 bytes
+        assert kept <= n * c * (2 + total.element_size()) + 4 * n + 8 * 512
+        g = torch.randn_like(out)
+        first = torch.autograd.grad(out, (leaf, weight), g, retain_graph=True)
+        second = torch.autograd.grad(out, (leaf, weight), g, create_graph=True)
+        for a, b in zip(first, second):
+            assert float((a - b).detach().abs().max()) <= 4 * 2.0 ** -8 * float(a.abs().max())
+        assert torch.autograd.grad(second[0].float().square().sum(), leaf)[0].isfinite().all()
+    x, r = (torch.randn(40, 24, device=device, requires_grad=True) for _ in range(2))
+    y = x * 1.0
+    out, total = add_rms_norm(y, r)
+    want = torch.autograd.grad(out.sum() + total.square().sum(), (x, r), retain_graph=True)
+    with torch.no_grad():
+        y.zero_()
+    got = torch.autograd.grad(out.sum() + total.square().sum(), (x, r))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
