@@ -17,6 +17,7 @@
 #include "gff_gemm.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace cgtp {
@@ -217,6 +218,7 @@ struct LogitArgs {
   int64_t n;                      // rows of the arrays below
   int c, ld, splits, each;        // each: kinds of a split, whole tiles
   float scale, cap;               // scale: to log2 units without a cap, else over the cap; cap: in log2 units, 0: none
+  float twice, over, series[4];   // with a cap: -2 log2 e |scale|; 1 / cap; the tangent's series behind its first term, times the cap
   float *loss, *lse_of;           // forward, of all rows
   const int* rows;
   float2* stats;                  // forward, several splits: maximum and sum of each split and row
@@ -232,18 +234,54 @@ struct LogitArgs {
   float scale_dx;
 };
 
+// Where |u| is at most this, tanh u is u times five terms of its series in u^2, to 6e-8 of itself; above, (1 - e) / (1 + e) with e =
+// exp(-2 |u|), which errs about 1e-7 below it too, where the tangent may be far smaller.
+constexpr float kSeries = 0.3f;
+template <typename T>
+__device__ __forceinline__ float cap_series(float z, float scale, const LogitArgs<T>& a) {
+  const float u = z * scale, q = u * u;
+  return u * fmaf(q, fmaf(q, fmaf(q, fmaf(q, a.series[3], a.series[2]), a.series[1]), a.series[0]), a.cap);
+}
+template <typename T>
+__device__ __forceinline__ float cap_exponential(float z, const LogitArgs<T>& a) {
+  const float e = __builtin_amdgcn_exp2f(fabsf(z) * a.twice);
+  return copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e) * a.cap, z);
+}
 // Logits in log2 units; slope: 1 - tanh^2.
 template <typename T>
-__device__ __forceinline__ float capped(float z, float scale, float cap, float& slope) {
-  const float u = z * scale;
+__device__ __forceinline__ float capped(float z, const LogitArgs<T>& a, float& slope) {
+  float t;
   if constexpr (sizeof(T) == 4) {
-    const float t = tanhf(u);
+    t = tanhf(z * a.scale);
     slope = 1.f - t * t;
-    return cap * t;
+    return a.cap * t;
   } else {
-    const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * (2.f * kLog2e)));
-    slope = 4.f * r * (1.f - r);
-    return cap - 2.f * cap * r;
+    const float signed_z = a.scale < 0.f ? -z : z, scale = fabsf(a.scale);
+    const float c = fabsf(z) * scale <= kSeries ? cap_series(signed_z, scale, a) : cap_exponential(signed_z, a);
+    t = c * a.over;
+    slope = 1.f - t * t;
+    return c;
+  }
+}
+// Where the gradients' kernels form them again, the scale's sign in the operands: the tangent to some 1e-7 of 1, far below what the gradient is
+// rounded to, by fewer registers (with the block's form 16384 rows, 30011 kinds, 256 bf16 channels take 1560 us a step, 1380 so).
+__device__ __forceinline__ float cap_for_gradient(float z, float scale, float cap, float& slope) {
+  const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * scale * (2.f * kLog2e)));
+  slope = 4.f * r * (1.f - r);
+  return cap - 2.f * cap * r;
+}
+// A block of a forward's: all by the series, or all by the other.
+template <typename T>
+__device__ __forceinline__ void cap_block(f32x16_t& z, float scale, const LogitArgs<T>& a) {
+  float most = fabsf(z[0]);
+#pragma unroll
+  for (int e = 1; e < 16; ++e) most = fmaxf(most, fabsf(z[e]));
+  if (__any(most * scale > kSeries)) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = cap_exponential(z[e], a);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = cap_series(z[e], scale, a);
   }
 }
 
@@ -341,7 +379,7 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_stats_kernel(LogitArgs<T
         for (int e = 0; e < 16; ++e) {
           const int64_t kind = k0 + 32 * (B * wn + j) + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
           float slope, z = acc[i][j][e];
-          z = a.cap > 0.f ? capped<T>(z, a.scale, a.cap, slope) : z * a.scale;
+          z = a.cap > 0.f ? capped(z, a, slope) : z * a.scale;
           if (kind == own[i]) {
             if (a.splits > 1) a.at[m0 + 32 * (B * wm + i) + (lane & 31)] = z;
             else own_places[32 * (B * wm + i) + (lane & 31)] = z;
@@ -413,7 +451,7 @@ __global__ void __launch_bounds__(kGemmThreads, 2) loss_dz_kernel(LogitArgs<T> a
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float slope = 1.f;
-      const float z = a.cap > 0.f ? capped<T>(v[e], a.scale, a.cap, slope) : v[e] * a.scale;
+      const float z = a.cap > 0.f ? capped(v[e], a, slope) : v[e] * a.scale;
       const float p = __builtin_amdgcn_exp2f(z - lse) - (k0 + c + e == own ? 1.f : 0.f);
       v[e] = k0 + c + e < a.k_end ? p * slope * kRaise<T> : 0.f;
     }
@@ -675,7 +713,7 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
               for (int k = 0; k < 2; ++k) {
                 const float z = acc[i][e + k];
                 float slope = 1.f;
-                if constexpr (CAP) v[k] = __builtin_amdgcn_exp2f(capped<T>(z, scale, a.cap, slope) - lse[i]);
+                if constexpr (CAP) v[k] = __builtin_amdgcn_exp2f(cap_for_gradient(z, scale, a.cap, slope) - lse[i]);
                 else v[k] = __builtin_amdgcn_exp2f(fmaf(z, scale, -lse[i]));
                 if (decltype(odd)::value && e + k == own[i] - k0) v[k] -= 1.f;
                 if constexpr (CAP) v[k] *= slope;
@@ -749,12 +787,7 @@ __global__ void __launch_bounds__(256, 2) loss_walk_kernel(LogitArgs<T> a) {
         for (int i = 0; i < RB; ++i) {
           const int at_own = own[i] - k0;
           const bool has_own = (unsigned)at_own < 16u && at_own < mine;
-          if constexpr (CAP)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float slope;
-              acc[i][e] = capped<T>(acc[i][e], scale, a.cap, slope);
-            }
+          if constexpr (CAP) cap_block(acc[i], scale, a);
           const float factor = CAP ? 1.f : scale;
           if (__any(has_own))
 #pragma unroll
@@ -1344,6 +1377,12 @@ LogitArgs<T> logit_args(const cgtp_kind_loss_args* a, const Plan& p, const RowsO
   l.ld = p.ld;
   l.cap = a->cap > 0 ? a->cap * kLog2e : 0.f;
   l.scale = a->cap > 0 ? a->scale / a->cap : a->scale * kLog2e;
+  if (a->cap > 0) {
+    l.twice = -2.f * kLog2e * std::fabs(l.scale);
+    l.over = 1.f / l.cap;
+    const double terms[] = {-1. / 3, 2. / 15, -17. / 315, 62. / 2835};
+    for (int i = 0; i < 4; ++i) l.series[i] = (float)(l.cap * terms[i]);
+  }
   return l;
 }
 
