@@ -366,3 +366,27 @@ def test_what_a_backward_keeps(device, route, monkeypatch):
         y.zero_()
     got = torch.autograd.grad(out.sum() + total.square().sum(), (x, r))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("route", ["extension", "ctypes"])
+def test_a_graph_ends_with_its_results(device, route, monkeypatch):
+    """The node keeps an output of its own; that must not keep the node: without a collector of cycles nothing is left of a pass."""
+    import gc
+    from equitorch_amd import _shim
+    from equitorch_amd.nn.functional import add_rms_norm
+    if route == "ctypes":
+        monkeypatch.setattr(_shim, "module", lambda: None)
+    x, r = (torch.randn(4096, 256, device=device, requires_grad=True) for _ in range(2))
+    gc.collect()
+    gc.disable()
+    try:
+        before = torch.cuda.memory_allocated()
+        for backward in (False, True):
+            for _ in range(3):
+                out, total = add_rms_norm(x, r)
+                if backward:
+                    torch.autograd.grad(out.sum() + total.sum(), (x, r))
+                del out, total
+            assert torch.cuda.memory_allocated() == before
+    finally:
+        gc.enable()
