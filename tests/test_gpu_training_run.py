@@ -124,3 +124,47 @@ def test_a_recorded_training_step(device):
             values.append(float(out))
         runs.append((values, [p.detach().clone() for p in params]))
     assert runs[0][0] == runs[1][0] and all(torch.equal(a, b) for a, b in zip(runs[0][1], runs[1][1]))
+
+
+def test_two_graphs_and_two_streams_at_once(device):
+    """Calls of different sizes side by side, eager on two streams and as two graphs that share a pool in turn: nothing of one is in another."""
+    from equitorch_amd.nn.functional import add_rms_norm, kind_cross_entropy
+    sizes = [(3000, 200, 64, torch.bfloat16), (900, 5000, 120, torch.float32)]
+    gen = torch.Generator(device=device).manual_seed(8)
+    work = []
+    for n, k, c, dtype in sizes:
+        x, r, table = (torch.randn(m, c, device=device, generator=gen).to(dtype).requires_grad_(True) for m in (n, n, k))
+        work.append((x, r, table, torch.randint(-50, k, (n,), device=device, generator=gen), torch.rand(n, device=device, generator=gen)))
+
+    def step(x, r, table, kind, g):
+        out, _ = add_rms_norm(x, r)
+        loss = kind_cross_entropy(out, table, kind, 0.1)
+        # no result holds the autograd graph: one of the same leaves that is alive while a backward is captured ends the capture, and the process
+        return [t.detach() for t in (loss, *torch.autograd.grad(loss, (x, r, table), g))]
+    want = [step(*w) for w in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[] for _ in work]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(*work[i]))
+    torch.cuda.synchronize()
+    for results, one in zip(got, want):
+        assert all(torch.equal(a, b) for result in results for a, b in zip(result, one))
+    del got
+    graphs, kept, pool = [], [], None
+    for w in work:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            kept.append(step(*w))
+        graphs.append(graph)
+        pool = graph.pool()
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+        step(*work[0])
+        torch.cuda.synchronize()
+        for results, one in zip(kept, want):
+            assert all(torch.equal(a, b) for a, b in zip(results, one))
