@@ -1,0 +1,80 @@
+"""Saving and loading of AdamW's states without a GPU, on states that are made by hand."""
+import pytest
+import torch
+
+from equitorch_amd.optim import BLOCK, AdamW
+
+F32, BF16, E4M3 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+
+
+def _params(*shapes, dtype=F32, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(s, generator=gen).to(dtype)) for s in shapes]
+
+
+def _states(opt, seed=1):
+    """States such as two steps leave, of random numbers."""
+    gen = torch.Generator().manual_seed(seed)
+    for group in opt.param_groups:
+        for p in group["params"]:
+            rand = lambda: torch.empty_like(p, dtype=F32).copy_(torch.rand(p.shape, generator=gen))      # in the order of p's elements
+            state = opt.state[p]
+            state["step"] = torch.tensor(2.0)
+            if group["state_bits"] == 32:
+                state["exp_avg"], state["exp_avg_sq"] = rand(), rand()
+            else:
+                for name in ("exp_avg", "root_avg_sq"):
+                    state[name] = (rand() * 400).to(E4M3)
+                    state[name + "_scale"] = torch.rand(-(-p.numel() // BLOCK), generator=gen)
+            if group["master"] and p.dtype != F32:
+                state["master"] = rand()
+    return opt
+
+
+def _equal(got, want):
+    assert got.keys() == want.keys()
+    for name, value in want.items():
+        assert got[name].dtype == value.dtype and torch.equal(got[name].float(), value.float()), name
+
+
+@pytest.mark.parametrize("bits,dtype", [(32, F32), (8, F32), (8, BF16), (32, BF16)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_hooks_before_loading_are_followed(bits, dtype, in_place):
+    """A hook that matches parameters by their names: the states go where it puts them, in their own types."""
+    first, second = _params((20, 30), (20, 30), dtype=dtype)
+    saved = _states(AdamW([first, second], state_bits=bits, master=True))
+    others = _params((20, 30), (20, 30), dtype=dtype)
+    opt = AdamW(others[::-1], state_bits=bits, master=True)
+
+    def match(_, read):
+        state = {1 - i: s for i, s in read["state"].items()}
+        if in_place:
+            read["state"] = state
+            return None
+        return {**read, "state": state}
+    opt.register_load_state_dict_pre_hook(match)
+    opt.load_state_dict(saved.state_dict())
+    for p, q in zip((first, second), others):
+        _equal(opt.state[q], saved.state[p])
+    assert not torch.equal(opt.state[others[0]]["exp_avg"].float(), opt.state[others[1]]["exp_avg"].float())
+    opt.load_state_dict(saved.state_dict())      # the optimizer's own hooks are gone, the user's stay
+    _equal(opt.state[others[0]], saved.state[first])
+
+
+@pytest.mark.parametrize("prepend", [False, True])
+def test_hooks_after_loading_have_the_last_word(prepend):
+    """A hook that runs after a load sees the states in their types, and what it changes stays."""
+    for bits, dtype in ((32, BF16), (8, BF16), (32, F32)):
+        (p,), (q,) = _params((20, 30), dtype=dtype), _params((20, 30), dtype=dtype)
+        saved, opt, seen = _states(AdamW([p], state_bits=bits)), AdamW([q], state_bits=bits), []
+
+        def change(opt):
+            seen.extend(v.dtype for v in opt.state[q].values())
+            opt.state[q]["step"] = torch.tensor(7.0)
+            opt.state[q]["exp_avg"].zero_()
+        opt.register_load_state_dict_post_hook(change, prepend=prepend)
+        opt.load_state_dict(saved.state_dict())
+        assert seen == [v.dtype for v in saved.state[p].values()]
+        assert float(opt.state[q]["step"]) == 7 and not opt.state[q]["exp_avg"].float().any()
+        _equal(opt.state[q], {**saved.state[p], "step": torch.tensor(7.0), "exp_avg": torch.zeros_like(saved.state[p]["exp_avg"].float()).to(
+            saved.state[p]["exp_avg"].dtype)})
