@@ -263,8 +263,8 @@ __device__ __forceinline__ float capped(float z, const LogitArgs<T>& a, float& s
     return c;
   }
 }
-// Where the gradients' kernels form them again, the scale's sign in the operands: the tangent to some 1e-7 of 1, far below what the gradient is
-// rounded to, by fewer registers (with the block's form 16384 rows, 30011 kinds, 256 bf16 channels take 1560 us a step, 1380 so).
+// Where the gradients' kernels form them again, the scale's sign in the operands: the tangent to some 1e-7 of 1, with the caps that come here (kWalkCap) far
+// below what the gradient is rounded to, by fewer registers (with the block's form 16384 rows, 30011 kinds, 256 bf16 channels take 1560 us a step, 1380 so).
 __device__ __forceinline__ float cap_for_gradient(float z, float scale, float cap, float& slope) {
   const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * scale * (2.f * kLog2e)));
   slope = 4.f * r * (1.f - r);
@@ -993,9 +993,13 @@ __global__ void __launch_bounds__(256) loss_walk_join_kernel(const float2* stats
   if (i < n && (int)threadIdx.x < per) give_loss(loss, lse, rows[i], at[i], top, sum);
 }
 
-// Steps of 16 channels of the kernels above for a width, 0: not theirs.
-int walk_steps(int channels, int size) {
-  if (size == 4 || channels > 512) return 0;
+// The kernels above form a capped logit in the backward, and in the forward in a block with large ones, from a tangent that errs some 1e-7 of
+// 1: as much of the cap, and that goes into the softmax.  Up to this cap it is 4e-5 of a probability at most, a tenth of what rounding dz to fp16 takes;
+// at 1e6 it would be a tenth of the probability.  Above it the tiles of both operands take each tangent to 1e-7 of itself.
+constexpr float kWalkCap = 256.f;
+// Steps of 16 channels of the kernels above for a width and a cap, 0: not theirs.
+int walk_steps(int channels, int size, float cap) {
+  if (size == 4 || channels > 512 || cap > kWalkCap) return 0;
   const int steps = (channels + 15) / 16;
   for (int s : {4, 8, 12, 16, 24, 32})
     if (steps <= s) return s;
@@ -1256,7 +1260,7 @@ struct Plan {
 Plan plan_of(const cgtp_kind_loss_args* a, bool backward) {
   Plan p = {};
   const int64_t size = a->dtype == CGTP_F32 ? 4 : 2, n = a->n_rows, k = a->n_kinds, c = a->channels;
-  p.steps = walk_steps(a->channels, (int)size);
+  p.steps = walk_steps(a->channels, (int)size, a->cap);
   p.tile = size == 4 ? kTileOf<float> : kTile;
   p.ld = (int)(p.steps ? 16 * p.steps : up_to(c, 16 / size));
   p.row_each = n <= 64 ? 64 : std::max<int64_t>(16, ceil_div(n, kRowBlocks));      // 64: one workgroup needs no other's count
