@@ -102,18 +102,22 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("parameters overlap in memory, or one is given twice: a step would update the same elements twice")
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As torch's, hooks included, with every state in its own type (torch's takes floating-point states to the parameter's)."""
+        """As torch's, hooks included, with every state in its own type (torch's takes floating-point states to the parameter's).  What is
+        refused leaves the optimizer as it was."""
         loaded = []
+
+        def check(_, read):
+            for group in read["param_groups"]:
+                self._check_numbers(group)
+            loaded.append(read)
         # last of the hooks before, first of those after: the states are those of the dict that the others leave, and stay what the others make of them
-        handles = [self.register_load_state_dict_pre_hook(lambda _, read: loaded.append(read)),
+        handles = [self.register_load_state_dict_pre_hook(check),
                    self.register_load_state_dict_post_hook(lambda _: self._load_states(loaded[0]), prepend=True)]
         try:
             super().load_state_dict(state_dict)
         finally:
             for handle in handles:
                 handle.remove()
-        for group in self.param_groups:
-            self._check_group(group)
 
     def _load_states(self, state_dict: dict) -> None:
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]

@@ -78,3 +78,34 @@ def test_hooks_after_loading_have_the_last_word(prepend):
         assert float(opt.state[q]["step"]) == 7 and not opt.state[q]["exp_avg"].float().any()
         _equal(opt.state[q], {**saved.state[p], "step": torch.tensor(7.0), "exp_avg": torch.zeros_like(saved.state[p]["exp_avg"].float()).to(
             saved.state[p]["exp_avg"].dtype)})
+
+
+def _copy(opt):
+    """(options of each group, states of each parameter)"""
+    return ([{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups],
+            [{k: v.clone() for k, v in opt.state[p].items()} for g in opt.param_groups for p in g["params"]])
+
+
+def _unchanged(opt, before):
+    options, states = _copy(opt)
+    assert options == before[0] and len(states) == len(before[1])
+    for got, want in zip(states, before[1]):
+        _equal(got, want)
+
+
+@pytest.mark.parametrize("name,value", [("lr", -1.0), ("lr", float("nan")), ("betas", (0.9, 1.0)), ("eps", -1.0), ("weight_decay", float("inf")),
+                                        ("state_bits", 16), ("seed", 1 << 32)])
+def test_a_refused_dict_leaves_the_optimizer_as_it_was(name, value):
+    """A number that the constructor refuses, in the last of two groups."""
+    groups = lambda: [{"params": [p]} for p in _params((20, 30), (7,))]
+    saved = _states(AdamW(groups(), lr=0.25)).state_dict()
+    saved["param_groups"][1][name] = value
+    opt = _states(AdamW(groups()), seed=5)
+    before = _copy(opt)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(saved)
+    _unchanged(opt, before)
+    del saved["param_groups"][1]
+    with pytest.raises(ValueError):
+        opt.load_state_dict(saved)
+    _unchanged(opt, before)
