@@ -14,6 +14,7 @@ from ._lib import AdamwArgs, AdamwTensor, CgtpError
 BLOCK = 256        # elements that share a scale
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _E4M3 = torch.float8_e4m3fn
+_OPTIONS = ("lr", "betas", "eps", "weight_decay", "state_bits", "master", "maximize", "seed")
 
 
 def _dense(t: Tensor) -> bool:
@@ -102,14 +103,14 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("parameters overlap in memory, or one is given twice: a step would update the same elements twice")
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As torch's, hooks included, with every state in its own type (torch's takes floating-point states to the parameter's).  What is
-        refused leaves the optimizer as it was."""
+        """As torch's, hooks included, with every state in its own type (torch's takes floating-point states to the parameter's).  A dict of
+        ``torch.optim.AdamW`` is taken too: options that it does not have keep their values, ``exp_avg`` and ``exp_avg_sq`` become fp32.  What
+        is refused leaves the optimizer as it was."""
         loaded = []
 
         def check(_, read):
-            for group in read["param_groups"]:
-                self._check_numbers(group)
-            loaded.append(read)
+            loaded.append(self._completed(read))
+            return loaded[0]
         # last of the hooks before, first of those after: the states are those of the dict that the others leave, and stay what the others make of them
         handles = [self.register_load_state_dict_pre_hook(check),
                    self.register_load_state_dict_post_hook(lambda _: self._load_states(loaded[0]), prepend=True)]
@@ -118,6 +119,30 @@ class AdamW(torch.optim.Optimizer):
         finally:
             for handle in handles:
                 handle.remove()
+
+    def _completed(self, state_dict: dict) -> dict:
+        """The dict with options and states as a step takes them."""
+        saved = state_dict["param_groups"]
+        if [len(g["params"]) for g in saved] != [len(g["params"]) for g in self.param_groups]:
+            return state_dict                    # torch refuses it
+        groups = [{**{k: now[k] for k in _OPTIONS}, **g} for now, g in zip(self.param_groups, saved)]
+        state = dict(state_dict["state"])
+        for group in groups:
+            self._check_numbers(group)
+            if group.get("amsgrad") or (group["weight_decay"] and not group.get("decoupled_weight_decay", True)):
+                raise ValueError("the dict is of another formula: amsgrad, or a weight decay that is added to the gradient")
+            for i in group["params"]:
+                if not state.get(i):
+                    continue
+                s = state[i] = dict(state[i])
+                if group["state_bits"] == 8 and "exp_avg_sq" in s:
+                    raise ValueError("states in 32 bits do not fit state_bits = 8: load them into an optimizer of 32")
+                if "step" in s:
+                    s["step"] = torch.as_tensor(s["step"], dtype=torch.float32).reshape(())
+                for name in ("exp_avg", "exp_avg_sq") if group["state_bits"] == 32 else ():
+                    if isinstance(s.get(name), Tensor) and s[name].is_floating_point():
+                        s[name] = s[name].float()
+        return {**state_dict, "state": state, "param_groups": groups}
 
     def _load_states(self, state_dict: dict) -> None:
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]

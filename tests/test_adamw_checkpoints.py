@@ -109,3 +109,53 @@ def test_a_refused_dict_leaves_the_optimizer_as_it_was(name, value):
     with pytest.raises(ValueError):
         opt.load_state_dict(saved)
     _unchanged(opt, before)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("options", [{}, {"foreach": False, "maximize": True}])
+def test_a_checkpoint_of_torchs_adamw(dtype, options):
+    """States and options of torch's optimizer, which has neither state_bits nor master nor seed."""
+    first = _params((20, 30), (7,), (), dtype=dtype)
+    theirs = torch.optim.AdamW(first, lr=0.03, betas=(0.8, 0.99), weight_decay=0.2, **options)
+    for _ in range(3):
+        for p in first:
+            p.grad = torch.randn_like(p)
+        theirs.step()
+    saved = theirs.state_dict()
+    opt = AdamW(_params((20, 30), (7,), (), dtype=dtype), lr=1.0, seed=9)
+    opt.load_state_dict(saved)
+    (group,) = opt.param_groups
+    assert (group["lr"], tuple(group["betas"]), group["weight_decay"], group["state_bits"], group["master"], group["seed"]) == (
+        0.03, (0.8, 0.99), 0.2, 32, False, 9) and group["maximize"] == options.get("maximize", False)
+    for p, q in zip(first, group["params"]):
+        got, want = opt.state[q], theirs.state[p]
+        assert float(got["step"]) == 3 and got["step"].shape == () and got["step"].dtype == F32
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert got[name].dtype == F32 and torch.equal(got[name], want[name].float()), name
+            assert want[name].dtype == dtype                             # the other optimizer's own
+    again = AdamW(_params((20, 30), (7,), (), dtype=dtype))
+    again.load_state_dict(opt.state_dict())
+    _equal(again.state[again.param_groups[0]["params"][0]], opt.state[group["params"][0]])
+
+
+def test_a_number_of_steps_that_is_no_tensor():
+    saved = _states(AdamW(_params((20, 30)))).state_dict()
+    saved["state"][0]["step"] = 11
+    opt = AdamW(_params((20, 30)))
+    opt.load_state_dict(saved)
+    step = opt.state[opt.param_groups[0]["params"][0]]["step"]
+    assert float(step) == 11 and step.dtype == F32 and step.shape == ()
+
+
+@pytest.mark.parametrize("make,bits", [(lambda p: torch.optim.AdamW(p, amsgrad=True), 32), (lambda p: torch.optim.Adam(p, weight_decay=0.1), 32),
+                                       (lambda p: torch.optim.AdamW(p), 8)])
+def test_checkpoints_of_another_formula_are_refused(make, bits):
+    first = _params((20, 30))
+    theirs = make(first)
+    first[0].grad = torch.ones_like(first[0])
+    theirs.step()
+    opt = _states(AdamW(_params((20, 30)), state_bits=bits))
+    before = _copy(opt)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(theirs.state_dict())
+    _unchanged(opt, before)
