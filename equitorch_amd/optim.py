@@ -127,16 +127,22 @@ class AdamW(torch.optim.Optimizer):
             return state_dict                    # torch refuses it
         groups = [{**{k: now[k] for k in _OPTIONS}, **g} for now, g in zip(self.param_groups, saved)]
         state = dict(state_dict["state"])
-        for group in groups:
+        for now, group in zip(self.param_groups, groups):
             self._check_numbers(group)
             if group.get("amsgrad") or (group["weight_decay"] and not group.get("decoupled_weight_decay", True)):
                 raise ValueError("the dict is of another formula: amsgrad, or a weight decay that is added to the gradient")
-            for i in group["params"]:
+            for p, i in zip(now["params"], group["params"]):
                 if not state.get(i):
                     continue
                 s = state[i] = dict(state[i])
                 if group["state_bits"] == 8 and "exp_avg_sq" in s:
                     raise ValueError("states in 32 bits do not fit state_bits = 8: load them into an optimizer of 32")
+                for name in ("exp_avg", "root_avg_sq") if group["state_bits"] == 8 else ():
+                    t = s.get(name)
+                    # the scales are those of 256 elements each in the order of memory as it was: of one block alone in any order
+                    if isinstance(t, Tensor) and t.shape == p.shape and p.numel() > BLOCK and not _same_order(t, p):
+                        raise CgtpError(f"state {name!r} in 8 bits was saved in another order of memory (strides {t.stride()}) than that of its parameter "
+                                        f"(strides {p.stride()} of {tuple(p.shape)}), whose blocks its scales do not fit")
                 if "step" in s:
                     s["step"] = torch.as_tensor(s["step"], dtype=torch.float32).reshape(())
                 for name in ("exp_avg", "exp_avg_sq") if group["state_bits"] == 32 else ():

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from equitorch_amd._lib import CgtpError
 from equitorch_amd.optim import BLOCK, AdamW
 
 F32, BF16, E4M3 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
@@ -159,3 +160,45 @@ def test_checkpoints_of_another_formula_are_refused(make, bits):
     with pytest.raises(ValueError):
         opt.load_state_dict(theirs.state_dict())
     _unchanged(opt, before)
+
+
+_ORDERS = {"rows": lambda p: p, "columns": lambda p: p.transpose(-1, -2).contiguous().transpose(-1, -2),
+           "channels last": lambda p: p.contiguous(memory_format=torch.channels_last)}
+
+
+def _decoded(state, name, p):
+    """Moments of 8 bits, laid out as the parameter."""
+    axes = sorted(range(p.ndim), key=lambda i: -p.stride(i))
+    flat = state[name].float().permute(axes).reshape(-1)
+    scales = state[name + "_scale"].repeat_interleave(BLOCK)[:flat.numel()]
+    back = sorted(range(p.ndim), key=lambda i: axes[i])
+    return (flat * scales).view([p.shape[i] for i in axes]).permute(back)
+
+
+@pytest.mark.parametrize("shape,orders", [((32, 64), ("rows", "columns")), ((5, 4, 6, 7), ("rows", "channels last"))])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_another_order_of_memory(shape, orders, bits):
+    """States follow their elements into another order; those of 8 bits, whose scales are of the order that was, are refused there."""
+    for first in orders:
+        for second in orders:
+            (p,), (q,) = ([torch.nn.Parameter(_ORDERS[o](t.detach()))] for o, t in zip((first, second), _params(shape) * 2))
+            saved, opt = _states(AdamW([p], state_bits=bits)), _states(AdamW([q], state_bits=bits), seed=6)
+            before, want = _copy(opt), saved.state[p]
+            if bits == 8 and first != second:
+                with pytest.raises(CgtpError):
+                    opt.load_state_dict(saved.state_dict())
+                _unchanged(opt, before)
+                continue
+            opt.load_state_dict(saved.state_dict())
+            assert opt.state[q]["exp_avg"].stride() == q.stride()
+            _equal(opt.state[q], want)
+            for name in ("exp_avg", "root_avg_sq") if bits == 8 else ():
+                assert torch.equal(_decoded(opt.state[q], name, q), _decoded(want, name, p))
+
+
+def test_one_block_may_change_its_order():
+    (p,), (q,) = ([torch.nn.Parameter(_ORDERS[o](t.detach()))] for o, t in zip(("rows", "columns"), _params((16, 16)) * 2))
+    saved, opt = _states(AdamW([p], state_bits=8)), AdamW([q], state_bits=8)
+    opt.load_state_dict(saved.state_dict())
+    assert opt.state[q]["exp_avg"].stride() == (1, 16)
+    assert torch.equal(_decoded(opt.state[q], "exp_avg", q), _decoded(saved.state[p], "exp_avg", p))
