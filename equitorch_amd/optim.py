@@ -77,7 +77,8 @@ class AdamW(torch.optim.Optimizer):
         if isinstance(lr, Tensor):
             if lr.numel() != 1 or (lr.is_cuda and lr.dtype != torch.float32):
                 raise ValueError(f"lr must be a number or one fp32 number on the GPU, got {lr.dtype} {tuple(lr.shape)}")
-        elif not 0.0 <= lr < float("inf"):
+            lr = None if lr.is_cuda else lr.item()      # on the GPU it is read when the kernels run
+        if lr is not None and not 0.0 <= lr < float("inf"):
             raise ValueError(f"lr must be finite and not negative, got {lr}")
         betas = group["betas"]
         if len(betas) != 2 or not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
