@@ -57,16 +57,22 @@ class AdamW(torch.optim.Optimizer):
     is fixed when a graph records the step, and states have to be there by then (one step before).  ``step`` in a parameter's state counts on the
     GPU.  Parameters without a gradient are passed over."""
 
+    _made = True                                 # whether the groups are there: a copy's, whose constructor does not run
+
     def __init__(self, params: Iterable, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, master: bool = False, maximize: bool = False, seed: int = 0):
+        self._made = False
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master=master,
                                       maximize=maximize, seed=seed))
+        self._made = True
+        self._check_overlap()                    # once for all groups
 
     def add_param_group(self, param_group: dict) -> None:
         super().add_param_group(param_group)
-        group = self.param_groups[-1]
         try:
-            self._check_group(group)
+            self._check_numbers(self.param_groups[-1])
+            if self._made:
+                self._check_overlap()
         except ValueError:
             self.param_groups.pop()
             raise
@@ -91,8 +97,7 @@ class AdamW(torch.optim.Optimizer):
         if not 0 <= group["seed"] < 1 << 32:
             raise ValueError(f"seed must be 0 <= seed < 2^32, got {group['seed']}")
 
-    def _check_group(self, group: dict) -> None:
-        self._check_numbers(group)
+    def _check_overlap(self) -> None:
         taken = []
         for p in (p for g in self.param_groups for p in g["params"]):
             if p.numel():
