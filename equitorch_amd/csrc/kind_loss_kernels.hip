@@ -1242,6 +1242,10 @@ int loss_check(const cgtp_kind_loss_args* a) {
   // 2^29 rows are 2^23 workgroups for tiles of 64: a grid has fewer than 2^32 threads
   if (a->n_rows < 0 || a->n_rows > (1 << 29) || a->n_kinds < 1 || a->n_kinds > (1 << 30) || a->channels < 1 || a->channels > 0x7fff)
     return CGTP_ERR_SHAPE;
+  // the kernels take scale * log2 e, or scale / cap and cap * log2 e, in 32 bits: below the normal numbers a quotient loses its bits, or is zero
+  auto holds = [](float v) { return v == 0.f || (std::fabs(v) >= 0x1p-126f && std::fabs(v) <= 1e38f); };
+  if (!holds(a->scale) || !(a->cap <= 0.f || (a->cap >= 1e-37f && a->cap <= 1e38f))) return CGTP_ERR_CONFIG;
+  if (a->cap > 0.f && a->scale != 0.f && (a->scale / a->cap == 0.f || !holds(a->scale / a->cap))) return CGTP_ERR_CONFIG;
   if (a->n_rows > 0 && (!a->x || !a->table || !a->kind)) return CGTP_ERR_NULL;
   return CGTP_OK;
 }

@@ -111,8 +111,9 @@ def kind_cross_entropy(x: Tensor, table: Tensor, kind: Tensor, scale: float = 1.
                         f"{tuple(table.shape)}, {tuple(kind.shape)}")
     scale, bounded = float(scale), cap is not None
     cap = float(cap) if bounded else 0.0
-    # the kernels take scale * log2 e, or scale / cap and cap * log2 e, as fp32
-    if not abs(scale) <= 1e38 or (bounded and not (1e-37 <= cap <= 1e38 and abs(scale) / cap <= 1e38)):
+    # the kernels take scale * log2 e, or scale / cap and cap * log2 e, as fp32, where a quotient below the normal numbers loses its bits, or is zero
+    least = 2.0 ** -126 if scale else 0.0
+    if not least <= abs(scale) <= 1e38 or (bounded and not (1e-37 <= cap <= 1e38 and least <= abs(scale) / cap <= 1e38)):
         raise CgtpError(f"scale, cap (above zero, or None) and their quotient must be in fp32's range, got {scale} and {cap}")
     if (x.numel() and kind.numel() > 1 << 29) or table.shape[0] > 1 << 30:
         raise CgtpError(f"at most 2^29 rows and 2^30 kinds, got {kind.numel()} and {table.shape[0]}")

@@ -884,7 +884,8 @@ int cgtp_add_rms_backward(const cgtp_add_rms_args* args, void* stream);
  * dtype, and for grad_table the rows of x times grad_loss over its largest magnitude.  All sums have an order that the sizes and the
  * rows with a kind determine.  The logits are never kept: workspace (cgtp_kind_loss_workspace_bytes, 16-byte aligned) holds a
  * copy of the rows that have a kind, statistics, and for the backward up to 512 MB of logits' gradients at a time and sums in fp32.
- * n_rows <= 2^29, n_kinds <= 2^30, channels < 2^15, else CGTP_ERR_SHAPE.  dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16.
+ * n_rows <= 2^29, n_kinds <= 2^30, channels < 2^15, else CGTP_ERR_SHAPE.  |scale| and, with a cap, |scale| / cap: 0 (scale alone) or 2^-126 to 1e38, cap
+ * 1e-37 to 1e38 (0 and below: none), else CGTP_ERR_CONFIG.  dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16.
  */
 typedef struct {
   const void *x, *table;
