@@ -10,8 +10,10 @@ def higher_order(expression, inputs, need, g: Tensor, create_graph: bool = True)
     Partial derivatives: the expression is evaluated on views of the inputs and differentiated with respect to the views.  The
     inputs come with their history, and one may be another, or computed from another (the features and the harmonics of a
     second layer, queries and keys of one tensor): with respect to the inputs themselves a path through another one would count
-    here and once more where the engine walks on from it."""
-    with torch.enable_grad():
+    here and once more where the engine walks on from it.
+
+    The expression chooses its types itself: under autocast its products in 32 bits would be taken in 16."""
+    with torch.enable_grad(), torch.autocast(g.device.type, enabled=False):
         own = [None if t is None else t.view_as(t) for t in inputs]
         grads = iter(torch.autograd.grad(expression(*own), [t for t, n in zip(own, need) if n], g, create_graph=create_graph,
                                          allow_unused=True))
