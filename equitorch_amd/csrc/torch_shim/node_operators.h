@@ -384,7 +384,7 @@ struct AddRms : torch::autograd::Function<AddRms> {
     const at::Tensor g_out = grad[0].defined() ? grad[0] : at::zeros(total.sizes(), total.options().dtype(type));
     if (at::GradMode::is_enabled()) {
       const variable_list g = call_fallback(d["fallback"].toInt(), g_out, {total, weight}, {need_x || need_residual, need_weight}, 2,
-                                            g_total.defined() ? Optional(g_total) : Optional(), type);
+                                            g_total.defined() ? Optional(g_total) : Optional(), type, d["eps"].toDouble());
       if (need_x) out[0] = g[0].to(type);
       if (need_residual) out[1] = g[0];
       out[2] = g[1];

@@ -40,7 +40,7 @@ def _forward(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], ep
     return out, total, rstd, scale
 
 
-def _higher(g_out, g_total, inputs, need, eps: float, dtype: torch.dtype):
+def _higher(g_out, inputs, need, g_total, dtype: torch.dtype, eps: float):
     """Gradients of ``(total, weight)`` through the tensor expression of ``out``, of type ``dtype``; what has come in for the total is added."""
     def expression(total, weight):
         t = total.float()
@@ -54,16 +54,14 @@ def _higher(g_out, g_total, inputs, need, eps: float, dtype: torch.dtype):
     return g_total if grads[0] is None else grads[0] + g_total, grads[1]
 
 
-_fallbacks = {}
+_fallbacks = []
 
 
-def _fallback(mod, eps: float):
+def _fallback(mod):
     """The extension's number for the tensor expression, which a backward under gradient mode evaluates."""
-    if eps not in _fallbacks:
-        def grads(g_out, inputs, need, g_total, dtype):
-            return _higher(g_out, g_total, inputs, need, eps, dtype)
-        _fallbacks[eps] = mod.Fallback(grads)
-    return _fallbacks[eps]
+    if not _fallbacks:
+        _fallbacks.append(mod.Fallback(_higher))
+    return _fallbacks[0]
 
 
 class _AddRmsNorm(Function):
@@ -84,7 +82,7 @@ class _AddRmsNorm(Function):
         if g_out is None and g_total is None:
             return None, None, None, None
         if torch.is_grad_enabled():
-            g, gw = _higher(g_out, g_total, (total, weight), (need[0] or need[1], need[2]), ctx.eps, ctx.dtype)
+            g, gw = _higher(g_out, (total, weight), (need[0] or need[1], need[2]), g_total, ctx.dtype, ctx.eps)
             return g.to(ctx.dtype) if need[0] else None, g if need[1] else None, gw, None
         same = total.dtype == ctx.dtype                       # then one tensor is the gradient of x and of the residual
         g_out = torch.zeros_like(total, dtype=ctx.dtype) if g_out is None else g_out.contiguous()
@@ -143,7 +141,7 @@ def add_rms_norm(x: Tensor, residual: Optional[Tensor] = None, weight: Optional[
     flat, flat_residual, w = _checked(x, residual, weight, eps)
     mod = _shim.module()
     if mod is not None:
-        out, total = mod.add_rms(flat, flat_residual, w, eps, keep, _fallback(mod, eps))
+        out, total = mod.add_rms(flat, flat_residual, w, eps, keep, _fallback(mod))
     elif keep:
         got = _AddRmsNorm.apply(flat, flat_residual, w, eps)
         out, total = (got, None) if residual is None else got
