@@ -335,6 +335,8 @@ int rms_check(const cgtp_add_rms_args* a) {
       (a->weight_dtype != a->dtype && a->weight_dtype != CGTP_F32))
     return CGTP_ERR_DTYPE;
   if (a->n_rows < 0 || a->n_rows > 0x7fffffff || a->channels <= 0 || a->channels > 0x7fff) return CGTP_ERR_SHAPE;
+  // the kernels add it in 32 bits, where a number below the normal ones loses its bits, or is zero
+  if (!(a->eps == 0 || (a->eps >= 0x1p-126 && a->eps <= 0x1.fffffep127))) return CGTP_ERR_CONFIG;
   return CGTP_OK;
 }
 

@@ -122,8 +122,8 @@ def _checked(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], ep
         raise CgtpError(f"residual must have x's shape, got {tuple(residual.shape)} and {tuple(x.shape)}")
     if weight is not None and weight.shape != (c,):
         raise CgtpError(f"weight must be ({c},), got {tuple(weight.shape)}")
-    if not 0.0 <= eps < float("inf"):
-        raise CgtpError(f"eps must be finite and not negative, got {eps}")
+    if not (eps == 0.0 or 2.0 ** -126 <= eps <= 2.0 ** 128 * (1 - 2.0 ** -24)):
+        raise CgtpError(f"eps must be 0, or above it in fp32's range, got {eps}")
     rows = [None if t is None else t.reshape(-1, c).contiguous() for t in (x, residual)]
     return *rows, None if weight is None else weight.contiguous()
 
@@ -135,7 +135,8 @@ def add_rms_norm(x: Tensor, residual: Optional[Tensor] = None, weight: Optional[
     beside fp32 are widened); ``weight`` ``(C,)`` likewise.  ``out`` has x's type, ``total`` the residual's, and the norm is that of ``total``
     as it is returned.  Without a residual ``total`` is ``x``.
 
-    Sums are held in 32 bits; the weight's gradient is summed over the rows in a fixed order.  Differentiable to any order."""
+    Squares and sums are held in 32 bits (elements whose squares leave fp32's range, above 1.8e19, or below 1e-19 where ``eps`` is 0, do not come out as
+    their norm; a row of zeros with ``eps`` 0 is NaN); the weight's gradient is summed over the rows in a fixed order.  Differentiable to any order."""
     eps = float(eps)
     keep = (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight))) or _lib.forward_mode()
     flat, flat_residual, w = _checked(x, residual, weight, eps)

@@ -857,7 +857,8 @@ int cgtp_attn_backward(const cgtp_attn_args* args, void* stream);
  * cgtp_add_rms_backward reads weight, total (t; x where there is no residual), rstd, grad_out and grad_total (the gradient of t
  * apart from out's, NULL: none) and writes those of grad_x, grad_residual (the same values in residual_dtype) and grad_weight
  * (weight_dtype) that are not NULL.  The sums over rows have an order that the sizes alone determine.
- * workspace: cgtp_add_rms_workspace_bytes (backward; 0: may be NULL).  channels < 2^15, n_rows < 2^31.
+ * workspace: cgtp_add_rms_workspace_bytes (backward; 0: may be NULL).  channels < 2^15, n_rows < 2^31, else CGTP_ERR_SHAPE.  eps: 0, or a normal
+ * number of fp32 above it, else CGTP_ERR_CONFIG.  Squares and their mean are held in fp32.
  * dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16; residual_dtype and weight_dtype: dtype or CGTP_F32.
  */
 typedef struct {
