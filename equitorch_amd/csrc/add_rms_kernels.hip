@@ -311,7 +311,7 @@ RmsShape shape_of(int c) {
   if (chunks <= 64) {
     for (s.group = 1; s.group < chunks;) s.group *= 2;
   } else if (chunks <= 64 * kWaveChunks) {
-    while (64 * s.chunks < chunks) s.chunks *= 2;
+    s.chunks = kWaveChunks;
   } else {
     s.block = true;
     if (chunks > 4 * kThreads) s.threads = 512;
@@ -361,11 +361,11 @@ void launch(const RmsArgs& k, const RmsShape& s, hipStream_t stream) {
   if constexpr (BACKWARD) hipLaunchKernelGGL((add_rms_grad_kernel<T, R, CHUNKS, BLOCK>), grid, block, 0, stream, k);
   else hipLaunchKernelGGL((add_rms_kernel<T, R, CHUNKS, BLOCK>), grid, block, 0, stream, k);
 }
+static_assert(kWaveChunks == 2, "a wavefront's row has one chunk a lane or two");
 template <typename T, typename R, bool BACKWARD>
 void launch_of(const RmsArgs& k, const RmsShape& s, hipStream_t stream) {
   if (!s.block && s.chunks == 1) launch<T, R, BACKWARD, 1, false>(k, s, stream);
-  else if (!s.block && s.chunks == 2) launch<T, R, BACKWARD, 2, false>(k, s, stream);
-  else if (!s.block) launch<T, R, BACKWARD, 4, false>(k, s, stream);
+  else if (!s.block) launch<T, R, BACKWARD, kWaveChunks, false>(k, s, stream);
   else if (s.chunks == 1) launch<T, R, BACKWARD, 1, true>(k, s, stream);
   else if (s.chunks == 2) launch<T, R, BACKWARD, 2, true>(k, s, stream);
   else if (s.chunks == 4) launch<T, R, BACKWARD, 4, true>(k, s, stream);
