@@ -152,7 +152,7 @@ class AdamW(torch.optim.Optimizer):
                 if "step" in s:
                     s["step"] = torch.as_tensor(s["step"], dtype=torch.float32).reshape(())
                 for name in ("exp_avg", "exp_avg_sq") if group["state_bits"] == 32 else ():
-                    if isinstance(s.get(name), Tensor) and s[name].is_floating_point():
+                    if isinstance(s.get(name), Tensor) and s[name].dtype in (torch.bfloat16, torch.float16, torch.float64):
                         s[name] = s[name].float()
         return {**state_dict, "state": state, "param_groups": groups}
 

@@ -202,3 +202,12 @@ def test_one_block_may_change_its_order():
     opt.load_state_dict(saved.state_dict())
     assert opt.state[q]["exp_avg"].stride() == (1, 16)
     assert torch.equal(_decoded(opt.state[q], "exp_avg", q), _decoded(saved.state[p], "exp_avg", p))
+
+
+def test_codes_of_8_bits_are_not_taken_for_numbers():
+    """States in 8 bits under an option of 32: left as they are, for the step to refuse."""
+    saved = _states(AdamW(_params((20, 30)), state_bits=8)).state_dict()
+    saved["param_groups"][0]["state_bits"] = 32
+    opt = AdamW(_params((20, 30)))
+    opt.load_state_dict(saved)
+    assert opt.state[opt.param_groups[0]["params"][0]]["exp_avg"].dtype == E4M3
