@@ -111,15 +111,19 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """As torch's, hooks included, with every state in its own type (torch's takes floating-point states to the parameter's).  A dict of
         ``torch.optim.AdamW`` is taken too: options that it does not have keep their values, ``exp_avg`` and ``exp_avg_sq`` become fp32.  What
-        is refused leaves the optimizer as it was."""
+        is refused leaves the optimizer as it was.
+
+        States that are there, and an ``lr`` on the GPU (unless groups that share it come with several), are written over where they lie: a
+        recorded graph that holds a step goes on from what was loaded."""
         loaded = []
 
         def check(_, read):
-            loaded.append(self._completed(read))
-            return loaded[0]
+            read = self._completed(read)
+            loaded.extend((read, {p: dict(s) for p, s in self.state.items()}, [g["lr"] for g in self.param_groups]))
+            return read
         # last of the hooks before, first of those after: the states are those of the dict that the others leave, and stay what the others make of them
         handles = [self.register_load_state_dict_pre_hook(check),
-                   self.register_load_state_dict_post_hook(lambda _: self._load_states(loaded[0]), prepend=True)]
+                   self.register_load_state_dict_post_hook(lambda _: self._load_states(*loaded), prepend=True)]
         try:
             super().load_state_dict(state_dict)
         finally:
@@ -156,19 +160,33 @@ class AdamW(torch.optim.Optimizer):
                         s[name] = s[name].float()
         return {**state_dict, "state": state, "param_groups": groups}
 
-    def _load_states(self, state_dict: dict) -> None:
+    @torch.no_grad()
+    def _load_states(self, state_dict: dict, before: dict, rates: list) -> None:
+        """before, rates: the states and learning rates that the load replaced."""
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
+        there = {t.untyped_storage().data_ptr() for s in before.values() for t in s.values() if isinstance(t, Tensor)}
+        values = []
         for i, p in zip(ids, params):
             for name, value in state_dict["state"].get(i, {}).items():
-                if not isinstance(value, Tensor):
-                    continue
-                with torch.no_grad():
-                    if value.shape == p.shape and value.ndim:
-                        value = _like(p, value.dtype).copy_(value)
-                    else:
-                        value = value.to(p.device, copy=True)
-                self.state[p][name] = value
+                if isinstance(value, Tensor):        # a state that the dict shares with this optimizer may be written over before its turn
+                    values.append((p, name, value.clone() if value.untyped_storage().data_ptr() in there else value))
+        for p, name, value in values:
+            like_p, old = value.shape == p.shape and value.ndim, before.get(p, {}).get(name)
+            if isinstance(old, Tensor) and (old.shape, old.dtype, old.device) == (value.shape, value.dtype, p.device) and (
+                    _same_order(old, p) if like_p else old.is_contiguous()):
+                old.copy_(value)
+            elif like_p:
+                old = _like(p, value.dtype).copy_(value)
+            else:
+                old = value.to(p.device, copy=True)
+            self.state[p][name] = old
+        for lr in {id(t): t for t in rates if isinstance(t, Tensor) and t.is_cuda}.values():
+            sharing = [g for g, t in zip(self.param_groups, rates) if t is lr]
+            if len({float(g["lr"]) for g in sharing}) == 1:      # else each group has its own from now on
+                lr.fill_(float(sharing[0]["lr"]))
+                for group in sharing:
+                    group["lr"] = lr
 
     def _init_state(self, p: Tensor, bits: int, master: bool) -> dict:
         if torch.cuda.is_current_stream_capturing():

@@ -211,3 +211,24 @@ def test_codes_of_8_bits_are_not_taken_for_numbers():
     opt = AdamW(_params((20, 30)))
     opt.load_state_dict(saved)
     assert opt.state[opt.param_groups[0]["params"][0]]["exp_avg"].dtype == E4M3
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_states_are_written_over_where_they_lie(bits):
+    """So that what holds their addresses goes on from what was loaded; a dict that shares them, turned round by a hook, too."""
+    opt = _states(AdamW(_params((20, 30), (20, 30)), state_bits=bits))
+    first, second = opt.param_groups[0]["params"]
+    places = [{k: v.data_ptr() for k, v in opt.state[p].items()} for p in (first, second)]
+    want = _copy(opt)[1]
+    hook = opt.register_load_state_dict_pre_hook(lambda _, read: {**read, "state": {1 - i: s for i, s in read["state"].items()}})
+    opt.load_state_dict(opt.state_dict())
+    hook.remove()
+    for p, s, place in zip((second, first), want, places[::-1]):
+        _equal(opt.state[p], s)
+        assert {k: v.data_ptr() for k, v in opt.state[p].items()} == place
+    saved = _states(AdamW(_params((20, 30), (20, 30)), state_bits=bits), seed=7).state_dict()
+    opt.load_state_dict(saved)
+    _equal(opt.state[second], saved["state"][1])
+    assert {k: v.data_ptr() for k, v in opt.state[second].items()} == places[1]
+    opt.state[second]["exp_avg"].copy_(opt.state[first]["exp_avg"])      # the loaded dict's stay as they are
+    assert not torch.equal(saved["state"][1]["exp_avg"].float(), opt.state[second]["exp_avg"].float())

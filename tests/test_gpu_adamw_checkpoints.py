@@ -1,4 +1,6 @@
 """Runs that go on from a saved state on the GPU."""
+import copy
+
 import pytest
 import torch
 
@@ -37,3 +39,75 @@ def test_goes_on_from_torchs_adamw(device):
     for q in second:
         assert bool(((q.detach().double() - q.want).abs() <= q.bound).all())
         assert float(opt.state[q]["step"]) == 4
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_recorded_step_goes_on_from_what_was_loaded(device, bits):
+    """Back to a saved state between two replays: weights, states, steps and the learning rate on the GPU are those of an eager run."""
+    gen = torch.Generator().manual_seed(4)
+    start = [torch.randn(s, generator=gen).to(device) for s in ((500,), (30, 41))]
+    grads = [[torch.randn(t.shape, generator=gen).to(device) for t in start] for _ in range(6)]
+
+    def make():
+        params = [torch.nn.Parameter(t.clone()) for t in start]
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        return params, AdamW(params, lr=torch.full((), 1e-2, device=device), state_bits=bits, seed=3)
+
+    def fill(params, gs):
+        for p, g in zip(params, gs):
+            p.grad.copy_(g)
+    params, opt = make()
+    fill(params, grads[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    saved = copy.deepcopy(opt.state_dict())
+    weights = [p.detach().clone() for p in params]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for lr in (1e-2, 3e-3):
+        for gs in grads[1:4]:
+            fill(params, gs)
+            graph.replay()
+        torch.cuda.synchronize()
+        saved["param_groups"][0]["lr"] = lr if lr == 3e-3 else torch.tensor(lr)
+        opt.load_state_dict(saved)
+        with torch.no_grad():
+            for p, w in zip(params, weights):
+                p.copy_(w)
+        others, eager = make()
+        eager.load_state_dict(saved)
+        with torch.no_grad():
+            for p, w in zip(others, weights):
+                p.copy_(w)
+        assert eager.param_groups[0]["lr"].is_cuda and float(opt.param_groups[0]["lr"]) == pytest.approx(lr)
+        noise = [torch.full((1000,), float("nan"), device=device) for _ in range(50)]      # what is freed is taken
+        for gs in grads[4:]:
+            fill(params, gs)
+            fill(others, gs)
+            graph.replay()
+            eager.step()
+        torch.cuda.synchronize()
+        for p, q in zip(params, others):
+            assert torch.equal(p, q)
+            for name, value in eager.state[q].items():
+                assert torch.equal(opt.state[p][name].float(), value.float()), name
+        del noise
+
+
+def test_a_learning_rate_that_groups_share(device):
+    """Loaded as one it stays one tensor; loaded as two each group has its own."""
+    params = [torch.nn.Parameter(torch.ones(4, device=device)) for _ in range(2)]
+    lr = torch.full((), 0.5, device=device)
+    opt = AdamW([{"params": [p]} for p in params], lr=lr)
+    saved = copy.deepcopy(opt.state_dict())
+    lr.fill_(0.1)
+    opt.load_state_dict(saved)
+    assert all(g["lr"] is lr for g in opt.param_groups) and float(lr) == 0.5
+    saved["param_groups"][1]["lr"] = 0.25
+    opt.load_state_dict(saved)
+    assert [float(g["lr"]) for g in opt.param_groups] == [0.5, 0.25]
