@@ -13,7 +13,8 @@
 // Bound by the matrix cores: 2 N K C operations forward, 6 N K C backward, where a calculation that kept all logits would do 4.
 // 16384 rows, 30011 kinds, 256 bf16 channels: statistics 250-290 us (870-1000 TFLOP/s), logits again and dx 500-580 (870-1000), the
 // table's gradient 320 (785), joins and copies of rows 75; 4253 rows with a kind, 50021 kinds, 500 fp16 channels, capped: 255-290 us (730-830).
-// Small calls: the launches, three forward and up to eight backward.
+// Small calls: the launches.  Forward the rows' copy and the statistics, with more than 64 rows their count before, with rows that are no whole aligned
+// chunks the table's copy, with more than one range of kinds a join: two to five; backward up to eight.
 #include "gff_gemm.h"
 
 #include <algorithm>
@@ -24,8 +25,9 @@ namespace cgtp {
 namespace {
 
 constexpr int kTile = 128, kRowBlocks = 1024, kRowThreads = 256;
-// Tiles of the products of both operands from LDS: in fp32, whose matrix instructions are slow, small ones cost nothing and keep more of the
-// GPU busy (9000 rows, 100 kinds, 128 channels: statistics 17 us with tiles of 128, 12 with these, the logits' gradients 18 and 11).
+// Tiles of the products of both operands from LDS: in fp32 small ones keep more of the GPU busy where there are few (9000 rows, 100 kinds, 128 channels:
+// statistics 17 us with tiles of 128, 12 with these, the logits' gradients 18 and 11).  Tables of thousands of kinds, where fp32 runs at 70 to 95 TFLOP/s of
+// the library's 153, were not timed with the larger ones, which bring half as many bytes for an operation.
 template <typename T> constexpr int kTileOf = sizeof(T) == 4 ? 64 : kTile;
 template <typename T> constexpr int kLds = kTileOf<T> * 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

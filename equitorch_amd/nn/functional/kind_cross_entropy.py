@@ -96,7 +96,7 @@ def kind_cross_entropy(x: Tensor, table: Tensor, kind: Tensor, scale: float = 1.
     Where ``kind`` is outside the table the loss is 0 and nothing has a gradient, whatever ``x`` holds there: nodes that are not
     asked for have kind -1 and cost nothing.  No logits are kept.  Sums are held in 32 bits and have a fixed order; the
     softmax is rounded to the operands' type where it enters the gradients' products, and for the table's so are the rows of ``x`` times
-    the incoming gradient."""
+    the incoming gradient over its largest magnitude (in fp16 rows whose gradient is below some 1e-5 of that keep few bits)."""
     tensors = x, table = _lib.of_one_type(x, table)
     _lib.require_gpu(x, table, kind)
     if x.dtype not in _DTYPES or table.dtype != x.dtype:
