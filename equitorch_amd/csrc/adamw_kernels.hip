@@ -291,6 +291,8 @@ int adamw_check(const cgtp_adamw_args* a) {
   if (a->state_bits != 8 && a->state_bits != 32) return CGTP_ERR_CONFIG;
   if (a->n_tensors < 0) return CGTP_ERR_SHAPE;
   if (!(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1)) return CGTP_ERR_CONFIG;
+  // it is added in 32 bits, and the sum's inverse is taken: where it is zero, or the inverse infinite, an element without a gradient would become NaN
+  if (!(a->eps == 0 || (a->eps >= 0x1p-126 && a->eps <= 0x1.fffffep127))) return CGTP_ERR_CONFIG;
   if (a->n_tensors > 0 && !a->tensors) return CGTP_ERR_NULL;
   for (int64_t i = 0; i < a->n_tensors; ++i) {
     const cgtp_adamw_tensor& t = a->tensors[i];

@@ -89,9 +89,10 @@ class AdamW(torch.optim.Optimizer):
         betas = group["betas"]
         if len(betas) != 2 or not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError(f"betas must be two numbers of 0 <= beta < 1, got {betas}")
-        for name in ("eps", "weight_decay"):
-            if not 0.0 <= group[name] < float("inf"):
-                raise ValueError(f"{name} must be finite and not negative, got {group[name]}")
+        if not 0.0 <= group["weight_decay"] < float("inf"):
+            raise ValueError(f"weight_decay must be finite and not negative, got {group['weight_decay']}")
+        if not (group["eps"] == 0.0 or 2.0 ** -126 <= group["eps"] <= 2.0 ** 128 * (1 - 2.0 ** -24)):
+            raise ValueError(f"eps must be 0, or above it in fp32's range, got {group['eps']}")
         if group["state_bits"] not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
         if not 0 <= group["seed"] < 1 << 32:

@@ -913,7 +913,8 @@ int cgtp_kind_loss_backward(const cgtp_kind_loss_args* args, void* stream);
  * exp_avg_sq_scale, fp32, one for each CGTP_ADAMW_BLOCK elements: the block's largest magnitude / 448.  m is rounded to nearest, sqrt(v) up
  * or down in proportion by 20 random bits, a hash of seed, number, t and the element's place, and not to zero from above it;
  * a block with an infinity or a NaN becomes NaN.  p is computed from m and v before they are rounded.
- * lr_ptr: lr in device memory (fp32), read when the kernels run; NULL: lr.  0 <= beta < 1 and known state_bits, else CGTP_ERR_CONFIG.
+ * lr_ptr: lr in device memory (fp32), read when the kernels run; NULL: lr.  0 <= beta < 1, eps 0 or a normal number of fp32 above
+ * it, and known state_bits, else CGTP_ERR_CONFIG.
  * n < 2^31.  Arrays of different tensors may not overlap.  dtype: CGTP_F32 | CGTP_BF16 | CGTP_F16, of all tensors.
  */
 enum { CGTP_ADAMW_BLOCK = 256 };

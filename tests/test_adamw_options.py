@@ -1,9 +1,12 @@
 """Checks of AdamW's options and parameters without a GPU."""
 import copy
+import ctypes as C
 
 import pytest
 import torch
 
+from equitorch_amd import _lib
+from equitorch_amd._lib import AdamwArgs
 from equitorch_amd.optim import AdamW
 
 
@@ -61,3 +64,35 @@ def test_construction_looks_at_each_parameter_once(monkeypatch):
     assert seen == [50]
     opt.add_param_group({"params": _params()})
     assert seen == [50, 51]
+
+
+# 1e-50 was zero in 32 bits and 1e-40 had no finite inverse: elements without a gradient became NaN; 1e39 was infinity
+@pytest.mark.parametrize("eps,taken", [(1e-50, False), (1e-40, False), (1e39, False), (float("nan"), False), (-1e-8, False), (0.0, True),
+                                       (2.0 ** -126, True), (1e-8, True), (3.4e38, True)])
+def test_an_eps_that_32_bits_do_not_hold_is_refused(eps, taken):
+    a = AdamwArgs()
+    a.n_tensors, a.beta1, a.beta2, a.state_bits, a.eps = 0, 0.9, 0.999, 32, eps
+    assert _lib.lib.cgtp_adamw_step(C.byref(a), None) == (0 if taken else 5)
+    if taken:
+        AdamW(_params(), eps=eps).step()
+        return
+    with pytest.raises(ValueError):
+        AdamW(_params(), eps=eps)
+    opt = AdamW(_params())
+    opt.param_groups[0]["eps"] = eps
+    with pytest.raises(ValueError):
+        opt.step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_the_smallest_eps(device, bits):
+    """Elements without a gradient stay where they are; one with a gradient takes a step of lr, whatever its size."""
+    p = torch.nn.Parameter(torch.ones(600, device=device))
+    p.grad = torch.zeros_like(p)
+    p.grad[5] = 1e-12
+    AdamW([p], lr=0.125, eps=2.0 ** -126, weight_decay=0.0, state_bits=bits).step()
+    want = torch.ones(600, dtype=torch.float64, device=device)
+    want[5] = 0.875
+    # m / sqrt(v) of a first step is 1 to some twelve roundings, of a step of 0.125
+    assert bool(((p.detach().double() - want).abs() <= 2.0 ** -24 * (12 * 0.125 + 1)).all())
