@@ -51,7 +51,8 @@ class AdamW(torch.optim.Optimizer):
     with a gradient that is not finite, or whose square is not, becomes NaN.
 
     ``master``: parameters in 16 bits have a copy in fp32 (``master``) that the steps are taken on, and receive it rounded.  Without it
-    a step below half a unit of a 16-bit weight is lost.
+    a step below half a unit of a 16-bit weight is lost.  Weights that are written into such a parameter from elsewhere have to be written into the copy
+    too: the next step is taken on that.
 
     ``lr`` may be an fp32 tensor on the GPU, which is read when the step runs: a recorded graph then follows it.  Every number else
     is fixed when a graph records the step, and states have to be there by then (one step before).  ``step`` in a parameter's state counts on the
